@@ -17,6 +17,9 @@
  *   subq_head_rmsnorm_fwd / _bwd
  *                       SubQLinearAttention's per-head nn.RMSNorm and the
  *                       transpose copy after it                          python/subq_audio/autograd.py:706-710,763-769
+ *   subq_delta_fwd / _bwd, subq_layer_norm_fwd / _bwd:
+ *                       no counterpart: the gated delta rule beside the scan,
+ *                       and the norm before a layer
  *   subq_*_workspace_bytes, subq_last_error, subq_abi_version, subq_device_info:
  *                       no single counterpart; they carry the reference's
  *                       scratch allocation (attention_backward.cpp:305-361 allocated
@@ -213,6 +216,103 @@ typedef struct subq_rmsnorm_args {
 int subq_head_rmsnorm_fwd(const subq_rmsnorm_args* args);
 int subq_head_rmsnorm_bwd(const subq_rmsnorm_args* args);
 size_t subq_head_rmsnorm_bwd_workspace_bytes(const subq_rmsnorm_args* args);
+
+/* Gated delta rule (no counterpart in the reference): the scan whose update
+ * corrects what the state already holds for a key instead of adding to it,
+ *   S_t = gamma_t S_{t-1} + beta_t k_t (v_t - gamma_t S_{t-1}^T k_t)^T,
+ *   o_t = scale S_t^T q_t,
+ * per (batch, head) with S [d, e] float32, gamma_t = exp(log_gamma_t). A masked
+ * token leaves S as it is, its o and gradients are 0, and nothing of its q, k,
+ * v, dout, beta or log_gamma is used. q, k, v and o are [B, heads, N, *] views;
+ * q, k and v may each have fewer heads (a divisor of `heads`), state head h
+ * then reading head h / (heads / x_heads), and their gradients sum over the
+ * group. fp32, fp16, bf16; products accumulate in float32, and operands are
+ * carried to 16 bits of mantissa (24 for fp32). For bounded states |k_t| <= 1
+ * with beta_t in [0, 2] and gamma_t <= 1, as usual for the rule; the kernels do
+ * not require it. A live token that is not finite makes its chunk of 64
+ * tokens, and what follows, not finite.
+ *
+ * Paths: SUBQ_PATH_EXACT is the token-recurrent kernel (d, e <= 256),
+ * SUBQ_PATH_CHUNKED the chunk kernels (d <= 128, e <= 256). AUTO takes the
+ * recurrent kernel for d > 128 and for calls of at most 16 tokens that fill no
+ * handover. The backward has the chunk form only (d <= 128). */
+typedef struct subq_gate {
+    const float* data; /* [B, heads, N] float32 with element strides (0 allowed) */
+    int64_t stride_b, stride_h, stride_n;
+} subq_gate;
+
+typedef struct subq_delta_desc {
+    int64_t batch, heads, seq_len, head_dim, value_dim;
+    int64_t q_heads, k_heads, v_heads; /* 0: `heads` */
+    int32_t dtype;
+    int32_t path;           /* AUTO, EXACT or CHUNKED                          */
+    float scale;
+    subq_gate beta;         /* data NULL: 1                                    */
+    subq_gate log_gamma;    /* data NULL: 0 (no decay)                         */
+    const uint8_t* mask;    /* as in subq_scan_desc                            */
+    int64_t mask_stride_b;
+} subq_delta_desc;
+
+typedef struct subq_delta_fwd_args {
+    subq_delta_desc desc;
+    subq_tensor4 q, k, v, o;
+    const float* state_in;  /* [B, heads, d, e], NULL = zeros                  */
+    float* state_out;       /* may equal state_in, NULL = not wanted           */
+    void* handover;         /* NULL, or subq_delta_handover_bytes (256-byte aligned)
+                               to keep for the backward of the same call       */
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} subq_delta_fwd_args;
+
+typedef struct subq_delta_bwd_args {
+    subq_delta_desc desc;
+    subq_tensor4 q, k, v, dout;
+    subq_tensor4 dq, dk, dv;     /* heads of q, k, v; must not alias the inputs  */
+    const float* state_in;       /* the forward's                                */
+    const float* dstate_out;     /* gradient of the final state, NULL = zeros    */
+    float* dstate_in;            /* gradient of state_in, NULL = not wanted      */
+    float* dbeta;                /* [B, heads, N] contiguous float32             */
+    float* dlog_gamma;           /* likewise, or NULL                            */
+    const void* handover;        /* what the forward of the same call left, or
+                                    NULL: formed again in the workspace          */
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} subq_delta_bwd_args;
+
+int subq_delta_fwd(const subq_delta_fwd_args* args);
+int subq_delta_bwd(const subq_delta_bwd_args* args);
+size_t subq_delta_fwd_workspace_bytes(const subq_delta_fwd_args* args);
+size_t subq_delta_bwd_workspace_bytes(const subq_delta_bwd_args* args);
+size_t subq_delta_handover_bytes(const subq_delta_desc* desc);
+
+/* Layer norm over the last dimension of [rows, dim] (rows at element strides,
+ * elements contiguous): y = (x - mean) rsqrt(var + eps) weight + bias, as
+ * torch's layer_norm, sums in float32. x_dtype and y_dtype are equal (fp32,
+ * fp16, bf16), or x is fp32 and y fp16 or bf16; dx has x's type and dy has y's.
+ * The backward recomputes the statistics from x; dweight = sum dy xh and
+ * dbias = sum dy are written (not accumulated), bitwise reproducible. */
+typedef struct subq_layer_norm_args {
+    int64_t rows, dim;
+    int32_t x_dtype, y_dtype;
+    float eps;
+    const void* x;  int64_t x_stride;
+    void* y;        int64_t y_stride;   /* forward  */
+    const void* dy; int64_t dy_stride;  /* backward */
+    void* dx;       int64_t dx_stride;  /* may be x or dy for dim <= 8192 */
+    const float* weight;                /* [dim] or NULL (1) */
+    const float* bias;                  /* [dim] or NULL (0) */
+    float* dweight;                     /* [dim] or NULL */
+    float* dbias;                       /* [dim] or NULL */
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} subq_layer_norm_args;
+
+int subq_layer_norm_fwd(const subq_layer_norm_args* args);
+int subq_layer_norm_bwd(const subq_layer_norm_args* args);
+size_t subq_layer_norm_bwd_workspace_bytes(const subq_layer_norm_args* args);
 
 /* Backward scan with no allocation and no caller workspace (no counterpart in
  * the reference, whose backward allocates its scratch on every call). For

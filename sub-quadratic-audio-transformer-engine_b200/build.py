@@ -8,6 +8,7 @@ Usage: python build.py [--force]
 """
 from __future__ import annotations
 
+import concurrent.futures
 import glob
 import os
 import subprocess
@@ -21,6 +22,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
+
+OBJ = os.path.join(HERE, "_build")  # one object per source, rebuilt when its sources change
 
 LIB = os.path.join(PKG, "libsubq_b200.so")
 EXT = os.path.join(PKG, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
@@ -57,11 +60,20 @@ def _run(cmd, verbose):
 def build_lib(force=False, verbose=False) -> str:
     cu, cpp = _sources()
     if force or _stale(LIB, cu + cpp + _headers() + [__file__]):
+        os.makedirs(OBJ, exist_ok=True)
+
+        def compile_one(src):
+            obj = os.path.join(OBJ, os.path.basename(src) + ".o")
+            if force or _stale(obj, [src, __file__] + _headers()):
+                _run([NVCC, *ARCH_FLAGS, *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-x", "cu", "-c", src, "-o", obj + ".tmp"],
+                     verbose)
+                os.replace(obj + ".tmp", obj)
+            return obj
+
+        with concurrent.futures.ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+            objs = list(pool.map(compile_one, cu + cpp))
         tmp = LIB + ".tmp"
-        cmd = [NVCC, *ARCH_FLAGS, *NVCC_FLAGS, "-shared", "-I", INCLUDE, "-I", CSRC, *cu]
-        cmd += [x for f in cpp for x in ("-x", "cu", f)]
-        cmd += ["-o", tmp]
-        _run(cmd, verbose)
+        _run([NVCC, *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", *objs, "-o", tmp], verbose)
         os.replace(tmp, LIB)
     return LIB
 

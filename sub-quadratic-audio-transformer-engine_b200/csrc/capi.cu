@@ -7,6 +7,8 @@
 #include <mutex>
 #include <string>
 
+#include "delta_common.cuh"
+#include "delta_launch.h"
 #include "kernels.hpp"
 #include "scan_common.cuh"
 #include "scan_launch.h"
@@ -444,6 +446,336 @@ int subq_head_rmsnorm_bwd(const subq_rmsnorm_args* a) {
     cudaError_t err = subq::launch_rms_bwd(p, a->dtype, st);
     if (err != cudaSuccess) return fail_cuda(err, "subq_head_rmsnorm_bwd launch");
     g_last_launches = p.dw ? 2 : 1;
+    return SUBQ_OK;
+}
+
+// ------------------------------------------------------------ gated delta rule
+namespace {
+
+// Calls of at most this many tokens take the token-recurrent kernel.
+constexpr int kDeltaRecurrentMaxTokens = 16;
+
+int delta_gate(const subq_gate& g, const char* name, subq::DeltaGate& out) {
+    if (reinterpret_cast<uintptr_t>(g.data) % 4 != 0)
+        return fail(SUBQ_ERR_INVALID_ARGUMENT, std::string(name) + " is not aligned to its element size");
+    if (g.data && (g.stride_b < 0 || g.stride_h < 0 || g.stride_n < 0))
+        return fail(SUBQ_ERR_INVALID_ARGUMENT, std::string(name) + " has a negative stride");
+    out = {g.data, g.stride_b, g.stride_h, g.stride_n};
+    return SUBQ_OK;
+}
+
+int check_delta(const subq_delta_desc& d, subq::DeltaParams& p) {
+    if (d.batch < 0 || d.heads < 0 || d.seq_len < 0)
+        return fail(SUBQ_ERR_INVALID_ARGUMENT, "negative batch, heads or seq_len");
+    if (d.head_dim <= 0 || d.value_dim <= 0)
+        return fail(SUBQ_ERR_INVALID_ARGUMENT, "head_dim and value_dim must be positive");
+    if (d.batch > 65535 || d.heads > 65535 || d.seq_len > (int64_t)1 << 30)
+        return fail(SUBQ_ERR_INVALID_ARGUMENT, "batch/heads above 65535 or seq_len above 2^30");
+    if (d.head_dim > 256 || d.value_dim > 256)
+        return fail(SUBQ_ERR_UNSUPPORTED, "head_dim and value_dim above 256 are not supported");
+    if (d.dtype != SUBQ_FP32 && d.dtype != SUBQ_FP16 && d.dtype != SUBQ_BF16)
+        return fail(SUBQ_ERR_INVALID_ARGUMENT, "the gated delta rule supports float32, float16 and bfloat16");
+    if (d.path != SUBQ_PATH_AUTO && d.path != SUBQ_PATH_EXACT && d.path != SUBQ_PATH_CHUNKED)
+        return fail(SUBQ_ERR_INVALID_ARGUMENT, "the gated delta rule has the paths auto, exact and chunked");
+    for (int64_t x : {d.q_heads, d.k_heads, d.v_heads})
+        if (x < 0 || (x > 0 && d.heads % x != 0))
+            return fail(SUBQ_ERR_INVALID_ARGUMENT, "q_heads, k_heads and v_heads must be 0 or divisors of heads");
+    if (!(d.scale >= -3e38f && d.scale <= 3e38f)) return fail(SUBQ_ERR_INVALID_ARGUMENT, "scale must be finite");
+    if (d.mask && d.mask_stride_b < 0) return fail(SUBQ_ERR_INVALID_ARGUMENT, "mask has a negative stride");
+    p = subq::DeltaParams{};
+    p.B = (int)d.batch; p.H = (int)d.heads; p.N = (int)d.seq_len; p.d = (int)d.head_dim; p.e = (int)d.value_dim;
+    p.nc = (int)((d.seq_len + subq::kDeltaC - 1) / subq::kDeltaC);
+    p.scale = d.scale;
+    p.mask = d.mask;
+    p.mask_sb = d.mask ? d.mask_stride_b : 0;
+    int rc = delta_gate(d.beta, "beta", p.beta);
+    if (rc) return rc;
+    if ((rc = delta_gate(d.log_gamma, "log_gamma", p.lg))) return rc;
+    // one CTA per (sequence, 64 tokens) and per (sequence, 32 value columns)
+    const int64_t bh = d.batch * d.heads;
+    if (bh * (p.nc > 8 ? p.nc : 8) > (int64_t)0x7fffffff)
+        return fail(SUBQ_ERR_UNSUPPORTED, "batch * heads * seq_len is too large for one call");
+    return SUBQ_OK;
+}
+
+int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc& d, int64_t heads, bool empty, subq::DeltaTensor& out) {
+    int rc = check_tensor(t, name, d.dtype, empty);
+    if (rc) return rc;
+    const int64_t es = (int64_t)elem_size(d.dtype);
+    out.p = t.data;
+    out.sb = t.stride_b; out.sh = t.stride_h; out.sn = t.stride_n;
+    out.group = heads > 0 && d.heads > 0 ? (int)(d.heads / heads) : 1;
+    out.vec = reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && t.stride_b * es % 16 == 0 && t.stride_h * es % 16 == 0 &&
+              t.stride_n * es % 16 == 0;
+    return SUBQ_OK;
+}
+
+struct DeltaBytes {
+    size_t Y, S0, W;  // the handover's three parts
+};
+DeltaBytes delta_bytes(const subq::DeltaParams& p, int dtype) {
+    const size_t nx = dtype == SUBQ_FP32 ? 3 : 2, chunks = (size_t)p.B * p.H * p.nc;
+    const size_t ncw = 2 * ((p.e + subq::kDeltaCols - 1) / subq::kDeltaCols), dp = p.d <= 64 ? 64 : 128;
+    return {align_up(chunks * nx * subq::kYBlocks * 512), align_up(chunks * ncw * (dp / 16) * nx * 512),
+            align_up(chunks * ncw * 4 * nx * 512)};
+}
+
+void delta_handover(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
+    p.Y = static_cast<unsigned char*>(at);
+    p.S0 = p.Y + n.Y;
+    p.W = p.S0 + n.S0;
+}
+
+int fill_delta_fwd(const subq_delta_fwd_args* a, subq::DeltaParams& p, int& path) {
+    if (!a) return fail(SUBQ_ERR_INVALID_ARGUMENT, "null argument block");
+    const subq_delta_desc& d = a->desc;
+    int rc = check_delta(d, p);
+    if (rc) return rc;
+    const bool empty = p.B == 0 || p.H == 0 || p.N == 0;
+    if ((rc = delta_tensor(a->q, "q", d, d.q_heads, empty, p.q)) || (rc = delta_tensor(a->k, "k", d, d.k_heads, empty, p.k)) ||
+        (rc = delta_tensor(a->v, "v", d, d.v_heads, empty, p.v)) || (rc = delta_tensor(a->o, "o", d, d.heads, empty, p.o)))
+        return rc;
+    p.S_in = a->state_in;
+    p.S_out = a->state_out;
+    path = d.path;
+    if (path == SUBQ_PATH_AUTO)
+        path = p.d > 128 || (p.N <= kDeltaRecurrentMaxTokens && !a->handover) ? SUBQ_PATH_EXACT : SUBQ_PATH_CHUNKED;
+    if (path == SUBQ_PATH_CHUNKED && p.d > 128)
+        return fail(SUBQ_ERR_UNSUPPORTED, "the chunked path needs head_dim <= 128");
+    if (path == SUBQ_PATH_EXACT && a->handover)
+        return fail(SUBQ_ERR_UNSUPPORTED, "the handover is filled by the chunked path (head_dim <= 128) only");
+    return SUBQ_OK;
+}
+
+int fill_delta_bwd(const subq_delta_bwd_args* a, subq::DeltaParams& p) {
+    if (!a) return fail(SUBQ_ERR_INVALID_ARGUMENT, "null argument block");
+    const subq_delta_desc& d = a->desc;
+    int rc = check_delta(d, p);
+    if (rc) return rc;
+    if (d.path == SUBQ_PATH_EXACT || p.d > 128)
+        return fail(SUBQ_ERR_UNSUPPORTED, "the backward of the gated delta rule has the chunked path (head_dim <= 128) only");
+    const bool empty = p.B == 0 || p.H == 0 || p.N == 0;
+    if ((rc = delta_tensor(a->q, "q", d, d.q_heads, empty, p.q)) || (rc = delta_tensor(a->k, "k", d, d.k_heads, empty, p.k)) ||
+        (rc = delta_tensor(a->v, "v", d, d.v_heads, empty, p.v)) || (rc = delta_tensor(a->dout, "dout", d, d.heads, empty, p.g)) ||
+        (rc = delta_tensor(a->dq, "dq", d, d.q_heads, empty, p.dq)) ||
+        (rc = delta_tensor(a->dk, "dk", d, d.k_heads, empty, p.dk)) ||
+        (rc = delta_tensor(a->dv, "dv", d, d.v_heads, empty, p.dv)))
+        return rc;
+    if (!empty) {
+        if (!a->dbeta) return fail(SUBQ_ERR_INVALID_ARGUMENT, "dbeta is null");
+        const void* outs[] = {a->dq.data, a->dk.data, a->dv.data};
+        for (const void* in : {a->q.data, a->k.data, a->v.data, a->dout.data})
+            for (const void* out : outs)
+                if (in == out) return fail(SUBQ_ERR_ALIAS, "gradient outputs must not alias inputs");
+        if (outs[0] == outs[1] || outs[0] == outs[2] || outs[1] == outs[2])
+            return fail(SUBQ_ERR_ALIAS, "gradient outputs must be distinct buffers");
+    }
+    p.S_in = a->state_in;
+    p.dS_out = a->dstate_out;
+    p.dS_in = a->dstate_in;
+    p.dbeta = a->dbeta;
+    p.dlg = a->dlog_gamma;
+    return SUBQ_OK;
+}
+
+// Workspace of the backward: dS, Z, float32 gradients per state head of shared
+// q, k, v, and the forward's part where no handover is given.
+struct DeltaBwdBytes {
+    DeltaBytes fwd;
+    size_t dq, dk, dv, total;
+};
+DeltaBwdBytes delta_bwd_bytes(const subq::DeltaParams& p, int dtype, bool handover) {
+    DeltaBwdBytes n;
+    n.fwd = delta_bytes(p, dtype);
+    const size_t tokens = (size_t)p.B * p.H * p.N;
+    n.dq = p.q.group > 1 ? align_up(tokens * p.d * 4) : 0;
+    n.dk = p.k.group > 1 ? align_up(tokens * p.d * 4) : 0;
+    n.dv = p.v.group > 1 ? align_up(tokens * p.e * 4) : 0;
+    n.total = n.fwd.S0 + n.fwd.W + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.Y + n.fwd.S0 + n.fwd.W);
+    return n;
+}
+
+}  // namespace
+
+size_t subq_delta_handover_bytes(const subq_delta_desc* d) {
+    subq::DeltaParams p;
+    if (!d || check_delta(*d, p) != SUBQ_OK || p.d > 128) return 0;
+    const DeltaBytes n = delta_bytes(p, d->dtype);
+    return n.Y + n.S0 + n.W;
+}
+
+size_t subq_delta_fwd_workspace_bytes(const subq_delta_fwd_args* a) {
+    subq::DeltaParams p;
+    int path;
+    if (fill_delta_fwd(a, p, path) != SUBQ_OK || path != SUBQ_PATH_CHUNKED || a->handover) return 0;
+    return delta_bytes(p, a->desc.dtype).Y;
+}
+
+size_t subq_delta_bwd_workspace_bytes(const subq_delta_bwd_args* a) {
+    subq::DeltaParams p;
+    if (fill_delta_bwd(a, p) != SUBQ_OK) return 0;
+    return delta_bwd_bytes(p, a->desc.dtype, a->handover != nullptr).total;
+}
+
+int subq_delta_fwd(const subq_delta_fwd_args* a) {
+    subq::DeltaParams p;
+    int path, launches = 1;
+    int rc = fill_delta_fwd(a, p, path);
+    if (rc) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+    g_last_launches = 0;
+    if (p.B == 0 || p.H == 0 || (p.N == 0 && !p.S_out)) {
+        g_last_path = path;
+        return SUBQ_OK;
+    }
+    cudaError_t err;
+    if (path == SUBQ_PATH_EXACT || p.N == 0) {
+        err = subq::launch_delta_step(p, a->desc.dtype, st);
+    } else {
+        const DeltaBytes n = delta_bytes(p, a->desc.dtype);
+        if (a->handover) {
+            if (reinterpret_cast<uintptr_t>(a->handover) % kAlign != 0)
+                return fail(SUBQ_ERR_WORKSPACE, "handover must be 256-byte aligned");
+            delta_handover(p, n, a->handover);
+        } else {
+            if ((rc = check_workspace(a->workspace, a->workspace_bytes, n.Y))) return rc;
+            p.Y = static_cast<unsigned char*>(a->workspace);
+        }
+        err = subq::launch_delta_fwd(p, a->desc.dtype, st);
+        launches = 2;
+    }
+    if (err != cudaSuccess) return fail_cuda(err, "subq_delta_fwd launch");
+    g_last_path = path;
+    g_last_launches = launches;
+    return SUBQ_OK;
+}
+
+int subq_delta_bwd(const subq_delta_bwd_args* a) {
+    subq::DeltaParams p;
+    int rc = fill_delta_bwd(a, p);
+    if (rc) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+    g_last_launches = 0;
+    cudaError_t err = cudaSuccess;
+    if (p.B == 0 || p.H == 0 || p.N == 0) {  // no token: the state's gradient passes through
+        const size_t bytes = (size_t)p.B * p.H * p.d * p.e * sizeof(float);
+        if (p.dS_in && bytes && p.dS_in != p.dS_out)
+            err = p.dS_out ? cudaMemcpyAsync(p.dS_in, p.dS_out, bytes, cudaMemcpyDeviceToDevice, st)
+                           : cudaMemsetAsync(p.dS_in, 0, bytes, st);
+        g_last_path = SUBQ_PATH_CHUNKED;
+        return err == cudaSuccess ? (int)SUBQ_OK : fail_cuda(err, "subq_delta_bwd state gradient");
+    }
+    const int dt = a->desc.dtype;
+    const DeltaBwdBytes n = delta_bwd_bytes(p, dt, a->handover != nullptr);
+    if ((rc = check_workspace(a->workspace, a->workspace_bytes, n.total))) return rc;
+    unsigned char* at = static_cast<unsigned char*>(a->workspace);
+    auto take = [&](size_t bytes) {
+        unsigned char* x = at;
+        at += bytes;
+        return x;
+    };
+    p.dS = take(n.fwd.S0);
+    p.Z = take(n.fwd.W);
+    if (n.dq) p.dq32 = reinterpret_cast<float*>(take(n.dq));
+    if (n.dk) p.dk32 = reinterpret_cast<float*>(take(n.dk));
+    if (n.dv) p.dv32 = reinterpret_cast<float*>(take(n.dv));
+    int first = 0, launches = 0;
+    if (a->handover) {
+        if (reinterpret_cast<uintptr_t>(a->handover) % kAlign != 0)
+            return fail(SUBQ_ERR_WORKSPACE, "handover must be 256-byte aligned");
+        delta_handover(p, n.fwd, const_cast<void*>(a->handover));
+    } else {
+        delta_handover(p, n.fwd, at);
+        err = subq::launch_delta_fwd(p, dt, st);  // (o is null: states and corrections only)
+        first = 2;
+    }
+    if (err == cudaSuccess) err = subq::launch_delta_bwd(p, dt, st, &launches);
+    if (err != cudaSuccess) return fail_cuda(err, "subq_delta_bwd launch");
+    g_last_path = SUBQ_PATH_CHUNKED;
+    g_last_launches = first + launches;
+    return SUBQ_OK;
+}
+
+// ------------------------------------------------------------------ layer norm
+static int fill_ln(const subq_layer_norm_args* a, subq::LnParams& p, bool bwd) {
+    if (!a) return fail(SUBQ_ERR_INVALID_ARGUMENT, "null argument block");
+    if (a->rows < 0 || a->dim <= 0) return fail(SUBQ_ERR_INVALID_ARGUMENT, "negative rows or dim <= 0");
+    if (a->dim > (int64_t)1 << 24) return fail(SUBQ_ERR_UNSUPPORTED, "dim above 2^24 is not supported");
+    for (int32_t t : {a->x_dtype, a->y_dtype})
+        if (t != SUBQ_FP32 && t != SUBQ_FP16 && t != SUBQ_BF16)
+            return fail(SUBQ_ERR_INVALID_ARGUMENT, "layer norm supports float32, float16 and bfloat16");
+    if (a->x_dtype != a->y_dtype && a->x_dtype != SUBQ_FP32)
+        return fail(SUBQ_ERR_UNSUPPORTED, "x and y must share one dtype, or x be float32");
+    if (!(a->eps >= 0.f) || a->eps > 1e30f) return fail(SUBQ_ERR_INVALID_ARGUMENT, "eps must be >= 0 and finite");
+    auto check = [&](const void* q, int64_t stride, int dtype, const char* name) {
+        if (a->rows > 0 && !q) return fail(SUBQ_ERR_INVALID_ARGUMENT, std::string(name) + " is null");
+        if (reinterpret_cast<uintptr_t>(q) % elem_size(dtype) != 0)
+            return fail(SUBQ_ERR_INVALID_ARGUMENT, std::string(name) + " is not aligned to its element size");
+        if (stride < 0) return fail(SUBQ_ERR_INVALID_ARGUMENT, std::string(name) + " has a negative stride");
+        return (int)SUBQ_OK;
+    };
+    p = subq::LnParams{};
+    p.rows = a->rows; p.D = (int)a->dim; p.eps = a->eps; p.w = a->weight;
+    int rc = check(a->x, a->x_stride, a->x_dtype, "x");
+    if (rc) return rc;
+    p.x = a->x; p.x_s = a->x_stride;
+    if (!bwd) {
+        if ((rc = check(a->y, a->y_stride, a->y_dtype, "y"))) return rc;
+        p.y = a->y; p.y_s = a->y_stride;
+        p.b = a->bias;
+        return SUBQ_OK;
+    }
+    if ((rc = check(a->dy, a->dy_stride, a->y_dtype, "dy")) || (rc = check(a->dx, a->dx_stride, a->x_dtype, "dx"))) return rc;
+    p.dy = a->dy; p.dy_s = a->dy_stride;
+    p.dx = a->dx; p.dx_s = a->dx_stride;
+    p.dw = a->dweight;
+    p.db = a->dbias;
+    return SUBQ_OK;
+}
+
+size_t subq_layer_norm_bwd_workspace_bytes(const subq_layer_norm_args* a) {
+    subq::LnParams p;
+    if (fill_ln(a, p, true) != SUBQ_OK || (!p.dw && !p.db) || p.rows == 0) return 0;
+    return align_up(subq::ln_bwd_workspace_floats(p.rows, p.D) * sizeof(float));
+}
+
+int subq_layer_norm_fwd(const subq_layer_norm_args* a) {
+    subq::LnParams p;
+    int rc = fill_ln(a, p, false), launches = 0;
+    if (rc) return rc;
+    if (p.rows > 0) {
+        cudaError_t err = subq::launch_layer_norm(p, a->x_dtype, a->y_dtype, false, static_cast<cudaStream_t>(a->stream), &launches);
+        if (err != cudaSuccess) return fail_cuda(err, "subq_layer_norm_fwd launch");
+    }
+    g_last_launches = launches;
+    return SUBQ_OK;
+}
+
+int subq_layer_norm_bwd(const subq_layer_norm_args* a) {
+    subq::LnParams p;
+    int rc = fill_ln(a, p, true), launches = 0;
+    if (rc) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+    if (p.rows == 0) {  // no rows: the sums are 0
+        for (float* x : {p.dw, p.db}) {
+            cudaError_t err = x ? cudaMemsetAsync(x, 0, sizeof(float) * p.D, st) : cudaSuccess;
+            if (err != cudaSuccess) return fail_cuda(err, "subq_layer_norm_bwd dweight");
+        }
+        g_last_launches = 0;
+        return SUBQ_OK;
+    }
+    if (p.D > 8192 && (a->dx == a->x || a->dx == a->dy))
+        return fail(SUBQ_ERR_ALIAS, "dx must not be x or dy for dim above 8192 (rows are read more than once)");
+    if (p.dw || p.db) {
+        const size_t need = align_up(subq::ln_bwd_workspace_floats(p.rows, p.D) * sizeof(float));
+        if ((rc = check_workspace(a->workspace, a->workspace_bytes, need))) return rc;
+        p.part = static_cast<float*>(a->workspace);
+        const int64_t most = subq::kLnLongSlices;
+        p.stats = p.part + (size_t)2 * p.D * (p.rows < most ? p.rows : most);
+    }
+    cudaError_t err = subq::launch_layer_norm(p, a->x_dtype, a->y_dtype, true, st, &launches);
+    if (err != cudaSuccess) return fail_cuda(err, "subq_layer_norm_bwd launch");
+    g_last_launches = launches;
     return SUBQ_OK;
 }
 

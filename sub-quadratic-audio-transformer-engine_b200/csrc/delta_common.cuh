@@ -1,0 +1,412 @@
+// Shared pieces of the gated delta rule kernels (delta_step.cu, delta_fwd.cu,
+// delta_bwd.cu). Per (batch, head) sequence with live tokens t:
+//   S_t = gamma_t S_{t-1} + beta_t k_t w_t^T,   w_t = v_t - gamma_t S_{t-1}^T k_t,
+//   o_t = scale S_t^T q_t;   a masked token leaves S as it is and has o = 0.
+//
+// Chunk form (C = 64 tokens from the state S0; g = running sum of log gamma in
+// the chunk, G_ij = exp(g_i - g_j) for i >= j, A_ij = G_ij k_i.k_j for i > j):
+//   R = V - e^g (K S0),   W = R - Y (beta R),   Y = (I + A beta)^-1 A
+//   O = scale (e^g (Q S0) + (G o Q K^T) (beta W))
+//   S' = e^{g_C} S0 + K^T (e^{g_C - g} beta W)
+// Y is strictly lower triangular and depends on k and the gates alone, so it is
+// formed for all chunks at once; the walk over the chunks is two products deep.
+//
+// Precision: operands go through the bf16 tensor-core instruction as sums of
+// bf16 planes (a float is hi + lo to 2^-17, hi + mid + lo to 2^-25, relative),
+// products accumulate in float32. Inputs are held exactly (bf16: 1 plane, fp16:
+// 2, fp32: 3); what is computed in between (states, W, Y, scores) is held in
+// NX = 2 planes for 16-bit inputs and 3 for float32, and plane products whose
+// planes' indices sum to NX or more are below that precision and left out.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kernels.hpp"
+#include "scan_common.cuh"
+
+namespace subq {
+
+struct DeltaTensor {
+    void* p;
+    int64_t sb, sh, sn;
+    int group;  // heads of the state per head of this tensor
+    int vec;    // rows start on 16-byte boundaries and hold a multiple of 8 elements
+};
+
+struct DeltaGate {
+    const float* p;  // null: the neutral value
+    int64_t sb, sh, sn;
+};
+
+struct DeltaParams {
+    int B, H, N, d, e;
+    int nc;  // chunks of 64 tokens
+    float scale;
+    DeltaGate beta, lg;
+    const uint8_t* mask;
+    int64_t mask_sb;
+    DeltaTensor q, k, v, o;
+    const float* S_in;  // [B, H, d, e]
+    float* S_out;
+    unsigned char* Y;   // [B * H][nc][NX][10 blocks of 512 bytes]
+    unsigned char* S0;  // [B * H][nc][ep / 16][dp / 16][NX][512], or null (not stored)
+    unsigned char* W;   // [B * H][nc][ep / 16][4][NX][512], or null
+    // backward
+    DeltaTensor g, dq, dk, dv;
+    unsigned char* dS;  // gradient of the state after each chunk, like S0
+    unsigned char* Z;   // like W
+    float* dq32;        // [B, H, N, d] per state head when q is shared by a group, else null
+    float* dk32;
+    float* dv32;        // [B, H, N, e]
+    const float* dS_out;  // gradient of the final state, or null
+    float* dS_in;         // gradient of the initial state, or null
+    float* dbeta;         // [B, H, N]
+    float* dlg;           // [B, H, N] or null
+};
+
+constexpr int kDeltaC = 64;      // tokens per chunk
+constexpr int kDeltaCols = 32;   // value columns per CTA of the chunk walks
+constexpr int kYBlocks = 10;     // 16 x 16 blocks of the lower triangle of a 64 x 64 matrix
+constexpr float kMinLogGamma = -120.f;  // exp() of anything lower is 0 in float32 as well
+
+template <typename T> struct DeltaType;
+template <> struct DeltaType<__nv_bfloat16> { static constexpr int kIn = 1, kX = 2; };
+template <> struct DeltaType<__half> { static constexpr int kIn = 2, kX = 2; };
+template <> struct DeltaType<float> { static constexpr int kIn = 3, kX = 3; };
+
+namespace dl {
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four 8 x 8 matrices of 16-bit elements; lane l gives the address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void ldm(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldm_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_bf16(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+// (x, y) as NP pairs of bf16 whose sums are x and y to NP * 8 bits. An infinity
+// or NaN stays what it is in plane 0 and leaves NaN in the others.
+template <int NP>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&r)[NP]) {
+    r[0] = pack_bf16(x, y);
+#pragma unroll
+    for (int i = 1; i < NP; ++i) {
+        const float2 h = unpack_bf16(r[i - 1]);
+        x -= h.x;
+        y -= h.y;
+        r[i] = pack_bf16(x, y);
+    }
+}
+
+// c += A B over the plane pairs kept for NX planes of precision.
+template <int NA, int NB, int NX>
+__device__ __forceinline__ void mma_planes(float (&c)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][2]) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (i + j < NX) mma(c, a[i], b[j][0], b[j][1]);
+}
+
+// Accumulators of two neighbouring 8-column blocks (16 rows x 16 columns) as the
+// A operand of the next product, times per-column factors f0 (columns 2t, 2t + 1
+// of the first block) and f1 (of the second).
+template <int NX>
+__device__ __forceinline__ void to_a(const float (&c0)[4], const float (&c1)[4], float2 f0, float2 f1, uint32_t (&a)[NX][4]) {
+    uint32_t r[NX];
+    split2<NX>(c0[0] * f0.x, c0[1] * f0.y, r);
+#pragma unroll
+    for (int i = 0; i < NX; ++i) a[i][0] = r[i];
+    split2<NX>(c0[2] * f0.x, c0[3] * f0.y, r);
+#pragma unroll
+    for (int i = 0; i < NX; ++i) a[i][1] = r[i];
+    split2<NX>(c1[0] * f1.x, c1[1] * f1.y, r);
+#pragma unroll
+    for (int i = 0; i < NX; ++i) a[i][2] = r[i];
+    split2<NX>(c1[2] * f1.x, c1[3] * f1.y, r);
+#pragma unroll
+    for (int i = 0; i < NX; ++i) a[i][3] = r[i];
+}
+
+// ---- shared-memory tiles
+// Row-major [64][W] bf16 planes in 16-byte pieces; the piece index is XORed so
+// that 8 consecutive rows of one piece column fall into 8 different bank groups
+// (ldmatrix and the 16-byte stores are then free of conflicts).
+template <int W>
+__device__ __forceinline__ uint32_t tile_off(int row, int piece) {
+    static_assert(W == 32 || W == 64 || W == 128, "tile width");
+    if (W == 32) return (uint32_t)(row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+    return (uint32_t)(row * (W * 2) + ((piece ^ (row & 7)) << 4));
+}
+
+// B operand for two 8-column blocks, B[k][n] = tile[n][k]: rows n0 .. n0 + 15, pieces 2 kk, 2 kk + 1.
+// r[0], r[1]: the first block's; r[2], r[3]: the second's.
+template <int W>
+__device__ __forceinline__ void b_rows(uint32_t (&r)[4], uint32_t tile, int n0, int kk, int lane) {
+    const int m = lane >> 3;
+    ldm(r, tile + tile_off<W>(n0 + ((m >> 1) << 3) + (lane & 7), 2 * kk + (m & 1)));
+}
+// B[k][n] = tile[k][n]: rows k0 .. k0 + 15, columns 16 np .. 16 np + 15.
+template <int W>
+__device__ __forceinline__ void b_cols(uint32_t (&r)[4], uint32_t tile, int k0, int np, int lane) {
+    const int m = lane >> 3;
+    ldm_t(r, tile + tile_off<W>(k0 + ((m & 1) << 3) + (lane & 7), 2 * np + (m >> 1)));
+}
+// A[m][k] = tile[m][k]: rows m0 .. m0 + 15, pieces 2 kk, 2 kk + 1.
+template <int W>
+__device__ __forceinline__ void a_rows(uint32_t (&r)[4], uint32_t tile, int m0, int kk, int lane) {
+    const int m = lane >> 3;
+    ldm(r, tile + tile_off<W>(m0 + ((m & 1) << 3) + (lane & 7), 2 * kk + (m >> 1)));
+}
+// A[m][k] = tile[k][m]: rows k0 .. k0 + 15, columns 16 mp .. 16 mp + 15.
+template <int W>
+__device__ __forceinline__ void a_cols(uint32_t (&r)[4], uint32_t tile, int k0, int mp, int lane) {
+    const int m = lane >> 3;
+    ldm_t(r, tile + tile_off<W>(k0 + ((m >> 1) << 3) + (lane & 7), 2 * mp + (m & 1)));
+}
+
+// Block (ib, jb) of a lower triangular 64 x 64 matrix kept as 16 x 16 blocks of
+// four 8 x 8 matrices (128 bytes each, order: row half, column half).
+__device__ __forceinline__ int tri(int ib, int jb) { return (ib * (ib + 1) >> 1) + jb; }
+
+// ---- gates of one chunk
+struct Gates {
+    float gh[kDeltaC], gl[kDeltaC];  // running sum of log gamma: g = gh + gl
+    float beta[kDeltaC];             // 0 on masked tokens
+    float eg[kDeltaC];               // e^g
+    float kd[kDeltaC];               // e^{g_C - g}
+    int live[kDeltaC];
+    float eC;                        // e^{g_C}
+    int any;                         // live tokens in the chunk
+};
+
+__device__ __forceinline__ float gamma_ij(const Gates& s, int i, int j) {  // i >= j
+    return expf((s.gh[i] - s.gh[j]) + (s.gl[i] - s.gl[j]));
+}
+
+// Fills `s` for tokens n0 .. n0 + 63 (one warp, every lane).
+__device__ __forceinline__ void load_gates(Gates& s, const DeltaParams& p, int b, int h, int n0, int lane) {
+    double g[2];
+    float be[2];
+    int lv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int n = n0 + 2 * lane + i;
+        lv[i] = n < p.N && (!p.mask || p.mask[(int64_t)b * p.mask_sb + n] != 0);
+        be[i] = 0.f;
+        g[i] = 0.0;
+        if (lv[i]) {
+            be[i] = p.beta.p ? p.beta.p[b * p.beta.sb + h * p.beta.sh + n * p.beta.sn] : 1.f;
+            if (p.lg.p) {
+                const float x = p.lg.p[b * p.lg.sb + h * p.lg.sh + n * p.lg.sn];
+                g[i] = x < kMinLogGamma ? kMinLogGamma : x;
+            }
+        }
+    }
+    double run = g[0] + g[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += up;
+    }
+    const double total = __shfl_sync(0xffffffffu, run, 31);
+    const int any = __any_sync(0xffffffffu, lv[0] | lv[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const double gi = i ? run : run - g[1];
+        const int t = 2 * lane + i;
+        const float hi = (float)gi;
+        s.gh[t] = hi;
+        s.gl[t] = (float)(gi - (double)hi);
+        s.beta[t] = be[i];
+        s.eg[t] = expf((float)gi);
+        s.kd[t] = expf((float)(total - gi));
+        s.live[t] = lv[i];
+    }
+    if (lane == 0) {
+        s.eC = expf((float)total);
+        s.any = any;
+    }
+}
+
+// ---- loads of [64][W] tiles from global memory
+template <typename T> __device__ __forceinline__ float as_float(T x) { return to_f<T>(x); }
+
+// Eight elements of row `n` from column c (zeros past the tensor's width or for dead rows).
+template <typename T>
+__device__ __forceinline__ void load8(float (&f)[8], const T* row, int c, int width, bool vec) {
+    if (vec && c + 8 <= width) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 u = *reinterpret_cast<const uint4*>(row + c);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                T t[2];
+                *reinterpret_cast<uint32_t*>(t) = w[i];
+                f[2 * i] = as_float<T>(t[0]);
+                f[2 * i + 1] = as_float<T>(t[1]);
+            }
+        } else {
+            const float4 a = reinterpret_cast<const float4*>(row + c)[0], b = reinterpret_cast<const float4*>(row + c)[1];
+            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+            f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = c + i < width ? as_float<T>(row[c + i]) : 0.f;
+    }
+}
+
+// [64][W] tile of columns c0 .. c0 + W - 1 as NP bf16 planes; dead rows are zero
+// whatever memory holds there. NT threads, `tid` of them.
+template <typename T, int W, int NP, int NT>
+__device__ __forceinline__ void load_planes(unsigned char* tile, const DeltaTensor& x, int64_t base, int n0, int c0, int width,
+                                            const int* live, int tid) {
+    constexpr int kPieces = W / 8, kPer = 64 * kPieces / NT, kBatch = kPer < 4 ? kPer : 4;
+    static_assert(64 * kPieces % NT == 0, "threads per tile");
+    const T* src = static_cast<const T*>(x.p) + base;
+#pragma unroll
+    for (int u0 = 0; u0 < kPer; u0 += kBatch) {
+        float f[kBatch][8];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int idx = tid + (u0 + u) * NT, row = idx / kPieces, piece = idx % kPieces;
+            if (live[row]) {
+                load8<T>(f[u], src + (n0 + row) * x.sn, c0 + piece * 8, width, x.vec);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int idx = tid + (u0 + u) * NT, row = idx / kPieces, piece = idx % kPieces;
+            uint32_t r[4][NP];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split2<NP>(f[u][2 * i], f[u][2 * i + 1], r[i]);
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl)
+                *reinterpret_cast<uint4*>(tile + pl * (64 * W * 2) + tile_off<W>(row, piece)) =
+                    make_uint4(r[0][pl], r[1][pl], r[2][pl], r[3][pl]);
+        }
+    }
+}
+
+constexpr int kVPitch = 36;  // floats per row of a [64][32] float tile: rows two apart fall 8 banks apart
+
+template <typename T, int NT>
+__device__ __forceinline__ void load_float_tile(float* tile, const DeltaTensor& x, int64_t base, int n0, int c0, int width,
+                                                const int* live, int tid) {
+    constexpr int kPer = 64 * 4 / NT;
+    static_assert(kPer >= 1, "threads per tile");
+    const T* src = static_cast<const T*>(x.p) + base;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+        const int idx = tid + u * NT, row = idx >> 2, piece = idx & 3;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (live[row]) load8<T>(f, src + (n0 + row) * x.sn, c0 + piece * 8, width, x.vec);
+        float4* dst = reinterpret_cast<float4*>(tile + row * kVPitch + piece * 8);
+        dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+        dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ void copy16(unsigned char* dst, const unsigned char* src, int bytes, int tid) {
+    for (int i = tid * 16; i < bytes; i += NT * 16)
+        *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
+}
+
+__device__ __forceinline__ int64_t tensor_base(const DeltaTensor& x, int b, int h) {
+    return b * x.sb + (h / x.group) * x.sh;
+}
+
+// scale G o (Q K^T) (times beta_j with `with_beta`) for row block rb, as NX planes in `out`
+// (10 lower triangular blocks per plane).
+template <int DP, int NIN, int NX>
+__device__ __forceinline__ void score_rows(unsigned char* out, uint32_t q, uint32_t k, const Gates& s, float scale, bool with_beta,
+                                           int rb, int lane) {
+    constexpr int kTile = 64 * DP * 2;
+    float acc[8][4];
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+#pragma unroll 2
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        uint32_t a[NIN][4];
+#pragma unroll
+        for (int pl = 0; pl < NIN; ++pl) a_rows<DP>(a[pl], q + pl * kTile, 16 * rb, kk, lane);
+#pragma unroll
+        for (int jb = 0; jb < 4; ++jb) {
+            if (jb <= rb) {
+                uint32_t b0[NIN][2], b1[NIN][2];
+#pragma unroll
+                for (int pl = 0; pl < NIN; ++pl) {
+                    uint32_t r[4];
+                    b_rows<DP>(r, k + pl * kTile, 16 * jb, kk, lane);
+                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                }
+                mma_planes<NIN, NIN, NX>(acc[2 * jb], a, b0);
+                mma_planes<NIN, NIN, NX>(acc[2 * jb + 1], a, b1);
+            }
+        }
+    }
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int jb = 0; jb < 4; ++jb) {
+        if (jb > rb) continue;
+        unsigned char* blk = out + tri(rb, jb) * 512 + lane * 4;
+#pragma unroll
+        for (int jh = 0; jh < 2; ++jh)
+#pragma unroll
+            for (int ih = 0; ih < 2; ++ih) {
+                const int i = 16 * rb + 8 * ih + g, j = 16 * jb + 8 * jh + 2 * t;
+                float x = 0.f, y = 0.f;
+                if (j <= i) x = scale * gamma_ij(s, i, j) * acc[2 * jb + jh][2 * ih];
+                if (j + 1 <= i) y = scale * gamma_ij(s, i, j + 1) * acc[2 * jb + jh][2 * ih + 1];
+                if (with_beta) {
+                    x *= s.beta[j];
+                    y *= s.beta[j + 1];
+                }
+                uint32_t r[NX];
+                split2<NX>(x, y, r);
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl)
+                    *reinterpret_cast<uint32_t*>(blk + pl * (kYBlocks * 512) + (ih * 2 + jh) * 128) = r[pl];
+            }
+    }
+}
+
+}  // namespace dl
+}  // namespace subq

@@ -1,0 +1,463 @@
+// Chunked forward of the gated delta rule (see delta_common.cuh for the algebra).
+//
+// delta_prep_kernel: Y of every chunk, all chunks at once.
+// delta_chain_kernel: the walk over the chunks. A warp owns 16 value columns of
+// one sequence and keeps S^T [16 x d] in its accumulators: the m16n8k16
+// accumulator layout is the A operand layout of the next product, so the chain
+// S0 -> R -> W -> S' stays in one warp's registers and no warp waits for another
+// value column. All products are transposed accordingly (rows = value columns,
+// columns = tokens or d). Per CTA, 32 columns: two such chain warps, two output
+// warps (scores, Q S0 and score W products of the chain warp with the same
+// columns, from the S0 and W planes it leaves in shared memory) and four warps
+// that load and convert the next chunk.
+#include "delta_common.cuh"
+#include "delta_launch.h"
+#include "scan_launch.h"
+
+namespace subq {
+namespace {
+
+using namespace dl;
+
+// ------------------------------------------------------------------ Y per chunk
+template <typename T, int DP>
+struct PrepSmem {
+    static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
+    Gates s;
+    alignas(16) float A[kDeltaC][kDeltaC + 4];
+    alignas(128) unsigned char k[kIn * 64 * DP * 2];
+    alignas(128) unsigned char y[kX * kYBlocks * 512];
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kTile = 64 * DP * 2;
+    extern __shared__ __align__(128) unsigned char raw[];
+    PrepSmem<T, DP>& sm = *reinterpret_cast<PrepSmem<T, DP>*>(raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t chunk = blockIdx.x;  // bh * nc + c
+    const int64_t bh = chunk / p.nc;
+    const int c = (int)(chunk % p.nc), b = (int)(bh / p.H), h = (int)(bh % p.H), n0 = c * kDeltaC;
+    if (warp == 0) load_gates(sm.s, p, b, h, n0, lane);
+    __syncthreads();
+    if (!sm.s.any) return;  // no kernel reads Y of a dead chunk
+    load_planes<T, DP, NIN, 128>(sm.k, p.k, tensor_base(p.k, b, h), n0, 0, p.d, sm.s.live, tid);
+    __syncthreads();
+    {  // A, rows 16 warp .. 16 warp + 15
+        float acc[8][4];
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+        const uint32_t k = smem_addr(sm.k);
+        for (int kk = 0; kk < DP / 16; ++kk) {
+            uint32_t a[NIN][4];
+#pragma unroll
+            for (int pl = 0; pl < NIN; ++pl) a_rows<DP>(a[pl], k + pl * kTile, 16 * warp, kk, lane);
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb)
+                if (jb <= warp) {
+                    uint32_t b0[NIN][2], b1[NIN][2];
+#pragma unroll
+                    for (int pl = 0; pl < NIN; ++pl) {
+                        uint32_t r[4];
+                        b_rows<DP>(r, k + pl * kTile, 16 * jb, kk, lane);
+                        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                    }
+                    mma_planes<NIN, NIN, NX>(acc[2 * jb], a, b0);
+                    mma_planes<NIN, NIN, NX>(acc[2 * jb + 1], a, b1);
+                }
+        }
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+            if (n <= 2 * warp + 1)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int i = 16 * warp + 8 * (x >> 1) + g, j = 8 * n + 2 * t + (x & 1);
+                    sm.A[i][j] = j < i ? gamma_ij(sm.s, i, j) * acc[n][x] : 0.f;
+                }
+    }
+    __syncthreads();
+    if (tid < kDeltaC) {  // column tid of Y by forward substitution: y_i = A_i - sum_j A_ij beta_j y_j
+        const int col = tid;
+        float z[kDeltaC];  // beta_j y_j
+#pragma unroll
+        for (int i = 0; i < kDeltaC; ++i) {
+            float y = col < i ? sm.A[i][col] : 0.f, y1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < i; j += 4) {
+                const float4 a = *reinterpret_cast<const float4*>(&sm.A[i][j]);
+                y = fmaf(-a.x, z[j], y);
+                if (j + 1 < i) y1 = fmaf(-a.y, z[j + 1], y1);
+                if (j + 2 < i) y = fmaf(-a.z, z[j + 2], y);
+                if (j + 3 < i) y1 = fmaf(-a.w, z[j + 3], y1);
+            }
+            y = col < i ? y + y1 : 0.f;
+            z[i] = sm.s.beta[i] * y;
+            if ((i >> 4) >= (col >> 4)) {
+                unsigned char* at = sm.y + tri(i >> 4, col >> 4) * 512 + (((i >> 3) & 1) * 2 + ((col >> 3) & 1)) * 128 +
+                                    (i & 7) * 16 + (col & 7) * 2;
+                float rest = y;
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    const __nv_bfloat16 q = __float2bfloat16_rn(rest);
+                    *reinterpret_cast<__nv_bfloat16*>(at + pl * (kYBlocks * 512)) = q;
+                    rest -= __bfloat162float(q);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    copy16<128>(p.Y + chunk * (NX * kYBlocks * 512), sm.y, NX * kYBlocks * 512, tid);
+}
+
+// ------------------------------------------------------------------ the walk
+template <typename T, int DP>
+struct ChainSmem {
+    static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
+    // chunks in shared memory: the one at work and the next, where both fit (not float32 with d > 64)
+    static constexpr int kStages = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+    struct Stage {
+        alignas(128) unsigned char k[kIn * 64 * DP * 2];
+        alignas(128) unsigned char q[kIn * 64 * DP * 2];
+        alignas(128) unsigned char y[kX * kYBlocks * 512];
+        alignas(16) float v[kDeltaC * kVPitch];
+        Gates s;
+    } st[kStages];
+    alignas(128) unsigned char S0[2][2][DP / 16 * kX * 512];  // [chunk parity][chain warp]
+    alignas(128) unsigned char W[2][4 * kX * 512];
+    alignas(128) unsigned char P[kX * kYBlocks * 512];
+    alignas(16) unsigned char out[2][kDeltaC * (16 * sizeof(T) + 16)];
+};
+
+// S^T accumulators (16 value columns x DP) as planes of 8 x 8 matrices, to shared memory and (`dst`) global memory.
+template <int DP, int NX>
+__device__ __forceinline__ void store_state_planes(const float (&S)[DP / 8][4], unsigned char* tile, unsigned char* dst, int lane) {
+    const float2 one = make_float2(1.f, 1.f);
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        uint32_t a[NX][4];
+        to_a<NX>(S[2 * kk], S[2 * kk + 1], one, one, a);
+#pragma unroll
+        for (int pl = 0; pl < NX; ++pl)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int off = (kk * NX + pl) * 512 + m * 128 + lane * 4;
+                *reinterpret_cast<uint32_t*>(tile + off) = a[pl][m];
+                if (dst) *reinterpret_cast<uint32_t*>(dst + off) = a[pl][m];
+            }
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kTile = 64 * DP * 2;
+    constexpr int NST = ChainSmem<T, DP>::kStages;
+    extern __shared__ __align__(128) unsigned char raw[];
+    ChainSmem<T, DP>& sm = *reinterpret_cast<ChainSmem<T, DP>*>(raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    const int64_t bh = blockIdx.x / ncb;
+    const int cb = blockIdx.x % ncb, b = (int)(bh / p.H), h = (int)(bh % p.H), c0 = cb * kDeltaCols;
+    const int g = lane >> 2, t = lane & 3;
+
+    auto load_stage = [&](int c) {  // warps 4..7
+        auto& st = sm.st[c % NST];
+        const int lt = tid - 128, n0 = c * kDeltaC;
+        if (warp == 4) load_gates(st.s, p, b, h, n0, lane);
+        bar_sync(3, 128);
+        if (!st.s.any) return;
+        load_planes<T, DP, NIN, 128>(st.k, p.k, tensor_base(p.k, b, h), n0, 0, p.d, st.s.live, lt);
+        copy16<128>(st.y, p.Y + (bh * p.nc + c) * (NX * kYBlocks * 512), NX * kYBlocks * 512, lt);
+        load_float_tile<T, 128>(st.v, p.v, tensor_base(p.v, b, h), n0, c0, p.e, st.s.live, lt);
+        load_planes<T, DP, NIN, 128>(st.q, p.q, tensor_base(p.q, b, h), n0, 0, p.d, st.s.live, lt);
+    };
+
+    if (warp < 2) {  // ---------------------------------------------------- chain
+        float S[DP / 8][4];
+        const int col0 = c0 + 16 * warp;
+        const float* S_in = p.S_in ? p.S_in + bh * p.d * p.e : nullptr;
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 8 * n + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
+                S[n][i] = (S_in && d < p.d && col < p.e) ? S_in[(int64_t)d * p.e + col] : 0.f;
+            }
+        const int64_t cw = 2 * cb + warp;  // 16-column group
+        const int64_t ncw = 2 * ncb;
+        auto s0_at = [&](int c) {
+            return p.S0 && c < p.nc ? p.S0 + ((bh * p.nc + c) * ncw + cw) * (DP / 16 * NX * 512) : nullptr;
+        };
+        store_state_planes<DP, NX>(S, sm.S0[0][warp], s0_at(0), lane);
+        __syncthreads();
+        for (int c = 0; c < p.nc; ++c) {
+            if (NST == 1) __syncthreads();  // the chunk is loaded
+            auto& st = sm.st[c % NST];
+            const Gates& s = st.s;
+            if (s.any) {
+                const uint32_t kt = smem_addr(st.k), s0 = smem_addr(sm.S0[c & 1][warp]) + lane * 16;
+                float X[8][4];
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) X[n][i] = 0.f;
+#pragma unroll 2
+                for (int kk = 0; kk < DP / 16; ++kk) {  // X = S0^T K^T
+                    uint32_t a[NX][4];
+#pragma unroll
+                    for (int pl = 0; pl < NX; ++pl) ldm(a[pl], s0 + (kk * NX + pl) * 512);
+#pragma unroll
+                    for (int jp = 0; jp < 4; ++jp) {
+                        uint32_t b0[NIN][2], b1[NIN][2];
+#pragma unroll
+                        for (int pl = 0; pl < NIN; ++pl) {
+                            uint32_t r[4];
+                            b_rows<DP>(r, kt + pl * kTile, 16 * jp, kk, lane);
+                            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                        }
+                        mma_planes<NX, NIN, NX>(X[2 * jp], a, b0);
+                        mma_planes<NX, NIN, NX>(X[2 * jp + 1], a, b1);
+                    }
+                }
+                // R = V - e^g X, and -beta R as the operand
+                uint32_t ra[4][NX][4];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const int j = 8 * n + 2 * t;
+                    const float* v = st.v + j * kVPitch + 16 * warp + g;
+                    const float2 eg = *reinterpret_cast<const float2*>(&s.eg[j]);
+                    X[n][0] = fmaf(-eg.x, X[n][0], v[0]);
+                    X[n][1] = fmaf(-eg.y, X[n][1], v[kVPitch]);
+                    X[n][2] = fmaf(-eg.x, X[n][2], v[8]);
+                    X[n][3] = fmaf(-eg.y, X[n][3], v[kVPitch + 8]);
+                }
+#pragma unroll
+                for (int jb = 0; jb < 4; ++jb) {
+                    const float2 b0 = *reinterpret_cast<const float2*>(&s.beta[16 * jb + 2 * t]);
+                    const float2 b1 = *reinterpret_cast<const float2*>(&s.beta[16 * jb + 8 + 2 * t]);
+                    to_a<NX>(X[2 * jb], X[2 * jb + 1], make_float2(-b0.x, -b0.y), make_float2(-b1.x, -b1.y), ra[jb]);
+                }
+                // W^T = R^T - (beta R)^T Y^T
+                const uint32_t yt = smem_addr(st.y) + lane * 16;
+#pragma unroll
+                for (int ib = 0; ib < 4; ++ib)
+#pragma unroll
+                    for (int jb = 0; jb <= ib; ++jb) {
+                        uint32_t b0[NX][2], b1[NX][2];
+#pragma unroll
+                        for (int pl = 0; pl < NX; ++pl) {
+                            uint32_t r[4];
+                            ldm(r, yt + pl * (kYBlocks * 512) + tri(ib, jb) * 512);
+                            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                        }
+                        mma_planes<NX, NX, NX>(X[2 * ib], ra[jb], b0);
+                        mma_planes<NX, NX, NX>(X[2 * ib + 1], ra[jb], b1);
+                    }
+                // W planes for the output warp (and the backward)
+                unsigned char* wdst = p.W ? p.W + ((bh * p.nc + c) * ncw + cw) * (4 * NX * 512) : nullptr;
+#pragma unroll
+                for (int jb = 0; jb < 4; ++jb) {
+                    uint32_t a[NX][4];
+                    const float2 one = make_float2(1.f, 1.f);
+                    to_a<NX>(X[2 * jb], X[2 * jb + 1], one, one, a);
+#pragma unroll
+                    for (int pl = 0; pl < NX; ++pl)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const int off = (jb * NX + pl) * 512 + m * 128 + lane * 4;
+                            *reinterpret_cast<uint32_t*>(sm.W[warp] + off) = a[pl][m];
+                            if (wdst) *reinterpret_cast<uint32_t*>(wdst + off) = a[pl][m];
+                        }
+                }
+                bar_arrive(1, 128);
+                // S'^T = e^{g_C} S0^T + (e^{g_C - g} beta W)^T K
+#pragma unroll
+                for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[n][i] *= s.eC;
+#pragma unroll
+                for (int jb = 0; jb < 4; ++jb) {
+                    uint32_t a[NX][4];
+                    float2 f[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = 16 * jb + 8 * i + 2 * t;
+                        f[i] = make_float2(s.beta[j] * s.kd[j], s.beta[j + 1] * s.kd[j + 1]);
+                    }
+                    to_a<NX>(X[2 * jb], X[2 * jb + 1], f[0], f[1], a);
+#pragma unroll
+                    for (int np = 0; np < DP / 16; ++np) {
+                        uint32_t b0[NIN][2], b1[NIN][2];
+#pragma unroll
+                        for (int pl = 0; pl < NIN; ++pl) {
+                            uint32_t r[4];
+                            b_cols<DP>(r, kt + pl * kTile, 16 * jb, np, lane);
+                            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                        }
+                        mma_planes<NX, NIN, NX>(S[2 * np], a, b0);
+                        mma_planes<NX, NIN, NX>(S[2 * np + 1], a, b1);
+                    }
+                }
+            } else {
+                bar_arrive(1, 128);
+            }
+            store_state_planes<DP, NX>(S, sm.S0[(c + 1) & 1][warp], s0_at(c + 1), lane);
+            __syncthreads();
+        }
+        if (p.S_out) {
+            float* S_out = p.S_out + bh * p.d * p.e;
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = 8 * n + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
+                    if (d < p.d && col < p.e) S_out[(int64_t)d * p.e + col] = S[n][i];
+                }
+        }
+    } else if (warp < 4) {  // -------------------------------------------- outputs
+        const int w = warp - 2;
+        T* o = p.o.p ? static_cast<T*>(p.o.p) + tensor_base(p.o, b, h) : nullptr;  // null: states and W only
+        constexpr int kPitch = 16 * sizeof(T) + 16;
+        __syncthreads();
+        for (int c = 0; c < p.nc; ++c) {
+            if (NST == 1) __syncthreads();  // the chunk is loaded
+            auto& st = sm.st[c % NST];
+            const Gates& s = st.s;
+            const int n0 = c * kDeltaC, rows = min(kDeltaC, p.N - n0);
+            unsigned char* stage = sm.out[w];
+            if (s.any && o) {
+                const uint32_t kt = smem_addr(st.k), qt = smem_addr(st.q);
+                score_rows<DP, NIN, NX>(sm.P, qt, kt, s, p.scale, true, w ? 1 : 0, lane);
+                score_rows<DP, NIN, NX>(sm.P, qt, kt, s, p.scale, true, w ? 2 : 3, lane);
+                float O[8][4];
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) O[n][i] = 0.f;
+                const uint32_t s0 = smem_addr(sm.S0[c & 1][w]) + lane * 16;
+#pragma unroll 2
+                for (int kk = 0; kk < DP / 16; ++kk) {  // S0^T Q^T
+                    uint32_t a[NX][4];
+#pragma unroll
+                    for (int pl = 0; pl < NX; ++pl) ldm(a[pl], s0 + (kk * NX + pl) * 512);
+#pragma unroll
+                    for (int jp = 0; jp < 4; ++jp) {
+                        uint32_t b0[NIN][2], b1[NIN][2];
+#pragma unroll
+                        for (int pl = 0; pl < NIN; ++pl) {
+                            uint32_t r[4];
+                            b_rows<DP>(r, qt + pl * kTile, 16 * jp, kk, lane);
+                            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                        }
+                        mma_planes<NX, NIN, NX>(O[2 * jp], a, b0);
+                        mma_planes<NX, NIN, NX>(O[2 * jp + 1], a, b1);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const float2 eg = *reinterpret_cast<const float2*>(&s.eg[8 * n + 2 * t]);
+                    O[n][0] *= p.scale * eg.x;
+                    O[n][1] *= p.scale * eg.y;
+                    O[n][2] *= p.scale * eg.x;
+                    O[n][3] *= p.scale * eg.y;
+                }
+                bar_sync(1, 128);  // both output warps' scores and both chain warps' W
+                const uint32_t wt = smem_addr(sm.W[w]) + lane * 16, pt = smem_addr(sm.P) + lane * 16;
+#pragma unroll
+                for (int jb = 0; jb < 4; ++jb) {
+                    uint32_t a[NX][4];
+#pragma unroll
+                    for (int pl = 0; pl < NX; ++pl) ldm(a[pl], wt + (jb * NX + pl) * 512);
+#pragma unroll
+                    for (int ib = jb; ib < 4; ++ib) {
+                        uint32_t b0[NX][2], b1[NX][2];
+#pragma unroll
+                        for (int pl = 0; pl < NX; ++pl) {
+                            uint32_t r[4];
+                            ldm(r, pt + pl * (kYBlocks * 512) + tri(ib, jb) * 512);
+                            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                        }
+                        mma_planes<NX, NX, NX>(O[2 * ib], a, b0);
+                        mma_planes<NX, NX, NX>(O[2 * ib + 1], a, b1);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    T* r0 = reinterpret_cast<T*>(stage + (8 * n + 2 * t) * kPitch);
+                    T* r1 = reinterpret_cast<T*>(stage + (8 * n + 2 * t + 1) * kPitch);
+                    r0[g] = from_f<T>(O[n][0]);
+                    r1[g] = from_f<T>(O[n][1]);
+                    r0[g + 8] = from_f<T>(O[n][2]);
+                    r1[g + 8] = from_f<T>(O[n][3]);
+                }
+                __syncwarp();
+            } else {
+                bar_sync(1, 128);
+            }
+            const int col0 = c0 + 16 * w, width = min(16, p.e - col0);
+            const bool whole = p.o.vec && width == 16;
+            constexpr int kPieces = 16 * sizeof(T) / 16;  // 16-byte pieces of a row of 16 columns
+            for (int i = lane; o && i < rows * kPieces; i += 32) {
+                const int row = i / kPieces, piece = i % kPieces;
+                T* dst = o + (n0 + row) * p.o.sn + col0;
+                const bool live = s.any && s.live[row];
+                const unsigned char* src = stage + row * kPitch + piece * 16;
+                if (whole) {
+                    reinterpret_cast<uint4*>(dst)[piece] =
+                        live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+                } else {
+                    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+                    for (int x = 0; x < kPer; ++x)
+                        if (piece * kPer + x < width)
+                            dst[piece * kPer + x] = live ? reinterpret_cast<const T*>(src)[x] : from_f<T>(0.f);
+                }
+            }
+            __syncthreads();
+        }
+    } else {  // ---------------------------------------------------------- loads
+        if (NST == 2) load_stage(0);
+        __syncthreads();
+        for (int c = 0; c < p.nc; ++c) {
+            if (NST == 1) {
+                load_stage(c);
+                __syncthreads();
+            } else if (c + 1 < p.nc) {
+                load_stage(c + 1);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+template <typename T, int DP>
+cudaError_t fwd_t(const DeltaParams& p, cudaStream_t st) {
+    const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    const size_t prep = sizeof(PrepSmem<T, DP>), chain = sizeof(ChainSmem<T, DP>);
+    static_assert(sizeof(ChainSmem<T, DP>) <= 227 * 1024, "shared memory");
+    cudaError_t err = cudaFuncSetAttribute(delta_prep_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prep);
+    if (err == cudaSuccess)
+        err = cudaFuncSetAttribute(delta_chain_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chain);
+    if (err != cudaSuccess) return err;
+    delta_prep_kernel<T, DP><<<(unsigned)(bh * p.nc), 128, prep, st>>>(p);
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    delta_chain_kernel<T, DP><<<(unsigned)(bh * ncb), 256, chain, st>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_delta_fwd(const DeltaParams& p, int dtype, cudaStream_t st) {
+    if (p.d <= 64) {
+        if (dtype == SUBQ_BF16) return fwd_t<__nv_bfloat16, 64>(p, st);
+        if (dtype == SUBQ_FP16) return fwd_t<__half, 64>(p, st);
+        return fwd_t<float, 64>(p, st);
+    }
+    if (dtype == SUBQ_BF16) return fwd_t<__nv_bfloat16, 128>(p, st);
+    if (dtype == SUBQ_FP16) return fwd_t<__half, 128>(p, st);
+    return fwd_t<float, 128>(p, st);
+}
+
+}  // namespace subq

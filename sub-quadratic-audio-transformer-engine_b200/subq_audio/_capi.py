@@ -33,6 +33,9 @@ EXPORTED = (
     "subq_abi_version", "subq_device_info", "subq_device_status", "subq_bwd_noalloc",
     "subq_segment_states_bytes", "subq_selftest_wait_timeout",
     "subq_head_rmsnorm_fwd", "subq_head_rmsnorm_bwd", "subq_head_rmsnorm_bwd_workspace_bytes",
+    "subq_delta_fwd", "subq_delta_bwd", "subq_delta_fwd_workspace_bytes", "subq_delta_bwd_workspace_bytes",
+    "subq_delta_handover_bytes",
+    "subq_layer_norm_fwd", "subq_layer_norm_bwd", "subq_layer_norm_bwd_workspace_bytes",
 )
 
 
@@ -84,6 +87,51 @@ class RmsArgs(ctypes.Structure):
         ("weight", ctypes.c_void_p), ("dweight", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
         ("stream", ctypes.c_void_p),
+    ]
+
+
+class Gate(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64),
+                ("stride_h", ctypes.c_int64), ("stride_n", ctypes.c_int64)]
+
+
+class DeltaDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("seq_len", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64), ("value_dim", ctypes.c_int64),
+        ("q_heads", ctypes.c_int64), ("k_heads", ctypes.c_int64), ("v_heads", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("path", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("beta", Gate), ("log_gamma", Gate),
+        ("mask", ctypes.c_void_p), ("mask_stride_b", ctypes.c_int64),
+    ]
+
+
+class DeltaFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("desc", DeltaDesc), ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("o", Tensor4),
+        ("state_in", ctypes.c_void_p), ("state_out", ctypes.c_void_p), ("handover", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class DeltaBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("desc", DeltaDesc), ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("dout", Tensor4),
+        ("dq", Tensor4), ("dk", Tensor4), ("dv", Tensor4),
+        ("state_in", ctypes.c_void_p), ("dstate_out", ctypes.c_void_p), ("dstate_in", ctypes.c_void_p),
+        ("dbeta", ctypes.c_void_p), ("dlog_gamma", ctypes.c_void_p), ("handover", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("dim", ctypes.c_int64), ("x_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64),
+        ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64), ("dx", ctypes.c_void_p), ("dx_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
     ]
 
 
@@ -141,6 +189,16 @@ def load() -> ctypes.CDLL:
                 getattr(lib, name).restype = ctypes.c_int
             lib.subq_head_rmsnorm_bwd_workspace_bytes.argtypes = [ctypes.POINTER(RmsArgs)]
             lib.subq_head_rmsnorm_bwd_workspace_bytes.restype = ctypes.c_size_t
+            for name, args in (("subq_delta_fwd", DeltaFwdArgs), ("subq_delta_bwd", DeltaBwdArgs),
+                               ("subq_layer_norm_fwd", LayerNormArgs), ("subq_layer_norm_bwd", LayerNormArgs)):
+                getattr(lib, name).argtypes = [ctypes.POINTER(args)]
+                getattr(lib, name).restype = ctypes.c_int
+            for name, args in (("subq_delta_fwd_workspace_bytes", DeltaFwdArgs),
+                               ("subq_delta_bwd_workspace_bytes", DeltaBwdArgs),
+                               ("subq_delta_handover_bytes", DeltaDesc),
+                               ("subq_layer_norm_bwd_workspace_bytes", LayerNormArgs)):
+                getattr(lib, name).argtypes = [ctypes.POINTER(args)]
+                getattr(lib, name).restype = ctypes.c_size_t
             _lib = lib
     return _lib
 
@@ -176,6 +234,38 @@ def head_rmsnorm_bwd(args: RmsArgs) -> None:
 
 def head_rmsnorm_bwd_workspace_bytes(args: RmsArgs) -> int:
     return int(load().subq_head_rmsnorm_bwd_workspace_bytes(ctypes.byref(args)))
+
+
+def delta_fwd(args: DeltaFwdArgs) -> None:
+    check(load().subq_delta_fwd(ctypes.byref(args)))
+
+
+def delta_bwd(args: DeltaBwdArgs) -> None:
+    check(load().subq_delta_bwd(ctypes.byref(args)))
+
+
+def delta_fwd_workspace_bytes(args: DeltaFwdArgs) -> int:
+    return int(load().subq_delta_fwd_workspace_bytes(ctypes.byref(args)))
+
+
+def delta_bwd_workspace_bytes(args: DeltaBwdArgs) -> int:
+    return int(load().subq_delta_bwd_workspace_bytes(ctypes.byref(args)))
+
+
+def delta_handover_bytes(desc: DeltaDesc) -> int:
+    return int(load().subq_delta_handover_bytes(ctypes.byref(desc)))
+
+
+def layer_norm_fwd(args: LayerNormArgs) -> None:
+    check(load().subq_layer_norm_fwd(ctypes.byref(args)))
+
+
+def layer_norm_bwd(args: LayerNormArgs) -> None:
+    check(load().subq_layer_norm_bwd(ctypes.byref(args)))
+
+
+def layer_norm_bwd_workspace_bytes(args: LayerNormArgs) -> int:
+    return int(load().subq_layer_norm_bwd_workspace_bytes(ctypes.byref(args)))
 
 
 def fwd_workspace_bytes(args: FwdArgs) -> int:

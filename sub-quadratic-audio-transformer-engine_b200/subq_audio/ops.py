@@ -420,6 +420,345 @@ def head_rmsnorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[to
     return dx, dw
 
 
+# ------------------------------------------------------------- gated delta rule
+Gate = Union[None, float, torch.Tensor]
+
+
+class DeltaHandover:
+    """Carrier of what ``gated_delta_forward`` leaves for the backward of the
+    same call (its per-chunk states, corrections and triangular factors): pass
+    one instance as ``handover=`` to the forward, which fills it, and then to
+    ``gated_delta_backward``, which otherwise forms them again. The backward
+    refuses a carrier from a call of another shape, type or device; one from a
+    call of the same shape but other inputs gives wrong gradients."""
+
+    def __init__(self) -> None:
+        self.buf: Optional[torch.Tensor] = None
+        self.key: Optional[tuple] = None
+
+
+def _gate(x: Gate, name: str, q: torch.Tensor, H: int, N: int, keep: list) -> _capi.Gate:
+    """None, a number, or a tensor [], [H] or broadcastable to [B, H, N]; float32 strides as they come."""
+    g = _capi.Gate()
+    if x is None:
+        return g
+    B = q.shape[0]
+    if not isinstance(x, torch.Tensor):
+        x = torch.full((), float(x), dtype=torch.float32, device=q.device)
+    elif x.device != q.device:
+        raise ValueError(f"{name} must be on the device of q")
+    t = x.detach()
+    if t.dtype != torch.float32:
+        if not t.is_floating_point():
+            raise TypeError(f"{name} must be a floating-point tensor, got {t.dtype}")
+        t = t.to(torch.float32)
+    if t.dim() == 1:
+        if t.shape[0] != H:
+            raise ValueError(f"{name} must have shape [], [H] or [B, H, N] = [{B}, {H}, {N}], got {tuple(t.shape)}")
+        t = t.view(1, H, 1)
+    if tuple(t.shape) != (B, H, N):
+        if t.dim() not in (0, 3) or any(a not in (1, b) for a, b in zip(t.shape, (B, H, N))):
+            raise ValueError(f"{name} must have shape [], [H] or [B, H, N] = [{B}, {H}, {N}], got {tuple(t.shape)}")
+        t = t.expand(B, H, N)
+    keep.append(t)
+    g.data = t.data_ptr()
+    g.stride_b, g.stride_h, g.stride_n = t.stride()
+    return g
+
+
+def _delta_heads(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: Gate, log_gamma: Gate) -> int:
+    """Checks q [B, Hq, N, d], k [B, Hk, N, d] and v [B, Hv, N, e]; returns H, the heads of the state:
+    those of a [B, H, N] or [H] gate, else the most that q, k or v have."""
+    if any(t.dim() != 4 for t in (q, k, v)):
+        raise ValueError("q, k and v must be [B, heads, N, dim] tensors")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must share one dtype")
+    if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {q.dtype}; use float32, float16 or bfloat16")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must be on one device")
+    B, _, N, d = q.shape
+    H = max(q.shape[1], k.shape[1], v.shape[1])
+    for g in (beta, log_gamma):
+        if isinstance(g, torch.Tensor) and g.dim() in (1, 3):
+            H = max(H, g.shape[0] if g.dim() == 1 else g.shape[1])
+    if (k.shape[0] != B or k.shape[2] != N or k.shape[3] != d or v.shape[0] != B or v.shape[2] != N
+            or any(t.shape[1] < 1 or H % t.shape[1] for t in (q, k, v))):
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} with {H} heads "
+                         "(the heads of each must divide it)")
+    return H
+
+
+def _delta_desc(desc: _capi.DeltaDesc, q, k, v, beta, log_gamma, mask, scale, path: str, H: int, keep: list) -> None:
+    B, _, N, d = q.shape
+    desc.batch, desc.heads, desc.seq_len, desc.head_dim, desc.value_dim = B, H, N, d, v.shape[-1]
+    desc.q_heads, desc.k_heads, desc.v_heads = q.shape[1], k.shape[1], v.shape[1]
+    desc.dtype = _DTYPES[q.dtype]
+    if path not in _PATHS:
+        raise ValueError(f"unknown path {path!r}")
+    desc.path = _PATHS[path]
+    desc.scale = d ** -0.5 if scale is None else float(scale)
+    desc.beta = _gate(beta, "beta", q, H, N, keep)
+    desc.log_gamma = _gate(log_gamma, "log_gamma", q, H, N, keep)
+    if mask is not None:
+        m = mask.detach()
+        if m.dim() != 2 or m.shape[0] != B or m.shape[1] != N:
+            raise ValueError(f"mask must be [B, N] = [{B}, {N}], got {tuple(m.shape)}")
+        if m.device != q.device:
+            raise ValueError("mask must be on the device of q")
+        if m.dtype == torch.bool and m.stride(1) == 1:
+            m = m.view(torch.uint8)
+        elif m.dtype != torch.uint8 or m.stride(1) != 1:
+            m = (m != 0).to(torch.uint8).contiguous()
+        keep.append(m)
+        desc.mask = m.data_ptr()
+        desc.mask_stride_b = m.stride(0)
+
+
+def _delta_state(state: Optional[torch.Tensor], name: str, q: torch.Tensor, shape, keep: list) -> Optional[int]:
+    if state is None:
+        return None
+    if tuple(state.shape) != shape:
+        raise ValueError(f"{name} must be [B, H, d, e] = {list(shape)}, got {tuple(state.shape)}")
+    if state.device != q.device:
+        raise ValueError(f"{name} must be on the device of q")
+    s = state.detach().to(torch.float32).contiguous()
+    keep.append(s)
+    return s.data_ptr()
+
+
+def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: Gate, *, log_gamma: Gate = None,
+                        mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                        state: Optional[torch.Tensor] = None, return_state: bool = False, path: str = "auto",
+                        out: Optional[torch.Tensor] = None, handover: Optional[DeltaHandover] = None):
+    """The gated delta rule. Returns ``(o, S | None)``; S [B, H, d, e] is float32.
+
+        S_t = gamma_t S_{t-1} + beta_t k_t (v_t - gamma_t S_{t-1}^T k_t)^T,   o_t = scale S_t^T q_t
+
+    ``q``, ``k`` [B, heads, N, d] and ``v`` [B, heads, N, e] (float32, float16 or
+    bfloat16) may each have fewer heads than the state's H (a divisor: head h
+    reads head h // (H // heads)); H is that of a [B, H, N] or [H] ``beta`` or
+    ``log_gamma``, else the most that q, k and v have. ``beta`` (None is 1) and
+    ``log_gamma`` (None is no decay) are a number or a tensor [], [H] or
+    [B, H, N], used in float32. ``mask`` [B, N]: a masked token leaves the state
+    as it is, its output is 0 and nothing of it is read. ``scale`` defaults to
+    d ** -0.5. For bounded states keys should have at most unit length.
+    Paths: "exact" is the token-recurrent kernel (d <= 256; the automatic choice
+    for up to 16 tokens), "chunked" the chunk kernels (d <= 128).
+    """
+    _require_cuda(q, k, v)
+    H = _delta_heads(q, k, v, beta, log_gamma)
+    q, k, v = _inner_contig(q), _inner_contig(k), _inner_contig(v)
+    B, _, N, d = q.shape
+    e = v.shape[-1]
+    keep: list = []
+    with torch.cuda.device(q.device):
+        if out is None:
+            o = _empty_in_order(q, (B, H, N, e), q.dtype)
+        else:
+            o = out
+            if tuple(o.shape) != (B, H, N, e) or o.dtype != q.dtype or o.device != q.device:
+                raise ValueError(f"out must be [B, H, N, e] = {[B, H, N, e]} of {q.dtype} on the device of q")
+        a = _capi.DeltaFwdArgs()
+        _delta_desc(a.desc, q, k, v, beta, log_gamma, mask, scale, path, H, keep)
+        a.q, a.k, a.v, a.o = _t4(q), _t4(k), _t4(v), _t4(o)
+        a.state_in = _delta_state(state, "state", q, (B, H, d, e), keep)
+        S_out = None
+        if return_state:
+            S_out = torch.empty((B, H, d, e), dtype=torch.float32, device=q.device)
+            a.state_out = S_out.data_ptr()
+        a.stream = torch.cuda.current_stream(q.device).cuda_stream
+        if handover is not None:
+            nbytes = _capi.delta_handover_bytes(a.desc)
+            handover.buf = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+            handover.key = (B, H, N, d, e, q.dtype, q.device)
+            if handover.buf is not None:
+                a.handover = handover.buf.data_ptr()
+        if handover is None or handover.buf is None:
+            a.workspace, a.workspace_bytes = _workspace(_capi.delta_fwd_workspace_bytes(a), q.device, keep)
+        _capi.delta_fwd(a)
+    return o, S_out
+
+
+def gated_delta_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: Gate, dout: torch.Tensor, *,
+                         log_gamma: Gate = None, mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                         state: Optional[torch.Tensor] = None, dstate: Optional[torch.Tensor] = None,
+                         need_dlog_gamma: bool = False, need_dstate: bool = False,
+                         handover: Optional[DeltaHandover] = None):
+    """Gradients of ``gated_delta_forward`` (d <= 128). Returns ``(dq, dk, dv,
+    dbeta, dlog_gamma | None, dstate | None)``: dq, dk, dv in the inputs' type
+    and heads (summed over a group in float32), dbeta and dlog_gamma float32
+    [B, H, N] per token (0 on masked ones), dstate float32, the gradient of
+    ``state``. ``dstate`` is the gradient of the returned state (None: 0)."""
+    _require_cuda(q, k, v, dout)
+    H = _delta_heads(q, k, v, beta, log_gamma)
+    q, k, v, dout = _inner_contig(q), _inner_contig(k), _inner_contig(v), _inner_contig(dout)
+    B, _, N, d = q.shape
+    e = v.shape[-1]
+    if tuple(dout.shape) != (B, H, N, e) or dout.device != q.device:
+        raise ValueError(f"dout must be [B, H, N, e] = {[B, H, N, e]} on the device of q, got {tuple(dout.shape)}")
+    if dout.dtype != q.dtype:
+        dout = dout.to(q.dtype)
+    keep: list = []
+    with torch.cuda.device(q.device):
+        dq = _empty_in_order(q, tuple(q.shape), q.dtype)
+        dk = _empty_in_order(k, tuple(k.shape), q.dtype)
+        dv = _empty_in_order(v, tuple(v.shape), q.dtype)
+        dgates = torch.empty((2 if need_dlog_gamma else 1, B, H, N), dtype=torch.float32, device=q.device)
+        a = _capi.DeltaBwdArgs()
+        _delta_desc(a.desc, q, k, v, beta, log_gamma, mask, scale, "auto", H, keep)
+        a.q, a.k, a.v, a.dout = _t4(q), _t4(k), _t4(v), _t4(dout)
+        a.dq, a.dk, a.dv = _t4(dq), _t4(dk), _t4(dv)
+        a.state_in = _delta_state(state, "state", q, (B, H, d, e), keep)
+        a.dstate_out = _delta_state(dstate, "dstate", q, (B, H, d, e), keep)
+        dS = None
+        if need_dstate:
+            dS = torch.empty((B, H, d, e), dtype=torch.float32, device=q.device)
+            a.dstate_in = dS.data_ptr()
+        a.dbeta = dgates[0].data_ptr()
+        dlg = dgates[1] if need_dlog_gamma else None
+        if dlg is not None:
+            a.dlog_gamma = dlg.data_ptr()
+        a.stream = torch.cuda.current_stream(q.device).cuda_stream
+        if handover is not None and handover.buf is not None:
+            if handover.key != (B, H, N, d, e, q.dtype, q.device):
+                raise ValueError("handover comes from a forward of another shape, type or device")
+            a.handover = handover.buf.data_ptr()
+        a.workspace, a.workspace_bytes = _workspace(_capi.delta_bwd_workspace_bytes(a), q.device, keep)
+        _capi.delta_bwd(a)
+    return dq, dk, dv, dgates[0], dlg, dS
+
+
+class GatedDeltaStep:
+    """Streaming decode of the gated delta rule over preallocated device
+    buffers: ``DecodeStep``'s counterpart, with the same use.
+
+    ``q``, ``k`` [B, heads, T, d], ``v`` [B, heads, T, e] and ``out``
+    [B, H, T, e] hold the step's T new tokens (usually 1), ``S`` [B, H, d, e] is
+    the contiguous float32 state. ``beta`` and ``log_gamma`` are None, or
+    float32 tensors [B, H, T] or [H] (any strides) that are read at each step;
+    ``mask`` a bool or uint8 [B, T] tensor. ``step()`` enqueues one call on the
+    current stream: out = the rule's outputs from S, then S <- the state after
+    them. It allocates nothing and does not synchronise, so a CUDA graph can
+    capture it; refill the buffers in place between steps."""
+
+    def __init__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: Optional[torch.Tensor],
+                 out: torch.Tensor, S: torch.Tensor, *, log_gamma: Optional[torch.Tensor] = None,
+                 mask: Optional[torch.Tensor] = None, scale: Optional[float] = None, path: str = "auto"):
+        _require_cuda(q, k, v, out, S)
+        H = _delta_heads(q, k, v, beta, log_gamma)
+        B, _, T, d = q.shape
+        e = v.shape[-1]
+        if any(t.shape[-1] > 1 and t.stride(-1) != 1 for t in (q, k, v, out)):
+            raise ValueError("q, k, v and out must have a contiguous last dimension")
+        if tuple(out.shape) != (B, H, T, e) or out.dtype != q.dtype or out.device != q.device:
+            raise ValueError(f"out must be {(B, H, T, e)} of {q.dtype} on the device of q")
+        if S.dtype != torch.float32 or tuple(S.shape) != (B, H, d, e) or not S.is_contiguous() or S.device != q.device:
+            raise ValueError(f"S must be a contiguous float32 [{B}, {H}, {d}, {e}] tensor on the device of q")
+        # the step must read the caller's buffers, not copies made at set-up
+        for name, g in (("beta", beta), ("log_gamma", log_gamma)):
+            if g is not None and (not isinstance(g, torch.Tensor) or g.dtype != torch.float32):
+                raise ValueError(f"{name} must be None or a float32 tensor")
+        if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.dim() != 2 or mask.stride(1) != 1):
+            raise ValueError("mask must be a bool or uint8 [B, T] tensor with contiguous rows")
+        self._keep: list = [q, k, v, out, S]
+        a = _capi.DeltaFwdArgs()
+        _delta_desc(a.desc, q, k, v, beta, log_gamma, mask, scale, path, H, self._keep)
+        a.q, a.k, a.v, a.o = _t4(q), _t4(k), _t4(v), _t4(out)
+        a.state_in = a.state_out = S.data_ptr()
+        self.device = q.device
+        with torch.cuda.device(q.device):
+            a.workspace, a.workspace_bytes = _workspace(_capi.delta_fwd_workspace_bytes(a), q.device, self._keep)
+        self._args = a
+
+    def step(self) -> None:
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.step()
+        self._args.stream = torch.cuda.current_stream(self.device).cuda_stream
+        _capi.delta_fwd(self._args)
+
+
+# ------------------------------------------------------------------- layer norm
+def _ln_check(x: torch.Tensor, y_dtype: torch.dtype) -> None:
+    half = (torch.float16, torch.bfloat16)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layer_norm needs a last dimension of at least 1")
+    if x.dtype not in (torch.float32,) + half or (y_dtype != x.dtype and not (x.dtype == torch.float32 and y_dtype in half)):
+        raise TypeError(f"layer_norm takes float32, float16 or bfloat16 (and float32 into a 16-bit type), not {x.dtype} into {y_dtype}")
+
+
+def _ln_rows(t: torch.Tensor) -> torch.Tensor:
+    """[rows, D] with contiguous rows: a view where the leading dimensions merge, else a copy."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _ln_param(w: Optional[torch.Tensor], name: str, x: torch.Tensor, keep: list) -> Optional[int]:
+    if w is None:
+        return None
+    if tuple(w.shape) != (x.shape[-1],):
+        raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
+    if w.device != x.device:
+        raise ValueError(f"{name} must be on the device of x")
+    w = w.detach().to(torch.float32).contiguous()
+    keep.append(w)
+    return w.data_ptr()
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Layer norm over the last dimension, y = (x - mean) * rsqrt(var + eps) * weight + bias
+    (float32 math). ``out_dtype``: x's type, or float16 / bfloat16 for a float32 x (a float32
+    residual stream normalised straight into a layer's 16-bit input). y is contiguous."""
+    _require_cuda(x)
+    y_dtype = x.dtype if out_dtype is None else out_dtype
+    _ln_check(x, y_dtype)
+    D = x.shape[-1]
+    x2 = _ln_rows(x)
+    keep: list = []
+    with torch.cuda.device(x.device):
+        y = torch.empty(x.shape, dtype=y_dtype, device=x.device)
+        a = _capi.LayerNormArgs()
+        a.rows, a.dim, a.x_dtype, a.y_dtype, a.eps = x2.shape[0], D, _DTYPES[x.dtype], _DTYPES[y_dtype], eps
+        a.x, a.x_stride, a.y, a.y_stride = x2.data_ptr(), x2.stride(0), y.data_ptr(), D
+        a.weight, a.bias = _ln_param(weight, "weight", x, keep), _ln_param(bias, "bias", x, keep)
+        a.stream = torch.cuda.current_stream(x.device).cuda_stream
+        _capi.layer_norm_fwd(a)
+    return y
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                        *, need_dweight: bool = True, need_dbias: bool = True
+                        ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Gradients of ``layer_norm`` from its input: ``(dx, dweight | None, dbias | None)``.
+    dx has x's type and is contiguous; dweight and dbias are float32 [D]."""
+    _require_cuda(dy, x)
+    _ln_check(x, dy.dtype)
+    if dy.shape != x.shape or dy.device != x.device:
+        raise ValueError("layer_norm_backward needs dy and x of one shape on one device")
+    D = x.shape[-1]
+    x2, dy2 = _ln_rows(x), _ln_rows(dy)
+    keep: list = []
+    with torch.cuda.device(x.device):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty(D, dtype=torch.float32, device=x.device) if need_dweight else None
+        db = torch.empty(D, dtype=torch.float32, device=x.device) if need_dbias else None
+        a = _capi.LayerNormArgs()
+        a.rows, a.dim, a.x_dtype, a.y_dtype, a.eps = x2.shape[0], D, _DTYPES[x.dtype], _DTYPES[dy.dtype], eps
+        a.x, a.x_stride, a.dy, a.dy_stride = x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0)
+        a.dx, a.dx_stride = dx.data_ptr(), D
+        a.weight = _ln_param(weight, "weight", x, keep)
+        if dw is not None:
+            a.dweight = dw.data_ptr()
+        if db is not None:
+            a.dbias = db.data_ptr()
+        a.stream = torch.cuda.current_stream(x.device).cuda_stream
+        a.workspace, a.workspace_bytes = _workspace(_capi.layer_norm_bwd_workspace_bytes(a), x.device, keep)
+        _capi.layer_norm_bwd(a)
+    return dx, dw, db
+
+
 def last_path() -> str:
     return {0: "auto", 1: "exact", 2: "tensorcore", 3: "chunked"}.get(_capi.last_path(), "?")
 
