@@ -52,18 +52,6 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
     const int cb = blockIdx.x % ncb, b = (int)(bh / p.H), h = (int)(bh % p.H), c0 = cb * kDeltaCols;
     const int g = lane >> 2, t = lane & 3;
 
-    auto load_stage = [&](int c) {
-        auto& st = sm.st[c % NST];
-        const int lt = tid - 128, n0 = c * kDeltaC;
-        if (warp == 4) load_gates(st.s, p, b, h, n0, lane);
-        bar_sync(3, 128);
-        if (!st.s.any) return;
-        load_planes<T, DP, NIN, 128>(st.k, p.k, tensor_base(p.k, b, h), n0, 0, p.d, st.s.live, lt);
-        load_planes<T, DP, NIN, 128>(st.q, p.q, tensor_base(p.q, b, h), n0, 0, p.d, st.s.live, lt);
-        load_planes<T, kDeltaCols, NIN, 128>(st.g, p.g, tensor_base(p.g, b, h), n0, c0, p.e, st.s.live, lt);
-        copy16<128>(st.y, p.Y + (bh * p.nc + c) * (NX * kYBlocks * 512), NX * kYBlocks * 512, lt);
-    };
-
     if (warp < 2) {  // ---------------------------------------------------- chain
         float S[DP / 8][4];  // G^T: 16 value columns x d
         const int col0 = c0 + 16 * warp;
@@ -286,15 +274,47 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
             __syncthreads();
         }
     } else {  // ---------------------------------------------------------- loads
-        if (NST == 2) load_stage(p.nc - 1);
+        const int lt = tid - 128;  // as in the forward's walk, from the last chunk to the first
+        const Gates* gates = p.gates + bh * p.nc;
+        TileRegs<T, DP, 128> k, q;
+        TileRegs<T, kDeltaCols, 128> x;
+        ByteRegs<NX * kYBlocks * 512, 128> y;
+        ByteRegs<sizeof(Gates), 128> s;
+        int any = 0, any_next = 0;
+        auto issue = [&](int c) {
+            any = any_next;
+            any_next = c > 0 ? gates[c - 1].any : 0;
+            if (c < 0) return;
+            s.issue(gates + c, lt);
+            if (!any) return;
+            const int n0 = c * kDeltaC;
+            k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, lt);
+            q.issue(p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, lt);
+            x.issue(p.g, tensor_base(p.g, b, h), n0, c0, p.e, p.N, lt);
+            y.issue(p.Y + (bh * p.nc + c) * (NX * kYBlocks * 512), lt);
+        };
+        auto store = [&](int c) {
+            if (c < 0) return;
+            auto& st = sm.st[c % NST];
+            s.store(&st.s, lt);
+            bar_sync(3, 128);
+            if (!any) return;
+            k.template store_planes<NIN>(st.k, st.s.live, lt);
+            q.template store_planes<NIN>(st.q, st.s.live, lt);
+            x.template store_planes<NIN>(st.g, st.s.live, lt);
+            y.store(st.y, lt);
+        };
+        any_next = gates[p.nc - 1].any;
+        issue(p.nc - 1);
+        if (NST == 2) {
+            store(p.nc - 1);
+            issue(p.nc - 2);
+        }
         __syncthreads();
         for (int c = p.nc - 1; c >= 0; --c) {
-            if (NST == 1) {
-                load_stage(c);
-                __syncthreads();
-            } else if (c > 0) {
-                load_stage(c - 1);
-            }
+            store(c - (NST - 1));
+            issue(c - NST);
+            if (NST == 1) __syncthreads();
             __syncthreads();
         }
     }
@@ -304,54 +324,124 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
 template <typename T, int DP>
 struct GradSmem {
     static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
+    static constexpr int kState = 2 * DP / 16 * kX * 512, kCol = 2 * 4 * kX * 512, kGTile = kIn * 64 * kDeltaCols * 2;
+    // CTAs per SM, and blocks of 32 value columns in flight (both of e = 64 where that fits twice on an SM)
+    static constexpr int kCtas = sizeof(T) == 2 && DP == 64 ? 2 : 1;
+    static constexpr int kBufs = kIn == 1 && DP == 64 ? 2 : 1;
     Gates s;
     float qdq[2][kDeltaC], vdv[kDeltaC], wz[kDeltaC], kdk[2][kDeltaC];
     float gs[8];
     alignas(128) unsigned char k[kIn * 64 * DP * 2];
     alignas(128) unsigned char q[kIn * 64 * DP * 2];
+    struct In {  // one block of 32 value columns
+        alignas(128) unsigned char S0[kState];
+        alignas(128) unsigned char G[kState];
+        alignas(128) unsigned char W[kCol];
+        alignas(128) unsigned char Z[kCol];
+        alignas(128) unsigned char dO[kGTile];
+        alignas(128) unsigned char v[kGTile];
+    };
+    struct Scores {
+        alignas(128) unsigned char d1[kX * kYBlocks * 512];
+        alignas(128) unsigned char d2[kX * kYBlocks * 512];
+    };
     union {
-        struct {  // one block of 32 value columns
-            alignas(128) unsigned char S0[2 * DP / 16 * kX * 512];
-            alignas(128) unsigned char G[2 * DP / 16 * kX * 512];
-            alignas(128) unsigned char W[2 * 4 * kX * 512];
-            alignas(128) unsigned char Z[2 * 4 * kX * 512];
-            alignas(128) unsigned char dO[kIn * 64 * kDeltaCols * 2];
-        } in;
-        struct {
-            alignas(128) unsigned char d1[kX * kYBlocks * 512];
-            alignas(128) unsigned char d2[kX * kYBlocks * 512];
-        } sc;
+        In in[kBufs];
+        Scores sc;
+        alignas(16) float rows[kDeltaC][DP + 4];
     } u;
+    alignas(16) float dv[kDeltaC][kDeltaCols + 4];
 };
 
 __device__ __forceinline__ float bf16_at(const unsigned char* p) {
     return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16);
 }
 
+// Rows 0 .. rows - 1 of a float tile to a gradient, 8 columns a thread; `x32` (per state head, [.., width]) instead of `x` where given.
+template <typename T, int NT>
+__device__ __forceinline__ void store_rows(const float* tile, int pitch, int cols, const DeltaTensor& x, int64_t base, float* x32,
+                                           int64_t base32, int n0, int rows, int c0, int width, int tid) {
+    const int pieces = cols / 8;
+    for (int i = tid; i < rows * pieces; i += NT) {
+        const int row = i / pieces, c = i % pieces * 8;
+        if (c0 + c >= width) continue;
+        const float* f = tile + row * pitch + c;
+        if (x32) {
+            float* at = x32 + base32 + (int64_t)(n0 + row) * width + c0 + c;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + c + j < width) at[j] = f[j];
+            continue;
+        }
+        T* at = static_cast<T*>(x.p) + base + (n0 + row) * x.sn + c0 + c;
+        if (x.vec && c0 + c + 8 <= width) {
+            alignas(16) T t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = from_f<T>(f[j]);
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(at)[j] = reinterpret_cast<const uint4*>(t)[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + c + j < width) at[j] = from_f<T>(f[j]);
+        }
+    }
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kTile = 64 * DP * 2, kGTile = 64 * kDeltaCols * 2;
+__global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel(const DeltaParams p) {
+    using Smem = GradSmem<T, DP>;
+    constexpr int NIN = Smem::kIn, NX = Smem::kX, kTile = 64 * DP * 2, kGTile = 64 * kDeltaCols * 2;
     constexpr int NB = DP / 16;  // 8-column blocks of a warp's half of d
     extern __shared__ __align__(128) unsigned char raw[];
-    GradSmem<T, DP>& sm = *reinterpret_cast<GradSmem<T, DP>*>(raw);
+    Smem& sm = *reinterpret_cast<Smem*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int rb = warp & 3, hf = warp >> 2;  // 16 tokens, half of d
     const int64_t chunk = blockIdx.x, bh = chunk / p.nc;
     const int c = (int)(chunk % p.nc), b = (int)(bh / p.H), h = (int)(bh % p.H), n0 = c * kDeltaC;
     const int rows = min(kDeltaC, p.N - n0);
     const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
-    if (warp == 0) load_gates(sm.s, p, b, h, n0, lane);
-    if (tid < kDeltaC) sm.vdv[tid] = sm.wz[tid] = 0.f;
-    __syncthreads();
-    const Gates& s = sm.s;
+    const int64_t at32 = bh * p.N;  // rows of the gradients per state head
+    const bool any = p.gates[chunk].any != 0;
 
-    // where the rows of this state head's gradients go
-    auto grad_row = [&](const DeltaTensor& x, float* x32, int width, int n, T*& row, float*& row32) {
-        row = nullptr;
-        row32 = nullptr;
-        if (x32) row32 = x32 + ((int64_t)bh * p.N + n) * width;
-        else row = static_cast<T*>(x.p) + tensor_base(x, b, h) + n * x.sn;
+    if (!any) {  // zeros
+        float* zero = &sm.u.rows[0][0];
+        for (int i = tid; i < kDeltaC * (DP + 4); i += 256) zero[i] = 0.f;
+        __syncthreads();
+        store_rows<T, 256>(zero, DP + 4, DP, p.dq, tensor_base(p.dq, b, h), p.dq32, at32 * p.d, n0, rows, 0, p.d, tid);
+        store_rows<T, 256>(zero, DP + 4, DP, p.dk, tensor_base(p.dk, b, h), p.dk32, at32 * p.d, n0, rows, 0, p.d, tid);
+        for (int eb = 0; eb < ncb; ++eb)
+            store_rows<T, 256>(zero, DP + 4, kDeltaCols, p.dv, tensor_base(p.dv, b, h), p.dv32, at32 * p.e, n0, rows,
+                               eb * kDeltaCols, p.e, tid);
+        if (tid < rows) {
+            p.dbeta[at32 + n0 + tid] = 0.f;
+            if (p.dlg) p.dlg[at32 + n0 + tid] = 0.f;
+        }
+        return;
+    }
+
+    auto start = [&](int eb) {  // the planes of a block of value columns
+        auto& in = sm.u.in[eb % Smem::kBufs];
+        const int64_t at = chunk * 2 * ncb + 2 * eb;
+        async16<256>(in.S0, p.S0 + at * (Smem::kState / 2), Smem::kState, tid);
+        async16<256>(in.G, p.dS + at * (Smem::kState / 2), Smem::kState, tid);
+        async16<256>(in.W, p.W + at * (Smem::kCol / 2), Smem::kCol, tid);
+        async16<256>(in.Z, p.Z + at * (Smem::kCol / 2), Smem::kCol, tid);
     };
+    async16<256>(reinterpret_cast<unsigned char*>(&sm.s), reinterpret_cast<const unsigned char*>(p.gates + chunk), sizeof(Gates), tid);
+    start(0);
+    if (Smem::kBufs == 2 && ncb > 1) start(1);
+    const Gates& s = sm.s;
+    {
+        TileRegs<T, DP, 256> k, q;
+        k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, tid);
+        q.issue(p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, tid);
+        if (tid < kDeltaC) sm.vdv[tid] = sm.wz[tid] = 0.f;
+        async_wait();
+        __syncthreads();
+        k.template store_planes<NIN>(sm.k, s.live, tid);
+        q.template store_planes<NIN>(sm.q, s.live, tid);
+    }
 
     float dq[NB][4], dk1[NB][4], dk2[NB][4], D[8][4];
 #pragma unroll
@@ -364,322 +454,305 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
         for (int i = 0; i < 4; ++i) D[n][i] = 0.f;  // dO W^T (hf = 0) or Z W^T (hf = 1), rows 16 rb ..
     float gs = 0.f;
 
-    if (s.any) {
-        load_planes<T, DP, NIN, 256>(sm.k, p.k, tensor_base(p.k, b, h), n0, 0, p.d, s.live, tid);
-        load_planes<T, DP, NIN, 256>(sm.q, p.q, tensor_base(p.q, b, h), n0, 0, p.d, s.live, tid);
-    }
     for (int eb = 0; eb < ncb; ++eb) {
-        if (s.any) {
-            const int64_t at = chunk * 2 * ncb + 2 * eb;
-            copy16<256>(sm.u.in.S0, p.S0 + at * (DP / 16 * NX * 512), 2 * DP / 16 * NX * 512, tid);
-            copy16<256>(sm.u.in.G, p.dS + at * (DP / 16 * NX * 512), 2 * DP / 16 * NX * 512, tid);
-            copy16<256>(sm.u.in.W, p.W + at * (4 * NX * 512), 2 * 4 * NX * 512, tid);
-            copy16<256>(sm.u.in.Z, p.Z + at * (4 * NX * 512), 2 * 4 * NX * 512, tid);
-            load_planes<T, kDeltaCols, NIN, 256>(sm.u.in.dO, p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, s.live, tid);
-            __syncthreads();
-            const uint32_t S0 = smem_addr(sm.u.in.S0) + lane * 16, G = smem_addr(sm.u.in.G) + lane * 16;
-            const uint32_t W = smem_addr(sm.u.in.W) + lane * 16, Z = smem_addr(sm.u.in.Z) + lane * 16;
-            const uint32_t dO = smem_addr(sm.u.in.dO);
-#pragma unroll
-            for (int cw = 0; cw < 2; ++cw) {  // 16 value columns: one k step
-                uint32_t ao[NIN][4], aw[NX][4], az[NX][4];
-#pragma unroll
-                for (int pl = 0; pl < NIN; ++pl) a_rows<kDeltaCols>(ao[pl], dO + pl * kGTile, 16 * rb, cw, lane);
-#pragma unroll
-                for (int pl = 0; pl < NX; ++pl) {
-                    uint32_t r[4];
-                    ldm_t(r, W + ((cw * 4 + rb) * NX + pl) * 512);
-                    aw[pl][0] = r[0]; aw[pl][1] = r[2]; aw[pl][2] = r[1]; aw[pl][3] = r[3];
-                    ldm_t(r, Z + ((cw * 4 + rb) * NX + pl) * 512);
-                    az[pl][0] = r[0]; az[pl][1] = r[2]; az[pl][2] = r[1]; az[pl][3] = r[3];
-                }
-#pragma unroll
-                for (int n = 0; n < NB / 2; ++n) {
-                    const int kk = hf * (NB / 2) + n;
-                    uint32_t b0[NX][2], b1[NX][2];
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl) {
-                        uint32_t r[4];
-                        ldm_t(r, S0 + ((cw * (DP / 16) + kk) * NX + pl) * 512);
-                        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                    }
-                    mma_planes<NIN, NX, NX>(dq[2 * n], ao, b0);
-                    mma_planes<NIN, NX, NX>(dq[2 * n + 1], ao, b1);
-                    mma_planes<NX, NX, NX>(dk2[2 * n], az, b0);
-                    mma_planes<NX, NX, NX>(dk2[2 * n + 1], az, b1);
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl) {
-                        uint32_t r[4];
-                        ldm_t(r, G + ((cw * (DP / 16) + kk) * NX + pl) * 512);
-                        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                    }
-                    mma_planes<NX, NX, NX>(dk1[2 * n], aw, b0);
-                    mma_planes<NX, NX, NX>(dk1[2 * n + 1], aw, b1);
-                }
-#pragma unroll
-                for (int jb = 0; jb < 4; ++jb) {
-                    if (jb > rb) continue;
-                    uint32_t b0[NX][2], b1[NX][2];
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl) {
-                        uint32_t r[4];
-                        ldm_t(r, W + ((cw * 4 + jb) * NX + pl) * 512);
-                        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                    }
-                    if (hf == 0) {
-                        mma_planes<NIN, NX, NX>(D[2 * jb], ao, b0);
-                        mma_planes<NIN, NX, NX>(D[2 * jb + 1], ao, b1);
-                    } else {
-                        mma_planes<NX, NX, NX>(D[2 * jb], az, b0);
-                        mma_planes<NX, NX, NX>(D[2 * jb + 1], az, b1);
-                    }
-                }
-            }
-        }
-        {  // dv = beta Z, and the row sums W.Z and v.dv: a token and 8 value columns per thread
-            const int tok = tid & 63, grp = tid >> 6, cw = grp >> 1, col = eb * kDeltaCols + grp * 8;
-            float wz = 0.f, vdv = 0.f;
-            if (tok < rows && col < p.e) {
-                const int n = n0 + tok;
-                const bool on = s.any && s.live[tok];
-                T* row;
-                float* row32;
-                grad_row(p.dv, p.dv32, p.e, n, row, row32);
-                const T* v = static_cast<const T*>(p.v.p) + tensor_base(p.v, b, h) + n * p.v.sn;
-                T ov[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float z = 0.f, w = 0.f;
-                    if (on) {
-                        // element (value column 8 (grp % 2) + i, token): matrix [token half][column half], row i
-                        const int off = (((tok >> 3) & 1) * 2 + (grp & 1)) * 128 + i * 16 + (tok & 7) * 2;
-#pragma unroll
-                        for (int pl = 0; pl < NX; ++pl) {
-                            const int tile = ((cw * 4 + (tok >> 4)) * NX + pl) * 512;
-                            z += bf16_at(sm.u.in.Z + tile + off);
-                            w += bf16_at(sm.u.in.W + tile + off);
-                        }
-                    }
-                    wz = fmaf(w, z, wz);
-                    z *= s.beta[tok];
-                    if (on && col + i < p.e) vdv = fmaf(z, to_f<T>(v[col + i]), vdv);
-                    ov[i] = from_f<T>(z);
-                    if (row32 && col + i < p.e) row32[col + i] = z;
-                }
-                if (row) {
-                    if (p.dv.vec && col + 8 <= p.e) {
-#pragma unroll
-                        for (int x = 0; x < (int)sizeof(T) / 2; ++x)
-                            reinterpret_cast<uint4*>(row + col)[x] = reinterpret_cast<const uint4*>(ov)[x];
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (col + i < p.e) row[col + i] = ov[i];
-                    }
-                }
-            }
-            // fixed order: the four groups add one after the other
-            for (int x = 0; x < 4; ++x) {
-                if (grp == x) {
-                    sm.wz[tok] += wz;
-                    sm.vdv[tok] += vdv;
-                }
-                __syncthreads();
-            }
-        }
-        if (s.any) {  // <G, S0>
-            for (int i = tid; i < 2 * DP / 16 * 128; i += 256) {
-                const int tile = i >> 7, off = (i & 127) * 4;
-                float2 x = make_float2(0.f, 0.f), y = x;
-#pragma unroll
-                for (int pl = 0; pl < NX; ++pl) {
-                    const float2 u0 = unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.u.in.S0 + (tile * NX + pl) * 512 + off));
-                    const float2 u1 = unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.u.in.G + (tile * NX + pl) * 512 + off));
-                    x.x += u0.x; x.y += u0.y;
-                    y.x += u1.x; y.y += u1.y;
-                }
-                gs = fmaf(x.x, y.x, gs);
-                gs = fmaf(x.y, y.y, gs);
-            }
-            __syncthreads();
-        }
-    }
-
-    if (s.any) {
-        {  // D1 or D2 as planes
-            unsigned char* dst = hf ? sm.u.sc.d2 : sm.u.sc.d1;
-#pragma unroll
-            for (int jb = 0; jb < 4; ++jb) {
-                if (jb > rb) continue;
-#pragma unroll
-                for (int jh = 0; jh < 2; ++jh)
-#pragma unroll
-                    for (int ih = 0; ih < 2; ++ih) {
-                        const int i = 16 * rb + 8 * ih + g, j = 16 * jb + 8 * jh + 2 * t;
-                        const float fi = hf ? -s.beta[i] : p.scale;
-                        float x = 0.f, y = 0.f;
-                        if (j < i || (j == i && !hf)) x = fi * s.beta[j] * gamma_ij(s, i, j) * D[2 * jb + jh][2 * ih];
-                        if (j + 1 < i || (j + 1 == i && !hf))
-                            y = fi * s.beta[j + 1] * gamma_ij(s, i, j + 1) * D[2 * jb + jh][2 * ih + 1];
-                        uint32_t r[NX];
-                        split2<NX>(x, y, r);
-#pragma unroll
-                        for (int pl = 0; pl < NX; ++pl)
-                            *reinterpret_cast<uint32_t*>(dst + (pl * kYBlocks + tri(rb, jb)) * 512 + (ih * 2 + jh) * 128 + lane * 4) = r[pl];
-                    }
-            }
-        }
-        // row factors of the products with the states; k.dk1 before anything is added to it
+        auto& in = sm.u.in[eb % Smem::kBufs];
         {
-            float kd[2] = {0.f, 0.f};
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int i = 16 * rb + 8 * x + g;
-                const float fq = p.scale * s.eg[i], f1 = s.kd[i] * s.beta[i], f2 = -s.eg[i] * s.beta[i];
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    const int piece = hf * NB + n;
-                    float2 kv = make_float2(0.f, 0.f);
-#pragma unroll
-                    for (int pl = 0; pl < NIN; ++pl) {
-                        const float2 u = unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.k + pl * kTile + tile_off<DP>(i, piece) + 4 * t));
-                        kv.x += u.x;
-                        kv.y += u.y;
-                    }
-                    const float a = f1 * dk1[n][2 * x], d = f1 * dk1[n][2 * x + 1];
-                    kd[x] = fmaf(a, kv.x, kd[x]);
-                    kd[x] = fmaf(d, kv.y, kd[x]);
-                    dk1[n][2 * x] = fmaf(f2, dk2[n][2 * x], a);
-                    dk1[n][2 * x + 1] = fmaf(f2, dk2[n][2 * x + 1], d);
-                    dq[n][2 * x] *= fq;
-                    dq[n][2 * x + 1] *= fq;
-                }
-                kd[x] += __shfl_xor_sync(0xffffffffu, kd[x], 1);
-                kd[x] += __shfl_xor_sync(0xffffffffu, kd[x], 2);
-                if (t == 0) sm.kdk[hf][i] = kd[x];
-            }
+            TileRegs<T, kDeltaCols, 256> x, v;
+            x.issue(p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
+            v.issue(p.v, tensor_base(p.v, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
+            if (eb >= Smem::kBufs) start(eb);
+            x.template store_planes<NIN>(in.dO, s.live, tid);
+            v.template store_planes<NIN>(in.v, s.live, tid);
         }
+        async_wait();
         __syncthreads();
-        const uint32_t d1 = smem_addr(sm.u.sc.d1) + lane * 16, d2 = smem_addr(sm.u.sc.d2) + lane * 16;
-        const uint32_t kt = smem_addr(sm.k), qt = smem_addr(sm.q);
-        constexpr int kP = kYBlocks * 512;
+        const uint32_t S0 = smem_addr(in.S0) + lane * 16, G = smem_addr(in.G) + lane * 16;
+        const uint32_t W = smem_addr(in.W) + lane * 16, Z = smem_addr(in.Z) + lane * 16;
+        const uint32_t dO = smem_addr(in.dO);
 #pragma unroll
-        for (int ob = 0; ob < 4; ++ob) {
-            // D1 K and D2 K: tokens ob <= rb; D1^T Q and D2^T K: tokens ob >= rb
-            uint32_t a1[NX][4], a2[NX][4], a1t[NX][4], a2t[NX][4];
+        for (int cw = 0; cw < 2; ++cw) {  // 16 value columns: one k step
+            uint32_t ao[NIN][4], aw[NX][4], az[NX][4];
+#pragma unroll
+            for (int pl = 0; pl < NIN; ++pl) a_rows<kDeltaCols>(ao[pl], dO + pl * kGTile, 16 * rb, cw, lane);
 #pragma unroll
             for (int pl = 0; pl < NX; ++pl) {
                 uint32_t r[4];
-                if (ob <= rb) {
-                    ldm(r, d1 + pl * kP + tri(rb, ob) * 512);
-                    a1[pl][0] = r[0]; a1[pl][1] = r[2]; a1[pl][2] = r[1]; a1[pl][3] = r[3];
-                    ldm(r, d2 + pl * kP + tri(rb, ob) * 512);
-                    a2[pl][0] = r[0]; a2[pl][1] = r[2]; a2[pl][2] = r[1]; a2[pl][3] = r[3];
-                }
-                if (ob >= rb) {
-                    ldm_t(a1t[pl], d1 + pl * kP + tri(ob, rb) * 512);
-                    ldm_t(a2t[pl], d2 + pl * kP + tri(ob, rb) * 512);
-                }
+                ldm_t(r, W + ((cw * 4 + rb) * NX + pl) * 512);
+                aw[pl][0] = r[0]; aw[pl][1] = r[2]; aw[pl][2] = r[1]; aw[pl][3] = r[3];
+                ldm_t(r, Z + ((cw * 4 + rb) * NX + pl) * 512);
+                az[pl][0] = r[0]; az[pl][1] = r[2]; az[pl][2] = r[1]; az[pl][3] = r[3];
             }
 #pragma unroll
             for (int n = 0; n < NB / 2; ++n) {
-                const int np = hf * (NB / 2) + n;
-                uint32_t k0[NIN][2], k1[NIN][2], q0[NIN][2], q1[NIN][2];
+                const int kk = hf * (NB / 2) + n;
+                uint32_t b0[NX][2], b1[NX][2];
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    uint32_t r[4];
+                    ldm_t(r, S0 + ((cw * (DP / 16) + kk) * NX + pl) * 512);
+                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                }
+                mma_planes<NIN, NX, NX>(dq[2 * n], ao, b0);
+                mma_planes<NIN, NX, NX>(dq[2 * n + 1], ao, b1);
+                mma_planes<NX, NX, NX>(dk2[2 * n], az, b0);
+                mma_planes<NX, NX, NX>(dk2[2 * n + 1], az, b1);
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    uint32_t r[4];
+                    ldm_t(r, G + ((cw * (DP / 16) + kk) * NX + pl) * 512);
+                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                }
+                mma_planes<NX, NX, NX>(dk1[2 * n], aw, b0);
+                mma_planes<NX, NX, NX>(dk1[2 * n + 1], aw, b1);
+            }
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {
+                if (jb > rb) continue;
+                uint32_t b0[NX][2], b1[NX][2];
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    uint32_t r[4];
+                    ldm_t(r, W + ((cw * 4 + jb) * NX + pl) * 512);
+                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                }
+                if (hf == 0) {
+                    mma_planes<NIN, NX, NX>(D[2 * jb], ao, b0);
+                    mma_planes<NIN, NX, NX>(D[2 * jb + 1], ao, b1);
+                } else {
+                    mma_planes<NX, NX, NX>(D[2 * jb], az, b0);
+                    mma_planes<NX, NX, NX>(D[2 * jb + 1], az, b1);
+                }
+            }
+        }
+        {  // dv = beta Z and the row sums W.Z, v.dv: warp (rb, hf) has tokens 16 rb + 8 hf .., lanes as in an 8 x 8 matrix
+            const int tok = 16 * rb + 8 * hf + 2 * t;
+            const float2 be = *reinterpret_cast<const float2*>(&s.beta[tok]);
+            float2 wz = make_float2(0.f, 0.f), vdv = wz;
+#pragma unroll
+            for (int cm = 0; cm < 4; ++cm) {  // value columns 8 cm + g
+                float2 z = make_float2(0.f, 0.f), w = z, v = z;
+                const int off = (hf * 2 + (cm & 1)) * 128 + lane * 4;
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    const int tile = (((cm >> 1) * 4 + rb) * NX + pl) * 512 + off;
+                    const float2 x = unpack_bf16(*reinterpret_cast<const uint32_t*>(in.Z + tile));
+                    const float2 y = unpack_bf16(*reinterpret_cast<const uint32_t*>(in.W + tile));
+                    z.x += x.x; z.y += x.y;
+                    w.x += y.x; w.y += y.y;
+                }
 #pragma unroll
                 for (int pl = 0; pl < NIN; ++pl) {
-                    uint32_t r[4];
-                    b_cols<DP>(r, kt + pl * kTile, 16 * ob, np, lane);
-                    k0[pl][0] = r[0]; k0[pl][1] = r[1]; k1[pl][0] = r[2]; k1[pl][1] = r[3];
-                    b_cols<DP>(r, qt + pl * kTile, 16 * ob, np, lane);
-                    q0[pl][0] = r[0]; q0[pl][1] = r[1]; q1[pl][0] = r[2]; q1[pl][1] = r[3];
+                    const unsigned char* at = in.v + pl * kGTile + 2 * g;
+                    v.x += bf16_at(at + tile_off<kDeltaCols>(tok, cm));
+                    v.y += bf16_at(at + tile_off<kDeltaCols>(tok + 1, cm));
                 }
-                if (ob <= rb) {
-                    mma_planes<NX, NIN, NX>(dq[2 * n], a1, k0);
-                    mma_planes<NX, NIN, NX>(dq[2 * n + 1], a1, k1);
-                    mma_planes<NX, NIN, NX>(dk1[2 * n], a2, k0);
-                    mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a2, k1);
-                }
-                if (ob >= rb) {
-                    mma_planes<NX, NIN, NX>(dk1[2 * n], a1t, q0);
-                    mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a1t, q1);
-                    mma_planes<NX, NIN, NX>(dk1[2 * n], a2t, k0);
-                    mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a2t, k1);
-                }
+                wz.x = fmaf(w.x, z.x, wz.x);
+                wz.y = fmaf(w.y, z.y, wz.y);
+                z.x *= be.x;
+                z.y *= be.y;
+                vdv.x = fmaf(z.x, v.x, vdv.x);
+                vdv.y = fmaf(z.y, v.y, vdv.y);
+                sm.dv[tok][8 * cm + g] = z.x;
+                sm.dv[tok + 1][8 * cm + g] = z.y;
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                wz.x += __shfl_xor_sync(0xffffffffu, wz.x, o);
+                wz.y += __shfl_xor_sync(0xffffffffu, wz.y, o);
+                vdv.x += __shfl_xor_sync(0xffffffffu, vdv.x, o);
+                vdv.y += __shfl_xor_sync(0xffffffffu, vdv.y, o);
+            }
+            if (lane < 4) {  // (these tokens are this warp's alone)
+                sm.wz[tok] += wz.x;
+                sm.wz[tok + 1] += wz.y;
+                sm.vdv[tok] += vdv.x;
+                sm.vdv[tok + 1] += vdv.y;
             }
         }
-        {  // q.dq
-            float qd[2] = {0.f, 0.f};
+        // <G, S0>
+        for (int i = tid; i < 2 * DP / 16 * 128; i += 256) {
+            const int tile = i >> 7, off = (i & 127) * 4;
+            float2 x = make_float2(0.f, 0.f), y = x;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int i = 16 * rb + 8 * x + g;
-#pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int pl = 0; pl < NIN; ++pl) {
-                        const float2 u = unpack_bf16(
-                            *reinterpret_cast<const uint32_t*>(sm.q + pl * kTile + tile_off<DP>(i, hf * NB + n) + 4 * t));
-                        qd[x] = fmaf(u.x, dq[n][2 * x], qd[x]);
-                        qd[x] = fmaf(u.y, dq[n][2 * x + 1], qd[x]);
-                    }
-                qd[x] += __shfl_xor_sync(0xffffffffu, qd[x], 1);
-                qd[x] += __shfl_xor_sync(0xffffffffu, qd[x], 2);
-                if (t == 0) sm.qdq[hf][i] = qd[x];
+            for (int pl = 0; pl < NX; ++pl) {
+                const float2 u0 = unpack_bf16(*reinterpret_cast<const uint32_t*>(in.S0 + (tile * NX + pl) * 512 + off));
+                const float2 u1 = unpack_bf16(*reinterpret_cast<const uint32_t*>(in.G + (tile * NX + pl) * 512 + off));
+                x.x += u0.x; x.y += u0.y;
+                y.x += u1.x; y.y += u1.y;
             }
+            gs = fmaf(x.x, y.x, gs);
+            gs = fmaf(x.y, y.y, gs);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) gs += __shfl_xor_sync(0xffffffffu, gs, o);
-        if (lane == 0) sm.gs[warp] = gs;
+        __syncthreads();
+        store_rows<T, 256>(&sm.dv[0][0], kDeltaCols + 4, kDeltaCols, p.dv, tensor_base(p.dv, b, h), p.dv32, at32 * p.e, n0, rows,
+                           eb * kDeltaCols, p.e, tid);
+        if (eb + 1 < ncb) __syncthreads();  // (a later block writes dv and the buffers again)
     }
-    // dq and dk rows: quads hold neighbouring columns
+
+    {  // D1 or D2 as planes
+        unsigned char* dst = hf ? sm.u.sc.d2 : sm.u.sc.d1;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const int i = 16 * rb + 8 * x + g;
-        if (i >= rows) continue;
-        T *rq, *rk;
-        float *rq32, *rk32;
-        grad_row(p.dq, p.dq32, p.d, n0 + i, rq, rq32);
-        grad_row(p.dk, p.dk32, p.d, n0 + i, rk, rk32);
+        for (int jb = 0; jb < 4; ++jb) {
+            if (jb > rb) continue;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int col = (hf * NB + n) * 8 + 2 * t;
+            for (int jh = 0; jh < 2; ++jh)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                if (col + y >= p.d) continue;
-                if (rq32) rq32[col + y] = dq[n][2 * x + y];
-                else rq[col + y] = from_f<T>(dq[n][2 * x + y]);
-                if (rk32) rk32[col + y] = dk1[n][2 * x + y];
-                else rk[col + y] = from_f<T>(dk1[n][2 * x + y]);
+                for (int ih = 0; ih < 2; ++ih) {
+                    const int i = 16 * rb + 8 * ih + g, j = 16 * jb + 8 * jh + 2 * t;
+                    const float fi = hf ? -s.beta[i] : p.scale;
+                    float x = 0.f, y = 0.f;
+                    if (j < i || (j == i && !hf)) x = fi * s.beta[j] * gamma_ij(s, i, j) * D[2 * jb + jh][2 * ih];
+                    if (j + 1 < i || (j + 1 == i && !hf))
+                        y = fi * s.beta[j + 1] * gamma_ij(s, i, j + 1) * D[2 * jb + jh][2 * ih + 1];
+                    uint32_t r[NX];
+                    split2<NX>(x, y, r);
+#pragma unroll
+                    for (int pl = 0; pl < NX; ++pl)
+                        *reinterpret_cast<uint32_t*>(dst + (pl * kYBlocks + tri(rb, jb)) * 512 + (ih * 2 + jh) * 128 + lane * 4) = r[pl];
+                }
+        }
+    }
+    {  // row factors of the products with the states; k.dk1 before anything is added to it
+        float kd[2] = {0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int i = 16 * rb + 8 * x + g;
+            const float fq = p.scale * s.eg[i], f1 = s.kd[i] * s.beta[i], f2 = -s.eg[i] * s.beta[i];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const int piece = hf * NB + n;
+                float2 kv = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int pl = 0; pl < NIN; ++pl) {
+                    const float2 u = unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.k + pl * kTile + tile_off<DP>(i, piece) + 4 * t));
+                    kv.x += u.x;
+                    kv.y += u.y;
+                }
+                const float a = f1 * dk1[n][2 * x], d = f1 * dk1[n][2 * x + 1];
+                kd[x] = fmaf(a, kv.x, kd[x]);
+                kd[x] = fmaf(d, kv.y, kd[x]);
+                dk1[n][2 * x] = fmaf(f2, dk2[n][2 * x], a);
+                dk1[n][2 * x + 1] = fmaf(f2, dk2[n][2 * x + 1], d);
+                dq[n][2 * x] *= fq;
+                dq[n][2 * x + 1] *= fq;
             }
+            kd[x] += __shfl_xor_sync(0xffffffffu, kd[x], 1);
+            kd[x] += __shfl_xor_sync(0xffffffffu, kd[x], 2);
+            if (t == 0) sm.kdk[hf][i] = kd[x];
         }
     }
     __syncthreads();
+    const uint32_t d1 = smem_addr(sm.u.sc.d1) + lane * 16, d2 = smem_addr(sm.u.sc.d2) + lane * 16;
+    const uint32_t kt = smem_addr(sm.k), qt = smem_addr(sm.q);
+    constexpr int kP = kYBlocks * 512;
+#pragma unroll
+    for (int ob = 0; ob < 4; ++ob) {
+        // D1 K and D2 K: tokens ob <= rb; D1^T Q and D2^T K: tokens ob >= rb
+        uint32_t a1[NX][4], a2[NX][4], a1t[NX][4], a2t[NX][4];
+#pragma unroll
+        for (int pl = 0; pl < NX; ++pl) {
+            uint32_t r[4];
+            if (ob <= rb) {
+                ldm(r, d1 + pl * kP + tri(rb, ob) * 512);
+                a1[pl][0] = r[0]; a1[pl][1] = r[2]; a1[pl][2] = r[1]; a1[pl][3] = r[3];
+                ldm(r, d2 + pl * kP + tri(rb, ob) * 512);
+                a2[pl][0] = r[0]; a2[pl][1] = r[2]; a2[pl][2] = r[1]; a2[pl][3] = r[3];
+            }
+            if (ob >= rb) {
+                ldm_t(a1t[pl], d1 + pl * kP + tri(ob, rb) * 512);
+                ldm_t(a2t[pl], d2 + pl * kP + tri(ob, rb) * 512);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NB / 2; ++n) {
+            const int np = hf * (NB / 2) + n;
+            uint32_t k0[NIN][2], k1[NIN][2], q0[NIN][2], q1[NIN][2];
+#pragma unroll
+            for (int pl = 0; pl < NIN; ++pl) {
+                uint32_t r[4];
+                b_cols<DP>(r, kt + pl * kTile, 16 * ob, np, lane);
+                k0[pl][0] = r[0]; k0[pl][1] = r[1]; k1[pl][0] = r[2]; k1[pl][1] = r[3];
+                b_cols<DP>(r, qt + pl * kTile, 16 * ob, np, lane);
+                q0[pl][0] = r[0]; q0[pl][1] = r[1]; q1[pl][0] = r[2]; q1[pl][1] = r[3];
+            }
+            if (ob <= rb) {
+                mma_planes<NX, NIN, NX>(dq[2 * n], a1, k0);
+                mma_planes<NX, NIN, NX>(dq[2 * n + 1], a1, k1);
+                mma_planes<NX, NIN, NX>(dk1[2 * n], a2, k0);
+                mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a2, k1);
+            }
+            if (ob >= rb) {
+                mma_planes<NX, NIN, NX>(dk1[2 * n], a1t, q0);
+                mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a1t, q1);
+                mma_planes<NX, NIN, NX>(dk1[2 * n], a2t, k0);
+                mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a2t, k1);
+            }
+        }
+    }
+    {  // q.dq
+        float qd[2] = {0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int i = 16 * rb + 8 * x + g;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int pl = 0; pl < NIN; ++pl) {
+                    const float2 u =
+                        unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.q + pl * kTile + tile_off<DP>(i, hf * NB + n) + 4 * t));
+                    qd[x] = fmaf(u.x, dq[n][2 * x], qd[x]);
+                    qd[x] = fmaf(u.y, dq[n][2 * x + 1], qd[x]);
+                }
+            qd[x] += __shfl_xor_sync(0xffffffffu, qd[x], 1);
+            qd[x] += __shfl_xor_sync(0xffffffffu, qd[x], 2);
+            if (t == 0) sm.qdq[hf][i] = qd[x];
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) gs += __shfl_xor_sync(0xffffffffu, gs, o);
+    if (lane == 0) sm.gs[warp] = gs;
+    // dq, then dk, through shared memory to whole rows
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float2 f;
+                if (which) f = make_float2(dk1[n][2 * x], dk1[n][2 * x + 1]);
+                else f = make_float2(dq[n][2 * x], dq[n][2 * x + 1]);
+                *reinterpret_cast<float2*>(&sm.u.rows[16 * rb + 8 * x + g][(hf * NB + n) * 8 + 2 * t]) = f;
+            }
+        __syncthreads();
+        if (which)
+            store_rows<T, 256>(&sm.u.rows[0][0], DP + 4, DP, p.dk, tensor_base(p.dk, b, h), p.dk32, at32 * p.d, n0, rows, 0, p.d, tid);
+        else
+            store_rows<T, 256>(&sm.u.rows[0][0], DP + 4, DP, p.dq, tensor_base(p.dq, b, h), p.dq32, at32 * p.d, n0, rows, 0, p.d, tid);
+    }
     if (warp == 0) {
         // suffix sums over the chunk (two tokens per lane) on top of <G, S'>
         const int i0 = 2 * lane, i1 = i0 + 1;
-        float x0 = 0.f, x1 = 0.f, k01 = 0.f, end = 0.f;
-        if (s.any) {
-            x0 = sm.qdq[0][i0] + sm.qdq[1][i0] - sm.vdv[i0];
-            x1 = sm.qdq[0][i1] + sm.qdq[1][i1] - sm.vdv[i1];
-            k01 = sm.kdk[0][i0] + sm.kdk[1][i0] + sm.kdk[0][i1] + sm.kdk[1][i1];
-            for (int w = 0; w < 8; ++w) end += sm.gs[w];
-        }
+        const float x0 = sm.qdq[0][i0] + sm.qdq[1][i0] - sm.vdv[i0], x1 = sm.qdq[0][i1] + sm.qdq[1][i1] - sm.vdv[i1];
+        float end = 0.f, k01 = sm.kdk[0][i0] + sm.kdk[1][i0] + sm.kdk[0][i1] + sm.kdk[1][i1];
+        for (int w = 0; w < 8; ++w) end += sm.gs[w];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) k01 += __shfl_xor_sync(0xffffffffu, k01, o);
         end = s.eC * end + k01;
-        float run = x0 + x1;  // suffix sum over lanes >= this one
+        float run = x0 + x1;  // over this lane's tokens and the later lanes'
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const float down = __shfl_down_sync(0xffffffffu, run, o);
             if (lane + o < 32) run += down;
         }
-        const int64_t at = bh * p.N + n0;
+        const int64_t at = at32 + n0;
         if (i0 < rows) {
-            p.dbeta[at + i0] = s.any && s.live[i0] ? sm.wz[i0] : 0.f;
-            if (p.dlg) p.dlg[at + i0] = s.any && s.live[i0] ? run + end : 0.f;
+            p.dbeta[at + i0] = s.live[i0] ? sm.wz[i0] : 0.f;
+            if (p.dlg) p.dlg[at + i0] = s.live[i0] ? run + end : 0.f;
         }
         if (i1 < rows) {
-            p.dbeta[at + i1] = s.any && s.live[i1] ? sm.wz[i1] : 0.f;
-            if (p.dlg) p.dlg[at + i1] = s.any && s.live[i1] ? run - x0 + end : 0.f;
+            p.dbeta[at + i1] = s.live[i1] ? sm.wz[i1] : 0.f;
+            if (p.dlg) p.dlg[at + i1] = s.live[i1] ? run - x0 + end : 0.f;
         }
     }
 }

@@ -51,6 +51,7 @@ struct DeltaParams {
     DeltaTensor q, k, v, o;
     const float* S_in;  // [B, H, d, e]
     float* S_out;
+    struct DeltaGates* gates;  // [B * H][nc]
     unsigned char* Y;   // [B * H][nc][NX][10 blocks of 512 bytes]
     unsigned char* S0;  // [B * H][nc][ep / 16][dp / 16][NX][512], or null (not stored)
     unsigned char* W;   // [B * H][nc][ep / 16][4][NX][512], or null
@@ -71,6 +72,18 @@ constexpr int kDeltaC = 64;      // tokens per chunk
 constexpr int kDeltaCols = 32;   // value columns per CTA of the chunk walks
 constexpr int kYBlocks = 10;     // 16 x 16 blocks of the lower triangle of a 64 x 64 matrix
 constexpr float kMinLogGamma = -120.f;  // exp() of anything lower is 0 in float32 as well
+
+// Gates of one chunk, formed once (delta_prep_kernel) and read by every kernel.
+struct alignas(16) DeltaGates {
+    float gh[kDeltaC], gl[kDeltaC];  // running sum of log gamma: g = gh + gl
+    float beta[kDeltaC];             // 0 on masked tokens
+    float eg[kDeltaC];               // e^g
+    float kd[kDeltaC];               // e^{g_C - g}
+    int live[kDeltaC];
+    float eC;                        // e^{g_C}
+    int any;                         // a live token in the chunk
+};
+static_assert(sizeof(DeltaGates) % 16 == 0 && sizeof(DeltaGates) <= 128 * 16, "one 16-byte piece per loading thread");
 
 template <typename T> struct DeltaType;
 template <> struct DeltaType<__nv_bfloat16> { static constexpr int kIn = 1, kX = 2; };
@@ -200,22 +213,14 @@ __device__ __forceinline__ void a_cols(uint32_t (&r)[4], uint32_t tile, int k0, 
 __device__ __forceinline__ int tri(int ib, int jb) { return (ib * (ib + 1) >> 1) + jb; }
 
 // ---- gates of one chunk
-struct Gates {
-    float gh[kDeltaC], gl[kDeltaC];  // running sum of log gamma: g = gh + gl
-    float beta[kDeltaC];             // 0 on masked tokens
-    float eg[kDeltaC];               // e^g
-    float kd[kDeltaC];               // e^{g_C - g}
-    int live[kDeltaC];
-    float eC;                        // e^{g_C}
-    int any;                         // live tokens in the chunk
-};
+using Gates = DeltaGates;
 
 __device__ __forceinline__ float gamma_ij(const Gates& s, int i, int j) {  // i >= j
     return expf((s.gh[i] - s.gh[j]) + (s.gl[i] - s.gl[j]));
 }
 
-// Fills `s` for tokens n0 .. n0 + 63 (one warp, every lane).
-__device__ __forceinline__ void load_gates(Gates& s, const DeltaParams& p, int b, int h, int n0, int lane) {
+// Forms the gates of tokens n0 .. n0 + 63 (one warp, every lane).
+__device__ __forceinline__ void form_gates(Gates& s, const DeltaParams& p, int b, int h, int n0, int lane) {
     double g[2];
     float be[2];
     int lv[2];
@@ -259,87 +264,122 @@ __device__ __forceinline__ void load_gates(Gates& s, const DeltaParams& p, int b
     }
 }
 
-// ---- loads of [64][W] tiles from global memory
-template <typename T> __device__ __forceinline__ float as_float(T x) { return to_f<T>(x); }
+// ---- [64][W] tiles from global memory, through registers
+// A tile's 16-byte pieces (8 elements) in the registers of NT threads, between
+// the load (issue) and, an iteration later, the store to shared memory: masked
+// rows are zeroed there, whatever memory holds.
+template <typename T, int W, int NT>
+struct TileRegs {
+    static constexpr int kPieces = W / 8, kPer = 64 * kPieces / NT, kQ = sizeof(T) / 2;
+    static_assert(64 * kPieces % NT == 0, "threads per tile");
+    uint4 r[kPer][kQ];
 
-// Eight elements of row `n` from column c (zeros past the tensor's width or for dead rows).
-template <typename T>
-__device__ __forceinline__ void load8(float (&f)[8], const T* row, int c, int width, bool vec) {
-    if (vec && c + 8 <= width) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 u = *reinterpret_cast<const uint4*>(row + c);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    __device__ __forceinline__ void issue(const DeltaTensor& x, int64_t base, int n0, int c0, int width, int N, int tid) {
+        const T* src = static_cast<const T*>(x.p) + base;
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int idx = tid + u * NT, n = n0 + idx / kPieces, c = c0 + idx % kPieces * 8;
+            const T* at = src + n * x.sn + c;
+            if (n < N && x.vec && c + 8 <= width) {
+#pragma unroll
+                for (int i = 0; i < kQ; ++i) r[u][i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
+            } else {
+                alignas(16) T t[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = n < N && c + i < width ? at[i] : from_f<T>(0.f);
+#pragma unroll
+                for (int i = 0; i < kQ; ++i) r[u][i] = reinterpret_cast<const uint4*>(t)[i];
+            }
+        }
+    }
+
+    __device__ __forceinline__ void values(int u, float (&f)[8]) const {
+        if constexpr (kQ == 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f[4 * i] = __uint_as_float(r[u][i].x);
+                f[4 * i + 1] = __uint_as_float(r[u][i].y);
+                f[4 * i + 2] = __uint_as_float(r[u][i].z);
+                f[4 * i + 3] = __uint_as_float(r[u][i].w);
+            }
+        } else {
+            const uint32_t w[4] = {r[u][0].x, r[u][0].y, r[u][0].z, r[u][0].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 T t[2];
                 *reinterpret_cast<uint32_t*>(t) = w[i];
-                f[2 * i] = as_float<T>(t[0]);
-                f[2 * i + 1] = as_float<T>(t[1]);
+                f[2 * i] = to_f<T>(t[0]);
+                f[2 * i + 1] = to_f<T>(t[1]);
             }
-        } else {
-            const float4 a = reinterpret_cast<const float4*>(row + c)[0], b = reinterpret_cast<const float4*>(row + c)[1];
-            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-            f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = c + i < width ? as_float<T>(row[c + i]) : 0.f;
     }
-}
 
-// [64][W] tile of columns c0 .. c0 + W - 1 as NP bf16 planes; dead rows are zero
-// whatever memory holds there. NT threads, `tid` of them.
-template <typename T, int W, int NP, int NT>
-__device__ __forceinline__ void load_planes(unsigned char* tile, const DeltaTensor& x, int64_t base, int n0, int c0, int width,
-                                            const int* live, int tid) {
-    constexpr int kPieces = W / 8, kPer = 64 * kPieces / NT, kBatch = kPer < 4 ? kPer : 4;
-    static_assert(64 * kPieces % NT == 0, "threads per tile");
-    const T* src = static_cast<const T*>(x.p) + base;
+    // as NP bf16 planes of [64][W]
+    template <int NP>
+    __device__ __forceinline__ void store_planes(unsigned char* tile, const int* live, int tid) const {
 #pragma unroll
-    for (int u0 = 0; u0 < kPer; u0 += kBatch) {
-        float f[kBatch][8];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int idx = tid + (u0 + u) * NT, row = idx / kPieces, piece = idx % kPieces;
-            if (live[row]) {
-                load8<T>(f[u], src + (n0 + row) * x.sn, c0 + piece * 8, width, x.vec);
+        for (int u = 0; u < kPer; ++u) {
+            const int idx = tid + u * NT, row = idx / kPieces, piece = idx % kPieces;
+            unsigned char* at = tile + tile_off<W>(row, piece);
+            const bool on = live[row] != 0;
+            if constexpr (NP == 1) {
+                *reinterpret_cast<uint4*>(at) = on ? r[u][0] : make_uint4(0, 0, 0, 0);
             } else {
+                float f[8];
+                values(u, f);
+                uint32_t q[4][NP];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+                for (int i = 0; i < 4; ++i) split2<NP>(on ? f[2 * i] : 0.f, on ? f[2 * i + 1] : 0.f, q[i]);
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl)
+                    *reinterpret_cast<uint4*>(at + pl * (64 * W * 2)) = make_uint4(q[0][pl], q[1][pl], q[2][pl], q[3][pl]);
             }
         }
+    }
+
+    // as float32 rows of kVPitch
+    __device__ __forceinline__ void store_float(float* tile, const int* live, int tid) const {
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int idx = tid + (u0 + u) * NT, row = idx / kPieces, piece = idx % kPieces;
-            uint32_t r[4][NP];
+        for (int u = 0; u < kPer; ++u) {
+            const int idx = tid + u * NT, row = idx / kPieces, piece = idx % kPieces;
+            const bool on = live[row] != 0;
+            float f[8];
+            values(u, f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) split2<NP>(f[u][2 * i], f[u][2 * i + 1], r[i]);
-#pragma unroll
-            for (int pl = 0; pl < NP; ++pl)
-                *reinterpret_cast<uint4*>(tile + pl * (64 * W * 2) + tile_off<W>(row, piece)) =
-                    make_uint4(r[0][pl], r[1][pl], r[2][pl], r[3][pl]);
+            for (int i = 0; i < 8; ++i) f[i] = on ? f[i] : 0.f;
+            float4* dst = reinterpret_cast<float4*>(tile + row * (W + 4) + piece * 8);
+            dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+            dst[1] = make_float4(f[4], f[5], f[6], f[7]);
         }
     }
-}
+};
 
 constexpr int kVPitch = 36;  // floats per row of a [64][32] float tile: rows two apart fall 8 banks apart
 
-template <typename T, int NT>
-__device__ __forceinline__ void load_float_tile(float* tile, const DeltaTensor& x, int64_t base, int n0, int c0, int width,
-                                                const int* live, int tid) {
-    constexpr int kPer = 64 * 4 / NT;
-    static_assert(kPer >= 1, "threads per tile");
-    const T* src = static_cast<const T*>(x.p) + base;
+// BYTES contiguous bytes (a multiple of 16) the same way.
+template <int BYTES, int NT>
+struct ByteRegs {
+    static constexpr int kPer = (BYTES / 16 + NT - 1) / NT;
+    uint4 r[kPer];
+    __device__ __forceinline__ void issue(const void* src, int tid) {
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-        const int idx = tid + u * NT, row = idx >> 2, piece = idx & 3;
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live[row]) load8<T>(f, src + (n0 + row) * x.sn, c0 + piece * 8, width, x.vec);
-        float4* dst = reinterpret_cast<float4*>(tile + row * kVPitch + piece * 8);
-        dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-        dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+        for (int u = 0; u < kPer; ++u)
+            if (tid + u * NT < BYTES / 16) r[u] = __ldg(static_cast<const uint4*>(src) + tid + u * NT);
     }
+    __device__ __forceinline__ void store(void* dst, int tid) const {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u)
+            if (tid + u * NT < BYTES / 16) static_cast<uint4*>(dst)[tid + u * NT] = r[u];
+    }
+};
+
+// NT threads start BYTES contiguous bytes on their way to shared memory.
+template <int NT>
+__device__ __forceinline__ void async16(unsigned char* dst, const unsigned char* src, int bytes, int tid) {
+    for (int i = tid * 16; i < bytes; i += NT * 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst + i)), "l"(src + i) : "memory");
 }
+__device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <int NT>
 __device__ __forceinline__ void copy16(unsigned char* dst, const unsigned char* src, int bytes, int tid) {

@@ -38,10 +38,13 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
     const int64_t chunk = blockIdx.x;  // bh * nc + c
     const int64_t bh = chunk / p.nc;
     const int c = (int)(chunk % p.nc), b = (int)(bh / p.H), h = (int)(bh % p.H), n0 = c * kDeltaC;
-    if (warp == 0) load_gates(sm.s, p, b, h, n0, lane);
+    TileRegs<T, DP, 128> k;
+    k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, tid);
+    if (warp == 0) form_gates(sm.s, p, b, h, n0, lane);
     __syncthreads();
+    copy16<128>(reinterpret_cast<unsigned char*>(p.gates + chunk), reinterpret_cast<const unsigned char*>(&sm.s), sizeof(Gates), tid);
     if (!sm.s.any) return;  // no kernel reads Y of a dead chunk
-    load_planes<T, DP, NIN, 128>(sm.k, p.k, tensor_base(p.k, b, h), n0, 0, p.d, sm.s.live, tid);
+    k.template store_planes<NIN>(sm.k, sm.s.live, tid);
     __syncthreads();
     {  // A, rows 16 warp .. 16 warp + 15
         float acc[8][4];
@@ -161,18 +164,6 @@ __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p
     const int64_t bh = blockIdx.x / ncb;
     const int cb = blockIdx.x % ncb, b = (int)(bh / p.H), h = (int)(bh % p.H), c0 = cb * kDeltaCols;
     const int g = lane >> 2, t = lane & 3;
-
-    auto load_stage = [&](int c) {  // warps 4..7
-        auto& st = sm.st[c % NST];
-        const int lt = tid - 128, n0 = c * kDeltaC;
-        if (warp == 4) load_gates(st.s, p, b, h, n0, lane);
-        bar_sync(3, 128);
-        if (!st.s.any) return;
-        load_planes<T, DP, NIN, 128>(st.k, p.k, tensor_base(p.k, b, h), n0, 0, p.d, st.s.live, lt);
-        copy16<128>(st.y, p.Y + (bh * p.nc + c) * (NX * kYBlocks * 512), NX * kYBlocks * 512, lt);
-        load_float_tile<T, 128>(st.v, p.v, tensor_base(p.v, b, h), n0, c0, p.e, st.s.live, lt);
-        load_planes<T, DP, NIN, 128>(st.q, p.q, tensor_base(p.q, b, h), n0, 0, p.d, st.s.live, lt);
-    };
 
     if (warp < 2) {  // ---------------------------------------------------- chain
         float S[DP / 8][4];
@@ -418,15 +409,49 @@ __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p
             __syncthreads();
         }
     } else {  // ---------------------------------------------------------- loads
-        if (NST == 2) load_stage(0);
+        // the loads of a chunk are in flight for a whole iteration: issued for chunk
+        // c + 2 (c + 1 with one stage) while c is computed, stored an iteration later
+        const int lt = tid - 128;
+        const Gates* gates = p.gates + bh * p.nc;
+        TileRegs<T, DP, 128> k, q;
+        TileRegs<T, kDeltaCols, 128> v;
+        ByteRegs<NX * kYBlocks * 512, 128> y;
+        ByteRegs<sizeof(Gates), 128> s;
+        int any = 0, any_next = 0;  // of the chunk in the registers, and of the one after it
+        auto issue = [&](int c) {
+            any = any_next;
+            any_next = c + 1 < p.nc ? gates[c + 1].any : 0;
+            if (c >= p.nc) return;
+            s.issue(gates + c, lt);
+            if (!any) return;
+            const int n0 = c * kDeltaC;
+            k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, lt);
+            y.issue(p.Y + (bh * p.nc + c) * (NX * kYBlocks * 512), lt);
+            v.issue(p.v, tensor_base(p.v, b, h), n0, c0, p.e, p.N, lt);
+            if (p.o.p) q.issue(p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, lt);
+        };
+        auto store = [&](int c) {
+            if (c >= p.nc) return;
+            auto& st = sm.st[c % NST];
+            s.store(&st.s, lt);
+            bar_sync(3, 128);
+            if (!any) return;
+            k.template store_planes<NIN>(st.k, st.s.live, lt);
+            y.store(st.y, lt);
+            v.store_float(st.v, st.s.live, lt);
+            if (p.o.p) q.template store_planes<NIN>(st.q, st.s.live, lt);
+        };
+        any_next = gates[0].any;
+        issue(0);
+        if (NST == 2) {
+            store(0);
+            issue(1);
+        }
         __syncthreads();
         for (int c = 0; c < p.nc; ++c) {
-            if (NST == 1) {
-                load_stage(c);
-                __syncthreads();
-            } else if (c + 1 < p.nc) {
-                load_stage(c + 1);
-            }
+            store(c + NST - 1);
+            issue(c + NST);
+            if (NST == 1) __syncthreads();
             __syncthreads();
         }
     }
