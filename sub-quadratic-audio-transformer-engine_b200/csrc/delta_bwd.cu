@@ -27,17 +27,20 @@ using namespace dl;
 template <typename T, int DP>
 struct RevSmem {
     static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
-    static constexpr int kStages = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+    static constexpr int kStages = kIn > 1 && DP == 128 ? 1 : 2;
     struct Stage {
         alignas(128) unsigned char k[kIn * 64 * DP * 2];
         alignas(128) unsigned char q[kIn * 64 * DP * 2];
         alignas(128) unsigned char y[kX * kYBlocks * 512];
         alignas(128) unsigned char g[kIn * 64 * kDeltaCols * 2];  // dO
+        alignas(128) unsigned char P[kX * kYBlocks * 512];        // scale G o (Q K^T)
         Gates s;
     } st[kStages];
-    alignas(128) unsigned char P[kX * kYBlocks * 512];
-    alignas(16) float e1[2][8 * 128];       // (P^T dO)^T accumulators per warp of 16 columns
-    alignas(16) float e2[2][DP / 8 * 128];  // (scale (e^g Q)^T dO)^T
+    // float32 accumulators between a chain warp and the warp beside it
+    float4 e1[2][8 * 32];       // (P^T dO)^T
+    float4 e2[2][DP / 8 * 32];  // (scale (e^g Q)^T dO)^T
+    float4 G[2][DP / 8 * 32];
+    float4 Z[2][8 * 32];
 };
 
 template <typename T, int DP>
@@ -63,10 +66,9 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                 const int d = 8 * n + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
                 S[n][i] = (G_in && d < p.d && col < p.e) ? G_in[(int64_t)d * p.e + col] : 0.f;
             }
-        const int64_t cw = 2 * cb + warp, ncw = 2 * ncb;
         bool pending = false;  // e2 of the chunk before has to be added
         auto add_e2 = [&]() {
-            const float4* e2 = reinterpret_cast<const float4*>(sm.e2[warp]);
+            const float4* e2 = sm.e2[warp];
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n) {
                 const float4 x = e2[n * 32 + lane];
@@ -82,7 +84,7 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
             pending = s.any;
             if (s.any) {
                 const uint32_t kt = smem_addr(st.k);
-                unsigned char* gdst = p.dS + ((bh * p.nc + c) * ncw + cw) * (DP / 16 * NX * 512) + lane * 4;
+                put_acc<DP / 8>(sm.G[warp], S, lane);
                 float X[8][4];
 #pragma unroll
                 for (int n = 0; n < 8; ++n)
@@ -93,11 +95,6 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                 for (int kk = 0; kk < DP / 16; ++kk) {  // (K G)^T
                     uint32_t a[NX][4];
                     to_a<NX>(S[2 * kk], S[2 * kk + 1], one, one, a);
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m)
-                            *reinterpret_cast<uint32_t*>(gdst + (kk * NX + pl) * 512 + m * 128) = a[pl][m];
 #pragma unroll
                     for (int jp = 0; jp < 4; ++jp) {
                         uint32_t b0[NIN][2], b1[NIN][2];
@@ -111,8 +108,8 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                         mma_planes<NX, NIN, NX>(X[2 * jp + 1], a, b1);
                     }
                 }
-                bar_sync(1, 128);  // e1 is there, and e2 of the chunk before has been read
-                const float4* e1 = reinterpret_cast<const float4*>(sm.e1[warp]);
+                bar_sync(1, 128);  // e1 and G are there, e2 and Z of the chunk before have been read
+                const float4* e1 = sm.e1[warp];
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {  // dU^T
                     const float4 x = e1[n * 32 + lane];
@@ -145,7 +142,7 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                         mma_planes<NX, NX, NX>(X[2 * jb], ra[ib], b0);
                         mma_planes<NX, NX, NX>(X[2 * jb + 1], ra[ib], b1);
                     }
-                unsigned char* zdst = p.Z + ((bh * p.nc + c) * ncw + cw) * (4 * NX * 512) + lane * 4;
+                put_acc<8>(sm.Z[warp], X, lane);
 #pragma unroll
                 for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
@@ -153,12 +150,6 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
 #pragma unroll
                 for (int jb = 0; jb < 4; ++jb) {
                     uint32_t a[NX][4];
-                    to_a<NX>(X[2 * jb], X[2 * jb + 1], one, one, a);
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m)
-                            *reinterpret_cast<uint32_t*>(zdst + (jb * NX + pl) * 512 + m * 128) = a[pl][m];
                     float2 f[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -193,25 +184,36 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                     if (d < p.d && col < p.e) G_out[(int64_t)d * p.e + col] = S[n][i];
                 }
         }
-    } else if (warp < 4) {  // ------------------------------- P^T dO and (e^g Q)^T dO
+    } else if (warp < 4) {  // ------------------------------- P^T dO, (e^g Q)^T dO, planes of G and Z
         const int w = warp - 2;
+        auto planes = [&](unsigned char* base, int c, int tiles) {  // of this warp's 16 columns
+            return base + ((bh * p.nc + c) * 2 * ncb + 2 * cb + w) * (tiles * NX * 512);
+        };
+        int last = -1;  // the chunk whose Z waits in shared memory
+        auto flush_z = [&]() {
+            if (last < 0) return;
+            unsigned char* dst = planes(p.Z, last, 4);
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {
+                uint32_t a[NX][4];
+                get_a<NX>(sm.Z[w], jb, a, dst, lane);
+            }
+            last = -1;
+        };
         __syncthreads();
         for (int c = p.nc - 1; c >= 0; --c) {
             if (NST == 1) __syncthreads();
             auto& st = sm.st[c % NST];
             const Gates& s = st.s;
+            flush_z();
             if (s.any) {
-                const uint32_t kt = smem_addr(st.k), qt = smem_addr(st.q), gt = smem_addr(st.g);
-                score_rows<DP, NIN, NX>(sm.P, qt, kt, s, p.scale, false, w ? 1 : 0, lane);
-                score_rows<DP, NIN, NX>(sm.P, qt, kt, s, p.scale, false, w ? 2 : 3, lane);
-                bar_sync(2, 64);
+                const uint32_t qt = smem_addr(st.q), gt = smem_addr(st.g), pt = smem_addr(st.P) + lane * 16;
                 uint32_t da[4][NIN][4];  // dO^T: 16 value columns x 64 tokens
 #pragma unroll
                 for (int ib = 0; ib < 4; ++ib)
 #pragma unroll
                     for (int pl = 0; pl < NIN; ++pl) a_cols<kDeltaCols>(da[ib][pl], gt + pl * kGTile, 16 * ib, w, lane);
-                const uint32_t pt = smem_addr(sm.P) + lane * 16;
-                float4* e1 = reinterpret_cast<float4*>(sm.e1[w]);
+                float4* e1 = sm.e1[w];
 #pragma unroll
                 for (int jb = 0; jb < 4; ++jb) {
                     float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -231,6 +233,13 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                     e1[(2 * jb + 1) * 32 + lane] = make_float4(a1[0], a1[1], a1[2], a1[3]);
                 }
                 bar_sync(1, 128);
+                last = c;
+                unsigned char* gdst = planes(p.dS, c, DP / 16);
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    uint32_t a[NX][4];
+                    get_a<NX>(sm.G[w], kk, a, gdst, lane);
+                }
                 float E[DP / 8][4];
 #pragma unroll
                 for (int n = 0; n < DP / 8; ++n)
@@ -267,12 +276,11 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                         mma_planes<NX, NIN, NX>(E[2 * np + 1], a, b1);
                     }
                 }
-                float4* e2 = reinterpret_cast<float4*>(sm.e2[w]);
-#pragma unroll
-                for (int n = 0; n < DP / 8; ++n) e2[n * 32 + lane] = make_float4(E[n][0], E[n][1], E[n][2], E[n][3]);
+                put_acc<DP / 8>(sm.e2[w], E, lane);
             }
             __syncthreads();
         }
+        flush_z();
     } else {  // ---------------------------------------------------------- loads
         const int lt = tid - 128;  // as in the forward's walk, from the last chunk to the first
         const Gates* gates = p.gates + bh * p.nc;
@@ -303,17 +311,27 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
             q.template store_planes<NIN>(st.q, st.s.live, lt);
             x.template store_planes<NIN>(st.g, st.s.live, lt);
             y.store(st.y, lt);
+            bar_sync(3, 128);
+        };
+        auto scores = [&](int c, bool on) {
+            auto& st = sm.st[c % NST];
+            if (on) score_rows<DP, NIN, NX>(st.P, smem_addr(st.q), smem_addr(st.k), st.s, p.scale, false, warp - 4, lane);
         };
         any_next = gates[p.nc - 1].any;
         issue(p.nc - 1);
         if (NST == 2) {
+            const bool on = any;
             store(p.nc - 1);
             issue(p.nc - 2);
+            scores(p.nc - 1, on);
         }
         __syncthreads();
         for (int c = p.nc - 1; c >= 0; --c) {
-            store(c - (NST - 1));
+            const int next = c - (NST - 1);
+            const bool on = any && next >= 0;
+            store(next);
             issue(c - NST);
+            if (on) scores(next, on);
             if (NST == 1) __syncthreads();
             __syncthreads();
         }
@@ -590,26 +608,26 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     }
 
     {  // D1 or D2 as planes
-        unsigned char* dst = hf ? sm.u.sc.d2 : sm.u.sc.d1;
+        unsigned char* dst = (hf ? sm.u.sc.d2 : sm.u.sc.d1) + lane * 4;
 #pragma unroll
-        for (int jb = 0; jb < 4; ++jb) {
-            if (jb > rb) continue;
+        for (int ih = 0; ih < 2; ++ih) {
+            const int i = 16 * rb + 8 * ih + g, keep = hf ? i - 1 : i;
+            const float gh = s.gh[i], gl = s.gl[i], fi = hf ? -s.beta[i] : p.scale;
 #pragma unroll
-            for (int jh = 0; jh < 2; ++jh)
+            for (int jb = 0; jb < 4; ++jb) {
+                if (jb > rb) continue;
 #pragma unroll
-                for (int ih = 0; ih < 2; ++ih) {
-                    const int i = 16 * rb + 8 * ih + g, j = 16 * jb + 8 * jh + 2 * t;
-                    const float fi = hf ? -s.beta[i] : p.scale;
-                    float x = 0.f, y = 0.f;
-                    if (j < i || (j == i && !hf)) x = fi * s.beta[j] * gamma_ij(s, i, j) * D[2 * jb + jh][2 * ih];
-                    if (j + 1 < i || (j + 1 == i && !hf))
-                        y = fi * s.beta[j + 1] * gamma_ij(s, i, j + 1) * D[2 * jb + jh][2 * ih + 1];
+                for (int jh = 0; jh < 2; ++jh) {
+                    const int j = 16 * jb + 8 * jh + 2 * t;
+                    const float2 ga = gamma_pair(gh, gl, s, j, keep), be = *reinterpret_cast<const float2*>(&s.beta[j]);
                     uint32_t r[NX];
-                    split2<NX>(x, y, r);
+                    split2<NX>(fi * be.x * ga.x * select0(j <= keep, D[2 * jb + jh][2 * ih]),
+                               fi * be.y * ga.y * select0(j + 1 <= keep, D[2 * jb + jh][2 * ih + 1]), r);
 #pragma unroll
                     for (int pl = 0; pl < NX; ++pl)
-                        *reinterpret_cast<uint32_t*>(dst + (pl * kYBlocks + tri(rb, jb)) * 512 + (ih * 2 + jh) * 128 + lane * 4) = r[pl];
+                        *reinterpret_cast<uint32_t*>(dst + (pl * kYBlocks + tri(rb, jb)) * 512 + (ih * 2 + jh) * 128) = r[pl];
                 }
+            }
         }
     }
     {  // row factors of the products with the states; k.dk1 before anything is added to it

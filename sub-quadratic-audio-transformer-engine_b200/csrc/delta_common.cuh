@@ -75,7 +75,7 @@ constexpr float kMinLogGamma = -120.f;  // exp() of anything lower is 0 in float
 
 // Gates of one chunk, formed once (delta_prep_kernel) and read by every kernel.
 struct alignas(16) DeltaGates {
-    float gh[kDeltaC], gl[kDeltaC];  // running sum of log gamma: g = gh + gl
+    float gh[kDeltaC], gl[kDeltaC];  // running sum of log2 gamma: g / ln 2 = gh + gl
     float beta[kDeltaC];             // 0 on masked tokens
     float eg[kDeltaC];               // e^g
     float kd[kDeltaC];               // e^{g_C - g}
@@ -215,9 +215,14 @@ __device__ __forceinline__ int tri(int ib, int jb) { return (ib * (ib + 1) >> 1)
 // ---- gates of one chunk
 using Gates = DeltaGates;
 
-__device__ __forceinline__ float gamma_ij(const Gates& s, int i, int j) {  // i >= j
-    return expf((s.gh[i] - s.gh[j]) + (s.gl[i] - s.gl[j]));
+// G_ij for row i (its gh, gl) and columns j, j + 1; `keep`: the largest column that counts,
+// the others are 0 (their exponent may overflow, so they are selected away, not multiplied).
+__device__ __forceinline__ float2 gamma_pair(float gh, float gl, const Gates& s, int j, int keep) {
+    const float2 h = *reinterpret_cast<const float2*>(&s.gh[j]), l = *reinterpret_cast<const float2*>(&s.gl[j]);
+    const float x = exp2f((gh - h.x) + (gl - l.x)), y = exp2f((gh - h.y) + (gl - l.y));
+    return make_float2(j <= keep ? x : 0.f, j + 1 <= keep ? y : 0.f);
 }
+__device__ __forceinline__ float select0(bool on, float x) { return on ? x : 0.f; }
 
 // Forms the gates of tokens n0 .. n0 + 63 (one warp, every lane).
 __device__ __forceinline__ void form_gates(Gates& s, const DeltaParams& p, int b, int h, int n0, int lane) {
@@ -250,9 +255,10 @@ __device__ __forceinline__ void form_gates(Gates& s, const DeltaParams& p, int b
     for (int i = 0; i < 2; ++i) {
         const double gi = i ? run : run - g[1];
         const int t = 2 * lane + i;
-        const float hi = (float)gi;
+        const double g2 = gi * 1.4426950408889634;  // 1 / ln 2
+        const float hi = (float)g2;
         s.gh[t] = hi;
-        s.gl[t] = (float)(gi - (double)hi);
+        s.gl[t] = (float)(g2 - (double)hi);
         s.beta[t] = be[i];
         s.eg[t] = expf((float)gi);
         s.kd[t] = expf((float)(total - gi));
@@ -422,29 +428,52 @@ __device__ __forceinline__ void score_rows(unsigned char* out, uint32_t q, uint3
             }
         }
     }
-    const int g = lane >> 2, t = lane & 3;
+    const int g = lane >> 2, t = lane & 3, i0 = 16 * rb + g;
+    const float gh[2] = {s.gh[i0], s.gh[i0 + 8]}, gl[2] = {s.gl[i0], s.gl[i0 + 8]};
 #pragma unroll
     for (int jb = 0; jb < 4; ++jb) {
         if (jb > rb) continue;
         unsigned char* blk = out + tri(rb, jb) * 512 + lane * 4;
 #pragma unroll
-        for (int jh = 0; jh < 2; ++jh)
+        for (int jh = 0; jh < 2; ++jh) {
+            const int j = 16 * jb + 8 * jh + 2 * t;
+            float2 f = make_float2(scale, scale);
+            if (with_beta) {
+                const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]);
+                f = make_float2(scale * be.x, scale * be.y);
+            }
 #pragma unroll
             for (int ih = 0; ih < 2; ++ih) {
-                const int i = 16 * rb + 8 * ih + g, j = 16 * jb + 8 * jh + 2 * t;
-                float x = 0.f, y = 0.f;
-                if (j <= i) x = scale * gamma_ij(s, i, j) * acc[2 * jb + jh][2 * ih];
-                if (j + 1 <= i) y = scale * gamma_ij(s, i, j + 1) * acc[2 * jb + jh][2 * ih + 1];
-                if (with_beta) {
-                    x *= s.beta[j];
-                    y *= s.beta[j + 1];
-                }
+                const float2 ga = gamma_pair(gh[ih], gl[ih], s, j, i0 + 8 * ih);
                 uint32_t r[NX];
-                split2<NX>(x, y, r);
+                split2<NX>(f.x * ga.x * select0(j <= i0 + 8 * ih, acc[2 * jb + jh][2 * ih]),
+                           f.y * ga.y * select0(j + 1 <= i0 + 8 * ih, acc[2 * jb + jh][2 * ih + 1]), r);
 #pragma unroll
                 for (int pl = 0; pl < NX; ++pl)
                     *reinterpret_cast<uint32_t*>(blk + pl * (kYBlocks * 512) + (ih * 2 + jh) * 128) = r[pl];
             }
+        }
+    }
+}
+
+// An accumulator tile (NB blocks of 16 rows x 8 columns) through shared memory, 16 bytes per lane and block.
+template <int NB>
+__device__ __forceinline__ void put_acc(float4* at, const float (&c)[NB][4], int lane) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) at[n * 32 + lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+}
+// Blocks 2 kk, 2 kk + 1 of such a tile as the planes of an A operand, and to memory (`dst`, or null) as 8 x 8 matrices.
+template <int NX>
+__device__ __forceinline__ void get_a(const float4* at, int kk, uint32_t (&a)[NX][4], unsigned char* dst, int lane) {
+    const float4 x = at[2 * kk * 32 + lane], y = at[(2 * kk + 1) * 32 + lane];
+    const float c0[4] = {x.x, x.y, x.z, x.w}, c1[4] = {y.x, y.y, y.z, y.w};
+    const float2 one = make_float2(1.f, 1.f);
+    to_a<NX>(c0, c1, one, one, a);
+    if (dst) {
+#pragma unroll
+        for (int pl = 0; pl < NX; ++pl)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) *reinterpret_cast<uint32_t*>(dst + (kk * NX + pl) * 512 + m * 128 + lane * 4) = a[pl][m];
     }
 }
 

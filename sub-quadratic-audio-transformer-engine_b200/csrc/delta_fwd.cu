@@ -6,10 +6,11 @@
 // accumulator layout is the A operand layout of the next product, so the chain
 // S0 -> R -> W -> S' stays in one warp's registers and no warp waits for another
 // value column. All products are transposed accordingly (rows = value columns,
-// columns = tokens or d). Per CTA, 32 columns: two such chain warps, two output
-// warps (scores, Q S0 and score W products of the chain warp with the same
-// columns, from the S0 and W planes it leaves in shared memory) and four warps
-// that load and convert the next chunk.
+// columns = tokens or d). Per CTA, 32 columns: two such chain warps; two output
+// warps (Q S0 and score W products of the chain warp with the same columns, from
+// the float32 S0 and W it leaves in shared memory; they also write the planes the
+// backward reads); and four warps that load and convert the next chunk and form
+// its scores. The chain warp does nothing that another warp can do.
 #include "delta_common.cuh"
 #include "delta_launch.h"
 #include "scan_launch.h"
@@ -73,13 +74,18 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
         }
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-            if (n <= 2 * warp + 1)
+        for (int ih = 0; ih < 2; ++ih) {
+            const int i = 16 * warp + 8 * ih + g;
+            const float gh = sm.s.gh[i], gl = sm.s.gl[i];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int i = 16 * warp + 8 * (x >> 1) + g, j = 8 * n + 2 * t + (x & 1);
-                    sm.A[i][j] = j < i ? gamma_ij(sm.s, i, j) * acc[n][x] : 0.f;
+            for (int n = 0; n < 8; ++n)
+                if (n <= 2 * warp + 1) {
+                    const int j = 8 * n + 2 * t;
+                    const float2 ga = gamma_pair(gh, gl, sm.s, j, i - 1);
+                    *reinterpret_cast<float2*>(&sm.A[i][j]) =
+                        make_float2(ga.x * select0(j < i, acc[n][2 * ih]), ga.y * select0(j + 1 < i, acc[n][2 * ih + 1]));
                 }
+        }
     }
     __syncthreads();
     if (tid < kDeltaC) {  // column tid of Y by forward substitution: y_i = A_i - sum_j A_ij beta_j y_j
@@ -119,39 +125,20 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
 template <typename T, int DP>
 struct ChainSmem {
     static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
-    // chunks in shared memory: the one at work and the next, where both fit (not float32 with d > 64)
-    static constexpr int kStages = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+    // chunks in shared memory: the one at work and the next, where both fit (with d > 64 for bf16 only)
+    static constexpr int kStages = kIn > 1 && DP == 128 ? 1 : 2;
     struct Stage {
         alignas(128) unsigned char k[kIn * 64 * DP * 2];
         alignas(128) unsigned char q[kIn * 64 * DP * 2];
         alignas(128) unsigned char y[kX * kYBlocks * 512];
         alignas(16) float v[kDeltaC * kVPitch];
+        alignas(128) unsigned char P[kX * kYBlocks * 512];  // scale G o (Q K^T) beta
         Gates s;
     } st[kStages];
-    alignas(128) unsigned char S0[2][2][DP / 16 * kX * 512];  // [chunk parity][chain warp]
-    alignas(128) unsigned char W[2][4 * kX * 512];
-    alignas(128) unsigned char P[kX * kYBlocks * 512];
+    float4 S0[2][2][DP / 8 * 32];  // S^T accumulators before the chunk: [chunk parity][chain warp]
+    float4 W[2][8 * 32];           // W^T accumulators
     alignas(16) unsigned char out[2][kDeltaC * (16 * sizeof(T) + 16)];
 };
-
-// S^T accumulators (16 value columns x DP) as planes of 8 x 8 matrices, to shared memory and (`dst`) global memory.
-template <int DP, int NX>
-__device__ __forceinline__ void store_state_planes(const float (&S)[DP / 8][4], unsigned char* tile, unsigned char* dst, int lane) {
-    const float2 one = make_float2(1.f, 1.f);
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-        uint32_t a[NX][4];
-        to_a<NX>(S[2 * kk], S[2 * kk + 1], one, one, a);
-#pragma unroll
-        for (int pl = 0; pl < NX; ++pl)
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const int off = (kk * NX + pl) * 512 + m * 128 + lane * 4;
-                *reinterpret_cast<uint32_t*>(tile + off) = a[pl][m];
-                if (dst) *reinterpret_cast<uint32_t*>(dst + off) = a[pl][m];
-            }
-    }
-}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p) {
@@ -176,29 +163,24 @@ __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p
                 const int d = 8 * n + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
                 S[n][i] = (S_in && d < p.d && col < p.e) ? S_in[(int64_t)d * p.e + col] : 0.f;
             }
-        const int64_t cw = 2 * cb + warp;  // 16-column group
-        const int64_t ncw = 2 * ncb;
-        auto s0_at = [&](int c) {
-            return p.S0 && c < p.nc ? p.S0 + ((bh * p.nc + c) * ncw + cw) * (DP / 16 * NX * 512) : nullptr;
-        };
-        store_state_planes<DP, NX>(S, sm.S0[0][warp], s0_at(0), lane);
+        put_acc<DP / 8>(sm.S0[0][warp], S, lane);
         __syncthreads();
         for (int c = 0; c < p.nc; ++c) {
             if (NST == 1) __syncthreads();  // the chunk is loaded
             auto& st = sm.st[c % NST];
             const Gates& s = st.s;
             if (s.any) {
-                const uint32_t kt = smem_addr(st.k), s0 = smem_addr(sm.S0[c & 1][warp]) + lane * 16;
+                const uint32_t kt = smem_addr(st.k);
+                const float2 one = make_float2(1.f, 1.f);
                 float X[8][4];
 #pragma unroll
                 for (int n = 0; n < 8; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) X[n][i] = 0.f;
-#pragma unroll 2
+#pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {  // X = S0^T K^T
                     uint32_t a[NX][4];
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl) ldm(a[pl], s0 + (kk * NX + pl) * 512);
+                    to_a<NX>(S[2 * kk], S[2 * kk + 1], one, one, a);
 #pragma unroll
                     for (int jp = 0; jp < 4; ++jp) {
                         uint32_t b0[NIN][2], b1[NIN][2];
@@ -246,22 +228,7 @@ __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p
                         mma_planes<NX, NX, NX>(X[2 * ib], ra[jb], b0);
                         mma_planes<NX, NX, NX>(X[2 * ib + 1], ra[jb], b1);
                     }
-                // W planes for the output warp (and the backward)
-                unsigned char* wdst = p.W ? p.W + ((bh * p.nc + c) * ncw + cw) * (4 * NX * 512) : nullptr;
-#pragma unroll
-                for (int jb = 0; jb < 4; ++jb) {
-                    uint32_t a[NX][4];
-                    const float2 one = make_float2(1.f, 1.f);
-                    to_a<NX>(X[2 * jb], X[2 * jb + 1], one, one, a);
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            const int off = (jb * NX + pl) * 512 + m * 128 + lane * 4;
-                            *reinterpret_cast<uint32_t*>(sm.W[warp] + off) = a[pl][m];
-                            if (wdst) *reinterpret_cast<uint32_t*>(wdst + off) = a[pl][m];
-                        }
-                }
+                put_acc<8>(sm.W[warp], X, lane);
                 bar_arrive(1, 128);
                 // S'^T = e^{g_C} S0^T + (e^{g_C - g} beta W)^T K
 #pragma unroll
@@ -294,7 +261,7 @@ __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p
             } else {
                 bar_arrive(1, 128);
             }
-            store_state_planes<DP, NX>(S, sm.S0[(c + 1) & 1][warp], s0_at(c + 1), lane);
+            put_acc<DP / 8>(sm.S0[(c + 1) & 1][warp], S, lane);
             __syncthreads();
         }
         if (p.S_out) {
@@ -318,21 +285,21 @@ __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p
             const Gates& s = st.s;
             const int n0 = c * kDeltaC, rows = min(kDeltaC, p.N - n0);
             unsigned char* stage = sm.out[w];
-            if (s.any && o) {
-                const uint32_t kt = smem_addr(st.k), qt = smem_addr(st.q);
-                score_rows<DP, NIN, NX>(sm.P, qt, kt, s, p.scale, true, w ? 1 : 0, lane);
-                score_rows<DP, NIN, NX>(sm.P, qt, kt, s, p.scale, true, w ? 2 : 3, lane);
+            if (s.any) {
+                const uint32_t qt = smem_addr(st.q), pt = smem_addr(st.P) + lane * 16;
+                const int64_t cw = (bh * p.nc + c) * 2 * ncb + 2 * cb + w;  // chunk and group of 16 columns
+                unsigned char* s0dst = p.S0 ? p.S0 + cw * (DP / 16 * NX * 512) : nullptr;
+                unsigned char* wdst = p.W ? p.W + cw * (4 * NX * 512) : nullptr;
                 float O[8][4];
 #pragma unroll
                 for (int n = 0; n < 8; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) O[n][i] = 0.f;
-                const uint32_t s0 = smem_addr(sm.S0[c & 1][w]) + lane * 16;
-#pragma unroll 2
+#pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {  // S0^T Q^T
                     uint32_t a[NX][4];
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl) ldm(a[pl], s0 + (kk * NX + pl) * 512);
+                    get_a<NX>(sm.S0[c & 1][w], kk, a, s0dst, lane);
+                    if (!o) continue;
 #pragma unroll
                     for (int jp = 0; jp < 4; ++jp) {
                         uint32_t b0[NIN][2], b1[NIN][2];
@@ -354,13 +321,12 @@ __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p
                     O[n][2] *= p.scale * eg.x;
                     O[n][3] *= p.scale * eg.y;
                 }
-                bar_sync(1, 128);  // both output warps' scores and both chain warps' W
-                const uint32_t wt = smem_addr(sm.W[w]) + lane * 16, pt = smem_addr(sm.P) + lane * 16;
+                bar_sync(1, 128);  // both chain warps' W
 #pragma unroll
                 for (int jb = 0; jb < 4; ++jb) {
                     uint32_t a[NX][4];
-#pragma unroll
-                    for (int pl = 0; pl < NX; ++pl) ldm(a[pl], wt + (jb * NX + pl) * 512);
+                    get_a<NX>(sm.W[w], jb, a, wdst, lane);
+                    if (!o) continue;
 #pragma unroll
                     for (int ib = jb; ib < 4; ++ib) {
                         uint32_t b0[NX][2], b1[NX][2];
@@ -440,17 +406,27 @@ __global__ void __launch_bounds__(256, 1) delta_chain_kernel(const DeltaParams p
             y.store(st.y, lt);
             v.store_float(st.v, st.s.live, lt);
             if (p.o.p) q.template store_planes<NIN>(st.q, st.s.live, lt);
+            bar_sync(3, 128);
+        };
+        auto scores = [&](int c, bool on) {  // row block per warp, from the tiles just stored
+            auto& st = sm.st[c % NST];
+            if (on && p.o.p)
+                score_rows<DP, NIN, NX>(st.P, smem_addr(st.q), smem_addr(st.k), st.s, p.scale, true, warp - 4, lane);
         };
         any_next = gates[0].any;
         issue(0);
         if (NST == 2) {
+            const bool on = any;
             store(0);
             issue(1);
+            scores(0, on);
         }
         __syncthreads();
         for (int c = 0; c < p.nc; ++c) {
+            const bool on = any && c + NST - 1 < p.nc;
             store(c + NST - 1);
             issue(c + NST);
+            scores(c + NST - 1, on);
             if (NST == 1) __syncthreads();
             __syncthreads();
         }
