@@ -511,19 +511,21 @@ int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc&
 }
 
 struct DeltaBytes {
-    size_t gates, Y, S0, W;  // the handover's parts
+    size_t gates, Y, P, S0, W;  // the handover's parts
 };
 DeltaBytes delta_bytes(const subq::DeltaParams& p, int dtype) {
     const size_t nx = dtype == SUBQ_FP32 ? 3 : 2, chunks = (size_t)p.B * p.H * p.nc;
     const size_t ncw = 2 * ((p.e + subq::kDeltaCols - 1) / subq::kDeltaCols), dp = p.d <= 64 ? 64 : 128;
-    return {align_up(chunks * sizeof(subq::DeltaGates)), align_up(chunks * nx * subq::kYBlocks * 512), align_up(chunks * ncw * (dp / 16) * nx * 512),
+    const size_t mat = align_up(chunks * nx * subq::kYBlocks * 512);
+    return {align_up(chunks * sizeof(subq::DeltaGates)), mat, mat, align_up(chunks * ncw * (dp / 16) * nx * 512),
             align_up(chunks * ncw * 4 * nx * 512)};
 }
 
 void delta_handover(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
     p.gates = static_cast<subq::DeltaGates*>(at);
     p.Y = static_cast<unsigned char*>(at) + n.gates;
-    p.S0 = p.Y + n.Y;
+    p.P = p.Y + n.Y;
+    p.S0 = p.P + n.P;
     p.W = p.S0 + n.S0;
 }
 
@@ -592,7 +594,7 @@ DeltaBwdBytes delta_bwd_bytes(const subq::DeltaParams& p, int dtype, bool handov
     n.dq = p.q.group > 1 ? align_up(tokens * p.d * 4) : 0;
     n.dk = p.k.group > 1 ? align_up(tokens * p.d * 4) : 0;
     n.dv = p.v.group > 1 ? align_up(tokens * p.e * 4) : 0;
-    n.total = n.fwd.S0 + n.fwd.W + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.gates + n.fwd.Y + n.fwd.S0 + n.fwd.W);
+    n.total = n.fwd.S0 + n.fwd.W + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.gates + n.fwd.Y + n.fwd.P + n.fwd.S0 + n.fwd.W);
     return n;
 }
 
@@ -602,7 +604,7 @@ size_t subq_delta_handover_bytes(const subq_delta_desc* d) {
     subq::DeltaParams p;
     if (!d || check_delta(*d, p) != SUBQ_OK || p.d > 128) return 0;
     const DeltaBytes n = delta_bytes(p, d->dtype);
-    return n.gates + n.Y + n.S0 + n.W;
+    return n.gates + n.Y + n.P + n.S0 + n.W;
 }
 
 size_t subq_delta_fwd_workspace_bytes(const subq_delta_fwd_args* a) {
@@ -610,7 +612,7 @@ size_t subq_delta_fwd_workspace_bytes(const subq_delta_fwd_args* a) {
     int path;
     if (fill_delta_fwd(a, p, path) != SUBQ_OK || path != SUBQ_PATH_CHUNKED || a->handover) return 0;
     const DeltaBytes n = delta_bytes(p, a->desc.dtype);
-    return n.gates + n.Y;
+    return n.gates + n.Y + n.P;
 }
 
 size_t subq_delta_bwd_workspace_bytes(const subq_delta_bwd_args* a) {
@@ -640,7 +642,7 @@ int subq_delta_fwd(const subq_delta_fwd_args* a) {
                 return fail(SUBQ_ERR_WORKSPACE, "handover must be 256-byte aligned");
             delta_handover(p, n, a->handover);
         } else {
-            if ((rc = check_workspace(a->workspace, a->workspace_bytes, n.gates + n.Y))) return rc;
+            if ((rc = check_workspace(a->workspace, a->workspace_bytes, n.gates + n.Y + n.P))) return rc;
             delta_handover(p, n, a->workspace);
             p.S0 = p.W = nullptr;  // not kept
         }

@@ -27,7 +27,7 @@ using namespace dl;
 template <typename T, int DP>
 struct RevSmem {
     static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
-    static constexpr int kStages = kIn > 1 && DP == 128 ? 1 : 2;
+    static constexpr int kStages = kIn == 1 ? 3 : DP == 64 ? 2 : 1;  // as in the forward's walk
     struct Stage {
         alignas(128) unsigned char k[kIn * 64 * DP * 2];
         alignas(128) unsigned char q[kIn * 64 * DP * 2];
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
 #pragma unroll
                         for (int pl = 0; pl < NX; ++pl) {
                             uint32_t r[4];
-                            ldm_t(r, yt + pl * (kYBlocks * 512) + tri(ib, jb) * 512);
+                            ldm(r, yt + pl * (kYBlocks * 512) + tri(ib, jb) * 512);
                             b0[pl][0] = r[0]; b0[pl][1] = r[2]; b1[pl][0] = r[1]; b1[pl][1] = r[3];
                         }
                         mma_planes<NX, NX, NX>(X[2 * jb], ra[ib], b0);
@@ -284,56 +284,94 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
     } else {  // ---------------------------------------------------------- loads
         const int lt = tid - 128;  // as in the forward's walk, from the last chunk to the first
         const Gates* gates = p.gates + bh * p.nc;
-        TileRegs<T, DP, 128> k, q;
-        TileRegs<T, kDeltaCols, 128> x;
-        ByteRegs<NX * kYBlocks * 512, 128> y;
-        ByteRegs<sizeof(Gates), 128> s;
-        int any = 0, any_next = 0;
-        auto issue = [&](int c) {
-            any = any_next;
-            any_next = c > 0 ? gates[c - 1].any : 0;
-            if (c < 0) return;
-            s.issue(gates + c, lt);
-            if (!any) return;
-            const int n0 = c * kDeltaC;
-            k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, lt);
-            q.issue(p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, lt);
-            x.issue(p.g, tensor_base(p.g, b, h), n0, c0, p.e, p.N, lt);
-            y.issue(p.Y + (bh * p.nc + c) * (NX * kYBlocks * 512), lt);
-        };
-        auto store = [&](int c) {
-            if (c < 0) return;
-            auto& st = sm.st[c % NST];
-            s.store(&st.s, lt);
-            bar_sync(3, 128);
-            if (!any) return;
-            k.template store_planes<NIN>(st.k, st.s.live, lt);
-            q.template store_planes<NIN>(st.q, st.s.live, lt);
-            x.template store_planes<NIN>(st.g, st.s.live, lt);
-            y.store(st.y, lt);
-            bar_sync(3, 128);
-        };
-        auto scores = [&](int c, bool on) {
-            auto& st = sm.st[c % NST];
-            if (on) score_rows<DP, NIN, NX>(st.P, smem_addr(st.q), smem_addr(st.k), st.s, p.scale, false, warp - 4, lane);
-        };
-        any_next = gates[p.nc - 1].any;
-        issue(p.nc - 1);
-        if (NST == 2) {
-            const bool on = any;
-            store(p.nc - 1);
-            issue(p.nc - 2);
-            scores(p.nc - 1, on);
-        }
-        __syncthreads();
-        for (int c = p.nc - 1; c >= 0; --c) {
-            const int next = c - (NST - 1);
-            const bool on = any && next >= 0;
-            store(next);
-            issue(c - NST);
-            if (on) scores(next, on);
-            if (NST == 1) __syncthreads();
+        const int64_t kb = tensor_base(p.k, b, h), qb = tensor_base(p.q, b, h), gb = tensor_base(p.g, b, h);
+        constexpr int kMat = NX * kYBlocks * 512;
+        const unsigned char* Y = p.Y + bh * p.nc * kMat;
+        const unsigned char* P = p.P + bh * p.nc * kMat;
+        if (NIN == 1 && p.k.vec && p.q.vec && p.g.vec && p.d % 8 == 0 && p.e % 8 == 0) {
+            int any_next = gates[p.nc - 1].any;
+            auto start = [&](int c) {
+                if (c >= 0) {
+                    const int any = any_next;
+                    any_next = c > 0 ? gates[c - 1].any : 0;
+                    auto& st = sm.st[c % NST];
+                    async16<128>(reinterpret_cast<unsigned char*>(&st.s), reinterpret_cast<const unsigned char*>(gates + c), sizeof(Gates), lt);
+                    if (any) {
+                        const int n0 = c * kDeltaC;
+                        async_tile<T, DP, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, lt);
+                        async_tile<T, DP, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, lt);
+                        async_tile<T, kDeltaCols, 128>(st.g, p.g, gb, n0, c0, p.e, p.N, lt);
+                        async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
+                        async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
+                    }
+                }
+                async_commit();
+            };
+            auto finish = [&](int c) {
+                async_wait_but_one();
+                if (c < 0) return;
+                bar_sync(3, 128);
+                auto& st = sm.st[c % NST];
+                if (st.s.any && !st.s.full) {
+                    clear_dead<DP, 128>(st.k, st.s.live, lt);
+                    clear_dead<DP, 128>(st.q, st.s.live, lt);
+                    clear_dead<kDeltaCols, 128>(st.g, st.s.live, lt);
+                }
+            };
+            start(p.nc - 1);
+            start(p.nc - 2);
+            finish(p.nc - 1);
             __syncthreads();
+            for (int c = p.nc - 1; c >= 0; --c) {
+                start(c - 2);
+                finish(c - 1);
+                __syncthreads();
+            }
+            async_wait();
+        } else {
+            TileRegs<T, DP, 128> k, q;
+            TileRegs<T, kDeltaCols, 128> x;
+            ByteRegs<kMat, 128> y, P_;
+            ByteRegs<sizeof(Gates), 128> s;
+            int any = 0, any_next = gates[p.nc - 1].any;
+            auto issue = [&](int c) {
+                any = any_next;
+                any_next = c > 0 ? gates[c - 1].any : 0;
+                if (c < 0) return;
+                s.issue(gates + c, lt);
+                if (!any) return;
+                const int n0 = c * kDeltaC;
+                k.issue(p.k, kb, n0, 0, p.d, p.N, lt);
+                q.issue(p.q, qb, n0, 0, p.d, p.N, lt);
+                x.issue(p.g, gb, n0, c0, p.e, p.N, lt);
+                y.issue(Y + (int64_t)c * kMat, lt);
+                P_.issue(P + (int64_t)c * kMat, lt);
+            };
+            auto store = [&](int c) {
+                if (c < 0) return;
+                auto& st = sm.st[c % NST];
+                s.store(&st.s, lt);
+                bar_sync(3, 128);
+                if (!any) return;
+                k.template store_planes<NIN>(st.k, st.s.live, lt);
+                q.template store_planes<NIN>(st.q, st.s.live, lt);
+                x.template store_planes<NIN>(st.g, st.s.live, lt);
+                y.store(st.y, lt);
+                P_.store(st.P, lt);
+            };
+            constexpr int kAhead = NST == 1 ? 0 : 1;
+            issue(p.nc - 1);
+            if (kAhead) {
+                store(p.nc - 1);
+                issue(p.nc - 2);
+            }
+            __syncthreads();
+            for (int c = p.nc - 1; c >= 0; --c) {
+                store(c - kAhead);
+                issue(c - kAhead - 1);
+                if (NST == 1) __syncthreads();
+                __syncthreads();
+            }
         }
     }
 }

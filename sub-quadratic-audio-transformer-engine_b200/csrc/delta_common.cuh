@@ -52,7 +52,8 @@ struct DeltaParams {
     const float* S_in;  // [B, H, d, e]
     float* S_out;
     struct DeltaGates* gates;  // [B * H][nc]
-    unsigned char* Y;   // [B * H][nc][NX][10 blocks of 512 bytes]
+    unsigned char* Y;   // Y^T: [B * H][nc][NX][10 blocks of 512 bytes]
+    unsigned char* P;   // scale G o (Q K^T), likewise
     unsigned char* S0;  // [B * H][nc][ep / 16][dp / 16][NX][512], or null (not stored)
     unsigned char* W;   // [B * H][nc][ep / 16][4][NX][512], or null
     // backward
@@ -81,7 +82,7 @@ struct alignas(16) DeltaGates {
     float kd[kDeltaC];               // e^{g_C - g}
     int live[kDeltaC];
     float eC;                        // e^{g_C}
-    int any;                         // a live token in the chunk
+    int any, full;                   // a live token in the chunk; all 64 live
 };
 static_assert(sizeof(DeltaGates) % 16 == 0 && sizeof(DeltaGates) <= 128 * 16, "one 16-byte piece per loading thread");
 
@@ -215,11 +216,18 @@ __device__ __forceinline__ int tri(int ib, int jb) { return (ib * (ib + 1) >> 1)
 // ---- gates of one chunk
 using Gates = DeltaGates;
 
+// 2^x to 2 units in the last place, denormal results as 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // G_ij for row i (its gh, gl) and columns j, j + 1; `keep`: the largest column that counts,
 // the others are 0 (their exponent may overflow, so they are selected away, not multiplied).
 __device__ __forceinline__ float2 gamma_pair(float gh, float gl, const Gates& s, int j, int keep) {
     const float2 h = *reinterpret_cast<const float2*>(&s.gh[j]), l = *reinterpret_cast<const float2*>(&s.gl[j]);
-    const float x = exp2f((gh - h.x) + (gl - l.x)), y = exp2f((gh - h.y) + (gl - l.y));
+    const float x = exp2_fast((gh - h.x) + (gl - l.x)), y = exp2_fast((gh - h.y) + (gl - l.y));
     return make_float2(j <= keep ? x : 0.f, j + 1 <= keep ? y : 0.f);
 }
 __device__ __forceinline__ float select0(bool on, float x) { return on ? x : 0.f; }
@@ -250,7 +258,7 @@ __device__ __forceinline__ void form_gates(Gates& s, const DeltaParams& p, int b
         if (lane >= o) run += up;
     }
     const double total = __shfl_sync(0xffffffffu, run, 31);
-    const int any = __any_sync(0xffffffffu, lv[0] | lv[1]);
+    const int any = __any_sync(0xffffffffu, lv[0] | lv[1]), full = __all_sync(0xffffffffu, lv[0] & lv[1]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const double gi = i ? run : run - g[1];
@@ -267,6 +275,7 @@ __device__ __forceinline__ void form_gates(Gates& s, const DeltaParams& p, int b
     if (lane == 0) {
         s.eC = expf((float)total);
         s.any = any;
+        s.full = full;
     }
 }
 
@@ -276,23 +285,28 @@ __device__ __forceinline__ void form_gates(Gates& s, const DeltaParams& p, int b
 // rows are zeroed there, whatever memory holds.
 template <typename T, int W, int NT>
 struct TileRegs {
-    static constexpr int kPieces = W / 8, kPer = 64 * kPieces / NT, kQ = sizeof(T) / 2;
+    static constexpr int kPieces = W / 8, kPer = 64 * kPieces / NT, kQ = sizeof(T) / 2, kRows = NT / kPieces;
     static_assert(64 * kPieces % NT == 0, "threads per tile");
     uint4 r[kPer][kQ];
 
     __device__ __forceinline__ void issue(const DeltaTensor& x, int64_t base, int n0, int c0, int width, int N, int tid) {
-        const T* src = static_cast<const T*>(x.p) + base;
+        const int c = c0 + tid % kPieces * 8, n1 = n0 + tid / kPieces;
+        const T* src = static_cast<const T*>(x.p) + base + n1 * x.sn + c;
+        if (x.vec && width % 8 == 0) {
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-            const int idx = tid + u * NT, n = n0 + idx / kPieces, c = c0 + idx % kPieces * 8;
-            const T* at = src + n * x.sn + c;
-            if (n < N && x.vec && c + 8 <= width) {
+            for (int u = 0; u < kPer; ++u) {
+                const bool in = n1 + u * kRows < N && c < width;
 #pragma unroll
-                for (int i = 0; i < kQ; ++i) r[u][i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
-            } else {
+                for (int i = 0; i < kQ; ++i)
+                    r[u][i] = in ? __ldg(reinterpret_cast<const uint4*>(src + u * kRows * x.sn) + i) : make_uint4(0, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
                 alignas(16) T t[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = n < N && c + i < width ? at[i] : from_f<T>(0.f);
+                for (int i = 0; i < 8; ++i)
+                    t[i] = n1 + u * kRows < N && c + i < width ? src[u * kRows * x.sn + i] : from_f<T>(0.f);
 #pragma unroll
                 for (int i = 0; i < kQ; ++i) r[u][i] = reinterpret_cast<const uint4*>(t)[i];
             }
@@ -342,25 +356,7 @@ struct TileRegs {
             }
         }
     }
-
-    // as float32 rows of kVPitch
-    __device__ __forceinline__ void store_float(float* tile, const int* live, int tid) const {
-#pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-            const int idx = tid + u * NT, row = idx / kPieces, piece = idx % kPieces;
-            const bool on = live[row] != 0;
-            float f[8];
-            values(u, f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = on ? f[i] : 0.f;
-            float4* dst = reinterpret_cast<float4*>(tile + row * (W + 4) + piece * 8);
-            dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-            dst[1] = make_float4(f[4], f[5], f[6], f[7]);
-        }
-    }
 };
-
-constexpr int kVPitch = 36;  // floats per row of a [64][32] float tile: rows two apart fall 8 banks apart
 
 // BYTES contiguous bytes (a multiple of 16) the same way.
 template <int BYTES, int NT>
@@ -386,6 +382,31 @@ __device__ __forceinline__ void async16(unsigned char* dst, const unsigned char*
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst + i)), "l"(src + i) : "memory");
 }
 __device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void async_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
+// A [64][W] tile of 16-bit elements straight to shared memory (one plane); rows from N and columns from `width`
+// (a multiple of 8) are zero, masked rows hold what memory holds (clear_dead removes it). Rows start on 16 bytes.
+template <typename T, int W, int NT>
+__device__ __forceinline__ void async_tile(unsigned char* tile, const DeltaTensor& x, int64_t base, int n0, int c0, int width, int N,
+                                           int tid) {
+    constexpr int kPieces = W / 8, kPer = 64 * kPieces / NT, kRows = NT / kPieces;
+    const int piece = tid % kPieces, row = tid / kPieces, c = c0 + piece * 8;
+    const T* src = static_cast<const T*>(x.p) + base + (n0 + row) * x.sn + c;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+        const bool in = n0 + row + u * kRows < N && c < width;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(tile + tile_off<W>(row + u * kRows, piece))),
+                     "l"(in ? src + u * kRows * x.sn : static_cast<const T*>(x.p)), "r"(in ? 16 : 0)
+                     : "memory");
+    }
+}
+template <int W, int NT>
+__device__ __forceinline__ void clear_dead(unsigned char* tile, const int* live, int tid) {
+    constexpr int kPieces = W / 8;
+    for (int i = tid; i < 64 * kPieces; i += NT)
+        if (!live[i / kPieces]) *reinterpret_cast<uint4*>(tile + tile_off<W>(i / kPieces, i % kPieces)) = make_uint4(0, 0, 0, 0);
+}
 
 template <int NT>
 __device__ __forceinline__ void copy16(unsigned char* dst, const unsigned char* src, int bytes, int tid) {
@@ -397,11 +418,10 @@ __device__ __forceinline__ int64_t tensor_base(const DeltaTensor& x, int b, int 
     return b * x.sb + (h / x.group) * x.sh;
 }
 
-// scale G o (Q K^T) (times beta_j with `with_beta`) for row block rb, as NX planes in `out`
+// scale G o (Q K^T) for row block rb, as NX planes in `out`
 // (10 lower triangular blocks per plane).
 template <int DP, int NIN, int NX>
-__device__ __forceinline__ void score_rows(unsigned char* out, uint32_t q, uint32_t k, const Gates& s, float scale, bool with_beta,
-                                           int rb, int lane) {
+__device__ __forceinline__ void score_rows(unsigned char* out, uint32_t q, uint32_t k, const Gates& s, float scale, int rb, int lane) {
     constexpr int kTile = 64 * DP * 2;
     float acc[8][4];
 #pragma unroll
@@ -437,17 +457,12 @@ __device__ __forceinline__ void score_rows(unsigned char* out, uint32_t q, uint3
 #pragma unroll
         for (int jh = 0; jh < 2; ++jh) {
             const int j = 16 * jb + 8 * jh + 2 * t;
-            float2 f = make_float2(scale, scale);
-            if (with_beta) {
-                const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]);
-                f = make_float2(scale * be.x, scale * be.y);
-            }
 #pragma unroll
             for (int ih = 0; ih < 2; ++ih) {
                 const float2 ga = gamma_pair(gh[ih], gl[ih], s, j, i0 + 8 * ih);
                 uint32_t r[NX];
-                split2<NX>(f.x * ga.x * select0(j <= i0 + 8 * ih, acc[2 * jb + jh][2 * ih]),
-                           f.y * ga.y * select0(j + 1 <= i0 + 8 * ih, acc[2 * jb + jh][2 * ih + 1]), r);
+                split2<NX>(scale * ga.x * select0(j <= i0 + 8 * ih, acc[2 * jb + jh][2 * ih]),
+                           scale * ga.y * select0(j + 1 <= i0 + 8 * ih, acc[2 * jb + jh][2 * ih + 1]), r);
 #pragma unroll
                 for (int pl = 0; pl < NX; ++pl)
                     *reinterpret_cast<uint32_t*>(blk + pl * (kYBlocks * 512) + (ih * 2 + jh) * 128) = r[pl];
@@ -462,19 +477,22 @@ __device__ __forceinline__ void put_acc(float4* at, const float (&c)[NB][4], int
 #pragma unroll
     for (int n = 0; n < NB; ++n) at[n * 32 + lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
 }
-// Blocks 2 kk, 2 kk + 1 of such a tile as the planes of an A operand, and to memory (`dst`, or null) as 8 x 8 matrices.
+// Blocks 2 kk, 2 kk + 1 of such a tile as the planes of an A operand, times per-column factors f0 and f1,
+// and without them to memory (`dst`, or null) as 8 x 8 matrices.
 template <int NX>
-__device__ __forceinline__ void get_a(const float4* at, int kk, uint32_t (&a)[NX][4], unsigned char* dst, int lane) {
+__device__ __forceinline__ void get_a(const float4* at, int kk, uint32_t (&a)[NX][4], unsigned char* dst, int lane,
+                                      float2 f0 = make_float2(1.f, 1.f), float2 f1 = make_float2(1.f, 1.f)) {
     const float4 x = at[2 * kk * 32 + lane], y = at[(2 * kk + 1) * 32 + lane];
     const float c0[4] = {x.x, x.y, x.z, x.w}, c1[4] = {y.x, y.y, y.z, y.w};
-    const float2 one = make_float2(1.f, 1.f);
-    to_a<NX>(c0, c1, one, one, a);
     if (dst) {
+        const float2 one = make_float2(1.f, 1.f);
+        to_a<NX>(c0, c1, one, one, a);
 #pragma unroll
         for (int pl = 0; pl < NX; ++pl)
 #pragma unroll
             for (int m = 0; m < 4; ++m) *reinterpret_cast<uint32_t*>(dst + (kk * NX + pl) * 512 + m * 128 + lane * 4) = a[pl][m];
     }
+    to_a<NX>(c0, c1, f0, f1, a);
 }
 
 }  // namespace dl
