@@ -14,9 +14,10 @@
 // symmetry of the recurrence: multiplying S_t by e^{x_t} only moves factors
 // between q_t, k_t and the gates, so g_i enters through q_i.dq_i and v_i.dv_i.
 // <G, S'> = e^{g_C} <G, S0> + sum_j k_j.(D beta W G^T)_j.
+#pragma once
+
 #include "delta_common.cuh"
 #include "delta_launch.h"
-#include "scan_launch.h"
 
 namespace subq {
 namespace {
@@ -27,25 +28,220 @@ using namespace dl;
 template <typename T, int DP>
 struct RevSmem {
     static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
-    static constexpr int kStages = kIn == 1 ? 3 : DP == 64 ? 2 : 1;  // as in the forward's walk
+    static constexpr int kStages = kIn == 1 ? (DP == 64 ? 3 : 2) : DP == 64 ? 2 : 1;  // as in the forward's walk
     struct Stage {
         alignas(128) unsigned char k[kIn * 64 * DP * 2];
         alignas(128) unsigned char q[kIn * 64 * DP * 2];
-        alignas(128) unsigned char y[kX * kYBlocks * 512];
         alignas(128) unsigned char g[kIn * 64 * kDeltaCols * 2];  // dO
-        alignas(128) unsigned char P[kX * kYBlocks * 512];        // scale G o (Q K^T)
+        alignas(128) unsigned char y[kX * kYBlocks * 512];
+        alignas(128) unsigned char P[kX * kYBlocks * 512];  // scale G o (Q K^T)
         Gates s;
     } st[kStages];
-    // float32 accumulators between a chain warp and the warp beside it
-    float4 e1[2][8 * 32];       // (P^T dO)^T
-    float4 e2[2][DP / 8 * 32];  // (scale (e^g Q)^T dO)^T
-    float4 G[2][DP / 8 * 32];
-    float4 Z[2][8 * 32];
+    // by pair of warps
+    alignas(16) unsigned char G[2][DP / 16][kX * 512];  // G^T, planes
+    alignas(16) unsigned char R[2][4][kX * 512];        // -(beta dU)^T, planes
+    float4 Z[2][8 * 32];                                // Z^T, float32
+    float4 e2[2][DP / 8 * 32];                          // (scale (e^g Q)^T dO)^T; before that, (P^T dO)^T of the same chunk
 };
 
+// One warp of a chain pair: half `A` of d of G^T in its accumulators; dU and Z of its token blocks.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kTile = 64 * DP * 2, kGTile = 64 * kDeltaCols * 2;
+__device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int col0, int lane) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = RevSmem<T, DP>::kStages;
+    constexpr int NH = DP / 16;
+    const int g = lane >> 2, t = lane & 3;
+    const Own own(A);
+    const float2 one = make_float2(1.f, 1.f);
+    float S[NH][4];  // G^T: 16 value columns x this half of d
+    const float* G_in = p.dS_out ? p.dS_out + bh * p.d * p.e : nullptr;
+#pragma unroll
+    for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
+            S[n][i] = (G_in && d < p.d && col < p.e) ? G_in[(int64_t)d * p.e + col] : 0.f;
+        }
+    auto put_state = [&]() {
+#pragma unroll
+        for (int kk = 0; kk < NH / 2; ++kk) {
+            uint32_t a[NX][4];
+            to_a<NX>(S[2 * kk], S[2 * kk + 1], one, one, a);
+            put_a<NX>(sm.G[pair][A * (NH / 2) + kk], a, lane);
+        }
+    };
+    put_state();
+    __syncthreads();
+    for (int c = p.nc - 1; c >= 0; --c) {
+        if (NST == 1) __syncthreads();
+        auto& st = sm.st[c % NST];
+        const Gates& s = st.s;
+        if (s.any) {
+            const uint32_t kt = smem_addr(st.k), yt = smem_addr(st.y) + lane * 16;
+            float X[4][4];  // (K G)^T, then dU^T, then Z^T: blocks 2 u + half of this warp's tokens
+            zero_acc<4>(X);
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                uint32_t a[NX][4];
+                get_a<NX>(a, sm.G[pair][kk], lane);
+                mma_rows<DP, NX, NIN, NX>(X[0], X[1], a, kt, 16 * own.b0, kk, lane);
+                mma_rows<DP, NX, NIN, NX>(X[2], X[3], a, kt, 16 * own.b1, kk, lane);
+            }
+            bar_sync(1, 256);  // P^T dO is there; G has been read
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {  // dU; -beta dU for both warps
+                const int tok = 16 * own.at(u) + 2 * t;
+                float2 be[2];
+#pragma unroll
+                for (int jh = 0; jh < 2; ++jh) {
+                    const float4 e1 = sm.e2[pair][(2 * own.at(u) + jh) * 32 + lane];
+                    const float2 kd = *reinterpret_cast<const float2*>(&s.kd[tok + 8 * jh]);
+                    be[jh] = *reinterpret_cast<const float2*>(&s.beta[tok + 8 * jh]);
+                    be[jh] = make_float2(-be[jh].x, -be[jh].y);
+                    float(&x)[4] = X[2 * u + jh];
+                    x[0] = fmaf(kd.x, x[0], e1.x);
+                    x[1] = fmaf(kd.y, x[1], e1.y);
+                    x[2] = fmaf(kd.x, x[2], e1.z);
+                    x[3] = fmaf(kd.y, x[3], e1.w);
+                }
+                uint32_t a[NX][4];
+                to_a<NX>(X[2 * u], X[2 * u + 1], be[0], be[1], a);
+                put_a<NX>(sm.R[pair][own.at(u)], a, lane);
+            }
+            bar_arrive(6 + pair, 128);  // P^T dO has been read: e2 may take its place
+            bar_sync(4 + pair, 64);
+#pragma unroll
+            for (int ib = 0; ib < 4; ++ib) {  // Z^T = dU^T - (beta dU)^T Y
+                if (ib < own.b0) continue;
+                uint32_t a[NX][4];
+                get_a<NX>(a, sm.R[pair][ib], lane);
+                mma_block<NX, NX, false>(X[0], X[1], a, yt + tri(ib, own.b0) * 512, kYBlocks * 512);
+                if (ib >= own.b1) mma_block<NX, NX, false>(X[2], X[3], a, yt + tri(ib, own.b1) * 512, kYBlocks * 512);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sm.Z[pair][(2 * own.at(x >> 1) + (x & 1)) * 32 + lane] = as_float4(X[x]);
+#pragma unroll
+            for (int n = 0; n < NH; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[n][i] *= s.eC;
+            bar_sync(2, 256);  // Z is there for the pair and the warps beside it; e2 is there
+#pragma unroll
+            for (int n = 0; n < NH; ++n) add_acc(S[n], sm.e2[pair][(A * NH + n) * 32 + lane]);
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {  // G0^T = e^{g_C} G^T + e2 - (e^g beta Z)^T K over this half of d
+                float z0[4], z1[4];
+                get_acc2(z0, z1, sm.Z[pair] + 2 * jb * 32, lane);
+                float2 f[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int j = 16 * jb + 8 * i + 2 * t;
+                    const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]), eg = *reinterpret_cast<const float2*>(&s.eg[j]);
+                    f[i] = make_float2(-be.x * eg.x, -be.y * eg.y);
+                }
+                uint32_t a[NX][4];
+                to_a<NX>(z0, z1, f[0], f[1], a);
+#pragma unroll
+                for (int np = 0; np < NH / 2; ++np)
+                    mma_cols<DP, NX, NIN, NX>(S[2 * np], S[2 * np + 1], a, kt, 16 * jb, A * (NH / 2) + np, lane);
+            }
+            put_state();
+        }
+        __syncthreads();
+    }
+    if (p.dS_in) {
+        float* G_out = p.dS_in + bh * p.d * p.e;
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
+                if (d < p.d && col < p.e) G_out[(int64_t)d * p.e + col] = S[n][i];
+            }
+    }
+}
+
+// One warp of the pair beside a chain pair: P^T dO for its token blocks, (e^g Q)^T dO for its half of d, and
+// its share of the planes of G and Z.
+template <typename T, int DP>
+__device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int cb, int lane) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kGTile = 64 * kDeltaCols * 2;
+    constexpr int NST = RevSmem<T, DP>::kStages, NH = DP / 16;
+    const int t = lane & 3, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    const Own own(A);
+    const float2 one = make_float2(1.f, 1.f);
+    __syncthreads();
+    for (int c = p.nc - 1; c >= 0; --c) {
+        if (NST == 1) __syncthreads();
+        auto& st = sm.st[c % NST];
+        const Gates& s = st.s;
+        if (s.any) {
+            const uint32_t qt = smem_addr(st.q), gt = smem_addr(st.g), pt = smem_addr(st.P) + lane * 16;
+            const int64_t cw = (bh * p.nc + c) * 2 * ncb + 2 * cb + pair;  // chunk and group of 16 columns
+            float E[4][4];
+            zero_acc<4>(E);
+#pragma unroll
+            for (int ib = 0; ib < 4; ++ib) {  // (P^T dO)^T
+                if (ib < own.b0) continue;
+                uint32_t a[NIN][4];  // dO^T: 16 value columns x 16 tokens
+#pragma unroll
+                for (int pl = 0; pl < NIN; ++pl) a_cols<kDeltaCols>(a[pl], gt + pl * kGTile, 16 * ib, pair, lane);
+                mma_block<NIN, NX, true>(E[0], E[1], a, pt + tri(ib, own.b0) * 512, kYBlocks * 512);
+                if (ib >= own.b1) mma_block<NIN, NX, true>(E[2], E[3], a, pt + tri(ib, own.b1) * 512, kYBlocks * 512);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sm.e2[pair][(2 * own.at(x >> 1) + (x & 1)) * 32 + lane] = as_float4(E[x]);
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                if (kk % 2 != A) continue;
+                uint32_t a[NX][4];
+                get_a<NX>(a, sm.G[pair][kk], lane);
+                store_matrices<NX>(p.dS + (cw * (DP / 16) + kk) * (NX * 512), a, lane);
+            }
+            bar_sync(1, 256);
+            float E2[NH][4];
+            zero_acc<NH>(E2);
+#pragma unroll
+            for (int ib = 0; ib < 4; ++ib) {
+                uint32_t r[NIN][4], a[NX][4];
+#pragma unroll
+                for (int pl = 0; pl < NIN; ++pl) a_cols<kDeltaCols>(r[pl], gt + pl * kGTile, 16 * ib, pair, lane);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {  // scale e^g dO, tokens 16 ib + 8 (m / 2) + 2 t, + 1
+                    float x = 0.f, y = 0.f;
+#pragma unroll
+                    for (int pl = 0; pl < NIN; ++pl) {
+                        const float2 u = unpack_bf16(r[pl][m]);
+                        x += u.x;
+                        y += u.y;
+                    }
+                    const float2 eg = *reinterpret_cast<const float2*>(&s.eg[16 * ib + 8 * (m >> 1) + 2 * t]);
+                    uint32_t q[NX];
+                    split2<NX>(x * (p.scale * eg.x), y * (p.scale * eg.y), q);
+#pragma unroll
+                    for (int pl = 0; pl < NX; ++pl) a[pl][m] = q[pl];
+                }
+#pragma unroll
+                for (int np = 0; np < NH / 2; ++np)
+                    mma_cols<DP, NX, NIN, NX>(E2[2 * np], E2[2 * np + 1], a, qt, 16 * ib, A * (NH / 2) + np, lane);
+            }
+            bar_sync(6 + pair, 128);
+            put_acc<NH>(sm.e2[pair] + A * NH * 32, E2, lane);
+            bar_sync(2, 256);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float z0[4], z1[4];
+                get_acc2(z0, z1, sm.Z[pair] + 2 * own.at(u) * 32, lane);
+                uint32_t a[NX][4];
+                to_a<NX>(z0, z1, one, one, a);
+                store_matrices<NX>(p.Z + (cw * 4 + own.at(u)) * (NX * 512), a, lane);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX;
     constexpr int NST = RevSmem<T, DP>::kStages;
     extern __shared__ __align__(128) unsigned char raw[];
     RevSmem<T, DP>& sm = *reinterpret_cast<RevSmem<T, DP>*>(raw);
@@ -53,242 +249,21 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
     const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
     const int64_t bh = blockIdx.x / ncb;
     const int cb = blockIdx.x % ncb, b = (int)(bh / p.H), h = (int)(bh % p.H), c0 = cb * kDeltaCols;
-    const int g = lane >> 2, t = lane & 3;
-
-    if (warp < 2) {  // ---------------------------------------------------- chain
-        float S[DP / 8][4];  // G^T: 16 value columns x d
-        const int col0 = c0 + 16 * warp;
-        const float* G_in = p.dS_out ? p.dS_out + bh * p.d * p.e : nullptr;
-#pragma unroll
-        for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = 8 * n + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
-                S[n][i] = (G_in && d < p.d && col < p.e) ? G_in[(int64_t)d * p.e + col] : 0.f;
-            }
-        bool pending = false;  // e2 of the chunk before has to be added
-        auto add_e2 = [&]() {
-            const float4* e2 = sm.e2[warp];
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-                const float4 x = e2[n * 32 + lane];
-                S[n][0] += x.x; S[n][1] += x.y; S[n][2] += x.z; S[n][3] += x.w;
-            }
-        };
-        __syncthreads();
-        for (int c = p.nc - 1; c >= 0; --c) {
-            if (NST == 1) __syncthreads();
-            auto& st = sm.st[c % NST];
-            const Gates& s = st.s;
-            if (pending) add_e2();
-            pending = s.any;
-            if (s.any) {
-                const uint32_t kt = smem_addr(st.k);
-                put_acc<DP / 8>(sm.G[warp], S, lane);
-                float X[8][4];
-#pragma unroll
-                for (int n = 0; n < 8; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) X[n][i] = 0.f;
-                const float2 one = make_float2(1.f, 1.f);
-#pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk) {  // (K G)^T
-                    uint32_t a[NX][4];
-                    to_a<NX>(S[2 * kk], S[2 * kk + 1], one, one, a);
-#pragma unroll
-                    for (int jp = 0; jp < 4; ++jp) {
-                        uint32_t b0[NIN][2], b1[NIN][2];
-#pragma unroll
-                        for (int pl = 0; pl < NIN; ++pl) {
-                            uint32_t r[4];
-                            b_rows<DP>(r, kt + pl * kTile, 16 * jp, kk, lane);
-                            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                        }
-                        mma_planes<NX, NIN, NX>(X[2 * jp], a, b0);
-                        mma_planes<NX, NIN, NX>(X[2 * jp + 1], a, b1);
-                    }
-                }
-                bar_sync(1, 128);  // e1 and G are there, e2 and Z of the chunk before have been read
-                const float4* e1 = sm.e1[warp];
-#pragma unroll
-                for (int n = 0; n < 8; ++n) {  // dU^T
-                    const float4 x = e1[n * 32 + lane];
-                    const float2 kd = *reinterpret_cast<const float2*>(&s.kd[8 * n + 2 * t]);
-                    X[n][0] = fmaf(kd.x, X[n][0], x.x);
-                    X[n][1] = fmaf(kd.y, X[n][1], x.y);
-                    X[n][2] = fmaf(kd.x, X[n][2], x.z);
-                    X[n][3] = fmaf(kd.y, X[n][3], x.w);
-                }
-                uint32_t ra[4][NX][4];
-#pragma unroll
-                for (int ib = 0; ib < 4; ++ib) {
-                    const float2 b0 = *reinterpret_cast<const float2*>(&s.beta[16 * ib + 2 * t]);
-                    const float2 b1 = *reinterpret_cast<const float2*>(&s.beta[16 * ib + 8 + 2 * t]);
-                    to_a<NX>(X[2 * ib], X[2 * ib + 1], make_float2(-b0.x, -b0.y), make_float2(-b1.x, -b1.y), ra[ib]);
-                }
-                // Z^T = dU^T - (beta dU)^T Y
-                const uint32_t yt = smem_addr(st.y) + lane * 16;
-#pragma unroll
-                for (int jb = 0; jb < 4; ++jb)
-#pragma unroll
-                    for (int ib = jb; ib < 4; ++ib) {
-                        uint32_t b0[NX][2], b1[NX][2];
-#pragma unroll
-                        for (int pl = 0; pl < NX; ++pl) {
-                            uint32_t r[4];
-                            ldm(r, yt + pl * (kYBlocks * 512) + tri(ib, jb) * 512);
-                            b0[pl][0] = r[0]; b0[pl][1] = r[2]; b1[pl][0] = r[1]; b1[pl][1] = r[3];
-                        }
-                        mma_planes<NX, NX, NX>(X[2 * jb], ra[ib], b0);
-                        mma_planes<NX, NX, NX>(X[2 * jb + 1], ra[ib], b1);
-                    }
-                put_acc<8>(sm.Z[warp], X, lane);
-#pragma unroll
-                for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) S[n][i] *= s.eC;
-#pragma unroll
-                for (int jb = 0; jb < 4; ++jb) {
-                    uint32_t a[NX][4];
-                    float2 f[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int j = 16 * jb + 8 * i + 2 * t;
-                        f[i] = make_float2(-s.beta[j] * s.eg[j], -s.beta[j + 1] * s.eg[j + 1]);
-                    }
-                    to_a<NX>(X[2 * jb], X[2 * jb + 1], f[0], f[1], a);
-#pragma unroll
-                    for (int np = 0; np < DP / 16; ++np) {
-                        uint32_t b0[NIN][2], b1[NIN][2];
-#pragma unroll
-                        for (int pl = 0; pl < NIN; ++pl) {
-                            uint32_t r[4];
-                            b_cols<DP>(r, kt + pl * kTile, 16 * jb, np, lane);
-                            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                        }
-                        mma_planes<NX, NIN, NX>(S[2 * np], a, b0);
-                        mma_planes<NX, NIN, NX>(S[2 * np + 1], a, b1);
-                    }
-                }
-            }
-            __syncthreads();
-        }
-        if (pending) add_e2();
-        if (p.dS_in) {
-            float* G_out = p.dS_in + bh * p.d * p.e;
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = 8 * n + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
-                    if (d < p.d && col < p.e) G_out[(int64_t)d * p.e + col] = S[n][i];
-                }
-        }
-    } else if (warp < 4) {  // ------------------------------- P^T dO, (e^g Q)^T dO, planes of G and Z
-        const int w = warp - 2;
-        auto planes = [&](unsigned char* base, int c, int tiles) {  // of this warp's 16 columns
-            return base + ((bh * p.nc + c) * 2 * ncb + 2 * cb + w) * (tiles * NX * 512);
-        };
-        int last = -1;  // the chunk whose Z waits in shared memory
-        auto flush_z = [&]() {
-            if (last < 0) return;
-            unsigned char* dst = planes(p.Z, last, 4);
-#pragma unroll
-            for (int jb = 0; jb < 4; ++jb) {
-                uint32_t a[NX][4];
-                get_a<NX>(sm.Z[w], jb, a, dst, lane);
-            }
-            last = -1;
-        };
-        __syncthreads();
-        for (int c = p.nc - 1; c >= 0; --c) {
-            if (NST == 1) __syncthreads();
-            auto& st = sm.st[c % NST];
-            const Gates& s = st.s;
-            flush_z();
-            if (s.any) {
-                const uint32_t qt = smem_addr(st.q), gt = smem_addr(st.g), pt = smem_addr(st.P) + lane * 16;
-                uint32_t da[4][NIN][4];  // dO^T: 16 value columns x 64 tokens
-#pragma unroll
-                for (int ib = 0; ib < 4; ++ib)
-#pragma unroll
-                    for (int pl = 0; pl < NIN; ++pl) a_cols<kDeltaCols>(da[ib][pl], gt + pl * kGTile, 16 * ib, w, lane);
-                float4* e1 = sm.e1[w];
-#pragma unroll
-                for (int jb = 0; jb < 4; ++jb) {
-                    float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int ib = jb; ib < 4; ++ib) {
-                        uint32_t b0[NX][2], b1[NX][2];
-#pragma unroll
-                        for (int pl = 0; pl < NX; ++pl) {
-                            uint32_t r[4];
-                            ldm_t(r, pt + pl * (kYBlocks * 512) + tri(ib, jb) * 512);
-                            b0[pl][0] = r[0]; b0[pl][1] = r[2]; b1[pl][0] = r[1]; b1[pl][1] = r[3];
-                        }
-                        mma_planes<NIN, NX, NX>(a0, da[ib], b0);
-                        mma_planes<NIN, NX, NX>(a1, da[ib], b1);
-                    }
-                    e1[(2 * jb) * 32 + lane] = make_float4(a0[0], a0[1], a0[2], a0[3]);
-                    e1[(2 * jb + 1) * 32 + lane] = make_float4(a1[0], a1[1], a1[2], a1[3]);
-                }
-                bar_sync(1, 128);
-                last = c;
-                unsigned char* gdst = planes(p.dS, c, DP / 16);
-#pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk) {
-                    uint32_t a[NX][4];
-                    get_a<NX>(sm.G[w], kk, a, gdst, lane);
-                }
-                float E[DP / 8][4];
-#pragma unroll
-                for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) E[n][i] = 0.f;
-#pragma unroll
-                for (int ib = 0; ib < 4; ++ib) {
-                    uint32_t a[NX][4];
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) {  // scale e^g dO, tokens 16 ib + 8 (m / 2) + 2 t, + 1
-                        float x = 0.f, y = 0.f;
-#pragma unroll
-                        for (int pl = 0; pl < NIN; ++pl) {
-                            const float2 u = unpack_bf16(da[ib][pl][m]);
-                            x += u.x;
-                            y += u.y;
-                        }
-                        const int i = 16 * ib + 8 * (m >> 1) + 2 * t;
-                        uint32_t r[NX];
-                        split2<NX>(x * p.scale * s.eg[i], y * p.scale * s.eg[i + 1], r);
-#pragma unroll
-                        for (int pl = 0; pl < NX; ++pl) a[pl][m] = r[pl];
-                    }
-#pragma unroll
-                    for (int np = 0; np < DP / 16; ++np) {
-                        uint32_t b0[NIN][2], b1[NIN][2];
-#pragma unroll
-                        for (int pl = 0; pl < NIN; ++pl) {
-                            uint32_t r[4];
-                            b_cols<DP>(r, qt + pl * kTile, 16 * ib, np, lane);
-                            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                        }
-                        mma_planes<NX, NIN, NX>(E[2 * np], a, b0);
-                        mma_planes<NX, NIN, NX>(E[2 * np + 1], a, b1);
-                    }
-                }
-                put_acc<DP / 8>(sm.e2[w], E, lane);
-            }
-            __syncthreads();
-        }
-        flush_z();
+    if (warp < 4) {
+        rev_chain_warp<T, DP>(sm, p, warp & 1, warp >> 1, bh, c0 + 16 * (warp >> 1), lane);
+    } else if (warp < 8) {
+        rev_side_warp<T, DP>(sm, p, warp & 1, (warp >> 1) & 1, bh, cb, lane);
     } else {  // ---------------------------------------------------------- loads
-        const int lt = tid - 128;  // as in the forward's walk, from the last chunk to the first
+        const int lt = tid - 256;  // as in the forward's walk, from the last chunk to the first
         const Gates* gates = p.gates + bh * p.nc;
         const int64_t kb = tensor_base(p.k, b, h), qb = tensor_base(p.q, b, h), gb = tensor_base(p.g, b, h);
         constexpr int kMat = NX * kYBlocks * 512;
         const unsigned char* Y = p.Y + bh * p.nc * kMat;
         const unsigned char* P = p.P + bh * p.nc * kMat;
-        if (NIN == 1 && p.k.vec && p.q.vec && p.g.vec && p.d % 8 == 0 && p.e % 8 == 0) {
+        bool async = false;
+        if constexpr (NIN == 1) async = p.k.vec && p.q.vec && p.g.vec && p.d % 8 == 0 && p.e % 8 == 0;
+        if (async) {
+            constexpr int kAhead = NST - 1;
             int any_next = gates[p.nc - 1].any;
             auto start = [&](int c) {
                 if (c >= 0) {
@@ -308,7 +283,7 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                 async_commit();
             };
             auto finish = [&](int c) {
-                async_wait_but_one();
+                async_wait_but<(kAhead > 1 ? kAhead - 1 : 0)>();
                 if (c < 0) return;
                 bar_sync(3, 128);
                 auto& st = sm.st[c % NST];
@@ -318,59 +293,73 @@ __global__ void __launch_bounds__(256, 1) delta_rev_kernel(const DeltaParams p) 
                     clear_dead<kDeltaCols, 128>(st.g, st.s.live, lt);
                 }
             };
-            start(p.nc - 1);
-            start(p.nc - 2);
+            for (int i = 1; i <= kAhead; ++i) start(p.nc - i);
             finish(p.nc - 1);
             __syncthreads();
             for (int c = p.nc - 1; c >= 0; --c) {
-                start(c - 2);
+                start(c - kAhead);
                 finish(c - 1);
                 __syncthreads();
             }
             async_wait();
         } else {
-            TileRegs<T, DP, 128> k, q;
-            TileRegs<T, kDeltaCols, 128> x;
-            ByteRegs<kMat, 128> y, P_;
-            ByteRegs<sizeof(Gates), 128> s;
-            int any = 0, any_next = gates[p.nc - 1].any;
-            auto issue = [&](int c) {
-                any = any_next;
-                any_next = c > 0 ? gates[c - 1].any : 0;
-                if (c < 0) return;
-                s.issue(gates + c, lt);
-                if (!any) return;
-                const int n0 = c * kDeltaC;
-                k.issue(p.k, kb, n0, 0, p.d, p.N, lt);
-                q.issue(p.q, qb, n0, 0, p.d, p.N, lt);
-                x.issue(p.g, gb, n0, c0, p.e, p.N, lt);
-                y.issue(Y + (int64_t)c * kMat, lt);
-                P_.issue(P + (int64_t)c * kMat, lt);
-            };
-            auto store = [&](int c) {
-                if (c < 0) return;
-                auto& st = sm.st[c % NST];
-                s.store(&st.s, lt);
-                bar_sync(3, 128);
-                if (!any) return;
-                k.template store_planes<NIN>(st.k, st.s.live, lt);
-                q.template store_planes<NIN>(st.q, st.s.live, lt);
-                x.template store_planes<NIN>(st.g, st.s.live, lt);
-                y.store(st.y, lt);
-                P_.store(st.P, lt);
-            };
-            constexpr int kAhead = NST == 1 ? 0 : 1;
-            issue(p.nc - 1);
-            if (kAhead) {
+            if constexpr (NST == 1) {
+                __syncthreads();
+                for (int c = p.nc - 1; c >= 0; --c) {
+                    auto& st = sm.st[0];
+                    copy16<128>(reinterpret_cast<unsigned char*>(&st.s), reinterpret_cast<const unsigned char*>(gates + c), sizeof(Gates), lt);
+                    bar_sync(3, 128);
+                    if (st.s.any) {
+                        const int n0 = c * kDeltaC;
+                        load_tile<T, DP, NIN, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, st.s.live, lt);
+                        load_tile<T, DP, NIN, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, st.s.live, lt);
+                        load_tile<T, kDeltaCols, NIN, 128>(st.g, p.g, gb, n0, c0, p.e, p.N, st.s.live, lt);
+                        async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
+                        async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
+                        async_wait();
+                    }
+                    __syncthreads();
+                    __syncthreads();
+                }
+            } else {
+                TileRegs<T, DP, 128> k, q;
+                TileRegs<T, kDeltaCols, 128> x;
+                ByteRegs<sizeof(Gates), 128> s;
+                int any = 0, any_next = gates[p.nc - 1].any;
+                auto issue = [&](int c) {
+                    any = any_next;
+                    any_next = c > 0 ? gates[c - 1].any : 0;
+                    if (c < 0) return;
+                    s.issue(gates + c, lt);
+                    if (!any) return;
+                    const int n0 = c * kDeltaC;
+                    k.issue(p.k, kb, n0, 0, p.d, p.N, lt);
+                    q.issue(p.q, qb, n0, 0, p.d, p.N, lt);
+                    x.issue(p.g, gb, n0, c0, p.e, p.N, lt);
+                };
+                auto store = [&](int c) {
+                    if (c < 0) return;
+                    auto& st = sm.st[c % NST];
+                    s.store(&st.s, lt);
+                    bar_sync(3, 128);
+                    if (!any) return;
+                    async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
+                    async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
+                    k.template store_planes<NIN>(st.k, st.s.live, lt);
+                    q.template store_planes<NIN>(st.q, st.s.live, lt);
+                    x.template store_planes<NIN>(st.g, st.s.live, lt);
+                };
+                issue(p.nc - 1);
                 store(p.nc - 1);
                 issue(p.nc - 2);
-            }
-            __syncthreads();
-            for (int c = p.nc - 1; c >= 0; --c) {
-                store(c - kAhead);
-                issue(c - kAhead - 1);
-                if (NST == 1) __syncthreads();
+                async_wait();
                 __syncthreads();
+                for (int c = p.nc - 1; c >= 0; --c) {
+                    store(c - 1);
+                    issue(c - 2);
+                    async_wait();
+                    __syncthreads();
+                }
             }
         }
     }
@@ -843,7 +832,7 @@ cudaError_t bwd_t(const DeltaParams& p, cudaStream_t st, int* launches) {
     if (err == cudaSuccess)
         err = cudaFuncSetAttribute(delta_grad_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)grad);
     if (err != cudaSuccess) return err;
-    delta_rev_kernel<T, DP><<<(unsigned)(bh * ncb), 256, rev, st>>>(p);
+    delta_rev_kernel<T, DP><<<(unsigned)(bh * ncb), 384, rev, st>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     delta_grad_kernel<T, DP><<<(unsigned)(bh * p.nc), 256, grad, st>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
@@ -854,16 +843,4 @@ cudaError_t bwd_t(const DeltaParams& p, cudaStream_t st, int* launches) {
 }
 
 }  // namespace
-
-cudaError_t launch_delta_bwd(const DeltaParams& p, int dtype, cudaStream_t st, int* launches) {
-    if (p.d <= 64) {
-        if (dtype == SUBQ_BF16) return bwd_t<__nv_bfloat16, 64>(p, st, launches);
-        if (dtype == SUBQ_FP16) return bwd_t<__half, 64>(p, st, launches);
-        return bwd_t<float, 64>(p, st, launches);
-    }
-    if (dtype == SUBQ_BF16) return bwd_t<__nv_bfloat16, 128>(p, st, launches);
-    if (dtype == SUBQ_FP16) return bwd_t<__half, 128>(p, st, launches);
-    return bwd_t<float, 128>(p, st, launches);
-}
-
 }  // namespace subq

@@ -1,0 +1,10 @@
+// Backward of the gated delta rule for float16 inputs (delta_bwd.cuh).
+#include "delta_bwd.cuh"
+
+namespace subq {
+
+cudaError_t launch_delta_bwd_fp16(const DeltaParams& p, cudaStream_t st, int* launches) {
+    return p.d <= 64 ? bwd_t<__half, 64>(p, st, launches) : bwd_t<__half, 128>(p, st, launches);
+}
+
+}  // namespace subq

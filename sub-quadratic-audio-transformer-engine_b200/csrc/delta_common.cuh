@@ -358,6 +358,15 @@ struct TileRegs {
     }
 };
 
+// A tile loaded and stored at once, a few pieces at a time.
+template <typename T, int W, int NP, int NT>
+__device__ __forceinline__ void load_tile(unsigned char* tile, const DeltaTensor& x, int64_t base, int n0, int c0, int width, int N,
+                                          const int* live, int tid) {
+    TileRegs<T, W, NT> r;
+    r.issue(x, base, n0, c0, width, N, tid);
+    r.template store_planes<NP>(tile, live, tid);
+}
+
 // BYTES contiguous bytes (a multiple of 16) the same way.
 template <int BYTES, int NT>
 struct ByteRegs {
@@ -383,7 +392,11 @@ __device__ __forceinline__ void async16(unsigned char* dst, const unsigned char*
 }
 __device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void async_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+// All but the last N groups have arrived.
+template <int N>
+__device__ __forceinline__ void async_wait_but() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // A [64][W] tile of 16-bit elements straight to shared memory (one plane); rows from N and columns from `width`
 // (a multiple of 8) are zero, masked rows hold what memory holds (clear_dead removes it). Rows start on 16 bytes.
@@ -471,28 +484,107 @@ __device__ __forceinline__ void score_rows(unsigned char* out, uint32_t q, uint3
     }
 }
 
+// The two warps of a pair share a chunk's four blocks of 16 tokens so that both have half of a triangle's blocks:
+// warp 0 has blocks 0 and 3, warp 1 has 1 and 2. (One code for both: the blocks are run-time values, so that the
+// walks' loops stay small enough for the instruction cache.)
+struct Own {
+    int b0, b1;
+    __device__ explicit Own(int a) : b0(a ? 1 : 0), b1(a ? 2 : 3) {}
+    __device__ int at(int u) const { return u ? b1 : b0; }
+};
+
+template <int NB>
+__device__ __forceinline__ void zero_acc(float (&c)[NB][4]) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
+}
+__device__ __forceinline__ void add_acc(float (&c)[4], float4 x) {
+    c[0] += x.x; c[1] += x.y; c[2] += x.z; c[3] += x.w;
+}
+__device__ __forceinline__ float4 as_float4(const float (&c)[4]) { return make_float4(c[0], c[1], c[2], c[3]); }
+
 // An accumulator tile (NB blocks of 16 rows x 8 columns) through shared memory, 16 bytes per lane and block.
 template <int NB>
 __device__ __forceinline__ void put_acc(float4* at, const float (&c)[NB][4], int lane) {
 #pragma unroll
     for (int n = 0; n < NB; ++n) at[n * 32 + lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
 }
-// Blocks 2 kk, 2 kk + 1 of such a tile as the planes of an A operand, times per-column factors f0 and f1,
-// and without them to memory (`dst`, or null) as 8 x 8 matrices.
+// The planes of an A operand (16 x 16) through shared memory, 16 bytes per lane and plane.
 template <int NX>
-__device__ __forceinline__ void get_a(const float4* at, int kk, uint32_t (&a)[NX][4], unsigned char* dst, int lane,
-                                      float2 f0 = make_float2(1.f, 1.f), float2 f1 = make_float2(1.f, 1.f)) {
-    const float4 x = at[2 * kk * 32 + lane], y = at[(2 * kk + 1) * 32 + lane];
-    const float c0[4] = {x.x, x.y, x.z, x.w}, c1[4] = {y.x, y.y, y.z, y.w};
-    if (dst) {
-        const float2 one = make_float2(1.f, 1.f);
-        to_a<NX>(c0, c1, one, one, a);
+__device__ __forceinline__ void put_a(unsigned char* tile, const uint32_t (&a)[NX][4], int lane) {
 #pragma unroll
-        for (int pl = 0; pl < NX; ++pl)
+    for (int pl = 0; pl < NX; ++pl)
+        *reinterpret_cast<uint4*>(tile + pl * 512 + lane * 16) = make_uint4(a[pl][0], a[pl][1], a[pl][2], a[pl][3]);
+}
+template <int NX>
+__device__ __forceinline__ void get_a(uint32_t (&a)[NX][4], const unsigned char* tile, int lane) {
 #pragma unroll
-            for (int m = 0; m < 4; ++m) *reinterpret_cast<uint32_t*>(dst + (kk * NX + pl) * 512 + m * 128 + lane * 4) = a[pl][m];
+    for (int pl = 0; pl < NX; ++pl) {
+        const uint4 x = *reinterpret_cast<const uint4*>(tile + pl * 512 + lane * 16);
+        a[pl][0] = x.x; a[pl][1] = x.y; a[pl][2] = x.z; a[pl][3] = x.w;
     }
-    to_a<NX>(c0, c1, f0, f1, a);
+}
+// Two neighbouring float32 accumulator blocks from shared memory.
+__device__ __forceinline__ void get_acc2(float (&c0)[4], float (&c1)[4], const float4* at, int lane) {
+    const float4 x = at[lane], y = at[32 + lane];
+    c0[0] = x.x; c0[1] = x.y; c0[2] = x.z; c0[3] = x.w;
+    c1[0] = y.x; c1[1] = y.y; c1[2] = y.z; c1[3] = y.w;
+}
+// Products of one A operand with the 16 rows n0 .. of a tile (B[k][n] = tile[n][k]), k block kk.
+template <int W, int NA, int NB, int NX>
+__device__ __forceinline__ void mma_rows(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], uint32_t tile, int n0, int kk, int lane) {
+    uint32_t b0[NB][2], b1[NB][2];
+#pragma unroll
+    for (int pl = 0; pl < NB; ++pl) {
+        uint32_t r[4];
+        b_rows<W>(r, tile + pl * (64 * W * 2), n0, kk, lane);
+        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+    }
+    mma_planes<NA, NB, NX>(c0, a, b0);
+    mma_planes<NA, NB, NX>(c1, a, b1);
+}
+// B[k][n] = tile[k][n]: rows k0 .., columns 16 np ..
+template <int W, int NA, int NB, int NX>
+__device__ __forceinline__ void mma_cols(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], uint32_t tile, int k0, int np, int lane) {
+    uint32_t b0[NB][2], b1[NB][2];
+#pragma unroll
+    for (int pl = 0; pl < NB; ++pl) {
+        uint32_t r[4];
+        b_cols<W>(r, tile + pl * (64 * W * 2), k0, np, lane);
+        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+    }
+    mma_planes<NA, NB, NX>(c0, a, b0);
+    mma_planes<NA, NB, NX>(c1, a, b1);
+}
+// B = a 16 x 16 block M[r][c] kept as four 8 x 8 matrices (row half, column half) per plane, planes `pitch` bytes
+// apart; `block` is its address plus lane * 16. KROWS: B[k][n] = M[k][n], else B[k][n] = M[n][k].
+template <int NA, int NX, bool KROWS>
+__device__ __forceinline__ void mma_block(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], uint32_t block, int pitch) {
+    uint32_t b0[NX][2], b1[NX][2];
+#pragma unroll
+    for (int pl = 0; pl < NX; ++pl) {
+        uint32_t r[4];
+        if (KROWS) {
+            ldm_t(r, block + pl * pitch);
+            b0[pl][0] = r[0]; b0[pl][1] = r[2]; b1[pl][0] = r[1]; b1[pl][1] = r[3];
+        } else {
+            ldm(r, block + pl * pitch);
+            b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+        }
+    }
+    mma_planes<NA, NX, NX>(c0, a, b0);
+    mma_planes<NA, NX, NX>(c1, a, b1);
+}
+
+// Two neighbouring blocks as the planes of an A operand, to memory as four 8 x 8 matrices of 128 bytes per plane.
+template <int NX>
+__device__ __forceinline__ void store_matrices(unsigned char* dst, const uint32_t (&a)[NX][4], int lane) {
+#pragma unroll
+    for (int pl = 0; pl < NX; ++pl)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) *reinterpret_cast<uint32_t*>(dst + pl * 512 + m * 128 + lane * 4) = a[pl][m];
 }
 
 }  // namespace dl

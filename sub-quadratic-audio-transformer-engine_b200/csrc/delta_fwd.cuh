@@ -1,0 +1,598 @@
+// Chunked forward of the gated delta rule (see delta_common.cuh for the algebra).
+//
+// delta_prep_kernel: gates, Y and scores of every chunk, all chunks at once.
+// delta_chain_kernel: the walk over the chunks, bound by the latency of its
+// dependent products (K S0, Y (beta R), K^T W per chunk). All products are
+// transposed (rows = value columns, columns = tokens or d), so that a result is,
+// in its registers, the A operand of the next product. A pair of warps owns 16
+// value columns of one sequence: each warp forms R and W of two of the chunk's
+// four blocks of 16 tokens and updates half of d of the state, float32 in its
+// accumulators; the operands pass between the two through shared memory. Per
+// CTA, 32 columns: two such pairs; two pairs of output warps (Q S0 and score W
+// products; they also write the planes that the backward reads); and four warps
+// that load the next chunks. Each SM sub-partition has one warp of each kind.
+#pragma once
+
+#include "delta_common.cuh"
+#include "delta_launch.h"
+#include "scan_launch.h"
+
+namespace subq {
+namespace {
+
+using namespace dl;
+
+// ------------------------------------------------------------------ gates, Y and scores per chunk
+template <typename T, int DP>
+struct PrepSmem {
+    static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
+    Gates s;
+    alignas(16) float A[kDeltaC][kDeltaC + 4];
+    alignas(128) unsigned char Ab[6 * kX * 512];  // -A_IK beta, blocks I > K: [block][plane]
+    alignas(128) unsigned char Ti[4 * kX * 512];  // (I + A_II beta)^-1
+    alignas(128) unsigned char k[kIn * 64 * DP * 2];
+    alignas(128) unsigned char q[kIn * 64 * DP * 2];
+};
+
+// Y by 16 x 16 blocks. With T_I = (I + A_II beta)^-1 (forward substitution, a
+// column per lane), block column J of Y is one warp's:
+//   Y_JJ^T = A_JJ^T T_J^T,   Y_IJ^T = (A_IJ^T - sum_{J <= K < I} Y_KJ^T (A_IK beta)^T) T_I^T,
+// transposed so that each result is, in its registers, the A operand of the next product.
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kTile = 64 * DP * 2;
+    extern __shared__ __align__(128) unsigned char raw[];
+    PrepSmem<T, DP>& sm = *reinterpret_cast<PrepSmem<T, DP>*>(raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int64_t chunk = blockIdx.x;  // bh * nc + c
+    const int64_t bh = chunk / p.nc;
+    const int c = (int)(chunk % p.nc), b = (int)(bh / p.H), h = (int)(bh % p.H), n0 = c * kDeltaC;
+    {
+        TileRegs<T, DP, 128> k, q;
+        k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, tid);
+        if (p.P) q.issue(p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, tid);
+        if (warp == 0) form_gates(sm.s, p, b, h, n0, lane);
+        __syncthreads();
+        copy16<128>(reinterpret_cast<unsigned char*>(p.gates + chunk), reinterpret_cast<const unsigned char*>(&sm.s), sizeof(Gates), tid);
+        if (!sm.s.any) return;  // nothing else of a dead chunk is read
+        k.template store_planes<NIN>(sm.k, sm.s.live, tid);
+        if (p.P) q.template store_planes<NIN>(sm.q, sm.s.live, tid);
+    }
+    __syncthreads();
+    {  // A, rows 16 warp .. 16 warp + 15
+        float acc[8][4];
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+        const uint32_t k = smem_addr(sm.k);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+            uint32_t a[NIN][4];
+#pragma unroll
+            for (int pl = 0; pl < NIN; ++pl) a_rows<DP>(a[pl], k + pl * kTile, 16 * warp, kk, lane);
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb)
+                if (jb <= warp) {
+                    uint32_t b0[NIN][2], b1[NIN][2];
+#pragma unroll
+                    for (int pl = 0; pl < NIN; ++pl) {
+                        uint32_t r[4];
+                        b_rows<DP>(r, k + pl * kTile, 16 * jb, kk, lane);
+                        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                    }
+                    mma_planes<NIN, NIN, NX>(acc[2 * jb], a, b0);
+                    mma_planes<NIN, NIN, NX>(acc[2 * jb + 1], a, b1);
+                }
+        }
+#pragma unroll
+        for (int ih = 0; ih < 2; ++ih) {
+            const int i = 16 * warp + 8 * ih + g;
+            const float gh = sm.s.gh[i], gl = sm.s.gl[i];
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (n <= 2 * warp + 1) {
+                    const int j = 8 * n + 2 * t;
+                    const float2 ga = gamma_pair(gh, gl, sm.s, j, i - 1);
+                    const float x = ga.x * select0(j < i, acc[n][2 * ih]), y = ga.y * select0(j + 1 < i, acc[n][2 * ih + 1]);
+                    *reinterpret_cast<float2*>(&sm.A[i][j]) = make_float2(x, y);
+                    if (n < 2 * warp) {
+                        const float2 be = *reinterpret_cast<const float2*>(&sm.s.beta[j]);
+                        uint32_t r[NX];
+                        split2<NX>(-be.x * x, -be.y * y, r);
+                        unsigned char* at = sm.Ab + tri(warp - 1, n >> 1) * (NX * 512) + (ih * 2 + (n & 1)) * 128 + lane * 4;
+#pragma unroll
+                        for (int pl = 0; pl < NX; ++pl) *reinterpret_cast<uint32_t*>(at + pl * 512) = r[pl];
+                    }
+                }
+        }
+    }
+    // scores, the longest rows where A's were the shortest
+    if (p.P)
+        score_rows<DP, NIN, NX>(p.P + chunk * (NX * kYBlocks * 512), smem_addr(sm.q), smem_addr(sm.k), sm.s, p.scale, 3 - warp, lane);
+    __syncwarp();  // the diagonal block is this warp's own
+    {
+        const int col = lane & 15, r0 = 16 * warp;
+        float ti[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {  // T e_col: t_i = delta - sum_j A_ij beta_j t_j, kept as beta_j t_j
+            float x = i == col ? 1.f : 0.f, y = 0.f;
+#pragma unroll
+            for (int j = 0; j < i; j += 2) {
+                const float2 a = *reinterpret_cast<const float2*>(&sm.A[r0 + i][r0 + j]);
+                x = fmaf(-a.x, ti[j], x);
+                if (j + 1 < i) y = fmaf(-a.y, ti[j + 1], y);
+            }
+            x += y;
+            if (lane < 16) {
+                unsigned char* at = sm.Ti + warp * (NX * 512) + ((i >> 3) * 2 + (col >> 3)) * 128 + (i & 7) * 16 + (col & 7) * 2;
+                float rest = x;
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    const __nv_bfloat16 u = __float2bfloat16_rn(rest);
+                    *reinterpret_cast<__nv_bfloat16*>(at + pl * 512) = u;
+                    rest -= __bfloat162float(u);
+                }
+            }
+            ti[i] = sm.s.beta[r0 + i] * x;
+        }
+    }
+    __syncthreads();
+    {
+        const int J = warp;
+        uint32_t y[4][NX][4];  // Y_KJ^T, K = J + index
+        unsigned char* Y = p.Y + chunk * (NX * kYBlocks * 512);
+        const uint32_t ab = smem_addr(sm.Ab) + lane * 16, ti = smem_addr(sm.Ti) + lane * 16;
+        const float2 one = make_float2(1.f, 1.f);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int I = J + x;
+            if (I > 3) break;
+            float acc[2][4], out[2][4];
+#pragma unroll
+            for (int ih = 0; ih < 2; ++ih)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {  // A_IJ^T: rows j, columns i
+                    acc[ih][v] = sm.A[16 * I + 8 * ih + 2 * t + (v & 1)][16 * J + g + 8 * (v >> 1)];
+                    out[ih][v] = 0.f;
+                }
+#pragma unroll
+            for (int kx = 0; kx < x; ++kx) {
+                uint32_t b0[NX][2], b1[NX][2];
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    uint32_t r[4];
+                    ldm(r, ab + (tri(I - 1, J + kx) * NX + pl) * 512);
+                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                }
+                mma_planes<NX, NX, NX>(acc[0], y[kx], b0);
+                mma_planes<NX, NX, NX>(acc[1], y[kx], b1);
+            }
+            uint32_t a[NX][4], b0[NX][2], b1[NX][2];
+            to_a<NX>(acc[0], acc[1], one, one, a);
+#pragma unroll
+            for (int pl = 0; pl < NX; ++pl) {
+                uint32_t r[4];
+                ldm(r, ti + (I * NX + pl) * 512);
+                b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+            }
+            mma_planes<NX, NX, NX>(out[0], a, b0);
+            mma_planes<NX, NX, NX>(out[1], a, b1);
+            to_a<NX>(out[0], out[1], one, one, y[x]);
+#pragma unroll
+            for (int pl = 0; pl < NX; ++pl)
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+                    *reinterpret_cast<uint32_t*>(Y + (pl * kYBlocks + tri(I, J)) * 512 + ((m & 1) * 2 + (m >> 1)) * 128 + lane * 4) =
+                        y[x][pl][m];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ the walk
+template <typename T, int DP>
+struct ChainSmem {
+    static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
+    // chunks in shared memory: the one at work, the next, and one more on its way where that fits
+    static constexpr int kStages = kIn == 1 ? (DP == 64 ? 3 : 2) : DP == 64 ? 2 : 1;
+    struct Stage {
+        alignas(128) unsigned char k[kIn * 64 * DP * 2];
+        alignas(128) unsigned char q[kIn * 64 * DP * 2];
+        alignas(128) unsigned char v[kIn * 64 * kDeltaCols * 2];
+        alignas(128) unsigned char y[kX * kYBlocks * 512];
+        alignas(128) unsigned char P[kX * kYBlocks * 512];
+        Gates s;
+    } st[kStages];
+    // by pair of warps
+    alignas(16) unsigned char S0[2][DP / 16][kX * 512];  // S^T before the chunk, planes
+    alignas(16) unsigned char R[2][4][kX * 512];         // -(beta R)^T, planes
+    float4 W[2][8 * 32];                                 // W^T, float32
+    alignas(16) unsigned char out[4][32 * (16 * sizeof(T) + 16)];
+};
+
+// One warp of a chain pair: half `A` of d of S^T in its accumulators; R and W of its token blocks.
+template <typename T, int DP>
+__device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int col0, int lane) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP>::kStages;
+    constexpr int NH = DP / 16;  // 8-column blocks of half of d
+    const int g = lane >> 2, t = lane & 3;
+    const Own own(A);
+    const float2 one = make_float2(1.f, 1.f);
+    float S[NH][4];
+    const float* S_in = p.S_in ? p.S_in + bh * p.d * p.e : nullptr;
+#pragma unroll
+    for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
+            S[n][i] = (S_in && d < p.d && col < p.e) ? S_in[(int64_t)d * p.e + col] : 0.f;
+        }
+    auto put_state = [&]() {
+#pragma unroll
+        for (int kk = 0; kk < NH / 2; ++kk) {
+            uint32_t a[NX][4];
+            to_a<NX>(S[2 * kk], S[2 * kk + 1], one, one, a);
+            put_a<NX>(sm.S0[pair][A * (NH / 2) + kk], a, lane);
+        }
+    };
+    put_state();
+    __syncthreads();
+    for (int c = 0; c < p.nc; ++c) {
+        if (NST == 1) __syncthreads();  // the chunk is loaded
+        auto& st = sm.st[c % NST];
+        const Gates& s = st.s;
+        if (s.any) {
+            const uint32_t kt = smem_addr(st.k), vt = smem_addr(st.v), yt = smem_addr(st.y) + lane * 16;
+            float W[4][4];  // (K S0)^T, then R^T, then W^T: blocks 2 u + half of this warp's tokens
+            zero_acc<4>(W);
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                uint32_t a[NX][4];
+                get_a<NX>(a, sm.S0[pair][kk], lane);
+                mma_rows<DP, NX, NIN, NX>(W[0], W[1], a, kt, 16 * own.b0, kk, lane);
+                mma_rows<DP, NX, NIN, NX>(W[2], W[3], a, kt, 16 * own.b1, kk, lane);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {  // R = V - e^g K S0; -beta R for both warps
+                const int tok = 16 * own.at(u) + 2 * t;
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int pl = 0; pl < NIN; ++pl) {
+                    uint32_t r[4];
+                    a_cols<kDeltaCols>(r, vt + pl * (64 * kDeltaCols * 2), 16 * own.at(u), pair, lane);
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        const float2 x = unpack_bf16(r[m]);
+                        v[2 * m] += x.x;
+                        v[2 * m + 1] += x.y;
+                    }
+                }
+                float2 be[2];
+#pragma unroll
+                for (int jh = 0; jh < 2; ++jh) {
+                    const float2 eg = *reinterpret_cast<const float2*>(&s.eg[tok + 8 * jh]);
+                    be[jh] = *reinterpret_cast<const float2*>(&s.beta[tok + 8 * jh]);
+                    be[jh] = make_float2(-be[jh].x, -be[jh].y);
+                    float(&w)[4] = W[2 * u + jh];
+                    w[0] = fmaf(-eg.x, w[0], v[4 * jh]);
+                    w[1] = fmaf(-eg.y, w[1], v[4 * jh + 1]);
+                    w[2] = fmaf(-eg.x, w[2], v[4 * jh + 2]);
+                    w[3] = fmaf(-eg.y, w[3], v[4 * jh + 3]);
+                }
+                uint32_t a[NX][4];
+                to_a<NX>(W[2 * u], W[2 * u + 1], be[0], be[1], a);
+                put_a<NX>(sm.R[pair][own.at(u)], a, lane);
+            }
+            bar_sync(4 + pair, 64);
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {  // W^T = R^T - (beta R)^T Y^T
+                if (jb > own.b1) break;
+                uint32_t a[NX][4];
+                get_a<NX>(a, sm.R[pair][jb], lane);
+                mma_block<NX, NX, true>(W[2], W[3], a, yt + tri(own.b1, jb) * 512, kYBlocks * 512);
+                if (jb <= own.b0) mma_block<NX, NX, true>(W[0], W[1], a, yt + tri(own.b0, jb) * 512, kYBlocks * 512);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sm.W[pair][(2 * own.at(x >> 1) + (x & 1)) * 32 + lane] = as_float4(W[x]);
+#pragma unroll
+            for (int n = 0; n < NH; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[n][i] *= s.eC;
+            bar_sync(1, 256);  // W is there for both pairs and the output warps, which have read S0
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {  // S'^T = e^{g_C} S0^T + (e^{g_C - g} beta W)^T K over this half of d
+                float w0[4], w1[4];
+                get_acc2(w0, w1, sm.W[pair] + 2 * jb * 32, lane);
+                float2 f[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int j = 16 * jb + 8 * i + 2 * t;
+                    const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]), kd = *reinterpret_cast<const float2*>(&s.kd[j]);
+                    f[i] = make_float2(be.x * kd.x, be.y * kd.y);
+                }
+                uint32_t a[NX][4];
+                to_a<NX>(w0, w1, f[0], f[1], a);
+#pragma unroll
+                for (int np = 0; np < NH / 2; ++np)
+                    mma_cols<DP, NX, NIN, NX>(S[2 * np], S[2 * np + 1], a, kt, 16 * jb, A * (NH / 2) + np, lane);
+            }
+            put_state();
+        }
+        __syncthreads();
+    }
+    if (p.S_out) {
+        float* S_out = p.S_out + bh * p.d * p.e;
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
+                if (d < p.d && col < p.e) S_out[(int64_t)d * p.e + col] = S[n][i];
+            }
+    }
+}
+
+// One warp of an output pair: the outputs of 16 columns for its token blocks, and its share of the planes.
+template <typename T, int DP, bool OUT, bool KEEP>
+__device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int cb, int lane) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP>::kStages;
+    const int g = lane >> 2, t = lane & 3;
+    const Own own(A);
+    const float2 one = make_float2(1.f, 1.f);
+    const int b = (int)(bh / p.H), h = (int)(bh % p.H), ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    T* o = OUT ? static_cast<T*>(p.o.p) + tensor_base(p.o, b, h) : nullptr;
+    constexpr int kPitch = 16 * sizeof(T) + 16, kPieces = 16 * sizeof(T) / 16;  // bytes of a staged row, its 16-byte pieces
+    const int col0 = cb * kDeltaCols + 16 * pair, width = min(16, p.e - col0);
+    const bool whole = OUT && p.o.vec && width == 16;
+    unsigned char* stage = sm.out[2 * pair + A];
+    __syncthreads();
+    for (int c = 0; c < p.nc; ++c) {
+        if (NST == 1) __syncthreads();
+        auto& st = sm.st[c % NST];
+        const Gates& s = st.s;
+        const int n0 = c * kDeltaC;
+        if (s.any) {
+            const uint32_t qt = smem_addr(st.q), pt = smem_addr(st.P) + lane * 16;
+            const int64_t cw = (bh * p.nc + c) * 2 * ncb + 2 * cb + pair;  // chunk and group of 16 columns
+            float O[4][4];  // blocks 2 u + half
+            zero_acc<4>(O);
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {  // (Q S0)^T
+                uint32_t a[NX][4];
+                get_a<NX>(a, sm.S0[pair][kk], lane);
+                if (KEEP && kk % 2 == A) store_matrices<NX>(p.S0 + (cw * (DP / 16) + kk) * (NX * 512), a, lane);
+                if (OUT) {
+                    mma_rows<DP, NX, NIN, NX>(O[0], O[1], a, qt, 16 * own.b0, kk, lane);
+                    mma_rows<DP, NX, NIN, NX>(O[2], O[3], a, qt, 16 * own.b1, kk, lane);
+                }
+            }
+            if (OUT)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const float2 eg = *reinterpret_cast<const float2*>(&s.eg[16 * own.at(n >> 1) + 8 * (n & 1) + 2 * t]);
+                    O[n][0] *= p.scale * eg.x;
+                    O[n][1] *= p.scale * eg.y;
+                    O[n][2] *= p.scale * eg.x;
+                    O[n][3] *= p.scale * eg.y;
+                }
+            bar_sync(1, 256);
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {
+                const bool mine = jb == own.b0 || jb == own.b1;
+                if (OUT ? jb > own.b1 : !mine) continue;
+                float w0[4], w1[4];
+                get_acc2(w0, w1, sm.W[pair] + 2 * jb * 32, lane);
+                uint32_t a[NX][4];
+                if (KEEP && mine) {
+                    to_a<NX>(w0, w1, one, one, a);
+                    store_matrices<NX>(p.W + (cw * 4 + jb) * (NX * 512), a, lane);
+                }
+                if (OUT) {
+                    to_a<NX>(w0, w1, *reinterpret_cast<const float2*>(&s.beta[16 * jb + 2 * t]),
+                             *reinterpret_cast<const float2*>(&s.beta[16 * jb + 8 + 2 * t]), a);
+                    mma_block<NX, NX, false>(O[2], O[3], a, pt + tri(own.b1, jb) * 512, kYBlocks * 512);
+                    if (jb <= own.b0) mma_block<NX, NX, false>(O[0], O[1], a, pt + tri(own.b0, jb) * 512, kYBlocks * 512);
+                }
+            }
+            if (OUT) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {  // staged rows: 16 u + 8 half + ..
+                    T* r0 = reinterpret_cast<T*>(stage + (8 * n + 2 * t) * kPitch);
+                    T* r1 = reinterpret_cast<T*>(stage + (8 * n + 2 * t + 1) * kPitch);
+                    r0[g] = from_f<T>(O[n][0]);
+                    r1[g] = from_f<T>(O[n][1]);
+                    r0[g + 8] = from_f<T>(O[n][2]);
+                    r1[g + 8] = from_f<T>(O[n][3]);
+                }
+                __syncwarp();
+            }
+        }
+        if (OUT) {
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x) {
+                const int i = lane + 32 * x, row = i / kPieces, piece = i % kPieces;
+                const int tok = 16 * own.at(row >> 4) + (row & 15);
+                if (n0 + tok >= p.N) continue;
+                T* dst = o + (n0 + tok) * p.o.sn + col0;
+                const bool live = s.any && s.live[tok];
+                const unsigned char* src = stage + row * kPitch + piece * 16;
+                if (whole) {
+                    reinterpret_cast<uint4*>(dst)[piece] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+                } else {
+                    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+                    for (int y = 0; y < kPer; ++y)
+                        if (piece * kPer + y < width)
+                            dst[piece * kPer + y] = live ? reinterpret_cast<const T*>(src)[y] : from_f<T>(0.f);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// OUT: writes o. KEEP: writes the planes of S0 and W that the backward reads.
+template <typename T, int DP, bool OUT, bool KEEP>
+__global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX;
+    constexpr int NST = ChainSmem<T, DP>::kStages;
+    extern __shared__ __align__(128) unsigned char raw[];
+    ChainSmem<T, DP>& sm = *reinterpret_cast<ChainSmem<T, DP>*>(raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    const int64_t bh = blockIdx.x / ncb;
+    const int cb = blockIdx.x % ncb, b = (int)(bh / p.H), h = (int)(bh % p.H), c0 = cb * kDeltaCols;
+    if (warp < 4) {
+        chain_warp<T, DP>(sm, p, warp & 1, warp >> 1, bh, c0 + 16 * (warp >> 1), lane);
+    } else if (warp < 8) {
+        output_warp<T, DP, OUT, KEEP>(sm, p, warp & 1, (warp >> 1) & 1, bh, cb, lane);
+    } else {  // ---------------------------------------------------------- loads
+        // the loads of a chunk are in flight for a whole iteration or two
+        const int lt = tid - 256;
+        const Gates* gates = p.gates + bh * p.nc;
+        const int64_t kb = tensor_base(p.k, b, h), qb = tensor_base(p.q, b, h), vb = tensor_base(p.v, b, h);
+        constexpr int kMat = NX * kYBlocks * 512;
+        const unsigned char* Y = p.Y + bh * p.nc * kMat;
+        const unsigned char* P = p.P + bh * p.nc * kMat;
+        bool async = false;
+        if constexpr (NIN == 1) async = p.k.vec && p.q.vec && p.v.vec && p.d % 8 == 0 && p.e % 8 == 0;
+        if (async) {
+            // bf16: asynchronous copies, chunk c + kAhead started while c is computed
+            constexpr int kAhead = NST - 1;
+            int any_next = gates[0].any;
+            auto start = [&](int c) {
+                if (c < p.nc) {
+                    const int any = any_next;
+                    any_next = c + 1 < p.nc ? gates[c + 1].any : 0;
+                    auto& st = sm.st[c % NST];
+                    async16<128>(reinterpret_cast<unsigned char*>(&st.s), reinterpret_cast<const unsigned char*>(gates + c), sizeof(Gates), lt);
+                    if (any) {
+                        const int n0 = c * kDeltaC;
+                        async_tile<T, DP, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, lt);
+                        async_tile<T, kDeltaCols, 128>(st.v, p.v, vb, n0, c0, p.e, p.N, lt);
+                        async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
+                        if (OUT) {
+                            async_tile<T, DP, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, lt);
+                            async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
+                        }
+                    }
+                }
+                async_commit();
+            };
+            auto finish = [&](int c) {  // every copy up to chunk c's is there
+                async_wait_but<(kAhead > 1 ? kAhead - 1 : 0)>();
+                if (c >= p.nc) return;
+                bar_sync(3, 128);
+                auto& st = sm.st[c % NST];
+                if (st.s.any && !st.s.full) {
+                    clear_dead<DP, 128>(st.k, st.s.live, lt);
+                    if (OUT) clear_dead<DP, 128>(st.q, st.s.live, lt);
+                    clear_dead<kDeltaCols, 128>(st.v, st.s.live, lt);
+                }
+            };
+            for (int c = 0; c < kAhead; ++c) start(c);
+            finish(0);
+            __syncthreads();
+            for (int c = 0; c < p.nc; ++c) {
+                start(c + kAhead);
+                finish(c + 1);
+                __syncthreads();
+            }
+            async_wait();
+        } else {
+            if constexpr (NST == 1) {  // (no room for a second chunk: each tile is loaded when its turn comes)
+                __syncthreads();
+                for (int c = 0; c < p.nc; ++c) {
+                    auto& st = sm.st[0];
+                    copy16<128>(reinterpret_cast<unsigned char*>(&st.s), reinterpret_cast<const unsigned char*>(gates + c), sizeof(Gates), lt);
+                    bar_sync(3, 128);
+                    if (st.s.any) {
+                        const int n0 = c * kDeltaC;
+                        load_tile<T, DP, NIN, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, st.s.live, lt);
+                        load_tile<T, kDeltaCols, NIN, 128>(st.v, p.v, vb, n0, c0, p.e, p.N, st.s.live, lt);
+                        async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
+                        if (OUT) {
+                            load_tile<T, DP, NIN, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, st.s.live, lt);
+                            async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
+                        }
+                        async_wait();
+                    }
+                    __syncthreads();
+                    __syncthreads();
+                }
+            } else {
+                TileRegs<T, DP, 128> k, q;
+                TileRegs<T, kDeltaCols, 128> v;
+                ByteRegs<sizeof(Gates), 128> s;
+                int any = 0, any_next = gates[0].any;  // of the chunk in the registers, and of the one after it
+                auto issue = [&](int c) {
+                    any = any_next;
+                    any_next = c + 1 < p.nc ? gates[c + 1].any : 0;
+                    if (c >= p.nc) return;
+                    s.issue(gates + c, lt);
+                    if (!any) return;
+                    const int n0 = c * kDeltaC;
+                    k.issue(p.k, kb, n0, 0, p.d, p.N, lt);
+                    v.issue(p.v, vb, n0, c0, p.e, p.N, lt);
+                    if (OUT) {
+                        q.issue(p.q, qb, n0, 0, p.d, p.N, lt);
+                    }
+                };
+                auto store = [&](int c) {
+                    if (c >= p.nc) return;
+                    auto& st = sm.st[c % NST];
+                    s.store(&st.s, lt);
+                    bar_sync(3, 128);
+                    if (!any) return;
+                    async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
+                    if (OUT) async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
+                    k.template store_planes<NIN>(st.k, st.s.live, lt);
+                    v.template store_planes<NIN>(st.v, st.s.live, lt);
+                    if (OUT) {
+                        q.template store_planes<NIN>(st.q, st.s.live, lt);
+                    }
+                };
+                issue(0);
+                store(0);
+                issue(1);
+                async_wait();
+                __syncthreads();
+                for (int c = 0; c < p.nc; ++c) {
+                    store(c + 1);
+                    issue(c + 2);
+                    async_wait();
+                    __syncthreads();
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int DP>
+cudaError_t chain_t(const DeltaParams& p, unsigned blocks, cudaStream_t st) {
+    const size_t smem = sizeof(ChainSmem<T, DP>);
+    static_assert(sizeof(ChainSmem<T, DP>) <= 227 * 1024, "shared memory");
+    auto run = [&](auto kernel) {
+        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return err;
+        kernel<<<blocks, 384, smem, st>>>(p);
+        return cudaGetLastError();
+    };
+    if (!p.o.p) return run(delta_chain_kernel<T, DP, false, true>);
+    if (p.S0) return run(delta_chain_kernel<T, DP, true, true>);
+    return run(delta_chain_kernel<T, DP, true, false>);
+}
+
+template <typename T, int DP>
+cudaError_t fwd_t(const DeltaParams& p, cudaStream_t st) {
+    const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    const size_t prep = sizeof(PrepSmem<T, DP>);
+    cudaError_t err = cudaFuncSetAttribute(delta_prep_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prep);
+    if (err != cudaSuccess) return err;
+    delta_prep_kernel<T, DP><<<(unsigned)(bh * p.nc), 128, prep, st>>>(p);
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    return chain_t<T, DP>(p, (unsigned)(bh * ncb), st);
+}
+
+}  // namespace
+}  // namespace subq

@@ -5,16 +5,29 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "kernels.hpp"
+
 namespace subq {
 
 struct DeltaParams;
 
 // Token-recurrent forward, any d, e <= 256 (delta_step.cu); S_out may be S_in.
 cudaError_t launch_delta_step(const DeltaParams& p, int dtype, cudaStream_t st);
-// Chunked forward, d <= 128 (delta_fwd.cu): fills p.Y, then walks the chunks. 2 launches.
-cudaError_t launch_delta_fwd(const DeltaParams& p, int dtype, cudaStream_t st);
-// Gradients from p.Y, p.S0 and p.W of the forward (delta_bwd.cu). 2 launches, and one per shared q, k, v.
-cudaError_t launch_delta_bwd(const DeltaParams& p, int dtype, cudaStream_t st, int* launches);
+// Chunked forward, d <= 128 (delta_fwd.cuh): fills p.gates, p.Y and p.P, then walks the chunks. 2 launches.
+cudaError_t launch_delta_fwd_bf16(const DeltaParams& p, cudaStream_t st);
+cudaError_t launch_delta_fwd_fp16(const DeltaParams& p, cudaStream_t st);
+cudaError_t launch_delta_fwd_fp32(const DeltaParams& p, cudaStream_t st);
+inline cudaError_t launch_delta_fwd(const DeltaParams& p, int dtype, cudaStream_t st) {
+    return dtype == SUBQ_BF16 ? launch_delta_fwd_bf16(p, st) : dtype == SUBQ_FP16 ? launch_delta_fwd_fp16(p, st) : launch_delta_fwd_fp32(p, st);
+}
+// Gradients from what the forward left (p.gates, p.Y, p.P, p.S0, p.W) (delta_bwd.cuh). 2 launches, and one per shared q, k, v.
+cudaError_t launch_delta_bwd_bf16(const DeltaParams& p, cudaStream_t st, int* launches);
+cudaError_t launch_delta_bwd_fp16(const DeltaParams& p, cudaStream_t st, int* launches);
+cudaError_t launch_delta_bwd_fp32(const DeltaParams& p, cudaStream_t st, int* launches);
+inline cudaError_t launch_delta_bwd(const DeltaParams& p, int dtype, cudaStream_t st, int* launches) {
+    return dtype == SUBQ_BF16 ? launch_delta_bwd_bf16(p, st, launches)
+                              : dtype == SUBQ_FP16 ? launch_delta_bwd_fp16(p, st, launches) : launch_delta_bwd_fp32(p, st, launches);
+}
 
 // Layer norm over the last dimension (layer_norm.cu): rows at element strides.
 struct LnParams {
