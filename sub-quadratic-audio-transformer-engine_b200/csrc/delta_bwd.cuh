@@ -40,7 +40,13 @@ struct RevSmem {
     // by pair of warps
     alignas(16) unsigned char G[2][DP / 16][kX * 512];  // G^T, planes
     alignas(16) unsigned char R[2][4][kX * 512];        // -(beta dU)^T, planes
-    float4 Z[2][8 * 32];                                // Z^T, float32
+    // as W in the forward's walk: planes of -e^g beta Z and of Z, or Z in float32
+    static constexpr bool kShared = kX == 2;
+    alignas(16) unsigned char Zk[2][kShared ? 4 : 1][kX * 512];
+    union {
+        float4 Z[2][8 * 32];
+        unsigned char Zp[2][4][1024];
+    } z;
     float4 e2[2][DP / 8 * 32];                          // (scale (e^g Q)^T dO)^T; before that, (P^T dO)^T of the same chunk
 };
 
@@ -49,6 +55,7 @@ template <typename T, int DP>
 __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int col0, int lane) {
     constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = RevSmem<T, DP>::kStages;
     constexpr int NH = DP / 16;
+    constexpr bool kShared = RevSmem<T, DP>::kShared;
     const int g = lane >> 2, t = lane & 3;
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
@@ -83,8 +90,7 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaPa
             for (int kk = 0; kk < DP / 16; ++kk) {
                 uint32_t a[NX][4];
                 get_a<NX>(a, sm.G[pair][kk], lane);
-                mma_rows<DP, NX, NIN, NX>(X[0], X[1], a, kt, 16 * own.b0, kk, lane);
-                mma_rows<DP, NX, NIN, NX>(X[2], X[3], a, kt, 16 * own.b1, kk, lane);
+                mma_rows<DP, NX, NIN, NX>(X, a, kt, 16 * own.b0, 16 * own.b1, kk, lane);
             }
             bar_sync(1, 256);  // P^T dO is there; G has been read
 #pragma unroll
@@ -114,11 +120,29 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaPa
                 if (ib < own.b0) continue;
                 uint32_t a[NX][4];
                 get_a<NX>(a, sm.R[pair][ib], lane);
-                mma_block<NX, NX, false>(X[0], X[1], a, yt + tri(ib, own.b0) * 512, kYBlocks * 512);
-                if (ib >= own.b1) mma_block<NX, NX, false>(X[2], X[3], a, yt + tri(ib, own.b1) * 512, kYBlocks * 512);
+                mma_blocks<NX, NX, false>(X, a, true, yt + tri(ib, own.b0) * 512, ib >= own.b1, yt + tri(ib, own.b1) * 512);
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) sm.Z[pair][(2 * own.at(x >> 1) + (x & 1)) * 32 + lane] = as_float4(X[x]);
+            for (int u = 0; u < 2; ++u) {
+                const int jb = own.at(u);
+                if constexpr (kShared) {
+                    float2 f[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = 16 * jb + 8 * i + 2 * t;
+                        const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]), eg = *reinterpret_cast<const float2*>(&s.eg[j]);
+                        f[i] = make_float2(-be.x * eg.x, -be.y * eg.y);
+                    }
+                    uint32_t a[NX][4];
+                    to_a<NX>(X[2 * u], X[2 * u + 1], f[0], f[1], a);
+                    put_a<NX>(sm.Zk[pair][jb], a, lane);
+                    to_a<NX>(X[2 * u], X[2 * u + 1], one, one, a);
+                    put_a<NX>(sm.z.Zp[pair][jb], a, lane);
+                } else {
+                    sm.z.Z[pair][2 * jb * 32 + lane] = as_float4(X[2 * u]);
+                    sm.z.Z[pair][(2 * jb + 1) * 32 + lane] = as_float4(X[2 * u + 1]);
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -128,20 +152,22 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaPa
             for (int n = 0; n < NH; ++n) add_acc(S[n], sm.e2[pair][(A * NH + n) * 32 + lane]);
 #pragma unroll
             for (int jb = 0; jb < 4; ++jb) {  // G0^T = e^{g_C} G^T + e2 - (e^g beta Z)^T K over this half of d
-                float z0[4], z1[4];
-                get_acc2(z0, z1, sm.Z[pair] + 2 * jb * 32, lane);
-                float2 f[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int j = 16 * jb + 8 * i + 2 * t;
-                    const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]), eg = *reinterpret_cast<const float2*>(&s.eg[j]);
-                    f[i] = make_float2(-be.x * eg.x, -be.y * eg.y);
-                }
                 uint32_t a[NX][4];
-                to_a<NX>(z0, z1, f[0], f[1], a);
+                if constexpr (kShared) {
+                    get_a<NX>(a, sm.Zk[pair][jb], lane);
+                } else {
+                    float z0[4], z1[4];
+                    get_acc2(z0, z1, sm.z.Z[pair] + 2 * jb * 32, lane);
+                    float2 f[2];
 #pragma unroll
-                for (int np = 0; np < NH / 2; ++np)
-                    mma_cols<DP, NX, NIN, NX>(S[2 * np], S[2 * np + 1], a, kt, 16 * jb, A * (NH / 2) + np, lane);
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = 16 * jb + 8 * i + 2 * t;
+                        const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]), eg = *reinterpret_cast<const float2*>(&s.eg[j]);
+                        f[i] = make_float2(-be.x * eg.x, -be.y * eg.y);
+                    }
+                    to_a<NX>(z0, z1, f[0], f[1], a);
+                }
+                mma_cols<NH, DP, NX, NIN, NX>(S, a, kt, 16 * jb, A * NH, lane);
             }
             put_state();
         }
@@ -184,8 +210,7 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
                 uint32_t a[NIN][4];  // dO^T: 16 value columns x 16 tokens
 #pragma unroll
                 for (int pl = 0; pl < NIN; ++pl) a_cols<kDeltaCols>(a[pl], gt + pl * kGTile, 16 * ib, pair, lane);
-                mma_block<NIN, NX, true>(E[0], E[1], a, pt + tri(ib, own.b0) * 512, kYBlocks * 512);
-                if (ib >= own.b1) mma_block<NIN, NX, true>(E[2], E[3], a, pt + tri(ib, own.b1) * 512, kYBlocks * 512);
+                mma_blocks<NIN, NX, true>(E, a, true, pt + tri(ib, own.b0) * 512, ib >= own.b1, pt + tri(ib, own.b1) * 512);
             }
 #pragma unroll
             for (int x = 0; x < 4; ++x) sm.e2[pair][(2 * own.at(x >> 1) + (x & 1)) * 32 + lane] = as_float4(E[x]);
@@ -219,19 +244,21 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
 #pragma unroll
                     for (int pl = 0; pl < NX; ++pl) a[pl][m] = q[pl];
                 }
-#pragma unroll
-                for (int np = 0; np < NH / 2; ++np)
-                    mma_cols<DP, NX, NIN, NX>(E2[2 * np], E2[2 * np + 1], a, qt, 16 * ib, A * (NH / 2) + np, lane);
+                mma_cols<NH, DP, NX, NIN, NX>(E2, a, qt, 16 * ib, A * NH, lane);
             }
             bar_sync(6 + pair, 128);
             put_acc<NH>(sm.e2[pair] + A * NH * 32, E2, lane);
             bar_sync(2, 256);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                float z0[4], z1[4];
-                get_acc2(z0, z1, sm.Z[pair] + 2 * own.at(u) * 32, lane);
                 uint32_t a[NX][4];
-                to_a<NX>(z0, z1, one, one, a);
+                if constexpr (RevSmem<T, DP>::kShared) {
+                    get_a<NX>(a, sm.z.Zp[pair][own.at(u)], lane);
+                } else {
+                    float z0[4], z1[4];
+                    get_acc2(z0, z1, sm.z.Z[pair] + 2 * own.at(u) * 32, lane);
+                    to_a<NX>(z0, z1, one, one, a);
+                }
                 store_matrices<NX>(p.Z + (cw * 4 + own.at(u)) * (NX * 512), a, lane);
             }
         }
@@ -537,18 +564,15 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
                     ldm_t(r, S0 + ((cw * (DP / 16) + kk) * NX + pl) * 512);
                     b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
                 }
-                mma_planes<NIN, NX, NX>(dq[2 * n], ao, b0);
-                mma_planes<NIN, NX, NX>(dq[2 * n + 1], ao, b1);
-                mma_planes<NX, NX, NX>(dk2[2 * n], az, b0);
-                mma_planes<NX, NX, NX>(dk2[2 * n + 1], az, b1);
+                mma_pair<NIN, NX, NX>(dq[2 * n], dq[2 * n + 1], ao, b0, b1);
+                mma_pair<NX, NX, NX>(dk2[2 * n], dk2[2 * n + 1], az, b0, b1);
 #pragma unroll
                 for (int pl = 0; pl < NX; ++pl) {
                     uint32_t r[4];
                     ldm_t(r, G + ((cw * (DP / 16) + kk) * NX + pl) * 512);
                     b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
                 }
-                mma_planes<NX, NX, NX>(dk1[2 * n], aw, b0);
-                mma_planes<NX, NX, NX>(dk1[2 * n + 1], aw, b1);
+                mma_pair<NX, NX, NX>(dk1[2 * n], dk1[2 * n + 1], aw, b0, b1);
             }
 #pragma unroll
             for (int jb = 0; jb < 4; ++jb) {
@@ -561,11 +585,9 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
                     b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
                 }
                 if (hf == 0) {
-                    mma_planes<NIN, NX, NX>(D[2 * jb], ao, b0);
-                    mma_planes<NIN, NX, NX>(D[2 * jb + 1], ao, b1);
+                    mma_pair<NIN, NX, NX>(D[2 * jb], D[2 * jb + 1], ao, b0, b1);
                 } else {
-                    mma_planes<NX, NX, NX>(D[2 * jb], az, b0);
-                    mma_planes<NX, NX, NX>(D[2 * jb + 1], az, b1);
+                    mma_pair<NX, NX, NX>(D[2 * jb], D[2 * jb + 1], az, b0, b1);
                 }
             }
         }
@@ -721,16 +743,12 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
                 q0[pl][0] = r[0]; q0[pl][1] = r[1]; q1[pl][0] = r[2]; q1[pl][1] = r[3];
             }
             if (ob <= rb) {
-                mma_planes<NX, NIN, NX>(dq[2 * n], a1, k0);
-                mma_planes<NX, NIN, NX>(dq[2 * n + 1], a1, k1);
-                mma_planes<NX, NIN, NX>(dk1[2 * n], a2, k0);
-                mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a2, k1);
+                mma_pair<NX, NIN, NX>(dq[2 * n], dq[2 * n + 1], a1, k0, k1);
+                mma_pair<NX, NIN, NX>(dk1[2 * n], dk1[2 * n + 1], a2, k0, k1);
             }
             if (ob >= rb) {
-                mma_planes<NX, NIN, NX>(dk1[2 * n], a1t, q0);
-                mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a1t, q1);
-                mma_planes<NX, NIN, NX>(dk1[2 * n], a2t, k0);
-                mma_planes<NX, NIN, NX>(dk1[2 * n + 1], a2t, k1);
+                mma_pair<NX, NIN, NX>(dk1[2 * n], dk1[2 * n + 1], a1t, q0, q1);
+                mma_pair<NX, NIN, NX>(dk1[2 * n], dk1[2 * n + 1], a2t, k0, k1);
             }
         }
     }

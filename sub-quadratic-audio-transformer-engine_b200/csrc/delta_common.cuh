@@ -152,6 +152,31 @@ __device__ __forceinline__ void mma_planes(float (&c)[4], const uint32_t (&a)[NA
             if (i + j < NX) mma(c, a[i], b[j][0], b[j][1]);
 }
 
+// c[n] += A B[n], plane pair by plane pair over all n: each accumulator is used again only after the others, which
+// hides the instruction's latency (22 cycles against 8 of issue: four accumulators at least).
+template <int N, int NA, int NB, int NX>
+__device__ __forceinline__ void mma_set(float (&c)[N][4], const uint32_t (&a)[NA][4], const uint32_t (&b)[N][NB][2]) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (i + j < NX)
+#pragma unroll
+                for (int n = 0; n < N; ++n) mma(c[n], a[i], b[n][j][0], b[n][j][1]);
+}
+template <int NA, int NB, int NX>
+__device__ __forceinline__ void mma_pair(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b0)[NB][2],
+                                         const uint32_t (&b1)[NB][2]) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (i + j < NX) {
+                mma(c0, a[i], b0[j][0], b0[j][1]);
+                mma(c1, a[i], b1[j][0], b1[j][1]);
+            }
+}
+
 // Accumulators of two neighbouring 8-column blocks (16 rows x 16 columns) as the
 // A operand of the next product, times per-column factors f0 (columns 2t, 2t + 1
 // of the first block) and f1 (of the second).
@@ -456,8 +481,7 @@ __device__ __forceinline__ void score_rows(unsigned char* out, uint32_t q, uint3
                     b_rows<DP>(r, k + pl * kTile, 16 * jb, kk, lane);
                     b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
                 }
-                mma_planes<NIN, NIN, NX>(acc[2 * jb], a, b0);
-                mma_planes<NIN, NIN, NX>(acc[2 * jb + 1], a, b1);
+                mma_pair<NIN, NIN, NX>(acc[2 * jb], acc[2 * jb + 1], a, b0, b1);
             }
         }
     }
@@ -532,50 +556,66 @@ __device__ __forceinline__ void get_acc2(float (&c0)[4], float (&c1)[4], const f
     c0[0] = x.x; c0[1] = x.y; c0[2] = x.z; c0[3] = x.w;
     c1[0] = y.x; c1[1] = y.y; c1[2] = y.z; c1[3] = y.w;
 }
-// Products of one A operand with the 16 rows n0 .. of a tile (B[k][n] = tile[n][k]), k block kk.
+// Products of one A operand with 16 rows n0 .. and 16 rows n1 .. of a tile (B[k][n] = tile[n][k]), k block kk.
 template <int W, int NA, int NB, int NX>
-__device__ __forceinline__ void mma_rows(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], uint32_t tile, int n0, int kk, int lane) {
-    uint32_t b0[NB][2], b1[NB][2];
+__device__ __forceinline__ void mma_rows(float (&c)[4][4], const uint32_t (&a)[NA][4], uint32_t tile, int n0, int n1, int kk, int lane) {
+    uint32_t b[4][NB][2];
 #pragma unroll
     for (int pl = 0; pl < NB; ++pl) {
-        uint32_t r[4];
+        uint32_t r[4], q[4];
         b_rows<W>(r, tile + pl * (64 * W * 2), n0, kk, lane);
-        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-    }
-    mma_planes<NA, NB, NX>(c0, a, b0);
-    mma_planes<NA, NB, NX>(c1, a, b1);
-}
-// B[k][n] = tile[k][n]: rows k0 .., columns 16 np ..
-template <int W, int NA, int NB, int NX>
-__device__ __forceinline__ void mma_cols(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], uint32_t tile, int k0, int np, int lane) {
-    uint32_t b0[NB][2], b1[NB][2];
+        b_rows<W>(q, tile + pl * (64 * W * 2), n1, kk, lane);
 #pragma unroll
-    for (int pl = 0; pl < NB; ++pl) {
-        uint32_t r[4];
-        b_cols<W>(r, tile + pl * (64 * W * 2), k0, np, lane);
-        b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+        for (int i = 0; i < 4; ++i) b[i >> 1][pl][i & 1] = r[i], b[2 + (i >> 1)][pl][i & 1] = q[i];
     }
-    mma_planes<NA, NB, NX>(c0, a, b0);
-    mma_planes<NA, NB, NX>(c1, a, b1);
+    mma_set<4, NA, NB, NX>(c, a, b);
 }
-// B = a 16 x 16 block M[r][c] kept as four 8 x 8 matrices (row half, column half) per plane, planes `pitch` bytes
+// B[k][n] = tile[k][n]: rows k0 .., columns 8 n0 .. 8 (n0 + N) - 1.
+template <int N, int W, int NA, int NB, int NX>
+__device__ __forceinline__ void mma_cols(float (&c)[N][4], const uint32_t (&a)[NA][4], uint32_t tile, int k0, int n0, int lane) {
+    uint32_t b[N][NB][2];
+#pragma unroll
+    for (int np = 0; np < N / 2; ++np)
+#pragma unroll
+        for (int pl = 0; pl < NB; ++pl) {
+            uint32_t r[4];
+            b_cols<W>(r, tile + pl * (64 * W * 2), k0, n0 / 2 + np, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[2 * np + (i >> 1)][pl][i & 1] = r[i];
+        }
+    mma_set<N, NA, NB, NX>(c, a, b);
+}
+// B = a 16 x 16 block M[r][c] kept as four 8 x 8 matrices (row half, column half) per plane, planes kYBlocks blocks
 // apart; `block` is its address plus lane * 16. KROWS: B[k][n] = M[k][n], else B[k][n] = M[n][k].
-template <int NA, int NX, bool KROWS>
-__device__ __forceinline__ void mma_block(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], uint32_t block, int pitch) {
-    uint32_t b0[NX][2], b1[NX][2];
+template <int NX, bool KROWS>
+__device__ __forceinline__ void load_block(uint32_t (&b0)[NX][2], uint32_t (&b1)[NX][2], uint32_t block) {
 #pragma unroll
     for (int pl = 0; pl < NX; ++pl) {
         uint32_t r[4];
         if (KROWS) {
-            ldm_t(r, block + pl * pitch);
+            ldm_t(r, block + pl * (kYBlocks * 512));
             b0[pl][0] = r[0]; b0[pl][1] = r[2]; b1[pl][0] = r[1]; b1[pl][1] = r[3];
         } else {
-            ldm(r, block + pl * pitch);
+            ldm(r, block + pl * (kYBlocks * 512));
             b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
         }
     }
-    mma_planes<NA, NX, NX>(c0, a, b0);
-    mma_planes<NA, NX, NX>(c1, a, b1);
+}
+// c[0], c[1] += A M0 where `first`, c[2], c[3] += A M1 where `second`.
+template <int NA, int NX, bool KROWS>
+__device__ __forceinline__ void mma_blocks(float (&c)[4][4], const uint32_t (&a)[NA][4], bool first, uint32_t m0, bool second, uint32_t m1) {
+    uint32_t b[4][NX][2];
+    if (first && second) {
+        load_block<NX, KROWS>(b[0], b[1], m0);
+        load_block<NX, KROWS>(b[2], b[3], m1);
+        mma_set<4, NA, NX, NX>(c, a, b);
+    } else if (first) {
+        load_block<NX, KROWS>(b[0], b[1], m0);
+        mma_pair<NA, NX, NX>(c[0], c[1], a, b[0], b[1]);
+    } else {
+        load_block<NX, KROWS>(b[2], b[3], m1);
+        mma_pair<NA, NX, NX>(c[2], c[3], a, b[2], b[3]);
+    }
 }
 
 // Two neighbouring blocks as the planes of an A operand, to memory as four 8 x 8 matrices of 128 bytes per plane.

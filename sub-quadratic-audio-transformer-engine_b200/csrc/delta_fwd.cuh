@@ -81,8 +81,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
                         b_rows<DP>(r, k + pl * kTile, 16 * jb, kk, lane);
                         b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
                     }
-                    mma_planes<NIN, NIN, NX>(acc[2 * jb], a, b0);
-                    mma_planes<NIN, NIN, NX>(acc[2 * jb + 1], a, b1);
+                    mma_pair<NIN, NIN, NX>(acc[2 * jb], acc[2 * jb + 1], a, b0, b1);
                 }
         }
 #pragma unroll
@@ -165,8 +164,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
                     ldm(r, ab + (tri(I - 1, J + kx) * NX + pl) * 512);
                     b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
                 }
-                mma_planes<NX, NX, NX>(acc[0], y[kx], b0);
-                mma_planes<NX, NX, NX>(acc[1], y[kx], b1);
+                mma_pair<NX, NX, NX>(acc[0], acc[1], y[kx], b0, b1);
             }
             uint32_t a[NX][4], b0[NX][2], b1[NX][2];
             to_a<NX>(acc[0], acc[1], one, one, a);
@@ -176,8 +174,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
                 ldm(r, ti + (I * NX + pl) * 512);
                 b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
             }
-            mma_planes<NX, NX, NX>(out[0], a, b0);
-            mma_planes<NX, NX, NX>(out[1], a, b1);
+            mma_pair<NX, NX, NX>(out[0], out[1], a, b0, b1);
             to_a<NX>(out[0], out[1], one, one, y[x]);
 #pragma unroll
             for (int pl = 0; pl < NX; ++pl)
@@ -206,15 +203,26 @@ struct ChainSmem {
     // by pair of warps
     alignas(16) unsigned char S0[2][DP / 16][kX * 512];  // S^T before the chunk, planes
     alignas(16) unsigned char R[2][4][kX * 512];         // -(beta R)^T, planes
-    float4 W[2][8 * 32];                                 // W^T, float32
-    alignas(16) unsigned char out[4][32 * (16 * sizeof(T) + 16)];
+    // W^T for the update and the outputs. 16-bit inputs: planes of beta W and of e^{g_C - g} beta W (and of W where
+    // it is kept), converted once by the warp that has it; float32 ones (no room): W, converted by each reader
+    static constexpr bool kShared = kX == 2;
+    alignas(16) unsigned char Wb[2][kShared ? 4 : 1][kX * 512];
+    alignas(16) unsigned char Wk[2][kShared ? 4 : 1][kX * 512];
+    union {
+        float4 W[2][8 * 32];
+        unsigned char Wp[2][4][1024];
+    } w;
+    // outputs on their way to memory: in the place of Y, which nobody reads any more by then
+    static constexpr int kOutPitch = 16 * sizeof(T) + 16;
+    static_assert(4 * 32 * kOutPitch <= kX * kYBlocks * 512, "staged outputs");
 };
 
 // One warp of a chain pair: half `A` of d of S^T in its accumulators; R and W of its token blocks.
-template <typename T, int DP>
+template <typename T, int DP, bool OUT, bool KEEP>
 __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int col0, int lane) {
     constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP>::kStages;
     constexpr int NH = DP / 16;  // 8-column blocks of half of d
+    constexpr bool kShared = ChainSmem<T, DP>::kShared;
     const int g = lane >> 2, t = lane & 3;
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
@@ -249,8 +257,7 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
             for (int kk = 0; kk < DP / 16; ++kk) {
                 uint32_t a[NX][4];
                 get_a<NX>(a, sm.S0[pair][kk], lane);
-                mma_rows<DP, NX, NIN, NX>(W[0], W[1], a, kt, 16 * own.b0, kk, lane);
-                mma_rows<DP, NX, NIN, NX>(W[2], W[3], a, kt, 16 * own.b1, kk, lane);
+                mma_rows<DP, NX, NIN, NX>(W, a, kt, 16 * own.b0, 16 * own.b1, kk, lane);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {  // R = V - e^g K S0; -beta R for both warps
@@ -289,11 +296,35 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
                 if (jb > own.b1) break;
                 uint32_t a[NX][4];
                 get_a<NX>(a, sm.R[pair][jb], lane);
-                mma_block<NX, NX, true>(W[2], W[3], a, yt + tri(own.b1, jb) * 512, kYBlocks * 512);
-                if (jb <= own.b0) mma_block<NX, NX, true>(W[0], W[1], a, yt + tri(own.b0, jb) * 512, kYBlocks * 512);
+                mma_blocks<NX, NX, true>(W, a, jb <= own.b0, yt + tri(own.b0, jb) * 512, true, yt + tri(own.b1, jb) * 512);
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) sm.W[pair][(2 * own.at(x >> 1) + (x & 1)) * 32 + lane] = as_float4(W[x]);
+            for (int u = 0; u < 2; ++u) {
+                const int jb = own.at(u);
+                if constexpr (kShared) {
+                    float2 fb[2], fk[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 kd = *reinterpret_cast<const float2*>(&s.kd[16 * jb + 8 * i + 2 * t]);
+                        fb[i] = *reinterpret_cast<const float2*>(&s.beta[16 * jb + 8 * i + 2 * t]);
+                        fk[i] = make_float2(fb[i].x * kd.x, fb[i].y * kd.y);
+                    }
+                    uint32_t a[NX][4];
+                    to_a<NX>(W[2 * u], W[2 * u + 1], fk[0], fk[1], a);
+                    put_a<NX>(sm.Wk[pair][jb], a, lane);
+                    if (OUT) {
+                        to_a<NX>(W[2 * u], W[2 * u + 1], fb[0], fb[1], a);
+                        put_a<NX>(sm.Wb[pair][jb], a, lane);
+                    }
+                    if (KEEP) {
+                        to_a<NX>(W[2 * u], W[2 * u + 1], one, one, a);
+                        put_a<NX>(sm.w.Wp[pair][jb], a, lane);
+                    }
+                } else {
+                    sm.w.W[pair][2 * jb * 32 + lane] = as_float4(W[2 * u]);
+                    sm.w.W[pair][(2 * jb + 1) * 32 + lane] = as_float4(W[2 * u + 1]);
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -301,20 +332,22 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
             bar_sync(1, 256);  // W is there for both pairs and the output warps, which have read S0
 #pragma unroll
             for (int jb = 0; jb < 4; ++jb) {  // S'^T = e^{g_C} S0^T + (e^{g_C - g} beta W)^T K over this half of d
-                float w0[4], w1[4];
-                get_acc2(w0, w1, sm.W[pair] + 2 * jb * 32, lane);
-                float2 f[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int j = 16 * jb + 8 * i + 2 * t;
-                    const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]), kd = *reinterpret_cast<const float2*>(&s.kd[j]);
-                    f[i] = make_float2(be.x * kd.x, be.y * kd.y);
-                }
                 uint32_t a[NX][4];
-                to_a<NX>(w0, w1, f[0], f[1], a);
+                if constexpr (kShared) {
+                    get_a<NX>(a, sm.Wk[pair][jb], lane);
+                } else {
+                    float w0[4], w1[4];
+                    get_acc2(w0, w1, sm.w.W[pair] + 2 * jb * 32, lane);
+                    float2 f[2];
 #pragma unroll
-                for (int np = 0; np < NH / 2; ++np)
-                    mma_cols<DP, NX, NIN, NX>(S[2 * np], S[2 * np + 1], a, kt, 16 * jb, A * (NH / 2) + np, lane);
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = 16 * jb + 8 * i + 2 * t;
+                        const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]), kd = *reinterpret_cast<const float2*>(&s.kd[j]);
+                        f[i] = make_float2(be.x * kd.x, be.y * kd.y);
+                    }
+                    to_a<NX>(w0, w1, f[0], f[1], a);
+                }
+                mma_cols<NH, DP, NX, NIN, NX>(S, a, kt, 16 * jb, A * NH, lane);
             }
             put_state();
         }
@@ -341,16 +374,17 @@ __device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaPar
     const float2 one = make_float2(1.f, 1.f);
     const int b = (int)(bh / p.H), h = (int)(bh % p.H), ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
     T* o = OUT ? static_cast<T*>(p.o.p) + tensor_base(p.o, b, h) : nullptr;
-    constexpr int kPitch = 16 * sizeof(T) + 16, kPieces = 16 * sizeof(T) / 16;  // bytes of a staged row, its 16-byte pieces
+    constexpr bool kShared = ChainSmem<T, DP>::kShared;
+    constexpr int kPitch = ChainSmem<T, DP>::kOutPitch, kPieces = 16 * sizeof(T) / 16;  // bytes of a staged row, its 16-byte pieces
     const int col0 = cb * kDeltaCols + 16 * pair, width = min(16, p.e - col0);
     const bool whole = OUT && p.o.vec && width == 16;
-    unsigned char* stage = sm.out[2 * pair + A];
     __syncthreads();
     for (int c = 0; c < p.nc; ++c) {
         if (NST == 1) __syncthreads();
         auto& st = sm.st[c % NST];
         const Gates& s = st.s;
         const int n0 = c * kDeltaC;
+        unsigned char* stage = st.y + (2 * pair + A) * (32 * kPitch);
         if (s.any) {
             const uint32_t qt = smem_addr(st.q), pt = smem_addr(st.P) + lane * 16;
             const int64_t cw = (bh * p.nc + c) * 2 * ncb + 2 * cb + pair;  // chunk and group of 16 columns
@@ -361,10 +395,7 @@ __device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaPar
                 uint32_t a[NX][4];
                 get_a<NX>(a, sm.S0[pair][kk], lane);
                 if (KEEP && kk % 2 == A) store_matrices<NX>(p.S0 + (cw * (DP / 16) + kk) * (NX * 512), a, lane);
-                if (OUT) {
-                    mma_rows<DP, NX, NIN, NX>(O[0], O[1], a, qt, 16 * own.b0, kk, lane);
-                    mma_rows<DP, NX, NIN, NX>(O[2], O[3], a, qt, 16 * own.b1, kk, lane);
-                }
+                if (OUT) mma_rows<DP, NX, NIN, NX>(O, a, qt, 16 * own.b0, 16 * own.b1, kk, lane);
             }
             if (OUT)
 #pragma unroll
@@ -380,19 +411,25 @@ __device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaPar
             for (int jb = 0; jb < 4; ++jb) {
                 const bool mine = jb == own.b0 || jb == own.b1;
                 if (OUT ? jb > own.b1 : !mine) continue;
-                float w0[4], w1[4];
-                get_acc2(w0, w1, sm.W[pair] + 2 * jb * 32, lane);
                 uint32_t a[NX][4];
-                if (KEEP && mine) {
-                    to_a<NX>(w0, w1, one, one, a);
-                    store_matrices<NX>(p.W + (cw * 4 + jb) * (NX * 512), a, lane);
+                if constexpr (kShared) {
+                    if (KEEP && mine) {
+                        get_a<NX>(a, sm.w.Wp[pair][jb], lane);
+                        store_matrices<NX>(p.W + (cw * 4 + jb) * (NX * 512), a, lane);
+                    }
+                    if (OUT) get_a<NX>(a, sm.Wb[pair][jb], lane);
+                } else {
+                    float w0[4], w1[4];
+                    get_acc2(w0, w1, sm.w.W[pair] + 2 * jb * 32, lane);
+                    if (KEEP && mine) {
+                        to_a<NX>(w0, w1, one, one, a);
+                        store_matrices<NX>(p.W + (cw * 4 + jb) * (NX * 512), a, lane);
+                    }
+                    if (OUT)
+                        to_a<NX>(w0, w1, *reinterpret_cast<const float2*>(&s.beta[16 * jb + 2 * t]),
+                                 *reinterpret_cast<const float2*>(&s.beta[16 * jb + 8 + 2 * t]), a);
                 }
-                if (OUT) {
-                    to_a<NX>(w0, w1, *reinterpret_cast<const float2*>(&s.beta[16 * jb + 2 * t]),
-                             *reinterpret_cast<const float2*>(&s.beta[16 * jb + 8 + 2 * t]), a);
-                    mma_block<NX, NX, false>(O[2], O[3], a, pt + tri(own.b1, jb) * 512, kYBlocks * 512);
-                    if (jb <= own.b0) mma_block<NX, NX, false>(O[0], O[1], a, pt + tri(own.b0, jb) * 512, kYBlocks * 512);
-                }
+                if (OUT) mma_blocks<NX, NX, false>(O, a, jb <= own.b0, pt + tri(own.b0, jb) * 512, true, pt + tri(own.b1, jb) * 512);
             }
             if (OUT) {
 #pragma unroll
@@ -443,7 +480,7 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
     const int64_t bh = blockIdx.x / ncb;
     const int cb = blockIdx.x % ncb, b = (int)(bh / p.H), h = (int)(bh % p.H), c0 = cb * kDeltaCols;
     if (warp < 4) {
-        chain_warp<T, DP>(sm, p, warp & 1, warp >> 1, bh, c0 + 16 * (warp >> 1), lane);
+        chain_warp<T, DP, OUT, KEEP>(sm, p, warp & 1, warp >> 1, bh, c0 + 16 * (warp >> 1), lane);
     } else if (warp < 8) {
         output_warp<T, DP, OUT, KEEP>(sm, p, warp & 1, (warp >> 1) & 1, bh, cb, lane);
     } else {  // ---------------------------------------------------------- loads
