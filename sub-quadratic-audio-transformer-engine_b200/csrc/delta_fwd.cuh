@@ -190,8 +190,10 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
 template <typename T, int DP>
 struct ChainSmem {
     static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
-    // chunks in shared memory: the one at work, the next, and one more on its way where that fits
-    static constexpr int kStages = kIn == 1 ? (DP == 64 ? 3 : 2) : DP == 64 ? 2 : 1;
+    // chunks in shared memory: the one at work and the next; where they fit, one more on its way, and the last one for
+    // the output warps, which then finish a chunk while the chain is at the next
+    static constexpr int kStages = kIn == 1 ? (DP == 64 ? 4 : 2) : DP == 64 ? 2 : 1;
+    static constexpr bool kLag = kStages == 4;
     struct Stage {
         alignas(128) unsigned char k[kIn * 64 * DP * 2];
         alignas(128) unsigned char q[kIn * 64 * DP * 2];
@@ -206,7 +208,7 @@ struct ChainSmem {
     // W^T for the update and the outputs. 16-bit inputs: planes of beta W and of e^{g_C - g} beta W (and of W where
     // it is kept), converted once by the warp that has it; float32 ones (no room): W, converted by each reader
     static constexpr bool kShared = kX == 2;
-    alignas(16) unsigned char Wb[2][kShared ? 4 : 1][kX * 512];
+    alignas(16) unsigned char Wb[kLag ? 2 : 1][2][kShared ? 4 : 1][kX * 512];  // (by chunk parity where outputs lag)
     alignas(16) unsigned char Wk[2][kShared ? 4 : 1][kX * 512];
     union {
         float4 W[2][8 * 32];
@@ -314,7 +316,7 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
                     put_a<NX>(sm.Wk[pair][jb], a, lane);
                     if (OUT) {
                         to_a<NX>(W[2 * u], W[2 * u + 1], fb[0], fb[1], a);
-                        put_a<NX>(sm.Wb[pair][jb], a, lane);
+                        put_a<NX>(sm.Wb[ChainSmem<T, DP>::kLag ? c & 1 : 0][pair][jb], a, lane);
                     }
                     if (KEEP) {
                         to_a<NX>(W[2 * u], W[2 * u + 1], one, one, a);
@@ -378,26 +380,95 @@ __device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaPar
     constexpr int kPitch = ChainSmem<T, DP>::kOutPitch, kPieces = 16 * sizeof(T) / 16;  // bytes of a staged row, its 16-byte pieces
     const int col0 = cb * kDeltaCols + 16 * pair, width = min(16, p.e - col0);
     const bool whole = OUT && p.o.vec && width == 16;
-    __syncthreads();
-    for (int c = 0; c < p.nc; ++c) {
-        if (NST == 1) __syncthreads();
+    constexpr bool kLag = ChainSmem<T, DP>::kLag;
+    float O[4][4];  // blocks 2 u + half of this warp's tokens
+    auto planes_of_w = [&](int c) {
+        const int64_t cw = (bh * p.nc + c) * 2 * ncb + 2 * cb + pair;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int jb = own.at(u);
+            uint32_t a[NX][4];
+            if constexpr (kShared) {
+                get_a<NX>(a, sm.w.Wp[pair][jb], lane);
+            } else {
+                float w0[4], w1[4];
+                get_acc2(w0, w1, sm.w.W[pair] + 2 * jb * 32, lane);
+                to_a<NX>(w0, w1, one, one, a);
+            }
+            store_matrices<NX>(p.W + (cw * 4 + jb) * (NX * 512), a, lane);
+        }
+    };
+    auto finish = [&](int c) {  // the scores' part of the outputs of chunk c, and the outputs to memory
         auto& st = sm.st[c % NST];
         const Gates& s = st.s;
         const int n0 = c * kDeltaC;
         unsigned char* stage = st.y + (2 * pair + A) * (32 * kPitch);
+        const bool any = s.any;
+        if (any) {
+            const uint32_t pt = smem_addr(st.P) + lane * 16;
+#pragma unroll
+            for (int jb = 0; jb < 4; ++jb) {
+                if (jb > own.b1) break;
+                uint32_t a[NX][4];
+                if constexpr (kShared) {
+                    get_a<NX>(a, sm.Wb[kLag ? c & 1 : 0][pair][jb], lane);
+                } else {
+                    float w0[4], w1[4];
+                    get_acc2(w0, w1, sm.w.W[pair] + 2 * jb * 32, lane);
+                    to_a<NX>(w0, w1, *reinterpret_cast<const float2*>(&s.beta[16 * jb + 2 * t]),
+                             *reinterpret_cast<const float2*>(&s.beta[16 * jb + 8 + 2 * t]), a);
+                }
+                mma_blocks<NX, NX, false>(O, a, jb <= own.b0, pt + tri(own.b0, jb) * 512, true, pt + tri(own.b1, jb) * 512);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {  // staged rows: 16 u + 8 half + ..
+                T* r0 = reinterpret_cast<T*>(stage + (8 * n + 2 * t) * kPitch);
+                T* r1 = reinterpret_cast<T*>(stage + (8 * n + 2 * t + 1) * kPitch);
+                r0[g] = from_f<T>(O[n][0]);
+                r1[g] = from_f<T>(O[n][1]);
+                r0[g + 8] = from_f<T>(O[n][2]);
+                r1[g + 8] = from_f<T>(O[n][3]);
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) {
+            const int i = lane + 32 * x, row = i / kPieces, piece = i % kPieces;
+            const int tok = 16 * own.at(row >> 4) + (row & 15);
+            if (n0 + tok >= p.N) continue;
+            T* dst = o + (n0 + tok) * p.o.sn + col0;
+            const bool live = any && s.live[tok];
+            const unsigned char* src = stage + row * kPitch + piece * 16;
+            if (whole) {
+                reinterpret_cast<uint4*>(dst)[piece] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+            } else {
+                constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+                for (int y = 0; y < kPer; ++y)
+                    if (piece * kPer + y < width)
+                        dst[piece * kPer + y] = live ? reinterpret_cast<const T*>(src)[y] : from_f<T>(0.f);
+            }
+        }
+    };
+    __syncthreads();
+    for (int c = 0; c < p.nc; ++c) {
+        if (NST == 1) __syncthreads();
+        if (OUT && kLag && c > 0) finish(c - 1);
+        auto& st = sm.st[c % NST];
+        const Gates& s = st.s;
         if (s.any) {
-            const uint32_t qt = smem_addr(st.q), pt = smem_addr(st.P) + lane * 16;
+            const uint32_t qt = smem_addr(st.q);
             const int64_t cw = (bh * p.nc + c) * 2 * ncb + 2 * cb + pair;  // chunk and group of 16 columns
-            float O[4][4];  // blocks 2 u + half
             zero_acc<4>(O);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {  // (Q S0)^T
+                if (!OUT && kk % 2 != A) continue;
                 uint32_t a[NX][4];
                 get_a<NX>(a, sm.S0[pair][kk], lane);
                 if (KEEP && kk % 2 == A) store_matrices<NX>(p.S0 + (cw * (DP / 16) + kk) * (NX * 512), a, lane);
                 if (OUT) mma_rows<DP, NX, NIN, NX>(O, a, qt, 16 * own.b0, 16 * own.b1, kk, lane);
             }
-            if (OUT)
+            if (OUT) {
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const float2 eg = *reinterpret_cast<const float2*>(&s.eg[16 * own.at(n >> 1) + 8 * (n & 1) + 2 * t]);
@@ -406,66 +477,14 @@ __device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaPar
                     O[n][2] *= p.scale * eg.x;
                     O[n][3] *= p.scale * eg.y;
                 }
+            }
             bar_sync(1, 256);
-#pragma unroll
-            for (int jb = 0; jb < 4; ++jb) {
-                const bool mine = jb == own.b0 || jb == own.b1;
-                if (OUT ? jb > own.b1 : !mine) continue;
-                uint32_t a[NX][4];
-                if constexpr (kShared) {
-                    if (KEEP && mine) {
-                        get_a<NX>(a, sm.w.Wp[pair][jb], lane);
-                        store_matrices<NX>(p.W + (cw * 4 + jb) * (NX * 512), a, lane);
-                    }
-                    if (OUT) get_a<NX>(a, sm.Wb[pair][jb], lane);
-                } else {
-                    float w0[4], w1[4];
-                    get_acc2(w0, w1, sm.w.W[pair] + 2 * jb * 32, lane);
-                    if (KEEP && mine) {
-                        to_a<NX>(w0, w1, one, one, a);
-                        store_matrices<NX>(p.W + (cw * 4 + jb) * (NX * 512), a, lane);
-                    }
-                    if (OUT)
-                        to_a<NX>(w0, w1, *reinterpret_cast<const float2*>(&s.beta[16 * jb + 2 * t]),
-                                 *reinterpret_cast<const float2*>(&s.beta[16 * jb + 8 + 2 * t]), a);
-                }
-                if (OUT) mma_blocks<NX, NX, false>(O, a, jb <= own.b0, pt + tri(own.b0, jb) * 512, true, pt + tri(own.b1, jb) * 512);
-            }
-            if (OUT) {
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {  // staged rows: 16 u + 8 half + ..
-                    T* r0 = reinterpret_cast<T*>(stage + (8 * n + 2 * t) * kPitch);
-                    T* r1 = reinterpret_cast<T*>(stage + (8 * n + 2 * t + 1) * kPitch);
-                    r0[g] = from_f<T>(O[n][0]);
-                    r1[g] = from_f<T>(O[n][1]);
-                    r0[g + 8] = from_f<T>(O[n][2]);
-                    r1[g + 8] = from_f<T>(O[n][3]);
-                }
-                __syncwarp();
-            }
+            if (KEEP) planes_of_w(c);
         }
-        if (OUT) {
-#pragma unroll
-            for (int x = 0; x < kPieces; ++x) {
-                const int i = lane + 32 * x, row = i / kPieces, piece = i % kPieces;
-                const int tok = 16 * own.at(row >> 4) + (row & 15);
-                if (n0 + tok >= p.N) continue;
-                T* dst = o + (n0 + tok) * p.o.sn + col0;
-                const bool live = s.any && s.live[tok];
-                const unsigned char* src = stage + row * kPitch + piece * 16;
-                if (whole) {
-                    reinterpret_cast<uint4*>(dst)[piece] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-                } else {
-                    constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-                    for (int y = 0; y < kPer; ++y)
-                        if (piece * kPer + y < width)
-                            dst[piece * kPer + y] = live ? reinterpret_cast<const T*>(src)[y] : from_f<T>(0.f);
-                }
-            }
-        }
+        if (OUT && !kLag) finish(c);
         __syncthreads();
     }
+    if (OUT && kLag) finish(p.nc - 1);
 }
 
 // OUT: writes o. KEEP: writes the planes of S0 and W that the backward reads.
@@ -495,7 +514,7 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
         if constexpr (NIN == 1) async = p.k.vec && p.q.vec && p.v.vec && p.d % 8 == 0 && p.e % 8 == 0;
         if (async) {
             // bf16: asynchronous copies, chunk c + kAhead started while c is computed
-            constexpr int kAhead = NST - 1;
+            constexpr int kAhead = NST > 2 ? NST - 2 : 1;
             int any_next = gates[0].any;
             auto start = [&](int c) {
                 if (c < p.nc) {
