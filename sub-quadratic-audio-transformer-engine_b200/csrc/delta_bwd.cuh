@@ -185,15 +185,20 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaPa
     }
 }
 
-// One warp of the pair beside a chain pair: P^T dO for its token blocks, (e^g Q)^T dO for its half of d, and
+// One warp of the pair beside a chain pair: P^T dO and dV for its token blocks, (e^g Q)^T dO for its half of d, and
 // its share of the planes of G and Z.
 template <typename T, int DP>
 __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int cb, int lane) {
     constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kGTile = 64 * kDeltaCols * 2;
     constexpr int NST = RevSmem<T, DP>::kStages, NH = DP / 16;
-    const int t = lane & 3, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    const int g = lane >> 2, t = lane & 3, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
+    constexpr int kPitch = 16 * sizeof(T) + 16, kPieces = 16 * sizeof(T) / 16;  // as the forward's staged outputs
+    static_assert(4 * 32 * kPitch <= NX * kYBlocks * 512, "staged dv");
+    const int col0 = cb * kDeltaCols + 16 * pair, width = min(16, p.e - col0);
+    const bool whole = p.dv.vec && width == 16;
+    T* dv = static_cast<T*>(p.dv.p) + tensor_base(p.dv, (int)(bh / p.H), (int)(bh % p.H));
     __syncthreads();
     for (int c = p.nc - 1; c >= 0; --c) {
         if (NST == 1) __syncthreads();
@@ -202,6 +207,7 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
         if (s.any) {
             const uint32_t qt = smem_addr(st.q), gt = smem_addr(st.g), pt = smem_addr(st.P) + lane * 16;
             const int64_t cw = (bh * p.nc + c) * 2 * ncb + 2 * cb + pair;  // chunk and group of 16 columns
+            const int n0 = c * kDeltaC;
             float E[4][4];
             zero_acc<4>(E);
 #pragma unroll
@@ -249,17 +255,60 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
             bar_sync(6 + pair, 128);
             put_acc<NH>(sm.e2[pair] + A * NH * 32, E2, lane);
             bar_sync(2, 256);
+            // planes of Z, and dv = beta Z, staged where Y was (which nobody reads any more)
+            unsigned char* stage = st.y + (2 * pair + A) * (32 * kPitch);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 uint32_t a[NX][4];
+                float z0[4], z1[4];
                 if constexpr (RevSmem<T, DP>::kShared) {
                     get_a<NX>(a, sm.z.Zp[pair][own.at(u)], lane);
+                    from_a<NX>(z0, z1, a);
                 } else {
-                    float z0[4], z1[4];
                     get_acc2(z0, z1, sm.z.Z[pair] + 2 * own.at(u) * 32, lane);
                     to_a<NX>(z0, z1, one, one, a);
                 }
                 store_matrices<NX>(p.Z + (cw * 4 + own.at(u)) * (NX * 512), a, lane);
+#pragma unroll
+                for (int jh = 0; jh < 2; ++jh) {
+                    const int tok = 16 * own.at(u) + 8 * jh + 2 * t;
+                    const float2 be = *reinterpret_cast<const float2*>(&s.beta[tok]);
+                    const float(&z)[4] = jh ? z1 : z0;
+                    const float f[4] = {z[0] * be.x, z[1] * be.y, z[2] * be.x, z[3] * be.y};
+                    if (p.dv32) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int n = n0 + tok + (i & 1), col = col0 + g + 8 * (i >> 1);
+                            if (n < p.N && col < p.e) p.dv32[(bh * p.N + n) * p.e + col] = f[i];
+                        }
+                    } else {
+                        T* r0 = reinterpret_cast<T*>(stage + (16 * u + 8 * jh + 2 * t) * kPitch);
+                        T* r1 = reinterpret_cast<T*>(stage + (16 * u + 8 * jh + 2 * t + 1) * kPitch);
+                        r0[g] = from_f<T>(f[0]);
+                        r1[g] = from_f<T>(f[1]);
+                        r0[g + 8] = from_f<T>(f[2]);
+                        r1[g + 8] = from_f<T>(f[3]);
+                    }
+                }
+            }
+            if (!p.dv32) {
+                __syncwarp();
+#pragma unroll
+                for (int x = 0; x < kPieces; ++x) {
+                    const int i = lane + 32 * x, row = i / kPieces, piece = i % kPieces;
+                    const int tok = 16 * own.at(row >> 4) + (row & 15);
+                    if (n0 + tok >= p.N) continue;
+                    T* dst = dv + (n0 + tok) * p.dv.sn + col0;
+                    const unsigned char* src = stage + row * kPitch + piece * 16;
+                    if (whole) {
+                        reinterpret_cast<uint4*>(dst)[piece] = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+                        for (int y = 0; y < kPer; ++y)
+                            if (piece * kPer + y < width) dst[piece * kPer + y] = reinterpret_cast<const T*>(src)[y];
+                    }
+                }
             }
         }
         __syncthreads();
@@ -274,8 +323,10 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
     RevSmem<T, DP>& sm = *reinterpret_cast<RevSmem<T, DP>*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
-    const int64_t bh = blockIdx.x / ncb;
-    const int cb = blockIdx.x % ncb, b = (int)(bh / p.H), h = (int)(bh % p.H), c0 = cb * kDeltaCols;
+    const unsigned bh32 = blockIdx.x / (unsigned)ncb;
+    const int64_t bh = bh32;
+    const int cb = (int)(blockIdx.x - bh32 * ncb), b = (int)(bh32 / (unsigned)p.H), h = (int)(bh32 - b * (unsigned)p.H);
+    const int c0 = cb * kDeltaCols;
     if (warp < 4) {
         rev_chain_warp<T, DP>(sm, p, warp & 1, warp >> 1, bh, c0 + 16 * (warp >> 1), lane);
     } else if (warp < 8) {
@@ -402,7 +453,7 @@ struct GradSmem {
     static constexpr int kBufs = kIn == 1 && DP == 64 ? 2 : 1;
     Gates s;
     float qdq[2][kDeltaC], vdv[kDeltaC], wz[kDeltaC], kdk[2][kDeltaC];
-    float gs[8];
+    float gs[2];
     alignas(128) unsigned char k[kIn * 64 * DP * 2];
     alignas(128) unsigned char q[kIn * 64 * DP * 2];
     struct In {  // one block of 32 value columns
@@ -420,42 +471,48 @@ struct GradSmem {
     union {
         In in[kBufs];
         Scores sc;
-        alignas(16) float rows[kDeltaC][DP + 4];
     } u;
-    alignas(16) float dv[kDeltaC][kDeltaCols + 4];
 };
 
-__device__ __forceinline__ float bf16_at(const unsigned char* p) {
-    return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16);
+// Rows of zeros.
+template <typename T>
+__device__ __forceinline__ void zero_rows(const DeltaTensor& x, int64_t base, float* x32, int64_t base32, int n0, int rows, int width, int tid) {
+    for (int i = tid; i < rows * width; i += 256) {
+        const int row = i / width, c = i % width;
+        if (x32) x32[base32 + (int64_t)(n0 + row) * width + c] = 0.f;
+        else (static_cast<T*>(x.p) + base + (n0 + row) * x.sn)[c] = from_f<T>(0.f);
+    }
 }
 
-// Rows 0 .. rows - 1 of a float tile to a gradient, 8 columns a thread; `x32` (per state head, [.., width]) instead of `x` where given.
-template <typename T, int NT>
-__device__ __forceinline__ void store_rows(const float* tile, int pitch, int cols, const DeltaTensor& x, int64_t base, float* x32,
-                                           int64_t base32, int n0, int rows, int c0, int width, int tid) {
-    const int pieces = cols / 8;
-    for (int i = tid; i < rows * pieces; i += NT) {
-        const int row = i / pieces, c = i % pieces * 8;
-        if (c0 + c >= width) continue;
-        const float* f = tile + row * pitch + c;
-        if (x32) {
-            float* at = x32 + base32 + (int64_t)(n0 + row) * width + c0 + c;
+// Accumulators of 16 tokens (from n) x 8 NB columns (from c) to the rows of a gradient (`x32`, per state head, where given).
+template <typename T, int NB>
+__device__ __forceinline__ void store_grad(const float (&f)[NB][4], const DeltaTensor& x, int64_t base, float* x32, int64_t base32, int n,
+                                           int end, int c, int width, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    c += 2 * t;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c0 + c + j < width) at[j] = f[j];
-            continue;
-        }
-        T* at = static_cast<T*>(x.p) + base + (n0 + row) * x.sn + c0 + c;
-        if (x.vec && c0 + c + 8 <= width) {
-            alignas(16) T t[8];
+    for (int h = 0; h < 2; ++h) {
+        const int row = n + 8 * h + g;
+        if (row >= end) continue;
+        if (!x32 && x.vec && c - 2 * t + 8 * NB <= width) {  // rows start on 16 bytes and c is even
+            T* at = static_cast<T*>(x.p) + base + row * x.sn + c;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = from_f<T>(f[j]);
-#pragma unroll
-            for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(at)[j] = reinterpret_cast<const uint4*>(t)[j];
+            for (int i = 0; i < NB; ++i) {
+                alignas(8) T v[2] = {from_f<T>(f[i][2 * h]), from_f<T>(f[i][2 * h + 1])};
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(at + 8 * i) = *reinterpret_cast<const uint32_t*>(v);
+                else *reinterpret_cast<uint2*>(at + 8 * i) = *reinterpret_cast<const uint2*>(v);
+            }
         } else {
+            float* at32 = x32 ? x32 + base32 + (int64_t)row * width + c : nullptr;
+            T* at = x32 ? nullptr : static_cast<T*>(x.p) + base + row * x.sn + c;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c0 + c + j < width) at[j] = from_f<T>(f[j]);
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    if (c + 8 * i + y < width) {
+                        if (x32) at32[8 * i + y] = f[i][2 * h + y];
+                        else at[8 * i + y] = from_f<T>(f[i][2 * h + y]);
+                    }
         }
     }
 }
@@ -469,22 +526,18 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     Smem& sm = *reinterpret_cast<Smem*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int rb = warp & 3, hf = warp >> 2;  // 16 tokens, half of d
-    const int64_t chunk = blockIdx.x, bh = chunk / p.nc;
-    const int c = (int)(chunk % p.nc), b = (int)(bh / p.H), h = (int)(bh % p.H), n0 = c * kDeltaC;
+    const unsigned chunk32 = blockIdx.x, bh32 = chunk32 / (unsigned)p.nc;  // (the grid fits 31 bits)
+    const int64_t chunk = chunk32, bh = bh32;
+    const int c = (int)(chunk32 - bh32 * p.nc), b = (int)(bh32 / (unsigned)p.H), h = (int)(bh32 - b * (unsigned)p.H), n0 = c * kDeltaC;
     const int rows = min(kDeltaC, p.N - n0);
     const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
     const int64_t at32 = bh * p.N;  // rows of the gradients per state head
     const bool any = p.gates[chunk].any != 0;
 
-    if (!any) {  // zeros
-        float* zero = &sm.u.rows[0][0];
-        for (int i = tid; i < kDeltaC * (DP + 4); i += 256) zero[i] = 0.f;
-        __syncthreads();
-        store_rows<T, 256>(zero, DP + 4, DP, p.dq, tensor_base(p.dq, b, h), p.dq32, at32 * p.d, n0, rows, 0, p.d, tid);
-        store_rows<T, 256>(zero, DP + 4, DP, p.dk, tensor_base(p.dk, b, h), p.dk32, at32 * p.d, n0, rows, 0, p.d, tid);
-        for (int eb = 0; eb < ncb; ++eb)
-            store_rows<T, 256>(zero, DP + 4, kDeltaCols, p.dv, tensor_base(p.dv, b, h), p.dv32, at32 * p.e, n0, rows,
-                               eb * kDeltaCols, p.e, tid);
+    if (!any) {
+        zero_rows<T>(p.dq, tensor_base(p.dq, b, h), p.dq32, at32 * p.d, n0, rows, p.d, tid);
+        zero_rows<T>(p.dk, tensor_base(p.dk, b, h), p.dk32, at32 * p.d, n0, rows, p.d, tid);
+        zero_rows<T>(p.dv, tensor_base(p.dv, b, h), p.dv32, at32 * p.e, n0, rows, p.e, tid);
         if (tid < rows) {
             p.dbeta[at32 + n0 + tid] = 0.f;
             if (p.dlg) p.dlg[at32 + n0 + tid] = 0.f;
@@ -492,6 +545,8 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
         return;
     }
 
+    bool direct = false;  // bf16: tiles straight to shared memory
+    if constexpr (NIN == 1) direct = p.k.vec && p.q.vec && p.v.vec && p.g.vec && p.d % 8 == 0 && p.e % 8 == 0;
     auto start = [&](int eb) {  // the planes of a block of value columns
         auto& in = sm.u.in[eb % Smem::kBufs];
         const int64_t at = chunk * 2 * ncb + 2 * eb;
@@ -499,20 +554,27 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
         async16<256>(in.G, p.dS + at * (Smem::kState / 2), Smem::kState, tid);
         async16<256>(in.W, p.W + at * (Smem::kCol / 2), Smem::kCol, tid);
         async16<256>(in.Z, p.Z + at * (Smem::kCol / 2), Smem::kCol, tid);
+        if (direct) {
+            async_tile<T, kDeltaCols, 256>(in.dO, p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
+            async_tile<T, kDeltaCols, 256>(in.v, p.v, tensor_base(p.v, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
+        }
     };
     async16<256>(reinterpret_cast<unsigned char*>(&sm.s), reinterpret_cast<const unsigned char*>(p.gates + chunk), sizeof(Gates), tid);
+    if (direct) {
+        async_tile<T, DP, 256>(sm.k, p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, tid);
+        async_tile<T, DP, 256>(sm.q, p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, tid);
+    }
     start(0);
     if (Smem::kBufs == 2 && ncb > 1) start(1);
     const Gates& s = sm.s;
-    {
-        TileRegs<T, DP, 256> k, q;
-        k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, tid);
-        q.issue(p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, tid);
-        if (tid < kDeltaC) sm.vdv[tid] = sm.wz[tid] = 0.f;
-        async_wait();
-        __syncthreads();
-        k.template store_planes<NIN>(sm.k, s.live, tid);
-        q.template store_planes<NIN>(sm.q, s.live, tid);
+    async_wait();
+    __syncthreads();
+    if (!direct) {
+        load_tile<T, DP, NIN, 256>(sm.k, p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, s.live, tid);
+        load_tile<T, DP, NIN, 256>(sm.q, p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, s.live, tid);
+    } else if (!s.full) {
+        clear_dead<DP, 256>(sm.k, s.live, tid);
+        clear_dead<DP, 256>(sm.q, s.live, tid);
     }
 
     float dq[NB][4], dk1[NB][4], dk2[NB][4], D[8][4];
@@ -524,23 +586,30 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     for (int n = 0; n < 8; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) D[n][i] = 0.f;  // dO W^T (hf = 0) or Z W^T (hf = 1), rows 16 rb ..
-    float gs = 0.f;
+    // diagonals: Z V^T of these tokens (hf = 0), S0^T G of a group of 16 columns (hf = 1, rb < 2)
+    float ex[2][4];
+    zero_acc<2>(ex);
 
     for (int eb = 0; eb < ncb; ++eb) {
         auto& in = sm.u.in[eb % Smem::kBufs];
-        {
-            TileRegs<T, kDeltaCols, 256> x, v;
-            x.issue(p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
-            v.issue(p.v, tensor_base(p.v, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
-            if (eb >= Smem::kBufs) start(eb);
-            x.template store_planes<NIN>(in.dO, s.live, tid);
-            v.template store_planes<NIN>(in.v, s.live, tid);
+        if (eb >= Smem::kBufs) {
+            __syncthreads();  // the block before has been read
+            start(eb);
+        }
+        if (!direct) {
+            load_tile<T, kDeltaCols, NIN, 256>(in.dO, p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, p.N, s.live, tid);
+            load_tile<T, kDeltaCols, NIN, 256>(in.v, p.v, tensor_base(p.v, b, h), n0, eb * kDeltaCols, p.e, p.N, s.live, tid);
         }
         async_wait();
+        if (direct && !s.full) {
+            __syncthreads();
+            clear_dead<kDeltaCols, 256>(in.dO, s.live, tid);
+            clear_dead<kDeltaCols, 256>(in.v, s.live, tid);
+        }
         __syncthreads();
         const uint32_t S0 = smem_addr(in.S0) + lane * 16, G = smem_addr(in.G) + lane * 16;
         const uint32_t W = smem_addr(in.W) + lane * 16, Z = smem_addr(in.Z) + lane * 16;
-        const uint32_t dO = smem_addr(in.dO);
+        const uint32_t dO = smem_addr(in.dO), V = smem_addr(in.v);
 #pragma unroll
         for (int cw = 0; cw < 2; ++cw) {  // 16 value columns: one k step
             uint32_t ao[NIN][4], aw[NX][4], az[NX][4];
@@ -590,71 +659,52 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
                     mma_pair<NX, NX, NX>(D[2 * jb], D[2 * jb + 1], az, b0, b1);
                 }
             }
-        }
-        {  // dv = beta Z and the row sums W.Z, v.dv: warp (rb, hf) has tokens 16 rb + 8 hf .., lanes as in an 8 x 8 matrix
-            const int tok = 16 * rb + 8 * hf + 2 * t;
-            const float2 be = *reinterpret_cast<const float2*>(&s.beta[tok]);
-            float2 wz = make_float2(0.f, 0.f), vdv = wz;
-#pragma unroll
-            for (int cm = 0; cm < 4; ++cm) {  // value columns 8 cm + g
-                float2 z = make_float2(0.f, 0.f), w = z, v = z;
-                const int off = (hf * 2 + (cm & 1)) * 128 + lane * 4;
-#pragma unroll
-                for (int pl = 0; pl < NX; ++pl) {
-                    const int tile = (((cm >> 1) * 4 + rb) * NX + pl) * 512 + off;
-                    const float2 x = unpack_bf16(*reinterpret_cast<const uint32_t*>(in.Z + tile));
-                    const float2 y = unpack_bf16(*reinterpret_cast<const uint32_t*>(in.W + tile));
-                    z.x += x.x; z.y += x.y;
-                    w.x += y.x; w.y += y.y;
-                }
+            if (hf == 0) {
+                uint32_t b0[NIN][2], b1[NIN][2];
 #pragma unroll
                 for (int pl = 0; pl < NIN; ++pl) {
-                    const unsigned char* at = in.v + pl * kGTile + 2 * g;
-                    v.x += bf16_at(at + tile_off<kDeltaCols>(tok, cm));
-                    v.y += bf16_at(at + tile_off<kDeltaCols>(tok + 1, cm));
+                    uint32_t r[4];
+                    b_rows<kDeltaCols>(r, V + pl * kGTile, 16 * rb, cw, lane);
+                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
                 }
-                wz.x = fmaf(w.x, z.x, wz.x);
-                wz.y = fmaf(w.y, z.y, wz.y);
-                z.x *= be.x;
-                z.y *= be.y;
-                vdv.x = fmaf(z.x, v.x, vdv.x);
-                vdv.y = fmaf(z.y, v.y, vdv.y);
-                sm.dv[tok][8 * cm + g] = z.x;
-                sm.dv[tok + 1][8 * cm + g] = z.y;
+                mma_pair<NX, NIN, NX>(ex[0], ex[1], az, b0, b1);
             }
+            if (hf == 1 && rb == cw) {
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                wz.x += __shfl_xor_sync(0xffffffffu, wz.x, o);
-                wz.y += __shfl_xor_sync(0xffffffffu, wz.y, o);
-                vdv.x += __shfl_xor_sync(0xffffffffu, vdv.x, o);
-                vdv.y += __shfl_xor_sync(0xffffffffu, vdv.y, o);
-            }
-            if (lane < 4) {  // (these tokens are this warp's alone)
-                sm.wz[tok] += wz.x;
-                sm.wz[tok + 1] += wz.y;
-                sm.vdv[tok] += vdv.x;
-                sm.vdv[tok + 1] += vdv.y;
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    uint32_t a[NX][4], b0[NX][2], b1[NX][2];
+#pragma unroll
+                    for (int pl = 0; pl < NX; ++pl) {
+                        uint32_t r[4];
+                        ldm(a[pl], S0 + ((cw * (DP / 16) + kk) * NX + pl) * 512);
+                        ldm(r, G + ((cw * (DP / 16) + kk) * NX + pl) * 512);
+                        b0[pl][0] = r[0]; b0[pl][1] = r[2]; b1[pl][0] = r[1]; b1[pl][1] = r[3];
+                    }
+                    mma_pair<NX, NX, NX>(ex[0], ex[1], a, b0, b1);
+                }
             }
         }
-        // <G, S0>
-        for (int i = tid; i < 2 * DP / 16 * 128; i += 256) {
-            const int tile = i >> 7, off = (i & 127) * 4;
-            float2 x = make_float2(0.f, 0.f), y = x;
-#pragma unroll
-            for (int pl = 0; pl < NX; ++pl) {
-                const float2 u0 = unpack_bf16(*reinterpret_cast<const uint32_t*>(in.S0 + (tile * NX + pl) * 512 + off));
-                const float2 u1 = unpack_bf16(*reinterpret_cast<const uint32_t*>(in.G + (tile * NX + pl) * 512 + off));
-                x.x += u0.x; x.y += u0.y;
-                y.x += u1.x; y.y += u1.y;
-            }
-            gs = fmaf(x.x, y.x, gs);
-            gs = fmaf(x.y, y.y, gs);
-        }
-        __syncthreads();
-        store_rows<T, 256>(&sm.dv[0][0], kDeltaCols + 4, kDeltaCols, p.dv, tensor_base(p.dv, b, h), p.dv32, at32 * p.e, n0, rows,
-                           eb * kDeltaCols, p.e, tid);
-        if (eb + 1 < ncb) __syncthreads();  // (a later block writes dv and the buffers again)
     }
+    // diagonals: lanes with g = 2 t or 2 t + 1 have them
+    const bool d0 = g == 2 * t, d1_ = g == 2 * t + 1;
+    if (hf) {
+#pragma unroll
+        for (int jb = 0; jb < 4; ++jb)  // W.Z
+            if (jb == rb && (d0 || d1_)) {
+                sm.wz[16 * rb + g] = d0 ? D[2 * jb][0] : D[2 * jb][1];
+                sm.wz[16 * rb + 8 + g] = d0 ? D[2 * jb + 1][2] : D[2 * jb + 1][3];
+            }
+    } else if (d0 || d1_) {  // v.dv
+        sm.vdv[16 * rb + g] = s.beta[16 * rb + g] * (d0 ? ex[0][0] : ex[0][1]);
+        sm.vdv[16 * rb + 8 + g] = s.beta[16 * rb + 8 + g] * (d0 ? ex[1][2] : ex[1][3]);
+    }
+    if (hf == 1 && rb < 2) {  // <G, S0>
+        float gs = d0 ? ex[0][0] + ex[1][2] : d1_ ? ex[0][1] + ex[1][3] : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) gs += __shfl_xor_sync(0xffffffffu, gs, o);
+        if (lane == 0) sm.gs[rb] = gs;
+    }
+    __syncthreads();  // the blocks of value columns have been read: D1 and D2 take their place
 
     {  // D1 or D2 as planes
         unsigned char* dst = (hf ? sm.u.sc.d2 : sm.u.sc.d1) + lane * 4;
@@ -771,34 +821,15 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
             if (t == 0) sm.qdq[hf][i] = qd[x];
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) gs += __shfl_xor_sync(0xffffffffu, gs, o);
-    if (lane == 0) sm.gs[warp] = gs;
-    // dq, then dk, through shared memory to whole rows
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float2 f;
-                if (which) f = make_float2(dk1[n][2 * x], dk1[n][2 * x + 1]);
-                else f = make_float2(dq[n][2 * x], dq[n][2 * x + 1]);
-                *reinterpret_cast<float2*>(&sm.u.rows[16 * rb + 8 * x + g][(hf * NB + n) * 8 + 2 * t]) = f;
-            }
-        __syncthreads();
-        if (which)
-            store_rows<T, 256>(&sm.u.rows[0][0], DP + 4, DP, p.dk, tensor_base(p.dk, b, h), p.dk32, at32 * p.d, n0, rows, 0, p.d, tid);
-        else
-            store_rows<T, 256>(&sm.u.rows[0][0], DP + 4, DP, p.dq, tensor_base(p.dq, b, h), p.dq32, at32 * p.d, n0, rows, 0, p.d, tid);
-    }
+    store_grad<T, NB>(dq, p.dq, tensor_base(p.dq, b, h), p.dq32, at32 * p.d, n0 + 16 * rb, n0 + rows, 8 * hf * NB, p.d, lane);
+    store_grad<T, NB>(dk1, p.dk, tensor_base(p.dk, b, h), p.dk32, at32 * p.d, n0 + 16 * rb, n0 + rows, 8 * hf * NB, p.d, lane);
+    __syncthreads();
     if (warp == 0) {
         // suffix sums over the chunk (two tokens per lane) on top of <G, S'>
         const int i0 = 2 * lane, i1 = i0 + 1;
         const float x0 = sm.qdq[0][i0] + sm.qdq[1][i0] - sm.vdv[i0], x1 = sm.qdq[0][i1] + sm.qdq[1][i1] - sm.vdv[i1];
         float end = 0.f, k01 = sm.kdk[0][i0] + sm.kdk[1][i0] + sm.kdk[0][i1] + sm.kdk[1][i1];
-        for (int w = 0; w < 8; ++w) end += sm.gs[w];
+        end = sm.gs[0] + sm.gs[1];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) k01 += __shfl_xor_sync(0xffffffffu, k01, o);
         end = s.eC * end + k01;

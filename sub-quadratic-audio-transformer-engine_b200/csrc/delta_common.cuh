@@ -550,6 +550,23 @@ __device__ __forceinline__ void get_a(uint32_t (&a)[NX][4], const unsigned char*
         a[pl][0] = x.x; a[pl][1] = x.y; a[pl][2] = x.z; a[pl][3] = x.w;
     }
 }
+// The values that an A operand's planes stand for, as two accumulator blocks.
+template <int NX>
+__device__ __forceinline__ void from_a(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NX][4]) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        float2 x = unpack_bf16(a[NX - 1][m]);
+#pragma unroll
+        for (int pl = NX - 2; pl >= 0; --pl) {
+            const float2 y = unpack_bf16(a[pl][m]);
+            x.x += y.x;
+            x.y += y.y;
+        }
+        float(&c)[4] = m < 2 ? c0 : c1;
+        c[2 * (m & 1)] = x.x;
+        c[2 * (m & 1) + 1] = x.y;
+    }
+}
 // Two neighbouring float32 accumulator blocks from shared memory.
 __device__ __forceinline__ void get_acc2(float (&c0)[4], float (&c1)[4], const float4* at, int lane) {
     const float4 x = at[lane], y = at[32 + lane];

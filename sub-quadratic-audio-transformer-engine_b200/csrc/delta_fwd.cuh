@@ -44,9 +44,9 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
     extern __shared__ __align__(128) unsigned char raw[];
     PrepSmem<T, DP>& sm = *reinterpret_cast<PrepSmem<T, DP>*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int64_t chunk = blockIdx.x;  // bh * nc + c
-    const int64_t bh = chunk / p.nc;
-    const int c = (int)(chunk % p.nc), b = (int)(bh / p.H), h = (int)(bh % p.H), n0 = c * kDeltaC;
+    const unsigned chunk32 = blockIdx.x, bh32 = chunk32 / (unsigned)p.nc;  // bh * nc + c (the grid fits 31 bits)
+    const int64_t chunk = chunk32;
+    const int c = (int)(chunk32 - bh32 * p.nc), b = (int)(bh32 / (unsigned)p.H), h = (int)(bh32 - b * (unsigned)p.H), n0 = c * kDeltaC;
     {
         TileRegs<T, DP, 128> k, q;
         k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, tid);
@@ -496,8 +496,10 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
     ChainSmem<T, DP>& sm = *reinterpret_cast<ChainSmem<T, DP>*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
-    const int64_t bh = blockIdx.x / ncb;
-    const int cb = blockIdx.x % ncb, b = (int)(bh / p.H), h = (int)(bh % p.H), c0 = cb * kDeltaCols;
+    const unsigned bh32 = blockIdx.x / (unsigned)ncb;
+    const int64_t bh = bh32;
+    const int cb = (int)(blockIdx.x - bh32 * ncb), b = (int)(bh32 / (unsigned)p.H), h = (int)(bh32 - b * (unsigned)p.H);
+    const int c0 = cb * kDeltaCols;
     if (warp < 4) {
         chain_warp<T, DP, OUT, KEEP>(sm, p, warp & 1, warp >> 1, bh, c0 + 16 * (warp >> 1), lane);
     } else if (warp < 8) {
