@@ -510,15 +510,41 @@ int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc&
     return SUBQ_OK;
 }
 
+// Segments of a sequence that are walked side by side when there are few sequences. A walk over n chunks takes n
+// steps of about t = 1.7 us whatever the number of CTAs, up to one CTA per SM. With G segments, a first pass (states
+// only, from the segments' value columns and the d columns of the identity) and the walk itself take n / G steps each,
+// times the waves of their CTAs, and the join about 2 us a segment and 8 us of launches. G is the count with the
+// least such time, taken where that is at least a fifth below the single walk's (B = 1, H = 4, N = 4096, d = e = 64:
+// G = 9, 162 -> 76 us measured; B = 8, H = 12: one).
+struct DeltaSplit {
+    int nseg, chunks;
+};
+DeltaSplit delta_split(const subq::DeltaParams& p) {
+    const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + 31) / 32, ndb = (p.d + 31) / 32;
+    constexpr double kStep = 1.7, kJoin = 2.0, kLaunch = 8.0;
+    auto waves = [](int64_t ctas) { return (double)((ctas + 147) / 148); };
+    double best = 0.8 * p.nc * kStep * waves(bh * ncb);
+    DeltaSplit s = {1, p.nc};
+    for (int g = 2; g <= 64 && 2 * g <= p.nc; ++g) {
+        const int chunks = (p.nc + g - 1) / g;
+        if ((p.nc + chunks - 1) / chunks != g) continue;  // (the same split with fewer segments)
+        const double t = chunks * kStep * (waves(bh * g * ncb) + waves(bh * (g - 1) * (ncb + ndb))) + g * kJoin + kLaunch;
+        if (t < best) best = t, s = {g, chunks};
+    }
+    return s;
+}
+
 struct DeltaBytes {
     size_t gates, Y, P, S0, W;  // the handover's parts
+    size_t seg_S, seg_M;        // workspace
 };
 DeltaBytes delta_bytes(const subq::DeltaParams& p, int dtype) {
     const size_t nx = dtype == SUBQ_FP32 ? 3 : 2, chunks = (size_t)p.B * p.H * p.nc;
     const size_t ncw = 2 * ((p.e + subq::kDeltaCols - 1) / subq::kDeltaCols), dp = p.d <= 64 ? 64 : 128;
     const size_t mat = align_up(chunks * nx * subq::kYBlocks * 512);
+    const size_t slots = (size_t)p.B * p.H * (delta_split(p).nseg - 1) * p.d * sizeof(float);
     return {align_up(chunks * sizeof(subq::DeltaGates)), mat, mat, align_up(chunks * ncw * (dp / 16) * nx * 512),
-            align_up(chunks * ncw * 4 * nx * 512)};
+            align_up(chunks * ncw * 4 * nx * 512), align_up(slots * p.e), align_up(slots * p.d)};
 }
 
 void delta_handover(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
@@ -527,6 +553,14 @@ void delta_handover(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
     p.P = p.Y + n.Y;
     p.S0 = p.P + n.P;
     p.W = p.S0 + n.S0;
+}
+
+void delta_segments(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
+    const DeltaSplit s = delta_split(p);
+    p.nseg = s.nseg;
+    p.seg_chunks = s.chunks;
+    p.seg_S = static_cast<float*>(at);
+    p.seg_M = reinterpret_cast<float*>(static_cast<char*>(at) + n.seg_S);
 }
 
 int fill_delta_fwd(const subq_delta_fwd_args* a, subq::DeltaParams& p, int& path) {
@@ -594,7 +628,7 @@ DeltaBwdBytes delta_bwd_bytes(const subq::DeltaParams& p, int dtype, bool handov
     n.dq = p.q.group > 1 ? align_up(tokens * p.d * 4) : 0;
     n.dk = p.k.group > 1 ? align_up(tokens * p.d * 4) : 0;
     n.dv = p.v.group > 1 ? align_up(tokens * p.e * 4) : 0;
-    n.total = n.fwd.S0 + n.fwd.W + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.gates + n.fwd.Y + n.fwd.P + n.fwd.S0 + n.fwd.W);
+    n.total = n.fwd.S0 + n.fwd.W + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.gates + n.fwd.Y + n.fwd.P + n.fwd.S0 + n.fwd.W + n.fwd.seg_S + n.fwd.seg_M);
     return n;
 }
 
@@ -610,9 +644,9 @@ size_t subq_delta_handover_bytes(const subq_delta_desc* d) {
 size_t subq_delta_fwd_workspace_bytes(const subq_delta_fwd_args* a) {
     subq::DeltaParams p;
     int path;
-    if (fill_delta_fwd(a, p, path) != SUBQ_OK || path != SUBQ_PATH_CHUNKED || a->handover) return 0;
+    if (fill_delta_fwd(a, p, path) != SUBQ_OK || path != SUBQ_PATH_CHUNKED) return 0;
     const DeltaBytes n = delta_bytes(p, a->desc.dtype);
-    return n.gates + n.Y + n.P;
+    return n.seg_S + n.seg_M + (a->handover ? 0 : n.gates + n.Y + n.P);
 }
 
 size_t subq_delta_bwd_workspace_bytes(const subq_delta_bwd_args* a) {
@@ -637,17 +671,19 @@ int subq_delta_fwd(const subq_delta_fwd_args* a) {
         err = subq::launch_delta_step(p, a->desc.dtype, st);
     } else {
         const DeltaBytes n = delta_bytes(p, a->desc.dtype);
+        const size_t segs = n.seg_S + n.seg_M;
+        if ((rc = check_workspace(a->workspace, a->workspace_bytes, segs + (a->handover ? 0 : n.gates + n.Y + n.P)))) return rc;
+        delta_segments(p, n, a->workspace);
         if (a->handover) {
             if (reinterpret_cast<uintptr_t>(a->handover) % kAlign != 0)
                 return fail(SUBQ_ERR_WORKSPACE, "handover must be 256-byte aligned");
             delta_handover(p, n, a->handover);
         } else {
-            if ((rc = check_workspace(a->workspace, a->workspace_bytes, n.gates + n.Y + n.P))) return rc;
-            delta_handover(p, n, a->workspace);
+            delta_handover(p, n, static_cast<char*>(a->workspace) + segs);
             p.S0 = p.W = nullptr;  // not kept
         }
         err = subq::launch_delta_fwd(p, a->desc.dtype, st);
-        launches = 2;
+        launches = p.nseg > 1 ? 4 : 2;
     }
     if (err != cudaSuccess) return fail_cuda(err, "subq_delta_fwd launch");
     g_last_path = path;
@@ -690,9 +726,10 @@ int subq_delta_bwd(const subq_delta_bwd_args* a) {
             return fail(SUBQ_ERR_WORKSPACE, "handover must be 256-byte aligned");
         delta_handover(p, n.fwd, const_cast<void*>(a->handover));
     } else {
-        delta_handover(p, n.fwd, at);
+        delta_segments(p, n.fwd, at);
+        delta_handover(p, n.fwd, at + n.fwd.seg_S + n.fwd.seg_M);
         err = subq::launch_delta_fwd(p, dt, st);  // (o is null: states and corrections only)
-        first = 2;
+        first = p.nseg > 1 ? 4 : 2;
     }
     if (err == cudaSuccess) err = subq::launch_delta_bwd(p, dt, st, &launches);
     if (err != cudaSuccess) return fail_cuda(err, "subq_delta_bwd launch");

@@ -56,6 +56,10 @@ struct DeltaParams {
     unsigned char* P;   // scale G o (Q K^T), likewise
     unsigned char* S0;  // [B * H][nc][ep / 16][dp / 16][NX][512], or null (not stored)
     unsigned char* W;   // [B * H][nc][ep / 16][4][NX][512], or null
+    // segments of a sequence walked side by side (few sequences): 1, or more than 1 with `seg_S` and `seg_M`
+    int nseg, seg_chunks;
+    float* seg_S;  // [B * H][nseg - 1][d, e]: state after a segment
+    float* seg_M;  // [B * H][nseg - 1][d, d]: what a segment does to the state before it
     // backward
     DeltaTensor g, dq, dk, dv;
     unsigned char* dS;  // gradient of the state after each chunk, like S0
@@ -451,6 +455,16 @@ __device__ __forceinline__ void copy16(unsigned char* dst, const unsigned char* 
     for (int i = tid * 16; i < bytes; i += NT * 16)
         *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
 }
+
+// What one CTA of a walk has to do: chunks [begin, end) of a sequence, 32 columns from c0.
+struct WalkJob {
+    int64_t bh;
+    int b, h, begin, end, cb, c0;
+    bool ident;        // columns of the identity (V = 0) in place of value columns: the walk then gives seg_M's columns
+    const float* in;   // state before, [d, ld], or null (0)
+    float* out;        // state after, or null
+    int ld;
+};
 
 __device__ __forceinline__ int64_t tensor_base(const DeltaTensor& x, int b, int h) {
     return b * x.sb + (h / x.group) * x.sh;

@@ -221,7 +221,7 @@ struct ChainSmem {
 
 // One warp of a chain pair: half `A` of d of S^T in its accumulators; R and W of its token blocks.
 template <typename T, int DP, bool OUT, bool KEEP>
-__device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int col0, int lane) {
+__device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
     constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP>::kStages;
     constexpr int NH = DP / 16;  // 8-column blocks of half of d
     constexpr bool kShared = ChainSmem<T, DP>::kShared;
@@ -229,13 +229,13 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
     float S[NH][4];
-    const float* S_in = p.S_in ? p.S_in + bh * p.d * p.e : nullptr;
+    const int col0 = job.c0 + 16 * pair;
 #pragma unroll
     for (int n = 0; n < NH; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
-            S[n][i] = (S_in && d < p.d && col < p.e) ? S_in[(int64_t)d * p.e + col] : 0.f;
+            S[n][i] = job.ident ? (d == col ? 1.f : 0.f) : (job.in && d < p.d && col < job.ld) ? job.in[(int64_t)d * job.ld + col] : 0.f;
         }
     auto put_state = [&]() {
 #pragma unroll
@@ -247,7 +247,7 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
     };
     put_state();
     __syncthreads();
-    for (int c = 0; c < p.nc; ++c) {
+    for (int c = job.begin; c < job.end; ++c) {
         if (NST == 1) __syncthreads();  // the chunk is loaded
         auto& st = sm.st[c % NST];
         const Gates& s = st.s;
@@ -355,27 +355,27 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
         }
         __syncthreads();
     }
-    if (p.S_out) {
-        float* S_out = p.S_out + bh * p.d * p.e;
+    if (job.out) {
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
-                if (d < p.d && col < p.e) S_out[(int64_t)d * p.e + col] = S[n][i];
+                if (d < p.d && col < job.ld) job.out[(int64_t)d * job.ld + col] = S[n][i];
             }
     }
 }
 
 // One warp of an output pair: the outputs of 16 columns for its token blocks, and its share of the planes.
 template <typename T, int DP, bool OUT, bool KEEP>
-__device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int cb, int lane) {
+__device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
     constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP>::kStages;
     const int g = lane >> 2, t = lane & 3;
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
-    const int b = (int)(bh / p.H), h = (int)(bh % p.H), ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
-    T* o = OUT ? static_cast<T*>(p.o.p) + tensor_base(p.o, b, h) : nullptr;
+    const int64_t bh = job.bh;
+    const int cb = job.cb, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    T* o = OUT ? static_cast<T*>(p.o.p) + tensor_base(p.o, job.b, job.h) : nullptr;
     constexpr bool kShared = ChainSmem<T, DP>::kShared;
     constexpr int kPitch = ChainSmem<T, DP>::kOutPitch, kPieces = 16 * sizeof(T) / 16;  // bytes of a staged row, its 16-byte pieces
     const int col0 = cb * kDeltaCols + 16 * pair, width = min(16, p.e - col0);
@@ -451,9 +451,9 @@ __device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaPar
         }
     };
     __syncthreads();
-    for (int c = 0; c < p.nc; ++c) {
+    for (int c = job.begin; c < job.end; ++c) {
         if (NST == 1) __syncthreads();
-        if (OUT && kLag && c > 0) finish(c - 1);
+        if (OUT && kLag && c > job.begin) finish(c - 1);
         auto& st = sm.st[c % NST];
         const Gates& s = st.s;
         if (s.any) {
@@ -484,7 +484,7 @@ __device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaPar
         if (OUT && !kLag) finish(c);
         __syncthreads();
     }
-    if (OUT && kLag) finish(p.nc - 1);
+    if (OUT && kLag) finish(job.end - 1);
 }
 
 // OUT: writes o. KEEP: writes the planes of S0 and W that the backward reads.
@@ -495,20 +495,47 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
     extern __shared__ __align__(128) unsigned char raw[];
     ChainSmem<T, DP>& sm = *reinterpret_cast<ChainSmem<T, DP>*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
-    const unsigned bh32 = blockIdx.x / (unsigned)ncb;
-    const int64_t bh = bh32;
-    const int cb = (int)(blockIdx.x - bh32 * ncb), b = (int)(bh32 / (unsigned)p.H), h = (int)(bh32 - b * (unsigned)p.H);
-    const int c0 = cb * kDeltaCols;
+    // (sequence, segment, block of columns), the last fastest. States only (neither OUT nor KEEP): the first
+    // nseg - 1 segments, with the identity's columns after the value columns
+    constexpr bool kStates = !OUT && !KEEP;
+    const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols, ncols = ncb + (kStates ? (p.d + kDeltaCols - 1) / kDeltaCols : 0);
+    const int nseg = kStates ? p.nseg - 1 : p.nseg;
+    const unsigned sq = blockIdx.x / (unsigned)ncols, bh32 = sq / (unsigned)nseg;
+    const int seg = (int)(sq - bh32 * nseg);
+    WalkJob job;
+    job.bh = bh32;
+    job.b = (int)(bh32 / (unsigned)p.H);
+    job.h = (int)(bh32 - job.b * (unsigned)p.H);
+    job.cb = (int)(blockIdx.x - sq * ncols);
+    job.ident = kStates && job.cb >= ncb;
+    job.c0 = (job.ident ? job.cb - ncb : job.cb) * kDeltaCols;
+    job.begin = seg * p.seg_chunks;
+    job.end = min(p.nc, job.begin + p.seg_chunks);
+    job.ld = job.ident ? p.d : p.e;
+    const int64_t before = job.bh * (p.nseg - 1) + seg;  // the segment's slot in seg_S and seg_M
+    if (kStates) {
+        job.in = seg == 0 && !job.ident && p.S_in ? p.S_in + job.bh * p.d * p.e : nullptr;
+        job.out = job.ident ? p.seg_M + before * p.d * p.d : p.seg_S + before * p.d * p.e;
+    } else {
+        job.in = seg ? p.seg_S + (before - 1) * p.d * p.e : p.S_in ? p.S_in + job.bh * p.d * p.e : nullptr;
+        job.out = seg + 1 == nseg && p.S_out ? p.S_out + job.bh * p.d * p.e : nullptr;
+    }
     if (warp < 4) {
-        chain_warp<T, DP, OUT, KEEP>(sm, p, warp & 1, warp >> 1, bh, c0 + 16 * (warp >> 1), lane);
+        chain_warp<T, DP, OUT, KEEP>(sm, p, job, warp & 1, warp >> 1, lane);
     } else if (warp < 8) {
-        output_warp<T, DP, OUT, KEEP>(sm, p, warp & 1, (warp >> 1) & 1, bh, cb, lane);
+        output_warp<T, DP, OUT, KEEP>(sm, p, job, warp & 1, (warp >> 1) & 1, lane);
     } else {  // ---------------------------------------------------------- loads
         // the loads of a chunk are in flight for a whole iteration or two
         const int lt = tid - 256;
+        const int64_t bh = job.bh;
+        const int b = job.b, h = job.h, begin = job.begin, end = job.end, c0 = job.c0;
         const Gates* gates = p.gates + bh * p.nc;
         const int64_t kb = tensor_base(p.k, b, h), qb = tensor_base(p.q, b, h), vb = tensor_base(p.v, b, h);
+        if (job.ident) {  // V is 0 in every stage
+            for (int i = 0; i < NST; ++i)
+                for (int x = lt * 16; x < (int)sizeof(sm.st[i].v); x += 128 * 16)
+                    *reinterpret_cast<uint4*>(sm.st[i].v + x) = make_uint4(0, 0, 0, 0);
+        }
         constexpr int kMat = NX * kYBlocks * 512;
         const unsigned char* Y = p.Y + bh * p.nc * kMat;
         const unsigned char* P = p.P + bh * p.nc * kMat;
@@ -517,17 +544,17 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
         if (async) {
             // bf16: asynchronous copies, chunk c + kAhead started while c is computed
             constexpr int kAhead = NST > 2 ? NST - 2 : 1;
-            int any_next = gates[0].any;
+            int any_next = gates[begin].any;
             auto start = [&](int c) {
-                if (c < p.nc) {
+                if (c < end) {
                     const int any = any_next;
-                    any_next = c + 1 < p.nc ? gates[c + 1].any : 0;
+                    any_next = c + 1 < end ? gates[c + 1].any : 0;
                     auto& st = sm.st[c % NST];
                     async16<128>(reinterpret_cast<unsigned char*>(&st.s), reinterpret_cast<const unsigned char*>(gates + c), sizeof(Gates), lt);
                     if (any) {
                         const int n0 = c * kDeltaC;
                         async_tile<T, DP, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, lt);
-                        async_tile<T, kDeltaCols, 128>(st.v, p.v, vb, n0, c0, p.e, p.N, lt);
+                        if (!job.ident) async_tile<T, kDeltaCols, 128>(st.v, p.v, vb, n0, c0, p.e, p.N, lt);
                         async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
                         if (OUT) {
                             async_tile<T, DP, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, lt);
@@ -539,7 +566,7 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
             };
             auto finish = [&](int c) {  // every copy up to chunk c's is there
                 async_wait_but<(kAhead > 1 ? kAhead - 1 : 0)>();
-                if (c >= p.nc) return;
+                if (c >= end) return;
                 bar_sync(3, 128);
                 auto& st = sm.st[c % NST];
                 if (st.s.any && !st.s.full) {
@@ -548,10 +575,10 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
                     clear_dead<kDeltaCols, 128>(st.v, st.s.live, lt);
                 }
             };
-            for (int c = 0; c < kAhead; ++c) start(c);
-            finish(0);
+            for (int c = 0; c < kAhead; ++c) start(begin + c);
+            finish(begin);
             __syncthreads();
-            for (int c = 0; c < p.nc; ++c) {
+            for (int c = begin; c < end; ++c) {
                 start(c + kAhead);
                 finish(c + 1);
                 __syncthreads();
@@ -560,14 +587,14 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
         } else {
             if constexpr (NST == 1) {  // (no room for a second chunk: each tile is loaded when its turn comes)
                 __syncthreads();
-                for (int c = 0; c < p.nc; ++c) {
+                for (int c = begin; c < end; ++c) {
                     auto& st = sm.st[0];
                     copy16<128>(reinterpret_cast<unsigned char*>(&st.s), reinterpret_cast<const unsigned char*>(gates + c), sizeof(Gates), lt);
                     bar_sync(3, 128);
                     if (st.s.any) {
                         const int n0 = c * kDeltaC;
                         load_tile<T, DP, NIN, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, st.s.live, lt);
-                        load_tile<T, kDeltaCols, NIN, 128>(st.v, p.v, vb, n0, c0, p.e, p.N, st.s.live, lt);
+                        if (!job.ident) load_tile<T, kDeltaCols, NIN, 128>(st.v, p.v, vb, n0, c0, p.e, p.N, st.s.live, lt);
                         async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
                         if (OUT) {
                             load_tile<T, DP, NIN, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, st.s.live, lt);
@@ -582,22 +609,22 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
                 TileRegs<T, DP, 128> k, q;
                 TileRegs<T, kDeltaCols, 128> v;
                 ByteRegs<sizeof(Gates), 128> s;
-                int any = 0, any_next = gates[0].any;  // of the chunk in the registers, and of the one after it
+                int any = 0, any_next = gates[begin].any;  // of the chunk in the registers, and of the one after it
                 auto issue = [&](int c) {
                     any = any_next;
-                    any_next = c + 1 < p.nc ? gates[c + 1].any : 0;
-                    if (c >= p.nc) return;
+                    any_next = c + 1 < end ? gates[c + 1].any : 0;
+                    if (c >= end) return;
                     s.issue(gates + c, lt);
                     if (!any) return;
                     const int n0 = c * kDeltaC;
                     k.issue(p.k, kb, n0, 0, p.d, p.N, lt);
-                    v.issue(p.v, vb, n0, c0, p.e, p.N, lt);
+                    if (!job.ident) v.issue(p.v, vb, n0, c0, p.e, p.N, lt);
                     if (OUT) {
                         q.issue(p.q, qb, n0, 0, p.d, p.N, lt);
                     }
                 };
                 auto store = [&](int c) {
-                    if (c >= p.nc) return;
+                    if (c >= end) return;
                     auto& st = sm.st[c % NST];
                     s.store(&st.s, lt);
                     bar_sync(3, 128);
@@ -605,17 +632,17 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
                     async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
                     if (OUT) async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
                     k.template store_planes<NIN>(st.k, st.s.live, lt);
-                    v.template store_planes<NIN>(st.v, st.s.live, lt);
+                    if (!job.ident) v.template store_planes<NIN>(st.v, st.s.live, lt);
                     if (OUT) {
                         q.template store_planes<NIN>(st.q, st.s.live, lt);
                     }
                 };
-                issue(0);
-                store(0);
-                issue(1);
+                issue(begin);
+                store(begin);
+                issue(begin + 1);
                 async_wait();
                 __syncthreads();
-                for (int c = 0; c < p.nc; ++c) {
+                for (int c = begin; c < end; ++c) {
                     store(c + 1);
                     issue(c + 2);
                     async_wait();
@@ -626,30 +653,79 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
     }
 }
 
+// ------------------------------------------------------------------ segments
+// seg_S[s] <- seg_M[s] S_s + seg_S[s] (what segment s makes of the state before it, S_s), s in order: seg_S[s - 1] is
+// then the state before segment s. A CTA has 16 columns of one sequence; 256 threads, 4 rows x 1 column each per 64 rows.
+__global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
+    extern __shared__ float sm_join[];  // S [d][16], M^T-free copy of M [d][d + 1]
+    float* S = sm_join;
+    float* M = sm_join + p.d * 16;
+    const int ncb = (p.e + 15) / 16;
+    const int64_t bh = blockIdx.x / (unsigned)ncb;
+    const int c0 = (int)(blockIdx.x % (unsigned)ncb) * 16, col = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+    const bool in = c0 + col < p.e;
+    // (the first segment's own state already holds what came before it: its walk started from the initial state)
+    for (int s = 1; s + 1 < p.nseg; ++s) {
+        const float* Ms = p.seg_M + (bh * (p.nseg - 1) + s) * p.d * p.d;
+        const float* before = p.seg_S + (bh * (p.nseg - 1) + s - 1) * p.d * p.e;
+        float* after = p.seg_S + (bh * (p.nseg - 1) + s) * p.d * p.e;
+        if (s == 1)
+            for (int r = r0; r < p.d; r += 16) S[r * 16 + col] = in ? before[r * p.e + c0 + col] : 0.f;
+        for (int i = threadIdx.x; i < p.d * p.d; i += 256) M[(i / p.d) * (p.d + 1) + i % p.d] = Ms[i];
+        __syncthreads();
+        float acc[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = r0 + 16 * k < p.d && in ? after[(r0 + 16 * k) * p.e + c0 + col] : 0.f;
+        for (int x = 0; x < p.d; ++x) {
+            const float v = S[x * 16 + col];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (16 * k < p.d) acc[k] = fmaf(M[min(r0 + 16 * k, p.d - 1) * (p.d + 1) + x], v, acc[k]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (r0 + 16 * k < p.d) {
+                S[(r0 + 16 * k) * 16 + col] = acc[k];
+                if (in) after[(r0 + 16 * k) * p.e + c0 + col] = acc[k];
+            }
+        // (the next M is loaded over the old one after every thread has passed the barrier above)
+    }
+}
+
 template <typename T, int DP>
-cudaError_t chain_t(const DeltaParams& p, unsigned blocks, cudaStream_t st) {
+cudaError_t chain_t(const DeltaParams& p, cudaStream_t st) {
     const size_t smem = sizeof(ChainSmem<T, DP>);
     static_assert(sizeof(ChainSmem<T, DP>) <= 227 * 1024, "shared memory");
-    auto run = [&](auto kernel) {
+    const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + kDeltaCols - 1) / kDeltaCols, ndb = (p.d + kDeltaCols - 1) / kDeltaCols;
+    auto run = [&](auto kernel, int64_t blocks) {
         cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (err != cudaSuccess) return err;
-        kernel<<<blocks, 384, smem, st>>>(p);
+        kernel<<<(unsigned)blocks, 384, smem, st>>>(p);
         return cudaGetLastError();
     };
-    if (!p.o.p) return run(delta_chain_kernel<T, DP, false, true>);
-    if (p.S0) return run(delta_chain_kernel<T, DP, true, true>);
-    return run(delta_chain_kernel<T, DP, true, false>);
+    if (p.nseg > 1) {
+        cudaError_t err = run(delta_chain_kernel<T, DP, false, false>, bh * (p.nseg - 1) * (ncb + ndb));
+        if (err != cudaSuccess) return err;
+        const int join = (p.d * 16 + p.d * (p.d + 1)) * (int)sizeof(float);
+        err = cudaFuncSetAttribute(delta_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, join);
+        if (err != cudaSuccess) return err;
+        delta_join_kernel<<<(unsigned)(bh * ((p.e + 15) / 16)), 256, join, st>>>(p);
+        if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    }
+    if (!p.o.p) return run(delta_chain_kernel<T, DP, false, true>, bh * p.nseg * ncb);
+    if (p.S0) return run(delta_chain_kernel<T, DP, true, true>, bh * p.nseg * ncb);
+    return run(delta_chain_kernel<T, DP, true, false>, bh * p.nseg * ncb);
 }
 
 template <typename T, int DP>
 cudaError_t fwd_t(const DeltaParams& p, cudaStream_t st) {
-    const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
     const size_t prep = sizeof(PrepSmem<T, DP>);
     cudaError_t err = cudaFuncSetAttribute(delta_prep_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prep);
     if (err != cudaSuccess) return err;
-    delta_prep_kernel<T, DP><<<(unsigned)(bh * p.nc), 128, prep, st>>>(p);
+    delta_prep_kernel<T, DP><<<(unsigned)((int64_t)p.B * p.H * p.nc), 128, prep, st>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
-    return chain_t<T, DP>(p, (unsigned)(bh * ncb), st);
+    return chain_t<T, DP>(p, st);
 }
 
 }  // namespace

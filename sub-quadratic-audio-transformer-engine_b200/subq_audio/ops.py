@@ -574,8 +574,7 @@ def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta:
             handover.key = (B, H, N, d, e, q.dtype, q.device)
             if handover.buf is not None:
                 a.handover = handover.buf.data_ptr()
-        if handover is None or handover.buf is None:
-            a.workspace, a.workspace_bytes = _workspace(_capi.delta_fwd_workspace_bytes(a), q.device, keep)
+        a.workspace, a.workspace_bytes = _workspace(_capi.delta_fwd_workspace_bytes(a), q.device, keep)
         _capi.delta_fwd(a)
     return o, S_out
 

@@ -146,6 +146,36 @@ def test_backward(case, carried):
             assert bool((a.transpose(1, 2)[~m] == 0).all()), name
 
 
+LONG = [(1, 2, 2, 1, 2, 3000, 64, 64, "bf16", None), (1, 1, 1, 1, 1, 5001, 64, 96, "fp16", "tail"),
+        (2, 1, 1, 1, 1, 4097, 100, 40, "fp32", "random"), (1, 3, 3, 3, 3, 2950, 128, 128, "bf16", "random")]
+
+
+@pytest.mark.parametrize("case", LONG, ids=["-".join(str(x) for x in c) for c in LONG])
+def test_long_and_few_sequences(case):
+    """Sequences that are cut into segments walked side by side, then joined; the backward from their handover and
+    from its own."""
+    B, H, Hq, Hk, Hv, N, d, e, dtype, mask = case
+    q, k, v, do, beta, lg, S0, dS, m = inputs(B, H, Hq, Hk, Hv, N, d, e, dtype, seed=N, mask=mask)
+    if mask == "random":
+        m[:, 640:1024] = False  # whole chunks, one of them the first of a segment
+    scale = d ** -0.5
+    with torch.no_grad():
+        o_ref, S_ref = ref.forward(q, k, v, beta, lg, m, scale, S0)
+    ho = ops.DeltaHandover()
+    o, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, mask=m, state=S0, return_state=True)
+    assert ops.last_launches() == 4
+    o2, S2 = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, mask=m, state=S0, return_state=True, handover=ho)
+    assert torch.equal(o, o2) and torch.equal(S, S2)
+    assert rel(o, o_ref) < tol(o.dtype, q.dtype) and rel(S, S_ref) < tol(S.dtype, q.dtype)
+    want = ref.gradients(q, k, v, beta, lg, m, scale, S0, do, dS)
+    runs = [ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, mask=m, state=S0, dstate=dS, need_dlog_gamma=True,
+                                     need_dstate=True, handover=h) for h in (ho, None)]
+    for name, a, b, w in zip(("dq", "dk", "dv", "dbeta", "dlog_gamma", "dstate"), *runs, want):
+        assert torch.equal(a, b), name
+        more = 4e-6 if name == "dlog_gamma" and q.dtype == torch.float32 else 0.0
+        assert rel(a, w) < tol(a.dtype, q.dtype) + more, name
+
+
 def test_backward_is_reproducible_and_equal_with_and_without_the_handover():
     q, k, v, do, beta, lg, S0, dS, m = inputs(2, 4, 4, 2, 2, 300, 64, 64, "bf16", mask="tail")
     ho = ops.DeltaHandover()
