@@ -26,6 +26,7 @@ from .autograd import (
     SubQuadraticAttention,
     chunkwise_flash_linear_attention,
 )
+from .delta import SubQGatedDeltaAttention, SubQLayerNorm, gated_delta_attention, layer_norm
 from .surgery import SubQAttentionOutput, SubQBypassAttention, bypass_transformer_with_subq
 
 sys.modules.setdefault("subq_engine", _C)
@@ -56,6 +57,7 @@ def generate(Q, K, V, decay_factor: float = 0.99):
 __all__: List[str] = [
     "_C", "SubQEngine", "AudioStreamBuffer", "get_device_info", "AudioTransformerEngine", "Engine",
     "SubQuadraticAttention", "SubQLinearAttention", "SubQAttentionFunction", "chunkwise_flash_linear_attention",
+    "gated_delta_attention", "SubQGatedDeltaAttention", "layer_norm", "SubQLayerNorm",
     "bypass_transformer_with_subq", "SubQBypassAttention", "SubQAttentionOutput",
     "setup_distributed", "cleanup_distributed", "wrap_model_ddp", "create_distributed_dataloader",
     "load", "generate", "__version__",

@@ -146,3 +146,94 @@ def head_rmsnorm_bwd(dy: Tensor, x: Tensor, weight: Optional[Tensor], eps: float
 def _head_rmsnorm_bwd_fake(dy, x, weight, eps):
     dx = ops._empty_in_order(x, tuple(x.shape), x.dtype)
     return dx, _empty_f32(x, (x.shape[-1],) if weight is not None else (0,))
+
+
+# The gated delta rule and its gradients:
+#     o, S, handover = torch.ops.subq_audio.gated_delta_fwd(q, k, v, beta, log_gamma, mask, S0, scale, want_state, want_handover)
+#     dq, dk, dv, dbeta, dlog_gamma, dS0 = torch.ops.subq_audio.gated_delta_bwd(q, k, v, beta, dout, log_gamma, mask, S0, dS,
+#                                                                             scale, handover, need_dlog_gamma, need_dS0)
+# beta and log_gamma are None or tensors [], [H] or [B, H, N]; dbeta and
+# dlog_gamma come per token, [B, H, N] float32. What a call does not produce is
+# an empty tensor; an empty handover lets the backward form it again.
+def _delta_H(q: Tensor, k: Tensor, v: Tensor, beta: Optional[Tensor], log_gamma: Optional[Tensor]) -> int:
+    return ops._delta_heads(q, k, v, beta, log_gamma)
+
+
+def _delta_handover(q: Tensor, k: Tensor, v: Tensor, H: int) -> int:
+    d = _capi.DeltaDesc()
+    d.batch, d.heads, d.seq_len, d.head_dim, d.value_dim = q.shape[0], H, q.shape[2], q.shape[3], v.shape[3]
+    d.q_heads, d.k_heads, d.v_heads, d.dtype, d.scale = q.shape[1], k.shape[1], v.shape[1], ops._DTYPES[q.dtype], 1.0
+    return _capi.delta_handover_bytes(d)
+
+
+@torch.library.custom_op("subq_audio::gated_delta_fwd", mutates_args=(), device_types="cuda")
+def gated_delta_fwd(q: Tensor, k: Tensor, v: Tensor, beta: Optional[Tensor], log_gamma: Optional[Tensor],
+                    mask: Optional[Tensor], S0: Optional[Tensor], scale: float, want_state: bool,
+                    want_handover: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    ho = ops.DeltaHandover() if want_handover else None
+    o, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=log_gamma, mask=mask, scale=scale, state=S0,
+                                   return_state=want_state, handover=ho)
+    buf = ho.buf if ho is not None and ho.buf is not None else torch.empty(0, dtype=torch.uint8, device=q.device)
+    return o, (S if want_state else _empty_f32(q, (0,))), buf
+
+
+@gated_delta_fwd.register_fake
+def _gated_delta_fwd_fake(q, k, v, beta, log_gamma, mask, S0, scale, want_state, want_handover):
+    H = _delta_H(q, k, v, beta, log_gamma)
+    B, _, N, d = q.shape
+    o = ops._empty_in_order(q, (B, H, N, v.shape[-1]), q.dtype)
+    S = _empty_f32(q, (B, H, d, v.shape[-1]) if want_state else (0,))
+    return o, S, torch.empty(_delta_handover(q, k, v, H) if want_handover else 0, dtype=torch.uint8, device=q.device)
+
+
+@torch.library.custom_op("subq_audio::gated_delta_bwd", mutates_args=(), device_types="cuda")
+def gated_delta_bwd(q: Tensor, k: Tensor, v: Tensor, beta: Optional[Tensor], dout: Tensor, log_gamma: Optional[Tensor],
+                    mask: Optional[Tensor], S0: Optional[Tensor], dS: Optional[Tensor], scale: float, handover: Tensor,
+                    need_dlog_gamma: bool, need_dS0: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    ho = None
+    if handover.numel() > 0:
+        H = _delta_H(q, k, v, beta, log_gamma)
+        ho = ops.DeltaHandover()
+        ho.buf, ho.key = handover, (q.shape[0], H, q.shape[2], q.shape[3], v.shape[3], q.dtype, q.device)
+    dq, dk, dv, dbeta, dlg, dS0 = ops.gated_delta_backward(q, k, v, beta, dout, log_gamma=log_gamma, mask=mask, scale=scale,
+                                                           state=S0, dstate=dS, need_dlog_gamma=need_dlog_gamma,
+                                                           need_dstate=need_dS0, handover=ho)
+    return (dq, dk, dv, dbeta, dlg if dlg is not None else _empty_f32(q, (0,)),
+            dS0 if dS0 is not None else _empty_f32(q, (0,)))
+
+
+@gated_delta_bwd.register_fake
+def _gated_delta_bwd_fake(q, k, v, beta, dout, log_gamma, mask, S0, dS, scale, handover, need_dlog_gamma, need_dS0):
+    H = _delta_H(q, k, v, beta, log_gamma)
+    B, _, N, d = q.shape
+    return (ops._empty_in_order(q, tuple(q.shape), q.dtype), ops._empty_in_order(k, tuple(k.shape), q.dtype),
+            ops._empty_in_order(v, tuple(v.shape), q.dtype), _empty_f32(q, (B, H, N)),
+            _empty_f32(q, (B, H, N) if need_dlog_gamma else (0,)), _empty_f32(q, (B, H, d, v.shape[-1]) if need_dS0 else (0,)))
+
+
+# Layer norm over the last dimension:
+#     y = torch.ops.subq_audio.layer_norm_fwd(x, weight, bias, eps, out_dtype)
+#     dx, dweight, dbias = torch.ops.subq_audio.layer_norm_bwd(dy, x, weight, eps, need_dweight, need_dbias)
+@torch.library.custom_op("subq_audio::layer_norm_fwd", mutates_args=(), device_types="cuda")
+def layer_norm_fwd(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                   out_dtype: Optional[torch.dtype]) -> Tensor:
+    return ops.layer_norm(x, weight, bias, eps, out_dtype=out_dtype)
+
+
+@layer_norm_fwd.register_fake
+def _layer_norm_fwd_fake(x, weight, bias, eps, out_dtype):
+    return torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+
+
+@torch.library.custom_op("subq_audio::layer_norm_bwd", mutates_args=(), device_types="cuda")
+def layer_norm_bwd(dy: Tensor, x: Tensor, weight: Optional[Tensor], eps: float, need_dweight: bool,
+                   need_dbias: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    dx, dw, db = ops.layer_norm_backward(dy, x, weight, eps, need_dweight=need_dweight, need_dbias=need_dbias)
+    return dx, (dw if dw is not None else _empty_f32(x, (0,))), (db if db is not None else _empty_f32(x, (0,)))
+
+
+@layer_norm_bwd.register_fake
+def _layer_norm_bwd_fake(dy, x, weight, eps, need_dweight, need_dbias):
+    D = x.shape[-1]
+    return (torch.empty(x.shape, dtype=x.dtype, device=x.device), _empty_f32(x, (D if need_dweight else 0,)),
+            _empty_f32(x, (D if need_dbias else 0,)))

@@ -603,7 +603,8 @@ def gated_delta_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta
         dq = _empty_in_order(q, tuple(q.shape), q.dtype)
         dk = _empty_in_order(k, tuple(k.shape), q.dtype)
         dv = _empty_in_order(v, tuple(v.shape), q.dtype)
-        dgates = torch.empty((2 if need_dlog_gamma else 1, B, H, N), dtype=torch.float32, device=q.device)
+        dbeta = torch.empty((B, H, N), dtype=torch.float32, device=q.device)
+        dlg = torch.empty_like(dbeta) if need_dlog_gamma else None
         a = _capi.DeltaBwdArgs()
         _delta_desc(a.desc, q, k, v, beta, log_gamma, mask, scale, "auto", H, keep)
         a.q, a.k, a.v, a.dout = _t4(q), _t4(k), _t4(v), _t4(dout)
@@ -614,8 +615,7 @@ def gated_delta_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta
         if need_dstate:
             dS = torch.empty((B, H, d, e), dtype=torch.float32, device=q.device)
             a.dstate_in = dS.data_ptr()
-        a.dbeta = dgates[0].data_ptr()
-        dlg = dgates[1] if need_dlog_gamma else None
+        a.dbeta = dbeta.data_ptr()
         if dlg is not None:
             a.dlog_gamma = dlg.data_ptr()
         a.stream = torch.cuda.current_stream(q.device).cuda_stream
@@ -625,7 +625,7 @@ def gated_delta_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta
             a.handover = handover.buf.data_ptr()
         a.workspace, a.workspace_bytes = _workspace(_capi.delta_bwd_workspace_bytes(a), q.device, keep)
         _capi.delta_bwd(a)
-    return dq, dk, dv, dgates[0], dlg, dS
+    return dq, dk, dv, dbeta, dlg, dS
 
 
 class GatedDeltaStep:
