@@ -513,7 +513,7 @@ int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc&
 // Segments of a sequence that are walked side by side when there are few sequences. A walk over n chunks takes n
 // steps of about t = 1.7 us whatever the number of CTAs, up to one CTA per SM. With G segments, a first pass (states
 // only, from the segments' value columns and the d columns of the identity) and the walk itself take n / G steps each,
-// times the waves of their CTAs, and the join about 2 us a segment and 8 us of launches. G is the count with the
+// times the waves of their CTAs, and the join about 0.8 us a segment and 8 us of launches. G is the count with the
 // least such time, taken where that is at least a fifth below the single walk's (B = 1, H = 4, N = 4096, d = e = 64:
 // G = 9, 162 -> 76 us measured; B = 8, H = 12: one).
 struct DeltaSplit {
@@ -521,7 +521,7 @@ struct DeltaSplit {
 };
 DeltaSplit delta_split(const subq::DeltaParams& p) {
     const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + 31) / 32, ndb = (p.d + 31) / 32;
-    constexpr double kStep = 1.7, kJoin = 2.0, kLaunch = 8.0;
+    constexpr double kStep = 1.7, kJoin = 0.8, kLaunch = 8.0;
     auto waves = [](int64_t ctas) { return (double)((ctas + 147) / 148); };
     double best = 0.8 * p.nc * kStep * waves(bh * ncb);
     DeltaSplit s = {1, p.nc};
@@ -542,9 +542,9 @@ DeltaBytes delta_bytes(const subq::DeltaParams& p, int dtype) {
     const size_t nx = dtype == SUBQ_FP32 ? 3 : 2, chunks = (size_t)p.B * p.H * p.nc;
     const size_t ncw = 2 * ((p.e + subq::kDeltaCols - 1) / subq::kDeltaCols), dp = p.d <= 64 ? 64 : 128;
     const size_t mat = align_up(chunks * nx * subq::kYBlocks * 512);
-    const size_t slots = (size_t)p.B * p.H * (delta_split(p).nseg - 1) * p.d * sizeof(float);
+    const size_t slots = (size_t)p.B * p.H * (delta_split(p).nseg - 1) * sizeof(float);
     return {align_up(chunks * sizeof(subq::DeltaGates)), mat, mat, align_up(chunks * ncw * (dp / 16) * nx * 512),
-            align_up(chunks * ncw * 4 * nx * 512), align_up(slots * p.e), align_up(slots * p.d)};
+            align_up(chunks * ncw * 4 * nx * 512), align_up(slots * p.d * p.e), align_up(slots * dp * dp)};
 }
 
 void delta_handover(subq::DeltaParams& p, const DeltaBytes& n, void* at) {

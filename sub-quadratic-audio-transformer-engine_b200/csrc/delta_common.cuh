@@ -59,7 +59,7 @@ struct DeltaParams {
     // segments of a sequence walked side by side (few sequences): 1, or more than 1 with `seg_S` and `seg_M`
     int nseg, seg_chunks;
     float* seg_S;  // [B * H][nseg - 1][d, e]: state after a segment
-    float* seg_M;  // [B * H][nseg - 1][d, d]: what a segment does to the state before it
+    float* seg_M;  // [B * H][nseg - 1][dp, dp] (d padded): what a segment does to the state before it
     // backward
     DeltaTensor g, dq, dk, dv;
     unsigned char* dS;  // gradient of the state after each chunk, like S0
@@ -463,11 +463,11 @@ struct WalkJob {
     bool ident;        // columns of the identity (V = 0) in place of value columns: the walk then gives seg_M's columns
     const float* in;   // state before, [d, ld], or null (0)
     float* out;        // state after, or null
-    int ld;
+    int ld, rows;      // of `in` and `out`
 };
 
 __device__ __forceinline__ int64_t tensor_base(const DeltaTensor& x, int b, int h) {
-    return b * x.sb + (h / x.group) * x.sh;
+    return b * x.sb + (x.group == 1 ? h : h / x.group) * x.sh;
 }
 
 // scale G o (Q K^T) for row block rb, as NX planes in `out`
