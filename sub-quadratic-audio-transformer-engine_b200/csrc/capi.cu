@@ -812,7 +812,7 @@ int subq_layer_norm_bwd(const subq_layer_norm_args* a) {
         const size_t need = align_up(subq::ln_bwd_workspace_floats(p.rows, p.D) * sizeof(float));
         if ((rc = check_workspace(a->workspace, a->workspace_bytes, need))) return rc;
         p.part = static_cast<float*>(a->workspace);
-        const int64_t most = subq::kLnLongSlices;
+        const int64_t most = subq::kLnPartials;
         p.stats = p.part + (size_t)2 * p.D * (p.rows < most ? p.rows : most);
     }
     cudaError_t err = subq::launch_layer_norm(p, a->x_dtype, a->y_dtype, true, st, &launches);

@@ -45,7 +45,7 @@ struct LnParams {
     float* part;     // partial rows of (dw, db), or null (neither wanted)
     float* stats;    // D > 8192: mean and rsqrt of each row
 };
-constexpr int kLnLongSlices = 2 * 148;  // partial rows of the long-row form
+constexpr int kLnPartials = 4 * 148;  // partial rows of (dw, db) at most
 size_t ln_bwd_workspace_floats(int64_t rows, int D);
 // The dtype pairs (x, y) are (T, T) for float32, float16, bfloat16 and (float32, float16 or bfloat16).
 cudaError_t launch_layer_norm(const LnParams& p, int x_dtype, int y_dtype, bool bwd, cudaStream_t st, int* launches);

@@ -6,16 +6,18 @@
 // from the centred values); x, dy and y, dx have types of their own (a float32
 // residual stream normalised into bf16 and back is one pass each way).
 //
-// HBM-bound: a row is read once and written once. kG threads hold a row, V
-// consecutive elements (16 or 32 bytes) K times per thread; CTAs stay for many
-// rows, so w and b are read once per thread and the backward's dw and db stay in
-// registers until the end: one partial row per CTA, summed by a second kernel in
+// HBM-bound: a row is read once and written once. G threads hold a row, V
+// consecutive elements (16 bytes of x) K times per thread; CTAs stay for many
+// rows, with the next row on its way while one is worked on, so w and b are read
+// once and the backward's dw and db stay in registers until the end: one partial row per CTA, summed by a second kernel in
 // a fixed order (bitwise reproducible). Rows longer than the registers hold
 // (D > 8192) are read again per pass, from L2.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "delta_launch.h"
 #include "kernels.hpp"
@@ -27,40 +29,36 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSMs = 148;
 
+// V elements as they are in memory: V of 16-byte pieces, of 8 bytes (4 of 16 bits) or single ones.
 template <typename T, int V>
-__device__ __forceinline__ void load_v(const T* p, float (&f)[V]) {
-    if constexpr (V == 1) {
-        f[0] = to_f<T>(*p);
-    } else if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Raw {
+    static constexpr int kBytes = V * (int)sizeof(T);
+    using Piece = typename std::conditional<kBytes >= 16, uint4, typename std::conditional<kBytes == 8, uint2, T>::type>::type;
+    static constexpr int kPieces = kBytes >= 16 ? kBytes / 16 : 1;
+    Piece p[kPieces];
+    __device__ __forceinline__ void load(const T* at) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            T t[2];
-            *reinterpret_cast<uint32_t*>(t) = w[i];
-            f[2 * i] = to_f<T>(t[0]);
-            f[2 * i + 1] = to_f<T>(t[1]);
-        }
+        for (int i = 0; i < kPieces; ++i) p[i] = reinterpret_cast<const Piece*>(at)[i];
     }
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void store_v(T* p, const float (&f)[V]) {
-    if constexpr (V == 1) {
-        *p = from_f<T>(f[0]);
-    } else if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-        alignas(16) T t[8];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = from_f<T>(f[i]);
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
+        for (int i = 0; i < kPieces; ++i) p[i] = Piece{};
     }
-}
+    __device__ __forceinline__ void store(T* at) const {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) reinterpret_cast<Piece*>(at)[i] = p[i];
+    }
+    __device__ __forceinline__ void get(float (&f)[V]) const {
+        const T* t = reinterpret_cast<const T*>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = to_f<T>(t[i]);
+    }
+    __device__ __forceinline__ void set(const float (&f)[V]) {
+        T* t = reinterpret_cast<T*>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = from_f<T>(f[i]);
+    }
+};
 
 // Sums of M values over the G threads of a row (G = 8, 32: lanes; 256: the CTA).
 template <int G, int M>
@@ -85,7 +83,7 @@ __device__ __forceinline__ void row_sums(float (&v)[M], float* red) {
 }
 
 template <typename TX, typename TY, int G, int V, int K>
-__global__ void __launch_bounds__(kThreads) ln_fwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(kThreads, K * V <= 16 ? 3 : K * V <= 24 ? 2 : 1) ln_fwd_kernel(const LnParams p) {
     __shared__ float red[kThreads / 32];
     constexpr int kRows = kThreads / G;
     const int li = threadIdx.x % G, D = p.D;
@@ -99,21 +97,26 @@ __global__ void __launch_bounds__(kThreads) ln_fwd_kernel(const LnParams p) {
             w[k][i] = p.w && c < D ? p.w[c] : 1.f;
             b[k][i] = p.b && c < D ? p.b[c] : 0.f;
         }
-    // the loop runs the same number of times in every thread of a row's group and of a warp
-#pragma unroll 1
-    for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < p.rows; r0 += (int64_t)gridDim.x * kRows) {
-        const int64_t row = r0 + threadIdx.x / G;
-        const bool live = row < p.rows;
+    Raw<TX, V> next[K];  // the next row, on its way
+    auto load = [&](int64_t row) {
         const TX* x = static_cast<const TX*>(p.x) + row * p.x_s;
-        float f[K][V], s[1] = {0.f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * G + li) * V;
-            if (live && c < D) load_v<TX, V>(x + c, f[k]);
-            else
-#pragma unroll
-                for (int i = 0; i < V; ++i) f[k][i] = 0.f;
+            if (row < p.rows && c < D) next[k].load(x + c);
+            else next[k].zero();
         }
+    };
+    const int64_t first = (int64_t)blockIdx.x * kRows;
+    load(first + threadIdx.x / G);
+    // the loop runs the same number of times in every thread of a row's group and of a warp
+#pragma unroll 1
+    for (int64_t r0 = first; r0 < p.rows; r0 += (int64_t)gridDim.x * kRows) {
+        const int64_t row = r0 + threadIdx.x / G;
+        float f[K][V], s[1] = {0.f};
+#pragma unroll
+        for (int k = 0; k < K; ++k) next[k].get(f[k]);
+        if (r0 + (int64_t)gridDim.x * kRows < p.rows) load(row + (int64_t)gridDim.x * kRows);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -135,83 +138,104 @@ __global__ void __launch_bounds__(kThreads) ln_fwd_kernel(const LnParams p) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * G + li) * V;
-            if (live && c < D) {
+            if (row < p.rows && c < D) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) f[k][i] = fmaf(f[k][i] * r, w[k][i], b[k][i]);
-                store_v<TY, V>(y + c, f[k]);
+                Raw<TY, V> out;
+                out.set(f[k]);
+                out.store(y + c);
             }
         }
     }
 }
 
 template <typename TX, typename TY, int G, int V, int K>
-__global__ void __launch_bounds__(kThreads) ln_bwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(kThreads, K * V <= 8 ? 4 : K * V <= 24 ? 2 : 1) ln_bwd_kernel(const LnParams p) {
     __shared__ float red[kThreads / 32 * 2];
-    extern __shared__ float cols[];  // [D] sums of the rows a CTA handles side by side
+    extern __shared__ __align__(16) float sm_ln[];  // [D] weight, [D] sums of the rows a CTA handles side by side
+    float* cols = sm_ln + p.D;
     constexpr int kRows = kThreads / G;
     const int li = threadIdx.x % G, D = p.D;
     const float inv = 1.f / D;
-    float w[K][V], dw[K][V], db[K][V];
+    for (int c = threadIdx.x; c < D; c += kThreads) sm_ln[c] = p.w ? p.w[c] : 1.f;
+    __syncthreads();
+    float dw[K][V], db[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = (k * G + li) * V + i;
-            w[k][i] = p.w && c < D ? p.w[c] : 1.f;
-            dw[k][i] = db[k][i] = 0.f;
-        }
-#pragma unroll 1
-    for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < p.rows; r0 += (int64_t)gridDim.x * kRows) {
-        const int64_t row = r0 + threadIdx.x / G;
-        const bool live = row < p.rows;
+        for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
+    constexpr bool kAhead = K * V <= 8;  // the next row of x and dy is on its way while one is worked on
+    Raw<TX, V> nx[K];
+    Raw<TY, V> ny[K];
+    auto load = [&](int64_t row) {
         const TX* x = static_cast<const TX*>(p.x) + row * p.x_s;
         const TY* dy = static_cast<const TY*>(p.dy) + row * p.dy_s;
-        float f[K][V], e[K][V], s[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * G + li) * V;
-            if (live && c < D) {
-                load_v<TX, V>(x + c, f[k]);
-                load_v<TY, V>(dy + c, e[k]);
+            if (row < p.rows && c < D) {
+                nx[k].load(x + c);
+                ny[k].load(dy + c);
             } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) f[k][i] = e[k][i] = 0.f;
+                nx[k].zero();
+                ny[k].zero();
             }
         }
+    };
+    const int64_t first = (int64_t)blockIdx.x * kRows;
+    if (kAhead) load(first + threadIdx.x / G);
+#pragma unroll 1
+    for (int64_t r0 = first; r0 < p.rows; r0 += (int64_t)gridDim.x * kRows) {
+        const int64_t row = r0 + threadIdx.x / G;
+        float f[K][V], e[K][V], s[2] = {0.f, 0.f};
+        if (!kAhead) load(row);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            nx[k].get(f[k]);
+            ny[k].get(e[k]);
+        }
+        if (kAhead && r0 + (int64_t)gridDim.x * kRows < p.rows) load(row + (int64_t)gridDim.x * kRows);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                s[0] += f[k][i];
-                s[1] += __fmul_rn(e[k][i], w[k][i]);
-            }
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * G + li) * V;
+            if (c < D)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    s[0] += f[k][i];
+                    s[1] += __fmul_rn(e[k][i], sm_ln[c + i]);
+                }
+        }
         row_sums<G, 2>(s, red);
         const float mean = s[0] * inv, mg = s[1] * inv;
         s[0] = s[1] = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-            if ((k * G + li) * V < D)
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * G + li) * V;
+            if (c < D)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     f[k][i] -= mean;
                     s[0] = fmaf(f[k][i], f[k][i], s[0]);
-                    s[1] = fmaf(e[k][i] * w[k][i], f[k][i], s[1]);
+                    s[1] = fmaf(e[k][i] * sm_ln[c + i], f[k][i], s[1]);
                 }
+        }
         row_sums<G, 2>(s, red);
         const float r = rsqrtf(s[0] * inv + p.eps), mgx = s[1] * inv * r;
         TX* dx = static_cast<TX*>(p.dx) + row * p.dx_s;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * G + li) * V;
-            if (live && c < D) {
+            if (row < p.rows && c < D) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float xh = f[k][i] * r;
                     dw[k][i] = fmaf(e[k][i], xh, dw[k][i]);
                     db[k][i] += e[k][i];
-                    f[k][i] = r * (__fmul_rn(e[k][i], w[k][i]) - mg - xh * mgx);
+                    f[k][i] = r * (__fmul_rn(e[k][i], sm_ln[c + i]) - mg - xh * mgx);
                 }
-                store_v<TX, V>(dx + c, f[k]);
+                Raw<TX, V> out;
+                out.set(f[k]);
+                out.store(dx + c);
             }
         }
     }
@@ -239,20 +263,20 @@ __global__ void __launch_bounds__(kThreads) ln_bwd_kernel(const LnParams p) {
     }
 }
 
-// dw[c], db[c]: the nb partial rows added in order by 8 threads a column, then those in order.
-__global__ void __launch_bounds__(256) ln_cols_kernel(const float* part, int nb, int D, float* dw, float* db) {
-    __shared__ float red[8][33];
+// dw[c], db[c]: the nb partial rows added by 32 threads a column, each every 32nd row in order, then those in order.
+__global__ void __launch_bounds__(1024) ln_cols_kernel(const float* part, int nb, int D, float* dw, float* db) {
+    __shared__ float red[32][33];
     const int which = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
     float s = 0.f;
     if (c < D)
-#pragma unroll 8
-        for (int i = k; i < nb; i += 8) s += part[((int64_t)i * 2 + which) * D + c];
+#pragma unroll 4
+        for (int i = k; i < nb; i += 32) s += part[((int64_t)i * 2 + which) * D + c];
     red[k][threadIdx.x & 31] = s;
     __syncthreads();
     float* out = which ? db : dw;
     if (k == 0 && c < D && out) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
+        for (int i = 1; i < 32; ++i) s += red[i][threadIdx.x];
         out[c] = s;
     }
 }
@@ -313,20 +337,35 @@ struct Shape {
 };
 
 // Threads per row and elements per thread: the smallest group whose threads hold
-// at most 32 elements each; 8 elements at a time where every row starts on a
-// 16-byte boundary, single ones otherwise. G = 0: the row is too long.
-Shape shape_of(int D, bool vec) {
-    if (vec && D % 8 == 0) {
-        const int n = D / 8;
-        if (n <= 32) return {8, 8, (n + 7) / 8};
-        if (n <= 128) return {32, 8, (n + 31) / 32};
-        if (n <= 1024) return {kThreads, 8, (n + kThreads - 1) / kThreads};
+// at most 32 elements each; V of them (16 bytes of x) at a time where every row of
+// x, y and their gradients starts on a 16-byte boundary, single ones otherwise.
+// G = 0: the row is too long.
+//
+// The backward holds a row of x and dy and the sums of dw and db: 24 elements a lane
+// are what two CTAs per SM have registers for.
+Shape shape_of(int D, bool vec, int V, bool bwd) {
+    const int lanes = bwd ? 24 : 32;  // elements a lane holds, at most, in a row of one warp
+    if (vec && D % V == 0) {
+        const int n = D / V;
+        if (n <= 8 * (lanes / V)) return {8, V, (n + 7) / 8};
+        if (n <= 32 * (lanes / V)) return {32, V, (n + 31) / 32};
+        if (n <= kThreads * (32 / V)) return {kThreads, V, (n + kThreads - 1) / kThreads};
         return {0, 1, 0};
     }
-    const int G = D <= 1024 ? 32 : kThreads;
+    const int G = D <= (bwd ? 256 : 1024) ? 32 : kThreads;
     const int k = (D + G - 1) / G;
     if (k > 32) return {0, 1, 0};
-    return {G, 1, k <= 8 ? 8 : k <= 16 ? 16 : 32};
+    return {G, 1, k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : 32};
+}
+
+template <typename F>
+int resident(F kernel, size_t smem) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = 1;
+    }
+    return n;
 }
 
 bool vec_of(const LnParams& p, bool bwd, int dx_size, int dy_size) {
@@ -335,22 +374,45 @@ bool vec_of(const LnParams& p, bool bwd, int dx_size, int dy_size) {
     return bwd ? ok(p.dy, p.dy_s, dy_size) && ok(p.dx, p.dx_s, dx_size) : ok(p.y, p.y_s, dy_size);
 }
 
+// Launches as many CTAs as fit at once (the backward at most kLnPartials: a partial row each), or fewer.
 template <typename TX, typename TY, int G, int V, int K>
-cudaError_t run(const LnParams& p, bool bwd, int blocks, cudaStream_t st) {
-    if (bwd) ln_bwd_kernel<TX, TY, G, V, K><<<blocks, kThreads, p.part && G < kThreads ? p.D * sizeof(float) : 0, st>>>(p);
-    else ln_fwd_kernel<TX, TY, G, V, K><<<blocks, kThreads, 0, st>>>(p);
+cudaError_t run(const LnParams& p, bool bwd, int* blocks, cudaStream_t st) {
+    constexpr int64_t kRows = kThreads / G;
+    const int64_t need = (p.rows + kRows - 1) / kRows;
+    if (!bwd) {
+        static const int per_sm = resident(ln_fwd_kernel<TX, TY, G, V, K>, 0);
+        *blocks = (int)(need < kSMs * per_sm ? need : kSMs * per_sm);
+        ln_fwd_kernel<TX, TY, G, V, K><<<*blocks, kThreads, 0, st>>>(p);
+    } else {
+        const int smem = p.D * (p.part && G < kThreads ? 2 : 1) * (int)sizeof(float);
+        static const int per_sm = resident(ln_bwd_kernel<TX, TY, G, V, K>, 2 * 4 * G * V * K);
+        const int64_t most = kSMs * per_sm < kLnPartials ? kSMs * per_sm : kLnPartials;
+        *blocks = (int)(need < most ? need : most);
+        if (smem > 48 * 1024) {
+            const cudaError_t err = cudaFuncSetAttribute(ln_bwd_kernel<TX, TY, G, V, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (err != cudaSuccess) return err;
+        }
+        ln_bwd_kernel<TX, TY, G, V, K><<<*blocks, kThreads, smem, st>>>(p);
+    }
     return cudaGetLastError();
 }
 
 template <typename TX, typename TY, int G>
-cudaError_t run_g(const LnParams& p, const Shape& s, bool bwd, int blocks, cudaStream_t st) {
-    if (s.V == 8) switch (s.K) {
-        case 1: return run<TX, TY, G, 8, 1>(p, bwd, blocks, st);
-        case 2: return run<TX, TY, G, 8, 2>(p, bwd, blocks, st);
-        case 3: return run<TX, TY, G, 8, 3>(p, bwd, blocks, st);
-        default: return run<TX, TY, G, 8, 4>(p, bwd, blocks, st);
+cudaError_t run_g(const LnParams& p, const Shape& s, bool bwd, int* blocks, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(TX);
+    if (s.V == V) switch (s.K) {
+        case 1: return run<TX, TY, G, V, 1>(p, bwd, blocks, st);
+        case 2: return run<TX, TY, G, V, 2>(p, bwd, blocks, st);
+        case 3: return run<TX, TY, G, V, 3>(p, bwd, blocks, st);
+        case 4: return run<TX, TY, G, V, 4>(p, bwd, blocks, st);
+        default:
+            if constexpr (V == 4) {
+                if (s.K <= 6) return run<TX, TY, G, V, 6>(p, bwd, blocks, st);
+                return run<TX, TY, G, V, 8>(p, bwd, blocks, st);
+            }
     }
     if constexpr (G > 8) switch (s.K) {
+        case 4: return run<TX, TY, G, 1, 4>(p, bwd, blocks, st);
         case 8: return run<TX, TY, G, 1, 8>(p, bwd, blocks, st);
         case 16: return run<TX, TY, G, 1, 16>(p, bwd, blocks, st);
         default: return run<TX, TY, G, 1, 32>(p, bwd, blocks, st);
@@ -358,26 +420,18 @@ cudaError_t run_g(const LnParams& p, const Shape& s, bool bwd, int blocks, cudaS
     return cudaErrorInvalidValue;
 }
 
-int blocks_of(const LnParams& p, const Shape& s, bool bwd) {
-    const int64_t rows = s.G ? kThreads / s.G : 1, need = (p.rows + rows - 1) / rows;
-    // 2 CTAs per SM fit with the backward's sums in registers; the forward's 8
-    const int64_t most = kSMs * (bwd ? 2 : 8);
-    return (int)(need < most ? (need > 0 ? need : 1) : most);
-}
-
 template <typename TX, typename TY>
 cudaError_t ln_t(LnParams p, bool bwd, cudaStream_t st, int* launches) {
-    const Shape s = shape_of(p.D, vec_of(p, bwd, sizeof(TX), sizeof(TY)));
-    const int blocks = blocks_of(p, s, bwd);
+    const Shape s = shape_of(p.D, vec_of(p, bwd, sizeof(TX), sizeof(TY)), 16 / sizeof(TX), bwd);
     *launches = 1;
     cudaError_t err;
-    int partial_rows = blocks;
+    int partial_rows = 1;
     if (s.G == 8) {
-        err = run_g<TX, TY, 8>(p, s, bwd, blocks, st);
+        err = run_g<TX, TY, 8>(p, s, bwd, &partial_rows, st);
     } else if (s.G == 32) {
-        err = run_g<TX, TY, 32>(p, s, bwd, blocks, st);
+        err = run_g<TX, TY, 32>(p, s, bwd, &partial_rows, st);
     } else if (s.G) {
-        err = run_g<TX, TY, kThreads>(p, s, bwd, blocks, st);
+        err = run_g<TX, TY, kThreads>(p, s, bwd, &partial_rows, st);
     } else {
         const int64_t most = kSMs * 8;
         const unsigned grid = (unsigned)(p.rows < most ? p.rows : most);
@@ -385,14 +439,14 @@ cudaError_t ln_t(LnParams p, bool bwd, cudaStream_t st, int* launches) {
         else ln_long_kernel<TX, TY, false><<<grid, kThreads, 0, st>>>(p);
         err = cudaGetLastError();
         if (err == cudaSuccess && p.part) {
-            partial_rows = (int)(p.rows < kLnLongSlices ? p.rows : kLnLongSlices);
+            partial_rows = (int)(p.rows < kLnPartials ? p.rows : kLnPartials);
             ln_long_cols_kernel<TX, TY><<<dim3((p.D + kThreads - 1) / kThreads, partial_rows), kThreads, 0, st>>>(p);
             err = cudaGetLastError();
             ++*launches;
         }
     }
     if (err == cudaSuccess && p.part) {
-        ln_cols_kernel<<<dim3((p.D + 31) / 32, 2), 256, 0, st>>>(p.part, partial_rows, p.D, p.dw, p.db);
+        ln_cols_kernel<<<dim3((p.D + 31) / 32, 2), 1024, 0, st>>>(p.part, partial_rows, p.D, p.dw, p.db);
         err = cudaGetLastError();
         ++*launches;
     }
@@ -403,7 +457,7 @@ cudaError_t ln_t(LnParams p, bool bwd, cudaStream_t st, int* launches) {
 
 // Partial rows of (dw, db), and for long rows each row's mean and rsqrt.
 size_t ln_bwd_workspace_floats(int64_t rows, int D) {
-    const int64_t most = kSMs * 2;
+    const int64_t most = kLnPartials;
     return (size_t)2 * D * (rows < most ? rows : most) + (D > 8192 ? (size_t)2 * rows : 0);
 }
 

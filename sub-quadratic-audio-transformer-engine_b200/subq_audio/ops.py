@@ -679,29 +679,38 @@ class GatedDeltaStep:
 
 
 # ------------------------------------------------------------------- layer norm
+_LN_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
 def _ln_check(x: torch.Tensor, y_dtype: torch.dtype) -> None:
-    half = (torch.float16, torch.bfloat16)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer_norm needs a last dimension of at least 1")
-    if x.dtype not in (torch.float32,) + half or (y_dtype != x.dtype and not (x.dtype == torch.float32 and y_dtype in half)):
+    if x.dtype not in _LN_TYPES or (y_dtype != x.dtype and not (x.dtype == torch.float32 and y_dtype in _LN_TYPES)):
         raise TypeError(f"layer_norm takes float32, float16 or bfloat16 (and float32 into a 16-bit type), not {x.dtype} into {y_dtype}")
 
 
-def _ln_rows(t: torch.Tensor) -> torch.Tensor:
-    """[rows, D] with contiguous rows: a view where the leading dimensions merge, else a copy."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+def _ln_rows(t: torch.Tensor, keep: list) -> Tuple[int, int]:
+    """(address, row stride) of t as [rows, D] with contiguous rows: t itself where the leading dimensions merge, else a copy."""
+    D = t.shape[-1]
+    if not t.is_contiguous():
+        t = t.reshape(-1, D)
+        if D > 1 and t.stride(-1) != 1:
+            t = t.contiguous()
+        keep.append(t)
+        return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), D
 
 
 def _ln_param(w: Optional[torch.Tensor], name: str, x: torch.Tensor, keep: list) -> Optional[int]:
     if w is None:
         return None
-    if tuple(w.shape) != (x.shape[-1],):
+    if w.dim() != 1 or w.shape[0] != x.shape[-1]:
         raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
     if w.device != x.device:
         raise ValueError(f"{name} must be on the device of x")
-    w = w.detach().to(torch.float32).contiguous()
-    keep.append(w)
+    if w.dtype != torch.float32 or not w.is_contiguous():
+        w = w.detach().to(torch.float32).contiguous()
+        keep.append(w)
     return w.data_ptr()
 
 
@@ -713,17 +722,17 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     _require_cuda(x)
     y_dtype = x.dtype if out_dtype is None else out_dtype
     _ln_check(x, y_dtype)
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return layer_norm(x, weight, bias, eps, out_dtype=out_dtype)
     D = x.shape[-1]
-    x2 = _ln_rows(x)
     keep: list = []
-    with torch.cuda.device(x.device):
-        y = torch.empty(x.shape, dtype=y_dtype, device=x.device)
-        a = _capi.LayerNormArgs()
-        a.rows, a.dim, a.x_dtype, a.y_dtype, a.eps = x2.shape[0], D, _DTYPES[x.dtype], _DTYPES[y_dtype], eps
-        a.x, a.x_stride, a.y, a.y_stride = x2.data_ptr(), x2.stride(0), y.data_ptr(), D
-        a.weight, a.bias = _ln_param(weight, "weight", x, keep), _ln_param(bias, "bias", x, keep)
-        a.stream = torch.cuda.current_stream(x.device).cuda_stream
-        _capi.layer_norm_fwd(a)
+    xp, xs = _ln_rows(x, keep)
+    y = torch.empty(x.shape, dtype=y_dtype, device=x.device)
+    _capi.layer_norm_fwd(_capi.LayerNormArgs(
+        x.numel() // D, D, _DTYPES[x.dtype], _DTYPES[y_dtype], eps, xp, xs, y.data_ptr(), D, None, 0, None, 0,
+        _ln_param(weight, "weight", x, keep), _ln_param(bias, "bias", x, keep), None, None, None, 0,
+        torch.cuda.current_stream().cuda_stream))
     return y
 
 
@@ -736,25 +745,22 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     _ln_check(x, dy.dtype)
     if dy.shape != x.shape or dy.device != x.device:
         raise ValueError("layer_norm_backward needs dy and x of one shape on one device")
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return layer_norm_backward(dy, x, weight, eps, need_dweight=need_dweight, need_dbias=need_dbias)
     D = x.shape[-1]
-    x2, dy2 = _ln_rows(x), _ln_rows(dy)
     keep: list = []
-    with torch.cuda.device(x.device):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty(D, dtype=torch.float32, device=x.device) if need_dweight else None
-        db = torch.empty(D, dtype=torch.float32, device=x.device) if need_dbias else None
-        a = _capi.LayerNormArgs()
-        a.rows, a.dim, a.x_dtype, a.y_dtype, a.eps = x2.shape[0], D, _DTYPES[x.dtype], _DTYPES[dy.dtype], eps
-        a.x, a.x_stride, a.dy, a.dy_stride = x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0)
-        a.dx, a.dx_stride = dx.data_ptr(), D
-        a.weight = _ln_param(weight, "weight", x, keep)
-        if dw is not None:
-            a.dweight = dw.data_ptr()
-        if db is not None:
-            a.dbias = db.data_ptr()
-        a.stream = torch.cuda.current_stream(x.device).cuda_stream
+    (xp, xs), (gp, gs) = _ln_rows(x, keep), _ln_rows(dy, keep)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty(D, dtype=torch.float32, device=x.device) if need_dweight else None
+    db = torch.empty(D, dtype=torch.float32, device=x.device) if need_dbias else None
+    a = _capi.LayerNormArgs(
+        x.numel() // D, D, _DTYPES[x.dtype], _DTYPES[dy.dtype], eps, xp, xs, None, 0, gp, gs, dx.data_ptr(), D,
+        _ln_param(weight, "weight", x, keep), None, dw.data_ptr() if need_dweight else None,
+        db.data_ptr() if need_dbias else None, None, 0, torch.cuda.current_stream().cuda_stream)
+    if need_dweight or need_dbias:
         a.workspace, a.workspace_bytes = _workspace(_capi.layer_norm_bwd_workspace_bytes(a), x.device, keep)
-        _capi.layer_norm_bwd(a)
+    _capi.layer_norm_bwd(a)
     return dx, dw, db
 
 
