@@ -158,27 +158,55 @@ __device__ __forceinline__ void mma_planes(float (&c)[4], const uint32_t (&a)[NA
 
 // c[n] += A B[n], plane pair by plane pair over all n: each accumulator is used again only after the others, which
 // hides the instruction's latency (22 cycles against 8 of issue: four accumulators at least).
+// The tensor cores cut a sum off where float32 addition rounds it, so every instruction on an accumulator loses up to
+// 2^-23 of it, always downwards. With three planes (float32 inputs) the five small products are therefore summed by
+// themselves and added once: 2.6e-6 -> see the tests' 2e-6 bound.
 template <int N, int NA, int NB, int NX>
 __device__ __forceinline__ void mma_set(float (&c)[N][4], const uint32_t (&a)[NA][4], const uint32_t (&b)[N][NB][2]) {
+    float small[N][4];
+    if constexpr (NX == 3) {
 #pragma unroll
-    for (int i = 0; i < NA; ++i)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+            for (int i = 0; i < 4; ++i) small[n][i] = 0.f;
+    }
+#pragma unroll
+    for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = NB - 1; j >= 0; --j)
             if (i + j < NX)
 #pragma unroll
-                for (int n = 0; n < N; ++n) mma(c[n], a[i], b[n][j][0], b[n][j][1]);
+                for (int n = 0; n < N; ++n) mma(NX == 3 && i + j > 0 ? small[n] : c[n], a[i], b[n][j][0], b[n][j][1]);
+    if constexpr (NX == 3) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[n][i] += small[n][i];
+    }
 }
 template <int NA, int NB, int NX>
 __device__ __forceinline__ void mma_pair(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b0)[NB][2],
                                          const uint32_t (&b1)[NB][2]) {
+    float small[2][4];
+    if constexpr (NX == 3) {
 #pragma unroll
-    for (int i = 0; i < NA; ++i)
+        for (int i = 0; i < 4; ++i) small[0][i] = small[1][i] = 0.f;
+    }
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+    for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = NB - 1; j >= 0; --j)
             if (i + j < NX) {
-                mma(c0, a[i], b0[j][0], b0[j][1]);
-                mma(c1, a[i], b1[j][0], b1[j][1]);
+                mma(NX == 3 && i + j > 0 ? small[0] : c0, a[i], b0[j][0], b0[j][1]);
+                mma(NX == 3 && i + j > 0 ? small[1] : c1, a[i], b1[j][0], b1[j][1]);
             }
+    if constexpr (NX == 3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            c0[i] += small[0][i];
+            c1[i] += small[1][i];
+        }
+    }
 }
 
 // Accumulators of two neighbouring 8-column blocks (16 rows x 16 columns) as the
