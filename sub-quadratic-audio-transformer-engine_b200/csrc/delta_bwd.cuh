@@ -9,11 +9,17 @@
 //   dQ = scale e^g (dO S0^T) + D1 K
 //   dK = D beta (W G^T) - e^g beta (Z S0^T) + D1^T Q + D2^T K + D2 K
 //   dV = beta Z,   dbeta_i = W_i.Z_i
-//   dlog gamma_t = sum over i >= t in the chunk of (q_i.dq_i - v_i.dv_i) + <G, S'>
-// for all chunks at once (delta_grad_kernel). The last line is the scaling
-// symmetry of the recurrence: multiplying S_t by e^{x_t} only moves factors
-// between q_t, k_t and the gates, so g_i enters through q_i.dq_i and v_i.dv_i.
-// <G, S'> = e^{g_C} <G, S0> + sum_j k_j.(D beta W G^T)_j.
+// for all chunks at once (delta_grad_kernel). log gamma_t (token t of the chunk)
+// scales every term that joins something before t to something from t on:
+//   dlog gamma_t = sum over i >= t > j of E_ij + sum over i >= t of a_i + sum over j < t of b_j + e^{g_C} <G, S0>,
+//   E_ij = D1_ij q_i.k_j + D2_ij k_i.k_j,   a_i = scale e^{g_i} q_i.(S0 dO_i) - e^{g_i} beta_i k_i.(S0 Z_i),
+//   b_j = e^{g_C - g_j} beta_j k_j.(G W_j).
+// From the end of the chunk backwards that is a running sum that row t of E and
+// a_t enter and column t of E and b_t leave, the very same numbers: what they are
+// off by leaves with them, and what is left is the error of the terms that count
+// for t. (The shorter running sum of q_i.dq_i - v_i.dv_i is the same in exact
+// arithmetic, but keeps the errors of tokens that have nothing to do with t: 3e-5
+// against 5e-6 with 16-bit inputs and fast decay.)
 #pragma once
 
 #include "delta_common.cuh"
@@ -452,7 +458,9 @@ struct GradSmem {
     static constexpr int kCtas = sizeof(T) == 2 && DP == 64 ? 2 : 1;
     static constexpr int kBufs = kIn == 1 && DP == 64 ? 2 : 1;
     Gates s;
-    float qdq[2][kDeltaC], vdv[kDeltaC], wz[kDeltaC], kdk[2][kDeltaC];
+    float wz[kDeltaC];
+    // halves (of d; D1's and D2's) of a_i, b_j and E's row sums, and E's column sums by block of rows
+    float in[2][kDeltaC], out[2][kDeltaC], row[2][kDeltaC], col[2][4][kDeltaC];
     float gs[2];
     alignas(128) unsigned char k[kIn * 64 * DP * 2];
     alignas(128) unsigned char q[kIn * 64 * DP * 2];
@@ -462,14 +470,13 @@ struct GradSmem {
         alignas(128) unsigned char W[kCol];
         alignas(128) unsigned char Z[kCol];
         alignas(128) unsigned char dO[kGTile];
-        alignas(128) unsigned char v[kGTile];
     };
     struct Scores {
         alignas(128) unsigned char d1[kX * kYBlocks * 512];
         alignas(128) unsigned char d2[kX * kYBlocks * 512];
     };
     union {
-        In in[kBufs];
+        In blk[kBufs];
         Scores sc;
     } u;
 };
@@ -546,18 +553,15 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     }
 
     bool direct = false;  // bf16: tiles straight to shared memory
-    if constexpr (NIN == 1) direct = p.k.vec && p.q.vec && p.v.vec && p.g.vec && p.d % 8 == 0 && p.e % 8 == 0;
+    if constexpr (NIN == 1) direct = p.k.vec && p.q.vec && p.g.vec && p.d % 8 == 0 && p.e % 8 == 0;
     auto start = [&](int eb) {  // the planes of a block of value columns
-        auto& in = sm.u.in[eb % Smem::kBufs];
+        auto& in = sm.u.blk[eb % Smem::kBufs];
         const int64_t at = chunk * 2 * ncb + 2 * eb;
         async16<256>(in.S0, p.S0 + at * (Smem::kState / 2), Smem::kState, tid);
         async16<256>(in.G, p.dS + at * (Smem::kState / 2), Smem::kState, tid);
         async16<256>(in.W, p.W + at * (Smem::kCol / 2), Smem::kCol, tid);
         async16<256>(in.Z, p.Z + at * (Smem::kCol / 2), Smem::kCol, tid);
-        if (direct) {
-            async_tile<T, kDeltaCols, 256>(in.dO, p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
-            async_tile<T, kDeltaCols, 256>(in.v, p.v, tensor_base(p.v, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
-        }
+        if (direct) async_tile<T, kDeltaCols, 256>(in.dO, p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, p.N, tid);
     };
     async16<256>(reinterpret_cast<unsigned char*>(&sm.s), reinterpret_cast<const unsigned char*>(p.gates + chunk), sizeof(Gates), tid);
     if (direct) {
@@ -586,30 +590,25 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     for (int n = 0; n < 8; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) D[n][i] = 0.f;  // dO W^T (hf = 0) or Z W^T (hf = 1), rows 16 rb ..
-    // diagonals: Z V^T of these tokens (hf = 0), S0^T G of a group of 16 columns (hf = 1, rb < 2)
-    float ex[2][4];
+    float ex[2][4];  // S0^T G of a group of 16 columns (hf = 1, rb < 2), of which the diagonal counts
     zero_acc<2>(ex);
 
     for (int eb = 0; eb < ncb; ++eb) {
-        auto& in = sm.u.in[eb % Smem::kBufs];
+        auto& in = sm.u.blk[eb % Smem::kBufs];
         if (eb >= Smem::kBufs) {
             __syncthreads();  // the block before has been read
             start(eb);
         }
-        if (!direct) {
-            load_tile<T, kDeltaCols, NIN, 256>(in.dO, p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, p.N, s.live, tid);
-            load_tile<T, kDeltaCols, NIN, 256>(in.v, p.v, tensor_base(p.v, b, h), n0, eb * kDeltaCols, p.e, p.N, s.live, tid);
-        }
+        if (!direct) load_tile<T, kDeltaCols, NIN, 256>(in.dO, p.g, tensor_base(p.g, b, h), n0, eb * kDeltaCols, p.e, p.N, s.live, tid);
         async_wait();
         if (direct && !s.full) {
             __syncthreads();
             clear_dead<kDeltaCols, 256>(in.dO, s.live, tid);
-            clear_dead<kDeltaCols, 256>(in.v, s.live, tid);
         }
         __syncthreads();
         const uint32_t S0 = smem_addr(in.S0) + lane * 16, G = smem_addr(in.G) + lane * 16;
         const uint32_t W = smem_addr(in.W) + lane * 16, Z = smem_addr(in.Z) + lane * 16;
-        const uint32_t dO = smem_addr(in.dO), V = smem_addr(in.v);
+        const uint32_t dO = smem_addr(in.dO);
 #pragma unroll
         for (int cw = 0; cw < 2; ++cw) {  // 16 value columns: one k step
             uint32_t ao[NIN][4], aw[NX][4], az[NX][4];
@@ -659,16 +658,6 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
                     mma_pair<NX, NX, NX>(D[2 * jb], D[2 * jb + 1], az, b0, b1);
                 }
             }
-            if (hf == 0) {
-                uint32_t b0[NIN][2], b1[NIN][2];
-#pragma unroll
-                for (int pl = 0; pl < NIN; ++pl) {
-                    uint32_t r[4];
-                    b_rows<kDeltaCols>(r, V + pl * kGTile, 16 * rb, cw, lane);
-                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                }
-                mma_pair<NX, NIN, NX>(ex[0], ex[1], az, b0, b1);
-            }
             if (hf == 1 && rb == cw) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
@@ -694,9 +683,6 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
                 sm.wz[16 * rb + g] = d0 ? D[2 * jb][0] : D[2 * jb][1];
                 sm.wz[16 * rb + 8 + g] = d0 ? D[2 * jb + 1][2] : D[2 * jb + 1][3];
             }
-    } else if (d0 || d1_) {  // v.dv
-        sm.vdv[16 * rb + g] = s.beta[16 * rb + g] * (d0 ? ex[0][0] : ex[0][1]);
-        sm.vdv[16 * rb + 8 + g] = s.beta[16 * rb + 8 + g] * (d0 ? ex[1][2] : ex[1][3]);
     }
     if (hf == 1 && rb < 2) {  // <G, S0>
         float gs = d0 ? ex[0][0] + ex[1][2] : d1_ ? ex[0][1] + ex[1][3] : 0.f;
@@ -706,56 +692,99 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     }
     __syncthreads();  // the blocks of value columns have been read: D1 and D2 take their place
 
-    {  // D1 or D2 as planes
+    {  // D1 or D2 as planes; E's row and column sums
         unsigned char* dst = (hf ? sm.u.sc.d2 : sm.u.sc.d1) + lane * 4;
+        const uint32_t at = smem_addr(hf ? sm.k : sm.q), kt = smem_addr(sm.k);
+        float row[2] = {0.f, 0.f};
 #pragma unroll
-        for (int ih = 0; ih < 2; ++ih) {
-            const int i = 16 * rb + 8 * ih + g, keep = hf ? i - 1 : i;
-            const float gh = s.gh[i], gl = s.gl[i], fi = hf ? -s.beta[i] : p.scale;
+        for (int jb = 0; jb < 4; ++jb) {
+            if (jb > rb) continue;
+            float sc[2][4];  // q_i.k_j or k_i.k_j
+            zero_acc<2>(sc);
 #pragma unroll
-            for (int jb = 0; jb < 4; ++jb) {
-                if (jb > rb) continue;
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                uint32_t a[NIN][4], b0[NIN][2], b1[NIN][2];
 #pragma unroll
-                for (int jh = 0; jh < 2; ++jh) {
-                    const int j = 16 * jb + 8 * jh + 2 * t;
-                    const float2 ga = gamma_pair(gh, gl, s, j, keep), be = *reinterpret_cast<const float2*>(&s.beta[j]);
+                for (int pl = 0; pl < NIN; ++pl) {
+                    uint32_t r[4];
+                    a_rows<DP>(a[pl], at + pl * kTile, 16 * rb, kk, lane);
+                    b_rows<DP>(r, kt + pl * kTile, 16 * jb, kk, lane);
+                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                }
+                mma_pair<NIN, NIN, NX>(sc[0], sc[1], a, b0, b1);
+            }
+#pragma unroll
+            for (int jh = 0; jh < 2; ++jh) {
+                const int j = 16 * jb + 8 * jh + 2 * t;
+                const float2 be = *reinterpret_cast<const float2*>(&s.beta[j]);
+                float2 col = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int ih = 0; ih < 2; ++ih) {
+                    const int i = 16 * rb + 8 * ih + g, keep = hf ? i - 1 : i;
+                    const float fi = hf ? -s.beta[i] : p.scale;
+                    const float2 ga = gamma_pair(s.gh[i], s.gl[i], s, j, keep);
+                    const float x = fi * be.x * ga.x * select0(j <= keep, D[2 * jb + jh][2 * ih]);
+                    const float y = fi * be.y * ga.y * select0(j + 1 <= keep, D[2 * jb + jh][2 * ih + 1]);
                     uint32_t r[NX];
-                    split2<NX>(fi * be.x * ga.x * select0(j <= keep, D[2 * jb + jh][2 * ih]),
-                               fi * be.y * ga.y * select0(j + 1 <= keep, D[2 * jb + jh][2 * ih + 1]), r);
+                    split2<NX>(x, y, r);
 #pragma unroll
                     for (int pl = 0; pl < NX; ++pl)
                         *reinterpret_cast<uint32_t*>(dst + (pl * kYBlocks + tri(rb, jb)) * 512 + (ih * 2 + jh) * 128) = r[pl];
+                    const float ex0 = select0(j < i, x * sc[jh][2 * ih]), ey0 = select0(j + 1 < i, y * sc[jh][2 * ih + 1]);
+                    row[ih] += ex0 + ey0;
+                    col.x += ex0;
+                    col.y += ey0;
                 }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    col.x += __shfl_xor_sync(0xffffffffu, col.x, o);
+                    col.y += __shfl_xor_sync(0xffffffffu, col.y, o);
+                }
+                if (g == 0) *reinterpret_cast<float2*>(&sm.col[hf][rb][j]) = col;
             }
         }
+#pragma unroll
+        for (int ih = 0; ih < 2; ++ih) {
+            row[ih] += __shfl_xor_sync(0xffffffffu, row[ih], 1);
+            row[ih] += __shfl_xor_sync(0xffffffffu, row[ih], 2);
+            if (t == 0) sm.row[hf][16 * rb + 8 * ih + g] = row[ih];
+        }
     }
-    {  // row factors of the products with the states; k.dk1 before anything is added to it
-        float kd[2] = {0.f, 0.f};
+    // row factors of the products with the states; a_i and b_j
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int i = 16 * rb + 8 * x + g;
-            const float fq = p.scale * s.eg[i], f1 = s.kd[i] * s.beta[i], f2 = -s.eg[i] * s.beta[i];
+    for (int x = 0; x < 2; ++x) {
+        const int i = 16 * rb + 8 * x + g;
+        const float fq = p.scale * s.eg[i], f1 = s.kd[i] * s.beta[i], f2 = -s.eg[i] * s.beta[i];
+        float in = 0.f, out = 0.f;
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                const int piece = hf * NB + n;
-                float2 kv = make_float2(0.f, 0.f);
+        for (int n = 0; n < NB; ++n) {
+            const uint32_t off = tile_off<DP>(i, hf * NB + n) + 4 * t;
+            float2 kv = make_float2(0.f, 0.f), qv = kv;
 #pragma unroll
-                for (int pl = 0; pl < NIN; ++pl) {
-                    const float2 u = unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.k + pl * kTile + tile_off<DP>(i, piece) + 4 * t));
-                    kv.x += u.x;
-                    kv.y += u.y;
-                }
-                const float a = f1 * dk1[n][2 * x], d = f1 * dk1[n][2 * x + 1];
-                kd[x] = fmaf(a, kv.x, kd[x]);
-                kd[x] = fmaf(d, kv.y, kd[x]);
-                dk1[n][2 * x] = fmaf(f2, dk2[n][2 * x], a);
-                dk1[n][2 * x + 1] = fmaf(f2, dk2[n][2 * x + 1], d);
-                dq[n][2 * x] *= fq;
-                dq[n][2 * x + 1] *= fq;
+            for (int pl = 0; pl < NIN; ++pl) {
+                const float2 u = unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.k + pl * kTile + off));
+                const float2 w = unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.q + pl * kTile + off));
+                kv.x += u.x; kv.y += u.y;
+                qv.x += w.x; qv.y += w.y;
             }
-            kd[x] += __shfl_xor_sync(0xffffffffu, kd[x], 1);
-            kd[x] += __shfl_xor_sync(0xffffffffu, kd[x], 2);
-            if (t == 0) sm.kdk[hf][i] = kd[x];
+            const float2 d1 = make_float2(f1 * dk1[n][2 * x], f1 * dk1[n][2 * x + 1]);
+            const float2 d2 = make_float2(f2 * dk2[n][2 * x], f2 * dk2[n][2 * x + 1]);
+            dq[n][2 * x] *= fq;
+            dq[n][2 * x + 1] *= fq;
+            out = fmaf(d1.x, kv.x, fmaf(d1.y, kv.y, out));
+            in = fmaf(d2.x, kv.x, fmaf(d2.y, kv.y, in));
+            in = fmaf(dq[n][2 * x], qv.x, fmaf(dq[n][2 * x + 1], qv.y, in));
+            dk1[n][2 * x] = d1.x + d2.x;
+            dk1[n][2 * x + 1] = d1.y + d2.y;
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            in += __shfl_xor_sync(0xffffffffu, in, o);
+            out += __shfl_xor_sync(0xffffffffu, out, o);
+        }
+        if (t == 0) {
+            sm.in[hf][i] = in;
+            sm.out[hf][i] = out;
         }
     }
     __syncthreads();
@@ -802,38 +831,28 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
             }
         }
     }
-    {  // q.dq
-        float qd[2] = {0.f, 0.f};
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int i = 16 * rb + 8 * x + g;
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int pl = 0; pl < NIN; ++pl) {
-                    const float2 u =
-                        unpack_bf16(*reinterpret_cast<const uint32_t*>(sm.q + pl * kTile + tile_off<DP>(i, hf * NB + n) + 4 * t));
-                    qd[x] = fmaf(u.x, dq[n][2 * x], qd[x]);
-                    qd[x] = fmaf(u.y, dq[n][2 * x + 1], qd[x]);
-                }
-            qd[x] += __shfl_xor_sync(0xffffffffu, qd[x], 1);
-            qd[x] += __shfl_xor_sync(0xffffffffu, qd[x], 2);
-            if (t == 0) sm.qdq[hf][i] = qd[x];
-        }
-    }
     store_grad<T, NB>(dq, p.dq, tensor_base(p.dq, b, h), p.dq32, at32 * p.d, n0 + 16 * rb, n0 + rows, 8 * hf * NB, p.d, lane);
     store_grad<T, NB>(dk1, p.dk, tensor_base(p.dk, b, h), p.dk32, at32 * p.d, n0 + 16 * rb, n0 + rows, 8 * hf * NB, p.d, lane);
     __syncthreads();
     if (warp == 0) {
-        // suffix sums over the chunk (two tokens per lane) on top of <G, S'>
-        const int i0 = 2 * lane, i1 = i0 + 1;
-        const float x0 = sm.qdq[0][i0] + sm.qdq[1][i0] - sm.vdv[i0], x1 = sm.qdq[0][i1] + sm.qdq[1][i1] - sm.vdv[i1];
-        float end = 0.f, k01 = sm.kdk[0][i0] + sm.kdk[1][i0] + sm.kdk[0][i1] + sm.kdk[1][i1];
-        end = sm.gs[0] + sm.gs[1];
+        // two tokens per lane, from the end of the chunk backwards
+        const int i0 = 2 * lane, i1 = i0 + 1, first = lane >> 3;
+        float x[2], out[2];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) k01 += __shfl_xor_sync(0xffffffffu, k01, o);
-        end = s.eC * end + k01;
-        float run = x0 + x1;  // over this lane's tokens and the later lanes'
+        for (int i = 0; i < 2; ++i) {
+            const int n = i0 + i;
+            float col = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k >= first) col += sm.col[0][k][n] + sm.col[1][k][n];
+            out[i] = sm.out[0][n] + sm.out[1][n];
+            x[i] = (sm.in[0][n] + sm.in[1][n]) + (sm.row[0][n] + sm.row[1][n]) - col - out[i];
+        }
+        float end = out[0] + out[1];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) end += __shfl_xor_sync(0xffffffffu, end, o);
+        end = fmaf(s.eC, sm.gs[0] + sm.gs[1], end);
+        float run = x[0] + x[1];  // over this lane's tokens and the later lanes'
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const float down = __shfl_down_sync(0xffffffffu, run, o);
@@ -846,7 +865,7 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
         }
         if (i1 < rows) {
             p.dbeta[at + i1] = s.live[i1] ? sm.wz[i1] : 0.f;
-            if (p.dlg) p.dlg[at + i1] = s.live[i1] ? run - x0 + end : 0.f;
+            if (p.dlg) p.dlg[at + i1] = s.live[i1] ? run - x[0] + end : 0.f;
         }
     }
 }
