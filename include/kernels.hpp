@@ -255,7 +255,7 @@ typedef struct subq_delta_desc {
 
 typedef struct subq_delta_fwd_args {
     subq_delta_desc desc;
-    subq_tensor4 q, k, v, o;
+    subq_tensor4 q, k, v, o; /* o must not alias the inputs                    */
     const float* state_in;  /* [B, heads, d, e], NULL = zeros                  */
     float* state_out;       /* may equal state_in, NULL = not wanted           */
     void* handover;         /* NULL, or subq_delta_handover_bytes (256-byte aligned)
@@ -298,9 +298,9 @@ typedef struct subq_layer_norm_args {
     int32_t x_dtype, y_dtype;
     float eps;
     const void* x;  int64_t x_stride;
-    void* y;        int64_t y_stride;   /* forward  */
+    void* y;        int64_t y_stride;   /* forward; may be x (of one type and stride) */
     const void* dy; int64_t dy_stride;  /* backward */
-    void* dx;       int64_t dx_stride;  /* may be x or dy for dim <= 8192 */
+    void* dx;       int64_t dx_stride;  /* may be x or dy (of one type and stride) for dim <= 8192 */
     const float* weight;                /* [dim] or NULL (1) */
     const float* bias;                  /* [dim] or NULL (0) */
     float* dweight;                     /* [dim] or NULL */

@@ -4,8 +4,10 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <mutex>
 #include <string>
+#include <tuple>
 
 #include "delta_common.cuh"
 #include "delta_launch.h"
@@ -536,15 +538,18 @@ DeltaSplit delta_split(const subq::DeltaParams& p) {
 
 struct DeltaBytes {
     size_t gates, Y, P, S0, W;  // the handover's parts
-    size_t seg_S, seg_M;        // workspace
+    size_t seg_S, seg_M, seg_in;  // workspace, where a sequence is cut into segments
+    size_t segs() const { return seg_S + seg_M + seg_in; }
 };
 DeltaBytes delta_bytes(const subq::DeltaParams& p, int dtype) {
     const size_t nx = dtype == SUBQ_FP32 ? 3 : 2, chunks = (size_t)p.B * p.H * p.nc;
     const size_t ncw = 2 * ((p.e + subq::kDeltaCols - 1) / subq::kDeltaCols), dp = p.d <= 64 ? 64 : 128;
     const size_t mat = align_up(chunks * nx * subq::kYBlocks * 512);
-    const size_t slots = (size_t)p.B * p.H * (delta_split(p).nseg - 1) * sizeof(float);
+    const int nseg = delta_split(p).nseg;
+    const size_t slots = (size_t)p.B * p.H * (nseg - 1) * sizeof(float);
+    const size_t copy = nseg > 1 && p.S_in && p.S_in == p.S_out ? (size_t)p.B * p.H * p.d * p.e * sizeof(float) : 0;
     return {align_up(chunks * sizeof(subq::DeltaGates)), mat, mat, align_up(chunks * ncw * (dp / 16) * nx * 512),
-            align_up(chunks * ncw * 4 * nx * 512), align_up(slots * p.d * p.e), align_up(slots * dp * dp)};
+            align_up(chunks * ncw * 4 * nx * 512), align_up(slots * p.d * p.e), align_up(slots * dp * dp), align_up(copy)};
 }
 
 void delta_handover(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
@@ -561,6 +566,7 @@ void delta_segments(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
     p.seg_chunks = s.chunks;
     p.seg_S = static_cast<float*>(at);
     p.seg_M = reinterpret_cast<float*>(static_cast<char*>(at) + n.seg_S);
+    p.seg_in = n.seg_in ? reinterpret_cast<float*>(static_cast<char*>(at) + n.seg_S + n.seg_M) : nullptr;
 }
 
 int fill_delta_fwd(const subq_delta_fwd_args* a, subq::DeltaParams& p, int& path) {
@@ -572,6 +578,8 @@ int fill_delta_fwd(const subq_delta_fwd_args* a, subq::DeltaParams& p, int& path
     if ((rc = delta_tensor(a->q, "q", d, d.q_heads, empty, p.q)) || (rc = delta_tensor(a->k, "k", d, d.k_heads, empty, p.k)) ||
         (rc = delta_tensor(a->v, "v", d, d.v_heads, empty, p.v)) || (rc = delta_tensor(a->o, "o", d, d.heads, empty, p.o)))
         return rc;
+    for (const void* in : {a->q.data, a->k.data, a->v.data})
+        if (!empty && a->o.data == in) return fail(SUBQ_ERR_ALIAS, "o must not be q, k or v");
     p.S_in = a->state_in;
     p.S_out = a->state_out;
     path = d.path;
@@ -628,7 +636,7 @@ DeltaBwdBytes delta_bwd_bytes(const subq::DeltaParams& p, int dtype, bool handov
     n.dq = p.q.group > 1 ? align_up(tokens * p.d * 4) : 0;
     n.dk = p.k.group > 1 ? align_up(tokens * p.d * 4) : 0;
     n.dv = p.v.group > 1 ? align_up(tokens * p.e * 4) : 0;
-    n.total = n.fwd.S0 + n.fwd.W + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.gates + n.fwd.Y + n.fwd.P + n.fwd.S0 + n.fwd.W + n.fwd.seg_S + n.fwd.seg_M);
+    n.total = n.fwd.S0 + n.fwd.W + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.gates + n.fwd.Y + n.fwd.P + n.fwd.S0 + n.fwd.W + n.fwd.segs());
     return n;
 }
 
@@ -646,7 +654,7 @@ size_t subq_delta_fwd_workspace_bytes(const subq_delta_fwd_args* a) {
     int path;
     if (fill_delta_fwd(a, p, path) != SUBQ_OK || path != SUBQ_PATH_CHUNKED) return 0;
     const DeltaBytes n = delta_bytes(p, a->desc.dtype);
-    return n.seg_S + n.seg_M + (a->handover ? 0 : n.gates + n.Y + n.P);
+    return n.segs() + (a->handover ? 0 : n.gates + n.Y + n.P);
 }
 
 size_t subq_delta_bwd_workspace_bytes(const subq_delta_bwd_args* a) {
@@ -671,7 +679,7 @@ int subq_delta_fwd(const subq_delta_fwd_args* a) {
         err = subq::launch_delta_step(p, a->desc.dtype, st);
     } else {
         const DeltaBytes n = delta_bytes(p, a->desc.dtype);
-        const size_t segs = n.seg_S + n.seg_M;
+        const size_t segs = n.segs();
         if ((rc = check_workspace(a->workspace, a->workspace_bytes, segs + (a->handover ? 0 : n.gates + n.Y + n.P)))) return rc;
         delta_segments(p, n, a->workspace);
         if (a->handover) {
@@ -727,7 +735,7 @@ int subq_delta_bwd(const subq_delta_bwd_args* a) {
         delta_handover(p, n.fwd, const_cast<void*>(a->handover));
     } else {
         delta_segments(p, n.fwd, at);
-        delta_handover(p, n.fwd, at + n.fwd.seg_S + n.fwd.seg_M);
+        delta_handover(p, n.fwd, at + n.fwd.segs());
         err = subq::launch_delta_fwd(p, dt, st);  // (o is null: states and corrections only)
         first = p.nseg > 1 ? 4 : 2;
     }
@@ -761,13 +769,23 @@ static int fill_ln(const subq_layer_norm_args* a, subq::LnParams& p, bool bwd) {
     int rc = check(a->x, a->x_stride, a->x_dtype, "x");
     if (rc) return rc;
     p.x = a->x; p.x_s = a->x_stride;
+    // rows of an output that overlap would be written by several CTAs; an output that is an input has to have its layout
+    auto check_out = [&](const void* out, int64_t stride, int dtype, std::initializer_list<std::tuple<const void*, int64_t, int>> ins) {
+        if (a->rows > 1 && stride < a->dim) return fail(SUBQ_ERR_INVALID_ARGUMENT, "rows of an output overlap");
+        for (const auto& [in, in_stride, in_dtype] : ins)
+            if (a->rows > 0 && in == out && (in_stride != stride || in_dtype != dtype))
+                return fail(SUBQ_ERR_ALIAS, "an output in an input's place needs its type and row stride");
+        return (int)SUBQ_OK;
+    };
     if (!bwd) {
         if ((rc = check(a->y, a->y_stride, a->y_dtype, "y"))) return rc;
+        if ((rc = check_out(a->y, a->y_stride, a->y_dtype, {{a->x, a->x_stride, a->x_dtype}}))) return rc;
         p.y = a->y; p.y_s = a->y_stride;
         p.b = a->bias;
         return SUBQ_OK;
     }
     if ((rc = check(a->dy, a->dy_stride, a->y_dtype, "dy")) || (rc = check(a->dx, a->dx_stride, a->x_dtype, "dx"))) return rc;
+    if ((rc = check_out(a->dx, a->dx_stride, a->x_dtype, {{a->x, a->x_stride, a->x_dtype}, {a->dy, a->dy_stride, a->y_dtype}}))) return rc;
     p.dy = a->dy; p.dy_s = a->dy_stride;
     p.dx = a->dx; p.dx_s = a->dx_stride;
     p.dw = a->dweight;

@@ -1,5 +1,5 @@
-// Shared pieces of the gated delta rule kernels (delta_step.cu, delta_fwd.cu,
-// delta_bwd.cu). Per (batch, head) sequence with live tokens t:
+// Shared pieces of the gated delta rule kernels (delta_step.cu, delta_fwd.cuh,
+// delta_bwd.cuh). Per (batch, head) sequence with live tokens t:
 //   S_t = gamma_t S_{t-1} + beta_t k_t w_t^T,   w_t = v_t - gamma_t S_{t-1}^T k_t,
 //   o_t = scale S_t^T q_t;   a masked token leaves S as it is and has o = 0.
 //
@@ -60,6 +60,7 @@ struct DeltaParams {
     int nseg, seg_chunks;
     float* seg_S;  // [B * H][nseg - 1][d, e]: state after a segment
     float* seg_M;  // [B * H][nseg - 1][dp, dp] (d padded): what a segment does to the state before it
+    float* seg_in;  // [B * H][d, e]: copy of S_in where S_out is S_in (one CTA reads it, another writes it), else null
     // backward
     DeltaTensor g, dq, dk, dv;
     unsigned char* dS;  // gradient of the state after each chunk, like S0
@@ -146,21 +147,11 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&r)[NP]) {
     }
 }
 
-// c += A B over the plane pairs kept for NX planes of precision.
-template <int NA, int NB, int NX>
-__device__ __forceinline__ void mma_planes(float (&c)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][2]) {
-#pragma unroll
-    for (int i = 0; i < NA; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-            if (i + j < NX) mma(c, a[i], b[j][0], b[j][1]);
-}
-
 // c[n] += A B[n], plane pair by plane pair over all n: each accumulator is used again only after the others, which
 // hides the instruction's latency (22 cycles against 8 of issue: four accumulators at least).
 // The tensor cores cut a sum off where float32 addition rounds it, so every instruction on an accumulator loses up to
-// 2^-23 of it, always downwards. With three planes (float32 inputs) the five small products are therefore summed by
-// themselves and added once: 2.6e-6 -> see the tests' 2e-6 bound.
+// 2^-23 of it, always towards zero. With three planes (float32 inputs) the five small products are therefore summed by
+// themselves and added once: outputs are then off by 4.4e-7 (2.6e-6 with one sum), for 5 % of the time of a training step.
 template <int N, int NA, int NB, int NX>
 __device__ __forceinline__ void mma_set(float (&c)[N][4], const uint32_t (&a)[NA][4], const uint32_t (&b)[N][NB][2]) {
     float small[N][4];

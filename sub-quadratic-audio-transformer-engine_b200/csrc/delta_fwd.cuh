@@ -50,13 +50,13 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
     {
         TileRegs<T, DP, 128> k, q;
         k.issue(p.k, tensor_base(p.k, b, h), n0, 0, p.d, p.N, tid);
-        if (p.P) q.issue(p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, tid);
+        q.issue(p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, tid);
         if (warp == 0) form_gates(sm.s, p, b, h, n0, lane);
         __syncthreads();
         copy16<128>(reinterpret_cast<unsigned char*>(p.gates + chunk), reinterpret_cast<const unsigned char*>(&sm.s), sizeof(Gates), tid);
         if (!sm.s.any) return;  // nothing else of a dead chunk is read
         k.template store_planes<NIN>(sm.k, sm.s.live, tid);
-        if (p.P) q.template store_planes<NIN>(sm.q, sm.s.live, tid);
+        q.template store_planes<NIN>(sm.q, sm.s.live, tid);
     }
     __syncthreads();
     {  // A, rows 16 warp .. 16 warp + 15
@@ -107,8 +107,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
         }
     }
     // scores, the longest rows where A's were the shortest
-    if (p.P)
-        score_rows<DP, NIN, NX>(p.P + chunk * (NX * kYBlocks * 512), smem_addr(sm.q), smem_addr(sm.k), sm.s, p.scale, 3 - warp, lane);
+    score_rows<DP, NIN, NX>(p.P + chunk * (NX * kYBlocks * 512), smem_addr(sm.q), smem_addr(sm.k), sm.s, p.scale, 3 - warp, lane);
     __syncwarp();  // the diagonal block is this warp's own
     {
         const int col = lane & 15, r0 = 16 * warp;
@@ -518,7 +517,8 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
         job.in = seg == 0 && !job.ident && p.S_in ? p.S_in + job.bh * p.d * p.e : nullptr;
         job.out = job.ident ? p.seg_M + before * (DP * DP) : p.seg_S + before * p.d * p.e;
     } else {
-        job.in = seg ? p.seg_S + (before - 1) * p.d * p.e : p.S_in ? p.S_in + job.bh * p.d * p.e : nullptr;
+        const float* S_in = p.seg_in ? p.seg_in : p.S_in;
+        job.in = seg ? p.seg_S + (before - 1) * p.d * p.e : S_in ? S_in + job.bh * p.d * p.e : nullptr;
         job.out = seg + 1 == nseg && p.S_out ? p.S_out + job.bh * p.d * p.e : nullptr;
     }
     if (warp < 4) {
@@ -681,6 +681,12 @@ __global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
         for (int k = 0; k < kRows; ++k) l[k] = r0 + 16 * k < p.d && c < p.e ? add[(r0 + 16 * k) * p.e] : 0.f;
     };
     load(0);
+    if (p.seg_in) {
+        const int64_t at = (int64_t)bh32 * p.d * p.e + c;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k)
+            if (r0 + 16 * k < p.d && c < p.e) p.seg_in[at + (r0 + 16 * k) * p.e] = p.S_in[at + (r0 + 16 * k) * p.e];
+    }
 #pragma unroll
     for (int k = 0; k < kRows; ++k) S[(r0 + 16 * k) * 16 + col] = l[k];
     if (p.nseg > 2) load(1);

@@ -622,6 +622,9 @@ def gated_delta_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta
         if handover is not None and handover.buf is not None:
             if handover.key != (B, H, N, d, e, q.dtype, q.device):
                 raise ValueError("handover comes from a forward of another shape, type or device")
+            buf = handover.buf
+            if buf.dtype != torch.uint8 or not buf.is_contiguous() or buf.numel() < _capi.delta_handover_bytes(a.desc):
+                raise ValueError("handover is not a buffer that the forward of this call filled")
             a.handover = handover.buf.data_ptr()
         a.workspace, a.workspace_bytes = _workspace(_capi.delta_bwd_workspace_bytes(a), q.device, keep)
         _capi.delta_bwd(a)

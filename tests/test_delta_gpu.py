@@ -390,3 +390,31 @@ def test_refusals():
         ops.GatedDeltaStep(q, k, v, beta, out, S.half())
     with pytest.raises(ValueError, match="mask"):
         ops.GatedDeltaStep(q, k, v, beta, out, S, mask=m.float())
+
+
+@pytest.mark.parametrize("d,e", [(64, 64), (100, 40)])
+def test_state_in_place_where_a_sequence_is_cut_into_segments(d, e):
+    """One segment's walk starts from the state that another one's overwrites at its end."""
+    q, k, v, _, beta, lg, S0, _, _ = inputs(1, 4, 4, 4, 4, 4096, d, e, "bf16", seed=7)
+    o, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, state=S0, return_state=True)
+    assert ops.last_launches() == 4
+    state, out = S0.clone(), torch.empty_like(o)
+    step = ops.GatedDeltaStep(q, k, v, beta, out, state, log_gamma=lg)
+    for _ in range(3):
+        state.copy_(S0)
+        step.step()
+        assert torch.equal(out, o) and torch.equal(state, S)
+
+
+def test_buffers_that_do_not_belong_to_the_call_are_refused():
+    q, k, v, do, beta, lg, _, _, _ = inputs(1, 2, 2, 2, 2, 100, 64, 64, "bf16")
+    with pytest.raises(ValueError, match="o must not be"):
+        ops.gated_delta_forward(q, k, v, beta, out=v)
+    ho = ops.DeltaHandover()
+    ops.gated_delta_forward(q, k, v, beta, handover=ho)
+    for buf in (ho.buf[:-1], ho.buf.view(torch.int32), torch.empty(256, dtype=torch.uint8, device="cuda")):
+        with pytest.raises(ValueError):
+            torch.ops.subq_audio.gated_delta_bwd(q, k, v, beta, do, lg, None, None, None, 0.125, buf, False, False)
+    ho.buf = ho.buf[::2]
+    with pytest.raises(ValueError):
+        ops.gated_delta_backward(q, k, v, beta, do, handover=ho)
