@@ -1,17 +1,21 @@
 // Layer norm over the last dimension of [rows, D], forward and backward:
 //   xh = (x - mean(x)) rsqrt(var(x) + eps),   y = xh w + b
 //   g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum dy xh,  db = sum dy
-// with r the rsqrt (g is rounded to float32 the same way, by itself, wherever it
-// is used, so that g - mean(g) is exactly 0 where it should be). Sums are float32 over values held in registers (the variance
-// from the centred values); x, dy and y, dx have types of their own (a float32
-// residual stream normalised into bf16 and back is one pass each way).
+// with r the rsqrt (g is rounded to float32 the same way, by itself, wherever it is
+// used, so that g - mean(g) is exactly 0 where it should be). Sums are float32 over
+// values held in registers (the variance from the centred values); x, dy and y, dx
+// have types of their own (a float32 residual stream normalised into bf16 and back
+// is one pass each way).
 //
 // HBM-bound: a row is read once and written once. G threads hold a row, V
-// consecutive elements (16 bytes of x) K times per thread; CTAs stay for many
-// rows, with the next row on its way while one is worked on, so w and b are read
-// once and the backward's dw and db stay in registers until the end: one partial row per CTA, summed by a second kernel in
-// a fixed order (bitwise reproducible). Rows longer than the registers hold
-// (D > 8192) are read again per pass, from L2.
+// consecutive elements (16 bytes of x) K times per thread; CTAs stay for many rows,
+// with the next row on its way while one is worked on, so w and b are read once and
+// the backward's dw and db stay in registers until the end: one partial row per CTA,
+// summed by a second kernel in a fixed order (bitwise reproducible). Rows longer than
+// the registers hold (D > 8192) are read again per pass, from L2.
+// 65536 x 768, float32 -> bf16: forward 49 us (94 % of the measured copy bandwidth),
+// backward 108 us (71 %: the sums of a row wait for its loads, and the registers that
+// hold x, dy, dw and db leave room for two CTAs per SM).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -60,24 +64,26 @@ struct Raw {
     }
 };
 
-// Sums of M values over the G threads of a row (G = 8, 32: lanes; 256: the CTA).
+// Sums of M values over the G threads of a row (G = 8, 32: lanes; 64, 128: warps of a part of the CTA; 256: the CTA).
 template <int G, int M>
 __device__ __forceinline__ void row_sums(float (&v)[M], float* red) {
 #pragma unroll
     for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1)
 #pragma unroll
         for (int i = 0; i < M; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if constexpr (G == kThreads) {
-        __syncthreads();  // the sums of the call before have been read
+    if constexpr (G > 32) {
+        const int group = threadIdx.x / G;
+        auto sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(G) : "memory"); };
+        sync();  // the sums of the call before have been read
         if ((threadIdx.x & 31) == 0)
 #pragma unroll
             for (int i = 0; i < M; ++i) red[(threadIdx.x >> 5) * M + i] = v[i];
-        __syncthreads();
+        sync();
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             v[i] = 0.f;
 #pragma unroll
-            for (int w = 0; w < kThreads / 32; ++w) v[i] += red[w * M + i];
+            for (int w = 0; w < G / 32; ++w) v[i] += red[(group * (G / 32) + w) * M + i];
         }
     }
 }
@@ -149,8 +155,15 @@ __global__ void __launch_bounds__(kThreads, K * V <= 16 ? 3 : K * V <= 24 ? 2 : 
     }
 }
 
+// CTAs per SM that the backward's registers are cut for (8 single elements: two rows of them on their way, 64 registers
+// spill; width 511: 65 us, 100 with four CTAs; 2047: 71 us with two, 93 with three).
+constexpr int bwd_ctas(int G, int V, int K) {
+    if (V == 1 && K == 8) return G == kThreads ? 2 : 3;
+    return K * V <= 8 ? 4 : K * V <= 24 ? 2 : 1;
+}
+
 template <typename TX, typename TY, int G, int V, int K>
-__global__ void __launch_bounds__(kThreads, K * V <= 8 ? 4 : K * V <= 24 ? 2 : 1) ln_bwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(kThreads, bwd_ctas(G, V, K)) ln_bwd_kernel(const LnParams p) {
     __shared__ float red[kThreads / 32 * 2];
     extern __shared__ __align__(16) float sm_ln[];  // [D] weight, [D] sums of the rows a CTA handles side by side
     float* cols = sm_ln + p.D;
@@ -336,26 +349,25 @@ struct Shape {
     int G, V, K;
 };
 
-// Threads per row and elements per thread: the smallest group whose threads hold
-// at most 32 elements each; V of them (16 bytes of x) at a time where every row of
-// x, y and their gradients starts on a 16-byte boundary, single ones otherwise.
-// G = 0: the row is too long.
+// Threads per row and elements per thread: the smallest group of threads that hold at most `most` elements of the row
+// each, V of them (16 bytes of x) at a time where every row of x, y and their gradients starts on a 16-byte boundary and
+// the width allows it, single ones otherwise. G = 0: the row is too long.
 //
-// The backward holds a row of x and dy and the sums of dw and db: 24 elements a lane
-// are what two CTAs per SM have registers for.
+// Fewer threads a row are more rows in flight per SM and shorter sums, until the registers run out. Measured, us, about
+// 50 M elements (25 M at the odd widths), the threads taken first, then the next choice:
+//   forward, float32 -> bf16   width 64: 8 10, 32 14;  256: 32 23, 8 27;  768: 32 55, 64 57;  1280: 64 57, 32 70;  2048: 128 55, 256 59
+//   backward, float32, bf16    width 64: 32 33, 8 49;  768: 32 114, 64 136;  1024: 64 118, 32 146, 256 148;  4096: 256 142, 128 157
+//   forward, odd widths        511: 32 39, 64 43;  767: 64 43, 32 53;  2047: 128 37, 256 43
+//   backward, odd widths       129: 32 42, 64 50;  511: 64 65, 128 75;  1021: 128 69, 64 77, 256 85;  2047: 256 71, 128 75
 Shape shape_of(int D, bool vec, int V, bool bwd) {
-    const int lanes = bwd ? 24 : 32;  // elements a lane holds, at most, in a row of one warp
-    if (vec && D % V == 0) {
-        const int n = D / V;
-        if (n <= 8 * (lanes / V)) return {8, V, (n + 7) / 8};
-        if (n <= 32 * (lanes / V)) return {32, V, (n + 31) / 32};
-        if (n <= kThreads * (32 / V)) return {kThreads, V, (n + kThreads - 1) / kThreads};
-        return {0, 1, 0};
-    }
-    const int G = D <= (bwd ? 256 : 1024) ? 32 : kThreads;
-    const int k = (D + G - 1) / G;
-    if (k > 32) return {0, 1, 0};
-    return {G, 1, k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : 32};
+    if (!vec || D % V != 0) V = 1;
+    const int n = D / V, most = V > 1 ? 24 : bwd ? 8 : 16;
+    auto each = [&](int G) { return (n + G - 1) / G; };
+    int G = V > 1 && !bwd ? 8 : 32;
+    while (G < kThreads && each(G) * V > most) G = G == 8 ? 32 : 2 * G;
+    const int k = each(G);
+    if (k * V > 32) return {0, 1, 0};
+    return {G, V, V > 1 ? k : k <= 4 ? 4 : k <= 8 ? 8 : k <= 16 ? 16 : 32};
 }
 
 template <typename F>
@@ -383,7 +395,7 @@ cudaError_t run(const LnParams& p, bool bwd, int* blocks, cudaStream_t st) {
         static const int per_sm = resident(ln_fwd_kernel<TX, TY, G, V, K>, 0);
         *blocks = (int)(need < kSMs * per_sm ? need : kSMs * per_sm);
         ln_fwd_kernel<TX, TY, G, V, K><<<*blocks, kThreads, 0, st>>>(p);
-    } else {
+    } else if constexpr (G > 8 && (V > 1 || K <= 8 || G == kThreads)) {
         const int smem = p.D * (p.part && G < kThreads ? 2 : 1) * (int)sizeof(float);
         static const int per_sm = resident(ln_bwd_kernel<TX, TY, G, V, K>, 2 * 4 * G * V * K);
         const int64_t most = kSMs * per_sm < kLnPartials ? kSMs * per_sm : kLnPartials;
@@ -393,6 +405,8 @@ cudaError_t run(const LnParams& p, bool bwd, int* blocks, cudaStream_t st) {
             if (err != cudaSuccess) return err;
         }
         ln_bwd_kernel<TX, TY, G, V, K><<<*blocks, kThreads, smem, st>>>(p);
+    } else {
+        return cudaErrorInvalidValue;  // (shape_of gives the backward no such shape)
     }
     return cudaGetLastError();
 }
@@ -400,22 +414,24 @@ cudaError_t run(const LnParams& p, bool bwd, int* blocks, cudaStream_t st) {
 template <typename TX, typename TY, int G>
 cudaError_t run_g(const LnParams& p, const Shape& s, bool bwd, int* blocks, cudaStream_t st) {
     constexpr int V = 16 / sizeof(TX);
+    constexpr bool kAll = G == kThreads;  // (up to 32 elements a thread, see shape_of)
     if (s.V == V) switch (s.K) {
         case 1: return run<TX, TY, G, V, 1>(p, bwd, blocks, st);
         case 2: return run<TX, TY, G, V, 2>(p, bwd, blocks, st);
         case 3: return run<TX, TY, G, V, 3>(p, bwd, blocks, st);
-        case 4: return run<TX, TY, G, V, 4>(p, bwd, blocks, st);
         default:
             if constexpr (V == 4) {
+                if (s.K == 4) return run<TX, TY, G, V, 4>(p, bwd, blocks, st);
                 if (s.K <= 6) return run<TX, TY, G, V, 6>(p, bwd, blocks, st);
-                return run<TX, TY, G, V, 8>(p, bwd, blocks, st);
             }
+            if constexpr (kAll) return run<TX, TY, G, V, 32 / V>(p, bwd, blocks, st);
     }
     if constexpr (G > 8) switch (s.K) {
         case 4: return run<TX, TY, G, 1, 4>(p, bwd, blocks, st);
         case 8: return run<TX, TY, G, 1, 8>(p, bwd, blocks, st);
         case 16: return run<TX, TY, G, 1, 16>(p, bwd, blocks, st);
-        default: return run<TX, TY, G, 1, 32>(p, bwd, blocks, st);
+        default:
+            if constexpr (kAll) return run<TX, TY, G, 1, 32>(p, bwd, blocks, st);
     }
     return cudaErrorInvalidValue;
 }
@@ -430,6 +446,10 @@ cudaError_t ln_t(LnParams p, bool bwd, cudaStream_t st, int* launches) {
         err = run_g<TX, TY, 8>(p, s, bwd, &partial_rows, st);
     } else if (s.G == 32) {
         err = run_g<TX, TY, 32>(p, s, bwd, &partial_rows, st);
+    } else if (s.G == 64) {
+        err = run_g<TX, TY, 64>(p, s, bwd, &partial_rows, st);
+    } else if (s.G == 128) {
+        err = run_g<TX, TY, 128>(p, s, bwd, &partial_rows, st);
     } else if (s.G) {
         err = run_g<TX, TY, kThreads>(p, s, bwd, &partial_rows, st);
     } else {

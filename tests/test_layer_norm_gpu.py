@@ -168,3 +168,16 @@ def test_refusals():
     a.x_stride = a.dy_stride = a.dx_stride = 9000
     with pytest.raises(ValueError, match="dx must not be"):
         _capi.layer_norm_bwd(a)
+
+
+@pytest.mark.parametrize("x,y", [("fp32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("D", [72, 96, 384, 768, 896, 1280, 1536, 1544, 2048, 2056, 3080, 6144,
+                               17, 129, 255, 257, 511, 515, 767, 1023, 1027, 2047, 2051, 4095, 6001])
+def test_every_number_of_threads_a_row(D, x, y):
+    """Widths on both sides of each step in the threads that hold a row, with rows enough for every CTA to loop."""
+    shape = (min(40007, 6000000 // D), D)
+    v, w, b, dy = make(shape, x, y, seed=D)
+    ry, rdx, rdw, rdb = reference(v, w, b, 1e-5, dy)
+    assert rel(ops.layer_norm(v, w, b, 1e-5, out_dtype=T[y]), ry) < tol(T[y])
+    dx, dw, db = ops.layer_norm_backward(dy, v, w, 1e-5)
+    assert rel(dx, rdx) < tol(T[x]) and rel(dw, rdw) < 3e-6 and rel(db, rdb) < 3e-6
