@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kSMs = 148;
+constexpr int kPlainSmem = 40 * 1024;  // dynamic shared memory that a kernel has without asking (48 KB less what it declares)
 
 // V elements as they are in memory: V of 16-byte pieces, of 8 bytes (4 of 16 bits) or single ones.
 template <typename T, int V>
@@ -162,10 +163,27 @@ constexpr int bwd_ctas(int G, int V, int K) {
     return K * V <= 8 ? 4 : K * V <= 24 ? 2 : 1;
 }
 
+// N bytes (8 or 16) straight to shared memory.
+template <int N>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+    const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(src), "n"(N) : "memory");
+}
+
+// Bytes of shared memory in which a thread's pieces of the next row wait, where the registers do not hold them. With
+// float32 x or up to 16 elements a thread (backward, 49152 x 1024 float32: 118 us without, 99 us with; 65536 x 768 bf16,
+// 24 elements: 84 us without, 95 us with).
+template <typename TX, typename TY, int V, int K>
+constexpr int stage_bytes() {
+    return V > 1 && K * V > 8 && (V == 4 || K * V <= 16) ? kThreads * K * V * (int)(sizeof(TX) + sizeof(TY)) : 0;
+}
+
 template <typename TX, typename TY, int G, int V, int K>
 __global__ void __launch_bounds__(kThreads, bwd_ctas(G, V, K)) ln_bwd_kernel(const LnParams p) {
     __shared__ float red[kThreads / 32 * 2];
-    extern __shared__ __align__(16) float sm_ln[];  // [D] weight, [D] sums of the rows a CTA handles side by side
+    // stage, [D] weight, [D] sums of the rows a CTA handles side by side
+    extern __shared__ __align__(16) unsigned char raw_ln[];
+    float* sm_ln = reinterpret_cast<float*>(raw_ln + stage_bytes<TX, TY, V, K>());
     float* cols = sm_ln + p.D;
     constexpr int kRows = kThreads / G;
     const int li = threadIdx.x % G, D = p.D;
@@ -177,7 +195,29 @@ __global__ void __launch_bounds__(kThreads, bwd_ctas(G, V, K)) ln_bwd_kernel(con
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
-    constexpr bool kAhead = K * V <= 8;  // the next row of x and dy is on its way while one is worked on
+    // The next row of x and dy is on its way while one is worked on: in registers up to 8 elements a thread, else in
+    // slots of shared memory that each thread fills and empties for itself, else not (see stage_bytes).
+    constexpr bool kAhead = K * V <= 8, kStage = stage_bytes<TX, TY, V, K>() > 0;
+    constexpr int kBx = 16, kBy = V > 1 ? V * (int)sizeof(TY) : 16;  // bytes of a piece of x (V > 1) and of dy
+    constexpr int kPy = kBy > 16 ? kBy / 16 : 1, kBp = kBy / kPy;
+    unsigned char* slot_x = raw_ln + threadIdx.x * kBx;                         // [K][thread]
+    unsigned char* slot_y = raw_ln + kThreads * K * kBx + threadIdx.x * kBp;    // [K][piece][thread]
+    auto send = [&](int64_t row) {
+        if (row < p.rows) {
+            const TX* x = static_cast<const TX*>(p.x) + row * p.x_s;
+            const TY* dy = static_cast<const TY*>(p.dy) + row * p.dy_s;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int c = (k * G + li) * V;
+                if (c < D) {
+                    copy_async<kBx>(slot_x + k * kThreads * kBx, x + c);
+#pragma unroll
+                    for (int i = 0; i < kPy; ++i)
+                        copy_async<kBp>(slot_y + (k * kPy + i) * kThreads * kBp, reinterpret_cast<const unsigned char*>(dy + c) + i * kBp);
+                }
+            }
+        }
+    };
     Raw<TX, V> nx[K];
     Raw<TY, V> ny[K];
     auto load = [&](int64_t row) {
@@ -197,11 +237,28 @@ __global__ void __launch_bounds__(kThreads, bwd_ctas(G, V, K)) ln_bwd_kernel(con
     };
     const int64_t first = (int64_t)blockIdx.x * kRows;
     if (kAhead) load(first + threadIdx.x / G);
+    if constexpr (kStage) send(first + threadIdx.x / G);
 #pragma unroll 1
     for (int64_t r0 = first; r0 < p.rows; r0 += (int64_t)gridDim.x * kRows) {
         const int64_t row = r0 + threadIdx.x / G;
         float f[K][V], e[K][V], s[2] = {0.f, 0.f};
-        if (!kAhead) load(row);
+        if constexpr (kStage) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const bool in = row < p.rows && (k * G + li) * V < D;
+                nx[k].zero();
+                ny[k].zero();
+                if (in) {
+                    nx[k].p[0] = *reinterpret_cast<const typename Raw<TX, V>::Piece*>(slot_x + k * kThreads * kBx);
+#pragma unroll
+                    for (int i = 0; i < kPy; ++i)
+                        ny[k].p[i] = *reinterpret_cast<const typename Raw<TY, V>::Piece*>(slot_y + (k * kPy + i) * kThreads * kBp);
+                }
+            }
+        } else if (!kAhead) {
+            load(row);
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             nx[k].get(f[k]);
@@ -219,6 +276,8 @@ __global__ void __launch_bounds__(kThreads, bwd_ctas(G, V, K)) ln_bwd_kernel(con
                 }
         }
         row_sums<G, 2>(s, red);
+        // (the sums have taken every slot's values: the slots are free)
+        if constexpr (kStage) send(row + (int64_t)gridDim.x * kRows);
         const float mean = s[0] * inv, mg = s[1] * inv;
         s[0] = s[1] = 0.f;
 #pragma unroll
@@ -356,7 +415,7 @@ struct Shape {
 // Fewer threads a row are more rows in flight per SM and shorter sums, until the registers run out. Measured, us, about
 // 50 M elements (25 M at the odd widths), the threads taken first, then the next choice:
 //   forward, float32 -> bf16   width 64: 8 10, 32 14;  256: 32 23, 8 27;  768: 32 55, 64 57;  1280: 64 57, 32 70;  2048: 128 55, 256 59
-//   backward, float32, bf16    width 64: 32 33, 8 49;  768: 32 114, 64 136;  1024: 64 118, 32 146, 256 148;  4096: 256 142, 128 157
+//   backward, float32, bf16    width 64: 32 33, 8 49;  512: 32 79, 64 91;  1024: 64 99, 128 116;  1280: 64 114, 128 116 (bf16: 93, 106)
 //   forward, odd widths        511: 32 39, 64 43;  767: 64 43, 32 53;  2047: 128 37, 256 43
 //   backward, odd widths       129: 32 42, 64 50;  511: 64 65, 128 75;  1021: 128 69, 64 77, 256 85;  2047: 256 71, 128 75
 Shape shape_of(int D, bool vec, int V, bool bwd) {
@@ -373,7 +432,8 @@ Shape shape_of(int D, bool vec, int V, bool bwd) {
 template <typename F>
 int resident(F kernel, size_t smem) {
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem) != cudaSuccess || n < 1) {
+    if ((smem > kPlainSmem && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem) != cudaSuccess || n < 1) {
         cudaGetLastError();
         n = 1;
     }
@@ -396,11 +456,12 @@ cudaError_t run(const LnParams& p, bool bwd, int* blocks, cudaStream_t st) {
         *blocks = (int)(need < kSMs * per_sm ? need : kSMs * per_sm);
         ln_fwd_kernel<TX, TY, G, V, K><<<*blocks, kThreads, 0, st>>>(p);
     } else if constexpr (G > 8 && (V > 1 || K <= 8 || G == kThreads)) {
-        const int smem = p.D * (p.part && G < kThreads ? 2 : 1) * (int)sizeof(float);
-        static const int per_sm = resident(ln_bwd_kernel<TX, TY, G, V, K>, 2 * 4 * G * V * K);
+        constexpr int kStage = stage_bytes<TX, TY, V, K>();
+        const int smem = kStage + p.D * (p.part && G < kThreads ? 2 : 1) * (int)sizeof(float);
+        static const int per_sm = resident(ln_bwd_kernel<TX, TY, G, V, K>, kStage + (G < kThreads ? 2 : 1) * 4 * G * V * K);
         const int64_t most = kSMs * per_sm < kLnPartials ? kSMs * per_sm : kLnPartials;
         *blocks = (int)(need < most ? need : most);
-        if (smem > 48 * 1024) {
+        if (smem > kPlainSmem) {
             const cudaError_t err = cudaFuncSetAttribute(ln_bwd_kernel<TX, TY, G, V, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
             if (err != cudaSuccess) return err;
         }
