@@ -27,11 +27,14 @@ template <typename T, int DP>
 struct PrepSmem {
     static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
     Gates s;
-    alignas(16) float A[kDeltaC][kDeltaC + 4];
+    alignas(16) float A[kYBlocks][16][20];        // its lower triangle's blocks
     alignas(128) unsigned char Ab[6 * kX * 512];  // -A_IK beta, blocks I > K: [block][plane]
-    alignas(128) unsigned char Ti[4 * kX * 512];  // (I + A_II beta)^-1
     alignas(128) unsigned char k[kIn * 64 * DP * 2];
     alignas(128) unsigned char q[kIn * 64 * DP * 2];
+    // where (I + A_II beta)^-1 goes: over the 16 rows of q that warp I alone reads, once it has. (Six CTAs per SM then
+    // have room for bf16 at d = 64.)
+    static __host__ __device__ constexpr int ti(int I) { return (3 - I) * 16 * DP * 2; }
+    static_assert(kX * 512 <= 16 * DP * 2, "T in q's rows");
 };
 
 // Y by 16 x 16 blocks. With T_I = (I + A_II beta)^-1 (forward substitution, a
@@ -94,7 +97,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
                     const int j = 8 * n + 2 * t;
                     const float2 ga = gamma_pair(gh, gl, sm.s, j, i - 1);
                     const float x = ga.x * select0(j < i, acc[n][2 * ih]), y = ga.y * select0(j + 1 < i, acc[n][2 * ih + 1]);
-                    *reinterpret_cast<float2*>(&sm.A[i][j]) = make_float2(x, y);
+                    *reinterpret_cast<float2*>(&sm.A[tri(warp, n >> 1)][8 * ih + g][j & 15]) = make_float2(x, y);
                     if (n < 2 * warp) {
                         const float2 be = *reinterpret_cast<const float2*>(&sm.s.beta[j]);
                         uint32_t r[NX];
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
     }
     // scores, the longest rows where A's were the shortest
     score_rows<DP, NIN, NX>(p.P + chunk * (NX * kYBlocks * 512), smem_addr(sm.q), smem_addr(sm.k), sm.s, p.scale, 3 - warp, lane);
-    __syncwarp();  // the diagonal block is this warp's own
+    __syncwarp();  // the diagonal block is this warp's own, as are the rows of q
     {
         const int col = lane & 15, r0 = 16 * warp;
         float ti[16];
@@ -117,13 +120,13 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
             float x = i == col ? 1.f : 0.f, y = 0.f;
 #pragma unroll
             for (int j = 0; j < i; j += 2) {
-                const float2 a = *reinterpret_cast<const float2*>(&sm.A[r0 + i][r0 + j]);
+                const float2 a = *reinterpret_cast<const float2*>(&sm.A[tri(warp, warp)][i][j]);
                 x = fmaf(-a.x, ti[j], x);
                 if (j + 1 < i) y = fmaf(-a.y, ti[j + 1], y);
             }
             x += y;
             if (lane < 16) {
-                unsigned char* at = sm.Ti + warp * (NX * 512) + ((i >> 3) * 2 + (col >> 3)) * 128 + (i & 7) * 16 + (col & 7) * 2;
+                unsigned char* at = sm.q + sm.ti(warp) + ((i >> 3) * 2 + (col >> 3)) * 128 + (i & 7) * 16 + (col & 7) * 2;
                 float rest = x;
 #pragma unroll
                 for (int pl = 0; pl < NX; ++pl) {
@@ -140,7 +143,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
         const int J = warp;
         uint32_t y[4][NX][4];  // Y_KJ^T, K = J + index
         unsigned char* Y = p.Y + chunk * (NX * kYBlocks * 512);
-        const uint32_t ab = smem_addr(sm.Ab) + lane * 16, ti = smem_addr(sm.Ti) + lane * 16;
+        const uint32_t ab = smem_addr(sm.Ab) + lane * 16, ti = smem_addr(sm.q) + lane * 16;
         const float2 one = make_float2(1.f, 1.f);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
             for (int ih = 0; ih < 2; ++ih)
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {  // A_IJ^T: rows j, columns i
-                    acc[ih][v] = sm.A[16 * I + 8 * ih + 2 * t + (v & 1)][16 * J + g + 8 * (v >> 1)];
+                    acc[ih][v] = sm.A[tri(I, J)][8 * ih + 2 * t + (v & 1)][g + 8 * (v >> 1)];
                     out[ih][v] = 0.f;
                 }
 #pragma unroll
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
 #pragma unroll
             for (int pl = 0; pl < NX; ++pl) {
                 uint32_t r[4];
-                ldm(r, ti + (I * NX + pl) * 512);
+                ldm(r, ti + sm.ti(I) + pl * 512);
                 b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
             }
             mma_pair<NX, NX, NX>(out[0], out[1], a, b0, b1);
