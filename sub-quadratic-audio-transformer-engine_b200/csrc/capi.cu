@@ -454,7 +454,8 @@ int subq_head_rmsnorm_bwd(const subq_rmsnorm_args* a) {
 // ------------------------------------------------------------ gated delta rule
 namespace {
 
-// Calls of at most this many tokens take the token-recurrent kernel.
+// Calls of at most this many tokens take the token-recurrent kernel (12 heads of 64 x 64: 13 us at 8 tokens, 19.5 at 16,
+// 28 at 24 against 19.5 us for a chunk; 16 x 12 heads: 21.5 at 16 and 36 at 32 against 30; 256 x 12: 140 and 263 against 259).
 constexpr int kDeltaRecurrentMaxTokens = 16;
 
 int delta_gate(const subq_gate& g, const char* name, subq::DeltaGate& out) {
@@ -512,25 +513,29 @@ int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc&
     return SUBQ_OK;
 }
 
-// Segments of a sequence that are walked side by side when there are few sequences. A walk over n chunks takes n
-// steps of about t = 1.7 us whatever the number of CTAs, up to one CTA per SM. With G segments, a first pass (states
-// only, from the segments' value columns and the d columns of the identity) and the walk itself take n / G steps each,
-// times the waves of their CTAs, and the join about 0.8 us a segment and 8 us of launches. G is the count with the
-// least such time, taken where that is at least a fifth below the single walk's (B = 1, H = 4, N = 4096, d = e = 64:
-// G = 9, 162 -> 76 us measured; B = 8, H = 12: one).
+// Segments of a sequence that are walked side by side when there are few sequences. A walk over n chunks takes n steps
+// of about 1.7 us (bf16, d = e = 64) whatever the number of CTAs, up to one CTA per SM. With G segments a first pass
+// finds the states: the first segment's own state, for the others their own state and what they do to the one before
+// them, but for the last. Its steps take 1.2 us, or 1.75 us where two CTAs share an SM (16-bit inputs). The walk itself
+// then takes n / G steps, the join about 0.8 us a segment, and the two launches 8 us. G is the count with the least sum,
+// taken where that is a tenth below the single walk's. Measured with the gates' kernel, us, single and cut:
+//   1 x 12 heads, 65536 tokens   1827, 778 (G = 6)      2 x 12, 8192    266, 191 (G = 3)     1 x 4, 4096     121, 61 (G = 16)
+//   3 x 12 heads, 16384 tokens    553, 510 (G = 2)      4 x 12, 4096    162, none (213 with G = 2, more CTAs than SMs)
 struct DeltaSplit {
     int nseg, chunks;
 };
-DeltaSplit delta_split(const subq::DeltaParams& p) {
+DeltaSplit delta_split(const subq::DeltaParams& p, int dtype) {
     const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + 31) / 32, ndb = (p.d + 31) / 32;
-    constexpr double kStep = 1.7, kJoin = 0.8, kLaunch = 8.0;
-    auto waves = [](int64_t ctas) { return (double)((ctas + 147) / 148); };
-    double best = 0.8 * p.nc * kStep * waves(bh * ncb);
+    constexpr double kStep = 1.7, kStates = 1.2, kStatesShared = 1.75, kJoin = 0.8, kLaunch = 8.0;
+    auto waves = [](int64_t ctas, int64_t slots) { return (double)((ctas + slots - 1) / slots); };
+    double best = 0.9 * p.nc * kStep * waves(bh * ncb, 148);
     DeltaSplit s = {1, p.nc};
     for (int g = 2; g <= 64 && 2 * g <= p.nc; ++g) {
         const int chunks = (p.nc + g - 1) / g;
         if ((p.nc + chunks - 1) / chunks != g) continue;  // (the same split with fewer segments)
-        const double t = chunks * kStep * (waves(bh * g * ncb) + waves(bh * (g - 1) * (ncb + ndb))) + g * kJoin + kLaunch;
+        const int64_t ctas = bh * ((g - 1) * (ncb + ndb) - ndb);
+        const double states = dtype == SUBQ_FP32 || ctas <= 148 ? kStates * waves(ctas, 148) : kStatesShared * waves(ctas, 296);
+        const double t = chunks * (kStep * waves(bh * g * ncb, 148) + states) + g * kJoin + kLaunch;
         if (t < best) best = t, s = {g, chunks};
     }
     return s;
@@ -545,7 +550,7 @@ DeltaBytes delta_bytes(const subq::DeltaParams& p, int dtype) {
     const size_t nx = dtype == SUBQ_FP32 ? 3 : 2, chunks = (size_t)p.B * p.H * p.nc;
     const size_t ncw = 2 * ((p.e + subq::kDeltaCols - 1) / subq::kDeltaCols), dp = p.d <= 64 ? 64 : 128;
     const size_t mat = align_up(chunks * nx * subq::kYBlocks * 512);
-    const int nseg = delta_split(p).nseg;
+    const int nseg = delta_split(p, dtype).nseg;
     const size_t slots = (size_t)p.B * p.H * (nseg - 1) * sizeof(float);
     const size_t copy = nseg > 1 && p.S_in && p.S_in == p.S_out ? (size_t)p.B * p.H * p.d * p.e * sizeof(float) : 0;
     return {align_up(chunks * sizeof(subq::DeltaGates)), mat, mat, align_up(chunks * ncw * (dp / 16) * nx * 512),
@@ -560,8 +565,8 @@ void delta_handover(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
     p.W = p.S0 + n.S0;
 }
 
-void delta_segments(subq::DeltaParams& p, const DeltaBytes& n, void* at) {
-    const DeltaSplit s = delta_split(p);
+void delta_segments(subq::DeltaParams& p, int dtype, const DeltaBytes& n, void* at) {
+    const DeltaSplit s = delta_split(p, dtype);
     p.nseg = s.nseg;
     p.seg_chunks = s.chunks;
     p.seg_S = static_cast<float*>(at);
@@ -681,7 +686,7 @@ int subq_delta_fwd(const subq_delta_fwd_args* a) {
         const DeltaBytes n = delta_bytes(p, a->desc.dtype);
         const size_t segs = n.segs();
         if ((rc = check_workspace(a->workspace, a->workspace_bytes, segs + (a->handover ? 0 : n.gates + n.Y + n.P)))) return rc;
-        delta_segments(p, n, a->workspace);
+        delta_segments(p, a->desc.dtype, n, a->workspace);
         if (a->handover) {
             if (reinterpret_cast<uintptr_t>(a->handover) % kAlign != 0)
                 return fail(SUBQ_ERR_WORKSPACE, "handover must be 256-byte aligned");
@@ -734,7 +739,7 @@ int subq_delta_bwd(const subq_delta_bwd_args* a) {
             return fail(SUBQ_ERR_WORKSPACE, "handover must be 256-byte aligned");
         delta_handover(p, n.fwd, const_cast<void*>(a->handover));
     } else {
-        delta_segments(p, n.fwd, at);
+        delta_segments(p, dt, n.fwd, at);
         delta_handover(p, n.fwd, at + n.fwd.segs());
         err = subq::launch_delta_fwd(p, dt, st);  // (o is null: states and corrections only)
         first = p.nseg > 1 ? 4 : 2;

@@ -189,32 +189,35 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
 }
 
 // ------------------------------------------------------------------ the walk
-template <typename T, int DP>
+// STATES: a walk for the states alone, without outputs and their operands.
+template <typename T, int DP, bool STATES>
 struct ChainSmem {
     static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
     // chunks in shared memory: the one at work and the next; where they fit, one more on its way, and the last one for
     // the output warps, which then finish a chunk while the chain is at the next
-    static constexpr int kStages = kIn == 1 ? (DP == 64 ? 4 : 2) : DP == 64 ? 2 : 1;
+    static constexpr int kStages = kIn == 1 ? (DP == 64 ? (STATES ? 3 : 4) : 2) : DP == 64 ? 2 : 1;
     static constexpr bool kLag = kStages == 4;
     struct Stage {
         alignas(128) unsigned char k[kIn * 64 * DP * 2];
-        alignas(128) unsigned char q[kIn * 64 * DP * 2];
+        alignas(128) unsigned char q[STATES ? 16 : kIn * 64 * DP * 2];
         alignas(128) unsigned char v[kIn * 64 * kDeltaCols * 2];
         alignas(128) unsigned char y[kX * kYBlocks * 512];
-        alignas(128) unsigned char P[kX * kYBlocks * 512];
+        alignas(128) unsigned char P[STATES ? 16 : kX * kYBlocks * 512];
         Gates s;
     } st[kStages];
+    // threads: the chain's 128, the output warps' 128, the loading 128; CTAs per SM
+    static constexpr int kThreads = STATES ? 256 : 384, kChain = STATES ? 128 : 256;
     // by pair of warps
     alignas(16) unsigned char S0[2][DP / 16][kX * 512];  // S^T before the chunk, planes
     alignas(16) unsigned char R[2][4][kX * 512];         // -(beta R)^T, planes
     // W^T for the update and the outputs. 16-bit inputs: planes of beta W and of e^{g_C - g} beta W (and of W where
     // it is kept), converted once by the warp that has it; float32 ones (no room): W, converted by each reader
     static constexpr bool kShared = kX == 2;
-    alignas(16) unsigned char Wb[kLag ? 2 : 1][2][kShared ? 4 : 1][kX * 512];  // (by chunk parity where outputs lag)
+    alignas(16) unsigned char Wb[kLag ? 2 : 1][2][kShared && !STATES ? 4 : 1][kX * 512];  // (by chunk parity where outputs lag)
     alignas(16) unsigned char Wk[2][kShared ? 4 : 1][kX * 512];
     union {
-        float4 W[2][8 * 32];
-        unsigned char Wp[2][4][1024];
+        float4 W[2][kShared ? 1 : 8 * 32];
+        unsigned char Wp[2][STATES ? 1 : 4][1024];
     } w;
     // outputs on their way to memory: in the place of Y, which nobody reads any more by then
     static constexpr int kOutPitch = 16 * sizeof(T) + 16;
@@ -223,10 +226,10 @@ struct ChainSmem {
 
 // One warp of a chain pair: half `A` of d of S^T in its accumulators; R and W of its token blocks.
 template <typename T, int DP, bool OUT, bool KEEP>
-__device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP>::kStages;
+__device__ __forceinline__ void chain_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP, !OUT && !KEEP>::kStages;
     constexpr int NH = DP / 16;  // 8-column blocks of half of d
-    constexpr bool kShared = ChainSmem<T, DP>::kShared;
+    constexpr bool kShared = ChainSmem<T, DP, !OUT && !KEEP>::kShared;
     const int g = lane >> 2, t = lane & 3;
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
@@ -318,7 +321,7 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
                     put_a<NX>(sm.Wk[pair][jb], a, lane);
                     if (OUT) {
                         to_a<NX>(W[2 * u], W[2 * u + 1], fb[0], fb[1], a);
-                        put_a<NX>(sm.Wb[ChainSmem<T, DP>::kLag ? c & 1 : 0][pair][jb], a, lane);
+                        put_a<NX>(sm.Wb[ChainSmem<T, DP, !OUT && !KEEP>::kLag ? c & 1 : 0][pair][jb], a, lane);
                     }
                     if (KEEP) {
                         to_a<NX>(W[2 * u], W[2 * u + 1], one, one, a);
@@ -333,7 +336,7 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
             for (int n = 0; n < NH; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) S[n][i] *= s.eC;
-            bar_sync(1, 256);  // W is there for both pairs and the output warps, which have read S0
+            bar_sync(1, ChainSmem<T, DP, !OUT && !KEEP>::kChain);  // W is there for both pairs and the output warps, which have read S0
 #pragma unroll
             for (int jb = 0; jb < 4; ++jb) {  // S'^T = e^{g_C} S0^T + (e^{g_C - g} beta W)^T K over this half of d
                 uint32_t a[NX][4];
@@ -370,19 +373,19 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP>& sm, const DeltaPara
 
 // One warp of an output pair: the outputs of 16 columns for its token blocks, and its share of the planes.
 template <typename T, int DP, bool OUT, bool KEEP>
-__device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP>::kStages;
+__device__ __forceinline__ void output_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP, !OUT && !KEEP>::kStages;
     const int g = lane >> 2, t = lane & 3;
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
     const int64_t bh = job.bh;
     const int cb = job.cb, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
     T* o = OUT ? static_cast<T*>(p.o.p) + tensor_base(p.o, job.b, job.h) : nullptr;
-    constexpr bool kShared = ChainSmem<T, DP>::kShared;
-    constexpr int kPitch = ChainSmem<T, DP>::kOutPitch, kPieces = 16 * sizeof(T) / 16;  // bytes of a staged row, its 16-byte pieces
+    constexpr bool kShared = ChainSmem<T, DP, !OUT && !KEEP>::kShared;
+    constexpr int kPitch = ChainSmem<T, DP, !OUT && !KEEP>::kOutPitch, kPieces = 16 * sizeof(T) / 16;  // bytes of a staged row, its 16-byte pieces
     const int col0 = cb * kDeltaCols + 16 * pair, width = min(16, p.e - col0);
     const bool whole = OUT && p.o.vec && width == 16;
-    constexpr bool kLag = ChainSmem<T, DP>::kLag;
+    constexpr bool kLag = ChainSmem<T, DP, !OUT && !KEEP>::kLag;
     float O[4][4];  // blocks 2 u + half of this warp's tokens
     auto planes_of_w = [&](int c) {
         const int64_t cw = (bh * p.nc + c) * 2 * ncb + 2 * cb + pair;
@@ -490,27 +493,36 @@ __device__ __forceinline__ void output_warp(ChainSmem<T, DP>& sm, const DeltaPar
 }
 
 // OUT: writes o. KEEP: writes the planes of S0 and W that the backward reads.
+// Neither: the states alone, in half the shared memory, so that two CTAs share an SM.
+template <typename T, int DP, bool STATES>
+constexpr int chain_ctas() {
+    return STATES && sizeof(ChainSmem<T, DP, STATES>) <= 112 * 1024 ? 2 : 1;
+}
+
 template <typename T, int DP, bool OUT, bool KEEP>
-__global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX;
-    constexpr int NST = ChainSmem<T, DP>::kStages;
-    extern __shared__ __align__(128) unsigned char raw[];
-    ChainSmem<T, DP>& sm = *reinterpret_cast<ChainSmem<T, DP>*>(raw);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // (sequence, segment, block of columns), the last fastest. States only (neither OUT nor KEEP): the first
-    // nseg - 1 segments, with the identity's columns after the value columns
+__global__ void __launch_bounds__(ChainSmem<T, DP, !OUT && !KEEP>::kThreads, chain_ctas<T, DP, !OUT && !KEEP>())
+delta_chain_kernel(const DeltaParams p) {
     constexpr bool kStates = !OUT && !KEEP;
-    const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols, ncols = ncb + (kStates ? (p.d + kDeltaCols - 1) / kDeltaCols : 0);
+    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX;
+    constexpr int NST = ChainSmem<T, DP, kStates>::kStages;
+    extern __shared__ __align__(128) unsigned char raw[];
+    using Smem = ChainSmem<T, DP, kStates>;
+    Smem& sm = *reinterpret_cast<Smem*>(raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // (sequence, segment, block of columns), the last fastest. States only: the first nseg - 1 segments, with the
+    // identity's columns after the value columns, but for the first segment (nobody asks what it does to a state)
+    const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols, ndb = kStates ? (p.d + kDeltaCols - 1) / kDeltaCols : 0, ncols = ncb + ndb;
     const int nseg = kStates ? p.nseg - 1 : p.nseg;
-    const unsigned sq = blockIdx.x / (unsigned)ncols, bh32 = sq / (unsigned)nseg;
-    const int seg = (int)(sq - bh32 * nseg);
+    const unsigned per_seq = (unsigned)(nseg * ncols - ndb), bh32 = blockIdx.x / per_seq;
+    const int at = (int)(blockIdx.x - bh32 * per_seq) + ndb;  // (the first segment's columns at ndb ..)
+    const int seg = at / ncols, col = at - seg * ncols;
     WalkJob job;
     job.bh = bh32;
     job.b = (int)(bh32 / (unsigned)p.H);
     job.h = (int)(bh32 - job.b * (unsigned)p.H);
-    job.cb = (int)(blockIdx.x - sq * ncols);
-    job.ident = kStates && job.cb >= ncb;
-    job.c0 = (job.ident ? job.cb - ncb : job.cb) * kDeltaCols;
+    job.ident = kStates && col < ndb;
+    job.cb = job.ident ? col : col - ndb;
+    job.c0 = job.cb * kDeltaCols;
     job.begin = seg * p.seg_chunks;
     job.end = min(p.nc, job.begin + p.seg_chunks);
     job.ld = job.ident ? DP : p.e;
@@ -526,11 +538,11 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
     }
     if (warp < 4) {
         chain_warp<T, DP, OUT, KEEP>(sm, p, job, warp & 1, warp >> 1, lane);
-    } else if (warp < 8) {
-        output_warp<T, DP, OUT, KEEP>(sm, p, job, warp & 1, (warp >> 1) & 1, lane);
+    } else if (!kStates && warp < 8) {
+        if constexpr (!kStates) output_warp<T, DP, OUT, KEEP>(sm, p, job, warp & 1, (warp >> 1) & 1, lane);
     } else {  // ---------------------------------------------------------- loads
         // the loads of a chunk are in flight for a whole iteration or two
-        const int lt = tid - 256;
+        const int lt = tid - Smem::kChain;
         const int64_t bh = job.bh;
         const int b = job.b, h = job.h, begin = job.begin, end = job.end, c0 = job.c0;
         const Gates* gates = p.gates + bh * p.nc;
@@ -547,7 +559,7 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
         if constexpr (NIN == 1) async = p.k.vec && p.q.vec && p.v.vec && p.d % 8 == 0 && p.e % 8 == 0;
         if (async) {
             // bf16: asynchronous copies, chunk c + kAhead started while c is computed
-            constexpr int kAhead = NST > 2 ? NST - 2 : 1;
+            constexpr int kAhead = Smem::kLag ? NST - 2 : NST > 1 ? NST - 1 : 1;
             int any_next = gates[begin].any;
             auto start = [&](int c) {
                 if (c < end) {
@@ -560,7 +572,7 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
                         async_tile<T, DP, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, lt);
                         if (!job.ident) async_tile<T, kDeltaCols, 128>(st.v, p.v, vb, n0, c0, p.e, p.N, lt);
                         async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
-                        if (OUT) {
+                        if constexpr (OUT) {
                             async_tile<T, DP, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, lt);
                             async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
                         }
@@ -575,7 +587,7 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
                 auto& st = sm.st[c % NST];
                 if (st.s.any && !st.s.full) {
                     clear_dead<DP, 128>(st.k, st.s.live, lt);
-                    if (OUT) clear_dead<DP, 128>(st.q, st.s.live, lt);
+                    if constexpr (OUT) clear_dead<DP, 128>(st.q, st.s.live, lt);
                     clear_dead<kDeltaCols, 128>(st.v, st.s.live, lt);
                 }
             };
@@ -600,7 +612,7 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
                         load_tile<T, DP, NIN, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, st.s.live, lt);
                         if (!job.ident) load_tile<T, kDeltaCols, NIN, 128>(st.v, p.v, vb, n0, c0, p.e, p.N, st.s.live, lt);
                         async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
-                        if (OUT) {
+                        if constexpr (OUT) {
                             load_tile<T, DP, NIN, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, st.s.live, lt);
                             async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
                         }
@@ -623,7 +635,7 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
                     const int n0 = c * kDeltaC;
                     k.issue(p.k, kb, n0, 0, p.d, p.N, lt);
                     if (!job.ident) v.issue(p.v, vb, n0, c0, p.e, p.N, lt);
-                    if (OUT) {
+                    if constexpr (OUT) {
                         q.issue(p.q, qb, n0, 0, p.d, p.N, lt);
                     }
                 };
@@ -634,10 +646,10 @@ __global__ void __launch_bounds__(384, 1) delta_chain_kernel(const DeltaParams p
                     bar_sync(3, 128);
                     if (!any) return;
                     async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
-                    if (OUT) async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
+                    if constexpr (OUT) async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
                     k.template store_planes<NIN>(st.k, st.s.live, lt);
                     if (!job.ident) v.template store_planes<NIN>(st.v, st.s.live, lt);
-                    if (OUT) {
+                    if constexpr (OUT) {
                         q.template store_planes<NIN>(st.q, st.s.live, lt);
                     }
                 };
@@ -676,9 +688,11 @@ __global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
     float4 m[kLoad];
     float l[kRows];
     auto load = [&](int s) {
-        const float4* src = reinterpret_cast<const float4*>(p.seg_M + (slot + s) * (DP * DP));
+        if (s > 0) {
+            const float4* src = reinterpret_cast<const float4*>(p.seg_M + (slot + s) * (DP * DP));
 #pragma unroll
-        for (int i = 0; i < kLoad; ++i) m[i] = src[threadIdx.x + 256 * i];
+            for (int i = 0; i < kLoad; ++i) m[i] = src[threadIdx.x + 256 * i];
+        }
         const float* add = p.seg_S + (slot + s) * p.d * p.e + c;
 #pragma unroll
         for (int k = 0; k < kRows; ++k) l[k] = r0 + 16 * k < p.d && c < p.e ? add[(r0 + 16 * k) * p.e] : 0.f;
@@ -731,17 +745,18 @@ __global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
 
 template <typename T, int DP>
 cudaError_t chain_t(const DeltaParams& p, cudaStream_t st) {
-    const size_t smem = sizeof(ChainSmem<T, DP>);
-    static_assert(sizeof(ChainSmem<T, DP>) <= 227 * 1024, "shared memory");
+    using Walk = ChainSmem<T, DP, false>;
+    using States = ChainSmem<T, DP, true>;
+    static_assert(sizeof(Walk) <= 227 * 1024 && sizeof(States) <= 227 * 1024, "shared memory");
     const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + kDeltaCols - 1) / kDeltaCols, ndb = (p.d + kDeltaCols - 1) / kDeltaCols;
-    auto run = [&](auto kernel, int64_t blocks) {
+    auto run = [&](auto kernel, int64_t blocks, int threads = Walk::kThreads, size_t smem = sizeof(Walk)) {
         cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (err != cudaSuccess) return err;
-        kernel<<<(unsigned)blocks, 384, smem, st>>>(p);
+        kernel<<<(unsigned)blocks, threads, smem, st>>>(p);
         return cudaGetLastError();
     };
     if (p.nseg > 1) {
-        cudaError_t err = run(delta_chain_kernel<T, DP, false, false>, bh * (p.nseg - 1) * (ncb + ndb));
+        cudaError_t err = run(delta_chain_kernel<T, DP, false, false>, bh * ((p.nseg - 1) * (ncb + ndb) - ndb), States::kThreads, sizeof(States));
         if (err != cudaSuccess) return err;
         const int join = DP * (DP + 4 + 16) * (int)sizeof(float);
         err = cudaFuncSetAttribute(delta_join_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, join);
