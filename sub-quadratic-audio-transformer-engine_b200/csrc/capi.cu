@@ -513,29 +513,34 @@ int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc&
     return SUBQ_OK;
 }
 
-// Segments of a sequence that are walked side by side when there are few sequences. A walk over n chunks takes n steps
-// of about 1.7 us (bf16, d = e = 64) whatever the number of CTAs, up to one CTA per SM. With G segments a first pass
-// finds the states: the first segment's own state, for the others their own state and what they do to the one before
-// them, but for the last. Its steps take 1.2 us, or 1.75 us where two CTAs share an SM (16-bit inputs). The walk itself
-// then takes n / G steps, the join about 0.8 us a segment, and the two launches 8 us. G is the count with the least sum,
-// taken where that is a tenth below the single walk's. Measured with the gates' kernel, us, single and cut:
-//   1 x 12 heads, 65536 tokens   1827, 778 (G = 6)      2 x 12, 8192    266, 191 (G = 3)     1 x 4, 4096     121, 61 (G = 16)
-//   3 x 12 heads, 16384 tokens    553, 510 (G = 2)      4 x 12, 4096    162, none (213 with G = 2, more CTAs than SMs)
+// Segments of a sequence that are walked side by side when there are few sequences. A walk over n chunks takes n steps of
+// a time that depends on the type and d (below) and not on the number of CTAs, up to one CTA per SM. With G segments a
+// first pass finds the states: the first segment's own state, for the others their own state and what they do to the one
+// before them, but for the last. Its steps take 0.7 of the walk's, or 1.1 where two CTAs share an SM (16-bit inputs). The
+// walk itself then takes n / G steps, the join 1 us a segment (2 us above d = 64), and the two launches 8 us. G is the
+// count with the least sum, taken where that is a tenth below the single walk's. Measured with the gates' kernel, us,
+// single and cut (the counts beside G were at most 4 % faster):
+//   bf16, d = 64:  1 x 12 heads, 65536 tokens   1822, 778 (G = 6)    2 x 12, 8192     267, 191 (G = 3)   1 x 4, 4096   122, 60 (G = 9)
+//                  3 x 12 heads, 16384 tokens    554, 510 (G = 2)    4 x 12, 4096     162, none (G = 2: 213, more CTAs than SMs)
+//   float32:       2 x 12 heads, 1537 tokens     148, 124 (G = 3)    1 x 4, 16384    1112, 243 (G = 18)
+//   d = 128:       1 x 4 heads, 8192 tokens      319, 134 (bf16, G = 8)   835, 251 (float16, G = 9)   1228, 441 (float32, G = 6)
 struct DeltaSplit {
     int nseg, chunks;
 };
 DeltaSplit delta_split(const subq::DeltaParams& p, int dtype) {
     const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + 31) / 32, ndb = (p.d + 31) / 32;
-    constexpr double kStep = 1.7, kStates = 1.2, kStatesShared = 1.75, kJoin = 0.8, kLaunch = 8.0;
+    const int wide = p.d > 64;
+    constexpr double kSteps[3][2] = {{4.3, 9.2}, {2.5, 6.4}, {1.7, 2.3}};  // us: float32, float16, bfloat16
+    const double step = kSteps[dtype == SUBQ_FP32 ? 0 : dtype == SUBQ_FP16 ? 1 : 2][wide], join = wide ? 2.0 : 1.0, launches = 8.0;
     auto waves = [](int64_t ctas, int64_t slots) { return (double)((ctas + slots - 1) / slots); };
-    double best = 0.9 * p.nc * kStep * waves(bh * ncb, 148);
+    double best = 0.9 * p.nc * step * waves(bh * ncb, 148);
     DeltaSplit s = {1, p.nc};
     for (int g = 2; g <= 64 && 2 * g <= p.nc; ++g) {
         const int chunks = (p.nc + g - 1) / g;
         if ((p.nc + chunks - 1) / chunks != g) continue;  // (the same split with fewer segments)
         const int64_t ctas = bh * ((g - 1) * (ncb + ndb) - ndb);
-        const double states = dtype == SUBQ_FP32 || ctas <= 148 ? kStates * waves(ctas, 148) : kStatesShared * waves(ctas, 296);
-        const double t = chunks * (kStep * waves(bh * g * ncb, 148) + states) + g * kJoin + kLaunch;
+        const double states = dtype == SUBQ_FP32 || ctas <= 148 ? 0.7 * waves(ctas, 148) : 1.1 * waves(ctas, 296);
+        const double t = chunks * step * (waves(bh * g * ncb, 148) + states) + g * join + launches;
         if (t < best) best = t, s = {g, chunks};
     }
     return s;

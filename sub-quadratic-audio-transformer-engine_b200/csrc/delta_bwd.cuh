@@ -20,6 +20,11 @@
 // for t. (The shorter running sum of q_i.dq_i - v_i.dv_i is the same in exact
 // arithmetic, but keeps the errors of tokens that have nothing to do with t: 3e-5
 // against 5e-6 with 16-bit inputs and fast decay.)
+//
+// Measured, bf16, d = e = 64, 8 x 8 heads of 8192 tokens (8192 chunks): the walk back
+// 275 us (2.1 us a chunk, bound like the forward's by shared memory and the latency of
+// its three products in a row), the gradients 400 us (105 KB read and written a chunk,
+// 0.33 of measured HBM; tensor pipe 41 %, shared memory 52 %, 16 warps per SM).
 #pragma once
 
 #include "delta_common.cuh"

@@ -59,7 +59,7 @@ struct DeltaParams {
     // segments of a sequence walked side by side (few sequences): 1, or more than 1 with `seg_S` and `seg_M`
     int nseg, seg_chunks;
     float* seg_S;  // [B * H][nseg - 1][d, e]: state after a segment
-    float* seg_M;  // [B * H][nseg - 1][dp, dp] (d padded): what a segment does to the state before it
+    float* seg_M;  // [B * H][nseg - 1][dp, dp] (d padded): what a segment does to the state before it, transposed
     float* seg_in;  // [B * H][d, e]: copy of S_in where S_out is S_in (one CTA reads it, another writes it), else null
     // backward
     DeltaTensor g, dq, dk, dv;

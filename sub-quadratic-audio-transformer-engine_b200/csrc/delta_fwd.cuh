@@ -11,6 +11,13 @@
 // CTA, 32 columns: two such pairs; two pairs of output warps (Q S0 and score W
 // products; they also write the planes that the backward reads); and four warps
 // that load the next chunks. Each SM sub-partition has one warp of each kind.
+// (Four warps per 16 columns move each operand through shared memory twice as often
+// and were slower.)
+//
+// Measured, bf16, d = e = 64, 8 x 8 heads of 8192 tokens (8192 chunks): gates and Y
+// 100 us (issue-bound: 46 % of the issue slots with 24 warps per SM, tensor pipe 17 %);
+// the walk 1.7 us a chunk, 1.9 us where the backward's planes are written (247 us:
+// shared memory 76 % busy on the SMs at work, tensor pipe 35 %).
 #pragma once
 
 #include "delta_common.cuh"
@@ -366,7 +373,7 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
-                if (d < job.rows && col < job.ld) job.out[(int64_t)d * job.ld + col] = S[n][i];
+                if (d < job.rows && col < job.ld) job.out[job.ident ? (int64_t)col * job.ld + d : (int64_t)d * job.ld + col] = S[n][i];
             }
     }
 }
@@ -558,7 +565,8 @@ delta_chain_kernel(const DeltaParams p) {
         bool async = false;
         if constexpr (NIN == 1) async = p.k.vec && p.q.vec && p.v.vec && p.d % 8 == 0 && p.e % 8 == 0;
         if (async) {
-            // bf16: asynchronous copies, chunk c + kAhead started while c is computed
+            // bf16: asynchronous copies, chunk c + kAhead started while c is computed (8 x 12 heads of 2047 tokens: 169 us
+            // with the gates' kernel and rows on 16 bytes, 341 us through registers, element by element, without)
             constexpr int kAhead = Smem::kLag ? NST - 2 : NST > 1 ? NST - 1 : 1;
             int any_next = gates[begin].any;
             auto start = [&](int c) {
@@ -670,77 +678,87 @@ delta_chain_kernel(const DeltaParams p) {
 }
 
 // ------------------------------------------------------------------ segments
-// seg_S[s] <- seg_M[s] S_s + seg_S[s] (what segment s makes of the state before it, S_s), s in order: seg_S[s - 1] is
-// then the state before segment s. (The first segment's own state already holds what came before it: its walk started
-// from the initial state.) A CTA has 16 columns of one sequence, a thread one column of every 16th row; the next
-// segment's operands are on their way, in registers, while one is computed (0.8 us a segment at d = 64 against 8 us
-// without).
+// seg_S[s] <- M_s S_s + seg_S[s] (what segment s makes of the state before it, S_s), s in order: seg_S[s - 1] is then the
+// state before segment s. (The first segment's own state already holds what came before it: its walk started from the
+// initial state.) seg_M holds M_s^T. A CTA has 16 columns of one sequence, a thread four rows of two of them, so that two
+// loads from shared memory feed eight multiplications; the operands of the next segments (three, two above d = 64) are on
+// their way while one is computed (about 1 us a segment at d = 64; 8 us where each waited for its own).
 template <int DP>
-__global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
-    constexpr int kRows = DP / 16, kLoad = DP * DP / 1024;  // rows a thread has, float4 pieces of M a thread loads
-    constexpr int kPitch = DP + 4;
-    extern __shared__ __align__(16) float sm_join[];
-    float* M = sm_join;               // [DP][kPitch]
-    float* S = sm_join + DP * kPitch;  // [DP][16]
+struct JoinSmem {
+    static constexpr int kThreads = 2 * DP, kBufs = DP == 64 ? 4 : 3;
+    alignas(16) float M[kBufs][DP * DP];  // [DP][DP], transposed
+    float S[2][DP * 16];
+};
+template <int DP>
+__global__ void __launch_bounds__(2 * DP) delta_join_kernel(const DeltaParams p) {
+    constexpr int kThreads = JoinSmem<DP>::kThreads, kBufs = JoinSmem<DP>::kBufs, kAhead = kBufs - 1;
+    extern __shared__ __align__(16) unsigned char raw[];
+    JoinSmem<DP>& sm = *reinterpret_cast<JoinSmem<DP>*>(raw);
     const unsigned ncb = (p.e + 15) / 16, bh32 = blockIdx.x / ncb;
     const int64_t slot = (int64_t)bh32 * (p.nseg - 1);
-    const int col = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = (int)(blockIdx.x - bh32 * ncb) * 16 + col;
-    float4 m[kLoad];
-    float l[kRows];
-    auto load = [&](int s) {
-        if (s > 0) {
-            const float4* src = reinterpret_cast<const float4*>(p.seg_M + (slot + s) * (DP * DP));
-#pragma unroll
-            for (int i = 0; i < kLoad; ++i) m[i] = src[threadIdx.x + 256 * i];
-        }
+    const int tid = threadIdx.x, r0 = tid / 8 * 4, cl = tid % 8 * 2, c = (int)(blockIdx.x - bh32 * ncb) * 16 + cl, last = p.nseg - 2;
+    auto send = [&](int s) {
+        if (s <= last) async16<kThreads>(reinterpret_cast<unsigned char*>(sm.M[s % kBufs]),
+                                         reinterpret_cast<const unsigned char*>(p.seg_M + (slot + s) * (DP * DP)), DP * DP * 4, tid);
+        async_commit();
+    };
+    auto load = [&](float (&l)[4][2], int s) {
         const float* add = p.seg_S + (slot + s) * p.d * p.e + c;
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) l[k] = r0 + 16 * k < p.d && c < p.e ? add[(r0 + 16 * k) * p.e] : 0.f;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) l[i][j] = s <= last && r0 + i < p.d && c + j < p.e ? add[(r0 + i) * p.e + j] : 0.f;
     };
-    load(0);
+    for (int s = 1; s <= kAhead; ++s) send(s);
+    float l[4][2], next[4][2], after[4][2];
+    load(l, 0);
+    load(next, 1);
+    load(after, 2);
     if (p.seg_in) {
         const int64_t at = (int64_t)bh32 * p.d * p.e + c;
 #pragma unroll
-        for (int k = 0; k < kRows; ++k)
-            if (r0 + 16 * k < p.d && c < p.e) p.seg_in[at + (r0 + 16 * k) * p.e] = p.S_in[at + (r0 + 16 * k) * p.e];
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (r0 + i < p.d && c + j < p.e) p.seg_in[at + (r0 + i) * p.e + j] = p.S_in[at + (r0 + i) * p.e + j];
     }
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) S[(r0 + 16 * k) * 16 + col] = l[k];
-    if (p.nseg > 2) load(1);
-    for (int s = 1; s + 1 < p.nseg; ++s) {
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(&sm.S[0][(r0 + i) * 16 + cl]) = make_float2(l[i][0], l[i][1]);
+    for (int s = 1; s <= last; ++s) {
+        const float* M = sm.M[s % kBufs];
+        const float* S = sm.S[(s - 1) & 1];
+        float acc[4][2];
 #pragma unroll
-        for (int i = 0; i < kLoad; ++i) {
-            const int x = (threadIdx.x + 256 * i) * 4;
-            *reinterpret_cast<float4*>(&M[(x / DP) * kPitch + x % DP]) = m[i];
-        }
-        float acc[kRows];
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) acc[k] = l[k];
-        __syncthreads();
-        if (s + 2 < p.nseg) load(s + 1);
+            for (int j = 0; j < 2; ++j) acc[i][j] = next[i][j], next[i][j] = after[i][j];
+        async_wait_but<kAhead - 1>();  // this thread's pieces of M_s
+        __syncthreads();               // everyone's, and S; M_{s - 1} has been read
+        send(s + kAhead);
+        load(after, s + 2);
         // (rows and columns from d: S is 0 there, and M, the identity's columns that were walked, finite; columns of M
         // that were not walked are left out by the bound)
         const int end = (p.d + 31) / 32 * 32;
-#pragma unroll 4
-        for (int x = 0; x < end; x += 4) {
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = S[(x + i) * 16 + col];
-#pragma unroll
-            for (int k = 0; k < kRows; ++k) {
-                const float4 w = *reinterpret_cast<const float4*>(&M[(r0 + 16 * k) * kPitch + x]);
-                acc[k] = fmaf(w.w, v[3], fmaf(w.z, v[2], fmaf(w.y, v[1], fmaf(w.x, v[0], acc[k]))));
-            }
+#pragma unroll 8
+        for (int x = 0; x < end; ++x) {
+            const float4 w = *reinterpret_cast<const float4*>(&M[x * DP + r0]);
+            const float2 v = *reinterpret_cast<const float2*>(&S[x * 16 + cl]);
+            acc[0][0] = fmaf(w.x, v.x, acc[0][0]); acc[0][1] = fmaf(w.x, v.y, acc[0][1]);
+            acc[1][0] = fmaf(w.y, v.x, acc[1][0]); acc[1][1] = fmaf(w.y, v.y, acc[1][1]);
+            acc[2][0] = fmaf(w.z, v.x, acc[2][0]); acc[2][1] = fmaf(w.z, v.y, acc[2][1]);
+            acc[3][0] = fmaf(w.w, v.x, acc[3][0]); acc[3][1] = fmaf(w.w, v.y, acc[3][1]);
         }
-        __syncthreads();
-        float* after = p.seg_S + (slot + s) * p.d * p.e + c;
+        float* out = p.seg_S + (slot + s) * p.d * p.e + c;
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) {
-            const bool in = r0 + 16 * k < p.d && c < p.e;
-            S[(r0 + 16 * k) * 16 + col] = in ? acc[k] : 0.f;
-            if (in) after[(r0 + 16 * k) * p.e] = acc[k];
+        for (int i = 0; i < 4; ++i) {
+            const bool row = r0 + i < p.d, in[2] = {row && c < p.e, row && c + 1 < p.e};
+            *reinterpret_cast<float2*>(&sm.S[s & 1][(r0 + i) * 16 + cl]) = make_float2(in[0] ? acc[i][0] : 0.f, in[1] ? acc[i][1] : 0.f);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (in[j]) out[(r0 + i) * p.e + j] = acc[i][j];
         }
     }
+    async_wait();
 }
 
 template <typename T, int DP>
@@ -758,10 +776,10 @@ cudaError_t chain_t(const DeltaParams& p, cudaStream_t st) {
     if (p.nseg > 1) {
         cudaError_t err = run(delta_chain_kernel<T, DP, false, false>, bh * ((p.nseg - 1) * (ncb + ndb) - ndb), States::kThreads, sizeof(States));
         if (err != cudaSuccess) return err;
-        const int join = DP * (DP + 4 + 16) * (int)sizeof(float);
+        const int join = (int)sizeof(JoinSmem<DP>);
         err = cudaFuncSetAttribute(delta_join_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, join);
         if (err != cudaSuccess) return err;
-        delta_join_kernel<DP><<<(unsigned)(bh * ((p.e + 15) / 16)), 256, join, st>>>(p);
+        delta_join_kernel<DP><<<(unsigned)(bh * ((p.e + 15) / 16)), 2 * DP, join, st>>>(p);
         if ((err = cudaGetLastError()) != cudaSuccess) return err;
     }
     if (!p.o.p) return run(delta_chain_kernel<T, DP, false, true>, bh * p.nseg * ncb);

@@ -13,7 +13,7 @@ struct DeltaParams;
 
 // Token-recurrent forward, any d, e <= 256 (delta_step.cu); S_out may be S_in.
 cudaError_t launch_delta_step(const DeltaParams& p, int dtype, cudaStream_t st);
-// Chunked forward, d <= 128 (delta_fwd.cuh): fills p.gates, p.Y and p.P, then walks the chunks. 2 launches.
+// Chunked forward, d <= 128 (delta_fwd.cuh): fills p.gates, p.Y and p.P, then walks the chunks. 2 launches, 4 with segments.
 cudaError_t launch_delta_fwd_bf16(const DeltaParams& p, cudaStream_t st);
 cudaError_t launch_delta_fwd_fp16(const DeltaParams& p, cudaStream_t st);
 cudaError_t launch_delta_fwd_fp32(const DeltaParams& p, cudaStream_t st);

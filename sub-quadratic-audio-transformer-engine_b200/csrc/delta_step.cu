@@ -143,7 +143,7 @@ cudaError_t step_t(const DeltaParams& p, cudaStream_t st) {
         return cudaGetLastError();
     };
     // two warps a tile: the work around a tile's 2048 state elements (d = 64) is as much as theirs, so fewer threads
-    // with more elements each are faster (256 x 12 heads of 64 x 64: 26.6 us with four warps)
+    // with more elements each are faster (256 x 12 heads of 64 x 64: 24.6 us, 26.6 us with four warps)
     const bool full = vec && p.e % 32 == 0;
     if (p.d <= 32) return run(delta_step_kernel<T, 4, 2, false>, 64, 12);
     if (p.d == 64 && full) return run(delta_step_kernel<T, 8, 2, true>, 64, 10);

@@ -14,8 +14,8 @@
 // summed by a second kernel in a fixed order (bitwise reproducible). Rows longer than
 // the registers hold (D > 8192) are read again per pass, from L2.
 // 65536 x 768, float32 -> bf16: forward 49 us (94 % of the measured copy bandwidth),
-// backward 108 us (71 %: the sums of a row wait for its loads, and the registers that
-// hold x, dy, dw and db leave room for two CTAs per SM).
+// backward 106 us (73 %: the registers that hold x, dy, dw and db leave room for two
+// CTAs per SM, whose two sums a row are not hidden).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
