@@ -418,3 +418,69 @@ def test_buffers_that_do_not_belong_to_the_call_are_refused():
     ho.buf = ho.buf[::2]
     with pytest.raises(ValueError):
         ops.gated_delta_backward(q, k, v, beta, do, handover=ho)
+
+
+@pytest.mark.parametrize("path", ["exact", "chunked"])
+def test_offsets_beyond_32_bits(path):
+    """Tokens 2^26 elements apart, heads interleaved: the last token's offset passes 2^31 elements."""
+    N, step = 40, 1 << 26
+    q, k, v, do, beta, lg, S0, dS, _ = inputs(1, 2, 2, 2, 2, N, 64, 64, "bf16", seed=3)
+    buf = torch.empty((N - 1) * step + 1024, dtype=torch.bfloat16, device="cuda")
+
+    def far(x, at):
+        y = buf.as_strided(x.shape, (0, 64, step, 1), at)
+        return y.copy_(x)
+
+    fq, fk, fv, out, fdo = far(q, 0), far(k, 128), far(v, 256), far(v, 384), far(do, 512)
+    args = dict(log_gamma=lg, state=S0)
+    want, S = ops.gated_delta_forward(q, k, v, beta, return_state=True, path=path, **args)
+    got, S2 = ops.gated_delta_forward(fq, fk, fv, beta, return_state=True, path=path, out=out, **args)
+    assert torch.equal(want, got) and torch.equal(S, S2)
+    if path == "chunked":
+        runs = [ops.gated_delta_backward(*x, beta, g, dstate=dS, need_dlog_gamma=True, need_dstate=True, **args)
+                for x, g in (((q, k, v), do), ((fq, fk, fv), fdo))]
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+        x, dy = fq[0, 0], fv[0, 0]  # [N, 64] rows, 2^26 apart
+        assert torch.equal(ops.layer_norm(x), ops.layer_norm(x.contiguous()))
+        assert all(torch.equal(a, b) for a, b in zip(ops.layer_norm_backward(dy, x), ops.layer_norm_backward(dy.contiguous(), x.contiguous())))
+
+
+@pytest.mark.parametrize("d,e,N", [(1, 1, 70), (1, 33, 17), (33, 1, 130), (8, 256, 65)])
+def test_smallest_heads(d, e, N):
+    q, k, v, do, beta, lg, S0, dS, m = inputs(2, 3, 3, 1, 3, N, d, e, "bf16", seed=d + e, mask="random")
+    want, S = ref.forward(q, k, v, beta, lg, m, d ** -0.5, S0)
+    for path in ("exact", "chunked"):
+        o, St = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, mask=m, state=S0, return_state=True, path=path)
+        assert rel(o, want) < tol(o.dtype, q.dtype) and rel(St, S) < tol(St.dtype, q.dtype)
+    got = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, mask=m, state=S0, dstate=dS, need_dlog_gamma=True, need_dstate=True)
+    for name, a, w in zip(("dq", "dk", "dv", "dbeta", "dlog_gamma", "dstate"), got, ref.gradients(q, k, v, beta, lg, m, d ** -0.5, S0, do, dS)):
+        assert rel(a, w) < tol(a.dtype, q.dtype), name
+
+
+def test_two_host_threads_at_once():
+    import threading
+    cases = [inputs(2, 4, 4, 2, 4, 700, 64, 64, "bf16", seed=s) for s in range(2)]
+
+    def work(i, out):
+        q, k, v, do, beta, lg, S0, dS, _ = cases[i]
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                ho = ops.DeltaHandover()
+                o, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, state=S0, return_state=True, handover=ho)
+                g = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, state=S0, dstate=dS, need_dlog_gamma=True,
+                                             need_dstate=True, handover=ho)
+                out[i] = (o, S) + g
+        stream.synchronize()
+
+    torch.cuda.synchronize()
+    alone, both = [None, None], [None, None]
+    for i in range(2):
+        work(i, alone)
+    threads = [threading.Thread(target=work, args=(i, both)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, both):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
