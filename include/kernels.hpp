@@ -271,7 +271,8 @@ typedef struct subq_delta_bwd_args {
     subq_tensor4 dq, dk, dv;     /* heads of q, k, v; must not alias the inputs  */
     const float* state_in;       /* the forward's                                */
     const float* dstate_out;     /* gradient of the final state, NULL = zeros    */
-    float* dstate_in;            /* gradient of state_in, NULL = not wanted      */
+    float* dstate_in;            /* gradient of state_in, NULL = not wanted; may
+                                    equal dstate_out                              */
     float* dbeta;                /* [B, heads, N] contiguous float32             */
     float* dlog_gamma;           /* likewise, or NULL                            */
     const void* handover;        /* what the forward of the same call left, or

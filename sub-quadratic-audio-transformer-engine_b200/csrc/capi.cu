@@ -524,22 +524,30 @@ int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc&
 //                  3 x 12 heads, 16384 tokens    554, 510 (G = 2)    4 x 12, 4096     162, none (G = 2: 213, more CTAs than SMs)
 //   float32:       2 x 12 heads, 1537 tokens     148, 124 (G = 3)    1 x 4, 16384    1112, 243 (G = 18)
 //   d = 128:       1 x 4 heads, 8192 tokens      319, 134 (bf16, G = 8)   835, 251 (float16, G = 9)   1228, 441 (float32, G = 6)
+//
+// The walk back over the chunks is cut the same way. Its first pass has a whole step's work (the products with dO beside
+// the chain), so the sum has to be a fifth below. The gradients' call from the forward's handover, us, single and cut:
+//   bf16, d = 64:  1 x 12 heads, 65536 tokens   2824, 1572 (G = 6)   2 x 12, 8192     450, 355 (G = 3)   1 x 4, 4096   197, 110 (G = 8)
+//                  3 x 12 heads, 16384 tokens   1035, none (G = 2: 982)                4 x 12, 4096     318, none (G = 2: 384)
+//   float32:       2 x 12 heads, 1537 tokens     278, none (G = 3: 272)
+//   d = 128:       1 x 4 heads, 8192 tokens      447, 243 (bf16, G = 6)   1633, 740 (float32, G = 6)
 struct DeltaSplit {
     int nseg, chunks;
 };
-DeltaSplit delta_split(const subq::DeltaParams& p, int dtype) {
+DeltaSplit delta_split(const subq::DeltaParams& p, int dtype, bool back = false) {
     const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + 31) / 32, ndb = (p.d + 31) / 32;
     const int wide = p.d > 64;
     constexpr double kSteps[3][2] = {{4.3, 9.2}, {2.5, 6.4}, {1.7, 2.3}};  // us: float32, float16, bfloat16
     const double step = kSteps[dtype == SUBQ_FP32 ? 0 : dtype == SUBQ_FP16 ? 1 : 2][wide], join = wide ? 2.0 : 1.0, launches = 8.0;
     auto waves = [](int64_t ctas, int64_t slots) { return (double)((ctas + slots - 1) / slots); };
-    double best = 0.9 * p.nc * step * waves(bh * ncb, 148);
+    double best = (back ? 0.8 : 0.9) * p.nc * step * waves(bh * ncb, 148);
     DeltaSplit s = {1, p.nc};
+    if (back && p.dS_in && p.dS_in == p.dS_out) return s;  // (one CTA reads what another one's result would overwrite)
     for (int g = 2; g <= 64 && 2 * g <= p.nc; ++g) {
         const int chunks = (p.nc + g - 1) / g;
         if ((p.nc + chunks - 1) / chunks != g) continue;  // (the same split with fewer segments)
         const int64_t ctas = bh * ((g - 1) * (ncb + ndb) - ndb);
-        const double states = dtype == SUBQ_FP32 || ctas <= 148 ? 0.7 * waves(ctas, 148) : 1.1 * waves(ctas, 296);
+        const double states = back ? waves(ctas, 148) : dtype == SUBQ_FP32 || ctas <= 148 ? 0.7 * waves(ctas, 148) : 1.1 * waves(ctas, 296);
         const double t = chunks * step * (waves(bh * g * ncb, 148) + states) + g * join + launches;
         if (t < best) best = t, s = {g, chunks};
     }
@@ -633,20 +641,25 @@ int fill_delta_bwd(const subq_delta_bwd_args* a, subq::DeltaParams& p) {
     return SUBQ_OK;
 }
 
-// Workspace of the backward: dS, Z, float32 gradients per state head of shared
+// Workspace of the backward: dS, Z, the walk back's segments, float32 gradients per state head of shared
 // q, k, v, and the forward's part where no handover is given.
 struct DeltaBwdBytes {
     DeltaBytes fwd;
-    size_t dq, dk, dv, total;
+    DeltaSplit rev;  // of the walk back
+    size_t rev_S, rev_M, dq, dk, dv, total;
 };
 DeltaBwdBytes delta_bwd_bytes(const subq::DeltaParams& p, int dtype, bool handover) {
     DeltaBwdBytes n;
     n.fwd = delta_bytes(p, dtype);
+    n.rev = delta_split(p, dtype, true);
+    const size_t slots = (size_t)p.B * p.H * (n.rev.nseg - 1) * sizeof(float), dp = p.d <= 64 ? 64 : 128;
+    n.rev_S = align_up(slots * p.d * p.e);
+    n.rev_M = align_up(slots * dp * dp);
     const size_t tokens = (size_t)p.B * p.H * p.N;
     n.dq = p.q.group > 1 ? align_up(tokens * p.d * 4) : 0;
     n.dk = p.k.group > 1 ? align_up(tokens * p.d * 4) : 0;
     n.dv = p.v.group > 1 ? align_up(tokens * p.e * 4) : 0;
-    n.total = n.fwd.S0 + n.fwd.W + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.gates + n.fwd.Y + n.fwd.P + n.fwd.S0 + n.fwd.W + n.fwd.segs());
+    n.total = n.fwd.S0 + n.fwd.W + n.rev_S + n.rev_M + n.dq + n.dk + n.dv + (handover ? 0 : n.fwd.gates + n.fwd.Y + n.fwd.P + n.fwd.S0 + n.fwd.W + n.fwd.segs());
     return n;
 }
 
@@ -735,6 +748,7 @@ int subq_delta_bwd(const subq_delta_bwd_args* a) {
     };
     p.dS = take(n.fwd.S0);
     p.Z = take(n.fwd.W);
+    unsigned char* rev = take(n.rev_S + n.rev_M);
     if (n.dq) p.dq32 = reinterpret_cast<float*>(take(n.dq));
     if (n.dk) p.dk32 = reinterpret_cast<float*>(take(n.dk));
     if (n.dv) p.dv32 = reinterpret_cast<float*>(take(n.dv));
@@ -749,6 +763,11 @@ int subq_delta_bwd(const subq_delta_bwd_args* a) {
         err = subq::launch_delta_fwd(p, dt, st);  // (o is null: states and corrections only)
         first = p.nseg > 1 ? 4 : 2;
     }
+    p.nseg = n.rev.nseg;
+    p.seg_chunks = n.rev.chunks;
+    p.seg_S = reinterpret_cast<float*>(rev);
+    p.seg_M = reinterpret_cast<float*>(rev + n.rev_S);
+    p.seg_in = nullptr;
     if (err == cudaSuccess) err = subq::launch_delta_bwd(p, dt, st, &launches);
     if (err != cudaSuccess) return fail_cuda(err, "subq_delta_bwd launch");
     g_last_path = SUBQ_PATH_CHUNKED;

@@ -23,11 +23,13 @@
 //
 // Measured, bf16, d = e = 64, 8 x 8 heads of 8192 tokens (8192 chunks): the walk back
 // 275 us (2.1 us a chunk, bound like the forward's by shared memory and the latency of
-// its three products in a row), the gradients 400 us (105 KB read and written a chunk,
+// its three products in a row; few sequences are cut into segments, see delta_join.cuh
+// and the rule in capi.cu), the gradients 400 us (105 KB read and written a chunk,
 // 0.33 of measured HBM; tensor pipe 41 %, shared memory 52 %, 16 warps per SM).
 #pragma once
 
 #include "delta_common.cuh"
+#include "delta_join.cuh"
 #include "delta_launch.h"
 
 namespace subq {
@@ -62,8 +64,8 @@ struct RevSmem {
 };
 
 // One warp of a chain pair: half `A` of d of G^T in its accumulators; dU and Z of its token blocks.
-template <typename T, int DP>
-__device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int col0, int lane) {
+template <typename T, int DP, bool STATES>
+__device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const WalkJob& job, int A, int pair, int lane) {
     constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = RevSmem<T, DP>::kStages;
     constexpr int NH = DP / 16;
     constexpr bool kShared = RevSmem<T, DP>::kShared;
@@ -71,13 +73,13 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaPa
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
     float S[NH][4];  // G^T: 16 value columns x this half of d
-    const float* G_in = p.dS_out ? p.dS_out + bh * p.d * p.e : nullptr;
+    const int col0 = job.c0 + 16 * pair;
 #pragma unroll
     for (int n = 0; n < NH; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
-            S[n][i] = (G_in && d < p.d && col < p.e) ? G_in[(int64_t)d * p.e + col] : 0.f;
+            S[n][i] = job.ident ? (d == col ? 1.f : 0.f) : job.in && d < job.rows && col < job.ld ? job.in[(int64_t)d * job.ld + col] : 0.f;
         }
     auto put_state = [&]() {
 #pragma unroll
@@ -89,7 +91,7 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaPa
     };
     put_state();
     __syncthreads();
-    for (int c = p.nc - 1; c >= 0; --c) {
+    for (int c = job.end - 1; c >= job.begin; --c) {
         if (NST == 1) __syncthreads();
         auto& st = sm.st[c % NST];
         const Gates& s = st.s;
@@ -147,8 +149,10 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaPa
                     uint32_t a[NX][4];
                     to_a<NX>(X[2 * u], X[2 * u + 1], f[0], f[1], a);
                     put_a<NX>(sm.Zk[pair][jb], a, lane);
-                    to_a<NX>(X[2 * u], X[2 * u + 1], one, one, a);
-                    put_a<NX>(sm.z.Zp[pair][jb], a, lane);
+                    if constexpr (!STATES) {
+                        to_a<NX>(X[2 * u], X[2 * u + 1], one, one, a);
+                        put_a<NX>(sm.z.Zp[pair][jb], a, lane);
+                    }
                 } else {
                     sm.z.Z[pair][2 * jb * 32 + lane] = as_float4(X[2 * u]);
                     sm.z.Z[pair][(2 * jb + 1) * 32 + lane] = as_float4(X[2 * u + 1]);
@@ -184,34 +188,34 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const DeltaPa
         }
         __syncthreads();
     }
-    if (p.dS_in) {
-        float* G_out = p.dS_in + bh * p.d * p.e;
+    if (job.out) {
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int d = 8 * (A * NH + n) + 2 * t + (i & 1), col = col0 + g + 8 * (i >> 1);
-                if (d < p.d && col < p.e) G_out[(int64_t)d * p.e + col] = S[n][i];
+                if (d < job.rows && col < job.ld) job.out[job.ident ? (int64_t)col * job.ld + d : (int64_t)d * job.ld + col] = S[n][i];
             }
     }
 }
 
 // One warp of the pair beside a chain pair: P^T dO and dV for its token blocks, (e^g Q)^T dO for its half of d, and
 // its share of the planes of G and Z.
-template <typename T, int DP>
-__device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaParams& p, int A, int pair, int64_t bh, int cb, int lane) {
+template <typename T, int DP, bool STATES>
+__device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
     constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kGTile = 64 * kDeltaCols * 2;
     constexpr int NST = RevSmem<T, DP>::kStages, NH = DP / 16;
-    const int g = lane >> 2, t = lane & 3, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
+    const int g = lane >> 2, t = lane & 3, ncb = (p.e + kDeltaCols - 1) / kDeltaCols, cb = job.cb;
+    const int64_t bh = job.bh;
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
     constexpr int kPitch = 16 * sizeof(T) + 16, kPieces = 16 * sizeof(T) / 16;  // as the forward's staged outputs
     static_assert(4 * 32 * kPitch <= NX * kYBlocks * 512, "staged dv");
     const int col0 = cb * kDeltaCols + 16 * pair, width = min(16, p.e - col0);
     const bool whole = p.dv.vec && width == 16;
-    T* dv = static_cast<T*>(p.dv.p) + tensor_base(p.dv, (int)(bh / p.H), (int)(bh % p.H));
+    T* dv = static_cast<T*>(p.dv.p) + tensor_base(p.dv, job.b, job.h);
     __syncthreads();
-    for (int c = p.nc - 1; c >= 0; --c) {
+    for (int c = job.end - 1; c >= job.begin; --c) {
         if (NST == 1) __syncthreads();
         auto& st = sm.st[c % NST];
         const Gates& s = st.s;
@@ -232,7 +236,7 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
 #pragma unroll
             for (int x = 0; x < 4; ++x) sm.e2[pair][(2 * own.at(x >> 1) + (x & 1)) * 32 + lane] = as_float4(E[x]);
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
+            for (int kk = 0; kk < (STATES ? 0 : DP / 16); ++kk) {
                 if (kk % 2 != A) continue;
                 uint32_t a[NX][4];
                 get_a<NX>(a, sm.G[pair][kk], lane);
@@ -269,7 +273,7 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
             // planes of Z, and dv = beta Z, staged where Y was (which nobody reads any more)
             unsigned char* stage = st.y + (2 * pair + A) * (32 * kPitch);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < (STATES ? 0 : 2); ++u) {
                 uint32_t a[NX][4];
                 float z0[4], z1[4];
                 if constexpr (RevSmem<T, DP>::kShared) {
@@ -302,7 +306,7 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
                     }
                 }
             }
-            if (!p.dv32) {
+            if (!STATES && !p.dv32) {
                 __syncwarp();
 #pragma unroll
                 for (int x = 0; x < kPieces; ++x) {
@@ -326,24 +330,48 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
     }
 }
 
-template <typename T, int DP>
+// STATES: the gradients of the states alone, of segments that are walked side by side (delta_join.cuh). Segments count
+// from the end; the last one's columns of the identity, as the first's results, nobody needs.
+template <typename T, int DP, bool STATES>
 __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) {
     constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX;
     constexpr int NST = RevSmem<T, DP>::kStages;
     extern __shared__ __align__(128) unsigned char raw[];
     RevSmem<T, DP>& sm = *reinterpret_cast<RevSmem<T, DP>*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
-    const unsigned bh32 = blockIdx.x / (unsigned)ncb;
-    const int64_t bh = bh32;
-    const int cb = (int)(blockIdx.x - bh32 * ncb), b = (int)(bh32 / (unsigned)p.H), h = (int)(bh32 - b * (unsigned)p.H);
-    const int c0 = cb * kDeltaCols;
+    const int ncb = (p.e + kDeltaCols - 1) / kDeltaCols, ndb = STATES ? (p.d + kDeltaCols - 1) / kDeltaCols : 0, ncols = ncb + ndb;
+    const int nseg = STATES ? p.nseg - 1 : p.nseg;
+    const unsigned per_seq = (unsigned)(nseg * ncols - ndb), bh32 = blockIdx.x / per_seq;
+    const int at = (int)(blockIdx.x - bh32 * per_seq) + ndb;  // (the last segment's columns at ndb ..)
+    const int seg = at / ncols, col = at - seg * ncols;
+    WalkJob job;
+    job.bh = bh32;
+    job.b = (int)(bh32 / (unsigned)p.H);
+    job.h = (int)(bh32 - job.b * (unsigned)p.H);
+    job.ident = STATES && col < ndb;
+    job.cb = job.ident ? col : col - ndb;
+    job.c0 = job.cb * kDeltaCols;
+    job.begin = (p.nseg - 1 - seg) * p.seg_chunks;
+    job.end = min(p.nc, job.begin + p.seg_chunks);
+    job.ld = job.ident ? DP : p.e;
+    job.rows = job.ident ? DP : p.d;
+    const int64_t slot = job.bh * (p.nseg - 1) + seg;
+    job.in = seg && !STATES ? p.seg_S + (slot - 1) * p.d * p.e : !seg && p.dS_out ? p.dS_out + job.bh * p.d * p.e : nullptr;
+    if (STATES) job.out = job.ident ? p.seg_M + slot * (DP * DP) : p.seg_S + slot * p.d * p.e;
+    else job.out = seg + 1 == nseg && p.dS_in ? p.dS_in + job.bh * p.d * p.e : nullptr;
     if (warp < 4) {
-        rev_chain_warp<T, DP>(sm, p, warp & 1, warp >> 1, bh, c0 + 16 * (warp >> 1), lane);
+        rev_chain_warp<T, DP, STATES>(sm, job, warp & 1, warp >> 1, lane);
     } else if (warp < 8) {
-        rev_side_warp<T, DP>(sm, p, warp & 1, (warp >> 1) & 1, bh, cb, lane);
+        rev_side_warp<T, DP, STATES>(sm, p, job, warp & 1, (warp >> 1) & 1, lane);
     } else {  // ---------------------------------------------------------- loads
         const int lt = tid - 256;  // as in the forward's walk, from the last chunk to the first
+        const int64_t bh = job.bh;
+        const int b = job.b, h = job.h, begin = job.begin, end = job.end, c0 = job.c0;
+        if (job.ident) {  // dO is 0 in every stage
+            for (int i = 0; i < NST; ++i)
+                for (int x = lt * 16; x < (int)sizeof(sm.st[i].g); x += 128 * 16)
+                    *reinterpret_cast<uint4*>(sm.st[i].g + x) = make_uint4(0, 0, 0, 0);
+        }
         const Gates* gates = p.gates + bh * p.nc;
         const int64_t kb = tensor_base(p.k, b, h), qb = tensor_base(p.q, b, h), gb = tensor_base(p.g, b, h);
         constexpr int kMat = NX * kYBlocks * 512;
@@ -353,18 +381,18 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
         if constexpr (NIN == 1) async = p.k.vec && p.q.vec && p.g.vec && p.d % 8 == 0 && p.e % 8 == 0;
         if (async) {
             constexpr int kAhead = NST - 1;
-            int any_next = gates[p.nc - 1].any;
+            int any_next = gates[end - 1].any;
             auto start = [&](int c) {
-                if (c >= 0) {
+                if (c >= begin) {
                     const int any = any_next;
-                    any_next = c > 0 ? gates[c - 1].any : 0;
+                    any_next = c > begin ? gates[c - 1].any : 0;
                     auto& st = sm.st[c % NST];
                     async16<128>(reinterpret_cast<unsigned char*>(&st.s), reinterpret_cast<const unsigned char*>(gates + c), sizeof(Gates), lt);
                     if (any) {
                         const int n0 = c * kDeltaC;
                         async_tile<T, DP, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, lt);
                         async_tile<T, DP, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, lt);
-                        async_tile<T, kDeltaCols, 128>(st.g, p.g, gb, n0, c0, p.e, p.N, lt);
+                        if (!STATES || !job.ident) async_tile<T, kDeltaCols, 128>(st.g, p.g, gb, n0, c0, p.e, p.N, lt);
                         async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
                         async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
                     }
@@ -373,7 +401,7 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
             };
             auto finish = [&](int c) {
                 async_wait_but<(kAhead > 1 ? kAhead - 1 : 0)>();
-                if (c < 0) return;
+                if (c < begin) return;
                 bar_sync(3, 128);
                 auto& st = sm.st[c % NST];
                 if (st.s.any && !st.s.full) {
@@ -382,10 +410,10 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
                     clear_dead<kDeltaCols, 128>(st.g, st.s.live, lt);
                 }
             };
-            for (int i = 1; i <= kAhead; ++i) start(p.nc - i);
-            finish(p.nc - 1);
+            for (int i = 1; i <= kAhead; ++i) start(end - i);
+            finish(end - 1);
             __syncthreads();
-            for (int c = p.nc - 1; c >= 0; --c) {
+            for (int c = end - 1; c >= begin; --c) {
                 start(c - kAhead);
                 finish(c - 1);
                 __syncthreads();
@@ -394,7 +422,7 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
         } else {
             if constexpr (NST == 1) {
                 __syncthreads();
-                for (int c = p.nc - 1; c >= 0; --c) {
+                for (int c = end - 1; c >= begin; --c) {
                     auto& st = sm.st[0];
                     copy16<128>(reinterpret_cast<unsigned char*>(&st.s), reinterpret_cast<const unsigned char*>(gates + c), sizeof(Gates), lt);
                     bar_sync(3, 128);
@@ -402,7 +430,7 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
                         const int n0 = c * kDeltaC;
                         load_tile<T, DP, NIN, 128>(st.k, p.k, kb, n0, 0, p.d, p.N, st.s.live, lt);
                         load_tile<T, DP, NIN, 128>(st.q, p.q, qb, n0, 0, p.d, p.N, st.s.live, lt);
-                        load_tile<T, kDeltaCols, NIN, 128>(st.g, p.g, gb, n0, c0, p.e, p.N, st.s.live, lt);
+                        if (!STATES || !job.ident) load_tile<T, kDeltaCols, NIN, 128>(st.g, p.g, gb, n0, c0, p.e, p.N, st.s.live, lt);
                         async16<128>(st.y, Y + (int64_t)c * kMat, kMat, lt);
                         async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
                         async_wait();
@@ -414,20 +442,20 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
                 TileRegs<T, DP, 128> k, q;
                 TileRegs<T, kDeltaCols, 128> x;
                 ByteRegs<sizeof(Gates), 128> s;
-                int any = 0, any_next = gates[p.nc - 1].any;
+                int any = 0, any_next = gates[end - 1].any;
                 auto issue = [&](int c) {
                     any = any_next;
-                    any_next = c > 0 ? gates[c - 1].any : 0;
-                    if (c < 0) return;
+                    any_next = c > begin ? gates[c - 1].any : 0;
+                    if (c < begin) return;
                     s.issue(gates + c, lt);
                     if (!any) return;
                     const int n0 = c * kDeltaC;
                     k.issue(p.k, kb, n0, 0, p.d, p.N, lt);
                     q.issue(p.q, qb, n0, 0, p.d, p.N, lt);
-                    x.issue(p.g, gb, n0, c0, p.e, p.N, lt);
+                    if (!STATES || !job.ident) x.issue(p.g, gb, n0, c0, p.e, p.N, lt);
                 };
                 auto store = [&](int c) {
-                    if (c < 0) return;
+                    if (c < begin) return;
                     auto& st = sm.st[c % NST];
                     s.store(&st.s, lt);
                     bar_sync(3, 128);
@@ -436,14 +464,14 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
                     async16<128>(st.P, P + (int64_t)c * kMat, kMat, lt);
                     k.template store_planes<NIN>(st.k, st.s.live, lt);
                     q.template store_planes<NIN>(st.q, st.s.live, lt);
-                    x.template store_planes<NIN>(st.g, st.s.live, lt);
+                    if (!STATES || !job.ident) x.template store_planes<NIN>(st.g, st.s.live, lt);
                 };
-                issue(p.nc - 1);
-                store(p.nc - 1);
-                issue(p.nc - 2);
+                issue(end - 1);
+                store(end - 1);
+                issue(end - 2);
                 async_wait();
                 __syncthreads();
-                for (int c = p.nc - 1; c >= 0; --c) {
+                for (int c = end - 1; c >= begin; --c) {
                     store(c - 1);
                     issue(c - 2);
                     async_wait();
@@ -901,15 +929,24 @@ cudaError_t bwd_t(const DeltaParams& p, cudaStream_t st, int* launches) {
     const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + kDeltaCols - 1) / kDeltaCols;
     static_assert(sizeof(RevSmem<T, DP>) <= 227 * 1024 && sizeof(GradSmem<T, DP>) <= 227 * 1024, "shared memory");
     const size_t rev = sizeof(RevSmem<T, DP>), grad = sizeof(GradSmem<T, DP>);
-    cudaError_t err = cudaFuncSetAttribute(delta_rev_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rev);
-    if (err == cudaSuccess)
-        err = cudaFuncSetAttribute(delta_grad_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)grad);
+    auto walk = [&](auto kernel, int64_t blocks) {
+        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rev);
+        if (err != cudaSuccess) return err;
+        kernel<<<(unsigned)blocks, 384, rev, st>>>(p);
+        return cudaGetLastError();
+    };
+    cudaError_t err = cudaFuncSetAttribute(delta_grad_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)grad);
     if (err != cudaSuccess) return err;
-    delta_rev_kernel<T, DP><<<(unsigned)(bh * ncb), 384, rev, st>>>(p);
-    if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    *launches = 2;
+    if (p.nseg > 1) {
+        const int64_t ndb = (p.d + kDeltaCols - 1) / kDeltaCols;
+        if ((err = walk(delta_rev_kernel<T, DP, true>, bh * ((p.nseg - 1) * (ncb + ndb) - ndb))) != cudaSuccess) return err;
+        if ((err = join_t<DP>(p, st)) != cudaSuccess) return err;
+        *launches = 4;
+    }
+    if ((err = walk(delta_rev_kernel<T, DP, false>, bh * p.nseg * ncb)) != cudaSuccess) return err;
     delta_grad_kernel<T, DP><<<(unsigned)(bh * p.nc), 256, grad, st>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
-    *launches = 2;
     if ((err = group_sum<T>(p.dq32, p.dq, p, p.d, st, launches)) != cudaSuccess) return err;
     if ((err = group_sum<T>(p.dk32, p.dk, p, p.d, st, launches)) != cudaSuccess) return err;
     return group_sum<T>(p.dv32, p.dv, p, p.e, st, launches);

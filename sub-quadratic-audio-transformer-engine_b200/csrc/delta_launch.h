@@ -20,7 +20,8 @@ cudaError_t launch_delta_fwd_fp32(const DeltaParams& p, cudaStream_t st);
 inline cudaError_t launch_delta_fwd(const DeltaParams& p, int dtype, cudaStream_t st) {
     return dtype == SUBQ_BF16 ? launch_delta_fwd_bf16(p, st) : dtype == SUBQ_FP16 ? launch_delta_fwd_fp16(p, st) : launch_delta_fwd_fp32(p, st);
 }
-// Gradients from what the forward left (p.gates, p.Y, p.P, p.S0, p.W) (delta_bwd.cuh). 2 launches, and one per shared q, k, v.
+// Gradients from what the forward left (p.gates, p.Y, p.P, p.S0, p.W) (delta_bwd.cuh). 2 launches, 4 with segments, and one per
+// shared q, k, v.
 cudaError_t launch_delta_bwd_bf16(const DeltaParams& p, cudaStream_t st, int* launches);
 cudaError_t launch_delta_bwd_fp16(const DeltaParams& p, cudaStream_t st, int* launches);
 cudaError_t launch_delta_bwd_fp32(const DeltaParams& p, cudaStream_t st, int* launches);

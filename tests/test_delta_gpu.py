@@ -484,3 +484,22 @@ def test_two_host_threads_at_once():
         t.join()
     for a, b in zip(alone, both):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("N,d,e,dtype,dead", [(4096, 64, 64, "bf16", None), (2049, 128, 96, "bf16", (512, 1100)), (3333, 48, 80, "fp16", (0, 700)),
+                                              (2500, 64, 64, "fp32", (1800, 2500)), (2500, 128, 128, "fp32", None)])
+def test_gradients_where_the_walk_back_is_cut_into_segments(N, d, e, dtype, dead):
+    q, k, v, do, beta, lg, S0, dS, _ = inputs(1, 2, 2, 1, 2, N, d, e, dtype, seed=N + d)
+    m = torch.ones(1, N, dtype=torch.bool, device="cuda")
+    if dead:
+        m[:, dead[0]:dead[1]] = False
+    ho = ops.DeltaHandover()
+    ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, mask=m, state=S0, handover=ho)
+    got = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, mask=m, state=S0, dstate=dS, need_dlog_gamma=True, need_dstate=True,
+                                   handover=ho)
+    assert ops.last_launches() == 4 + 1  # states, join, walk, gradients; dk summed over its group
+    want = ref.gradients(q, k, v, beta, lg, m, d ** -0.5, S0, do, dS)
+    for name, a, w in zip(("dq", "dk", "dv", "dbeta", "dlog_gamma", "dstate"), got, want):
+        assert rel(a, w) < tol(a.dtype, q.dtype), name
+    none = ops.gated_delta_backward(q, k, v, beta, torch.zeros_like(do), log_gamma=lg, mask=m, state=S0, need_dlog_gamma=True, need_dstate=True)
+    assert all(not x.any() for x in none)
