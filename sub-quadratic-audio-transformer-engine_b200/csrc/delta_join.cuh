@@ -23,7 +23,7 @@ struct JoinSmem {
 template <int DP>
 __global__ void __launch_bounds__(2 * DP) delta_join_kernel(const DeltaParams p) {
     constexpr int kThreads = JoinSmem<DP>::kThreads, kBufs = JoinSmem<DP>::kBufs, kAhead = kBufs - 1;
-    extern __shared__ __align__(16) unsigned char raw[];
+    extern __shared__ __align__(128) unsigned char raw[];
     JoinSmem<DP>& sm = *reinterpret_cast<JoinSmem<DP>*>(raw);
     const unsigned ncb = (p.e + 15) / 16, bh32 = blockIdx.x / ncb;
     const int64_t slot = (int64_t)bh32 * (p.nseg - 1);

@@ -567,7 +567,7 @@ def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta:
         if return_state:
             S_out = torch.empty((B, H, d, e), dtype=torch.float32, device=q.device)
             a.state_out = S_out.data_ptr()
-        a.stream = torch.cuda.current_stream(q.device).cuda_stream
+        a.stream = torch.cuda.current_stream(q.device.index).cuda_stream
         if handover is not None:
             nbytes = _capi.delta_handover_bytes(a.desc)
             handover.buf = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
@@ -618,7 +618,7 @@ def gated_delta_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta
         a.dbeta = dbeta.data_ptr()
         if dlg is not None:
             a.dlog_gamma = dlg.data_ptr()
-        a.stream = torch.cuda.current_stream(q.device).cuda_stream
+        a.stream = torch.cuda.current_stream(q.device.index).cuda_stream
         if handover is not None and handover.buf is not None:
             if handover.key != (B, H, N, d, e, q.dtype, q.device):
                 raise ValueError("handover comes from a forward of another shape, type or device")
@@ -677,18 +677,18 @@ class GatedDeltaStep:
         if torch.cuda.current_device() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.step()
-        self._args.stream = torch.cuda.current_stream(self.device).cuda_stream
+        self._args.stream = torch.cuda.current_stream(self.device.index).cuda_stream
         _capi.delta_fwd(self._args)
 
 
 # ------------------------------------------------------------------- layer norm
-_LN_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+_LN_PAIRS = {(t, t) for t in (torch.float32, torch.float16, torch.bfloat16)} | {(torch.float32, torch.float16), (torch.float32, torch.bfloat16)}
 
 
 def _ln_check(x: torch.Tensor, y_dtype: torch.dtype) -> None:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer_norm needs a last dimension of at least 1")
-    if x.dtype not in _LN_TYPES or (y_dtype != x.dtype and not (x.dtype == torch.float32 and y_dtype in _LN_TYPES)):
+    if (x.dtype, y_dtype) not in _LN_PAIRS:
         raise TypeError(f"layer_norm takes float32, float16 or bfloat16 (and float32 into a 16-bit type), not {x.dtype} into {y_dtype}")
 
 
@@ -707,7 +707,7 @@ def _ln_rows(t: torch.Tensor, keep: list) -> Tuple[int, int]:
 def _ln_param(w: Optional[torch.Tensor], name: str, x: torch.Tensor, keep: list) -> Optional[int]:
     if w is None:
         return None
-    if w.dim() != 1 or w.shape[0] != x.shape[-1]:
+    if w.shape != x.shape[-1:]:
         raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
     if w.device != x.device:
         raise ValueError(f"{name} must be on the device of x")
@@ -731,11 +731,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     D = x.shape[-1]
     keep: list = []
     xp, xs = _ln_rows(x, keep)
-    y = torch.empty(x.shape, dtype=y_dtype, device=x.device)
+    y = torch.empty_like(x, dtype=y_dtype, memory_format=torch.contiguous_format)
     _capi.layer_norm_fwd(_capi.LayerNormArgs(
         x.numel() // D, D, _DTYPES[x.dtype], _DTYPES[y_dtype], eps, xp, xs, y.data_ptr(), D, None, 0, None, 0,
         _ln_param(weight, "weight", x, keep), _ln_param(bias, "bias", x, keep), None, None, None, 0,
-        torch.cuda.current_stream().cuda_stream))
+        torch.cuda.current_stream(x.device.index).cuda_stream))
     return y
 
 
@@ -754,13 +754,13 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     D = x.shape[-1]
     keep: list = []
     (xp, xs), (gp, gs) = _ln_rows(x, keep), _ln_rows(dy, keep)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = torch.empty(D, dtype=torch.float32, device=x.device) if need_dweight else None
     db = torch.empty(D, dtype=torch.float32, device=x.device) if need_dbias else None
     a = _capi.LayerNormArgs(
         x.numel() // D, D, _DTYPES[x.dtype], _DTYPES[dy.dtype], eps, xp, xs, None, 0, gp, gs, dx.data_ptr(), D,
         _ln_param(weight, "weight", x, keep), None, dw.data_ptr() if need_dweight else None,
-        db.data_ptr() if need_dbias else None, None, 0, torch.cuda.current_stream().cuda_stream)
+        db.data_ptr() if need_dbias else None, None, 0, torch.cuda.current_stream(x.device.index).cuda_stream)
     if need_dweight or need_dbias:
         a.workspace, a.workspace_bytes = _workspace(_capi.layer_norm_bwd_workspace_bytes(a), x.device, keep)
     _capi.layer_norm_bwd(a)
