@@ -245,3 +245,11 @@ def test_layer_norm_workspace():
     a = _ln(rows=0)
     a.x = a.y = None
     assert _code("subq_layer_norm_fwd", a) == _capi.SUBQ_OK
+
+
+def test_state_gradient_in_place_is_not_cut_into_segments():
+    b = _bwd(B=1, H=4, N=4096)
+    b.dstate_out, b.dstate_in = 0x20000000, 0x30000000
+    cut = _capi.delta_bwd_workspace_bytes(b)
+    b.dstate_in = b.dstate_out
+    assert 0 < _capi.delta_bwd_workspace_bytes(b) < cut
