@@ -158,13 +158,11 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const WalkJob
                     sm.z.Z[pair][(2 * jb + 1) * 32 + lane] = as_float4(X[2 * u + 1]);
                 }
             }
-#pragma unroll
-            for (int n = 0; n < NH; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) S[n][i] *= s.eC;
+            float U[NH][4];  // the chunk's part, summed by itself as in the forward's walk
+            zero_acc<NH>(U);
             bar_sync(2, 256);  // Z is there for the pair and the warps beside it; e2 is there
 #pragma unroll
-            for (int n = 0; n < NH; ++n) add_acc(S[n], sm.e2[pair][(A * NH + n) * 32 + lane]);
+            for (int n = 0; n < NH; ++n) add_acc(U[n], sm.e2[pair][(A * NH + n) * 32 + lane]);
 #pragma unroll
             for (int jb = 0; jb < 4; ++jb) {  // G0^T = e^{g_C} G^T + e2 - (e^g beta Z)^T K over this half of d
                 uint32_t a[NX][4];
@@ -182,8 +180,9 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const WalkJob
                     }
                     to_a<NX>(z0, z1, f[0], f[1], a);
                 }
-                mma_cols<NH, DP, NX, NIN, NX>(S, a, kt, 16 * jb, A * NH, lane);
+                mma_cols<NH, DP, NX, NIN, NX>(U, a, kt, 16 * jb, A * NH, lane);
             }
+            next_state<NH>(S, s.eC, U);
             put_state();
         }
         __syncthreads();

@@ -557,6 +557,15 @@ __device__ __forceinline__ void zero_acc(float (&c)[NB][4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
 }
+// The state after a chunk: f S + the chunk's part U. (Products added to S itself would each cut it off towards zero: 256
+// chunks without decay were 8e-5 off in float32, 5e-5 in bf16.)
+template <int NB>
+__device__ __forceinline__ void next_state(float (&S)[NB][4], float f, const float (&U)[NB][4]) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[n][i] = fmaf(f, S[n][i], U[n][i]);
+}
 __device__ __forceinline__ void add_acc(float (&c)[4], float4 x) {
     c[0] += x.x; c[1] += x.y; c[2] += x.z; c[3] += x.w;
 }

@@ -340,10 +340,8 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, 
                     sm.w.W[pair][(2 * jb + 1) * 32 + lane] = as_float4(W[2 * u + 1]);
                 }
             }
-#pragma unroll
-            for (int n = 0; n < NH; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) S[n][i] *= s.eC;
+            float U[NH][4];  // the chunk's update, summed by itself (see mma_set) and added to the state once, rounded
+            zero_acc<NH>(U);
             bar_sync(1, ChainSmem<T, DP, !OUT && !KEEP>::kChain);  // W is there for both pairs and the output warps, which have read S0
 #pragma unroll
             for (int jb = 0; jb < 4; ++jb) {  // S'^T = e^{g_C} S0^T + (e^{g_C - g} beta W)^T K over this half of d
@@ -362,8 +360,9 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, 
                     }
                     to_a<NX>(w0, w1, f[0], f[1], a);
                 }
-                mma_cols<NH, DP, NX, NIN, NX>(S, a, kt, 16 * jb, A * NH, lane);
+                mma_cols<NH, DP, NX, NIN, NX>(U, a, kt, 16 * jb, A * NH, lane);
             }
+            next_state<NH>(S, s.eC, U);
             put_state();
         }
         __syncthreads();
