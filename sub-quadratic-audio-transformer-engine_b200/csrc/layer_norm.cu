@@ -457,12 +457,13 @@ cudaError_t run(const LnParams& p, bool bwd, int* blocks, cudaStream_t st) {
         ln_fwd_kernel<TX, TY, G, V, K><<<*blocks, kThreads, 0, st>>>(p);
     } else if constexpr (G > 8 && (V > 1 || K <= 8 || G == kThreads)) {
         constexpr int kStage = stage_bytes<TX, TY, V, K>();
+        constexpr int kMost = kStage + (G < kThreads ? 2 : 1) * (int)sizeof(float) * G * V * K;  // of the widest row
         const int smem = kStage + p.D * (p.part && G < kThreads ? 2 : 1) * (int)sizeof(float);
-        static const int per_sm = resident(ln_bwd_kernel<TX, TY, G, V, K>, kStage + (G < kThreads ? 2 : 1) * 4 * G * V * K);
+        static const int per_sm = resident(ln_bwd_kernel<TX, TY, G, V, K>, kMost);
         const int64_t most = kSMs * per_sm < kLnPartials ? kSMs * per_sm : kLnPartials;
         *blocks = (int)(need < most ? need : most);
-        if (smem > kPlainSmem) {
-            const cudaError_t err = cudaFuncSetAttribute(ln_bwd_kernel<TX, TY, G, V, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (smem > kPlainSmem) {  // (every call sets the same limit: calls from other threads, of other widths, may be between here and the launch)
+            const cudaError_t err = cudaFuncSetAttribute(ln_bwd_kernel<TX, TY, G, V, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
             if (err != cudaSuccess) return err;
         }
         ln_bwd_kernel<TX, TY, G, V, K><<<*blocks, kThreads, smem, st>>>(p);
