@@ -255,7 +255,8 @@ typedef struct subq_delta_desc {
 
 typedef struct subq_delta_fwd_args {
     subq_delta_desc desc;
-    subq_tensor4 q, k, v, o; /* o must not alias the inputs                    */
+    subq_tensor4 q, k, v, o; /* o shares no memory with an input (views of one
+                               buffer between each other are fine)             */
     const float* state_in;  /* [B, heads, d, e], NULL = zeros                  */
     float* state_out;       /* may equal state_in, NULL = not wanted           */
     void* handover;         /* NULL, or subq_delta_handover_bytes (256-byte aligned)
@@ -268,7 +269,8 @@ typedef struct subq_delta_fwd_args {
 typedef struct subq_delta_bwd_args {
     subq_delta_desc desc;
     subq_tensor4 q, k, v, dout;
-    subq_tensor4 dq, dk, dv;     /* heads of q, k, v; must not alias the inputs  */
+    subq_tensor4 dq, dk, dv;     /* heads of q, k, v; no output shares memory with
+                                    an input or with another output              */
     const float* state_in;       /* the forward's                                */
     const float* dstate_out;     /* gradient of the final state, NULL = zeros    */
     float* dstate_in;            /* gradient of state_in, NULL = not wanted; may
@@ -293,7 +295,8 @@ size_t subq_delta_handover_bytes(const subq_delta_desc* desc);
  * torch's layer_norm, sums in float32. x_dtype and y_dtype are equal (fp32,
  * fp16, bf16), or x is fp32 and y fp16 or bf16; dx has x's type and dy has y's.
  * The backward recomputes the statistics from x; dweight = sum dy xh and
- * dbias = sum dy are written (not accumulated), bitwise reproducible. */
+ * dbias = sum dy are written (not accumulated), bitwise reproducible. Outputs
+ * share no memory with inputs or one another, but for y or dx in place. */
 typedef struct subq_layer_norm_args {
     int64_t rows, dim;
     int32_t x_dtype, y_dtype;

@@ -12,6 +12,7 @@
 #include "delta_common.cuh"
 #include "delta_launch.h"
 #include "kernels.hpp"
+#include "overlap.h"
 #include "scan_common.cuh"
 #include "scan_launch.h"
 
@@ -587,6 +588,58 @@ void delta_segments(subq::DeltaParams& p, int dtype, const DeltaBytes& n, void* 
     p.seg_in = n.seg_in ? reinterpret_cast<float*>(static_cast<char*>(at) + n.seg_S + n.seg_M) : nullptr;
 }
 
+struct Memory {
+    const char* name;
+    subq::MemRows rows;
+};
+Memory of_tensor(const char* name, const subq::DeltaTensor& t, const subq::DeltaParams& p, int width, int dtype) {
+    const __int128 es = (__int128)elem_size(dtype);
+    return {name, {reinterpret_cast<uintptr_t>(t.p), (int64_t)(width * es), {p.B, p.H / t.group, p.N}, {t.sb * es, t.sh * es, t.sn * es}}};
+}
+Memory of_gate(const char* name, const subq::DeltaGate& g, const subq::DeltaParams& p) {
+    return {name, {reinterpret_cast<uintptr_t>(g.p), 4, {p.B, p.H, p.N}, {(__int128)4 * g.sb, (__int128)4 * g.sh, (__int128)4 * g.sn}}};
+}
+Memory of_bytes(const char* name, const void* at, int64_t bytes) { return {name, {reinterpret_cast<uintptr_t>(at), bytes}}; }
+Memory of_mask(const subq::DeltaParams& p) {
+    return {"mask", {reinterpret_cast<uintptr_t>(p.mask), p.N, {p.B, 1, 1}, {p.mask_sb, 0, 0}}};
+}
+
+// An output's rows must be apart, from one another and from every input's and other output's.
+int check_apart(std::initializer_list<Memory> out_list, std::initializer_list<Memory> in_list) {
+    const Memory *outs = out_list.begin(), *ins = in_list.begin();
+    const int no = (int)out_list.size(), ni = (int)in_list.size();
+    for (int i = 0; i < no; ++i) {
+        if (subq::rows_overlap_themselves(outs[i].rows))
+            return fail(SUBQ_ERR_INVALID_ARGUMENT, std::string("rows of ") + outs[i].name + " overlap");
+        for (int j = 0; j < ni + i; ++j) {
+            const Memory& other = j < ni ? ins[j] : outs[j - ni];
+            if (subq::rows_overlap(outs[i].rows, other.rows))
+                return fail(SUBQ_ERR_ALIAS, std::string(outs[i].name) + " shares memory with " + other.name);
+        }
+    }
+    return SUBQ_OK;
+}
+
+int check_delta_fwd_apart(const subq::DeltaParams& p, int dtype) {
+    const int64_t state = (int64_t)p.B * p.H * p.d * p.e * 4;
+    const std::initializer_list<Memory> outs = {of_tensor("o", p.o, p, p.e, dtype), of_bytes("state_out", p.S_out, state)};
+    const std::initializer_list<Memory> ins = {of_tensor("q", p.q, p, p.d, dtype), of_tensor("k", p.k, p, p.d, dtype), of_tensor("v", p.v, p, p.e, dtype),
+                          of_gate("beta", p.beta, p), of_gate("log_gamma", p.lg, p), of_mask(p),
+                          of_bytes("state_in", p.S_in == p.S_out ? nullptr : p.S_in, state)};  // (in place is allowed)
+    return check_apart(outs, ins);
+}
+
+int check_delta_bwd_apart(const subq::DeltaParams& p, int dtype) {
+    const int64_t state = (int64_t)p.B * p.H * p.d * p.e * 4, gates = (int64_t)p.B * p.H * p.N * 4;
+    const std::initializer_list<Memory> outs = {of_tensor("dq", p.dq, p, p.d, dtype), of_tensor("dk", p.dk, p, p.d, dtype), of_tensor("dv", p.dv, p, p.e, dtype),
+                           of_bytes("dbeta", p.dbeta, gates), of_bytes("dlog_gamma", p.dlg, gates), of_bytes("dstate_in", p.dS_in, state)};
+    const std::initializer_list<Memory> ins = {of_tensor("q", p.q, p, p.d, dtype), of_tensor("k", p.k, p, p.d, dtype), of_tensor("v", p.v, p, p.e, dtype),
+                          of_tensor("dout", p.g, p, p.e, dtype), of_gate("beta", p.beta, p), of_gate("log_gamma", p.lg, p), of_mask(p),
+                          of_bytes("state_in", p.S_in, state),
+                          of_bytes("dstate_out", p.dS_out == p.dS_in ? nullptr : p.dS_out, state)};
+    return check_apart(outs, ins);
+}
+
 int fill_delta_fwd(const subq_delta_fwd_args* a, subq::DeltaParams& p, int& path) {
     if (!a) return fail(SUBQ_ERR_INVALID_ARGUMENT, "null argument block");
     const subq_delta_desc& d = a->desc;
@@ -690,7 +743,7 @@ int subq_delta_fwd(const subq_delta_fwd_args* a) {
     subq::DeltaParams p;
     int path, launches = 1;
     int rc = fill_delta_fwd(a, p, path);
-    if (rc) return rc;
+    if (rc || (rc = check_delta_fwd_apart(p, a->desc.dtype))) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(a->stream);
     g_last_launches = 0;
     if (p.B == 0 || p.H == 0 || (p.N == 0 && !p.S_out)) {
@@ -725,7 +778,7 @@ int subq_delta_fwd(const subq_delta_fwd_args* a) {
 int subq_delta_bwd(const subq_delta_bwd_args* a) {
     subq::DeltaParams p;
     int rc = fill_delta_bwd(a, p);
-    if (rc) return rc;
+    if (rc || (rc = check_delta_bwd_apart(p, a->desc.dtype))) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(a->stream);
     g_last_launches = 0;
     cudaError_t err = cudaSuccess;
@@ -822,6 +875,24 @@ static int fill_ln(const subq_layer_norm_args* a, subq::LnParams& p, bool bwd) {
     return SUBQ_OK;
 }
 
+// (An output in an input's place, which fill_ln has seen to be laid out like it, is read before it is written.)
+static int check_ln_apart(const subq_layer_norm_args* a, bool bwd) {
+    auto rows = [&](const char* name, const void* at, int64_t stride, int dtype, const void* in_place = nullptr) -> Memory {
+        const __int128 es = (__int128)elem_size(dtype);
+        return {name, {reinterpret_cast<uintptr_t>(at == in_place ? nullptr : at), (int64_t)(a->dim * es), {a->rows, 1, 1}, {stride * es, 0, 0}}};
+    };
+    auto param = [&](const char* name, const void* at) { return of_bytes(name, at, a->dim * 4); };
+    if (!bwd) {
+        const std::initializer_list<Memory> outs = {rows("y", a->y, a->y_stride, a->y_dtype)};
+        const std::initializer_list<Memory> ins = {rows("x", a->x, a->x_stride, a->x_dtype, a->y), param("weight", a->weight), param("bias", a->bias)};
+        return check_apart(outs, ins);
+    }
+    const std::initializer_list<Memory> outs = {rows("dx", a->dx, a->dx_stride, a->x_dtype), param("dweight", a->dweight), param("dbias", a->dbias)};
+    const std::initializer_list<Memory> ins = {rows("x", a->x, a->x_stride, a->x_dtype, a->dx), rows("dy", a->dy, a->dy_stride, a->y_dtype, a->dx),
+                          param("weight", a->weight)};
+    return check_apart(outs, ins);
+}
+
 size_t subq_layer_norm_bwd_workspace_bytes(const subq_layer_norm_args* a) {
     subq::LnParams p;
     if (fill_ln(a, p, true) != SUBQ_OK || (!p.dw && !p.db) || p.rows == 0) return 0;
@@ -831,7 +902,7 @@ size_t subq_layer_norm_bwd_workspace_bytes(const subq_layer_norm_args* a) {
 int subq_layer_norm_fwd(const subq_layer_norm_args* a) {
     subq::LnParams p;
     int rc = fill_ln(a, p, false), launches = 0;
-    if (rc) return rc;
+    if (rc || (rc = check_ln_apart(a, false))) return rc;
     if (p.rows > 0) {
         cudaError_t err = subq::launch_layer_norm(p, a->x_dtype, a->y_dtype, false, static_cast<cudaStream_t>(a->stream), &launches);
         if (err != cudaSuccess) return fail_cuda(err, "subq_layer_norm_fwd launch");
@@ -843,7 +914,7 @@ int subq_layer_norm_fwd(const subq_layer_norm_args* a) {
 int subq_layer_norm_bwd(const subq_layer_norm_args* a) {
     subq::LnParams p;
     int rc = fill_ln(a, p, true), launches = 0;
-    if (rc) return rc;
+    if (rc || (rc = check_ln_apart(a, true))) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(a->stream);
     if (p.rows == 0) {  // no rows: the sums are 0
         for (float* x : {p.dw, p.db}) {
