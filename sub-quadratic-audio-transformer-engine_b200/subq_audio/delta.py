@@ -136,10 +136,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 class SubQLayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` over the last dimension on the library's kernels. Under autocast a float32 input gives the
     autocast type (the layer that follows reads its 16-bit input as it is; torch's norm returns float32, cast again
-    for each projection). Inputs the kernels do not take (CPU, float64, several dimensions) go to torch's norm."""
+    for each projection). Inputs the kernels do not take (CPU, float64, several dimensions, another width) go to torch's norm."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if not x.is_cuda or len(self.normalized_shape) != 1 or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        if (not x.is_cuda or len(self.normalized_shape) != 1 or x.shape[-1:] != self.normalized_shape
+                or x.dtype not in (torch.float32, torch.float16, torch.bfloat16)):
             return super().forward(x)
         out = x.dtype
         if x.dtype == torch.float32 and torch.is_autocast_enabled("cuda"):
