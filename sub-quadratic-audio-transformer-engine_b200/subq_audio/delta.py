@@ -174,13 +174,14 @@ class SubQGatedDeltaAttention(nn.Module):
         self.head_norm = nn.RMSNorm(self.head_dim, eps=1e-5)
         d0 = min(max(decay_init, 1e-4), 1.0 - 1e-4)
         self.raw_decay = nn.Parameter(torch.full((num_heads,), math.log(d0 / (1.0 - d0)), dtype=torch.float32))
-        # x / |x| is the per-head RMSNorm kernel with this weight
+        # x / sqrt(|x|^2 + 1e-6) is the per-head RMSNorm kernel with this weight
         self.register_buffer("unit", torch.full((self.head_dim,), self.head_dim ** -0.5), persistent=False)
 
     def _unit_heads(self, x: torch.Tensor) -> torch.Tensor:
         if ops.head_rmsnorm_supported(x):
             return _HeadRMSNorm.apply(x, self.unit, 1e-6 / self.head_dim)
-        return F.normalize(x.float(), dim=-1).to(x.dtype)
+        y = x.float()  # a width the kernel does not take: the same function
+        return (y * torch.rsqrt(y.square().sum(-1, keepdim=True) + 1e-6)).to(x.dtype)
 
     def forward(self, hidden_states: torch.Tensor, past_state: Any = None, attention_mask: Optional[torch.Tensor] = None,
                 use_cache: bool = False, position_embeddings: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, **kwargs: Any):

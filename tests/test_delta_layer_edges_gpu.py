@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from subq_audio import SubQLayerNorm
+from test_delta_layer_gpu import Block, plain_block, rel
 
 pytestmark = pytest.mark.gpu
 
@@ -14,3 +15,24 @@ def test_layer_norm_refuses_another_width_as_torch_does(affine):
             with pytest.raises((RuntimeError, ValueError)):
                 norm(torch.randn(*shape, device="cuda"))
         assert norm(torch.randn(5, 64, device="cuda")).shape == (5, 64)
+
+
+@pytest.mark.parametrize("small", [1.0, 1e-3])
+def test_heads_of_every_width_scale_queries_and_keys_alike(small):
+    """x / sqrt(|x|^2 + 1e-6), by the norm's kernel (64) and without it (80): also where |x| is near the root of 1e-6."""
+    for d in (64, 80):
+        torch.manual_seed(d)
+        m = Block(d=2 * d, heads=2, kv=1).cuda()
+        with torch.no_grad():
+            m.attn.q_proj.weight.mul_(small)
+            m.attn.k_proj.weight.mul_(small)
+        x = torch.randn(2, 70, 2 * d, device="cuda", requires_grad=True)
+        w = torch.randn(2, 70, 2 * d, device="cuda")
+        got = torch.autograd.grad((m(x)[0] * w).sum(), [x, *m.parameters()])
+        x64 = x.detach().double().requires_grad_(True)
+        y64, p = plain_block(m, x64)
+        want = torch.autograd.grad((y64 * w.double()).sum(), [x64, *p.values()])
+        # the tolerances of test_delta_layer_gpu.py's float32 block
+        assert rel(m(x)[0], y64) < 1e-5
+        for (n, _), a, b in zip([("x", x), *m.named_parameters()], got, want):
+            assert rel(a, b) < 3e-5, (d, n)
