@@ -152,7 +152,8 @@ class SubQGatedDeltaAttention(nn.Module):
     """A gated-delta layer with ``SubQLinearAttention``'s call contract: q/k/v/out projections, optional rotary
     positions, grouped K/V, queries and keys scaled to unit length per head, beta = sigmoid of a projection, decay
     = sigmoid(raw_decay + projection) per token and head, per-head RMSNorm of the output. Causal only. ``past_state``
-    and the returned state are [B, H, D, D] float32; single tokens run the token-recurrent kernel."""
+    and the returned state are [B, H, D, D] float32; single tokens run the token-recurrent kernel. Heads of at most 256
+    dimensions; of at most 128 where the layer is trained (the kernels have no backward above)."""
 
     def __init__(self, hidden_size: int, num_heads: int = 1, num_key_value_heads: Optional[int] = None,
                  decay_init: float = 0.99, bias: bool = False):
@@ -164,6 +165,8 @@ class SubQGatedDeltaAttention(nn.Module):
             raise ValueError(f"hidden_size {hidden_size} must be divisible by num_heads {num_heads}")
         if self.num_heads % self.num_key_value_heads != 0:
             raise ValueError(f"num_heads {num_heads} must be divisible by num_key_value_heads {self.num_key_value_heads}")
+        if self.head_dim > 256:
+            raise ValueError(f"heads of {self.head_dim} dimensions are wider than the kernels' 256: more heads are needed")
         kv = self.num_key_value_heads * self.head_dim
         self.q_proj = nn.Linear(hidden_size, hidden_size, bias=bias)
         self.k_proj = nn.Linear(hidden_size, kv, bias=bias)
