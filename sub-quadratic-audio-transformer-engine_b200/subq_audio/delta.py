@@ -84,7 +84,8 @@ def gated_delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bet
     ``q``, ``k``, ``v`` are [B, T, D] or [B, H, T, D]; ``beta`` and ``log_gamma`` (log of the decay, at most 0) are
     None, a number, or a tensor [], [H] or [B, H, T] ([B, T] with 3-D inputs); ``past_state`` a state [B, H, d, e] or a
     tuple that starts with one; ``attention_mask`` as in ``chunkwise_flash_linear_attention``. Returns
-    ``(out, S_next)``, out in q's memory order; gradients also flow through the states. The backward needs d <= 128.
+    ``(out, S_next)``, out in q's memory order; gradients also flow through the states. The backward needs d <= 128, and is
+    of first order and reverse mode (second gradients, forward mode and ``torch.func`` transforms raise).
     """
     is_3d = q.ndim == 3
     if is_3d:
@@ -129,22 +130,35 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """Layer norm over the last dimension, differentiable (``ops.layer_norm``)."""
+    """Layer norm over the last dimension, differentiable once, in reverse mode (``ops.layer_norm``). ``torch.func``
+    transforms, forward mode and second gradients raise: torch's ``layer_norm`` has them."""
     return _LayerNorm.apply(x, weight, bias, eps, out_dtype)
 
 
 class SubQLayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` over the last dimension on the library's kernels. Under autocast a float32 input gives the
     autocast type (the layer that follows reads its 16-bit input as it is; torch's norm returns float32, cast again
-    for each projection). Inputs the kernels do not take (CPU, float64, several dimensions, another width) go to torch's norm."""
+    for each projection); where something else than a projection follows, ``out_dtype=torch.float32`` keeps torch's
+    result. ``out_dtype`` holds for float32 inputs, with or without autocast; a 16-bit input gives its own type. Inputs
+    the kernels do not take (CPU, float64, several dimensions, another width) go to torch's norm. The gradient is
+    ``layer_norm``'s: first order, reverse mode (no second gradients, forward mode or ``torch.func`` transforms)."""
+
+    out_dtype: Optional[torch.dtype] = None
+
+    def __init__(self, *args: Any, out_dtype: Optional[torch.dtype] = None, **kwargs: Any):
+        super().__init__(*args, **kwargs)
+        self.out_dtype = out_dtype
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if (not x.is_cuda or len(self.normalized_shape) != 1 or x.shape[-1:] != self.normalized_shape
                 or x.dtype not in (torch.float32, torch.float16, torch.bfloat16)):
             return super().forward(x)
         out = x.dtype
-        if x.dtype == torch.float32 and torch.is_autocast_enabled("cuda"):
-            out = torch.get_autocast_dtype("cuda")
+        if x.dtype == torch.float32:
+            if self.out_dtype is not None:
+                out = self.out_dtype
+            elif torch.is_autocast_enabled("cuda"):
+                out = torch.get_autocast_dtype("cuda")
         return layer_norm(x, self.weight, self.bias, self.eps, out)
 
 

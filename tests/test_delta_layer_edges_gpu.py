@@ -36,3 +36,28 @@ def test_heads_of_every_width_scale_queries_and_keys_alike(small):
         assert rel(m(x)[0], y64) < 1e-5
         for (n, _), a, b in zip([("x", x), *m.named_parameters()], got, want):
             assert rel(a, b) < 3e-5, (d, n)
+
+
+def test_layer_norm_keeps_float32_under_autocast_where_it_is_asked_to():
+    torch.manual_seed(3)
+    x = torch.randn(7, 96, device="cuda", requires_grad=True)
+    plain, norm = torch.nn.LayerNorm(96).cuda(), SubQLayerNorm(96, out_dtype=torch.float32).cuda()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        want, got, default = plain(x), norm(x), SubQLayerNorm(96).cuda()(x)
+    assert want.dtype == got.dtype == torch.float32 and default.dtype == torch.bfloat16
+    assert rel(got, want) < 1e-6  # float32 sums of 96 terms on both sides (test_layer_norm_gpu.py)
+    w = torch.randn_like(want)
+    assert rel(torch.autograd.grad((got * w).sum(), x)[0], torch.autograd.grad((want * w).sum(), x)[0]) < 2e-6
+    assert SubQLayerNorm(96, out_dtype=torch.float16).cuda()(x).dtype == torch.float16
+    assert norm(x.half()).dtype == torch.float16
+
+
+def test_what_layer_norm_does_not_differentiate_raises():
+    x = torch.randn(3, 96, device="cuda", requires_grad=True)
+    norm = SubQLayerNorm(96).cuda()
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: norm(t).square().sum())(x.detach())
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(norm, (x.detach(),), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(norm(x).square().sum(), x, create_graph=True)[0].sum().backward()
