@@ -235,7 +235,18 @@ size_t subq_head_rmsnorm_bwd_workspace_bytes(const subq_rmsnorm_args* args);
  * Paths: SUBQ_PATH_EXACT is the token-recurrent kernel (d, e <= 256),
  * SUBQ_PATH_CHUNKED the chunk kernels (d <= 128, e <= 256). AUTO takes the
  * recurrent kernel for d > 128 and for calls of at most 16 tokens that fill no
- * handover. The backward has the chunk form only (d <= 128). */
+ * handover. The backward has the chunk form only (d <= 128).
+ *
+ * Memory, KB for each (batch, head) and 64 tokens (d = e = 64; d = e = 128), q, k,
+ * v and o being 32 (64) in 16 bits and 64 (128) in float32:
+ *                                    16-bit inputs     float32
+ *   forward's workspace               22  (22)          32  (32)   0 with a handover
+ *   handover                          54 (118)          80 (176)
+ *   backward's workspace              32  (96)          48 (144)   with a handover
+ *                                     86 (214)         128 (320)   without
+ * Where a call with few sequences is cut into segments, 32 KB (128 KB above
+ * d = 64) for each (batch, head) and segment; the backward also holds float32
+ * gradients per state head of shared q, k and v. The recurrent kernel needs none. */
 typedef struct subq_gate {
     const float* data; /* [B, heads, N] float32 with element strides (0 allowed) */
     int64_t stride_b, stride_h, stride_n;

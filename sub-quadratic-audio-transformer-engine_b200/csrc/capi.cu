@@ -519,19 +519,22 @@ int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc&
 // first pass finds the states: the first segment's own state, for the others their own state and what they do to the one
 // before them, but for the last. Its steps take 0.7 of the walk's, or 1.1 where two CTAs share an SM (16-bit inputs). The
 // walk itself then takes n / G steps, the join 1 us a segment (2 us above d = 64), and the two launches 8 us. G is the
-// count with the least sum, taken where that is a tenth below the single walk's. Measured with the gates' kernel, us,
-// single and cut (the counts beside G were at most 4 % faster):
-//   bf16, d = 64:  1 x 12 heads, 65536 tokens   1822, 778 (G = 6)    2 x 12, 8192     267, 191 (G = 3)   1 x 4, 4096   122, 60 (G = 9)
-//                  3 x 12 heads, 16384 tokens    554, 510 (G = 2)    4 x 12, 4096     162, none (G = 2: 213, more CTAs than SMs)
-//   float32:       2 x 12 heads, 1537 tokens     148, 124 (G = 3)    1 x 4, 16384    1112, 243 (G = 18)
-//   d = 128:       1 x 4 heads, 8192 tokens      319, 134 (bf16, G = 8)   835, 251 (float16, G = 9)   1228, 441 (float32, G = 6)
+// count with the least sum, taken where that is a tenth below the single walk's. Device time of a captured call, us, single
+// and cut with the count that the rule takes (other counts were at most 4 % faster, 2 % but for one):
+//   bf16, d = 64:  1 x 12 heads, 65536 tokens   1843, 782 (G = 6)    2 x 12, 8192     268, 190 (G = 3)   1 x 4, 4096   121, 53 (G = 10)
+//                  3 x 12 heads, 16384 tokens    555, 512 (G = 2)    4 x 12, 4096     164, none (G = 2: 211, more CTAs than SMs)
+//                  1 x 1 head, 65536 tokens     1690, 160 (G = 38)   float16:  1 x 4, 4096   180, 66 (G = 16)
+//   float32:       2 x 12 heads, 1537 tokens     152, 117 (G = 3)    1 x 4, 16384    1106, 227 (G = 18)
+//   d = 128:       1 x 4 heads, 8192 tokens      316, 129 (bf16, G = 9)   823, 238 (float16, G = 9)   1245, 426 (float32, G = 9)
 //
 // The walk back over the chunks is cut the same way. Its first pass has a whole step's work (the products with dO beside
-// the chain), so the sum has to be a fifth below. The gradients' call from the forward's handover, us, single and cut:
-//   bf16, d = 64:  1 x 12 heads, 65536 tokens   2824, 1572 (G = 6)   2 x 12, 8192     450, 355 (G = 3)   1 x 4, 4096   197, 110 (G = 8)
-//                  3 x 12 heads, 16384 tokens   1035, none (G = 2: 982)                4 x 12, 4096     318, none (G = 2: 384)
-//   float32:       2 x 12 heads, 1537 tokens     278, none (G = 3: 272)
-//   d = 128:       1 x 4 heads, 8192 tokens      447, 243 (bf16, G = 6)   1633, 740 (float32, G = 6)
+// the chain, for the identity's columns too, where dO is 0), so the sum has to be a fifth below. The gradients' call from
+// the forward's handover, us, single and cut:
+//   bf16, d = 64:  1 x 12 heads, 65536 tokens   2748, 1585 (G = 23; G = 6: 1563)   2 x 12, 8192  446, 350 (G = 3)   1 x 4, 4096  158, 72 (G = 10)
+//                  3 x 12 heads, 16384 tokens   1030, none (G = 2: 977)            4 x 12, 4096  315, none (G = 2: 377)
+//                  1 x 1 head, 65536 tokens     2144, 223 (G = 38)                 float16:  1 x 4, 4096   215, 92 (G = 10)
+//   float32:       2 x 12 heads, 1537 tokens     238, none (G = 3: 229)            1 x 4, 16384  1237, 418 (G = 18)
+//   d = 128:       1 x 4 heads, 8192 tokens      446, 238 (bf16, G = 6)   1116, 471 (float16, G = 6)   1634, 725 (float32, G = 6)
 struct DeltaSplit {
     int nseg, chunks;
 };

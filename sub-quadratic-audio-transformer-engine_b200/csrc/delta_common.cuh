@@ -17,6 +17,13 @@
 // 2, fp32: 3); what is computed in between (states, W, Y, scores) is held in
 // NX = 2 planes for 16-bit inputs and 3 for float32, and plane products whose
 // planes' indices sum to NX or more are below that precision and left out.
+// With 16-bit inputs that is 1.3e-4 of an output in bf16 (one rounding in a
+// thousand goes the other way) and 3e-6 to 6e-6 of float32 results. Who needs
+// three planes passes float32 copies of the inputs (exact) and has the outputs
+// in float32 (4e-7), for 2.7 times the time of a training step and 3.1 times
+// that of a prompt (8 x 12 heads of 2047 tokens). Summing the small plane
+// products apart, as for float32, changes nothing with two planes: their
+// rounding is the larger error.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -16,7 +16,7 @@
 //
 // Measured, bf16, d = e = 64, 8 x 8 heads of 8192 tokens (8192 chunks): gates and Y
 // 100 us (issue-bound: 46 % of the issue slots with 24 warps per SM, tensor pipe 17 %);
-// the walk 1.7 us a chunk, 1.9 us where the backward's planes are written (247 us:
+// the walk 1.7 us a chunk, 2.0 us where the backward's planes are written (254 us:
 // shared memory 76 % busy on the SMs at work, tensor pipe 35 %).
 #pragma once
 

@@ -5,8 +5,9 @@
 // one 128-byte access. S is read once and written once; per token
 //   r = S^T k, s = S^T q (one reduction),  u = beta (v - gamma r),
 //   S <- gamma S + k u^T,  o = scale (gamma s + (q.k) u),
-// in float32. Bound by the state's 8 d e bytes for many sequences (one token),
-// by launch latency for few.
+// in float32. Bound by the state's 8 d e bytes for many sequences (one token; 0.63
+// of the measured copy bandwidth: the grid's second round is not full), by launch
+// latency for few.
 #include "delta_common.cuh"
 #include "delta_launch.h"
 #include "scan_launch.h"
@@ -143,7 +144,8 @@ cudaError_t step_t(const DeltaParams& p, cudaStream_t st) {
         return cudaGetLastError();
     };
     // two warps a tile: the work around a tile's 2048 state elements (d = 64) is as much as theirs, so fewer threads
-    // with more elements each are faster (256 x 12 heads of 64 x 64: 24.6 us, 26.6 us with four warps)
+    // with more elements each are faster (256 x 12 heads of 64 x 64: 24.6 us, 26.6 us with four warps). At 128 registers
+    // 8 of the 10 CTAs an SM are resident (4 of 5 at d = 128): 1184 CTAs, then the other 296 on a quarter of the places.
     const bool full = vec && p.e % 32 == 0;
     if (p.d <= 32) return run(delta_step_kernel<T, 4, 2, false>, 64, 12);
     if (p.d == 64 && full) return run(delta_step_kernel<T, 8, 2, true>, 64, 10);

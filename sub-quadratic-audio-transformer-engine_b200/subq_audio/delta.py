@@ -47,7 +47,8 @@ def _gate_grad(g: Optional[torch.Tensor], x: Optional[torch.Tensor], strided: bo
 
 class _GatedDelta(torch.autograd.Function):
     """The rule on the kernels; differentiable in q, k, v, beta, log_gamma and the initial state, and through the
-    final state. The forward keeps its handover for the backward where one will follow."""
+    final state. The forward keeps its handover for the backward where one will follow (``ops.DeltaHandover`` has its
+    size; ``torch.utils.checkpoint`` around the layer keeps it from staying)."""
 
     @staticmethod
     def forward(ctx, q, k, v, beta, lg, mask, S0, scale, want_state, keep):

@@ -59,3 +59,17 @@ def test_a_state_that_lasts_keeps_its_bits(B, H, N, d, e, dtype):
     got = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, state=S0, dstate=dS, need_dlog_gamma=True, need_dstate=True, handover=ho)
     for name, a, w in zip(NAMES, got, ref.gradients(q, k, v, beta, lg, None, d ** -0.5, S0, do, dS)):
         assert rel(a, w) < tol(a, dtype, d), name
+
+
+def test_float32_copies_of_16_bit_inputs_carry_24_bits():
+    """The way to ask for more than the 16 bits that 16-bit inputs' operands have."""
+    d = 64
+    q, k, v, do, beta, S0, dS = inputs(2, 4, 2, 700, d, d, "bf16", 1, 0.1, 0.9)
+    lg = -0.02 * beta
+    o_ref, S_ref = ref.forward(q, k, v, beta, lg, None, d ** -0.5, S0)
+    q, k, v, do = (x.float() for x in (q, k, v, do))
+    o, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, state=S0, return_state=True)
+    assert rel(S, S_ref) < tol(S, "fp32", d) and rel(o, o_ref) < tol(o, "fp32", d)
+    got = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, state=S0, dstate=dS, need_dlog_gamma=True, need_dstate=True)
+    for name, a, w in zip(NAMES, got, ref.gradients(q, k, v, beta, lg, None, d ** -0.5, S0, do, dS)):
+        assert rel(a, w) < tol(a, "fp32", d), name
