@@ -226,8 +226,8 @@ size_t subq_head_rmsnorm_bwd_workspace_bytes(const subq_rmsnorm_args* args);
  * v, dout, beta or log_gamma is used. q, k, v and o are [B, heads, N, *] views;
  * q, k and v may each have fewer heads (a divisor of `heads`), state head h
  * then reading head h / (heads / x_heads), and their gradients sum over the
- * group. fp32, fp16, bf16; products accumulate in float32, and operands are
- * carried to 16 bits of mantissa (24 for fp32). For bounded states |k_t| <= 1
+ * group. fp32, fp16, bf16; products accumulate in float32, and operands in
+ * between are carried to 24 bits of mantissa. For bounded states |k_t| <= 1
  * with beta_t in [0, 2] and gamma_t <= 1, as usual for the rule; the kernels do
  * not require it. A live token that is not finite makes its chunk of 64
  * tokens, and what follows, not finite.
@@ -239,11 +239,9 @@ size_t subq_head_rmsnorm_bwd_workspace_bytes(const subq_rmsnorm_args* args);
  *
  * Memory, KB for each (batch, head) and 64 tokens (d = e = 64; d = e = 128), q, k,
  * v and o being 32 (64) in 16 bits and 64 (128) in float32:
- *                                    16-bit inputs     float32
- *   forward's workspace               22  (22)          32  (32)   0 with a handover
- *   handover                          54 (118)          80 (176)
- *   backward's workspace              32  (96)          48 (144)   with a handover
- *                                     86 (214)         128 (320)   without
+ *   forward's workspace                32  (32), none with a handover
+ *   handover                           80 (176)
+ *   backward's workspace               48 (144) with a handover, 128 (320) without
  * Where a call with few sequences is cut into segments, 32 KB (128 KB above
  * d = 64) for each (batch, head) and segment; the backward also holds float32
  * gradients per state head of shared q, k and v. The recurrent kernel needs none. */

@@ -514,45 +514,46 @@ int delta_tensor(const subq_tensor4& t, const char* name, const subq_delta_desc&
     return SUBQ_OK;
 }
 
-// Segments of a sequence that are walked side by side when there are few sequences. A walk over n chunks takes n steps of
-// a time that depends on the type and d (below) and not on the number of CTAs, up to one CTA per SM. With G segments a
-// first pass finds the states: the first segment's own state, for the others their own state and what they do to the one
-// before them, but for the last. Its steps take 0.7 of the walk's, or 1.1 where two CTAs share an SM (16-bit inputs). The
-// walk itself then takes n / G steps, the join 1 us a segment (2 us above d = 64), and the two launches 8 us. G is the
-// count with the least sum, taken where that is a tenth below the single walk's. Device time of a captured call, us, single
-// and cut with the count that the rule takes (other counts were at most 4 % faster, 2 % but for one):
-//   bf16, d = 64:  1 x 12 heads, 65536 tokens   1843, 782 (G = 6)    2 x 12, 8192     268, 190 (G = 3)   1 x 4, 4096   121, 53 (G = 10)
-//                  3 x 12 heads, 16384 tokens    555, 512 (G = 2)    4 x 12, 4096     164, none (G = 2: 211, more CTAs than SMs)
-//                  1 x 1 head, 65536 tokens     1690, 160 (G = 38)   float16:  1 x 4, 4096   180, 66 (G = 16)
-//   float32:       2 x 12 heads, 1537 tokens     152, 117 (G = 3)    1 x 4, 16384    1106, 227 (G = 18)
-//   d = 128:       1 x 4 heads, 8192 tokens      316, 129 (bf16, G = 9)   823, 238 (float16, G = 9)   1245, 426 (float32, G = 9)
+// Segments of a sequence that are walked side by side when there are few sequences. A walk over n chunks takes n steps, and
+// about 3 more to begin and end, of a time that depends on the type and d (below) and not on the number of CTAs, up to one
+// CTA per SM. With G segments a first pass finds the states: the first segment's own state, for the others their own state
+// and what they do to the one before them, but for the last. Its steps take 0.7 of the walk's, or 1.1 where two CTAs share
+// an SM. The walk itself then takes n / G steps, the join 1.4 us a segment (2 us above d = 64), and the two launches 8 us.
+// G is the count with the least sum, taken where that is a tenth below the single walk's. Device time of a captured call,
+// us, single and cut with the count that the rule takes (other counts were at most 2 % faster):
+//   bf16, d = 64:  1 x 12 heads, 65536 tokens   2696, 1139 (G = 6)   2 x 12, 8192     381, 260 (G = 3)   1 x 4, 4096   174, 66 (G = 10)
+//                  3 x 12 heads, 16384 tokens    795, 721 (G = 2)    4 x 12, 4096     227, none (G = 2: 291, more CTAs than SMs)
+//                  1 x 1 head, 65536 tokens     2509, 201 (G = 38)   float16:  1 x 4, 4096   238, 82 (G = 10)
+//   float32:       2 x 12 heads, 1537 tokens     150, 119 (G = 3)    1 x 4, 16384    1102, 231 (G = 18)
+//   d = 128:       1 x 4 heads, 8192 tokens      481, 176 (bf16, G = 6)   1036, 303 (float16, G = 9)   1243, 430 (float32, G = 6)
 //
 // The walk back over the chunks is cut the same way. Its first pass has a whole step's work (the products with dO beside
 // the chain, for the identity's columns too, where dO is 0), so the sum has to be a fifth below. The gradients' call from
 // the forward's handover, us, single and cut:
-//   bf16, d = 64:  1 x 12 heads, 65536 tokens   2748, 1585 (G = 23; G = 6: 1563)   2 x 12, 8192  446, 350 (G = 3)   1 x 4, 4096  158, 72 (G = 10)
-//                  3 x 12 heads, 16384 tokens   1030, none (G = 2: 977)            4 x 12, 4096  315, none (G = 2: 377)
-//                  1 x 1 head, 65536 tokens     2144, 223 (G = 38)                 float16:  1 x 4, 4096   215, 92 (G = 10)
-//   float32:       2 x 12 heads, 1537 tokens     238, none (G = 3: 229)            1 x 4, 16384  1237, 418 (G = 18)
-//   d = 128:       1 x 4 heads, 8192 tokens      446, 238 (bf16, G = 6)   1116, 471 (float16, G = 6)   1634, 725 (float32, G = 6)
+//   bf16, d = 64:  1 x 12 heads, 65536 tokens   3809, 2194 (G = 4)   2 x 12, 8192     612, 490 (G = 3)   1 x 4, 4096   217, 90 (G = 10)
+//                  3 x 12 heads, 16384 tokens   1415, none (G = 2: 1382)              4 x 12, 4096     432, none (G = 2: 516)
+//                  1 x 1 head, 65536 tokens     2996, 289 (G = 38)   float16:  1 x 4, 4096   270, 119 (G = 10)
+//   float32:       2 x 12 heads, 1537 tokens     238, none (G = 3: 229)                1 x 4, 16384   1231, 420 (G = 18)
+//   d = 128:       1 x 4 heads, 8192 tokens      631, 342 (bf16, G = 6)   1395, 623 (float16, G = 6)   1620, 721 (float32, G = 6)
 struct DeltaSplit {
     int nseg, chunks;
 };
 DeltaSplit delta_split(const subq::DeltaParams& p, int dtype, bool back = false) {
     const int64_t bh = (int64_t)p.B * p.H, ncb = (p.e + 31) / 32, ndb = (p.d + 31) / 32;
     const int wide = p.d > 64;
-    constexpr double kSteps[3][2] = {{4.3, 9.2}, {2.5, 6.4}, {1.7, 2.3}};  // us: float32, float16, bfloat16
-    const double step = kSteps[dtype == SUBQ_FP32 ? 0 : dtype == SUBQ_FP16 ? 1 : 2][wide], join = wide ? 2.0 : 1.0, launches = 8.0;
+    constexpr double kSteps[3][2] = {{4.3, 9.2}, {3.6, 8.0}, {2.4, 3.7}};  // us: float32, float16, bfloat16
+    const double step = kSteps[dtype == SUBQ_FP32 ? 0 : dtype == SUBQ_FP16 ? 1 : 2][wide], join = wide ? 2.0 : 1.4, launches = 8.0;
+    const bool pairs = dtype == (wide ? SUBQ_FP16 : SUBQ_BF16);  // two CTAs of the first pass per SM (chain_ctas)
     auto waves = [](int64_t ctas, int64_t slots) { return (double)((ctas + slots - 1) / slots); };
-    double best = (back ? 0.8 : 0.9) * p.nc * step * waves(bh * ncb, 148);
+    double best = (back ? 0.8 : 0.9) * (p.nc + 3) * step * waves(bh * ncb, 148);
     DeltaSplit s = {1, p.nc};
     if (back && p.dS_in && p.dS_in == p.dS_out) return s;  // (one CTA reads what another one's result would overwrite)
     for (int g = 2; g <= 64 && 2 * g <= p.nc; ++g) {
         const int chunks = (p.nc + g - 1) / g;
         if ((p.nc + chunks - 1) / chunks != g) continue;  // (the same split with fewer segments)
         const int64_t ctas = bh * ((g - 1) * (ncb + ndb) - ndb);
-        const double states = back ? waves(ctas, 148) : dtype == SUBQ_FP32 || ctas <= 148 ? 0.7 * waves(ctas, 148) : 1.1 * waves(ctas, 296);
-        const double t = chunks * step * (waves(bh * g * ncb, 148) + states) + g * join + launches;
+        const double states = back ? waves(ctas, 148) : !pairs || ctas <= 148 ? 0.7 * waves(ctas, 148) : 1.1 * waves(ctas, 296);
+        const double t = (chunks + 3) * step * (waves(bh * g * ncb, 148) + states) + g * join + launches;
         if (t < best) best = t, s = {g, chunks};
     }
     return s;
@@ -564,7 +565,7 @@ struct DeltaBytes {
     size_t segs() const { return seg_S + seg_M + seg_in; }
 };
 DeltaBytes delta_bytes(const subq::DeltaParams& p, int dtype) {
-    const size_t nx = dtype == SUBQ_FP32 ? 3 : 2, chunks = (size_t)p.B * p.H * p.nc;
+    const size_t nx = subq::kDeltaPlanes, chunks = (size_t)p.B * p.H * p.nc;
     const size_t ncw = 2 * ((p.e + subq::kDeltaCols - 1) / subq::kDeltaCols), dp = p.d <= 64 ? 64 : 128;
     const size_t mat = align_up(chunks * nx * subq::kYBlocks * 512);
     const int nseg = delta_split(p, dtype).nseg;

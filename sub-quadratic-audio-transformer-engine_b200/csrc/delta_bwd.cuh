@@ -18,14 +18,15 @@
 // a_t enter and column t of E and b_t leave, the very same numbers: what they are
 // off by leaves with them, and what is left is the error of the terms that count
 // for t. (The shorter running sum of q_i.dq_i - v_i.dv_i is the same in exact
-// arithmetic, but keeps the errors of tokens that have nothing to do with t: 3e-5
-// against 5e-6 with 16-bit inputs and fast decay.)
+// arithmetic, but keeps the errors of tokens that have nothing to do with t: six
+// times as far off with fast decay.)
 //
 // Measured, bf16, d = e = 64, 8 x 8 heads of 8192 tokens (8192 chunks): the walk back
-// 275 us (2.1 us a chunk, bound like the forward's by shared memory and the latency of
-// its three products in a row; few sequences are cut into segments, see delta_join.cuh
-// and the rule in capi.cu), the gradients 400 us (105 KB read and written a chunk,
-// 0.33 of measured HBM; tensor pipe 41 %, shared memory 52 %, 16 warps per SM).
+// 396 us (3.1 us a chunk, bound like the forward's by shared memory, 60 % busy, and
+// the latency of its three products in a row; few sequences are cut into segments, see
+// delta_join.cuh and the rule in capi.cu), the gradients 543 us (140 KB read and
+// written a chunk, 0.32 of measured HBM; tensor pipe 38 %, shared memory 53 %, 16
+// warps per SM, whose 128 registers a thread spill 168 bytes).
 #pragma once
 
 #include "delta_common.cuh"
@@ -40,8 +41,9 @@ using namespace dl;
 // ------------------------------------------------------------------ the walk back
 template <typename T, int DP>
 struct RevSmem {
-    static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
-    static constexpr int kStages = kIn == 1 ? (DP == 64 ? 3 : 2) : DP == 64 ? 2 : 1;  // as in the forward's walk
+    static constexpr int kIn = kDeltaIn<T>, kX = kDeltaPlanes;
+    // chunks in shared memory: the one at work and the next, where they fit one more on its way
+    static constexpr int kStages = kIn == 1 ? (DP == 64 ? 3 : 2) : DP == 64 ? 2 : 1;
     struct Stage {
         alignas(128) unsigned char k[kIn * 64 * DP * 2];
         alignas(128) unsigned char q[kIn * 64 * DP * 2];
@@ -54,11 +56,11 @@ struct RevSmem {
     alignas(16) unsigned char G[2][DP / 16][kX * 512];  // G^T, planes
     alignas(16) unsigned char R[2][4][kX * 512];        // -(beta dU)^T, planes
     // as W in the forward's walk: planes of -e^g beta Z and of Z, or Z in float32
-    static constexpr bool kShared = kX == 2;
+    static constexpr bool kShared = kIn < 3;
     alignas(16) unsigned char Zk[2][kShared ? 4 : 1][kX * 512];
     union {
-        float4 Z[2][8 * 32];
-        unsigned char Zp[2][4][1024];
+        float4 Z[2][kShared ? 1 : 8 * 32];
+        unsigned char Zp[2][kShared ? 4 : 1][kX * 512];
     } z;
     float4 e2[2][DP / 8 * 32];                          // (scale (e^g Q)^T dO)^T; before that, (P^T dO)^T of the same chunk
 };
@@ -66,7 +68,7 @@ struct RevSmem {
 // One warp of a chain pair: half `A` of d of G^T in its accumulators; dU and Z of its token blocks.
 template <typename T, int DP, bool STATES>
 __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const WalkJob& job, int A, int pair, int lane) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = RevSmem<T, DP>::kStages;
+    constexpr int NIN = kDeltaIn<T>, NX = kDeltaPlanes, NST = RevSmem<T, DP>::kStages;
     constexpr int NH = DP / 16;
     constexpr bool kShared = RevSmem<T, DP>::kShared;
     const int g = lane >> 2, t = lane & 3;
@@ -202,7 +204,7 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const WalkJob
 // its share of the planes of G and Z.
 template <typename T, int DP, bool STATES>
 __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kGTile = 64 * kDeltaCols * 2;
+    constexpr int NIN = kDeltaIn<T>, NX = kDeltaPlanes, kGTile = 64 * kDeltaCols * 2;
     constexpr int NST = RevSmem<T, DP>::kStages, NH = DP / 16;
     const int g = lane >> 2, t = lane & 3, ncb = (p.e + kDeltaCols - 1) / kDeltaCols, cb = job.cb;
     const int64_t bh = job.bh;
@@ -333,7 +335,7 @@ __device__ __forceinline__ void rev_side_warp(RevSmem<T, DP>& sm, const DeltaPar
 // from the end; the last one's columns of the identity, as the first's results, nobody needs.
 template <typename T, int DP, bool STATES>
 __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX;
+    constexpr int NIN = kDeltaIn<T>, NX = kDeltaPlanes;
     constexpr int NST = RevSmem<T, DP>::kStages;
     extern __shared__ __align__(128) unsigned char raw[];
     RevSmem<T, DP>& sm = *reinterpret_cast<RevSmem<T, DP>*>(raw);
@@ -484,11 +486,11 @@ __global__ void __launch_bounds__(384, 1) delta_rev_kernel(const DeltaParams p) 
 // ------------------------------------------------------------------ the gradients
 template <typename T, int DP>
 struct GradSmem {
-    static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
+    static constexpr int kIn = kDeltaIn<T>, kX = kDeltaPlanes;
     static constexpr int kState = 2 * DP / 16 * kX * 512, kCol = 2 * 4 * kX * 512, kGTile = kIn * 64 * kDeltaCols * 2;
-    // CTAs per SM, and blocks of 32 value columns in flight (both of e = 64 where that fits twice on an SM)
+    // CTAs per SM (two with room for one block of 32 value columns each: 991 us for the backward of 8 x 8 heads of 8192
+    // tokens in bf16; one with two blocks, or with more registers, 1140 and 1190)
     static constexpr int kCtas = sizeof(T) == 2 && DP == 64 ? 2 : 1;
-    static constexpr int kBufs = kIn == 1 && DP == 64 ? 2 : 1;
     Gates s;
     float wz[kDeltaC];
     // halves (of d; D1's and D2's) of a_i, b_j and E's row sums, and E's column sums by block of rows
@@ -508,7 +510,7 @@ struct GradSmem {
         alignas(128) unsigned char d2[kX * kYBlocks * 512];
     };
     union {
-        In blk[kBufs];
+        In in;
         Scores sc;
     } u;
 };
@@ -587,7 +589,7 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     bool direct = false;  // bf16: tiles straight to shared memory
     if constexpr (NIN == 1) direct = p.k.vec && p.q.vec && p.g.vec && p.d % 8 == 0 && p.e % 8 == 0;
     auto start = [&](int eb) {  // the planes of a block of value columns
-        auto& in = sm.u.blk[eb % Smem::kBufs];
+        auto& in = sm.u.in;
         const int64_t at = chunk * 2 * ncb + 2 * eb;
         async16<256>(in.S0, p.S0 + at * (Smem::kState / 2), Smem::kState, tid);
         async16<256>(in.G, p.dS + at * (Smem::kState / 2), Smem::kState, tid);
@@ -601,7 +603,6 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
         async_tile<T, DP, 256>(sm.q, p.q, tensor_base(p.q, b, h), n0, 0, p.d, p.N, tid);
     }
     start(0);
-    if (Smem::kBufs == 2 && ncb > 1) start(1);
     const Gates& s = sm.s;
     async_wait();
     __syncthreads();
@@ -626,8 +627,8 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     zero_acc<2>(ex);
 
     for (int eb = 0; eb < ncb; ++eb) {
-        auto& in = sm.u.blk[eb % Smem::kBufs];
-        if (eb >= Smem::kBufs) {
+        auto& in = sm.u.in;
+        if (eb) {
             __syncthreads();  // the block before has been read
             start(eb);
         }
@@ -643,52 +644,50 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
         const uint32_t dO = smem_addr(in.dO);
 #pragma unroll
         for (int cw = 0; cw < 2; ++cw) {  // 16 value columns: one k step
-            uint32_t ao[NIN][4], aw[NX][4], az[NX][4];
+            uint32_t ao[NIN][4], a[NX][4];  // dO; Z, then W (one at a time: the accumulators leave no registers for both)
+            auto load_a = [&](uint32_t from) {
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    uint32_t r[4];
+                    ldm_t(r, from + ((cw * 4 + rb) * NX + pl) * 512);
+                    a[pl][0] = r[0]; a[pl][1] = r[2]; a[pl][2] = r[1]; a[pl][3] = r[3];
+                }
+            };
+            auto load_b = [&](uint32_t (&b0)[NX][2], uint32_t (&b1)[NX][2], uint32_t from) {
+#pragma unroll
+                for (int pl = 0; pl < NX; ++pl) {
+                    uint32_t r[4];
+                    ldm_t(r, from + pl * 512);
+                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
+                }
+            };
 #pragma unroll
             for (int pl = 0; pl < NIN; ++pl) a_rows<kDeltaCols>(ao[pl], dO + pl * kGTile, 16 * rb, cw, lane);
-#pragma unroll
-            for (int pl = 0; pl < NX; ++pl) {
-                uint32_t r[4];
-                ldm_t(r, W + ((cw * 4 + rb) * NX + pl) * 512);
-                aw[pl][0] = r[0]; aw[pl][1] = r[2]; aw[pl][2] = r[1]; aw[pl][3] = r[3];
-                ldm_t(r, Z + ((cw * 4 + rb) * NX + pl) * 512);
-                az[pl][0] = r[0]; az[pl][1] = r[2]; az[pl][2] = r[1]; az[pl][3] = r[3];
-            }
+            load_a(Z);
 #pragma unroll
             for (int n = 0; n < NB / 2; ++n) {
-                const int kk = hf * (NB / 2) + n;
                 uint32_t b0[NX][2], b1[NX][2];
-#pragma unroll
-                for (int pl = 0; pl < NX; ++pl) {
-                    uint32_t r[4];
-                    ldm_t(r, S0 + ((cw * (DP / 16) + kk) * NX + pl) * 512);
-                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                }
+                load_b(b0, b1, S0 + (cw * (DP / 16) + hf * (NB / 2) + n) * NX * 512);
                 mma_pair<NIN, NX, NX>(dq[2 * n], dq[2 * n + 1], ao, b0, b1);
-                mma_pair<NX, NX, NX>(dk2[2 * n], dk2[2 * n + 1], az, b0, b1);
-#pragma unroll
-                for (int pl = 0; pl < NX; ++pl) {
-                    uint32_t r[4];
-                    ldm_t(r, G + ((cw * (DP / 16) + kk) * NX + pl) * 512);
-                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                }
-                mma_pair<NX, NX, NX>(dk1[2 * n], dk1[2 * n + 1], aw, b0, b1);
+                mma_pair<NX, NX, NX>(dk2[2 * n], dk2[2 * n + 1], a, b0, b1);
             }
 #pragma unroll
             for (int jb = 0; jb < 4; ++jb) {
                 if (jb > rb) continue;
                 uint32_t b0[NX][2], b1[NX][2];
-#pragma unroll
-                for (int pl = 0; pl < NX; ++pl) {
-                    uint32_t r[4];
-                    ldm_t(r, W + ((cw * 4 + jb) * NX + pl) * 512);
-                    b0[pl][0] = r[0]; b0[pl][1] = r[1]; b1[pl][0] = r[2]; b1[pl][1] = r[3];
-                }
+                load_b(b0, b1, W + (cw * 4 + jb) * NX * 512);
                 if (hf == 0) {
                     mma_pair<NIN, NX, NX>(D[2 * jb], D[2 * jb + 1], ao, b0, b1);
                 } else {
-                    mma_pair<NX, NX, NX>(D[2 * jb], D[2 * jb + 1], az, b0, b1);
+                    mma_pair<NX, NX, NX>(D[2 * jb], D[2 * jb + 1], a, b0, b1);
                 }
+            }
+            load_a(W);
+#pragma unroll
+            for (int n = 0; n < NB / 2; ++n) {
+                uint32_t b0[NX][2], b1[NX][2];
+                load_b(b0, b1, G + (cw * (DP / 16) + hf * (NB / 2) + n) * NX * 512);
+                mma_pair<NX, NX, NX>(dk1[2 * n], dk1[2 * n + 1], a, b0, b1);
             }
             if (hf == 1 && rb == cw) {
 #pragma unroll

@@ -12,18 +12,13 @@
 // formed for all chunks at once; the walk over the chunks is two products deep.
 //
 // Precision: operands go through the bf16 tensor-core instruction as sums of
-// bf16 planes (a float is hi + lo to 2^-17, hi + mid + lo to 2^-25, relative),
-// products accumulate in float32. Inputs are held exactly (bf16: 1 plane, fp16:
-// 2, fp32: 3); what is computed in between (states, W, Y, scores) is held in
-// NX = 2 planes for 16-bit inputs and 3 for float32, and plane products whose
-// planes' indices sum to NX or more are below that precision and left out.
-// With 16-bit inputs that is 1.3e-4 of an output in bf16 (one rounding in a
-// thousand goes the other way) and 3e-6 to 6e-6 of float32 results. Who needs
-// three planes passes float32 copies of the inputs (exact) and has the outputs
-// in float32 (4e-7), for 2.7 times the time of a training step and 3.1 times
-// that of a prompt (8 x 12 heads of 2047 tokens). Summing the small plane
-// products apart, as for float32, changes nothing with two planes: their
-// rounding is the larger error.
+// bf16 planes (a float is hi + mid + lo to 2^-25, relative), products accumulate
+// in float32. Inputs are held exactly (bf16: 1 plane, fp16: 2, fp32: 3); what is
+// computed in between (states, W, Y, scores) is held in three planes for every
+// type, and plane products whose planes' indices sum to 3 or more are below that
+// precision and left out. (Two planes for 16-bit inputs would take 0.7 of the
+// time, but turn one rounding of a bf16 output in a thousand and leave float32
+// results 3e-6 to 8e-6 off instead of 3e-7 to 6e-7.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -98,10 +93,9 @@ struct alignas(16) DeltaGates {
 };
 static_assert(sizeof(DeltaGates) % 16 == 0 && sizeof(DeltaGates) <= 128 * 16, "one 16-byte piece per loading thread");
 
-template <typename T> struct DeltaType;
-template <> struct DeltaType<__nv_bfloat16> { static constexpr int kIn = 1, kX = 2; };
-template <> struct DeltaType<__half> { static constexpr int kIn = 2, kX = 2; };
-template <> struct DeltaType<float> { static constexpr int kIn = 3, kX = 3; };
+constexpr int kDeltaPlanes = 3;  // of what is computed in between
+template <typename T> constexpr int kDeltaIn = sizeof(T) == 4 ? 3 : 2;  // of inputs
+template <> constexpr int kDeltaIn<__nv_bfloat16> = 1;
 
 namespace dl {
 
@@ -157,12 +151,13 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&r)[NP]) {
 // c[n] += A B[n], plane pair by plane pair over all n: each accumulator is used again only after the others, which
 // hides the instruction's latency (22 cycles against 8 of issue: four accumulators at least).
 // The tensor cores cut a sum off where float32 addition rounds it, so every instruction on an accumulator loses up to
-// 2^-23 of it, always towards zero. With three planes (float32 inputs) the five small products are therefore summed by
-// themselves and added once: outputs are then off by 4.4e-7 (2.6e-6 with one sum), for 5 % of the time of a training step.
+// 2^-23 of it, always towards zero. The small products (planes' indices not both 0) are therefore summed by themselves and
+// added once: outputs of float32 inputs are then off by 4.4e-7 (2.6e-6 with one sum), for 5 % of the time of a training step.
 template <int N, int NA, int NB, int NX>
 __device__ __forceinline__ void mma_set(float (&c)[N][4], const uint32_t (&a)[NA][4], const uint32_t (&b)[N][NB][2]) {
+    constexpr bool kSmall = NA * NB > 1;
     float small[N][4];
-    if constexpr (NX == 3) {
+    if constexpr (kSmall) {
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -174,8 +169,8 @@ __device__ __forceinline__ void mma_set(float (&c)[N][4], const uint32_t (&a)[NA
         for (int j = NB - 1; j >= 0; --j)
             if (i + j < NX)
 #pragma unroll
-                for (int n = 0; n < N; ++n) mma(NX == 3 && i + j > 0 ? small[n] : c[n], a[i], b[n][j][0], b[n][j][1]);
-    if constexpr (NX == 3) {
+                for (int n = 0; n < N; ++n) mma(i + j > 0 ? small[n] : c[n], a[i], b[n][j][0], b[n][j][1]);
+    if constexpr (kSmall) {
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -185,8 +180,9 @@ __device__ __forceinline__ void mma_set(float (&c)[N][4], const uint32_t (&a)[NA
 template <int NA, int NB, int NX>
 __device__ __forceinline__ void mma_pair(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b0)[NB][2],
                                          const uint32_t (&b1)[NB][2]) {
+    constexpr bool kSmall = NA * NB > 1;
     float small[2][4];
-    if constexpr (NX == 3) {
+    if constexpr (kSmall) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) small[0][i] = small[1][i] = 0.f;
     }
@@ -195,10 +191,10 @@ __device__ __forceinline__ void mma_pair(float (&c0)[4], float (&c1)[4], const u
 #pragma unroll
         for (int j = NB - 1; j >= 0; --j)
             if (i + j < NX) {
-                mma(NX == 3 && i + j > 0 ? small[0] : c0, a[i], b0[j][0], b0[j][1]);
-                mma(NX == 3 && i + j > 0 ? small[1] : c1, a[i], b1[j][0], b1[j][1]);
+                mma(i + j > 0 ? small[0] : c0, a[i], b0[j][0], b0[j][1]);
+                mma(i + j > 0 ? small[1] : c1, a[i], b1[j][0], b1[j][1]);
             }
-    if constexpr (NX == 3) {
+    if constexpr (kSmall) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             c0[i] += small[0][i];

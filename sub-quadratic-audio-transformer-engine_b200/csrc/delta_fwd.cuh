@@ -15,9 +15,9 @@
 // and were slower.)
 //
 // Measured, bf16, d = e = 64, 8 x 8 heads of 8192 tokens (8192 chunks): gates and Y
-// 100 us (issue-bound: 46 % of the issue slots with 24 warps per SM, tensor pipe 17 %);
-// the walk 1.7 us a chunk, 2.0 us where the backward's planes are written (254 us:
-// shared memory 76 % busy on the SMs at work, tensor pipe 35 %).
+// 128 us (issue-bound: 54 % of the issue slots with 20 warps per SM, tensor pipe 22 %);
+// the walk 2.4 us a chunk, 2.7 us where the backward's planes are written (351 us:
+// shared memory 70 % busy on the SMs at work, tensor pipe 43 %).
 #pragma once
 
 #include "delta_common.cuh"
@@ -33,13 +33,13 @@ using namespace dl;
 // ------------------------------------------------------------------ gates, Y and scores per chunk
 template <typename T, int DP>
 struct PrepSmem {
-    static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
+    static constexpr int kIn = kDeltaIn<T>, kX = kDeltaPlanes;
     Gates s;
     alignas(16) float A[kYBlocks][16][20];        // its lower triangle's blocks
     alignas(128) unsigned char Ab[6 * kX * 512];  // -A_IK beta, blocks I > K: [block][plane]
     alignas(128) unsigned char k[kIn * 64 * DP * 2];
     alignas(128) unsigned char q[kIn * 64 * DP * 2];
-    // where (I + A_II beta)^-1 goes: over the 16 rows of q that warp I alone reads, once it has. (Six CTAs per SM then
+    // where (I + A_II beta)^-1 goes: over the 16 rows of q that warp I alone reads, once it has. (Five CTAs per SM then
     // have room for bf16 at d = 64.)
     static __host__ __device__ constexpr int ti(int I) { return (3 - I) * 16 * DP * 2; }
     static_assert(kX * 512 <= 16 * DP * 2, "T in q's rows");
@@ -51,7 +51,7 @@ struct PrepSmem {
 // transposed so that each result is, in its registers, the A operand of the next product.
 template <typename T, int DP>
 __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, kTile = 64 * DP * 2;
+    constexpr int NIN = kDeltaIn<T>, NX = kDeltaPlanes, kTile = 64 * DP * 2;
     extern __shared__ __align__(128) unsigned char raw[];
     PrepSmem<T, DP>& sm = *reinterpret_cast<PrepSmem<T, DP>*>(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -200,11 +200,12 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(const DeltaParams p) {
 // STATES: a walk for the states alone, without outputs and their operands.
 template <typename T, int DP, bool STATES>
 struct ChainSmem {
-    static constexpr int kIn = DeltaType<T>::kIn, kX = DeltaType<T>::kX;
-    // chunks in shared memory: the one at work and the next; where they fit, one more on its way, and the last one for
-    // the output warps, which then finish a chunk while the chain is at the next
-    static constexpr int kStages = kIn == 1 ? (DP == 64 ? (STATES ? 3 : 4) : 2) : DP == 64 ? 2 : 1;
-    static constexpr bool kLag = kStages == 4;
+    static constexpr int kIn = kDeltaIn<T>, kX = kDeltaPlanes;
+    // chunks in shared memory: the one at work and the next; where it fits, the last one for the output warps, which then
+    // finish a chunk while the chain is at the next (8 x 8 heads of 8192 tokens, bf16: 496 us with the gates' kernel and the
+    // planes kept, 535 us with a chunk more on its way in that place); where only one fits, it waits for its turn
+    static constexpr int kStages = kIn == 1 ? (DP == 64 && !STATES ? 3 : 2) : DP == 64 ? 2 : 1;
+    static constexpr bool kLag = kStages == 3;
     struct Stage {
         alignas(128) unsigned char k[kIn * 64 * DP * 2];
         alignas(128) unsigned char q[STATES ? 16 : kIn * 64 * DP * 2];
@@ -219,13 +220,14 @@ struct ChainSmem {
     alignas(16) unsigned char S0[2][DP / 16][kX * 512];  // S^T before the chunk, planes
     alignas(16) unsigned char R[2][4][kX * 512];         // -(beta R)^T, planes
     // W^T for the update and the outputs. 16-bit inputs: planes of beta W and of e^{g_C - g} beta W (and of W where
-    // it is kept), converted once by the warp that has it; float32 ones (no room): W, converted by each reader
-    static constexpr bool kShared = kX == 2;
-    alignas(16) unsigned char Wb[kLag ? 2 : 1][2][kShared && !STATES ? 4 : 1][kX * 512];  // (by chunk parity where outputs lag)
+    // it is kept), converted once by the warp that has it. float32 inputs (no room), and the states' pass (two CTAs
+    // share an SM without): W, converted by each reader
+    static constexpr bool kShared = kIn < 3 && !STATES;
+    alignas(16) unsigned char Wb[kLag ? 2 : 1][2][kShared ? 4 : 1][kX * 512];  // (by chunk parity where outputs lag)
     alignas(16) unsigned char Wk[2][kShared ? 4 : 1][kX * 512];
     union {
         float4 W[2][kShared ? 1 : 8 * 32];
-        unsigned char Wp[2][STATES ? 1 : 4][1024];
+        unsigned char Wp[2][STATES ? 1 : 4][kX * 512];
     } w;
     // outputs on their way to memory: in the place of Y, which nobody reads any more by then
     static constexpr int kOutPitch = 16 * sizeof(T) + 16;
@@ -235,7 +237,7 @@ struct ChainSmem {
 // One warp of a chain pair: half `A` of d of S^T in its accumulators; R and W of its token blocks.
 template <typename T, int DP, bool OUT, bool KEEP>
 __device__ __forceinline__ void chain_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP, !OUT && !KEEP>::kStages;
+    constexpr int NIN = kDeltaIn<T>, NX = kDeltaPlanes, NST = ChainSmem<T, DP, !OUT && !KEEP>::kStages;
     constexpr int NH = DP / 16;  // 8-column blocks of half of d
     constexpr bool kShared = ChainSmem<T, DP, !OUT && !KEEP>::kShared;
     const int g = lane >> 2, t = lane & 3;
@@ -381,7 +383,7 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, 
 // One warp of an output pair: the outputs of 16 columns for its token blocks, and its share of the planes.
 template <typename T, int DP, bool OUT, bool KEEP>
 __device__ __forceinline__ void output_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, const DeltaParams& p, const WalkJob& job, int A, int pair, int lane) {
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX, NST = ChainSmem<T, DP, !OUT && !KEEP>::kStages;
+    constexpr int NIN = kDeltaIn<T>, NX = kDeltaPlanes, NST = ChainSmem<T, DP, !OUT && !KEEP>::kStages;
     const int g = lane >> 2, t = lane & 3;
     const Own own(A);
     const float2 one = make_float2(1.f, 1.f);
@@ -510,7 +512,7 @@ template <typename T, int DP, bool OUT, bool KEEP>
 __global__ void __launch_bounds__(ChainSmem<T, DP, !OUT && !KEEP>::kThreads, chain_ctas<T, DP, !OUT && !KEEP>())
 delta_chain_kernel(const DeltaParams p) {
     constexpr bool kStates = !OUT && !KEEP;
-    constexpr int NIN = DeltaType<T>::kIn, NX = DeltaType<T>::kX;
+    constexpr int NIN = kDeltaIn<T>, NX = kDeltaPlanes;
     constexpr int NST = ChainSmem<T, DP, kStates>::kStages;
     extern __shared__ __align__(128) unsigned char raw[];
     using Smem = ChainSmem<T, DP, kStates>;
@@ -565,9 +567,8 @@ delta_chain_kernel(const DeltaParams p) {
         bool async = false;
         if constexpr (NIN == 1) async = p.k.vec && p.q.vec && p.v.vec && p.d % 8 == 0 && p.e % 8 == 0;
         if (async) {
-            // bf16: asynchronous copies, chunk c + kAhead started while c is computed (8 x 12 heads of 2047 tokens: 169 us
-            // with the gates' kernel and rows on 16 bytes, 341 us through registers, element by element, without)
-            constexpr int kAhead = Smem::kLag ? NST - 2 : NST > 1 ? NST - 1 : 1;
+            // bf16: asynchronous copies, chunk c + 1's while c is computed (8 x 12 heads of 2047 tokens: 229 us with the
+            // gates' kernel and rows on 16 bytes, 367 us through registers, element by element, without)
             int any_next = gates[begin].any;
             auto start = [&](int c) {
                 if (c < end) {
@@ -586,10 +587,9 @@ delta_chain_kernel(const DeltaParams p) {
                         }
                     }
                 }
-                async_commit();
             };
-            auto finish = [&](int c) {  // every copy up to chunk c's is there
-                async_wait_but<(kAhead > 1 ? kAhead - 1 : 0)>();
+            auto finish = [&](int c) {
+                async_wait();
                 if (c >= end) return;
                 bar_sync(3, 128);
                 auto& st = sm.st[c % NST];
@@ -599,15 +599,14 @@ delta_chain_kernel(const DeltaParams p) {
                     clear_dead<kDeltaCols, 128>(st.v, st.s.live, lt);
                 }
             };
-            for (int c = 0; c < kAhead; ++c) start(begin + c);
+            start(begin);
             finish(begin);
             __syncthreads();
             for (int c = begin; c < end; ++c) {
-                start(c + kAhead);
+                start(c + 1);
                 finish(c + 1);
                 __syncthreads();
             }
-            async_wait();
         } else {
             if constexpr (NST == 1) {  // (no room for a second chunk: each tile is loaded when its turn comes)
                 __syncthreads();

@@ -430,9 +430,8 @@ class DeltaHandover:
     one instance as ``handover=`` to the forward, which fills it, and then to
     ``gated_delta_backward``, which otherwise forms them again. The backward
     refuses a carrier from a call of another shape, type or device; one from a
-    call of the same shape but other inputs gives wrong gradients. It holds 54 KB
-    per 64 tokens and head at d = e = 64 in 16 bits (80 KB in float32), more than
-    q, k and v themselves; a backward without it forms it again in its workspace,
+    call of the same shape but other inputs gives wrong gradients. It holds 80 KB
+    per 64 tokens and head at d = e = 64, more than q, k and v themselves; a backward without it forms it again in its workspace,
     which lives for the call only."""
 
     def __init__(self) -> None:
@@ -546,9 +545,9 @@ def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta:
     [B, H, N], used in float32. ``mask`` [B, N]: a masked token leaves the state
     as it is, its output is 0 and nothing of it is read. ``scale`` defaults to
     d ** -0.5. For bounded states keys should have at most unit length.
-    With 16-bit inputs the operands inside carry 16 bits of mantissa (float32
-    results are off by about 5e-6 of their norm); float32 copies of them carry 24.
-    ``out`` shares no memory with the inputs.
+    Operands inside carry 24 bits of mantissa whatever the inputs' type (float32
+    results are off by less than 1e-6 of their norm). ``out`` shares no memory with
+    the inputs.
     Paths: "exact" is the token-recurrent kernel (d <= 256; the automatic choice
     for up to 16 tokens), "chunked" the chunk kernels (d <= 128).
     """

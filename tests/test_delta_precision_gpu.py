@@ -1,0 +1,32 @@
+"""The gated delta rule's float32 results with 16-bit inputs are as exact as with float32 ones: operands in between are held
+in three bf16 planes whatever the inputs' type. The tolerance is test_delta_gpu.py's for float32 inputs, 2e-6 in the 2-norm
+(planes to 2^-24, float32 sums of up to 64 products, a factor of 4 for how the recurrence passes errors on)."""
+import pytest
+import torch
+
+import delta_chunk_reference as ref
+from subq_audio import ops
+from test_delta_gpu import inputs, poison, rel
+
+pytestmark = pytest.mark.gpu
+
+CASES = [(2, 4, 4, 2, 2, 700, 64, 64, "bf16", "bnhd", "tail"), (8, 12, 12, 12, 12, 400, 64, 64, "bf16", "bnhd", None),
+         (1, 2, 2, 2, 2, 4096, 64, 64, "bf16", "bhnd", "random"), (2, 4, 4, 1, 4, 500, 128, 128, "bf16", "bnhd", "tail"),
+         (2, 3, 3, 3, 3, 300, 80, 48, "bf16", "odd", "random"), (1, 2, 1, 2, 2, 333, 32, 32, "bf16", "bnhd", None),
+         (2, 4, 2, 4, 2, 300, 64, 128, "fp16", "bnhd", "tail"), (1, 4, 4, 4, 4, 4096, 64, 64, "fp16", "bnhd", None),
+         (2, 2, 2, 2, 2, 250, 128, 64, "fp16", "bnhd", "random"), (1, 3, 3, 3, 3, 178, 32, 32, "fp16", "bnhd", None)]
+
+
+@pytest.mark.parametrize("case", CASES, ids=["-".join(str(x) for x in c) for c in CASES])
+def test_float32_results_of_16_bit_inputs(case):
+    B, H, Hq, Hk, Hv, N, d, e, dtype, layout, mask = case
+    q, k, v, do, beta, lg, S0, dS, m = inputs(B, H, Hq, Hk, Hv, N, d, e, dtype, seed=N + e, layout=layout, mask=mask)
+    scale = d ** -0.5
+    o_ref, S_ref = ref.forward(q, k, v, beta, lg, m, scale, S0)
+    want = ref.gradients(q, k, v, beta, lg, m, scale, S0, do, dS)
+    q, k, v, do, beta, lg = (poison(x, m) for x in (q, k, v, do, beta, lg))
+    _, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, mask=m, state=S0, return_state=True, path="chunked")
+    assert rel(S, S_ref) < 2e-6
+    got = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, mask=m, state=S0, dstate=dS, need_dlog_gamma=True, need_dstate=True)
+    for name, a, w in list(zip(("dq", "dk", "dv", "dbeta", "dlog_gamma", "dstate"), got, want))[3:]:
+        assert rel(a, w) < 2e-6, name

@@ -23,7 +23,7 @@ def test_segments_hand_the_state_on(case):
     ho = ops.DeltaHandover()
     o, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=gate, mask=m, state=S0, return_state=True, handover=ho)
     assert ops.last_launches() == 4  # gates, segments, join, walk
-    assert rel(S, S_ref) < tol(S, dtype, d) and rel(o, o_ref) < tol(o, dtype, d)
+    assert rel(S, S_ref) < tol(S, d) and rel(o, o_ref) < tol(o, d)
     state, out = S0.clone(), torch.empty_like(o)  # the state updated in place
     ops.GatedDeltaStep(q, k, v, beta, out, state, log_gamma=gate, mask=m).step()
     assert torch.equal(state, S) and torch.equal(out, o)
@@ -31,4 +31,4 @@ def test_segments_hand_the_state_on(case):
                                    need_dstate=True, handover=ho)
     assert ops.last_launches() == 4 + 1  # and dk summed over its group
     for name, a, w in zip(NAMES, got, ref.gradients(q, k, v, beta, lg, m, scale, S0, do, dS)):
-        assert rel(a, w) < tol(a, dtype, d), name
+        assert rel(a, w) < tol(a, d), name
