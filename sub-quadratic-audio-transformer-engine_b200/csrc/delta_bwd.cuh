@@ -14,12 +14,14 @@
 //   dlog gamma_t = sum over i >= t > j of E_ij + sum over i >= t of a_i + sum over j < t of b_j + e^{g_C} <G, S0>,
 //   E_ij = D1_ij q_i.k_j + D2_ij k_i.k_j,   a_i = scale e^{g_i} q_i.(S0 dO_i) - e^{g_i} beta_i k_i.(S0 Z_i),
 //   b_j = e^{g_C - g_j} beta_j k_j.(G W_j).
-// From the end of the chunk backwards that is a running sum that row t of E and
-// a_t enter and column t of E and b_t leave, the very same numbers: what they are
-// off by leaves with them, and what is left is the error of the terms that count
-// for t. (The shorter running sum of q_i.dq_i - v_i.dv_i is the same in exact
-// arithmetic, but keeps the errors of tokens that have nothing to do with t: six
-// times as far off with fast decay.)
+// From the end of the chunk backwards the first two are a running sum that row t of E
+// and a_t enter and column t of E leaves, the very same numbers: what they are off by
+// leaves with them, and what is left is the error of the terms that count for t. The
+// third is a running sum from the begin of the chunk: all of b less those from t on
+// would keep what b_j of late tokens, which may be large, are off by. (The shorter
+// running sum of q_i.dq_i - v_i.dv_i is the same in exact arithmetic, but keeps the
+// errors of tokens that have nothing to do with t: six times as far off with fast
+// decay.)
 //
 // Measured, bf16, d = e = 64, 8 x 8 heads of 8192 tokens (8192 chunks): the walk back
 // 396 us (3.1 us a chunk, bound like the forward's by shared memory, 60 % busy, and
@@ -866,7 +868,7 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
     store_grad<T, NB>(dk1, p.dk, tensor_base(p.dk, b, h), p.dk32, at32 * p.d, n0 + 16 * rb, n0 + rows, 8 * hf * NB, p.d, lane);
     __syncthreads();
     if (warp == 0) {
-        // two tokens per lane, from the end of the chunk backwards
+        // two tokens per lane: a_i and E from the end of the chunk backwards, b_j from its begin
         const int i0 = 2 * lane, i1 = i0 + 1, first = lane >> 3;
         float x[2], out[2];
 #pragma unroll
@@ -877,26 +879,28 @@ __global__ void __launch_bounds__(256, GradSmem<T, DP>::kCtas) delta_grad_kernel
             for (int k = 0; k < 4; ++k)
                 if (k >= first) col += sm.col[0][k][n] + sm.col[1][k][n];
             out[i] = sm.out[0][n] + sm.out[1][n];
-            x[i] = (sm.in[0][n] + sm.in[1][n]) + (sm.row[0][n] + sm.row[1][n]) - col - out[i];
+            x[i] = (sm.in[0][n] + sm.in[1][n]) + (sm.row[0][n] + sm.row[1][n]) - col;
         }
-        float end = out[0] + out[1];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) end += __shfl_xor_sync(0xffffffffu, end, o);
-        end = fmaf(s.eC, sm.gs[0] + sm.gs[1], end);
-        float run = x[0] + x[1];  // over this lane's tokens and the later lanes'
+        float run = x[0] + x[1], past = out[0] + out[1];  // over this lane's tokens and the later (earlier) lanes'
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const float down = __shfl_down_sync(0xffffffffu, run, o);
+            const float down = __shfl_down_sync(0xffffffffu, run, o), up = __shfl_up_sync(0xffffffffu, past, o);
             if (lane + o < 32) run += down;
+            if (lane >= o) past += up;
         }
+        float later = __shfl_down_sync(0xffffffffu, run, 1), before = __shfl_up_sync(0xffffffffu, past, 1);
+        if (lane == 31) later = 0.f;
+        if (lane == 0) before = 0.f;
+        const float all = s.eC * (sm.gs[0] + sm.gs[1]);
+        const float g1 = (x[1] + later) + (before + out[0]) + all, g0 = (x[0] + (x[1] + later)) + before + all;
         const int64_t at = at32 + n0;
         if (i0 < rows) {
             p.dbeta[at + i0] = s.live[i0] ? sm.wz[i0] : 0.f;
-            if (p.dlg) p.dlg[at + i0] = s.live[i0] ? run + end : 0.f;
+            if (p.dlg) p.dlg[at + i0] = s.live[i0] ? g0 : 0.f;
         }
         if (i1 < rows) {
             p.dbeta[at + i1] = s.live[i1] ? sm.wz[i1] : 0.f;
-            if (p.dlg) p.dlg[at + i1] = s.live[i1] ? run - x[0] + end : 0.f;
+            if (p.dlg) p.dlg[at + i1] = s.live[i1] ? g1 : 0.f;
         }
     }
 }

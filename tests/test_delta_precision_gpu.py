@@ -30,3 +30,14 @@ def test_float32_results_of_16_bit_inputs(case):
     got = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, mask=m, state=S0, dstate=dS, need_dlog_gamma=True, need_dstate=True)
     for name, a, w in list(zip(("dq", "dk", "dv", "dbeta", "dlog_gamma", "dstate"), got, want))[3:]:
         assert rel(a, w) < 2e-6, name
+
+
+@pytest.mark.parametrize("dtype,d,e,N", [("fp16", 64, 1, 30), ("bf16", 64, 64, 700), ("fp32", 64, 64, 200), ("fp32", 128, 33, 64)])
+def test_log_gamma_gradient_where_the_last_token_forgets_all(dtype, d, e, N):
+    """What the last token writes is all that the final state has, and a large gradient of that state has nothing to do with
+    any log gamma. The other terms of a token's gradient are at most 64 of the gradients' own size: 2e-6 as above."""
+    q, k, v, do, beta, lg, S0, dS, _ = inputs(1, 3, 3, 1, 3, N, d, e, dtype, seed=N + e)
+    lg[:, :, -1] = -30.0
+    want = ref.gradients(q, k, v, beta, lg, None, 1.0, S0, 0.1 * do, 10 * dS)
+    got = ops.gated_delta_backward(q, k, v, beta, 0.1 * do, log_gamma=lg, scale=1.0, state=S0, dstate=10 * dS, need_dlog_gamma=True)
+    assert rel(got[4], want[4]) < 2e-6
