@@ -41,3 +41,17 @@ def test_log_gamma_gradient_where_the_last_token_forgets_all(dtype, d, e, N):
     want = ref.gradients(q, k, v, beta, lg, None, 1.0, S0, 0.1 * do, 10 * dS)
     got = ops.gated_delta_backward(q, k, v, beta, 0.1 * do, log_gamma=lg, scale=1.0, state=S0, dstate=10 * dS, need_dlog_gamma=True)
     assert rel(got[4], want[4]) < 2e-6
+
+
+@pytest.mark.parametrize("d,e,N,lowest", [(64, 64, 4096, -1e-4), (256, 64, 4096, -1e-3), (33, 40, 3000, -1e-3)])
+def test_token_steps_with_slow_decay(d, e, N, lowest):
+    """The token-recurrent kernel over thousands of tokens that hardly decay, with little written: gamma is near 1, and a
+    rounding of it to float32 (2^-25) would be the same at every token, N 2^-25 in all (1.2e-4). Each token's own
+    roundings of the state (2^-24 of it, two) do not add up: sqrt(N) 2^-24 in the mean square, 4e-6 for 4096 tokens, with
+    a margin of 2 for what beta passes on."""
+    q, k, v, do, beta, _, S0, dS, _ = inputs(1, 2, 2, 2, 2, N, d, e, "fp32", seed=d)
+    lg, beta = torch.full_like(beta, lowest), 0.01 * beta
+    lg[:, 1] *= 0.7
+    _, S_ref = ref.forward(q, k, v, beta, lg, None, 1.0, S0)
+    _, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, scale=1.0, state=S0, return_state=True, path="exact")
+    assert rel(S, S_ref) < 2 * N ** 0.5 * 2.0 ** -24
