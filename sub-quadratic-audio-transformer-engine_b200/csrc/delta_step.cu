@@ -65,9 +65,12 @@ __global__ void __launch_bounds__(32 * NW) delta_step_kernel(const DeltaParams p
                 continue;
             }
             float kr[RPL], sums[9] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            // gamma - 1, and S + (gamma - 1) S below: a gamma near 1 that is rounded by itself is off by 2^-25 the same way
-            // at every token (4096 tokens at log gamma = -1e-4: the state 1.2e-4 off)
-            const float decay = p.lg.p ? expm1f(p.lg.p[b * p.lg.sb + h * p.lg.sh + n * p.lg.sn]) : 0.f, gamma = 1.f + decay;
+            // The state's decay: gamma S, or S + (gamma - 1) S where gamma is near 1 (the series' rest is below 2^-26 of
+            // S). Rounded by itself a gamma near 1 is off by up to 2^-25, the same way at every token (4096 tokens at
+            // log gamma = -1e-4: the state 1.2e-4 off); and gamma - 1 has few bits of a small gamma.
+            const float lg = p.lg.p ? p.lg.p[b * p.lg.sb + h * p.lg.sh + n * p.lg.sn] : 0.f, gamma = expf(lg);
+            const bool near1 = fabsf(lg) < 0.0625f;
+            const float decay = near1 ? lg * fmaf(lg, fmaf(lg, fmaf(lg, 1.f / 24.f, 1.f / 6.f), 0.5f), 1.f) : gamma;
             const float beta = p.beta.p ? p.beta.p[b * p.beta.sb + h * p.beta.sh + n * p.beta.sn] : 1.f;
             float vv[4];
 #pragma unroll
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(32 * NW) delta_step_kernel(const DeltaParams p
 #pragma unroll
             for (int i = 0; i < RPL; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) S[i][j] = fmaf(kr[i], u[j], fmaf(decay, S[i][j], S[i][j]));
+                for (int j = 0; j < 4; ++j) S[i][j] = fmaf(kr[i], u[j], fmaf(decay, S[i][j], near1 ? S[i][j] : 0.f));
             if (tid < 8)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)

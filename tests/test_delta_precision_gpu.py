@@ -55,3 +55,17 @@ def test_token_steps_with_slow_decay(d, e, N, lowest):
     _, S_ref = ref.forward(q, k, v, beta, lg, None, 1.0, S0)
     _, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, scale=1.0, state=S0, return_state=True, path="exact")
     assert rel(S, S_ref) < 2 * N ** 0.5 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("d", [64, 100, 200])
+@pytest.mark.parametrize("lowest", [1.0, -0.05, -0.07, -0.6, -6.0])
+def test_a_state_that_nothing_is_written_to(d, lowest):
+    """beta 0: the state is the product of the decays, each within 2^-23 of itself (an exponential and a product), however
+    little is left of it."""
+    N = 12
+    q, k, v, _, beta, _, S0, _, _ = inputs(1, 2, 2, 2, 2, N, d, 40, "fp32", seed=d)
+    lg = torch.full_like(beta, lowest)
+    want = S0.double() * torch.exp(lg.double().sum(-1))[..., None, None]
+    for path in ("exact", "chunked") if d <= 128 else ("exact",):
+        _, S = ops.gated_delta_forward(q, k, v, 0.0, log_gamma=lg, state=S0, return_state=True, path=path)
+        assert float(((S.double() - want) / want).abs().max()) < 2 * N * 2.0 ** -23, path
