@@ -186,7 +186,7 @@ __device__ __forceinline__ void rev_chain_warp(RevSmem<T, DP>& sm, const WalkJob
                 }
                 mma_cols<NH, DP, NX, NIN, NX>(U, a, kt, 16 * jb, A * NH, lane);
             }
-            next_state<NH>(S, s.eC, U);
+            next_state<NH>(S, s, U);
             put_state();
         }
         __syncthreads();

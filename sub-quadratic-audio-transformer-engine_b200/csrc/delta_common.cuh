@@ -88,7 +88,7 @@ struct alignas(16) DeltaGates {
     float eg[kDeltaC];               // e^g
     float kd[kDeltaC];               // e^{g_C - g}
     int live[kDeltaC];
-    float eC;                        // e^{g_C}
+    float eC, dC;                    // e^{g_C}, e^{g_C} - 1
     int any, full;                   // a live token in the chunk; all 64 live
 };
 static_assert(sizeof(DeltaGates) % 16 == 0 && sizeof(DeltaGates) <= 128 * 16, "one 16-byte piece per loading thread");
@@ -325,6 +325,7 @@ __device__ __forceinline__ void form_gates(Gates& s, const DeltaParams& p, int b
     }
     if (lane == 0) {
         s.eC = expf((float)total);
+        s.dC = expm1f((float)total);
         s.any = any;
         s.full = full;
     }
@@ -560,14 +561,23 @@ __device__ __forceinline__ void zero_acc(float (&c)[NB][4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
 }
-// The state after a chunk: f S + the chunk's part U. (Products added to S itself would each cut it off towards zero: 256
-// chunks without decay were 8e-5 off in float32, 5e-5 in bf16.)
+// The state after a chunk: e^{g_C} S + the chunk's part U. (Products added to S itself would each cut it off towards zero:
+// 256 chunks without decay were 8e-5 off in float32, 5e-5 in bf16. An e^{g_C} near 1 that is rounded by itself is off by
+// up to 2^-25, the same way at every chunk of a constant decay: 256 chunks 7.6e-6.)
 template <int NB>
-__device__ __forceinline__ void next_state(float (&S)[NB][4], float f, const float (&U)[NB][4]) {
+__device__ __forceinline__ void next_state(float (&S)[NB][4], const Gates& s, const float (&U)[NB][4]) {
+    const float eC = s.eC, dC = s.dC;
+    if (fabsf(dC) < 0.0625f) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S[n][i] = fmaf(f, S[n][i], U[n][i]);
+            for (int i = 0; i < 4; ++i) S[n][i] += fmaf(dC, S[n][i], U[n][i]);
+    } else {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[n][i] = fmaf(eC, S[n][i], U[n][i]);
+    }
 }
 __device__ __forceinline__ void add_acc(float (&c)[4], float4 x) {
     c[0] += x.x; c[1] += x.y; c[2] += x.z; c[3] += x.w;

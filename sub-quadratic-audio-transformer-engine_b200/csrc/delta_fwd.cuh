@@ -364,7 +364,7 @@ __device__ __forceinline__ void chain_warp(ChainSmem<T, DP, !OUT && !KEEP>& sm, 
                 }
                 mma_cols<NH, DP, NX, NIN, NX>(U, a, kt, 16 * jb, A * NH, lane);
             }
-            next_state<NH>(S, s.eC, U);
+            next_state<NH>(S, s, U);
             put_state();
         }
         __syncthreads();

@@ -58,3 +58,18 @@ def test_a_state_that_lasts_keeps_its_bits(B, H, N, d, e, dtype):
     got = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, state=S0, dstate=dS, need_dlog_gamma=True, need_dstate=True, handover=ho)
     for name, a, w in zip(NAMES, got, ref.gradients(q, k, v, beta, lg, None, d ** -0.5, S0, do, dS)):
         assert rel(a, w) < tol(a, d), name
+
+
+@pytest.mark.parametrize("lowest", [-9.02e-5, -6.6e-5, -3.88e-5])
+@pytest.mark.parametrize("B,H,N,d,e,dtype", [(1, 2, 16384, 64, 64, "fp32"), (1, 76, 16384, 64, 32, "bf16")])
+def test_a_slow_decay_keeps_its_bits(B, H, N, d, e, dtype, lowest):
+    """The same decay at every token: what a chunk leaves of the state is near 1, and a rounding of it must not be the same
+    one 256 times over (2^-25 at the worst, as at these)."""
+    q, k, v, do, beta, S0, dS = inputs(B, H, 1, N, d, e, dtype, N + d, 0.0005, 0.001)
+    lg = torch.full_like(beta, lowest)
+    _, S_ref = ref.forward(q, k, v, beta, lg, None, d ** -0.5, S0)
+    _, S = ops.gated_delta_forward(q, k, v, beta, log_gamma=lg, state=S0, return_state=True)
+    assert rel(S, S_ref) < 3e-6  # 256 roundings that do not add up, 16 x 2^-24, and 2e-6 as in test_delta_gpu.py
+    got = ops.gated_delta_backward(q, k, v, beta, do, log_gamma=lg, state=S0, dstate=dS, need_dstate=True)
+    want = ref.gradients(q, k, v, beta, lg, None, d ** -0.5, S0, do, dS)
+    assert rel(got[5], want[5]) < 3e-6
