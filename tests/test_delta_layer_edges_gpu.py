@@ -61,3 +61,28 @@ def test_what_layer_norm_does_not_differentiate_raises():
         torch.func.jvp(norm, (x.detach(),), (torch.ones_like(x),))
     with pytest.raises(RuntimeError, match="once_differentiable"):
         torch.autograd.grad(norm(x).square().sum(), x, create_graph=True)[0].sum().backward()
+
+
+def test_checkpointed_layer_and_inference_mode():
+    """Under torch.utils.checkpoint the forward's handover is not kept until the backward; the gradients are the same."""
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(6)
+    m = Block().cuda()
+    x = torch.randn(4, 2048, 256, device="cuda", requires_grad=True)
+    params = [x, *m.parameters()]
+
+    def run(call):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y = call(x)
+        held = torch.cuda.memory_allocated() - before
+        return held, torch.autograd.grad(y.square().mean(), params)
+
+    whole, want = run(lambda t: m(t)[0])
+    less, got = run(lambda t: checkpoint(lambda u: m(u)[0], t, use_reentrant=False))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    handover = 4 * 4 * (2048 // 64) * 79 * 1024  # of 4 x 4 heads of 32 chunks
+    assert whole > handover and less < whole - handover
+    with torch.inference_mode():
+        assert torch.equal(m(x)[0], m(x.detach())[0])
