@@ -20,6 +20,9 @@
  *   subq_delta_fwd / _bwd, subq_layer_norm_fwd / _bwd:
  *                       no counterpart: the gated delta rule beside the scan,
  *                       and the norm before a layer
+ *   subq_selective_scan_fwd / _bwd, subq_causal_conv_fwd / _bwd, subq_rms_norm_fwd /
+ *   _bwd, subq_scaled_matmul:
+ *                       no counterpart: a selective state space block's operators
  *   subq_*_workspace_bytes, subq_last_error, subq_abi_version, subq_device_info:
  *                       no single counterpart; they carry the reference's
  *                       scratch allocation (attention_backward.cpp:305-361 allocated
@@ -326,6 +329,165 @@ typedef struct subq_layer_norm_args {
 int subq_layer_norm_fwd(const subq_layer_norm_args* args);
 int subq_layer_norm_bwd(const subq_layer_norm_args* args);
 size_t subq_layer_norm_bwd_workspace_bytes(const subq_layer_norm_args* args);
+
+/* Selective scan (no counterpart in the reference): per channel d of D and state
+ * n of N, float32 states,
+ *   dt_t = softplus(raw_t + dt_bias_d)            (softplus = 0: raw_t + dt_bias_d)
+ *   h_t[n] = exp(dt_t A[d, n]) h_{t-1}[n] + dt_t u_t B_t[n]
+ *   out_t = (sum_n C_t[n] h_t[n] + D_d u_t) silu(z_t)   (no z: without the last factor)
+ * u, dt (raw), z and out are [B, L, D] views, B and C [B, L, G, N] views that the
+ * D / G channels of a group share, all of one type (fp32, fp16, bf16) with
+ * element strides and a contiguous innermost dimension. A masked token leaves h as
+ * it is, its out and gradients are 0, and nothing of it is read. N <= 128.
+ *
+ * The forward can leave the states before every eighth token (handover) for the
+ * backward of the same call, which forms them again without: 4 bytes x the states
+ * rounded up to 16, 32, 64 or 128, for each channel and 8 tokens (8 bytes a token
+ * and channel at N <= 16). */
+typedef struct subq_tensor3 {
+    void* data;
+    int64_t stride_b, stride_l, stride_g; /* element strides; stride_g: B, C and their gradients only */
+} subq_tensor3;
+
+typedef struct subq_selective_desc {
+    int64_t batch, seq_len, channels, states, groups;
+    int32_t dtype;
+    int32_t softplus;
+    const float* A;         /* [channels, states]                              */
+    const float* D;         /* [channels], or NULL (0)                         */
+    const float* dt_bias;   /* [channels], or NULL (0)                         */
+    const uint8_t* mask;    /* as in subq_scan_desc                            */
+    int64_t mask_stride_b;
+} subq_selective_desc;
+
+typedef struct subq_selective_fwd_args {
+    subq_selective_desc desc;
+    subq_tensor3 u, dt, z, B, C;  /* z.data NULL: no gate                      */
+    subq_tensor3 out;             /* shares no memory with an input             */
+    const float* state_in;        /* [B, channels, states], NULL = zeros        */
+    float* state_out;             /* may equal state_in, NULL = not wanted      */
+    void* handover;               /* NULL, or subq_selective_scan_handover_bytes
+                                     (256-byte aligned)                         */
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} subq_selective_fwd_args;
+
+typedef struct subq_selective_bwd_args {
+    subq_selective_desc desc;
+    subq_tensor3 u, dt, z, B, C, dout;
+    subq_tensor3 du, ddt, dz, dB, dC; /* like u, dt, z, B, C; no output shares memory
+                                         with an input or another output        */
+    const float* state_in;
+    const float* dstate_out;      /* gradient of the final state, NULL = zeros  */
+    float* dstate_in;             /* or NULL; may equal dstate_out              */
+    float* dA;                    /* [channels, states]                         */
+    float* dD;                    /* [channels], or NULL                        */
+    float* ddt_bias;              /* [channels], or NULL                        */
+    const void* handover;         /* what the forward of the same call left, or NULL */
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} subq_selective_bwd_args;
+
+int subq_selective_scan_fwd(const subq_selective_fwd_args* args);
+int subq_selective_scan_bwd(const subq_selective_bwd_args* args);
+size_t subq_selective_scan_fwd_workspace_bytes(const subq_selective_fwd_args* args);
+size_t subq_selective_scan_bwd_workspace_bytes(const subq_selective_bwd_args* args);
+size_t subq_selective_scan_handover_bytes(const subq_selective_desc* desc);
+
+/* Short causal convolution over [B, L, D], one filter of width 2, 3 or 4 a channel:
+ *   pre_t = bias + sum_j weight[d, j] x_{t-width+1+j},   y_t = silu(pre_t) or pre_t.
+ * Before the first token stand the width - 1 inputs of state_in (zeros without);
+ * a masked token's input counts as 0, its y and dx are 0 and nothing of it is read;
+ * state_out receives the width - 1 inputs up to the last live token (those of
+ * state_in among them where there are fewer; state_in itself without a live
+ * token). Sums in float32; weights and their gradients float32, written (not
+ * accumulated) and bitwise reproducible. */
+typedef struct subq_causal_conv_args {
+    int64_t batch, seq_len, channels, width;
+    int32_t dtype;
+    int32_t silu;
+    subq_tensor3 x, y;      /* forward: y shares no memory with an input        */
+    subq_tensor3 dy, dx;    /* backward                                         */
+    const float* weight;    /* [channels, width]                                */
+    const float* bias;      /* [channels], or NULL (0)                          */
+    const uint8_t* mask;
+    int64_t mask_stride_b;
+    const void* state_in;   /* [B, width - 1, channels] of x's type, or NULL    */
+    void* state_out;        /* forward; may equal state_in, NULL = not wanted   */
+    const void* dstate_out; /* backward: gradient of state_out, or NULL         */
+    void* dstate_in;        /* backward: gradient of state_in, or NULL          */
+    float* dweight;         /* backward: [channels, width]                      */
+    float* dbias;           /* backward: [channels], or NULL                    */
+    void* workspace;        /* backward                                         */
+    size_t workspace_bytes;
+    void* stream;
+} subq_causal_conv_args;
+
+int subq_causal_conv_fwd(const subq_causal_conv_args* args);
+int subq_causal_conv_bwd(const subq_causal_conv_args* args);
+size_t subq_causal_conv_bwd_workspace_bytes(const subq_causal_conv_args* args);
+
+/* Root-mean-square norm over the last dimension of [rows, dim] with the residual's
+ * addition: r = x + residual (rounded to r's type; without a residual r is x),
+ *   y = r rsqrt(mean(r^2) + eps) weight.
+ * Types (x, r, y): r_dtype is that of residual and r, x's or fp32; y_dtype is x's,
+ * or for an fp32 x also fp16 or bf16, or SUBQ_E4M3: then every 128 columns of a row
+ * have a float32 scale = max(amax |y|, 1e-30) / 448 in `scale` [rows, ceil(dim /
+ * 128)] and y holds y / scale rounded to e4m3. norm = 0 leaves the norm out (y is
+ * r weight: quantising alone). dim <= 16384. Outputs share no memory with an input or
+ * one another, but for r in x's or residual's place (of one type and row stride).
+ *
+ * The backward is given r: dr = rsqrt(..) (g - xh mean(g xh)) + dr_next with g = dy
+ * weight (dy of x's type), dx and dres are dr in x's and r's types (either may be
+ * NULL), dweight = sum over rows of dy xh (written, bitwise reproducible). */
+#define SUBQ_E4M3 4
+
+typedef struct subq_rms_norm_args {
+    int64_t rows, dim;
+    int32_t x_dtype, r_dtype, y_dtype;
+    float eps;
+    int32_t norm;
+    const void* x;        int64_t x_stride;
+    const void* residual; int64_t residual_stride;  /* or NULL */
+    void* r;              int64_t r_stride;          /* or NULL; the backward's input */
+    void* y;              int64_t y_stride;
+    float* scale;         int64_t scale_stride;
+    const float* weight;                             /* [dim], or NULL (1) */
+    const void* dy;       int64_t dy_stride;
+    const void* dr_next;  int64_t dr_next_stride;    /* of r's type, or NULL */
+    void* dx;             int64_t dx_stride;
+    void* dres;           int64_t dres_stride;
+    float* dweight;                                  /* [dim], or NULL */
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} subq_rms_norm_args;
+
+int subq_rms_norm_fwd(const subq_rms_norm_args* args);
+int subq_rms_norm_bwd(const subq_rms_norm_args* args);
+size_t subq_rms_norm_bwd_workspace_bytes(const subq_rms_norm_args* args);
+
+/* Product of e4m3 matrices with float32 scales for every 1 x 128 of a and every
+ * 128 x 128 of b:
+ *   out[m, n] = bias[n] + sum_kb a_scale[m, kb] b_scale[n / 128, kb] sum_{k in kb} a[m, k] b[n, k]
+ * (b as a linear layer's weight [N, K]). The rows of a and b start on 16-byte
+ * boundaries (data and strides, in bytes); any M, N and K. Sums in float32; out is
+ * fp32, fp16 or bf16 and shares no memory with an input. */
+typedef struct subq_scaled_matmul_args {
+    int64_t M, N, K;
+    int32_t out_dtype;
+    const void* a;        int64_t a_stride;
+    const float* a_scale; int64_t a_scale_stride;  /* [M, ceil(K / 128)]             */
+    const void* b;        int64_t b_stride;
+    const float* b_scale; int64_t b_scale_stride;  /* [ceil(N / 128), ceil(K / 128)] */
+    const float* bias;                             /* [N], or NULL                   */
+    void* out;            int64_t out_stride;
+    void* stream;
+} subq_scaled_matmul_args;
+
+int subq_scaled_matmul(const subq_scaled_matmul_args* args);
 
 /* Backward scan with no allocation and no caller workspace (no counterpart in
  * the reference, whose backward allocates its scratch on every call). For

@@ -9,10 +9,10 @@
 #include <string>
 #include <tuple>
 
+#include "capi_common.h"
 #include "delta_common.cuh"
 #include "delta_launch.h"
 #include "kernels.hpp"
-#include "overlap.h"
 #include "scan_common.cuh"
 #include "scan_launch.h"
 
@@ -22,19 +22,24 @@ thread_local std::string g_last_error;
 thread_local int g_last_path = SUBQ_PATH_AUTO;
 thread_local int g_last_launches = 0;
 
+}  // namespace
+
+namespace subq {
+namespace capi {
 int fail(int code, const std::string& msg) {
     g_last_error = msg;
     return code;
 }
-
 int fail_cuda(cudaError_t err, const char* where) {
     return fail(SUBQ_ERR_CUDA, std::string(where) + ": " + cudaGetErrorString(err));
 }
+void set_launches(int n) { g_last_launches = n; }
+}  // namespace capi
+}  // namespace subq
 
-size_t elem_size(int dtype) { return dtype == SUBQ_FP64 ? 8 : dtype == SUBQ_FP32 ? 4 : 2; }
+namespace {
 
-constexpr size_t kAlign = 256;
-size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+using namespace subq::capi;
 
 // Common checks of a scan description; fills the scalar part of ScanParams.
 int check_desc(const subq_scan_desc& d, subq::ScanParams& p) {
@@ -194,16 +199,6 @@ size_t scan_bwd_ws(const subq::ScanParams& p, int dtype, bool tc) {
     return subq::bwd1_usable(p) ? subq::bwd1_workspace_bytes(p) : subq::tc_bwd_workspace_bytes(p);
 }
 
-int check_workspace(void* ws, size_t have, size_t need) {
-    if (need == 0) return SUBQ_OK;
-    if (!ws) return fail(SUBQ_ERR_WORKSPACE, "workspace required: " + std::to_string(need) + " bytes");
-    if (have < need)
-        return fail(SUBQ_ERR_WORKSPACE, "workspace too small: need " + std::to_string(need) +
-                                            " bytes, got " + std::to_string(have));
-    if (reinterpret_cast<uintptr_t>(ws) % kAlign != 0)
-        return fail(SUBQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-    return SUBQ_OK;
-}
 
 }  // namespace
 
@@ -592,10 +587,6 @@ void delta_segments(subq::DeltaParams& p, int dtype, const DeltaBytes& n, void* 
     p.seg_in = n.seg_in ? reinterpret_cast<float*>(static_cast<char*>(at) + n.seg_S + n.seg_M) : nullptr;
 }
 
-struct Memory {
-    const char* name;
-    subq::MemRows rows;
-};
 Memory of_tensor(const char* name, const subq::DeltaTensor& t, const subq::DeltaParams& p, int width, int dtype) {
     const __int128 es = (__int128)elem_size(dtype);
     return {name, {reinterpret_cast<uintptr_t>(t.p), (int64_t)(width * es), {p.B, p.H / t.group, p.N}, {t.sb * es, t.sh * es, t.sn * es}}};
@@ -603,25 +594,8 @@ Memory of_tensor(const char* name, const subq::DeltaTensor& t, const subq::Delta
 Memory of_gate(const char* name, const subq::DeltaGate& g, const subq::DeltaParams& p) {
     return {name, {reinterpret_cast<uintptr_t>(g.p), 4, {p.B, p.H, p.N}, {(__int128)4 * g.sb, (__int128)4 * g.sh, (__int128)4 * g.sn}}};
 }
-Memory of_bytes(const char* name, const void* at, int64_t bytes) { return {name, {reinterpret_cast<uintptr_t>(at), bytes}}; }
 Memory of_mask(const subq::DeltaParams& p) {
     return {"mask", {reinterpret_cast<uintptr_t>(p.mask), p.N, {p.B, 1, 1}, {p.mask_sb, 0, 0}}};
-}
-
-// An output's rows must be apart, from one another and from every input's and other output's.
-int check_apart(std::initializer_list<Memory> out_list, std::initializer_list<Memory> in_list) {
-    const Memory *outs = out_list.begin(), *ins = in_list.begin();
-    const int no = (int)out_list.size(), ni = (int)in_list.size();
-    for (int i = 0; i < no; ++i) {
-        if (subq::rows_overlap_themselves(outs[i].rows))
-            return fail(SUBQ_ERR_INVALID_ARGUMENT, std::string("rows of ") + outs[i].name + " overlap");
-        for (int j = 0; j < ni + i; ++j) {
-            const Memory& other = j < ni ? ins[j] : outs[j - ni];
-            if (subq::rows_overlap(outs[i].rows, other.rows))
-                return fail(SUBQ_ERR_ALIAS, std::string(outs[i].name) + " shares memory with " + other.name);
-        }
-    }
-    return SUBQ_OK;
 }
 
 int check_delta_fwd_apart(const subq::DeltaParams& p, int dtype) {

@@ -1,0 +1,392 @@
+// Selective scan, backward. With g_t = dout_t silu(z_t) and the adjoint of the state
+//   G_t = C_t g_t + a_{t+1} G_{t+1},
+//   dC_t = sum_d h_t g_t,   dB_t = sum_d G_t dt_t u_t,   du_t = dt_t (B_t . G_t) + D g_t,
+//   d dt_t = u_t (B_t . G_t) + sum_n A G_t a_t h_{t-1},   dA = sum_t dt_t G_t a_t h_{t-1},
+//   dz_t = dout_t y_t silu'(z_t),   dD = sum_t g_t u_t,   d raw_t = d dt_t sigmoid(raw_t + bias),   dbias = sum_t d raw_t.
+//
+// One CTA walks its channels' tiles of 32 tokens from the last to the first. The forward left the state before every
+// eighth token; from it eight tokens' states and a - 1 are formed forwards in registers and used up backwards, so that each
+// exponential is formed once. dB and dC are sums over channels: over a warp's by shuffles that halve the values at each
+// step, over the CTA's warps in shared memory, over CTAs by a second launch, all in a fixed order. Sums over tokens (dA, dD,
+// dbias) are added per eight tokens or tile with their rounding kept (two float32 a sum). Segments as in the forward.
+//
+// Bound by instruction issue.
+#pragma once
+
+#include "sel_fwd.cuh"
+
+namespace subq {
+namespace sel {
+
+// s += x with what the sum's rounding leaves out kept in `rest`.
+__device__ __forceinline__ void add_exactly(float& s, float& rest, float x) {
+    const float t = __fadd_rn(s, x), z = __fsub_rn(t, s);
+    rest = __fadd_rn(rest, __fadd_rn(__fsub_rn(s, __fsub_rn(t, z)), __fsub_rn(x, z)));
+    s = t;
+}
+
+// Sums v[0..7] over the 32 / LPC channels of a warp: the lane of channel c is left with the values [c * LPC / 4, ...).
+template <int LPC>
+__device__ __forceinline__ void channel_sums8(float (&v)[8], int lane) {
+#pragma unroll
+    for (int o = 16, n = 8; o >= LPC; o >>= 1, n >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < n / 2; ++i) {
+            const float keep = up ? v[i + n / 2] : v[i], give = up ? v[i] : v[i + n / 2];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+}
+
+// The adjoint that enters segment `seg` from behind: what the segments after it make of dS_out.
+template <int LPC>
+__device__ __forceinline__ void chain_back(const SelParams& p, int seg, int b, int d, int q, const float (&A2)[4], float (&g)[4]) {
+    constexpr int kNp = 4 * LPC;
+    for (int s = p.nseg - 1; s > seg; --s) {
+        const int64_t at = ((int64_t)s * p.B + b) * p.D + d;
+        const float4 x = *reinterpret_cast<const float4*>(p.seg_h + at * kNp + 4 * q);
+        const float dt = p.seg_dt[at];
+        g[0] = fmaf(decay(A2[0] * dt), g[0], g[0]) + x.x;
+        g[1] = fmaf(decay(A2[1] * dt), g[1], g[1]) + x.y;
+        g[2] = fmaf(decay(A2[2] * dt), g[2], g[2]) + x.z;
+        g[3] = fmaf(decay(A2[3] * dt), g[3], g[3]) + x.w;
+    }
+}
+
+template <typename T, int LPC>
+struct BwdSmem {
+    static constexpr int kCh = kSelThreads / LPC, kNp = 4 * LPC, kWarps = kSelThreads / 32, kVals = LPC / 4;
+    float2 sdt[kSelTile * kCh];  // dt, u; then B.G and sum A G a h
+    float sg[kSelTile * kCh];    // g; then y
+    float sB[kSelTile * kNp], sC[kSelTile * kNp];
+    float red[kWarps][kSelKeep][32 * kVals];
+};
+
+template <typename T, int LPC, bool WALK>
+__global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(const SelParams p) {
+    using P = Place<T, LPC>;
+    using S = BwdSmem<T, LPC>;
+    constexpr int kNp = 4 * LPC, V = P::kV, kCh = P::kCh, kCPW = 32 / LPC, kVals = S::kVals;
+    extern __shared__ __align__(16) unsigned char smem[];
+    S& s = *reinterpret_cast<S*>(smem);
+    const P at(p);
+    const int seg = WALK ? blockIdx.y : blockIdx.y + 1, first = seg * p.seg_tokens, last = min(p.L, first + p.seg_tokens);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & (LPC - 1), ch = threadIdx.x / LPC, d = at.d0 + ch;
+    const bool in = ch < at.nch;
+    float A2[4], g0[4] = {0.f, 0.f, 0.f, 0.f};
+    load_A<LPC>(p, d, in, q, A2);
+    const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
+    if (WALK && in) {
+        if (p.dS_out)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * q + i < p.N) g0[i] = p.dS_out[((int64_t)at.b * p.D + d) * p.N + 4 * q + i];
+        chain_back<LPC>(p, seg, at.b, d, q, A2, g0);
+    }
+    F2 P01 = f2(g0[0], g0[1]), P23 = f2(g0[2], g0[3]);  // a_{t+1} G_{t+1}
+    float bias[V], Dw[V], dt_sum[V], dD[V], dD_rest[V], db[V], db_rest[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const bool has = i < at.left;
+        bias[i] = has && p.dt_bias ? p.dt_bias[at.d0 + at.c0 + i] : 0.f;
+        Dw[i] = has && p.Dw ? p.Dw[at.d0 + at.c0 + i] : 0.f;
+        dt_sum[i] = dD[i] = dD_rest[i] = db[i] = db_rest[i] = 0.f;
+    }
+    float dA[4] = {0.f, 0.f, 0.f, 0.f}, dA_rest[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kBytes = need_vec<V * (int)sizeof(T)>();
+    const bool even = at.d0 % V == 0;
+    const bool vu = even && p.u.vec >= kBytes, vd = even && p.dt.vec >= kBytes, vz = even && p.z.vec >= kBytes, vg = even && p.dout.vec >= kBytes;
+    const bool vdu = even && p.du.vec >= kBytes, vdd = even && p.ddt.vec >= kBytes, vdz = even && p.dz.vec >= kBytes;
+    const int64_t keeps = (p.L + kSelKeep - 1) / kSelKeep;
+    for (int l0 = first + (last - 1 - first) / kSelTile * kSelTile; l0 >= first; l0 -= kSelTile) {
+        Piece<T, V> u, dt, z, go;
+        const int l = l0 + at.row;
+        const bool live = l < last && live_at<T>(p, at.b, l);
+        auto load = [&]() {
+            u.zero(); dt.zero(); z.zero(); go.zero();
+            if (live) {
+                if (WALK) u.load(row_of<T>(p.u, at.b, l, at.d0 + at.c0), at.left, vu);
+                dt.load(row_of<T>(p.dt, at.b, l, at.d0 + at.c0), at.left, vd);
+                if (p.z.p) z.load(row_of<T>(p.z, at.b, l, at.d0 + at.c0), at.left, vz);
+                go.load(row_of<T>(p.dout, at.b, l, at.d0 + at.c0), at.left, vg);
+            }
+        };
+        load();
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float x = to_f<T>(dt.x[i]) + bias[i], g = to_f<T>(go.x[i]);
+            if (p.softplus) x = softplus(x);
+            if (!live || i >= at.left) x = 0.f;
+            if (!WALK) dt_sum[i] += x;
+            if (p.z.p) {
+                const float zf = to_f<T>(z.x[i]);
+                g *= zf * sigmoid(zf);
+            }
+            s.sdt[at.row * kCh + at.c0 + i] = make_float2(x, to_f<T>(u.x[i]));
+            s.sg[at.row * kCh + at.c0 + i] = g;
+        }
+        {
+            States<T, LPC> x;
+            if (WALK) {
+                x.load(p, p.Bm, at.b, at.g, l0, last);
+                x.put(s.sB);
+            }
+            x.load(p, p.C, at.b, at.g, l0, last);
+            x.put(s.sC);
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int t8 = kSelTile - kSelKeep; t8 >= 0; t8 -= kSelKeep) {
+            if (l0 + t8 >= last) continue;  // (every token there is behind the end: nothing of the adjoint changes)
+            if constexpr (!WALK) {
+#pragma unroll
+                for (int i = kSelKeep - 1; i >= 0; --i) {
+                    const int t = t8 + i;
+                    const F2 dt2 = f2(s.sdt[t * kCh + ch].x), g2 = f2(s.sg[t * kCh + ch]);
+                    const float4 Cv = *reinterpret_cast<const float4*>(s.sC + t * kNp + 4 * q);
+                    const F2 G01 = fma(f2(Cv.x, Cv.y), g2, P01), G23 = fma(f2(Cv.z, Cv.w), g2, P23);
+                    P01 = fma(decay(mul(dt2, A01)), G01, G01);
+                    P23 = fma(decay(mul(dt2, A23)), G23, G23);
+                }
+            } else {
+                F2 e01[kSelKeep], e23[kSelKeep], h01[kSelKeep + 1], h23[kSelKeep + 1];
+                {
+                    const float4 x = in ? *reinterpret_cast<const float4*>(p.kept + (((int64_t)at.b * keeps + (l0 + t8) / kSelKeep) * p.D + d) * kNp + 4 * q)
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+                    h01[0] = f2(x.x, x.y);
+                    h23[0] = f2(x.z, x.w);
+                }
+                float ys[2];  // y of tokens q and 4 + q
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = 4 * half + j, t = t8 + i;
+                        const float2 x = s.sdt[t * kCh + ch];
+                        const float4 Bv = *reinterpret_cast<const float4*>(s.sB + t * kNp + 4 * q);
+                        const F2 dt2 = f2(x.x), du2 = f2(x.x * x.y);
+                        e01[i] = decay(mul(dt2, A01));
+                        e23[i] = decay(mul(dt2, A23));
+                        h01[i + 1] = add(h01[i], fma(e01[i], h01[i], mul(du2, f2(Bv.x, Bv.y))));
+                        h23[i + 1] = add(h23[i], fma(e23[i], h23[i], mul(du2, f2(Bv.z, Bv.w))));
+                        if (p.z.p) {
+                            const float4 Cv = *reinterpret_cast<const float4*>(s.sC + t * kNp + 4 * q);
+                            y[j] = both(fma(h23[i + 1], f2(Cv.z, Cv.w), mul(h01[i + 1], f2(Cv.x, Cv.y))));
+                        }
+                    }
+                    if (p.z.p) ys[half] = lane_sums4<LPC>(y, lane);
+                }
+                F2 a01 = f2(0.f), a23 = f2(0.f);
+#pragma unroll
+                for (int half = 1; half >= 0; --half) {
+                    float bg[4], ag[4];
+#pragma unroll
+                    for (int j = 3; j >= 0; --j) {
+                        const int i = 4 * half + j, t = t8 + i;
+                        const float2 x = s.sdt[t * kCh + ch];
+                        const float4 Bv = *reinterpret_cast<const float4*>(s.sB + t * kNp + 4 * q), Cv = *reinterpret_cast<const float4*>(s.sC + t * kNp + 4 * q);
+                        const F2 g2 = f2(s.sg[t * kCh + ch]), dt2 = f2(x.x), du2 = f2(x.x * x.y);
+                        const F2 G01 = fma(f2(Cv.x, Cv.y), g2, P01), G23 = fma(f2(Cv.z, Cv.w), g2, P23);
+                        bg[j] = both(fma(G23, f2(Bv.z, Bv.w), mul(G01, f2(Bv.x, Bv.y))));
+                        const F2 n01 = mul(G01, fma(e01[i], h01[i], h01[i])), n23 = mul(G23, fma(e23[i], h23[i], h23[i]));
+                        ag[j] = both(fma(n23, A23, mul(n01, A01)));
+                        a01 = fma(dt2, n01, a01);
+                        a23 = fma(dt2, n23, a23);
+                        float v[8];
+                        get(mul(G01, du2), v[0], v[1]);
+                        get(mul(G23, du2), v[2], v[3]);
+                        get(mul(h01[i + 1], g2), v[4], v[5]);
+                        get(mul(h23[i + 1], g2), v[6], v[7]);
+                        channel_sums8<LPC>(v, lane);
+#pragma unroll
+                        for (int k = 0; k < kVals; ++k) s.red[warp][i][k * 32 + lane] = v[k];
+                        P01 = fma(e01[i], G01, G01);
+                        P23 = fma(e23[i], G23, G23);
+                    }
+                    const float b4 = lane_sums4<LPC>(bg, lane), a4 = lane_sums4<LPC>(ag, lane);
+                    __syncwarp();  // every lane of the channel has read these tokens' dt, u and g
+                    if (q < 4) {
+                        const int t = t8 + 4 * half + q;
+                        s.sdt[t * kCh + ch] = make_float2(b4, a4 * 0.6931471805599453f);
+                        s.sg[t * kCh + ch] = ys[half];
+                    }
+                }
+                float x[4];
+                get(a01, x[0], x[1]);
+                get(a23, x[2], x[3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) add_exactly(dA[i], dA_rest[i], x[i]);
+                __syncthreads();
+                // values (token, value k, lane) of every warp: k * 32 + lane is value c * kVals + k of quad q
+                for (int i = threadIdx.x; i < kSelKeep * 32 * kVals; i += kSelThreads) {
+                    const int t = i / (32 * kVals), k = i / 32 % kVals, ln = i & 31;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < S::kWarps; ++w) sum += s.red[w][t][k * 32 + ln];
+                    const int val = ln / LPC * kVals + k, n = 4 * (ln & (LPC - 1)) + (val & 3), tok = l0 + t8 + t;
+                    if (tok < last)
+                        p.part_bc[((((int64_t)at.block(p) * p.B + at.b) * p.L + tok) * p.G + at.g) * (2 * kNp) + (val >> 2) * kNp + n] = sum;
+                }
+                __syncthreads();
+            }
+        }
+        if constexpr (WALK) {
+            if (l < last && at.left > 0) {
+                load();
+                Piece<T, V> du, dd, dzv;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float2 x = s.sdt[at.row * kCh + at.c0 + i];  // B.G, sum A G a h
+                    const float uf = to_f<T>(u.x[i]), gf = to_f<T>(go.x[i]), raw = to_f<T>(dt.x[i]) + bias[i];
+                    float y = s.sg[at.row * kCh + at.c0 + i], g = gf;
+                    if (p.z.p) {
+                        const float zf = to_f<T>(z.x[i]), sz = sigmoid(zf);
+                        y = fmaf(Dw[i], uf, y);
+                        dzv.x[i] = from_f<T>(live ? gf * y * sz * fmaf(zf, 1.f - sz, 1.f) : 0.f);
+                        g *= zf * sz;
+                    }
+                    const float step = p.softplus ? softplus(raw) : raw;
+                    float ddt = fmaf(uf, x.x, x.y);
+                    if (p.softplus) ddt *= sigmoid(raw);
+                    if (!live) ddt = 0.f;
+                    du.x[i] = from_f<T>(live ? fmaf(step, x.x, Dw[i] * g) : 0.f);
+                    dd.x[i] = from_f<T>(ddt);
+                    if (live && i < at.left) {
+                        add_exactly(dD[i], dD_rest[i], g * uf);
+                        add_exactly(db[i], db_rest[i], ddt);
+                    }
+                }
+                du.store(const_cast<T*>(row_of<T>(p.du, at.b, l, at.d0 + at.c0)), at.left, vdu);
+                dd.store(const_cast<T*>(row_of<T>(p.ddt, at.b, l, at.d0 + at.c0)), at.left, vdd);
+                if (p.z.p) dzv.store(const_cast<T*>(row_of<T>(p.dz, at.b, l, at.d0 + at.c0)), at.left, vdz);
+            }
+        }
+        __syncthreads();  // the next tile takes the place of this one
+    }
+    float g[4];
+    get(P01, g[0], g[1]);
+    get(P23, g[2], g[3]);
+    float* rows = reinterpret_cast<float*>(s.sdt);  // [tile][channels]
+    if constexpr (!WALK) {
+        const int64_t to = ((int64_t)seg * p.B + at.b) * p.D;
+        if (in) *reinterpret_cast<float4*>(p.seg_h + (to + d) * kNp + 4 * q) = make_float4(g[0], g[1], g[2], g[3]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) rows[at.row * kCh + at.c0 + i] = dt_sum[i];
+        __syncthreads();
+        if (threadIdx.x < at.nch) {
+            float x = 0.f;
+            for (int r = 0; r < kSelTile; ++r) x += rows[r * kCh + threadIdx.x];
+            p.seg_dt[to + at.d0 + threadIdx.x] = x;
+        }
+        return;
+    }
+    if (in && seg == 0 && p.dS_in)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * q + i < p.N) p.dS_in[((int64_t)at.b * p.D + d) * p.N + 4 * q + i] = g[i];
+    const int64_t part = (int64_t)at.b * p.nseg + seg;
+    if (in)
+        *reinterpret_cast<float4*>(p.part_a + (part * p.D + d) * kNp + 4 * q) =
+            make_float4(dA[0] + dA_rest[0], dA[1] + dA_rest[1], dA[2] + dA_rest[2], dA[3] + dA_rest[3]);
+    float* rows2 = rows + kSelTile * kCh;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        rows[at.row * kCh + at.c0 + i] = dD[i] + dD_rest[i];
+        rows2[at.row * kCh + at.c0 + i] = db[i] + db_rest[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2 * kCh) {
+        const int which = threadIdx.x / kCh, c = threadIdx.x % kCh;
+        if (c < at.nch) {
+            float x = 0.f, rest = 0.f;
+            for (int r = 0; r < kSelTile; ++r) add_exactly(x, rest, (which ? rows2 : rows)[r * kCh + c]);
+            p.part_d[(part * 2 + which) * p.D + at.d0 + c] = x + rest;
+        }
+    }
+}
+
+// dB and dC: the parts of a group's channel blocks, added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) sel_sum_bc_kernel(const SelParams p, int np, int blocks) {
+    const int64_t n = (int64_t)p.B * p.L * p.G * 2 * np;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int state = (int)(i % np);
+        if (state >= p.N) continue;
+        float s = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < blocks; ++k) s += p.part_bc[k * n + i];
+        int64_t r = i / np;
+        const int which = (int)(r & 1);
+        r >>= 1;
+        const int g = (int)(r % p.G);
+        r /= p.G;
+        const int64_t l = r % p.L, b = r / p.L;
+        if (which) static_cast<T*>(p.dC)[b * p.dC_sb + l * p.dC_sl + g * p.dC_sg + state] = from_f<T>(s);
+        else static_cast<T*>(p.dB)[b * p.dB_sb + l * p.dB_sl + g * p.dB_sg + state] = from_f<T>(s);
+    }
+}
+
+// dA, dD and dbias: the parts of sequences and segments, added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) sel_sum_weights_kernel(const SelParams p, int np) {
+    const int64_t n = (int64_t)p.D * (np + 2), parts = (int64_t)p.B * p.nseg;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t na = (int64_t)p.D * np;
+        float s = 0.f, rest = 0.f;
+        if (i < na) {
+            if (i % np >= p.N) continue;
+#pragma unroll 4
+            for (int64_t k = 0; k < parts; ++k) add_exactly(s, rest, p.part_a[k * na + i]);
+            p.dA[i / np * p.N + i % np] = s + rest;
+        } else {
+            const int64_t j = i - na;
+            const int which = j >= p.D;
+            float* to = which ? p.dbias : p.dD;
+            if (!to) continue;
+#pragma unroll 4
+            for (int64_t k = 0; k < parts; ++k) add_exactly(s, rest, p.part_d[k * 2 * p.D + j]);
+            to[j - (which ? p.D : 0)] = s + rest;
+        }
+    }
+}
+
+template <typename T, int LPC, bool WALK>
+cudaError_t launch_bwd_kernel(const SelParams& p, cudaStream_t st) {
+    constexpr size_t smem = sizeof(BwdSmem<T, LPC>);
+    if (smem > 48 * 1024) {
+        cudaError_t err = cudaFuncSetAttribute(sel_bwd_kernel<T, LPC, WALK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return err;
+    }
+    const int kCh = kSelThreads / LPC;
+    const dim3 grid((unsigned)(p.B * p.G * ((p.Dg + kCh - 1) / kCh)), (unsigned)(WALK ? p.nseg : p.nseg - 1));
+    sel_bwd_kernel<T, LPC, WALK><<<grid, kSelThreads, smem, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_bwd(const SelParams& p, SelPass pass, cudaStream_t st) {
+    auto run = [&](auto lpc) {
+        constexpr int LPC = decltype(lpc)::value;
+        return pass == kSelWalk ? launch_bwd_kernel<T, LPC, true>(p, st) : launch_bwd_kernel<T, LPC, false>(p, st);
+    };
+    switch (sel_lanes(p.N)) {
+        case 4: return run(std::integral_constant<int, 4>{});
+        case 8: return run(std::integral_constant<int, 8>{});
+        case 16: return run(std::integral_constant<int, 16>{});
+        default: return run(std::integral_constant<int, 32>{});
+    }
+}
+
+template <typename T>
+cudaError_t launch_sums(const SelParams& p, cudaStream_t st) {
+    const int np = 4 * sel_lanes(p.N), kCh = sel_channels(p.N), blocks = (p.Dg + kCh - 1) / kCh;
+    auto grid = [](int64_t n) { return (unsigned)((n + 255) / 256 < 148 * 16 ? (n + 255) / 256 : 148 * 16); };
+    sel_sum_bc_kernel<T><<<grid((int64_t)p.B * p.L * p.G * 2 * np), 256, 0, st>>>(p, np, blocks);
+    sel_sum_weights_kernel<T><<<grid((int64_t)p.D * (np + 2)), 256, 0, st>>>(p, np);
+    return cudaGetLastError();
+}
+
+}  // namespace sel
+}  // namespace subq

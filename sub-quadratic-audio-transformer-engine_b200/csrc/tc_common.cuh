@@ -586,6 +586,9 @@ struct Cursor {
 // Launch plumbing (scan_tc.cu).
 struct Maps;
 bool make_map(CUtensorMap* m, const void* base, int dtype, int N, int H, int B, int64_t sn, int64_t sh, int64_t sb);
+// [rows, cols] bytes with rows `stride` bytes apart (a multiple of 16, as the base), boxes of 128 bytes x box_rows, 128-byte
+// swizzle; zeros behind the last row and column.
+bool make_byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t stride, int box_rows);
 int pick_segments(const ScanParams& p, const void* kern, int threads, size_t smem);
 int* status_ptr();  // device address of the status word (current device)
 int fwd_segment_count(const ScanParams& p);

@@ -22,7 +22,7 @@ SUBQ_ERR_TIMEOUT = 5
 SUBQ_ERR_WORKSPACE = 6
 SUBQ_ERR_STATE = 7
 
-SUBQ_FP32, SUBQ_FP16, SUBQ_BF16, SUBQ_FP64 = 0, 1, 2, 3
+SUBQ_FP32, SUBQ_FP16, SUBQ_BF16, SUBQ_FP64, SUBQ_E4M3 = 0, 1, 2, 3, 4
 SUBQ_DECAY_NONE, SUBQ_DECAY_SCALAR, SUBQ_DECAY_PER_HEAD, SUBQ_DECAY_PER_TOKEN = 0, 1, 2, 3
 SUBQ_PATH_AUTO, SUBQ_PATH_EXACT, SUBQ_PATH_TENSORCORE, SUBQ_PATH_CHUNKED = 0, 1, 2, 3
 
@@ -36,6 +36,11 @@ EXPORTED = (
     "subq_delta_fwd", "subq_delta_bwd", "subq_delta_fwd_workspace_bytes", "subq_delta_bwd_workspace_bytes",
     "subq_delta_handover_bytes",
     "subq_layer_norm_fwd", "subq_layer_norm_bwd", "subq_layer_norm_bwd_workspace_bytes",
+    "subq_selective_scan_fwd", "subq_selective_scan_bwd", "subq_selective_scan_fwd_workspace_bytes",
+    "subq_selective_scan_bwd_workspace_bytes", "subq_selective_scan_handover_bytes",
+    "subq_causal_conv_fwd", "subq_causal_conv_bwd", "subq_causal_conv_bwd_workspace_bytes",
+    "subq_rms_norm_fwd", "subq_rms_norm_bwd", "subq_rms_norm_bwd_workspace_bytes",
+    "subq_scaled_matmul",
 )
 
 
@@ -135,6 +140,75 @@ class LayerNormArgs(ctypes.Structure):
     ]
 
 
+class Tensor3(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64),
+                ("stride_l", ctypes.c_int64), ("stride_g", ctypes.c_int64)]
+
+
+class SelectiveDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64), ("seq_len", ctypes.c_int64), ("channels", ctypes.c_int64),
+        ("states", ctypes.c_int64), ("groups", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("softplus", ctypes.c_int32),
+        ("A", ctypes.c_void_p), ("D", ctypes.c_void_p), ("dt_bias", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p), ("mask_stride_b", ctypes.c_int64),
+    ]
+
+
+class SelectiveFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("desc", SelectiveDesc), ("u", Tensor3), ("dt", Tensor3), ("z", Tensor3), ("B", Tensor3), ("C", Tensor3),
+        ("out", Tensor3), ("state_in", ctypes.c_void_p), ("state_out", ctypes.c_void_p), ("handover", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class SelectiveBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("desc", SelectiveDesc), ("u", Tensor3), ("dt", Tensor3), ("z", Tensor3), ("B", Tensor3), ("C", Tensor3),
+        ("dout", Tensor3), ("du", Tensor3), ("ddt", Tensor3), ("dz", Tensor3), ("dB", Tensor3), ("dC", Tensor3),
+        ("state_in", ctypes.c_void_p), ("dstate_out", ctypes.c_void_p), ("dstate_in", ctypes.c_void_p),
+        ("dA", ctypes.c_void_p), ("dD", ctypes.c_void_p), ("ddt_bias", ctypes.c_void_p), ("handover", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class CausalConvArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64), ("seq_len", ctypes.c_int64), ("channels", ctypes.c_int64), ("width", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("silu", ctypes.c_int32),
+        ("x", Tensor3), ("y", Tensor3), ("dy", Tensor3), ("dx", Tensor3),
+        ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("mask_stride_b", ctypes.c_int64),
+        ("state_in", ctypes.c_void_p), ("state_out", ctypes.c_void_p), ("dstate_out", ctypes.c_void_p),
+        ("dstate_in", ctypes.c_void_p), ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("dim", ctypes.c_int64),
+        ("x_dtype", ctypes.c_int32), ("r_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float), ("norm", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+        ("r", ctypes.c_void_p), ("r_stride", ctypes.c_int64), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64),
+        ("scale", ctypes.c_void_p), ("scale_stride", ctypes.c_int64), ("weight", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64), ("dr_next", ctypes.c_void_p), ("dr_next_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p), ("dx_stride", ctypes.c_int64), ("dres", ctypes.c_void_p), ("dres_stride", ctypes.c_int64),
+        ("dweight", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class ScaledMatmulArgs(ctypes.Structure):
+    _fields_ = [
+        ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("out_dtype", ctypes.c_int32),
+        ("a", ctypes.c_void_p), ("a_stride", ctypes.c_int64), ("a_scale", ctypes.c_void_p), ("a_scale_stride", ctypes.c_int64),
+        ("b", ctypes.c_void_p), ("b_stride", ctypes.c_int64), ("b_scale", ctypes.c_void_p), ("b_scale_stride", ctypes.c_int64),
+        ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64), ("stream", ctypes.c_void_p),
+    ]
+
+
 class SubqError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(message)
@@ -190,13 +264,22 @@ def load() -> ctypes.CDLL:
             lib.subq_head_rmsnorm_bwd_workspace_bytes.argtypes = [ctypes.POINTER(RmsArgs)]
             lib.subq_head_rmsnorm_bwd_workspace_bytes.restype = ctypes.c_size_t
             for name, args in (("subq_delta_fwd", DeltaFwdArgs), ("subq_delta_bwd", DeltaBwdArgs),
-                               ("subq_layer_norm_fwd", LayerNormArgs), ("subq_layer_norm_bwd", LayerNormArgs)):
+                               ("subq_layer_norm_fwd", LayerNormArgs), ("subq_layer_norm_bwd", LayerNormArgs),
+                               ("subq_selective_scan_fwd", SelectiveFwdArgs), ("subq_selective_scan_bwd", SelectiveBwdArgs),
+                               ("subq_causal_conv_fwd", CausalConvArgs), ("subq_causal_conv_bwd", CausalConvArgs),
+                               ("subq_rms_norm_fwd", RmsNormArgs), ("subq_rms_norm_bwd", RmsNormArgs),
+                               ("subq_scaled_matmul", ScaledMatmulArgs)):
                 getattr(lib, name).argtypes = [ctypes.POINTER(args)]
                 getattr(lib, name).restype = ctypes.c_int
             for name, args in (("subq_delta_fwd_workspace_bytes", DeltaFwdArgs),
                                ("subq_delta_bwd_workspace_bytes", DeltaBwdArgs),
                                ("subq_delta_handover_bytes", DeltaDesc),
-                               ("subq_layer_norm_bwd_workspace_bytes", LayerNormArgs)):
+                               ("subq_layer_norm_bwd_workspace_bytes", LayerNormArgs),
+                               ("subq_selective_scan_fwd_workspace_bytes", SelectiveFwdArgs),
+                               ("subq_selective_scan_bwd_workspace_bytes", SelectiveBwdArgs),
+                               ("subq_selective_scan_handover_bytes", SelectiveDesc),
+                               ("subq_causal_conv_bwd_workspace_bytes", CausalConvArgs),
+                               ("subq_rms_norm_bwd_workspace_bytes", RmsNormArgs)):
                 getattr(lib, name).argtypes = [ctypes.POINTER(args)]
                 getattr(lib, name).restype = ctypes.c_size_t
             _lib = lib
@@ -266,6 +349,54 @@ def layer_norm_bwd(args: LayerNormArgs) -> None:
 
 def layer_norm_bwd_workspace_bytes(args: LayerNormArgs) -> int:
     return int(load().subq_layer_norm_bwd_workspace_bytes(ctypes.byref(args)))
+
+
+def selective_scan_fwd(args: SelectiveFwdArgs) -> None:
+    check(load().subq_selective_scan_fwd(ctypes.byref(args)))
+
+
+def selective_scan_bwd(args: SelectiveBwdArgs) -> None:
+    check(load().subq_selective_scan_bwd(ctypes.byref(args)))
+
+
+def selective_scan_fwd_workspace_bytes(args: SelectiveFwdArgs) -> int:
+    return int(load().subq_selective_scan_fwd_workspace_bytes(ctypes.byref(args)))
+
+
+def selective_scan_bwd_workspace_bytes(args: SelectiveBwdArgs) -> int:
+    return int(load().subq_selective_scan_bwd_workspace_bytes(ctypes.byref(args)))
+
+
+def selective_scan_handover_bytes(desc: SelectiveDesc) -> int:
+    return int(load().subq_selective_scan_handover_bytes(ctypes.byref(desc)))
+
+
+def causal_conv_fwd(args: CausalConvArgs) -> None:
+    check(load().subq_causal_conv_fwd(ctypes.byref(args)))
+
+
+def causal_conv_bwd(args: CausalConvArgs) -> None:
+    check(load().subq_causal_conv_bwd(ctypes.byref(args)))
+
+
+def causal_conv_bwd_workspace_bytes(args: CausalConvArgs) -> int:
+    return int(load().subq_causal_conv_bwd_workspace_bytes(ctypes.byref(args)))
+
+
+def rms_norm_fwd(args: RmsNormArgs) -> None:
+    check(load().subq_rms_norm_fwd(ctypes.byref(args)))
+
+
+def rms_norm_bwd(args: RmsNormArgs) -> None:
+    check(load().subq_rms_norm_bwd(ctypes.byref(args)))
+
+
+def rms_norm_bwd_workspace_bytes(args: RmsNormArgs) -> int:
+    return int(load().subq_rms_norm_bwd_workspace_bytes(ctypes.byref(args)))
+
+
+def scaled_matmul(args: ScaledMatmulArgs) -> None:
+    check(load().subq_scaled_matmul(ctypes.byref(args)))
 
 
 def fwd_workspace_bytes(args: FwdArgs) -> int:

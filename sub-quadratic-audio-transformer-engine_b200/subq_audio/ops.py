@@ -778,3 +778,9 @@ def last_path() -> str:
 
 def last_launches() -> int:
     return _capi.last_launches()
+
+
+# --------------------------------------------- a selective state space block (block_ops.py)
+from .block_ops import (  # noqa: E402  (it uses what stands above)
+    CausalConvStep, ScanHandover, SelectiveGrads, SelectiveScanStep, causal_conv_backward, causal_conv_forward, quantize_fp8,
+    quantize_fp8_weight, rms_norm, rms_norm_backward, rms_norm_fp8, scaled_matmul, selective_scan_backward, selective_scan_forward)
