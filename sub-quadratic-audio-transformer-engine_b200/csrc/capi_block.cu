@@ -95,8 +95,14 @@ int check_sel(const subq_selective_desc& d, SelParams& p) {
 // Segments of a sequence that are walked side by side where there are few channels.
 void sel_split(SelParams& p, bool back) {
     const int64_t ch = sel_channels(p.N), ctas = (int64_t)p.B * p.G * ((p.Dg + ch - 1) / ch);
-    const int64_t slots = back ? 296 : 444, tiles = (p.L + kSelTile - 1) / kSelTile;
-    if (ctas <= 0 || 2 * ctas > slots || tiles < 8) return;
+#ifndef SEL_SLOTS
+#define SEL_SLOTS 444
+#endif
+#ifndef SEL_MUL
+#define SEL_MUL 2
+#endif
+    const int64_t slots = back ? 296 : SEL_SLOTS, tiles = (p.L + kSelTile - 1) / kSelTile;
+    if (ctas <= 0 || SEL_MUL * ctas > slots || tiles < 8) return;
     int64_t g = std::min<int64_t>(slots / ctas, tiles / 4);
     const int64_t per = (tiles + g - 1) / g;
     p.seg_tokens = (int)(per * kSelTile);

@@ -5,7 +5,7 @@
 //   dz_t = dout_t y_t silu'(z_t),   dD = sum_t g_t u_t,   d raw_t = d dt_t sigmoid(raw_t + bias),   dbias = sum_t d raw_t.
 //
 // One CTA walks its channels' tiles of 32 tokens from the last to the first. The forward left the state before every
-// eighth token; from it eight tokens' states and a - 1 are formed forwards in registers and used up backwards, so that each
+// eighth token; from it eight tokens' a h and factors are formed forwards in registers and used up backwards, so that each
 // exponential is formed once. dB and dC are sums over channels: over a warp's by shuffles that halve the values at each
 // step, over the CTA's warps in shared memory, over CTAs by a second launch, all in a fixed order. Sums over tokens (dA, dD,
 // dbias) are added per eight tokens or tile with their rounding kept (two float32 a sum). Segments as in the forward.
@@ -17,13 +17,6 @@
 
 namespace subq {
 namespace sel {
-
-// s += x with what the sum's rounding leaves out kept in `rest`.
-__device__ __forceinline__ void add_exactly(float& s, float& rest, float x) {
-    const float t = __fadd_rn(s, x), z = __fsub_rn(t, s);
-    rest = __fadd_rn(rest, __fadd_rn(__fsub_rn(s, __fsub_rn(t, z)), __fsub_rn(x, z)));
-    s = t;
-}
 
 // Sums v[0..7] over the 32 / LPC channels of a warp: the lane of channel c is left with the values [c * LPC / 4, ...).
 template <int LPC>
@@ -47,10 +40,10 @@ __device__ __forceinline__ void chain_back(const SelParams& p, int seg, int b, i
         const int64_t at = ((int64_t)s * p.B + b) * p.D + d;
         const float4 x = *reinterpret_cast<const float4*>(p.seg_h + at * kNp + 4 * q);
         const float dt = p.seg_dt[at];
-        g[0] = fmaf(decay(A2[0] * dt), g[0], g[0]) + x.x;
-        g[1] = fmaf(decay(A2[1] * dt), g[1], g[1]) + x.y;
-        g[2] = fmaf(decay(A2[2] * dt), g[2], g[2]) + x.z;
-        g[3] = fmaf(decay(A2[3] * dt), g[3], g[3]) + x.w;
+        g[0] = decayed(A2[0] * dt, g[0]) + x.x;
+        g[1] = decayed(A2[1] * dt, g[1]) + x.y;
+        g[2] = decayed(A2[2] * dt, g[2]) + x.z;
+        g[3] = decayed(A2[3] * dt, g[3]) + x.w;
     }
 }
 
@@ -63,7 +56,7 @@ struct BwdSmem {
     float red[kWarps][kSelKeep][32 * kVals];
 };
 
-template <typename T, int LPC, bool WALK>
+template <typename T, int LPC>
 __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(const SelParams p) {
     using P = Place<T, LPC>;
     using S = BwdSmem<T, LPC>;
@@ -71,13 +64,13 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     extern __shared__ __align__(16) unsigned char smem[];
     S& s = *reinterpret_cast<S*>(smem);
     const P at(p);
-    const int seg = WALK ? blockIdx.y : blockIdx.y + 1, first = seg * p.seg_tokens, last = min(p.L, first + p.seg_tokens);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & (LPC - 1), ch = threadIdx.x / LPC, d = at.d0 + ch;
+    const int seg = blockIdx.y, first = seg * p.seg_tokens, last = min(p.L, first + p.seg_tokens);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & (LPC - 1), ch = threadIdx.x / LPC, cp = pair_at(ch), cs = single_at(ch), d = at.d0 + ch;
     const bool in = ch < at.nch;
     float A2[4], g0[4] = {0.f, 0.f, 0.f, 0.f};
     load_A<LPC>(p, d, in, q, A2);
     const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
-    if (WALK && in) {
+    if (in) {
         if (p.dS_out)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -85,13 +78,13 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
         chain_back<LPC>(p, seg, at.b, d, q, A2, g0);
     }
     F2 P01 = f2(g0[0], g0[1]), P23 = f2(g0[2], g0[3]);  // a_{t+1} G_{t+1}
-    float bias[V], Dw[V], dt_sum[V], dD[V], dD_rest[V], db[V], db_rest[V];
+    float bias[V], Dw[V], dD[V], dD_rest[V], db[V], db_rest[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const bool has = i < at.left;
         bias[i] = has && p.dt_bias ? p.dt_bias[at.d0 + at.c0 + i] : 0.f;
         Dw[i] = has && p.Dw ? p.Dw[at.d0 + at.c0 + i] : 0.f;
-        dt_sum[i] = dD[i] = dD_rest[i] = db[i] = db_rest[i] = 0.f;
+        dD[i] = dD_rest[i] = db[i] = db_rest[i] = 0.f;
     }
     float dA[4] = {0.f, 0.f, 0.f, 0.f}, dA_rest[4] = {0.f, 0.f, 0.f, 0.f};
     constexpr int kBytes = need_vec<V * (int)sizeof(T)>();
@@ -106,32 +99,35 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
         auto load = [&]() {
             u.zero(); dt.zero(); z.zero(); go.zero();
             if (live) {
-                if (WALK) u.load(row_of<T>(p.u, at.b, l, at.d0 + at.c0), at.left, vu);
+                u.load(row_of<T>(p.u, at.b, l, at.d0 + at.c0), at.left, vu);
                 dt.load(row_of<T>(p.dt, at.b, l, at.d0 + at.c0), at.left, vd);
                 if (p.z.p) z.load(row_of<T>(p.z, at.b, l, at.d0 + at.c0), at.left, vz);
                 go.load(row_of<T>(p.dout, at.b, l, at.d0 + at.c0), at.left, vg);
             }
         };
         load();
+        {
+            float x[V], g[V], uf[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float x = to_f<T>(dt.x[i]) + bias[i], g = to_f<T>(go.x[i]);
-            if (p.softplus) x = softplus(x);
-            if (!live || i >= at.left) x = 0.f;
-            if (!WALK) dt_sum[i] += x;
-            if (p.z.p) {
-                const float zf = to_f<T>(z.x[i]);
-                g *= zf * sigmoid(zf);
+            for (int i = 0; i < V; ++i) {
+                x[i] = to_f<T>(dt.x[i]) + bias[i];
+                g[i] = to_f<T>(z.x[i]);
+                uf[i] = to_f<T>(u.x[i]);
             }
-            s.sdt[at.row * kCh + at.c0 + i] = make_float2(x, to_f<T>(u.x[i]));
-            s.sg[at.row * kCh + at.c0 + i] = g;
+            if (p.softplus) softplus_all(x);
+            if (p.z.p) sigmoid_all(g);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (!live || i >= at.left) x[i] = 0.f;
+                g[i] = p.z.p ? to_f<T>(go.x[i]) * (to_f<T>(z.x[i]) * g[i]) : to_f<T>(go.x[i]);
+            }
+            put_pairs(s.sdt + at.row * kCh, at.c0, x, uf);
+            put_singles(s.sg + at.row * kCh, at.c0, g);
         }
         {
             States<T, LPC> x;
-            if (WALK) {
-                x.load(p, p.Bm, at.b, at.g, l0, last);
-                x.put(s.sB);
-            }
+            x.load(p, p.Bm, at.b, at.g, l0, last);
+            x.put(s.sB);
             x.load(p, p.C, at.b, at.g, l0, last);
             x.put(s.sC);
         }
@@ -139,23 +135,15 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
 #pragma unroll 1
         for (int t8 = kSelTile - kSelKeep; t8 >= 0; t8 -= kSelKeep) {
             if (l0 + t8 >= last) continue;  // (every token there is behind the end: nothing of the adjoint changes)
-            if constexpr (!WALK) {
-#pragma unroll
-                for (int i = kSelKeep - 1; i >= 0; --i) {
-                    const int t = t8 + i;
-                    const F2 dt2 = f2(s.sdt[t * kCh + ch].x), g2 = f2(s.sg[t * kCh + ch]);
-                    const float4 Cv = *reinterpret_cast<const float4*>(s.sC + t * kNp + 4 * q);
-                    const F2 G01 = fma(f2(Cv.x, Cv.y), g2, P01), G23 = fma(f2(Cv.z, Cv.w), g2, P23);
-                    P01 = fma(decay(mul(dt2, A01)), G01, G01);
-                    P23 = fma(decay(mul(dt2, A23)), G23, G23);
-                }
-            } else {
-                F2 e01[kSelKeep], e23[kSelKeep], h01[kSelKeep + 1], h23[kSelKeep + 1];
+            {
+                Factor f01[kSelKeep], f23[kSelKeep];
+                F2 ah01[kSelKeep], ah23[kSelKeep];  // a_t h_{t-1}
+                F2 h01, h23;
                 {
                     const float4 x = in ? *reinterpret_cast<const float4*>(p.kept + (((int64_t)at.b * keeps + (l0 + t8) / kSelKeep) * p.D + d) * kNp + 4 * q)
                                         : make_float4(0.f, 0.f, 0.f, 0.f);
-                    h01[0] = f2(x.x, x.y);
-                    h23[0] = f2(x.z, x.w);
+                    h01 = f2(x.x, x.y);
+                    h23 = f2(x.z, x.w);
                 }
                 float ys[2];  // y of tokens q and 4 + q
 #pragma unroll
@@ -164,16 +152,18 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int i = 4 * half + j, t = t8 + i;
-                        const float2 x = s.sdt[t * kCh + ch];
+                        const float2 x = s.sdt[t * kCh + cp];
                         const float4 Bv = *reinterpret_cast<const float4*>(s.sB + t * kNp + 4 * q);
                         const F2 dt2 = f2(x.x), du2 = f2(x.x * x.y);
-                        e01[i] = decay(mul(dt2, A01));
-                        e23[i] = decay(mul(dt2, A23));
-                        h01[i + 1] = add(h01[i], fma(e01[i], h01[i], mul(du2, f2(Bv.x, Bv.y))));
-                        h23[i + 1] = add(h23[i], fma(e23[i], h23[i], mul(du2, f2(Bv.z, Bv.w))));
+                        f01[i] = factor(mul(dt2, A01));
+                        f23[i] = factor(mul(dt2, A23));
+                        ah01[i] = decayed(f01[i], h01);
+                        ah23[i] = decayed(f23[i], h23);
+                        h01 = fma(du2, f2(Bv.x, Bv.y), ah01[i]);
+                        h23 = fma(du2, f2(Bv.z, Bv.w), ah23[i]);
                         if (p.z.p) {
                             const float4 Cv = *reinterpret_cast<const float4*>(s.sC + t * kNp + 4 * q);
-                            y[j] = both(fma(h23[i + 1], f2(Cv.z, Cv.w), mul(h01[i + 1], f2(Cv.x, Cv.y))));
+                            y[j] = both(fma(h23, f2(Cv.z, Cv.w), mul(h01, f2(Cv.x, Cv.y))));
                         }
                     }
                     if (p.z.p) ys[half] = lane_sums4<LPC>(y, lane);
@@ -185,32 +175,32 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
 #pragma unroll
                     for (int j = 3; j >= 0; --j) {
                         const int i = 4 * half + j, t = t8 + i;
-                        const float2 x = s.sdt[t * kCh + ch];
+                        const float2 x = s.sdt[t * kCh + cp];
                         const float4 Bv = *reinterpret_cast<const float4*>(s.sB + t * kNp + 4 * q), Cv = *reinterpret_cast<const float4*>(s.sC + t * kNp + 4 * q);
-                        const F2 g2 = f2(s.sg[t * kCh + ch]), dt2 = f2(x.x), du2 = f2(x.x * x.y);
+                        const F2 g2 = f2(s.sg[t * kCh + cs]), dt2 = f2(x.x), du2 = f2(x.x * x.y);
                         const F2 G01 = fma(f2(Cv.x, Cv.y), g2, P01), G23 = fma(f2(Cv.z, Cv.w), g2, P23);
                         bg[j] = both(fma(G23, f2(Bv.z, Bv.w), mul(G01, f2(Bv.x, Bv.y))));
-                        const F2 n01 = mul(G01, fma(e01[i], h01[i], h01[i])), n23 = mul(G23, fma(e23[i], h23[i], h23[i]));
+                        const F2 n01 = mul(G01, ah01[i]), n23 = mul(G23, ah23[i]);
                         ag[j] = both(fma(n23, A23, mul(n01, A01)));
                         a01 = fma(dt2, n01, a01);
                         a23 = fma(dt2, n23, a23);
                         float v[8];
                         get(mul(G01, du2), v[0], v[1]);
                         get(mul(G23, du2), v[2], v[3]);
-                        get(mul(h01[i + 1], g2), v[4], v[5]);
-                        get(mul(h23[i + 1], g2), v[6], v[7]);
+                        get(mul(fma(du2, f2(Bv.x, Bv.y), ah01[i]), g2), v[4], v[5]);
+                        get(mul(fma(du2, f2(Bv.z, Bv.w), ah23[i]), g2), v[6], v[7]);
                         channel_sums8<LPC>(v, lane);
 #pragma unroll
                         for (int k = 0; k < kVals; ++k) s.red[warp][i][k * 32 + lane] = v[k];
-                        P01 = fma(e01[i], G01, G01);
-                        P23 = fma(e23[i], G23, G23);
+                        P01 = decayed(f01[i], G01);
+                        P23 = decayed(f23[i], G23);
                     }
                     const float b4 = lane_sums4<LPC>(bg, lane), a4 = lane_sums4<LPC>(ag, lane);
                     __syncwarp();  // every lane of the channel has read these tokens' dt, u and g
                     if (q < 4) {
                         const int t = t8 + 4 * half + q;
-                        s.sdt[t * kCh + ch] = make_float2(b4, a4 * 0.6931471805599453f);
-                        s.sg[t * kCh + ch] = ys[half];
+                        s.sdt[t * kCh + cp] = make_float2(b4, a4 * 0.6931471805599453f);
+                        s.sg[t * kCh + cs] = ys[half];
                     }
                 }
                 float x[4];
@@ -232,26 +222,36 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                 __syncthreads();
             }
         }
-        if constexpr (WALK) {
+        {
             if (l < last && at.left > 0) {
                 load();
                 Piece<T, V> du, dd, dzv;
+                float bg[V], ag[V], y[V], sz[V], step[V], slope[V];
+                get_pairs(s.sdt + at.row * kCh, at.c0, bg, ag);  // B.G, sum A G a h
+                get_singles(s.sg + at.row * kCh, at.c0, y);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float2 x = s.sdt[at.row * kCh + at.c0 + i];  // B.G, sum A G a h
-                    const float uf = to_f<T>(u.x[i]), gf = to_f<T>(go.x[i]), raw = to_f<T>(dt.x[i]) + bias[i];
-                    float y = s.sg[at.row * kCh + at.c0 + i], g = gf;
+                    step[i] = slope[i] = to_f<T>(dt.x[i]) + bias[i];
+                    sz[i] = to_f<T>(z.x[i]);
+                }
+                if (p.softplus) {
+                    softplus_all(step);
+                    sigmoid_all(slope);
+                }
+                if (p.z.p) sigmoid_all(sz);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float uf = to_f<T>(u.x[i]), gf = to_f<T>(go.x[i]);
+                    float g = gf;
                     if (p.z.p) {
-                        const float zf = to_f<T>(z.x[i]), sz = sigmoid(zf);
-                        y = fmaf(Dw[i], uf, y);
-                        dzv.x[i] = from_f<T>(live ? gf * y * sz * fmaf(zf, 1.f - sz, 1.f) : 0.f);
-                        g *= zf * sz;
+                        const float zf = to_f<T>(z.x[i]);
+                        dzv.x[i] = from_f<T>(live ? gf * fmaf(Dw[i], uf, y[i]) * sz[i] * fmaf(zf, 1.f - sz[i], 1.f) : 0.f);
+                        g *= zf * sz[i];
                     }
-                    const float step = p.softplus ? softplus(raw) : raw;
-                    float ddt = fmaf(uf, x.x, x.y);
-                    if (p.softplus) ddt *= sigmoid(raw);
+                    float ddt = fmaf(uf, bg[i], ag[i]);
+                    if (p.softplus) ddt *= slope[i];
                     if (!live) ddt = 0.f;
-                    du.x[i] = from_f<T>(live ? fmaf(step, x.x, Dw[i] * g) : 0.f);
+                    du.x[i] = from_f<T>(live ? fmaf(step[i], bg[i], Dw[i] * g) : 0.f);
                     dd.x[i] = from_f<T>(ddt);
                     if (live && i < at.left) {
                         add_exactly(dD[i], dD_rest[i], g * uf);
@@ -269,19 +269,6 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     get(P01, g[0], g[1]);
     get(P23, g[2], g[3]);
     float* rows = reinterpret_cast<float*>(s.sdt);  // [tile][channels]
-    if constexpr (!WALK) {
-        const int64_t to = ((int64_t)seg * p.B + at.b) * p.D;
-        if (in) *reinterpret_cast<float4*>(p.seg_h + (to + d) * kNp + 4 * q) = make_float4(g[0], g[1], g[2], g[3]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) rows[at.row * kCh + at.c0 + i] = dt_sum[i];
-        __syncthreads();
-        if (threadIdx.x < at.nch) {
-            float x = 0.f;
-            for (int r = 0; r < kSelTile; ++r) x += rows[r * kCh + threadIdx.x];
-            p.seg_dt[to + at.d0 + threadIdx.x] = x;
-        }
-        return;
-    }
     if (in && seg == 0 && p.dS_in)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -352,31 +339,13 @@ __global__ void __launch_bounds__(256) sel_sum_weights_kernel(const SelParams p,
     }
 }
 
-template <typename T, int LPC, bool WALK>
-cudaError_t launch_bwd_kernel(const SelParams& p, cudaStream_t st) {
-    constexpr size_t smem = sizeof(BwdSmem<T, LPC>);
-    if (smem > 48 * 1024) {
-        cudaError_t err = cudaFuncSetAttribute(sel_bwd_kernel<T, LPC, WALK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (err != cudaSuccess) return err;
-    }
-    const int kCh = kSelThreads / LPC;
-    const dim3 grid((unsigned)(p.B * p.G * ((p.Dg + kCh - 1) / kCh)), (unsigned)(WALK ? p.nseg : p.nseg - 1));
-    sel_bwd_kernel<T, LPC, WALK><<<grid, kSelThreads, smem, st>>>(p);
-    return cudaGetLastError();
-}
-
 template <typename T>
 cudaError_t launch_bwd(const SelParams& p, SelPass pass, cudaStream_t st) {
-    auto run = [&](auto lpc) {
+    return by_lanes(p.N, [&](auto lpc) {
         constexpr int LPC = decltype(lpc)::value;
-        return pass == kSelWalk ? launch_bwd_kernel<T, LPC, true>(p, st) : launch_bwd_kernel<T, LPC, false>(p, st);
-    };
-    switch (sel_lanes(p.N)) {
-        case 4: return run(std::integral_constant<int, 4>{});
-        case 8: return run(std::integral_constant<int, 8>{});
-        case 16: return run(std::integral_constant<int, 16>{});
-        default: return run(std::integral_constant<int, 32>{});
-    }
+        if (pass != kSelWalk) return launch_sel(sel_seg_kernel<T, LPC, true>, seg_smem<T, LPC>(), p, p.nseg - 1, st);
+        return launch_sel(sel_bwd_kernel<T, LPC>, sizeof(BwdSmem<T, LPC>), p, p.nseg, st);
+    });
 }
 
 template <typename T>

@@ -3,10 +3,10 @@
 // dt_t = softplus(raw_t + bias). A channel's states lie four to a lane on LPC lanes (4, 8, 16 or 32: up to 16, 32, 64, 128
 // states), so that B and C are read as 16-byte pieces that every channel of a warp shares, and y is a sum over LPC lanes.
 //
-// A step multiplies by a = exp(dt A). Rounded by itself an a near 1 is off by up to 2^-25 the same way at every token, and
-// the state remembers 1 / (1 - a) of them; so the step is h + (a - 1) h, with a - 1 = 2^y - 1 (y = dt A log2 e) from a
-// polynomial where |y| < 1/4 (Chebyshev fit of (2^y - 1) / y, 2e-8 off), and from the exponential unit beyond, where the
-// state remembers six tokens.
+// A step multiplies by a = exp(dt A) = 2^y. Rounded by itself an a near 1 is off by up to 2^-25 the same way at every token,
+// and the state remembers 1 / (1 - a) of them; so where |y| < 1/4 the step is h + (a - 1) h with a - 1 from a polynomial
+// (Chebyshev fit of (2^y - 1) / y, 2e-8 off). Beyond, where the state remembers six tokens, it is a h with a from the
+// exponential unit (1e-7 off), which a - 1 would leave no bits of a small a.
 #pragma once
 
 #include <type_traits>
@@ -55,31 +55,128 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr float kNear = 0.25f;
-// 2^y - 1.
-__device__ __forceinline__ F2 decay(F2 y) {
+// A step's factor: 2^y - 1 where y is near 0, 2^y beyond.
+struct Factor {
+    F2 c;
+    bool n0, n1;
+};
+__device__ __forceinline__ Factor factor(F2 y) {
     F2 p = fma(y, f2(0.0013347864f), f2(0.00963017f));
     p = fma(p, y, f2(0.055504076f));
     p = fma(p, y, f2(0.24022631f));
     p = fma(p, y, f2(0.6931472f));
     p = mul(p, y);
-    float y0, y1, p0, p1, e0, e1;
+    float y0, y1, p0, p1;
     get(y, y0, y1);
     get(p, p0, p1);
-    get(add(f2(ex2(y0), ex2(y1)), f2(-1.f)), e0, e1);
-    return f2(fabsf(y0) < kNear ? p0 : e0, fabsf(y1) < kNear ? p1 : e1);
+    Factor r;
+    r.n0 = fabsf(y0) < kNear;
+    r.n1 = fabsf(y1) < kNear;
+    const float e0 = ex2(y0), e1 = ex2(y1);
+    r.c = f2(r.n0 ? p0 : e0, r.n1 ? p1 : e1);
+    return r;
 }
-__device__ __forceinline__ float decay(float y) {
+// a h.
+__device__ __forceinline__ F2 decayed(const Factor& f, F2 h) {
+    float h0, h1;
+    get(h, h0, h1);
+    return fma(f.c, h, f2(f.n0 ? h0 : 0.f, f.n1 ? h1 : 0.f));
+}
+__device__ __forceinline__ float decayed(float y, float h) {
     float p = fmaf(y, 0.0013347864f, 0.00963017f);
     p = fmaf(p, y, 0.055504076f);
     p = fmaf(p, y, 0.24022631f);
     p = fmaf(p, y, 0.6931472f) * y;
-    return fabsf(y) < kNear ? p : ex2(y) - 1.f;
+    return fabsf(y) < kNear ? fmaf(p, h, h) : ex2(y) * h;
 }
 
-__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
+__device__ __forceinline__ float rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// exp(-|x|): the product with log2 e is carried to 48 bits, so that a far x costs no accuracy (3e-7 off at most).
+__device__ __forceinline__ float exp_neg(float x) {
+    const float a = -fabsf(x), t = a * 1.4426950408889634f;
+    const float rest = fmaf(a, 1.4426950408889634f, -t);
+    const float e = ex2(t);
+    return fmaf(e * 0.6931472f, fmaf(a, 1.925963033e-8f, rest), e);
+}
+// max(x, 0) + log(1 + exp(-|x|)); log(1 + e) / e by a Chebyshev fit of degree 8 on [0, 1] (3e-8 off), accurate for small e.
+__device__ __forceinline__ float softplus(float x) {
+    const float e = exp_neg(x);
+    float p = fmaf(e, 0.005253458f, -0.029588507f);
+    p = fmaf(p, e, 0.07836167f);
+    p = fmaf(p, e, -0.1367477f);
+    p = fmaf(p, e, 0.1911143f);
+    p = fmaf(p, e, -0.2484437f);
+    p = fmaf(p, e, 0.3331927f);
+    p = fmaf(p, e, -0.49999502f);
+    p = fmaf(p, e, 1.f);
+    return fmaf(p, e, fmaxf(x, 0.f));
+}
 __device__ __forceinline__ float sigmoid(float x) {  // from exp(-|x|), so that neither side overflows
-    const float e = expf(-fabsf(x)), r = __fdividef(1.f, 1.f + e);
+    const float e = exp_neg(x), r = rcp(1.f + e);
     return x >= 0.f ? r : e * r;
+}
+
+// The same for two.
+__device__ __forceinline__ F2 exp_neg(F2 x) {
+    float a, b;
+    get(x, a, b);
+    const F2 m = f2(-fabsf(a), -fabsf(b)), t = mul(m, f2(1.4426950408889634f));
+    F2 rest = fma(m, f2(1.4426950408889634f), mul(t, f2(-1.f)));
+    rest = fma(m, f2(1.925963033e-8f), rest);
+    get(t, a, b);
+    const F2 e = f2(ex2(a), ex2(b));
+    return fma(mul(e, f2(0.6931472f)), rest, e);
+}
+__device__ __forceinline__ F2 softplus(F2 x) {
+    const F2 e = exp_neg(x);
+    F2 p = fma(e, f2(0.005253458f), f2(-0.029588507f));
+    p = fma(p, e, f2(0.07836167f));
+    p = fma(p, e, f2(-0.1367477f));
+    p = fma(p, e, f2(0.1911143f));
+    p = fma(p, e, f2(-0.2484437f));
+    p = fma(p, e, f2(0.3331927f));
+    p = fma(p, e, f2(-0.49999502f));
+    p = fma(p, e, f2(1.f));
+    float a, b;
+    get(x, a, b);
+    return fma(p, e, f2(fmaxf(a, 0.f), fmaxf(b, 0.f)));
+}
+__device__ __forceinline__ F2 sigmoid(F2 x) {
+    const F2 e = exp_neg(x), n = add(e, f2(1.f));
+    float a, b, ea, eb, na, nb;
+    get(x, a, b);
+    get(e, ea, eb);
+    get(n, na, nb);
+    const F2 s = mul(f2(rcp(na), rcp(nb)), f2(a >= 0.f ? 1.f : ea, b >= 0.f ? 1.f : eb));
+    return s;
+}
+template <int V>
+__device__ __forceinline__ void softplus_all(float (&x)[V]) {
+    if constexpr (V == 1) {
+        x[0] = softplus(x[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) get(softplus(f2(x[i], x[i + 1])), x[i], x[i + 1]);
+    }
+}
+template <int V>
+__device__ __forceinline__ void sigmoid_all(float (&x)[V]) {
+    if constexpr (V == 1) {
+        x[0] = sigmoid(x[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) get(sigmoid(f2(x[i], x[i + 1])), x[i], x[i + 1]);
+    }
+}
+// s += x with what the sum's rounding leaves out kept in `rest`.
+__device__ __forceinline__ void add_exactly(float& s, float& rest, float x) {
+    const float t = __fadd_rn(s, x), z = __fsub_rn(t, s);
+    rest = __fadd_rn(rest, __fadd_rn(__fsub_rn(s, __fsub_rn(t, z)), __fsub_rn(x, z)));
+    s = t;
 }
 
 // Sums v[0..3] over the LPC lanes of a channel: lane q of them (q < 4) has the sum of v[q].
@@ -145,6 +242,89 @@ struct Piece {
 template <int B>
 __host__ __device__ constexpr int need_vec() {
     return B > 16 ? 16 : B;
+}
+
+// One such piece from global into shared memory, by the thread that reads it there: asynchronously where `vec` bytes allow it.
+template <typename T, int V>
+__device__ __forceinline__ void fetch(T* to, const T* from, int n, bool vec) {
+    constexpr int kB = V * (int)sizeof(T);
+    if constexpr (kB >= 4) {
+        if (vec && n >= V) {
+            const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+            if constexpr (kB >= 16) {
+#pragma unroll
+                for (int i = 0; i < kB; i += 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i), "l"(reinterpret_cast<const char*>(from) + i) : "memory");
+            } else {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(kB) : "memory");
+            }
+            return;
+        }
+    }
+    Piece<T, V> x;
+    x.load(from, n, vec);
+    x.store(to, V, false);
+}
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Places of channel c in a tile's row of pairs and of single values: 16-byte units, permuted so that the eight threads that
+// stage a row, V channels each, write and read without bank conflicts (a thread's channels lie V apart from its neighbour's).
+__device__ __forceinline__ int pair_at(int c) {
+    const int u = c >> 1;
+    return (u ^ ((u >> 3) & 3)) * 2 + (c & 1);
+}
+__device__ __forceinline__ int single_at(int c) {
+    const int u = c >> 2;
+    return (u ^ ((u >> 3) & 1)) * 4 + (c & 3);
+}
+template <int V>
+__device__ __forceinline__ void put_pairs(float2* row, int c0, const float (&a)[V], const float (&b)[V]) {
+    if constexpr (V == 1) {
+        row[pair_at(c0)] = make_float2(a[0], b[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) *reinterpret_cast<float4*>(row + pair_at(c0 + i)) = make_float4(a[i], b[i], a[i + 1], b[i + 1]);
+    }
+}
+template <int V>
+__device__ __forceinline__ void get_pairs(const float2* row, int c0, float (&a)[V], float (&b)[V]) {
+    if constexpr (V == 1) {
+        const float2 x = row[pair_at(c0)];
+        a[0] = x.x, b[0] = x.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float4 x = *reinterpret_cast<const float4*>(row + pair_at(c0 + i));
+            a[i] = x.x, b[i] = x.y, a[i + 1] = x.z, b[i + 1] = x.w;
+        }
+    }
+}
+template <int V>
+__device__ __forceinline__ void put_singles(float* row, int c0, const float (&a)[V]) {
+    if constexpr (V == 1) {
+        row[single_at(c0)] = a[0];
+    } else if constexpr (V == 2) {
+        *reinterpret_cast<float2*>(row + single_at(c0)) = make_float2(a[0], a[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(row + single_at(c0 + i)) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+    }
+}
+template <int V>
+__device__ __forceinline__ void get_singles(const float* row, int c0, float (&a)[V]) {
+    if constexpr (V == 1) {
+        a[0] = row[single_at(c0)];
+    } else if constexpr (V == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(row + single_at(c0));
+        a[0] = x.x, a[1] = x.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(row + single_at(c0 + i));
+            a[i] = x.x, a[i + 1] = x.y, a[i + 2] = x.z, a[i + 3] = x.w;
+        }
+    }
 }
 
 // Which channels and tokens a CTA has, and what of it a thread stages: row `row` of a tile, V channels from `c0`.
