@@ -52,6 +52,7 @@ constexpr int kSelTile = 32;    // tokens that a CTA holds in shared memory
 constexpr int kSelKeep = 8;     // tokens between two kept states
 constexpr int kSelThreads = 256;
 constexpr int kSelMaxN = 128;
+constexpr int kSelResident = 4;  // CTAs of the walk that an SM holds (up to 32 states a channel; 2 above)
 // Lanes of a channel, four states each.
 inline int sel_lanes(int N) { return N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32; }
 inline int sel_channels(int N) { return kSelThreads / sel_lanes(N); }  // channels of a CTA

@@ -92,21 +92,25 @@ int check_sel(const subq_selective_desc& d, SelParams& p) {
     return SUBQ_OK;
 }
 
-// Segments of a sequence that are walked side by side where there are few channels.
+// Segments of a sequence that are walked side by side. The walk is bound by instruction issue: an SM with c CTAs takes c times
+// a CTA's time (at least 1.6 times: fewer warps than that leave it waiting), so what counts is how evenly the grid fills the
+// SMs. A segment costs `first` of the walk again for its sum in the launch before, 4 us for that launch, and a step of the
+// chain in front of the walk. In units of a CTA's 32 tokens, which take `tile` us when the SM is full; the least sum wins.
+// us, bf16, D = 1536, N = 16, one segment and as chosen:
+//   SPLIT_FIGURES
 void sel_split(SelParams& p, bool back) {
-    const int64_t ch = sel_channels(p.N), ctas = (int64_t)p.B * p.G * ((p.Dg + ch - 1) / ch);
-#ifndef SEL_SLOTS
-#define SEL_SLOTS 444
-#endif
-#ifndef SEL_MUL
-#define SEL_MUL 2
-#endif
-    const int64_t slots = back ? 296 : SEL_SLOTS, tiles = (p.L + kSelTile - 1) / kSelTile;
-    if (ctas <= 0 || SEL_MUL * ctas > slots || tiles < 8) return;
-    int64_t g = std::min<int64_t>(slots / ctas, tiles / 4);
-    const int64_t per = (tiles + g - 1) / g;
-    p.seg_tokens = (int)(per * kSelTile);
-    p.nseg = (int)((tiles + per - 1) / per);
+    const int64_t ch = sel_channels(p.N), ctas = (int64_t)p.B * p.G * ((p.Dg + ch - 1) / ch), tiles = (p.L + kSelTile - 1) / kSelTile;
+    if (ctas <= 0 || tiles <= 0) return;
+    const double tile = back ? 8.5 : 3.3, first = back ? 0.2 : 0.4;
+    auto full = [](int64_t n) { return std::max<double>(1.6, (double)((n + 147) / 148)); };
+    double best = 1e30;
+    for (int64_t g = 1; g <= 256 && (g == 1 || 4 * g <= tiles); ++g) {
+        const int64_t per = (tiles + g - 1) / g;
+        if ((tiles + per - 1) / per != g) continue;  // (the same split with fewer segments)
+        double t = (double)per * full(ctas * g) * tile;
+        if (g > 1) t += (double)per * full(ctas * (g - 1)) * tile * first + 4.0 + 0.15 * (double)g;
+        if (t < best) best = t, p.nseg = (int)g, p.seg_tokens = (int)(per * kSelTile);
+    }
 }
 
 size_t np_of(const SelParams& p) { return 4 * (size_t)sel_lanes(p.N); }

@@ -196,7 +196,7 @@ __device__ __forceinline__ float lane_sums4(const float (&v)[4], int lane) {
 // V consecutive elements of a row in one access where `vec` bytes allow it.
 template <typename T, int V>
 struct Piece {
-    T x[V];
+    alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) T x[V];
     __device__ __forceinline__ void load(const T* at, int n, bool vec) {
         constexpr int kB = V * (int)sizeof(T);
         if (vec && n >= V) {
@@ -356,22 +356,29 @@ __device__ __forceinline__ bool live_at(const SelParams& p, int b, int l) {
     return l < p.L && (!p.mask || p.mask[(int64_t)b * p.mask_sb + l]);
 }
 
-// A tile's rows of B or C as float32, zeros on masked tokens, behind the last token and behind the N-th state.
+// A tile's rows of B or C as float32, zeros on masked tokens, behind the last token and behind the N-th state: four
+// neighbouring states of a token for each of the first (or every) 8 LPC x 32 / 8 threads.
 template <typename T, int LPC>
 struct States {
-    static constexpr int kNp = 4 * LPC, kPer = kSelTile * kNp / kSelThreads;
-    T x[kPer];
+    static constexpr int kNp = 4 * LPC, kPieces = kSelTile * LPC, kPer = (kPieces + kSelThreads - 1) / kSelThreads;
+    Piece<T, 4> x[kPer];
     __device__ __forceinline__ void load(const SelParams& p, const SelTensor& t, int b, int g, int l0, int l1) {
+        const bool vec = t.vec >= 4 * (int)sizeof(T) && (t.sg * (int64_t)sizeof(T)) % (4 * sizeof(T)) == 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int at = threadIdx.x + i * kSelThreads, l = l0 + at / kNp, n = at % kNp;
-            const bool in = n < p.N && l < l1 && live_at<T>(p, b, l);
-            x[i] = in ? (static_cast<const T*>(t.p) + b * t.sb + l * t.sl + g * t.sg)[n] : from_f<T>(0.f);
+            const int at = threadIdx.x + i * kSelThreads, l = l0 + at / LPC, n = at % LPC * 4;
+            x[i].zero();
+            if ((kPieces % kSelThreads == 0 || at < kPieces) && n < p.N && l < l1 && live_at<T>(p, b, l))
+                x[i].load(static_cast<const T*>(t.p) + b * t.sb + l * t.sl + g * t.sg + n, p.N - n, vec);
         }
     }
     __device__ __forceinline__ void put(float* to) const {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) to[threadIdx.x + i * kSelThreads] = to_f<T>(x[i]);
+        for (int i = 0; i < kPer; ++i) {
+            const int at = threadIdx.x + i * kSelThreads;
+            if (kPieces % kSelThreads == 0 || at < kPieces)
+                *reinterpret_cast<float4*>(to + 4 * at) = make_float4(to_f<T>(x[i].x[0]), to_f<T>(x[i].x[1]), to_f<T>(x[i].x[2]), to_f<T>(x[i].x[3]));
+        }
     }
 };
 

@@ -36,16 +36,10 @@ __device__ __forceinline__ void load_A(const SelParams& p, int d, bool in, int q
     for (int i = 0; i < 4; ++i) A2[i] = in && 4 * q + i < p.N ? p.A[(int64_t)d * p.N + 4 * q + i] * kLog2e : 0.f;
 }
 
-#ifndef SEL_CTAS
-#define SEL_CTAS 3
-#endif
-#ifndef SEL_UNROLL
-#define SEL_UNROLL 2
-#endif
 template <typename T, int LPC, bool OUTS>
-__global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? SEL_CTAS : 2) sel_fwd_kernel(const SelParams p) {
+__global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? kSelResident : 2) sel_fwd_kernel(const SelParams p) {
     using P = Place<T, LPC>;
-    constexpr int kNp = 4 * LPC, V = P::kV, kCh = P::kCh, kUnroll = SEL_UNROLL;
+    constexpr int kNp = 4 * LPC, V = P::kV, kCh = P::kCh;
     extern __shared__ __align__(16) unsigned char smem[];
     float2* sdt = reinterpret_cast<float2*>(smem);                      // [tile][channels]: dt, dt u; then y
     float* sB = reinterpret_cast<float*>(sdt + kSelTile * kCh);         // [tile][states]
@@ -118,7 +112,7 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? SEL_CTAS : 2) sel_fwd_
         if (outs) Cs.put(sC);
         if (l0 + kSelTile < last) load(l0 + kSelTile, turn ^ 1);
         __syncthreads();
-#pragma unroll kUnroll
+#pragma unroll 2
         for (int t4 = 0; t4 < kSelTile; t4 += 4) {
             if (p.kept && t4 % kSelKeep == 0 && in && l0 + t4 < p.L) {
                 float4 x;
