@@ -50,23 +50,59 @@ __device__ __forceinline__ void chain_back(const SelParams& p, int seg, int b, i
 template <typename T, int LPC>
 struct BwdSmem {
     static constexpr int kCh = kSelThreads / LPC, kNp = 4 * LPC, kWarps = kSelThreads / 32, kVals = LPC / 4;
-    float2 sdt[kSelTile * kCh];  // dt, u; then B.G and sum A G a h
-    float sg[kSelTile * kCh];    // g; then y
+    float2 sdt[kSelTile * kCh];    // dt, u; then du, d raw
+    float sg[kSelTile * kCh];      // g; then dz
+    float sgz[kSelTile * kCh];     // dout silu'(z)
+    float slope[kSelTile * kCh];   // d dt / d raw
     float sB[kSelTile * kNp], sC[kSelTile * kNp];
+    float sbias[kCh];
     float red[kWarps][kSelKeep][32 * kVals];
+    float4 kept[kSelTile / kSelKeep][kSelThreads];           // a thread's own: the states before every eighth token
+    alignas(16) T raw[4][kSelTile * kCh];  // a thread's own pieces of u, dt, z, dout of the next tile
 };
 
 template <typename T, int LPC>
 __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(const SelParams p) {
     using P = Place<T, LPC>;
     using S = BwdSmem<T, LPC>;
-    constexpr int kNp = 4 * LPC, V = P::kV, kCh = P::kCh, kCPW = 32 / LPC, kVals = S::kVals;
+    constexpr int kNp = 4 * LPC, V = P::kV, kCh = P::kCh, kVals = S::kVals;
     extern __shared__ __align__(16) unsigned char smem[];
     S& s = *reinterpret_cast<S*>(smem);
     const P at(p);
     const int seg = blockIdx.y, first = seg * p.seg_tokens, last = min(p.L, first + p.seg_tokens);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & (LPC - 1), ch = threadIdx.x / LPC, cp = pair_at(ch), cs = single_at(ch), d = at.d0 + ch;
     const bool in = ch < at.nch;
+    constexpr int kBytes = need_vec<V * (int)sizeof(T)>();
+    const bool even = at.d0 % V == 0;
+    const bool vu = even && p.u.vec >= kBytes, vd = even && p.dt.vec >= kBytes, vz = even && p.z.vec >= kBytes, vg = even && p.dout.vec >= kBytes;
+    const bool vdu = even && p.du.vec >= kBytes, vdd = even && p.ddt.vec >= kBytes, vdz = even && p.dz.vec >= kBytes;
+    const int64_t keeps = (p.L + kSelKeep - 1) / kSelKeep;
+    const int turn = threadIdx.x * V;
+    auto fetch_rows = [&](int l0) {
+        const int l = l0 + at.row;
+        if (l < last && at.left > 0) {  // (a masked token's piece is fetched, but not used)
+            fetch<T, V>(s.raw[0] + turn, row_of<T>(p.u, at.b, l, at.d0 + at.c0), at.left, vu);
+            fetch<T, V>(s.raw[1] + turn, row_of<T>(p.dt, at.b, l, at.d0 + at.c0), at.left, vd);
+            if (p.z.p) fetch<T, V>(s.raw[2] + turn, row_of<T>(p.z, at.b, l, at.d0 + at.c0), at.left, vz);
+            fetch<T, V>(s.raw[3] + turn, row_of<T>(p.dout, at.b, l, at.d0 + at.c0), at.left, vg);
+        }
+    };
+    auto fetch_kept = [&](int l) {  // l: a multiple of kSelKeep
+        if (in && l < last)
+            fetch<float, 4>(reinterpret_cast<float*>(&s.kept[l / kSelKeep % (kSelTile / kSelKeep)][threadIdx.x]),
+                            p.kept + (((int64_t)at.b * keeps + l / kSelKeep) * p.D + d) * kNp + 4 * q, 4, true);
+    };
+    States<T, LPC> Bs, Cs;
+    auto load_states = [&](int l0) {
+        Bs.load(p, p.Bm, at.b, at.g, l0, last);
+        Cs.load(p, p.C, at.b, at.g, l0, last);
+    };
+    const int top = first + (last - 1 - first) / kSelTile * kSelTile;
+    fetch_rows(top);
+    for (int t8 = 0; t8 < kSelTile; t8 += kSelKeep) fetch_kept(top + t8);
+    fetch_commit();
+    load_states(top);
+    for (int i = threadIdx.x; i < kCh; i += kSelThreads) s.sbias[i] = i < at.nch && p.dt_bias ? p.dt_bias[at.d0 + i] : 0.f;
     float A2[4], g0[4] = {0.f, 0.f, 0.f, 0.f};
     load_A<LPC>(p, d, in, q, A2);
     const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
@@ -78,74 +114,75 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
         chain_back<LPC>(p, seg, at.b, d, q, A2, g0);
     }
     F2 P01 = f2(g0[0], g0[1]), P23 = f2(g0[2], g0[3]);  // a_{t+1} G_{t+1}
-    float bias[V], Dw[V], dD[V], dD_rest[V], db[V], db_rest[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const bool has = i < at.left;
-        bias[i] = has && p.dt_bias ? p.dt_bias[at.d0 + at.c0 + i] : 0.f;
-        Dw[i] = has && p.Dw ? p.Dw[at.d0 + at.c0 + i] : 0.f;
-        dD[i] = dD_rest[i] = db[i] = db_rest[i] = 0.f;
-    }
+    const float Dw = in && p.Dw ? p.Dw[d] : 0.f;
+    // the lane's sums over its tokens (q, q + 4, ...), and its states' over all of them
+    float dD = 0.f, dD_rest = 0.f, db = 0.f, db_rest = 0.f;
     float dA[4] = {0.f, 0.f, 0.f, 0.f}, dA_rest[4] = {0.f, 0.f, 0.f, 0.f};
-    constexpr int kBytes = need_vec<V * (int)sizeof(T)>();
-    const bool even = at.d0 % V == 0;
-    const bool vu = even && p.u.vec >= kBytes, vd = even && p.dt.vec >= kBytes, vz = even && p.z.vec >= kBytes, vg = even && p.dout.vec >= kBytes;
-    const bool vdu = even && p.du.vec >= kBytes, vdd = even && p.ddt.vec >= kBytes, vdz = even && p.dz.vec >= kBytes;
-    const int64_t keeps = (p.L + kSelKeep - 1) / kSelKeep;
-    for (int l0 = first + (last - 1 - first) / kSelTile * kSelTile; l0 >= first; l0 -= kSelTile) {
-        Piece<T, V> u, dt, z, go;
+    __syncthreads();
+    for (int l0 = top; l0 >= first; l0 -= kSelTile) {
         const int l = l0 + at.row;
         const bool live = l < last && live_at<T>(p, at.b, l);
-        auto load = [&]() {
-            u.zero(); dt.zero(); z.zero(); go.zero();
-            if (live) {
-                u.load(row_of<T>(p.u, at.b, l, at.d0 + at.c0), at.left, vu);
-                dt.load(row_of<T>(p.dt, at.b, l, at.d0 + at.c0), at.left, vd);
-                if (p.z.p) z.load(row_of<T>(p.z, at.b, l, at.d0 + at.c0), at.left, vz);
-                go.load(row_of<T>(p.dout, at.b, l, at.d0 + at.c0), at.left, vg);
-            }
-        };
-        load();
+        fetch_wait<0>();
         {
-            float x[V], g[V], uf[V];
+            Piece<T, V> u, dt, z, go;
+            u.load(s.raw[0] + turn, V, true);
+            dt.load(s.raw[1] + turn, V, true);
+            go.load(s.raw[3] + turn, V, true);
+            float x[V], g[V], uf[V], sl[V], gz[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                x[i] = to_f<T>(dt.x[i]) + bias[i];
-                g[i] = to_f<T>(z.x[i]);
-                uf[i] = to_f<T>(u.x[i]);
+                x[i] = to_f<T>(dt.x[i]) + s.sbias[at.c0 + i];
+                g[i] = to_f<T>(go.x[i]);
+                gz[i] = 0.f;
+                sl[i] = 1.f;
             }
-            if (p.softplus) softplus_all(x);
-            if (p.z.p) sigmoid_all(g);
+            if (p.softplus) softplus_slope_all(x, sl);
+            if (p.z.p) {
+                z.load(s.raw[2] + turn, V, true);
+#pragma unroll
+                for (int i = 0; i < V; ++i) gz[i] = to_f<T>(z.x[i]);
+                sigmoid_all(gz);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float zf = to_f<T>(z.x[i]), gs = g[i] * gz[i];
+                    gz[i] = gs * fmaf(zf, 1.f - gz[i], 1.f);
+                    g[i] = gs * zf;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                if (!live || i >= at.left) x[i] = 0.f;
-                g[i] = p.z.p ? to_f<T>(go.x[i]) * (to_f<T>(z.x[i]) * g[i]) : to_f<T>(go.x[i]);
+                const bool has = live && i < at.left;
+                x[i] = has ? x[i] : 0.f;
+                uf[i] = has ? to_f<T>(u.x[i]) : 0.f;
+                g[i] = has ? g[i] : 0.f;
+                gz[i] = has ? gz[i] : 0.f;
+                sl[i] = has ? sl[i] : 0.f;
             }
             put_pairs(s.sdt + at.row * kCh, at.c0, x, uf);
             put_singles(s.sg + at.row * kCh, at.c0, g);
+            put_singles(s.sgz + at.row * kCh, at.c0, gz);
+            put_singles(s.slope + at.row * kCh, at.c0, sl);
         }
-        {
-            States<T, LPC> x;
-            x.load(p, p.Bm, at.b, at.g, l0, last);
-            x.put(s.sB);
-            x.load(p, p.C, at.b, at.g, l0, last);
-            x.put(s.sC);
+        Bs.put(s.sB);
+        Cs.put(s.sC);
+        const bool more = l0 > first;
+        if (more) {
+            fetch_rows(l0 - kSelTile);
+            load_states(l0 - kSelTile);
         }
         __syncthreads();
 #pragma unroll 1
         for (int t8 = kSelTile - kSelKeep; t8 >= 0; t8 -= kSelKeep) {
-            if (l0 + t8 >= last) continue;  // (every token there is behind the end: nothing of the adjoint changes)
-            {
+            if (l0 + t8 < last) {  // (else every token there is behind the end: nothing of the adjoint changes)
                 Factor f01[kSelKeep], f23[kSelKeep];
                 F2 ah01[kSelKeep], ah23[kSelKeep];  // a_t h_{t-1}
-                F2 h01, h23;
-                {
-                    const float4 x = in ? *reinterpret_cast<const float4*>(p.kept + (((int64_t)at.b * keeps + (l0 + t8) / kSelKeep) * p.D + d) * kNp + 4 * q)
-                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+                F2 h01 = f2(0.f), h23 = f2(0.f);
+                if (in) {
+                    const float4 x = s.kept[t8 / kSelKeep][threadIdx.x];
                     h01 = f2(x.x, x.y);
                     h23 = f2(x.z, x.w);
                 }
-                float ys[2];  // y of tokens q and 4 + q
+                float ys[2] = {0.f, 0.f};  // y of tokens q and 4 + q
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     float y[4];
@@ -169,6 +206,7 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                     if (p.z.p) ys[half] = lane_sums4<LPC>(y, lane);
                 }
                 F2 a01 = f2(0.f), a23 = f2(0.f);
+                float gu = 0.f, dr = 0.f;
 #pragma unroll
                 for (int half = 1; half >= 0; --half) {
                     float bg[4], ag[4];
@@ -197,12 +235,19 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                     }
                     const float b4 = lane_sums4<LPC>(bg, lane), a4 = lane_sums4<LPC>(ag, lane);
                     __syncwarp();  // every lane of the channel has read these tokens' dt, u and g
-                    if (q < 4) {
+                    if (q < 4) {   // what is left of token q of the four
                         const int t = t8 + 4 * half + q;
-                        s.sdt[t * kCh + cp] = make_float2(b4, a4 * 0.6931471805599453f);
-                        s.sg[t * kCh + cs] = ys[half];
+                        const float2 x = s.sdt[t * kCh + cp];
+                        const float g = s.sg[t * kCh + cs];
+                        const float ddt = fmaf(x.y, b4, a4 * 0.6931471805599453f) * s.slope[t * kCh + cs];
+                        s.sdt[t * kCh + cp] = make_float2(fmaf(x.x, b4, Dw * g), ddt);
+                        s.sg[t * kCh + cs] = s.sgz[t * kCh + cs] * fmaf(Dw, x.y, ys[half]);
+                        gu = fmaf(g, x.y, gu);
+                        dr += ddt;
                     }
                 }
+                add_exactly(dD, dD_rest, gu);
+                add_exactly(db, db_rest, dr);
                 float x[4];
                 get(a01, x[0], x[1]);
                 get(a23, x[2], x[3]);
@@ -221,46 +266,25 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                 }
                 __syncthreads();
             }
+            if (more) fetch_kept(l0 - kSelTile + t8);
         }
-        {
-            if (l < last && at.left > 0) {
-                load();
-                Piece<T, V> du, dd, dzv;
-                float bg[V], ag[V], y[V], sz[V], step[V], slope[V];
-                get_pairs(s.sdt + at.row * kCh, at.c0, bg, ag);  // B.G, sum A G a h
-                get_singles(s.sg + at.row * kCh, at.c0, y);
+        fetch_commit();
+        if (l < last && at.left > 0) {
+            float a[V], b[V];
+            Piece<T, V> du, dd, dz;
+            get_pairs(s.sdt + at.row * kCh, at.c0, a, b);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    step[i] = slope[i] = to_f<T>(dt.x[i]) + bias[i];
-                    sz[i] = to_f<T>(z.x[i]);
-                }
-                if (p.softplus) {
-                    softplus_all(step);
-                    sigmoid_all(slope);
-                }
-                if (p.z.p) sigmoid_all(sz);
+            for (int i = 0; i < V; ++i) {
+                du.x[i] = from_f<T>(a[i]);
+                dd.x[i] = from_f<T>(b[i]);
+            }
+            du.store(const_cast<T*>(row_of<T>(p.du, at.b, l, at.d0 + at.c0)), at.left, vdu);
+            dd.store(const_cast<T*>(row_of<T>(p.ddt, at.b, l, at.d0 + at.c0)), at.left, vdd);
+            if (p.z.p) {
+                get_singles(s.sg + at.row * kCh, at.c0, a);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float uf = to_f<T>(u.x[i]), gf = to_f<T>(go.x[i]);
-                    float g = gf;
-                    if (p.z.p) {
-                        const float zf = to_f<T>(z.x[i]);
-                        dzv.x[i] = from_f<T>(live ? gf * fmaf(Dw[i], uf, y[i]) * sz[i] * fmaf(zf, 1.f - sz[i], 1.f) : 0.f);
-                        g *= zf * sz[i];
-                    }
-                    float ddt = fmaf(uf, bg[i], ag[i]);
-                    if (p.softplus) ddt *= slope[i];
-                    if (!live) ddt = 0.f;
-                    du.x[i] = from_f<T>(live ? fmaf(step[i], bg[i], Dw[i] * g) : 0.f);
-                    dd.x[i] = from_f<T>(ddt);
-                    if (live && i < at.left) {
-                        add_exactly(dD[i], dD_rest[i], g * uf);
-                        add_exactly(db[i], db_rest[i], ddt);
-                    }
-                }
-                du.store(const_cast<T*>(row_of<T>(p.du, at.b, l, at.d0 + at.c0)), at.left, vdu);
-                dd.store(const_cast<T*>(row_of<T>(p.ddt, at.b, l, at.d0 + at.c0)), at.left, vdd);
-                if (p.z.p) dzv.store(const_cast<T*>(row_of<T>(p.dz, at.b, l, at.d0 + at.c0)), at.left, vdz);
+                for (int i = 0; i < V; ++i) dz.x[i] = from_f<T>(a[i]);
+                dz.store(const_cast<T*>(row_of<T>(p.dz, at.b, l, at.d0 + at.c0)), at.left, vdz);
             }
         }
         __syncthreads();  // the next tile takes the place of this one
@@ -268,7 +292,6 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     float g[4];
     get(P01, g[0], g[1]);
     get(P23, g[2], g[3]);
-    float* rows = reinterpret_cast<float*>(s.sdt);  // [tile][channels]
     if (in && seg == 0 && p.dS_in)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -277,21 +300,12 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     if (in)
         *reinterpret_cast<float4*>(p.part_a + (part * p.D + d) * kNp + 4 * q) =
             make_float4(dA[0] + dA_rest[0], dA[1] + dA_rest[1], dA[2] + dA_rest[2], dA[3] + dA_rest[3]);
-    float* rows2 = rows + kSelTile * kCh;
+    float sums[2] = {q < 4 ? dD + dD_rest : 0.f, q < 4 ? db + db_rest : 0.f};
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        rows[at.row * kCh + at.c0 + i] = dD[i] + dD_rest[i];
-        rows2[at.row * kCh + at.c0 + i] = db[i] + db_rest[i];
-    }
-    __syncthreads();
-    if (threadIdx.x < 2 * kCh) {
-        const int which = threadIdx.x / kCh, c = threadIdx.x % kCh;
-        if (c < at.nch) {
-            float x = 0.f, rest = 0.f;
-            for (int r = 0; r < kSelTile; ++r) add_exactly(x, rest, (which ? rows2 : rows)[r * kCh + c]);
-            p.part_d[(part * 2 + which) * p.D + at.d0 + c] = x + rest;
-        }
-    }
+    for (int o = 1; o < LPC; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], o);
+    if (in && q < 2) p.part_d[(part * 2 + q) * p.D + d] = sums[q];
 }
 
 // dB and dC: the parts of a group's channel blocks, added in order.

@@ -172,6 +172,14 @@ __device__ __forceinline__ void sigmoid_all(float (&x)[V]) {
         for (int i = 0; i < V; i += 2) get(sigmoid(f2(x[i], x[i + 1])), x[i], x[i + 1]);
     }
 }
+// x becomes softplus(x), `slope` its derivative sigmoid(x).
+template <int V>
+__device__ __forceinline__ void softplus_slope_all(float (&x)[V], float (&slope)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) slope[i] = x[i];
+    softplus_all(x);
+    sigmoid_all(slope);
+}
 // s += x with what the sum's rounding leaves out kept in `rest`.
 __device__ __forceinline__ void add_exactly(float& s, float& rest, float x) {
     const float t = __fadd_rn(s, x), z = __fsub_rn(t, s);
