@@ -7,7 +7,7 @@
 // One CTA walks its channels' tiles of 32 tokens from the last to the first. The forward left the state before every
 // eighth token; from it eight tokens' a h and factors are formed forwards in registers and used up backwards, so that each
 // exponential is formed once. dB and dC are sums over channels: over a warp's by shuffles that halve the values at each
-// step, over the CTA's warps in shared memory, over CTAs by a second launch, all in a fixed order. Sums over tokens (dA, dD,
+// step (lanes hold their states in an order by which nothing has to be selected), over the CTA's warps in shared memory, over CTAs by a second launch, all in a fixed order. Sums over tokens (dA, dD,
 // dbias) are added per eight tokens or tile with their rounding kept (two float32 a sum). Segments as in the forward.
 //
 // Bound by instruction issue.
@@ -18,17 +18,62 @@
 namespace subq {
 namespace sel {
 
-// Sums v[0..7] over the 32 / LPC channels of a warp: the lane of channel c is left with the values [c * LPC / 4, ...).
+// The order in which a lane holds its four states, n ^ order: lanes of channels with the upper bits set hold them swapped, so
+// that in the sums over channels every lane keeps its first registers and gives its last ones, with nothing to select.
 template <int LPC>
-__device__ __forceinline__ void channel_sums8(float (&v)[8], int lane) {
+__device__ __forceinline__ int state_order(int lane) {
+    return (LPC <= 16 && (lane & 16) ? 2 : 0) | (LPC <= 8 && (lane & 8) ? 1 : 0);
+}
+__device__ __forceinline__ void reorder(float (&x)[4], int order) {
+    const float a[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-    for (int o = 16, n = 8; o >= LPC; o >>= 1, n >>= 1) {
-        const bool up = lane & o;
+    for (int i = 0; i < 4; ++i) {
+        const float lo = order & 1 ? a[i ^ 1] : a[i], hi = order & 1 ? a[i ^ 3] : a[i ^ 2];
+        x[i] = order & 2 ? hi : lo;
+    }
+}
+// Sums of dB (b) and dC (c) over the 32 / LPC channels of a warp. out: LPC / 4 values of this lane (channel_value names them).
+template <int LPC>
+__device__ __forceinline__ void channel_sums(F2 b01, F2 b23, F2 c01, F2 c23, int lane, float (&out)[LPC / 4]) {
+    float b[4], c[4];
+    get(b01, b[0], b[1]);
+    get(b23, b[2], b[3]);
+    get(c01, c[0], c[1]);
+    get(c23, c[2], c[3]);
+    if constexpr (LPC <= 16) {
 #pragma unroll
-        for (int i = 0; i < n / 2; ++i) {
-            const float keep = up ? v[i + n / 2] : v[i], give = up ? v[i] : v[i + n / 2];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        for (int i = 0; i < 2; ++i) {
+            b[i] += __shfl_xor_sync(0xffffffffu, b[i + 2], 16);
+            c[i] += __shfl_xor_sync(0xffffffffu, c[i + 2], 16);
         }
+    }
+    if constexpr (LPC <= 8) {
+        b[0] += __shfl_xor_sync(0xffffffffu, b[1], 8);
+        c[0] += __shfl_xor_sync(0xffffffffu, c[1], 8);
+    }
+    if constexpr (LPC == 4) {
+        const bool up = lane & 4;
+        out[0] = (up ? c[0] : b[0]) + __shfl_xor_sync(0xffffffffu, up ? b[0] : c[0], 4);
+    } else {
+        constexpr int n = LPC / 8;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            out[i] = b[i];
+            out[n + i] = c[i];
+        }
+    }
+}
+// What value k of lane ln is: state n of dB (false) or dC (true).
+template <int LPC>
+__device__ __forceinline__ bool channel_value(int ln, int k, int& n) {
+    const int quad = 4 * (ln & (LPC - 1));
+    if constexpr (LPC == 4) {
+        n = quad + state_order<LPC>(ln);
+        return ln & 4;
+    } else {
+        constexpr int per = LPC / 8;
+        n = quad + ((k % per) ^ state_order<LPC>(ln));
+        return k >= per;
     }
 }
 
@@ -54,7 +99,8 @@ struct BwdSmem {
     float sg[kSelTile * kCh];      // g; then dz
     float sgz[kSelTile * kCh];     // dout silu'(z)
     float slope[kSelTile * kCh];   // d dt / d raw
-    float sB[kSelTile * kNp], sC[kSelTile * kNp];
+    static constexpr int kOrders = LPC <= 8 ? 4 : LPC == 16 ? 2 : 1;  // copies of B and C, one for each order of a lane's states
+    float sB[kOrders][kSelTile * kNp], sC[kOrders][kSelTile * kNp];
     float sbias[kCh];
     float red[kWarps][kSelKeep][32 * kVals];
     float4 kept[kSelTile / kSelKeep][kSelThreads];           // a thread's own: the states before every eighth token
@@ -105,7 +151,6 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     for (int i = threadIdx.x; i < kCh; i += kSelThreads) s.sbias[i] = i < at.nch && p.dt_bias ? p.dt_bias[at.d0 + i] : 0.f;
     float A2[4], g0[4] = {0.f, 0.f, 0.f, 0.f};
     load_A<LPC>(p, d, in, q, A2);
-    const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
     if (in) {
         if (p.dS_out)
 #pragma unroll
@@ -113,6 +158,12 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                 if (4 * q + i < p.N) g0[i] = p.dS_out[((int64_t)at.b * p.D + d) * p.N + 4 * q + i];
         chain_back<LPC>(p, seg, at.b, d, q, A2, g0);
     }
+    const int order = state_order<LPC>(lane);
+    reorder(A2, order);
+    reorder(g0, order);
+    const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
+    const float* myB = s.sB[S::kOrders == 2 ? order / 2 : order] + 4 * q;
+    const float* myC = s.sC[S::kOrders == 2 ? order / 2 : order] + 4 * q;
     F2 P01 = f2(g0[0], g0[1]), P23 = f2(g0[2], g0[3]);  // a_{t+1} G_{t+1}
     const float Dw = in && p.Dw ? p.Dw[d] : 0.f;
     // the lane's sums over its tokens (q, q + 4, ...), and its states' over all of them
@@ -163,8 +214,11 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
             put_singles(s.sgz + at.row * kCh, at.c0, gz);
             put_singles(s.slope + at.row * kCh, at.c0, sl);
         }
-        Bs.put(s.sB);
-        Cs.put(s.sC);
+#pragma unroll
+        for (int o = 0; o < S::kOrders; ++o) {
+            Bs.put(s.sB[o], S::kOrders == 2 ? 2 * o : o);
+            Cs.put(s.sC[o], S::kOrders == 2 ? 2 * o : o);
+        }
         const bool more = l0 > first;
         if (more) {
             fetch_rows(l0 - kSelTile);
@@ -178,9 +232,11 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                 F2 ah01[kSelKeep], ah23[kSelKeep];  // a_t h_{t-1}
                 F2 h01 = f2(0.f), h23 = f2(0.f);
                 if (in) {
-                    const float4 x = s.kept[t8 / kSelKeep][threadIdx.x];
-                    h01 = f2(x.x, x.y);
-                    h23 = f2(x.z, x.w);
+                    const float4 k = s.kept[t8 / kSelKeep][threadIdx.x];
+                    float x[4] = {k.x, k.y, k.z, k.w};
+                    reorder(x, order);
+                    h01 = f2(x[0], x[1]);
+                    h23 = f2(x[2], x[3]);
                 }
                 float ys[2] = {0.f, 0.f};  // y of tokens q and 4 + q
 #pragma unroll
@@ -190,7 +246,7 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                     for (int j = 0; j < 4; ++j) {
                         const int i = 4 * half + j, t = t8 + i;
                         const float2 x = s.sdt[t * kCh + cp];
-                        const float4 Bv = *reinterpret_cast<const float4*>(s.sB + t * kNp + 4 * q);
+                        const float4 Bv = *reinterpret_cast<const float4*>(myB + t * kNp);
                         const F2 dt2 = f2(x.x), du2 = f2(x.x * x.y);
                         f01[i] = factor(mul(dt2, A01));
                         f23[i] = factor(mul(dt2, A23));
@@ -199,7 +255,7 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                         h01 = fma(du2, f2(Bv.x, Bv.y), ah01[i]);
                         h23 = fma(du2, f2(Bv.z, Bv.w), ah23[i]);
                         if (p.z.p) {
-                            const float4 Cv = *reinterpret_cast<const float4*>(s.sC + t * kNp + 4 * q);
+                            const float4 Cv = *reinterpret_cast<const float4*>(myC + t * kNp);
                             y[j] = both(fma(h23, f2(Cv.z, Cv.w), mul(h01, f2(Cv.x, Cv.y))));
                         }
                     }
@@ -214,7 +270,7 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                     for (int j = 3; j >= 0; --j) {
                         const int i = 4 * half + j, t = t8 + i;
                         const float2 x = s.sdt[t * kCh + cp];
-                        const float4 Bv = *reinterpret_cast<const float4*>(s.sB + t * kNp + 4 * q), Cv = *reinterpret_cast<const float4*>(s.sC + t * kNp + 4 * q);
+                        const float4 Bv = *reinterpret_cast<const float4*>(myB + t * kNp), Cv = *reinterpret_cast<const float4*>(myC + t * kNp);
                         const F2 g2 = f2(s.sg[t * kCh + cs]), dt2 = f2(x.x), du2 = f2(x.x * x.y);
                         const F2 G01 = fma(f2(Cv.x, Cv.y), g2, P01), G23 = fma(f2(Cv.z, Cv.w), g2, P23);
                         bg[j] = both(fma(G23, f2(Bv.z, Bv.w), mul(G01, f2(Bv.x, Bv.y))));
@@ -222,12 +278,8 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                         ag[j] = both(fma(n23, A23, mul(n01, A01)));
                         a01 = fma(dt2, n01, a01);
                         a23 = fma(dt2, n23, a23);
-                        float v[8];
-                        get(mul(G01, du2), v[0], v[1]);
-                        get(mul(G23, du2), v[2], v[3]);
-                        get(mul(fma(du2, f2(Bv.x, Bv.y), ah01[i]), g2), v[4], v[5]);
-                        get(mul(fma(du2, f2(Bv.z, Bv.w), ah23[i]), g2), v[6], v[7]);
-                        channel_sums8<LPC>(v, lane);
+                        float v[kVals];
+                        channel_sums<LPC>(mul(G01, du2), mul(G23, du2), mul(fma(du2, f2(Bv.x, Bv.y), ah01[i]), g2), mul(fma(du2, f2(Bv.z, Bv.w), ah23[i]), g2), lane, v);
 #pragma unroll
                         for (int k = 0; k < kVals; ++k) s.red[warp][i][k * 32 + lane] = v[k];
                         P01 = decayed(f01[i], G01);
@@ -254,15 +306,14 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
 #pragma unroll
                 for (int i = 0; i < 4; ++i) add_exactly(dA[i], dA_rest[i], x[i]);
                 __syncthreads();
-                // values (token, value k, lane) of every warp: k * 32 + lane is value c * kVals + k of quad q
                 for (int i = threadIdx.x; i < kSelKeep * 32 * kVals; i += kSelThreads) {
-                    const int t = i / (32 * kVals), k = i / 32 % kVals, ln = i & 31;
+                    const int t = i / (32 * kVals), k = i / 32 % kVals, ln = i & 31, tok = l0 + t8 + t;
                     float sum = 0.f;
 #pragma unroll
                     for (int w = 0; w < S::kWarps; ++w) sum += s.red[w][t][k * 32 + ln];
-                    const int val = ln / LPC * kVals + k, n = 4 * (ln & (LPC - 1)) + (val & 3), tok = l0 + t8 + t;
-                    if (tok < last)
-                        p.part_bc[((((int64_t)at.block(p) * p.B + at.b) * p.L + tok) * p.G + at.g) * (2 * kNp) + (val >> 2) * kNp + n] = sum;
+                    int n;
+                    const bool c = channel_value<LPC>(ln, k, n);
+                    if (tok < last) p.part_bc[((((int64_t)at.block(p) * p.B + at.b) * p.L + tok) * p.G + at.g) * (2 * kNp) + (c ? kNp : 0) + n] = sum;
                 }
                 __syncthreads();
             }
@@ -292,14 +343,16 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     float g[4];
     get(P01, g[0], g[1]);
     get(P23, g[2], g[3]);
+    reorder(g, order);
     if (in && seg == 0 && p.dS_in)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (4 * q + i < p.N) p.dS_in[((int64_t)at.b * p.D + d) * p.N + 4 * q + i] = g[i];
     const int64_t part = (int64_t)at.b * p.nseg + seg;
-    if (in)
-        *reinterpret_cast<float4*>(p.part_a + (part * p.D + d) * kNp + 4 * q) =
-            make_float4(dA[0] + dA_rest[0], dA[1] + dA_rest[1], dA[2] + dA_rest[2], dA[3] + dA_rest[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dA[i] += dA_rest[i];
+    reorder(dA, order);
+    if (in) *reinterpret_cast<float4*>(p.part_a + (part * p.D + d) * kNp + 4 * q) = make_float4(dA[0], dA[1], dA[2], dA[3]);
     float sums[2] = {q < 4 ? dD + dD_rest : 0.f, q < 4 ? db + db_rest : 0.f};
 #pragma unroll
     for (int o = 1; o < LPC; o <<= 1)

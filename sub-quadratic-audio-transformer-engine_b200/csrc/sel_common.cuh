@@ -380,12 +380,13 @@ struct States {
                 x[i].load(static_cast<const T*>(t.p) + b * t.sb + l * t.sl + g * t.sg + n, p.N - n, vec);
         }
     }
-    __device__ __forceinline__ void put(float* to) const {
+    // (each four with their places n ^ order)
+    __device__ __forceinline__ void put(float* to, int order = 0) const {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int at = threadIdx.x + i * kSelThreads;
             if (kPieces % kSelThreads == 0 || at < kPieces)
-                *reinterpret_cast<float4*>(to + 4 * at) = make_float4(to_f<T>(x[i].x[0]), to_f<T>(x[i].x[1]), to_f<T>(x[i].x[2]), to_f<T>(x[i].x[3]));
+                *reinterpret_cast<float4*>(to + 4 * at) = make_float4(to_f<T>(x[i].x[order]), to_f<T>(x[i].x[1 ^ order]), to_f<T>(x[i].x[2 ^ order]), to_f<T>(x[i].x[3 ^ order]));
         }
     }
 };
