@@ -83,7 +83,7 @@ struct ConvParams {
     float* dw;           // [D, W]
     float* db;           // [D] or null
     float* part;         // [parts][W + 1][D]
-    int parts, run;      // token runs of a channel, tokens of each
+    int parts, run;      // partial sums of a channel; groups of token runs of each
 };
 cudaError_t launch_conv_fwd(const ConvParams& p, int dtype, cudaStream_t st, int* launches);
 cudaError_t launch_conv_bwd(const ConvParams& p, int dtype, cudaStream_t st, int* launches);

@@ -252,8 +252,8 @@ int fill_conv(const subq_causal_conv_args* a, ConvParams& p, bool bwd) {
         (rc = aligned(a->state_in, es, "state_in")))
         return rc;
     if (p.D > 0 && !p.w) return fail(SUBQ_ERR_INVALID_ARGUMENT, "weight is null");
-    // (the largest pieces of work: one thread a channel piece and run of 16 tokens, or a CTA of 32 x 8 of them)
-    if ((int64_t)p.B * ((p.L + 15) / 16) * p.D / 256 >= 0x7fffffff) return fail(SUBQ_ERR_UNSUPPORTED, "batch * seq_len * channels is too large for one call");
+    // (a CTA has 8 runs of 8 tokens; a grid at most 65535 rows of CTAs)
+    if ((int64_t)p.B * ((p.L + 7) / 8) > (int64_t)8 * 65535) return fail(SUBQ_ERR_UNSUPPORTED, "batch * seq_len is too large for one call (4,194,240 tokens)");
     const int64_t window = (int64_t)p.B * (p.W - 1) * p.D * (int64_t)es, one = (int64_t)p.D * 4;
     if (!bwd) {
         p.S_out = a->state_out;

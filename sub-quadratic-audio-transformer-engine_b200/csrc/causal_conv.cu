@@ -4,107 +4,124 @@
 // counts as 0 and its output is 0; the window that is handed on is of the W - 1 inputs up to the last live token.
 //   dpre_t = dy_t act'(pre_t),   dx_s = sum_j w_j dpre_{s+W-1-j},   dw_j = sum_t dpre_t x_{t-W+1+j},   db = sum_t dpre_t.
 //
-// HBM-bound: a thread has 16 bytes of neighbouring channels (backward: 4 channels) and walks a run of tokens with the last
-// W inputs in registers, so that an input is read once, but for the W - 1 before each run (from L2); the next tokens' loads
-// are in flight. The backward forms pre again from x; its dw and db are summed over a run, over the CTA's eight runs in
-// shared memory and then over CTAs by a second launch, in a fixed order.
+// HBM-bound: a thread has four neighbouring channels (backward of 16-bit types: two; single ones where rows are not aligned) and a
+// run of eight tokens, all of whose rows it asks for at once, those of the tokens that its taps reach into among them (L1 has
+// them for the CTA's next run). The backward forms pre again from x; its dw and db are summed over a run, over the CTA's
+// eight runs in shared memory and then over CTAs by a second launch, in a fixed order.
+#include <algorithm>
+
 #include "sel_common.cuh"
 
 namespace subq {
 namespace {
 
 using sel::Piece;
-using sel::need_vec;
 using sel::row_of;
 
 constexpr int kConvThreads = 256;
-constexpr int kRows = 8;   // backward: runs of a CTA
-constexpr int kAhead = 4;  // tokens whose loads are in flight
+constexpr int kRun = 8;   // tokens of a thread
+constexpr int kRows = 8;  // runs of a CTA, one after another
 
 template <typename T>
 __device__ __forceinline__ bool conv_live(const ConvParams& p, int b, int t) {
     return t >= 0 && t < p.L && (!p.mask || p.mask[(int64_t)b * p.mask_sb + t]);
 }
 
-// Input of token t (negative: the carried window).
+// Input of token t (negative: the carried window). What a masked token holds is loaded, but not used.
 template <typename T, int V, int W>
-__device__ __forceinline__ void conv_input(const ConvParams& p, int b, int t, int c, int n, bool vec, bool vec_s, Piece<T, V>& x) {
+__device__ __forceinline__ void conv_input(const ConvParams& p, int b, int t, int c, Piece<T, V>& x) {
+    x.zero();
     if (t < 0) {
-        if (p.S_in && t >= 1 - W) x.load(static_cast<const T*>(p.S_in) + ((int64_t)b * (W - 1) + t + W - 1) * p.D + c, n, vec_s);
-        else x.zero();
-    } else if (conv_live<T>(p, b, t)) {
-        x.load(row_of<T>(p.x, b, t, c), n, vec);
-    } else {
-        x.zero();
+        if (p.S_in && t >= 1 - W) x.load(static_cast<const T*>(p.S_in) + ((int64_t)b * (W - 1) + t + W - 1) * p.D + c);
+    } else if (t < p.L) {
+        const bool live = conv_live<T>(p, b, t);
+        x.load(row_of<T>(p.x, b, t, c));
+        if (!live) x.zero();
     }
 }
 
 template <typename T, int V, int W>
 struct Taps {
     float w[W][V], bias[V];
-    __device__ __forceinline__ void load(const ConvParams& p, int c, int n) {
+    __device__ __forceinline__ void load(const ConvParams& p, int c) {
+        constexpr int kAll = V * W;
+        if (kAll % 4 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0) {  // (c is a multiple of V)
+            float x[kAll];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < kAll / 4; ++i) {
+                const float4 v = reinterpret_cast<const float4*>(p.w + (int64_t)c * W)[i];
+                x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+            }
 #pragma unroll
-            for (int j = 0; j < W; ++j) w[j][i] = i < n ? p.w[(int64_t)(c + i) * W + j] : 0.f;
-            bias[i] = i < n && p.bias ? p.bias[c + i] : 0.f;
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j) w[j][i] = x[i * W + j];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j) w[j][i] = p.w[(int64_t)(c + i) * W + j];
         }
+#pragma unroll
+        for (int i = 0; i < V; ++i) bias[i] = p.bias ? p.bias[c + i] : 0.f;
     }
 };
 
+// 32 channel pieces x 8 runs a CTA.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kConvThreads) conv_fwd_kernel(const ConvParams p, int run, int runs, int keep) {
-    const int nv = (p.D + V - 1) / V;
-    const int64_t item = (int64_t)blockIdx.x * kConvThreads + threadIdx.x;
-    if (item >= (int64_t)p.B * runs * nv) return;
-    const int c = (int)(item % nv) * V, n = min(V, p.D - c);
-    const int64_t r = item / nv;
-    const int b = (int)(r / runs), t0 = (int)(r % runs) * run, t1 = min(p.L, t0 + run);
-    constexpr int kB = need_vec<V * (int)sizeof(T)>();
-    const bool vx = p.x.vec >= kB, vy = p.y.vec >= kB;
-    const bool vs = (p.D * (int)sizeof(T)) % kB == 0 && ((reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.S_out)) & (kB - 1)) == 0;
-    Taps<T, V, W> tap;
-    tap.load(p, c, n);
-    float x[W][V];  // the last W inputs, oldest first
+__global__ void __launch_bounds__(kConvThreads, 4) conv_fwd_kernel(const ConvParams p, int runs, int keep) {
+    const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * V;
+    const int64_t r = (int64_t)blockIdx.y * kRows + (threadIdx.x >> 5);
+    if (c >= p.D || r >= (int64_t)p.B * runs) return;
+    const int b = (int)(r / runs), t0 = (int)(r - (int64_t)b * runs) * kRun;
+    Piece<T, V> x[W - 1 + kRun];
+    uint32_t live = 0;
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) {
-        Piece<T, V> h;
-        conv_input<T, V, W>(p, b, t0 - (W - 1) + j, c, n, vx, vs, h);
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[j + 1][i] = to_f<T>(h.x[i]);
-    }
-    Piece<T, V> next[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) conv_input<T, V, W>(p, b, t0 + k < t1 ? t0 + k : p.L, c, n, vx, vs, next[k]);
-    for (int tb = t0; tb < t1; tb += kAhead) {
-        Piece<T, V> now[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) now[k] = next[k];
-        if (tb + kAhead < t1)
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) conv_input<T, V, W>(p, b, tb + kAhead + k < t1 ? tb + kAhead + k : p.L, c, n, vx, vs, next[k]);
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int t = tb + k;
-            if (t >= t1) break;
-            Piece<T, V> o;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-#pragma unroll
-                for (int j = 0; j < W - 1; ++j) x[j][i] = x[j + 1][i];
-                x[W - 1][i] = to_f<T>(now[k].x[i]);
-                float s = tap.bias[i];
-#pragma unroll
-                for (int j = 0; j < W; ++j) s = fmaf(tap.w[j][i], x[j][i], s);
-                if (p.silu) s *= sel::sigmoid(s);
-                o.x[i] = from_f<T>(s);
-            }
-            if (p.mask && !conv_live<T>(p, b, t)) o.zero();
-            o.store(const_cast<T*>(row_of<T>(p.y, b, t, c)), n, vy);
-            // the window behind the last token, where no mask ends the sequence before
-            if (keep && t >= p.L - (W - 1))
-                now[k].store(static_cast<T*>(p.S_out) + ((int64_t)b * (W - 1) + t - (p.L - (W - 1))) * p.D + c, n, vs);
+    for (int k = 0; k < W - 1 + kRun; ++k) {
+        const int t = t0 + k - (W - 1);
+        x[k].zero();
+        if (t < 0) {
+            if (p.S_in) x[k].load(static_cast<const T*>(p.S_in) + ((int64_t)b * (W - 1) + t + W - 1) * p.D + c);
+            live |= 1u << k;
+        } else if (t < p.L) {
+            x[k].load(row_of<T>(p.x, b, t, c));
+            if (conv_live<T>(p, b, t)) live |= 1u << k;
         }
+    }
+    Taps<T, V, W> tap;
+    tap.load(p, c);
+    float f[W - 1 + kRun][V];
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[k][i] = live >> k & 1 ? to_f<T>(x[k].x[i]) : 0.f;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+        const int t = t0 + k;
+        if (t >= p.L) break;
+        const bool on = live >> (k + W - 1) & 1;
+        float s[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            f[k + W - 1][i] = on ? to_f<T>(x[k + W - 1].x[i]) : 0.f;
+            s[i] = tap.bias[i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) s[i] = fmaf(tap.w[j][i], f[k + j][i], s[i]);
+        }
+        if (p.silu) {
+            float g[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) g[i] = s[i];
+            sel::sigmoid_all(g);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] *= g[i];
+        }
+        Piece<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.x[i] = from_f<T>(on ? s[i] : 0.f);
+        o.store(const_cast<T*>(row_of<T>(p.y, b, t, c)));
+        // the window behind the last token, where no mask ends the sequence before
+        if (keep && t >= p.L - (W - 1)) x[k + W - 1].store(static_cast<T*>(p.S_out) + ((int64_t)b * (W - 1) + t - (p.L - (W - 1))) * p.D + c);
     }
 }
 
@@ -114,23 +131,20 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const ConvParam
     const int nv = (p.D + V - 1) / V;
     const int64_t item = (int64_t)blockIdx.x * kConvThreads + threadIdx.x;
     if (item >= (int64_t)p.B * nv) return;
-    const int c = (int)(item % nv) * V, n = min(V, p.D - c), b = (int)(item / nv);
-    constexpr int kB = need_vec<V * (int)sizeof(T)>();
-    const bool vx = p.x.vec >= kB, vy = p.y.vec >= kB;
-    const bool vs = (p.D * (int)sizeof(T)) % kB == 0 && ((reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.S_out)) & (kB - 1)) == 0;
+    const int c = (int)(item % nv) * V, b = (int)(item / nv);
     Taps<T, V, W> tap;
-    tap.load(p, c, n);
+    tap.load(p, c);
     Piece<T, V> x[W], kept[W - 1];  // the last W inputs; the window up to the last live token
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) {
-        conv_input<T, V, W>(p, b, j - (W - 1), c, n, vx, vs, x[j + 1]);
+        conv_input<T, V, W>(p, b, j - (W - 1), c, x[j + 1]);
         kept[j] = x[j + 1];
     }
     for (int t = 0; t < p.L; ++t) {
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) x[j] = x[j + 1];
         const bool live = conv_live<T>(p, b, t);
-        conv_input<T, V, W>(p, b, t, c, n, vx, vs, x[W - 1]);
+        conv_input<T, V, W>(p, b, t, c, x[W - 1]);
         Piece<T, V> o;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -140,14 +154,14 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const ConvParam
             if (p.silu) s *= sel::sigmoid(s);
             o.x[i] = from_f<T>(live ? s : 0.f);
         }
-        o.store(const_cast<T*>(row_of<T>(p.y, b, t, c)), n, vy);
+        o.store(const_cast<T*>(row_of<T>(p.y, b, t, c)));
         if (live)
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) kept[j] = x[j + 1];
     }
     if (p.S_out)
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) kept[j].store(static_cast<T*>(p.S_out) + ((int64_t)b * (W - 1) + j) * p.D + c, n, vs);
+        for (int j = 0; j < W - 1; ++j) kept[j].store(static_cast<T*>(p.S_out) + ((int64_t)b * (W - 1) + j) * p.D + c);
 }
 
 // One past the last live token of a sequence, by all threads of a CTA.
@@ -172,7 +186,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_window_kernel(const ConvPar
     if (c >= p.D) return;
     Piece<T, 1> x[W - 1];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) conv_input<T, 1, W>(p, b, e - (W - 1) + j, c, 1, false, false, x[j]);
+    for (int j = 0; j < W - 1; ++j) conv_input<T, 1, W>(p, b, e - (W - 1) + j, c, x[j]);
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) static_cast<T*>(p.S_out)[((int64_t)b * (W - 1) + j) * p.D + c] = x[j].x[0];
 }
@@ -185,16 +199,11 @@ __global__ void __launch_bounds__(kConvThreads) conv_ends_kernel(const ConvParam
 // 32 channel pieces x 8 runs. Gradients of the run's inputs (the first run's: of the carried window, too) and its part of
 // dw and db: the tokens behind the run whose taps reach into it are formed again.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kConvThreads) conv_bwd_kernel(const ConvParams p, const int* ends) {
+__global__ void __launch_bounds__(kConvThreads, V == 4 ? 2 : 3) conv_bwd_kernel(const ConvParams p, const int* ends) {
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
-    const int c = (blockIdx.x * 32 + lane) * V, n = max(0, min(V, p.D - c));
-    const int runs = (p.L + p.run - 1) / p.run;
-    const int64_t r = (int64_t)blockIdx.y * kRows + row;
-    const bool in = n > 0 && r < (int64_t)p.B * runs;
-    constexpr int kB = need_vec<V * (int)sizeof(T)>();
-    const bool vx = p.x.vec >= kB, vg = p.dy.vec >= kB, vo = p.dx.vec >= kB;
-    const bool vs = (p.D * (int)sizeof(T)) % kB == 0 &&
-                    ((reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.dS_out) | reinterpret_cast<uintptr_t>(p.dS_in)) & (kB - 1)) == 0;
+    const int c = (blockIdx.x * 32 + lane) * V;
+    const int runs = (p.L + kRun - 1) / kRun;
+    constexpr int kTail = kRun + W - 1;
     float dw[W][V], db[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -202,89 +211,89 @@ __global__ void __launch_bounds__(kConvThreads) conv_bwd_kernel(const ConvParams
 #pragma unroll
         for (int j = 0; j < W; ++j) dw[j][i] = 0.f;
     }
-    if (in) {
-        const int b = (int)(r / runs), t0 = (int)(r % runs) * p.run, t1 = min(p.L, t0 + p.run);
-        const int end = ends ? ends[b] : p.L;
-        Taps<T, V, W> tap;
-        tap.load(p, c, n);
-        float x[W][V], dp[W][V];  // the last W inputs; dpre of the last W tokens
+    for (int turn = 0; turn < p.run; ++turn) {  // groups of eight runs
+        const int64_t r = ((int64_t)blockIdx.y * p.run + turn) * kRows + row;
+        if (c >= p.D || r >= (int64_t)p.B * runs) break;
+        const int b = (int)(r / runs), t0 = (int)(r - (int64_t)b * runs) * kRun, t1 = min(p.L, t0 + kRun);
+        const int end = p.dS_out ? ends ? ends[b] : p.L : 0;
+        // tokens t0 - (W - 1) .. t0 + kRun + W - 2 of x, t0 .. of dy: the taps of the last ones reach into the run
+        Piece<T, V> x[W - 1 + kTail], g[kTail];
+        uint32_t live = 0;
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) {
-            Piece<T, V> h;
-            conv_input<T, V, W>(p, b, t0 - (W - 1) + j, c, n, vx, vs, h);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                x[j + 1][i] = to_f<T>(h.x[i]);
-                dp[j + 1][i] = 0.f;
+        for (int k = 0; k < W - 1 + kTail; ++k) {
+            const int t = t0 + k - (W - 1);
+            x[k].zero();
+            if (k >= W - 1) g[k - (W - 1)].zero();
+            if (t < 0) {
+                if (p.S_in) x[k].load(static_cast<const T*>(p.S_in) + ((int64_t)b * (W - 1) + t + W - 1) * p.D + c);
+                live |= 1u << k;
+            } else if (t < p.L) {
+                x[k].load(row_of<T>(p.x, b, t, c));
+                if (k >= W - 1) g[k - (W - 1)].load(row_of<T>(p.dy, b, t, c));
+                if (conv_live<T>(p, b, t)) live |= 1u << k;
             }
         }
-        auto load = [&](int t, Piece<T, V>& xs, Piece<T, V>& gs) {
-            xs.zero();
-            gs.zero();
-            if (t < t1 + W - 1 && conv_live<T>(p, b, t)) {
-                xs.load(row_of<T>(p.x, b, t, c), n, vx);
-                gs.load(row_of<T>(p.dy, b, t, c), n, vg);
-            }
-        };
-        Piece<T, V> nx[kAhead], ng[kAhead];
+        Taps<T, V, W> tap;
+        tap.load(p, c);
+        float f[W - 1 + kTail][V], dp[W - 1 + kTail][V];  // inputs; dpre, 0 before the run
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) load(t0 + k, nx[k], ng[k]);
-        for (int tb = t0; tb < t1 + W - 1; tb += kAhead) {
-            Piece<T, V> cx[kAhead], cg[kAhead];
+        for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                cx[k] = nx[k];
-                cg[k] = ng[k];
+            for (int i = 0; i < V; ++i) {
+                f[k][i] = live >> k & 1 ? to_f<T>(x[k].x[i]) : 0.f;
+                dp[k][i] = 0.f;
             }
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) load(tb + kAhead + k, nx[k], ng[k]);
+        for (int k = 0; k < kTail; ++k) {
+            const int at = k + W - 1;
+            const bool on = live >> at & 1;
+            float pre[V], d[V];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const int t = tb + k, s = t - (W - 1);
-                if (t >= t1 + W - 1) break;
-                Piece<T, V> o;
-                float d[V];
+            for (int i = 0; i < V; ++i) {
+                f[at][i] = on ? to_f<T>(x[at].x[i]) : 0.f;
+                pre[i] = tap.bias[i];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
+                for (int j = 0; j < W; ++j) pre[i] = fmaf(tap.w[j][i], f[k + j][i], pre[i]);
+                d[i] = to_f<T>(g[k].x[i]);
+            }
+            if (p.silu) {
+                float sg[V];
 #pragma unroll
-                    for (int j = 0; j < W - 1; ++j) {
-                        x[j][i] = x[j + 1][i];
-                        dp[j][i] = dp[j + 1][i];
-                    }
-                    x[W - 1][i] = to_f<T>(cx[k].x[i]);
-                    float g = to_f<T>(cg[k].x[i]);  // 0 on tokens that are not live
-                    if (p.silu) {
-                        float pre = tap.bias[i];
+                for (int i = 0; i < V; ++i) sg[i] = pre[i];
+                sel::sigmoid_all(sg);
 #pragma unroll
-                        for (int j = 0; j < W; ++j) pre = fmaf(tap.w[j][i], x[j][i], pre);
-                        const float sg = sel::sigmoid(pre);
-                        const float slope = sg * fmaf(pre, 1.f - sg, 1.f);
-                        g = conv_live<T>(p, b, t) ? g * slope : 0.f;
-                    }
-                    dp[W - 1][i] = g;
-                    if (t < t1) {
-                        db[i] += g;
+                for (int i = 0; i < V; ++i) d[i] *= sg[i] * fmaf(pre[i], 1.f - sg[i], 1.f);
+            }
 #pragma unroll
-                        for (int j = 0; j < W; ++j) dw[j][i] = fmaf(g, x[j][i], dw[j][i]);
-                    }
-                    d[i] = 0.f;
+            for (int i = 0; i < V; ++i) {
+                dp[at][i] = on ? d[i] : 0.f;
+                if (k < kRun) {
+                    db[i] += dp[at][i];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) d[i] = fmaf(tap.w[j][i], dp[W - 1 - j][i], d[i]);
+                    for (int j = 0; j < W; ++j) dw[j][i] = fmaf(dp[at][i], f[k + j][i], dw[j][i]);
                 }
-                // (the run before this one, whose last tokens these are, writes tokens before t0)
-                if (s < t0 && !(t0 == 0 && p.dS_in)) continue;
-                const int at = s - end + W - 1;  // its place in the window that was handed on
-                if (p.dS_out && at >= 0 && at < W - 1) {
-                    Piece<T, V> h;
-                    h.load(static_cast<const T*>(p.dS_out) + ((int64_t)b * (W - 1) + at) * p.D + c, n, vs);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) d[i] += to_f<T>(h.x[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < V; ++i) o.x[i] = from_f<T>(s < 0 || conv_live<T>(p, b, s) ? d[i] : 0.f);
-                if (s >= 0) o.store(const_cast<T*>(row_of<T>(p.dx, b, s, c)), n, vo);
-                else o.store(static_cast<T*>(p.dS_in) + ((int64_t)b * (W - 1) + s + W - 1) * p.D + c, n, vs);
             }
+            // token s, whose taps have all been seen (before the run's first: the carried window's, of the first run)
+            const int s = t0 + k - (W - 1);
+            if (s >= t1 || (k < W - 1 && !(t0 == 0 && p.dS_in))) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                d[i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < W; ++j) d[i] = fmaf(tap.w[j][i], dp[at - j][i], d[i]);
+            }
+            const int place = s - end + W - 1;  // in the window that was handed on
+            if (p.dS_out && place >= 0 && place < W - 1) {
+                Piece<T, V> h;
+                h.load(static_cast<const T*>(p.dS_out) + ((int64_t)b * (W - 1) + place) * p.D + c);
+#pragma unroll
+                for (int i = 0; i < V; ++i) d[i] += to_f<T>(h.x[i]);
+            }
+            Piece<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.x[i] = from_f<T>(live >> k & 1 ? d[i] : 0.f);
+            if (k >= W - 1) o.store(const_cast<T*>(row_of<T>(p.dx, b, s, c)));
+            else o.store(static_cast<T*>(p.dS_in) + ((int64_t)b * (W - 1) + s + W - 1) * p.D + c);
         }
     }
     __shared__ float red[kRows][W + 1][32 * V];
@@ -329,11 +338,19 @@ __global__ void __launch_bounds__(kConvThreads) conv_sum_kernel(const ConvParams
     else if (p.db) p.db[c] = s + rest;
 }
 
-// The widest pieces that the rows' alignment allows, or single channels.
+// Channels of a thread: four, or two in the backward of 16-bit types (whose eight runs of four spill).
+template <typename T>
+constexpr int pieces(bool bwd) {
+    return bwd && sizeof(T) == 2 ? 2 : 4;
+}
+// Do the channels come out even, and all rows' alignments allow them?
 template <typename T>
 bool pieces_fit(const ConvParams& p, bool bwd) {
-    const int need = bwd ? 4 * (int)sizeof(T) : 16;
-    return bwd ? p.x.vec >= need && p.dy.vec >= need && p.dx.vec >= need : p.x.vec >= need && p.y.vec >= need;
+    const int n = pieces<T>(bwd), need = n * (int)sizeof(T);
+    const uintptr_t windows = bwd ? reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.dS_out) | reinterpret_cast<uintptr_t>(p.dS_in)
+                                  : reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.S_out);
+    if (p.D % n || windows % need || p.x.vec < need) return false;
+    return bwd ? p.dy.vec >= need && p.dx.vec >= need : p.y.vec >= need;
 }
 
 template <typename T, int V, int W>
@@ -345,9 +362,8 @@ cudaError_t conv_fwd(const ConvParams& p, cudaStream_t st, int* launches) {
         *launches = 1;
         return cudaGetLastError();
     }
-    const int run = (int64_t)p.B * p.L * nv >= (int64_t)148 * 2048 * 16 ? 32 : 16;
-    const int runs = (p.L + run - 1) / run, keep = p.S_out && !p.mask && p.S_out != p.S_in && p.L >= W - 1;
-    conv_fwd_kernel<T, V, W><<<blocks((int64_t)p.B * runs * nv), kConvThreads, 0, st>>>(p, run, runs, keep);
+    const int runs = (p.L + kRun - 1) / kRun, keep = p.S_out && !p.mask && p.S_out != p.S_in && p.L >= W - 1;
+    conv_fwd_kernel<T, V, W><<<dim3((unsigned)((nv + 31) / 32), (unsigned)(((int64_t)p.B * runs + kRows - 1) / kRows)), kConvThreads, 0, st>>>(p, runs, keep);
     *launches = 1;
     if (p.S_out && !keep) {
         conv_window_kernel<T, W><<<dim3(blocks(p.D), p.B), kConvThreads, 0, st>>>(p);
@@ -373,15 +389,13 @@ cudaError_t conv_bwd(const ConvParams& p, cudaStream_t st, int* launches) {
 
 template <typename T>
 cudaError_t conv_any(const ConvParams& p, bool bwd, cudaStream_t st, int* launches) {
-    auto width = [&](auto v) {
-        constexpr int V = decltype(v)::value, B = V == 1 ? 1 : 4;
-        switch (p.W) {
-            case 2: return bwd ? conv_bwd<T, B, 2>(p, st, launches) : conv_fwd<T, V, 2>(p, st, launches);
-            case 3: return bwd ? conv_bwd<T, B, 3>(p, st, launches) : conv_fwd<T, V, 3>(p, st, launches);
-            default: return bwd ? conv_bwd<T, B, 4>(p, st, launches) : conv_fwd<T, V, 4>(p, st, launches);
-        }
+    auto width = [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        if (bwd) return pieces_fit<T>(p, true) ? conv_bwd<T, pieces<T>(true), W>(p, st, launches) : conv_bwd<T, 1, W>(p, st, launches);
+        return pieces_fit<T>(p, false) ? conv_fwd<T, pieces<T>(false), W>(p, st, launches) : conv_fwd<T, 1, W>(p, st, launches);
     };
-    return pieces_fit<T>(p, bwd) ? width(std::integral_constant<int, 16 / (int)sizeof(T)>{}) : width(std::integral_constant<int, 1>{});
+    if (p.W == 2) return width(std::integral_constant<int, 2>{});
+    return p.W == 3 ? width(std::integral_constant<int, 3>{}) : width(std::integral_constant<int, 4>{});
 }
 
 cudaError_t conv_typed(const ConvParams& p, int dtype, bool bwd, cudaStream_t st, int* launches) {
@@ -394,13 +408,13 @@ cudaError_t conv_typed(const ConvParams& p, int dtype, bool bwd, cudaStream_t st
 cudaError_t launch_conv_fwd(const ConvParams& p, int dtype, cudaStream_t st, int* launches) { return conv_typed(p, dtype, false, st, launches); }
 cudaError_t launch_conv_bwd(const ConvParams& p, int dtype, cudaStream_t st, int* launches) { return conv_typed(p, dtype, true, st, launches); }
 
+// Groups of eight runs that a CTA goes through: one for each place on the card (three CTAs an SM) or so, so that there are few
+// partial sums (and a grid has at most 65535 rows of CTAs).
 void conv_bwd_split(ConvParams& p) {
-    p.run = 32;
-    for (;; p.run *= 2) {  // (a grid has at most 65535 rows of CTAs)
-        const int64_t runs = (int64_t)p.B * ((p.L + p.run - 1) / p.run), parts = (runs + kRows - 1) / kRows;
-        p.parts = (int)parts;
-        if (parts <= 65535) return;
-    }
+    const int64_t groups = ((int64_t)p.B * ((p.L + kRun - 1) / kRun) + kRows - 1) / kRows, across = (p.D + 63) / 64;
+    const int64_t places = std::max<int64_t>(1, 4 * 444 / across);
+    p.run = (int)std::max<int64_t>(1, std::max((groups + 65534) / 65535, groups / places));
+    p.parts = (int)((groups + p.run - 1) / p.run);
 }
 
 }  // namespace subq

@@ -79,20 +79,54 @@ __device__ __noinline__ void exact_quotients(float (&f)[V], const float (&r)[V],
     }
 }
 
+// A piece of a row: whole and aligned, or element by element.
+template <bool WHOLE, typename T, int V>
+__device__ __forceinline__ void rows_load(Piece<T, V>& x, const T* at, int n) {
+    if constexpr (WHOLE) x.load(at);
+    else x.load(at, n, false);
+}
+template <bool WHOLE, typename T, int V>
+__device__ __forceinline__ void rows_store(const Piece<T, V>& x, T* at, int n) {
+    if constexpr (WHOLE) {
+        x.store(at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) at[i] = x.x[i];
+    }
+}
+
+// Weights of eight columns (1 without any, 0 behind the last column).
+template <bool WHOLE, int V>
+__device__ __forceinline__ void weights(const RmsNormParams& p, int c, int n, float (&w)[V]) {
+    if (!p.w) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = 1.f;
+    } else if (WHOLE) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 x = n > 0 ? *reinterpret_cast<const float4*>(p.w + c + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = i < n ? p.w[c + i] : 0.f;
+    }
+}
+
 // A CTA of kWarps warps works on kWarps / NW rows at once.
 template <int NW>
 struct Rows {
     static constexpr int kWarps = NW > 4 ? NW : 4, kGroups = kWarps / NW, kThreads = 32 * kWarps;
 };
 
-template <typename TX, typename TR, typename TY, int K, int NW>
-__global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNormParams p, int vec) {
+template <typename TX, typename TR, typename TY, int K, int NW, bool WHOLE>
+__global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNormParams p) {
     constexpr int V = 8;
     __shared__ float red[Rows<NW>::kGroups][NW][1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / NW, in_row = warp % NW;
     const int c0 = (in_row * 32 + lane) * V;
     constexpr int kStep = NW * 32 * V;
-    const bool vx = vec & 1, vres = vec & 2, vr = vec & 4, vy = vec & 8;
     const int64_t step = (int64_t)gridDim.x * Rows<NW>::kGroups;
     Piece<TX, V> nx[K];
     Piece<TR, V> nr[K];
@@ -103,8 +137,8 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNo
             nx[k].zero();
             nr[k].zero();
             if (n > 0) {
-                nx[k].load(static_cast<const TX*>(p.x) + row * p.x_s + c, n, vx);
-                if (p.res) nr[k].load(static_cast<const TR*>(p.res) + row * p.res_s + c, n, vres);
+                rows_load<WHOLE>(nx[k], static_cast<const TX*>(p.x) + row * p.x_s + c, n);
+                if (p.res) rows_load<WHOLE>(nr[k], static_cast<const TR*>(p.res) + row * p.res_s + c, n);
             }
         }
     };
@@ -130,7 +164,7 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNo
                 if (!p.res)
 #pragma unroll
                     for (int i = 0; i < V; ++i) r.x[i] = from_f<TR>(f[k][i]);
-                r.store(static_cast<TR*>(p.r) + row * p.r_s + c, n, vr);
+                rows_store<WHOLE>(r, static_cast<TR*>(p.r) + row * p.r_s + c, n);
             }
         }
         if (row + step < p.rows) load(row + step);
@@ -142,12 +176,13 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNo
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = c0 + k * kStep, n = p.D - c;
-            float rk[V];
+            float rk[V], w[V];
+            weights<WHOLE>(p, c, n, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 rk[i] = f[k][i];
                 if (p.norm) f[k][i] *= rms;
-                if (p.w) f[k][i] *= i < n ? p.w[c + i] : 0.f;
+                if (p.w) f[k][i] *= w[i];
             }
             if constexpr (std::is_same<TY, Fp8>::value) {
                 float top = 0.f;
@@ -170,43 +205,32 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNo
 #pragma unroll
                     for (int i = 0; i < V; ++i) q.x[i] = __nv_cvt_float_to_fp8(f[k][i], __NV_SATFINITE, __NV_E4M3);
                     uint8_t* to = static_cast<uint8_t*>(p.y) + row * p.y_s + c;
-                    if (vy && n >= V) {
-                        *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(q.x);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            if (i < n) to[i] = q.x[i];
-                    }
+                    rows_store<WHOLE>(q, to, n);
                 }
             } else if (n > 0) {
                 Piece<TY, V> y;
 #pragma unroll
                 for (int i = 0; i < V; ++i) y.x[i] = from_f<TY>(f[k][i]);
-                y.store(static_cast<TY*>(p.y) + row * p.y_s + c, n, vy);
+                rows_store<WHOLE>(y, static_cast<TY*>(p.y) + row * p.y_s + c, n);
             }
         }
     }
 }
 
 // TY: type of dy (and of dx, where it is not TR).
-template <typename TX, typename TR, typename TY, int K, int NW>
-__global__ void __launch_bounds__(Rows<NW>::kThreads) rms_bwd_kernel(const RmsNormParams p, int vec) {
+template <typename TX, typename TR, typename TY, int K, int NW, bool WHOLE>
+__global__ void __launch_bounds__(Rows<NW>::kThreads) rms_bwd_kernel(const RmsNormParams p) {
     constexpr int V = 8;
     __shared__ float red[Rows<NW>::kGroups][NW][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / NW, in_row = warp % NW;
     const int c0 = (in_row * 32 + lane) * V;
     constexpr int kStep = NW * 32 * V;
-    const bool vg = vec & 1, vr = vec & 2, vn = vec & 4, vx = vec & 8, vres = vec & 16;
     const int64_t step = (int64_t)gridDim.x * Rows<NW>::kGroups;
-    float dw[K][V], w[K][V];
+    float dw[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = c0 + k * kStep + i;
-            dw[k][i] = 0.f;
-            w[k][i] = p.w && c < p.D ? p.w[c] : 1.f;
-        }
+        for (int i = 0; i < V; ++i) dw[k][i] = 0.f;
     for (int64_t row = (int64_t)blockIdx.x * Rows<NW>::kGroups + group; row < p.rows; row += step) {
         Piece<TY, V> dy[K];
         Piece<TR, V> r[K], dn[K];
@@ -218,19 +242,22 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_bwd_kernel(const RmsNo
             r[k].zero();
             dn[k].zero();
             if (n > 0) {
-                r[k].load(static_cast<const TR*>(p.r) + row * p.r_s + c, n, vr);
-                dy[k].load(static_cast<const TY*>(p.dy) + row * p.dy_s + c, n, vg);
-                if (p.dr) dn[k].load(static_cast<const TR*>(p.dr) + row * p.dr_s + c, n, vn);
+                rows_load<WHOLE>(r[k], static_cast<const TR*>(p.r) + row * p.r_s + c, n);
+                rows_load<WHOLE>(dy[k], static_cast<const TY*>(p.dy) + row * p.dy_s + c, n);
+                if (p.dr) rows_load<WHOLE>(dn[k], static_cast<const TR*>(p.dr) + row * p.dr_s + c, n);
             }
         }
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            float w[V];
+            weights<WHOLE>(p, c0 + k * kStep, p.D - c0 - k * kStep, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float rf = to_f<TR>(r[k].x[i]);
                 sums[0] = fmaf(rf, rf, sums[0]);
-                sums[1] = fmaf(to_f<TY>(dy[k].x[i]) * w[k][i], rf, sums[1]);
+                sums[1] = fmaf(to_f<TY>(dy[k].x[i]) * w[i], rf, sums[1]);
             }
+        }
         row_sums<NW, 2>(sums, red[group], in_row, group);
         const float rms = 1.f / sqrtf(sums[0] / (float)p.D + p.eps), m = rms * (sums[1] / (float)p.D);  // mean(g xh)
 #pragma unroll
@@ -238,17 +265,19 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_bwd_kernel(const RmsNo
             const int c = c0 + k * kStep, n = p.D - c;
             Piece<TX, V> ox;
             Piece<TR, V> ores;
+            float w[V];
+            weights<WHOLE>(p, c, n, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float xh = to_f<TR>(r[k].x[i]) * rms, g = to_f<TY>(dy[k].x[i]);
                 dw[k][i] = fmaf(g, xh, dw[k][i]);
-                const float d = fmaf(rms, fmaf(-xh, m, g * w[k][i]), to_f<TR>(dn[k].x[i]));
+                const float d = fmaf(rms, fmaf(-xh, m, g * w[i]), to_f<TR>(dn[k].x[i]));
                 ox.x[i] = from_f<TX>(d);
                 ores.x[i] = from_f<TR>(d);
             }
             if (n > 0) {
-                if (p.dx) ox.store(static_cast<TX*>(p.dx) + row * p.dx_s + c, n, vx);
-                if (p.dres) ores.store(static_cast<TR*>(p.dres) + row * p.dres_s + c, n, vres);
+                if (p.dx) rows_store<WHOLE>(ox, static_cast<TX*>(p.dx) + row * p.dx_s + c, n);
+                if (p.dres) rows_store<WHOLE>(ores, static_cast<TR*>(p.dres) + row * p.dres_s + c, n);
             }
         }
     }
@@ -284,11 +313,12 @@ __global__ void __launch_bounds__(256) rms_dw_kernel(const float* part, float* d
 }
 
 int es(int dtype) { return dtype == SUBQ_FP32 ? 4 : 2; }
-// May 8 elements of `size` bytes at every row's start + a multiple of 8 be read at once?
+// Do rows of `size`-byte elements allow whole pieces of 8 (or are there none)?
 bool rows_fit(const void* at, int64_t stride, int size) {
     const int need = size == 1 ? 8 : 16;
-    return reinterpret_cast<uintptr_t>(at) % need == 0 && stride * size % need == 0;
+    return !at || (reinterpret_cast<uintptr_t>(at) % need == 0 && stride * size % need == 0);
 }
+bool whole(const RmsNormParams& p) { return p.D % 8 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0; }
 
 template <typename F>
 cudaError_t by_width(int D, F f) {
@@ -306,12 +336,13 @@ cudaError_t by_width(int D, F f) {
 
 template <typename TX, typename TR, typename TY>
 cudaError_t fwd_typed(const RmsNormParams& p, cudaStream_t st) {
-    const int vec = (rows_fit(p.x, p.x_s, sizeof(TX)) ? 1 : 0) | (rows_fit(p.res, p.res_s, sizeof(TR)) ? 2 : 0) | (rows_fit(p.r, p.r_s, sizeof(TR)) ? 4 : 0) |
-                    (rows_fit(p.y, p.y_s, sizeof(TY)) ? 8 : 0);
+    const bool all = whole(p) && rows_fit(p.x, p.x_s, sizeof(TX)) && rows_fit(p.res, p.res_s, sizeof(TR)) && rows_fit(p.r, p.r_s, sizeof(TR)) && rows_fit(p.y, p.y_s, sizeof(TY));
     return by_width(p.D, [&](auto k, auto nw) {
         constexpr int K = decltype(k)::value, NW = decltype(nw)::value;
         const int64_t most = (int64_t)kSMs * (2048 / Rows<NW>::kThreads), need = (p.rows + Rows<NW>::kGroups - 1) / Rows<NW>::kGroups;
-        rms_fwd_kernel<TX, TR, TY, K, NW><<<(unsigned)(need < most ? need : most), Rows<NW>::kThreads, 0, st>>>(p, vec);
+        const unsigned blocks = (unsigned)(need < most ? need : most);
+        if (all) rms_fwd_kernel<TX, TR, TY, K, NW, true><<<blocks, Rows<NW>::kThreads, 0, st>>>(p);
+        else rms_fwd_kernel<TX, TR, TY, K, NW, false><<<blocks, Rows<NW>::kThreads, 0, st>>>(p);
         return cudaGetLastError();
     });
 }
@@ -319,13 +350,14 @@ cudaError_t fwd_typed(const RmsNormParams& p, cudaStream_t st) {
 template <typename TX, typename TR>
 cudaError_t bwd_typed(const RmsNormParams& p, cudaStream_t st, int* launches) {
     using TY = TX;
-    const int vec = (rows_fit(p.dy, p.dy_s, sizeof(TY)) ? 1 : 0) | (rows_fit(p.r, p.r_s, sizeof(TR)) ? 2 : 0) | (rows_fit(p.dr, p.dr_s, sizeof(TR)) ? 4 : 0) |
-                    (rows_fit(p.dx, p.dx_s, sizeof(TX)) ? 8 : 0) | (rows_fit(p.dres, p.dres_s, sizeof(TR)) ? 16 : 0);
+    const bool all = whole(p) && rows_fit(p.dy, p.dy_s, sizeof(TY)) && rows_fit(p.r, p.r_s, sizeof(TR)) && rows_fit(p.dr, p.dr_s, sizeof(TR)) && rows_fit(p.dx, p.dx_s, sizeof(TX)) &&
+                     rows_fit(p.dres, p.dres_s, sizeof(TR));
     return by_width(p.D, [&](auto k, auto nw) {
         constexpr int K = decltype(k)::value, NW = decltype(nw)::value;
         const int64_t most = NW >= 8 ? kSMs : kRmsParts, need = (p.rows + Rows<NW>::kGroups - 1) / Rows<NW>::kGroups;
         const int blocks = (int)(need < most ? need : most);
-        rms_bwd_kernel<TX, TR, TY, K, NW><<<blocks, Rows<NW>::kThreads, 0, st>>>(p, vec);
+        if (all) rms_bwd_kernel<TX, TR, TY, K, NW, true><<<blocks, Rows<NW>::kThreads, 0, st>>>(p);
+        else rms_bwd_kernel<TX, TR, TY, K, NW, false><<<blocks, Rows<NW>::kThreads, 0, st>>>(p);
         *launches = 1;
         if (p.part) {
             rms_dw_kernel<<<(p.D + 31) / 32, 256, 0, st>>>(p.part, p.dw, p.D, blocks);

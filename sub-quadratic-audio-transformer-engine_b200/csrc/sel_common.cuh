@@ -223,6 +223,19 @@ struct Piece {
             for (int i = 0; i < V; ++i) x[i] = i < n ? at[i] : from_f<T>(0.f);
         }
     }
+    // (the whole piece, aligned)
+    __device__ __forceinline__ void load(const T* at) {
+        constexpr int kB = V * (int)sizeof(T);
+        using Word = typename std::conditional<kB >= 16, uint4, typename std::conditional<kB == 8, uint2, typename std::conditional<kB == 4, uint32_t, T>::type>::type>::type;
+#pragma unroll
+        for (int i = 0; i < kB / (int)sizeof(Word); ++i) reinterpret_cast<Word*>(x)[i] = reinterpret_cast<const Word*>(at)[i];
+    }
+    __device__ __forceinline__ void store(T* at) const {
+        constexpr int kB = V * (int)sizeof(T);
+        using Word = typename std::conditional<kB >= 16, uint4, typename std::conditional<kB == 8, uint2, typename std::conditional<kB == 4, uint32_t, T>::type>::type>::type;
+#pragma unroll
+        for (int i = 0; i < kB / (int)sizeof(Word); ++i) reinterpret_cast<Word*>(at)[i] = reinterpret_cast<const Word*>(x)[i];
+    }
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int i = 0; i < V; ++i) x[i] = from_f<T>(0.f);
