@@ -40,32 +40,93 @@ __device__ __forceinline__ void conv_input(const ConvParams& p, int b, int t, in
     }
 }
 
+using sel::F2;
+using sel::f2;
+
+// A thread's channels two at a time (a single one beside a 0).
+template <typename T, int V>
+__device__ __forceinline__ void to_pairs(const Piece<T, V>& x, F2 (&f)[(V + 1) / 2]) {
+#pragma unroll
+    for (int i = 0; i < (V + 1) / 2; ++i) f[i] = f2(to_f<T>(x.x[2 * i]), V > 1 ? to_f<T>(x.x[2 * i + (V > 1)]) : 0.f);
+}
+template <typename T, int V>
+__device__ __forceinline__ void from_pairs(const F2 (&f)[(V + 1) / 2], Piece<T, V>& x) {
+#pragma unroll
+    for (int i = 0; i < (V + 1) / 2; ++i) {
+        float a, b;
+        sel::get(f[i], a, b);
+        x.x[2 * i] = from_f<T>(a);
+        if (V > 1) x.x[2 * i + (V > 1)] = from_f<T>(b);
+    }
+}
+
 template <typename T, int V, int W>
 struct Taps {
-    float w[W][V], bias[V];
+    static constexpr int H = (V + 1) / 2;
+    F2 w[W][H], bias[H];
     __device__ __forceinline__ void load(const ConvParams& p, int c) {
         constexpr int kAll = V * W;
+        float x[2 * H * W];
         if (kAll % 4 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0) {  // (c is a multiple of V)
-            float x[kAll];
 #pragma unroll
             for (int i = 0; i < kAll / 4; ++i) {
                 const float4 v = reinterpret_cast<const float4*>(p.w + (int64_t)c * W)[i];
                 x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
             }
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-#pragma unroll
-                for (int j = 0; j < W; ++j) w[j][i] = x[i * W + j];
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-#pragma unroll
-                for (int j = 0; j < W; ++j) w[j][i] = p.w[(int64_t)(c + i) * W + j];
+            for (int i = 0; i < kAll; ++i) x[i] = p.w[(int64_t)c * W + i];
         }
+        if (V == 1)
 #pragma unroll
-        for (int i = 0; i < V; ++i) bias[i] = p.bias ? p.bias[c + i] : 0.f;
+            for (int j = 0; j < W; ++j) x[W + j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) w[j][i] = f2(x[2 * i * W + j], x[(2 * i + 1) * W + j]);
+            bias[i] = p.bias ? f2(p.bias[c + 2 * i], V > 1 ? p.bias[c + 2 * i + (V > 1)] : 0.f) : f2(0.f);
+        }
     }
 };
+
+// Rows t0 .. t0 + M - 1 of a tensor, all asked for before the first is used (a run at an end of the sequence asks one by one).
+template <typename T, int V, int M>
+__device__ __forceinline__ void load_rows(const SelTensor& x, int L, int b, int t0, int c, Piece<T, V>* to) {
+    if (t0 >= 0 && t0 + M <= L) {
+        const T* at = row_of<T>(x, b, t0, c);
+#pragma unroll
+        for (int k = 0; k < M; ++k) to[k].load(at + k * x.sl);
+    } else {
+#pragma unroll
+        for (int k = 0; k < M; ++k) {
+            to[k].zero();
+            if (t0 + k >= 0 && t0 + k < L) to[k].load(row_of<T>(x, b, t0 + k, c));
+        }
+    }
+}
+// Which of them are live, a bit each; rows before the first token are.
+template <int M>
+__device__ __forceinline__ uint32_t live_rows(const ConvParams& p, int b, int t0) {
+    uint32_t live = 0;
+    if (!p.mask) {
+#pragma unroll
+        for (int k = 0; k < M; ++k) live |= t0 + k < p.L ? 1u << k : 0u;
+        return live;
+    }
+    const uint8_t* at = p.mask + (int64_t)b * p.mask_sb;
+    uint8_t m[M];
+#pragma unroll
+    for (int k = 0; k < M; ++k) m[k] = at[min(max(t0 + k, 0), p.L - 1)];
+#pragma unroll
+    for (int k = 0; k < M; ++k) live |= t0 + k < 0 || (m[k] && t0 + k < p.L) ? 1u << k : 0u;
+    return live;
+}
+template <typename T, int V, int W>
+__device__ __forceinline__ void load_window(const ConvParams& p, int b, int t0, int c, Piece<T, V>* to) {
+    if (t0 != 0 || !p.S_in) return;  // (runs are longer than a window)
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) to[k].load(static_cast<const T*>(p.S_in) + ((int64_t)b * (W - 1) + k) * p.D + c);
+}
 
 // 32 channel pieces x 8 runs a CTA.
 template <typename T, int V, int W>
@@ -75,53 +136,43 @@ __global__ void __launch_bounds__(kConvThreads, 4) conv_fwd_kernel(const ConvPar
     if (c >= p.D || r >= (int64_t)p.B * runs) return;
     const int b = (int)(r / runs), t0 = (int)(r - (int64_t)b * runs) * kRun;
     Piece<T, V> x[W - 1 + kRun];
-    uint32_t live = 0;
-#pragma unroll
-    for (int k = 0; k < W - 1 + kRun; ++k) {
-        const int t = t0 + k - (W - 1);
-        x[k].zero();
-        if (t < 0) {
-            if (p.S_in) x[k].load(static_cast<const T*>(p.S_in) + ((int64_t)b * (W - 1) + t + W - 1) * p.D + c);
-            live |= 1u << k;
-        } else if (t < p.L) {
-            x[k].load(row_of<T>(p.x, b, t, c));
-            if (conv_live<T>(p, b, t)) live |= 1u << k;
-        }
-    }
+    load_rows<T, V, W - 1 + kRun>(p.x, p.L, b, t0 - (W - 1), c, x);
+    load_window<T, V, W>(p, b, t0, c, x);
+    const uint32_t live = live_rows<W - 1 + kRun>(p, b, t0 - (W - 1));
     Taps<T, V, W> tap;
     tap.load(p, c);
-    float f[W - 1 + kRun][V];
+    constexpr int H = (V + 1) / 2;
+    F2 f[W - 1 + kRun][H];
+    // (a row is a warp's: whether its token is live is no divergence)
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[k][i] = live >> k & 1 ? to_f<T>(x[k].x[i]) : 0.f;
+    for (int k = 0; k < W - 1; ++k) {
+        if (!(live >> k & 1)) x[k].zero();
+        to_pairs(x[k], f[k]);
+    }
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
         const int t = t0 + k;
         if (t >= p.L) break;
+        Piece<T, V>& now = x[k + W - 1];
         const bool on = live >> (k + W - 1) & 1;
-        float s[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            f[k + W - 1][i] = on ? to_f<T>(x[k + W - 1].x[i]) : 0.f;
-            s[i] = tap.bias[i];
-#pragma unroll
-            for (int j = 0; j < W; ++j) s[i] = fmaf(tap.w[j][i], f[k + j][i], s[i]);
-        }
-        if (p.silu) {
-            float g[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) g[i] = s[i];
-            sel::sigmoid_all(g);
-#pragma unroll
-            for (int i = 0; i < V; ++i) s[i] *= g[i];
-        }
+        if (!on) now.zero();
+        to_pairs(now, f[k + W - 1]);
         Piece<T, V> o;
+        o.zero();
+        if (on) {
+            F2 s[H];
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.x[i] = from_f<T>(on ? s[i] : 0.f);
+            for (int i = 0; i < H; ++i) {
+                s[i] = tap.bias[i];
+#pragma unroll
+                for (int j = 0; j < W; ++j) s[i] = sel::fma(tap.w[j][i], f[k + j][i], s[i]);
+                if (p.silu) s[i] = sel::mul(s[i], sel::sigmoid(s[i]));
+            }
+            from_pairs(s, o);
+        }
         o.store(const_cast<T*>(row_of<T>(p.y, b, t, c)));
         // the window behind the last token, where no mask ends the sequence before
-        if (keep && t >= p.L - (W - 1)) x[k + W - 1].store(static_cast<T*>(p.S_out) + ((int64_t)b * (W - 1) + t - (p.L - (W - 1))) * p.D + c);
+        if (keep && t >= p.L - (W - 1)) now.store(static_cast<T*>(p.S_out) + ((int64_t)b * (W - 1) + t - (p.L - (W - 1))) * p.D + c);
     }
 }
 
@@ -146,14 +197,22 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const ConvParam
         const bool live = conv_live<T>(p, b, t);
         conv_input<T, V, W>(p, b, t, c, x[W - 1]);
         Piece<T, V> o;
+        constexpr int H = (V + 1) / 2;
+        F2 s[H];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float s = tap.bias[i];
+        for (int i = 0; i < H; ++i) s[i] = tap.bias[i];
 #pragma unroll
-            for (int j = 0; j < W; ++j) s = fmaf(tap.w[j][i], to_f<T>(x[j].x[i]), s);
-            if (p.silu) s *= sel::sigmoid(s);
-            o.x[i] = from_f<T>(live ? s : 0.f);
+        for (int j = 0; j < W; ++j) {
+            F2 f[H];
+            to_pairs(x[j], f);
+#pragma unroll
+            for (int i = 0; i < H; ++i) s[i] = sel::fma(tap.w[j][i], f[i], s[i]);
         }
+        if (p.silu)
+#pragma unroll
+            for (int i = 0; i < H; ++i) s[i] = sel::mul(s[i], sel::sigmoid(s[i]));
+        from_pairs(s, o);
+        if (!live) o.zero();
         o.store(const_cast<T*>(row_of<T>(p.y, b, t, c)));
         if (live)
 #pragma unroll
@@ -204,12 +263,13 @@ __global__ void __launch_bounds__(kConvThreads, V == 4 ? 2 : 3) conv_bwd_kernel(
     const int c = (blockIdx.x * 32 + lane) * V;
     const int runs = (p.L + kRun - 1) / kRun;
     constexpr int kTail = kRun + W - 1;
-    float dw[W][V], db[V];
+    constexpr int H = (V + 1) / 2;
+    F2 dw[W][H], db[H];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        db[i] = 0.f;
+    for (int i = 0; i < H; ++i) {
+        db[i] = f2(0.f);
 #pragma unroll
-        for (int j = 0; j < W; ++j) dw[j][i] = 0.f;
+        for (int j = 0; j < W; ++j) dw[j][i] = f2(0.f);
     }
     for (int turn = 0; turn < p.run; ++turn) {  // groups of eight runs
         const int64_t r = ((int64_t)blockIdx.y * p.run + turn) * kRows + row;
@@ -218,91 +278,83 @@ __global__ void __launch_bounds__(kConvThreads, V == 4 ? 2 : 3) conv_bwd_kernel(
         const int end = p.dS_out ? ends ? ends[b] : p.L : 0;
         // tokens t0 - (W - 1) .. t0 + kRun + W - 2 of x, t0 .. of dy: the taps of the last ones reach into the run
         Piece<T, V> x[W - 1 + kTail], g[kTail];
-        uint32_t live = 0;
-#pragma unroll
-        for (int k = 0; k < W - 1 + kTail; ++k) {
-            const int t = t0 + k - (W - 1);
-            x[k].zero();
-            if (k >= W - 1) g[k - (W - 1)].zero();
-            if (t < 0) {
-                if (p.S_in) x[k].load(static_cast<const T*>(p.S_in) + ((int64_t)b * (W - 1) + t + W - 1) * p.D + c);
-                live |= 1u << k;
-            } else if (t < p.L) {
-                x[k].load(row_of<T>(p.x, b, t, c));
-                if (k >= W - 1) g[k - (W - 1)].load(row_of<T>(p.dy, b, t, c));
-                if (conv_live<T>(p, b, t)) live |= 1u << k;
-            }
-        }
+        load_rows<T, V, W - 1 + kTail>(p.x, p.L, b, t0 - (W - 1), c, x);
+        load_rows<T, V, kTail>(p.dy, p.L, b, t0, c, g);
+        load_window<T, V, W>(p, b, t0, c, x);
+        const uint32_t live = live_rows<W - 1 + kTail>(p, b, t0 - (W - 1));
         Taps<T, V, W> tap;
         tap.load(p, c);
-        float f[W - 1 + kTail][V], dp[W - 1 + kTail][V];  // inputs; dpre, 0 before the run
+        F2 f[W - 1 + kTail][H], dp[W - 1 + kTail][H];  // inputs; dpre, 0 before the run
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k)
+        for (int k = 0; k < W - 1; ++k) {
+            if (!(live >> k & 1)) x[k].zero();
+            to_pairs(x[k], f[k]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                f[k][i] = live >> k & 1 ? to_f<T>(x[k].x[i]) : 0.f;
-                dp[k][i] = 0.f;
-            }
+            for (int i = 0; i < H; ++i) dp[k][i] = f2(0.f);
+        }
 #pragma unroll
         for (int k = 0; k < kTail; ++k) {
             const int at = k + W - 1;
             const bool on = live >> at & 1;
-            float pre[V], d[V];
+            if (!on) x[at].zero();
+            to_pairs(x[at], f[at]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                f[at][i] = on ? to_f<T>(x[at].x[i]) : 0.f;
-                pre[i] = tap.bias[i];
+            for (int i = 0; i < H; ++i) dp[at][i] = f2(0.f);
+            if (on) {
+                to_pairs(g[k], dp[at]);
+                if (p.silu)
 #pragma unroll
-                for (int j = 0; j < W; ++j) pre[i] = fmaf(tap.w[j][i], f[k + j][i], pre[i]);
-                d[i] = to_f<T>(g[k].x[i]);
-            }
-            if (p.silu) {
-                float sg[V];
+                    for (int i = 0; i < H; ++i) {
+                        F2 pre = tap.bias[i];
 #pragma unroll
-                for (int i = 0; i < V; ++i) sg[i] = pre[i];
-                sel::sigmoid_all(sg);
+                        for (int j = 0; j < W; ++j) pre = sel::fma(tap.w[j][i], f[k + j][i], pre);
+                        const F2 sg = sel::sigmoid(pre);  // silu' = sg (1 + pre (1 - sg))
+                        dp[at][i] = sel::mul(dp[at][i], sel::mul(sg, sel::fma(pre, sel::fma(sg, f2(-1.f), f2(1.f)), f2(1.f))));
+                    }
+                if (k < kRun)
 #pragma unroll
-                for (int i = 0; i < V; ++i) d[i] *= sg[i] * fmaf(pre[i], 1.f - sg[i], 1.f);
-            }
+                    for (int i = 0; i < H; ++i) {
+                        db[i] = sel::add(db[i], dp[at][i]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                dp[at][i] = on ? d[i] : 0.f;
-                if (k < kRun) {
-                    db[i] += dp[at][i];
-#pragma unroll
-                    for (int j = 0; j < W; ++j) dw[j][i] = fmaf(dp[at][i], f[k + j][i], dw[j][i]);
-                }
+                        for (int j = 0; j < W; ++j) dw[j][i] = sel::fma(dp[at][i], f[k + j][i], dw[j][i]);
+                    }
             }
             // token s, whose taps have all been seen (before the run's first: the carried window's, of the first run)
             const int s = t0 + k - (W - 1);
             if (s >= t1 || (k < W - 1 && !(t0 == 0 && p.dS_in))) continue;
+            F2 d[H];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                d[i] = 0.f;
+            for (int i = 0; i < H; ++i) {
+                d[i] = f2(0.f);
 #pragma unroll
-                for (int j = 0; j < W; ++j) d[i] = fmaf(tap.w[j][i], dp[at - j][i], d[i]);
+                for (int j = 0; j < W; ++j) d[i] = sel::fma(tap.w[j][i], dp[at - j][i], d[i]);
             }
             const int place = s - end + W - 1;  // in the window that was handed on
             if (p.dS_out && place >= 0 && place < W - 1) {
                 Piece<T, V> h;
+                F2 more[H];
                 h.load(static_cast<const T*>(p.dS_out) + ((int64_t)b * (W - 1) + place) * p.D + c);
+                to_pairs(h, more);
 #pragma unroll
-                for (int i = 0; i < V; ++i) d[i] += to_f<T>(h.x[i]);
+                for (int i = 0; i < H; ++i) d[i] = sel::add(d[i], more[i]);
             }
             Piece<T, V> o;
-#pragma unroll
-            for (int i = 0; i < V; ++i) o.x[i] = from_f<T>(live >> k & 1 ? d[i] : 0.f);
+            from_pairs(d, o);
+            if (!(live >> k & 1)) o.zero();
             if (k >= W - 1) o.store(const_cast<T*>(row_of<T>(p.dx, b, s, c)));
             else o.store(static_cast<T*>(p.dS_in) + ((int64_t)b * (W - 1) + s + W - 1) * p.D + c);
         }
     }
     __shared__ float red[kRows][W + 1][32 * V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        red[row][W][lane * V + i] = db[i];
+    for (int i = 0; i < H; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) red[row][j][lane * V + i] = dw[j][i];
-    }
+        for (int j = 0; j <= W; ++j) {
+            float a, b;
+            sel::get(j < W ? dw[j < W ? j : 0][i] : db[i], a, b);
+            red[row][j][lane * V + 2 * i] = a;
+            if (V > 1) red[row][j][lane * V + 2 * i + (V > 1)] = b;
+        }
     __syncthreads();
     for (int i = threadIdx.x; i < (W + 1) * 32 * V; i += kConvThreads) {
         const int j = i / (32 * V), at = i % (32 * V), ch = blockIdx.x * 32 * V + at;

@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNo
                     if ((lane & 15) == 0) p.scale[row * p.scale_s + c / 128] = scale;
                     Piece<uint8_t, V> q;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) q.x[i] = __nv_cvt_float_to_fp8(f[k][i], __NV_SATFINITE, __NV_E4M3);
+                    for (int i = 0; i < V; i += 2)
+                        reinterpret_cast<__nv_fp8x2_storage_t*>(q.x)[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(f[k][i], f[k][i + 1]), __NV_SATFINITE, __NV_E4M3);
                     uint8_t* to = static_cast<uint8_t*>(p.y) + row * p.y_s + c;
                     rows_store<WHOLE>(q, to, n);
                 }
