@@ -1,24 +1,43 @@
 // Matrix product of e4m3 operands with a float32 scale for every 1 x 128 of a and every 128 x 128 of b:
 //   out[m, n] = bias[n] + sum_kb a_scale[m, kb] b_scale[n / 128, kb] sum_{k in block kb} a[m, k] b[n, k].
 //
-// Tensor-core kernel: a CTA forms 128 x BN outputs. One thread loads the 128-byte rows of a k-block of both operands by TMA
-// (zeros behind the last row and column), one issues its four tcgen05.mma (kind::f8f6f4, K = 32 each) into one of two TMEM
-// accumulators, and four warps read the finished one back, row m in lane m, multiply it by the block's two scales and add it to
-// float32 sums in registers, while the other accumulator is being formed: a scale for every k-block is a rounding of 24
-// bits, and what the tensor core adds up by itself is 128 products. Two CTAs per SM, so that one's prologue and stores run
-// beside the other's products.
+// Tensor-core kernels: one thread loads the 128-byte rows of a k-block of both operands by TMA (zeros behind the last row and
+// column), one issues its four tcgen05.mma (kind::f8f6f4, K = 32 each) into one of two TMEM accumulators, and the epilogue's
+// warps read the finished one back, row m in lane m, multiply it by the block's two scales and add it to float32 sums in
+// registers, while the other accumulator is being formed: a scale for every k-block is a rounding of 24 bits, and what the
+// tensor core adds up by itself is 128 products.
 //
+// Large products: 128 x 256 tiles by one CTA an SM that goes on from tile to tile (k-blocks of the next one are loaded and
+// multiplied while this one is written), eight epilogue warps with 128 columns each. A k-block's products take 512 cycles,
+// its way through the epilogue (TMEM read and multiply-add, two warps to a scheduler) about as long.
+// Smaller ones: 128 x BN tiles, a CTA each, two to an SM.
 // A few rows (streaming steps) are bound by the weights' bytes, or by the launch: there a warp has a column of b, its lanes
 // 16 values each at a time, and every row of a.
 #include <cuda_fp8.h>
 
 #include "block_launch.h"
+#include "sel_common.cuh"
 #include "tc_common.cuh"
 
 namespace subq {
 namespace {
 
+using sel::F2;
+using sel::f2;
+
 constexpr int kBM = 128, kBK = 128;
+#ifndef MM_BIG
+#define MM_BIG 120
+#endif
+#ifndef MM_MID
+#define MM_MID 148
+#endif
+#ifndef MM_64
+#define MM_64 100
+#endif
+#ifndef MM_ROWS
+#define MM_ROWS 8
+#endif
 
 template <typename T, int BN>
 struct MatmulShape {
@@ -138,13 +157,15 @@ __global__ void __launch_bounds__(192, 2) scaled_matmul_kernel(const __grid_cons
         if (ok) {
             T* stage = reinterpret_cast<T*>(smem) + (size_t)warp * 32 * (BN + S::kPad);
             T* mine = stage + lane * (BN + S::kPad);
+            constexpr int kV = 16 / (int)sizeof(T), kPer = BN / kV;  // 16-byte pieces of a row
 #pragma unroll
-            for (int c = 0; c < BN; ++c) {
-                const float x = acc[c] + (p.bias && n0 + c < p.N ? p.bias[n0 + c] : 0.f);
-                mine[c] = from_f<T>(x);
+            for (int c = 0; c < BN; c += kV) {
+                sel::Piece<T, kV> o;
+#pragma unroll
+                for (int i = 0; i < kV; ++i) o.x[i] = from_f<T>(p.bias && n0 + c + i < p.N ? acc[c + i] + p.bias[n0 + c + i] : acc[c + i]);
+                o.store(mine + c);
             }
             __syncwarp();
-            constexpr int kV = 16 / (int)sizeof(T), kPer = BN / kV;  // 16-byte pieces of a row
             const bool vec = n0 + BN <= p.N && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_s * (int64_t)sizeof(T) % 16 == 0;
             T* out = static_cast<T*>(p.out);
             const int64_t mw = m0 + warp * 32;
@@ -164,6 +185,180 @@ __global__ void __launch_bounds__(192, 2) scaled_matmul_kernel(const __grid_cons
     tc::tc_fence_before();
     __syncthreads();
     if (warp == 5) tc::tmem_dealloc(tmem, S::kTmemCols);
+}
+
+// ------------------------------------------------------------------ 128 x 256 tiles, one CTA an SM
+template <typename T>
+struct BigShape {
+    static constexpr int kBN = 256, kStages = 3, kABytes = kBM * kBK, kStageBytes = kABytes + kBN * kBK;
+    static constexpr int kRow = 128 + 16;              // bytes of a staged output row, against bank conflicts
+    static constexpr int kOut = 8 * 32 * kRow;         // eight warps' 32 rows
+    static constexpr int kSmem = kStages * kStageBytes + kOut + 1024;
+    static constexpr int kThreads = 384;  // two warpgroups for the epilogue, one whose first two warps load and multiply
+};
+
+template <typename T>
+__global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const MatmulParams p,
+                                                                   int64_t tiles, int ntiles) {
+    using S = BigShape<T>;
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_slot;
+    unsigned char* smem = raw + (1024 - (tc::smem_u32(raw) & 1023)) % 1024;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            tc::mbar_init(&full[i], 1);
+            tc::mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&acc_full[i], 1);
+            tc::mbar_init(&acc_empty[i], 8);
+        }
+        tc::fence_mbar_init();
+    }
+    if (warp == 9) tc::tmem_alloc(&tmem_slot, 512);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    bool ok = true;
+    // The epilogue's sums and the 64 values that are on their way to them take 200 registers: 256 x 200 + 128 x 104 = 384 x 168.
+    // (k-blocks are counted through all of the CTA's tiles: block i uses stage i % 3 and accumulator i % 2)
+    if (warp >= 8) {
+    tc::regs_down<104>();
+    if (warp == 8) {
+        if (lane == 0) {
+            int64_t it = 0;
+            for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+                const int m0 = (int)(tile / ntiles) * kBM, n0 = (int)(tile % ntiles) * S::kBN;
+                for (int kb = 0; kb < p.nk; ++kb, ++it) {
+                    const int s = (int)(it % S::kStages);
+                    if (it >= S::kStages) ok = tcs::wait_bar(&empty[s], (uint32_t)(it / S::kStages - 1) & 1, p.status);
+                    if (!ok) break;
+                    unsigned char* at = smem + s * S::kStageBytes;
+                    tc::mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+                    tc::tma_load_2d(at, &ta, kb * kBK, m0, &full[s]);
+                    tc::tma_load_2d(at + S::kABytes, &tb, kb * kBK, n0, &full[s]);
+                }
+            }
+            if (!ok)  // the copies in flight land before the CTA ends
+                for (int64_t i = it > S::kStages ? it - S::kStages : 0; i < it; ++i) tcs::wait_bar(&full[i % S::kStages], (uint32_t)(i / S::kStages) & 1, p.status);
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (lane == 0) {
+            constexpr uint32_t id = tc::idesc_e4m3(kBM, S::kBN);
+            const uint32_t base = tc::smem_u32(smem);
+            int64_t it = 0;
+            for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x)
+                for (int kb = 0; kb < p.nk; ++kb, ++it) {
+                    const int s = (int)(it % S::kStages), buf = (int)(it & 1);
+                    ok = tcs::wait_bar(&full[s], (uint32_t)(it / S::kStages) & 1, p.status);
+                    if (ok && it >= 2) ok = tcs::wait_bar(&acc_empty[buf], (uint32_t)(it / 2 - 1) & 1, p.status);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint64_t ad = tc::sdesc_sw128(base + s * S::kStageBytes, 0, 1024), bd = tc::sdesc_sw128(base + s * S::kStageBytes + S::kABytes, 0, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc::mma_f8(tmem + buf * S::kBN, ad + 2 * k, bd + 2 * k, id, k > 0);
+                    tc::mma_commit(&empty[s]);
+                    tc::mma_commit(&acc_full[buf]);
+                }
+            if (!ok && it) tcs::wait_bar(&acc_full[(it - 1) & 1], (uint32_t)((it - 1) / 2) & 1, p.status);
+        }
+        __syncwarp();
+    }
+    } else {
+        tc::regs_up<200>();
+        const int quad = warp & 3, half = warp >> 2;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        unsigned char* stage = smem + S::kStages * S::kStageBytes + warp * 32 * S::kRow;
+        T* out = static_cast<T*>(p.out);
+        const bool aligned = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_s * (int64_t)sizeof(T) % 16 == 0;
+        int64_t it = 0;
+        for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            const int64_t mw = tile / ntiles * kBM + quad * 32, m = mw + lane;
+            const int n0 = (int)(tile % ntiles) * S::kBN + half * 128;
+            const bool in = m < p.M && n0 < p.N;
+            const float* as = p.a_scale + (in ? m : 0) * p.as_s;
+            const float* bs = p.b_scale + (in ? n0 / 128 : 0) * p.bs_s;
+            F2 acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = f2(0.f);
+            float sa = as[0], sb = bs[0], sa1 = p.nk > 1 ? as[1] : 0.f, sb1 = p.nk > 1 ? bs[1] : 0.f;  // two k-blocks ahead
+            for (int kb = 0; kb < p.nk; ++kb, ++it) {
+                const int buf = (int)(it & 1);
+                const F2 scale = f2(in ? sa * sb : 0.f);
+                sa = sa1;
+                sb = sb1;
+                if (kb + 2 < p.nk) {
+                    sa1 = as[kb + 2];
+                    sb1 = bs[kb + 2];
+                }
+                ok = __all_sync(0xffffffffu, tcs::wait_bar(&acc_full[buf], (uint32_t)(it / 2) & 1, p.status));
+                if (!ok) break;
+                tc::tc_fence_after();
+                const uint32_t from = tmem + buf * S::kBN + half * 128 + lanes;
+                uint32_t v[2][32];  // one half is added while the other is read
+                tc::tmem_ld32_issue(from, v[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tc::tmem_wait_ld();
+                    tc::tmem_regs_ready<32>(v[c & 1]);
+                    if (c < 3) {
+                        tc::tmem_ld32_issue(from + 32 * (c + 1), v[(c + 1) & 1]);
+                    } else {  // everything has been read
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        acc[16 * c + i] = sel::fma(f2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), scale, acc[16 * c + i]);
+                }
+            }
+            if (!ok) break;
+            // 128 bytes of each of the warp's 32 rows at a time, through shared memory to rows that are written whole
+            constexpr int kC = 128 / (int)sizeof(T), kV = 16 / (int)sizeof(T);
+#pragma unroll
+            for (int c = 0; c < 128; c += kC) {
+                if (n0 + c < p.N) {
+#pragma unroll
+                    for (int i = 0; i < kC; i += kV) {
+                        sel::Piece<T, kV> o;
+#pragma unroll
+                        for (int k = 0; k < kV; k += 2) {
+                            float x, y;
+                            sel::get(acc[(c + i + k) / 2], x, y);
+                            if (p.bias) {
+                                x += n0 + c + i + k < p.N ? p.bias[n0 + c + i + k] : 0.f;
+                                y += n0 + c + i + k + 1 < p.N ? p.bias[n0 + c + i + k + 1] : 0.f;
+                            }
+                            o.x[k] = from_f<T>(x);
+                            o.x[k + 1] = from_f<T>(y);
+                        }
+                        o.store(reinterpret_cast<T*>(stage + lane * S::kRow) + i);
+                    }
+                    __syncwarp();
+                    if (aligned && n0 + c + kC <= p.N) {
+#pragma unroll
+                        for (int r = lane / 8; r < 32; r += 4)
+                            if (mw + r < p.M)
+                                *reinterpret_cast<uint4*>(out + (mw + r) * p.out_s + n0 + c + lane % 8 * kV) = *reinterpret_cast<const uint4*>(stage + r * S::kRow + lane % 8 * 16);
+                    } else {
+                        for (int i = lane; i < 32 * kC; i += 32) {
+                            const int r = i / kC, x = i % kC;
+                            if (mw + r < p.M && n0 + c + x < p.N) out[(mw + r) * p.out_s + n0 + c + x] = reinterpret_cast<const T*>(stage + r * S::kRow)[x];
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 9) tc::tmem_dealloc(tmem, 512);
 }
 
 // 16 values of a row of e4m3 as float32 (zeros behind `left`).
@@ -244,8 +439,23 @@ cudaError_t launch_tiles(MatmulParams p, cudaStream_t st) {
 }
 
 template <typename T>
+cudaError_t launch_big(MatmulParams p, cudaStream_t st) {
+    using S = BigShape<T>;
+    alignas(64) CUtensorMap ta, tb;
+    if (!tcs::make_byte_map(&ta, p.a, p.M, p.K, p.a_s, kBM) || !tcs::make_byte_map(&tb, p.b, p.N, p.K, p.b_s, S::kBN)) return cudaErrorInvalidValue;
+    p.status = tcs::status_ptr();
+    if (!p.status) return cudaErrorInvalidDevice;
+    cudaError_t err = cudaFuncSetAttribute(scaled_matmul_big_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (err != cudaSuccess) return err;
+    const int ntiles = (p.N + S::kBN - 1) / S::kBN;
+    const int64_t tiles = (p.M + kBM - 1) / kBM * ntiles;
+    scaled_matmul_big_kernel<T><<<(unsigned)(tiles < 148 ? tiles : 148), S::kThreads, S::kSmem, st>>>(ta, tb, p, tiles, ntiles);
+    return cudaGetLastError();
+}
+
+template <typename T>
 cudaError_t launch_typed(const MatmulParams& p, cudaStream_t st) {
-    if (p.M <= 8 || p.K == 0) {
+    if (p.M <= MM_ROWS || p.K == 0) {
         const unsigned nb = (unsigned)((p.N + 7) / 8);
         if (p.K == 0) scaled_rows_kernel<T, 8><<<dim3(nb, (unsigned)((p.M + 7) / 8)), 256, 0, st>>>(p);
         else if (p.M == 1) scaled_rows_kernel<T, 1><<<dim3(nb, 1), 256, 0, st>>>(p);
@@ -254,7 +464,9 @@ cudaError_t launch_typed(const MatmulParams& p, cudaStream_t st) {
         return cudaGetLastError();
     }
     const int64_t tiles = (p.M + kBM - 1) / kBM * ((p.N + 127) / 128);
-    return tiles >= 148 ? launch_tiles<T, 128>(p, st) : launch_tiles<T, 32>(p, st);
+    const int64_t big = (p.M + kBM - 1) / kBM * ((p.N + 255) / 256);
+    if (big >= MM_BIG) return launch_big<T>(p, st);
+    return tiles >= MM_MID ? launch_tiles<T, 128>(p, st) : tiles >= MM_64 ? launch_tiles<T, 64>(p, st) : launch_tiles<T, 32>(p, st);
 }
 
 }  // namespace
