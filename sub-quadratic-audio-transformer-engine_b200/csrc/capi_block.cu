@@ -528,7 +528,7 @@ int subq_scaled_matmul(const subq_scaled_matmul_args* a) {
     if (some && !a->out) return fail(SUBQ_ERR_INVALID_ARGUMENT, "out is null");
     if (a->out_stride < 0) return fail(SUBQ_ERR_INVALID_ARGUMENT, "out has a negative stride");
     if ((a->M + 127) / 128 * ((a->N + 31) / 32) > 0x7fffffff) return fail(SUBQ_ERR_UNSUPPORTED, "M * N is too large for one call");
-    if (a->K == 0 && a->M > 8 * 65535) return fail(SUBQ_ERR_UNSUPPORTED, "M is too large for a product without columns");
+    if (a->K == 0 && a->M > 4 * 65535) return fail(SUBQ_ERR_UNSUPPORTED, "M is too large for a product without columns");
     auto rows = [&](const char* name, const void* at, int64_t n, int64_t stride, int64_t size, int64_t width) -> Memory {
         return {name, {reinterpret_cast<uintptr_t>(at), width * size, {n, 1, 1}, {(__int128)stride * size, 0, 0}}};
     };

@@ -26,18 +26,6 @@ using sel::F2;
 using sel::f2;
 
 constexpr int kBM = 128, kBK = 128;
-#ifndef MM_BIG
-#define MM_BIG 120
-#endif
-#ifndef MM_MID
-#define MM_MID 148
-#endif
-#ifndef MM_64
-#define MM_64 100
-#endif
-#ifndef MM_ROWS
-#define MM_ROWS 8
-#endif
 
 template <typename T, int BN>
 struct MatmulShape {
@@ -190,8 +178,8 @@ __global__ void __launch_bounds__(192, 2) scaled_matmul_kernel(const __grid_cons
 // ------------------------------------------------------------------ 128 x 256 tiles, one CTA an SM
 template <typename T>
 struct BigShape {
-    static constexpr int kBN = 256, kStages = 3, kABytes = kBM * kBK, kStageBytes = kABytes + kBN * kBK;
-    static constexpr int kRow = 128 + 16;              // bytes of a staged output row, against bank conflicts
+    static constexpr int kBN = 256, kStages = 4, kABytes = kBM * kBK, kStageBytes = kABytes + kBN * kBK;
+    static constexpr int kRow = 64 + 16;              // bytes of a staged output row, against bank conflicts
     static constexpr int kOut = 8 * 32 * kRow;         // eight warps' 32 rows
     static constexpr int kSmem = kStages * kStageBytes + kOut + 1024;
     static constexpr int kThreads = 384;  // two warpgroups for the epilogue, one whose first two warps load and multiply
@@ -224,7 +212,7 @@ __global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_
     const uint32_t tmem = tmem_slot;
     bool ok = true;
     // The epilogue's sums and the 64 values that are on their way to them take 200 registers: 256 x 200 + 128 x 104 = 384 x 168.
-    // (k-blocks are counted through all of the CTA's tiles: block i uses stage i % 3 and accumulator i % 2)
+    // (k-blocks are counted through all of the CTA's tiles: block i uses stage i % 4 and accumulator i % 2)
     if (warp >= 8) {
     tc::regs_down<104>();
     if (warp == 8) {
@@ -318,8 +306,8 @@ __global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_
                 }
             }
             if (!ok) break;
-            // 128 bytes of each of the warp's 32 rows at a time, through shared memory to rows that are written whole
-            constexpr int kC = 128 / (int)sizeof(T), kV = 16 / (int)sizeof(T);
+            // 64 bytes of each of the warp's 32 rows at a time, through shared memory to whole sectors of the rows
+            constexpr int kC = 64 / (int)sizeof(T), kV = 16 / (int)sizeof(T);
 #pragma unroll
             for (int c = 0; c < 128; c += kC) {
                 if (n0 + c < p.N) {
@@ -342,9 +330,9 @@ __global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_
                     __syncwarp();
                     if (aligned && n0 + c + kC <= p.N) {
 #pragma unroll
-                        for (int r = lane / 8; r < 32; r += 4)
+                        for (int r = lane / 4; r < 32; r += 8)
                             if (mw + r < p.M)
-                                *reinterpret_cast<uint4*>(out + (mw + r) * p.out_s + n0 + c + lane % 8 * kV) = *reinterpret_cast<const uint4*>(stage + r * S::kRow + lane % 8 * 16);
+                                *reinterpret_cast<uint4*>(out + (mw + r) * p.out_s + n0 + c + lane % 4 * kV) = *reinterpret_cast<const uint4*>(stage + r * S::kRow + lane % 4 * 16);
                     } else {
                         for (int i = lane; i < 32 * kC; i += 32) {
                             const int r = i / kC, x = i % kC;
@@ -453,20 +441,35 @@ cudaError_t launch_big(MatmulParams p, cudaStream_t st) {
     return cudaGetLastError();
 }
 
+// Device time, us (bf16 out), of the kernels by rows, and of 128 x BN tiles:
+//   M, N, K            rows   BN = 32     64    128   256 (persistent)
+//   1, 4096, 1024       2.9         -    8.9      -
+//   4, 4096, 1024       5.5         -    8.9      -
+//   8, 4096, 1024       9.0       8.0    8.8      -
+//   8, 4096, 4096      38.1      22.1   22.6      -
+//   128, 4096, 1024       -       7.5    8.5    9.1
+//   512, 1536, 768        -       7.3    7.4    8.0
+//   700, 1000, 2000       -      15.3   15.7   19.0
+//   2000, 1000, 2000      -      27.6   18.7   19.7
+//   1024, 4096, 1024      -      29.0   18.8   11.9   10.7
+//   2048, 4096, 4096      -         -      -     61     51
+//   16384, 4096, 1024     -         -      -    140    108
+//   5000, 769, 2049       -         -      -     53     78  (fp32 out; the last 256 columns hold one)
+// Up to four rows: by rows. Else the narrowest tiles whose CTAs the card holds at once (two an SM); beyond, 128 or 256 columns
+// by their waves' times: a wave of two 128 x 128 tiles an SM takes 0.95 of a time in which one of 128 x 256 takes 0.8.
 template <typename T>
 cudaError_t launch_typed(const MatmulParams& p, cudaStream_t st) {
-    if (p.M <= MM_ROWS || p.K == 0) {
+    if (p.M <= 4 || p.K == 0) {
         const unsigned nb = (unsigned)((p.N + 7) / 8);
-        if (p.K == 0) scaled_rows_kernel<T, 8><<<dim3(nb, (unsigned)((p.M + 7) / 8)), 256, 0, st>>>(p);
-        else if (p.M == 1) scaled_rows_kernel<T, 1><<<dim3(nb, 1), 256, 0, st>>>(p);
-        else if (p.M <= 4) scaled_rows_kernel<T, 4><<<dim3(nb, 1), 256, 0, st>>>(p);
-        else scaled_rows_kernel<T, 8><<<dim3(nb, 1), 256, 0, st>>>(p);
+        if (p.M == 1) scaled_rows_kernel<T, 1><<<dim3(nb, 1), 256, 0, st>>>(p);
+        else scaled_rows_kernel<T, 4><<<dim3(nb, (unsigned)((p.M + 3) / 4)), 256, 0, st>>>(p);
         return cudaGetLastError();
     }
-    const int64_t tiles = (p.M + kBM - 1) / kBM * ((p.N + 127) / 128);
-    const int64_t big = (p.M + kBM - 1) / kBM * ((p.N + 255) / 256);
-    if (big >= MM_BIG) return launch_big<T>(p, st);
-    return tiles >= MM_MID ? launch_tiles<T, 128>(p, st) : tiles >= MM_64 ? launch_tiles<T, 64>(p, st) : launch_tiles<T, 32>(p, st);
+    const int64_t rows = (p.M + kBM - 1) / kBM;
+    auto tiles = [&](int bn) { return rows * ((p.N + bn - 1) / bn); };
+    if (tiles(32) <= 296) return launch_tiles<T, 32>(p, st);
+    if (tiles(64) <= 296) return launch_tiles<T, 64>(p, st);
+    return 0.8 * (double)((tiles(256) + 147) / 148) < 0.95 * (double)((tiles(128) + 295) / 296) ? launch_big<T>(p, st) : launch_tiles<T, 128>(p, st);
 }
 
 }  // namespace

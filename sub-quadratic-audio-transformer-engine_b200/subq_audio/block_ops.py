@@ -7,6 +7,7 @@ Sequences are [B, L, D] CUDA tensors (any strides with a contiguous last dimensi
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -19,23 +20,31 @@ _E4M3 = torch.float8_e4m3fn
 _BLOCK = 128
 
 
+try:  # (the handle alone, without the object around it: a third of a short call's host time)
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device.index).cuda_stream
+    return _raw_stream(device.index)
 
 
-class _on:
-    """Makes a device the current one, where it is not already."""
+def _on_its_device(call):
+    """The call with the device of its first tensor as the current one."""
 
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    @functools.wraps(call)
+    def run(first, *args, **kwargs):
+        if not (isinstance(first, torch.Tensor) and first.is_cuda):
+            _require_cuda(first)
+        index = first.get_device()
+        if index == torch.cuda.current_device():
+            return call(first, *args, **kwargs)
+        with torch.cuda.device(index):
+            return call(first, *args, **kwargs)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+    return run
 
 
 def _t3(t: Optional[torch.Tensor]) -> _capi.Tensor3:
@@ -100,7 +109,7 @@ def _activation(activation: Optional[str]) -> int:
     return 1 if activation == "silu" else 0
 
 
-def _conv_args(x, weight, bias, activation, mask, state, keep: list) -> _capi.CausalConvArgs:
+def _conv_args(x, weight, bias, activation, mask, state, keep: list, y: Optional[torch.Tensor] = None, state_out: Optional[int] = None) -> _capi.CausalConvArgs:
     if x.dim() != 3 or weight.dim() != 2:
         raise ValueError("x must be [B, L, D] and weight [D, W]")
     if x.dtype not in _TYPES:
@@ -109,17 +118,12 @@ def _conv_args(x, weight, bias, activation, mask, state, keep: list) -> _capi.Ca
     W = weight.shape[1]
     if not 2 <= W <= 4:
         raise ValueError(f"the convolution's width must be 2, 3 or 4, got {W}")
-    a = _capi.CausalConvArgs()
-    a.batch, a.seq_len, a.channels, a.width = B, L, D, W
-    a.dtype = _DTYPES[x.dtype]
-    a.silu = _activation(activation)
-    a.x = _t3(x)
-    a.weight = _param(weight, "weight", (D, W), x.device, keep)
-    a.bias = _param(bias, "bias", (D,), x.device, keep)
-    a.mask, a.mask_stride_b = _mask(mask, B, L, x.device, keep)
-    if state is not None:
-        a.state_in = _window(state, "state", x, W, keep)
-    return a
+    dev = x.device
+    m, m_stride = (None, 0) if mask is None else _mask(mask, B, L, dev, keep)
+    none = _capi.Tensor3()
+    return _capi.CausalConvArgs(B, L, D, W, _DTYPES[x.dtype], _activation(activation), _t3(x), none if y is None else _t3(y), none, none,
+                                _param(weight, "weight", (D, W), dev, keep), _param(bias, "bias", (D,), dev, keep), m, m_stride,
+                                None if state is None else _window(state, "state", x, W, keep), state_out, None, None, None, None, None, 0, _stream(dev))
 
 
 def _window(state: torch.Tensor, name: str, x: torch.Tensor, W: int, keep: list) -> int:
@@ -133,6 +137,7 @@ def _window(state: torch.Tensor, name: str, x: torch.Tensor, W: int, keep: list)
     return s.data_ptr()
 
 
+@_on_its_device
 def causal_conv_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
                         activation: Optional[str] = "silu", mask: Optional[torch.Tensor] = None,
                         state: Optional[torch.Tensor] = None, return_state: bool = False,
@@ -143,26 +148,21 @@ def causal_conv_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     ``state`` [B, W - 1, D] (x's type) holds the inputs before the first token (None: zeros). A masked token's input counts
     as 0 and its output is 0; nothing of it is read. The returned state is of the W - 1 inputs up to the last live token,
     so that a padded batch of prompts goes on with its next tokens. Math in float32."""
-    _require_cuda(x)
     x = _inner_contig(x)
     keep: list = []
-    with _on(x.device):
-        a = _conv_args(x, weight, bias, activation, mask, state, keep)
-        if out is None:
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        else:
-            y = out
-            _check_out(y, x)
-        a.y = _t3(y)
-        new = None
-        if return_state:
-            new = torch.empty((x.shape[0], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device)
-            a.state_out = new.data_ptr()
-        a.stream = _stream(x.device)
-        _capi.causal_conv_fwd(a)
+    if out is None:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        y = out
+        _check_out(y, x)
+    new = None
+    if return_state:
+        new = torch.empty((x.shape[0], weight.shape[1] - 1 if weight.dim() == 2 and 2 <= weight.shape[1] <= 4 else 0, x.shape[-1]), dtype=x.dtype, device=x.device)
+    _capi.causal_conv_fwd(_conv_args(x, weight, bias, activation, mask, state, keep, y, None if new is None else new.data_ptr()))
     return y, new
 
 
+@_on_its_device
 def causal_conv_backward(x: torch.Tensor, weight: torch.Tensor, dout: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
                          activation: Optional[str] = "silu", mask: Optional[torch.Tensor] = None,
                          state: Optional[torch.Tensor] = None, dstate: Optional[torch.Tensor] = None, need_dstate: bool = False
@@ -174,24 +174,23 @@ def causal_conv_backward(x: torch.Tensor, weight: torch.Tensor, dout: torch.Tens
     x, dout = _inner_contig(x), _inner_contig(dout)
     _check_seq(dout, "dout", x)
     keep: list = []
-    with _on(x.device):
-        a = _conv_args(x, weight, bias, activation, mask, state, keep)
-        D, W = weight.shape
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty((D, W), dtype=torch.float32, device=x.device)
-        db = torch.empty(D, dtype=torch.float32, device=x.device) if bias is not None else None
-        a.dy, a.dx, a.dweight = _t3(dout), _t3(dx), dw.data_ptr()
-        if db is not None:
-            a.dbias = db.data_ptr()
-        if dstate is not None:
-            a.dstate_out = _window(dstate, "dstate", x, W, keep)
-        ds = None
-        if need_dstate:
-            ds = torch.empty((x.shape[0], W - 1, D), dtype=x.dtype, device=x.device)
-            a.dstate_in = ds.data_ptr()
-        a.stream = _stream(x.device)
-        a.workspace, a.workspace_bytes = _workspace(_capi.causal_conv_bwd_workspace_bytes(a), x.device, keep)
-        _capi.causal_conv_bwd(a)
+    a = _conv_args(x, weight, bias, activation, mask, state, keep)
+    D, W = weight.shape
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty((D, W), dtype=torch.float32, device=x.device)
+    db = torch.empty(D, dtype=torch.float32, device=x.device) if bias is not None else None
+    a.dy, a.dx, a.dweight = _t3(dout), _t3(dx), dw.data_ptr()
+    if db is not None:
+        a.dbias = db.data_ptr()
+    if dstate is not None:
+        a.dstate_out = _window(dstate, "dstate", x, W, keep)
+    ds = None
+    if need_dstate:
+        ds = torch.empty((x.shape[0], W - 1, D), dtype=x.dtype, device=x.device)
+        a.dstate_in = ds.data_ptr()
+    a.stream = _stream(x.device)
+    a.workspace, a.workspace_bytes = _workspace(_capi.causal_conv_bwd_workspace_bytes(a), x.device, keep)
+    _capi.causal_conv_bwd(a)
     return dx, dw, db, ds
 
 
@@ -206,11 +205,14 @@ class _Step:
         self._ref = ctypes.byref(args)
 
     def step(self) -> None:
-        if torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
+        index = self.device.index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
                 return self.step()
-        self._args.stream = _stream(self.device)
-        _capi.check(self._call(self._ref))
+        self._args.stream = _raw_stream(index)
+        rc = self._call(self._ref)
+        if rc:
+            _capi.check(rc)
 
 
 def _own_buffer(t: Optional[torch.Tensor], name: str, shape: tuple, device: torch.device) -> Optional[int]:
@@ -254,7 +256,7 @@ class CausalConvStep(_Step):
         if state.dtype != x.dtype or not state.is_contiguous() or state.device != x.device:
             raise ValueError(f"state must be a contiguous {x.dtype} tensor on the device of x")
         _check_out(out, x)
-        with _on(x.device):
+        with torch.cuda.device(x.device):
             a = _conv_args(x, weight, bias, activation, mask, state, keep)
             a.state_out = a.state_in
             a.y = _t3(out)
@@ -342,6 +344,7 @@ def _state(state: Optional[torch.Tensor], name: str, u: torch.Tensor, N: int, ke
     return s.data_ptr()
 
 
+@_on_its_device
 def selective_scan_forward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
                            D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None,
                            dt_softplus: bool = True, mask: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
@@ -355,37 +358,36 @@ def selective_scan_forward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     have one type (float32, float16 or bfloat16); ``A`` [D, N], ``D`` [D] and ``dt_bias`` [D] are used in float32.
     ``z`` None: no gate; ``dt_softplus=False``: dt + dt_bias itself. ``mask`` [B, L]: a masked token leaves the state as it
     is, its output is 0 and nothing of it is read. N <= 128. Math in float32, a decay near 1 applied as h + (a - 1) h."""
-    _require_cuda(u, dt, B, C)
     G = _scan_inputs(u, dt, A, B, C, z)
     u, dt, B, C = (_inner_contig(t) for t in (u, dt, B, C))
     z = None if z is None else _inner_contig(z)
     keep: list = []
-    with _on(u.device):
-        a = _capi.SelectiveFwdArgs()
-        _scan_desc(a.desc, u, A, D, dt_bias, dt_softplus, mask, G, keep)
-        if out is None:
-            y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
-        else:
-            y = out
-            _check_out(y, u)
-        a.u, a.dt, a.z, a.B, a.C, a.out = _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(y)
-        N = A.shape[1]
-        a.state_in = _state(state, "state", u, N, keep)
-        new = None
-        if return_state:
-            new = torch.empty((u.shape[0], u.shape[2], N), dtype=torch.float32, device=u.device)
-            a.state_out = new.data_ptr()
-        a.stream = _stream(u.device)
-        if handover is not None:
-            handover.buf = torch.empty(_capi.selective_scan_handover_bytes(a.desc), dtype=torch.uint8, device=u.device)
-            handover.key = (tuple(u.shape), N, G, u.dtype, u.device)
-            if handover.buf.numel():
-                a.handover = handover.buf.data_ptr()
-        a.workspace, a.workspace_bytes = _workspace(_capi.selective_scan_fwd_workspace_bytes(a), u.device, keep)
-        _capi.selective_scan_fwd(a)
+    a = _capi.SelectiveFwdArgs()
+    _scan_desc(a.desc, u, A, D, dt_bias, dt_softplus, mask, G, keep)
+    if out is None:
+        y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    else:
+        y = out
+        _check_out(y, u)
+    a.u, a.dt, a.z, a.B, a.C, a.out = _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(y)
+    N = A.shape[1]
+    a.state_in = _state(state, "state", u, N, keep)
+    new = None
+    if return_state:
+        new = torch.empty((u.shape[0], u.shape[2], N), dtype=torch.float32, device=u.device)
+        a.state_out = new.data_ptr()
+    a.stream = _stream(u.device)
+    if handover is not None:
+        handover.buf = torch.empty(_capi.selective_scan_handover_bytes(a.desc), dtype=torch.uint8, device=u.device)
+        handover.key = (tuple(u.shape), N, G, u.dtype, u.device)
+        if handover.buf.numel():
+            a.handover = handover.buf.data_ptr()
+    a.workspace, a.workspace_bytes = _workspace(_capi.selective_scan_fwd_workspace_bytes(a), u.device, keep)
+    _capi.selective_scan_fwd(a)
     return y, new
 
 
+@_on_its_device
 def selective_scan_backward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, dout: torch.Tensor, *,
                             D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None,
                             dt_softplus: bool = True, mask: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
@@ -401,38 +403,37 @@ def selective_scan_backward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, 
     z = None if z is None else _inner_contig(z)
     keep: list = []
     dev = u.device
-    with _on(dev):
-        a = _capi.SelectiveBwdArgs()
-        _scan_desc(a.desc, u, A, D, dt_bias, dt_softplus, mask, G, keep)
-        N = A.shape[1]
+    a = _capi.SelectiveBwdArgs()
+    _scan_desc(a.desc, u, A, D, dt_bias, dt_softplus, mask, G, keep)
+    N = A.shape[1]
 
-        def like(t):
-            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+    def like(t):
+        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
 
-        def f32(*shape):
-            return torch.empty(shape, dtype=torch.float32, device=dev)
+    def f32(*shape):
+        return torch.empty(shape, dtype=torch.float32, device=dev)
 
-        Dn = u.shape[2]
-        g = SelectiveGrads(like(u), like(dt), f32(Dn, N), like(B), like(C), None if D is None else f32(Dn), like(z),
-                           None if dt_bias is None else f32(Dn), f32(u.shape[0], Dn, N) if need_dstate else None)
-        a.u, a.dt, a.z, a.B, a.C, a.dout = _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(dout)
-        a.du, a.ddt, a.dz, a.dB, a.dC = _t3(g.du), _t3(g.ddt), _t3(g.dz), _t3(g.dB), _t3(g.dC)
-        a.dA = g.dA.data_ptr()
-        for name, t in (("dD", g.dD), ("ddt_bias", g.ddt_bias), ("dstate_in", g.dstate)):
-            if t is not None:
-                setattr(a, name, t.data_ptr())
-        a.state_in = _state(state, "state", u, N, keep)
-        a.dstate_out = _state(dstate, "dstate", u, N, keep)
-        if handover is not None and handover.buf is not None and handover.buf.numel():
-            if handover.key != (tuple(u.shape), N, G, u.dtype, dev):
-                raise ValueError("handover comes from a forward of another shape, type or device")
-            if (handover.buf.dtype != torch.uint8 or not handover.buf.is_contiguous()
-                    or handover.buf.numel() < _capi.selective_scan_handover_bytes(a.desc)):
-                raise ValueError("handover is not a buffer that the forward of this call filled")
-            a.handover = handover.buf.data_ptr()
-        a.stream = _stream(dev)
-        a.workspace, a.workspace_bytes = _workspace(_capi.selective_scan_bwd_workspace_bytes(a), dev, keep)
-        _capi.selective_scan_bwd(a)
+    Dn = u.shape[2]
+    g = SelectiveGrads(like(u), like(dt), f32(Dn, N), like(B), like(C), None if D is None else f32(Dn), like(z),
+                       None if dt_bias is None else f32(Dn), f32(u.shape[0], Dn, N) if need_dstate else None)
+    a.u, a.dt, a.z, a.B, a.C, a.dout = _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(dout)
+    a.du, a.ddt, a.dz, a.dB, a.dC = _t3(g.du), _t3(g.ddt), _t3(g.dz), _t3(g.dB), _t3(g.dC)
+    a.dA = g.dA.data_ptr()
+    for name, t in (("dD", g.dD), ("ddt_bias", g.ddt_bias), ("dstate_in", g.dstate)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    a.state_in = _state(state, "state", u, N, keep)
+    a.dstate_out = _state(dstate, "dstate", u, N, keep)
+    if handover is not None and handover.buf is not None and handover.buf.numel():
+        if handover.key != (tuple(u.shape), N, G, u.dtype, dev):
+            raise ValueError("handover comes from a forward of another shape, type or device")
+        if (handover.buf.dtype != torch.uint8 or not handover.buf.is_contiguous()
+                or handover.buf.numel() < _capi.selective_scan_handover_bytes(a.desc)):
+            raise ValueError("handover is not a buffer that the forward of this call filled")
+        a.handover = handover.buf.data_ptr()
+    a.stream = _stream(dev)
+    a.workspace, a.workspace_bytes = _workspace(_capi.selective_scan_bwd_workspace_bytes(a), dev, keep)
+    _capi.selective_scan_bwd(a)
     return g
 
 
@@ -458,7 +459,7 @@ class SelectiveScanStep(_Step):
         _own_buffer(dt_bias, "dt_bias", (u.shape[2],), u.device)
         _check_out(out, u)
         keep: list = [u, dt, A, B, C, out, state, D, z, dt_bias, mask]
-        with _on(u.device):
+        with torch.cuda.device(u.device):
             a = _capi.SelectiveFwdArgs()
             _scan_desc(a.desc, u, A, D, dt_bias, dt_softplus, mask, G, keep)
             a.u, a.dt, a.z, a.B, a.C, a.out = _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(out)
@@ -480,55 +481,47 @@ def _flat(t: torch.Tensor, keep: list) -> Tuple[int, int]:
     return t.data_ptr(), D
 
 
-def _norm_args(x: torch.Tensor, weight, eps: float, residual, keep: list, norm: int = 1) -> Tuple[_capi.RmsNormArgs, torch.dtype]:
+def _norm_types(x: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.dtype:
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 16384:
         raise ValueError("the norm needs a last dimension of 1 to 16384")
     if x.dtype not in _TYPES:
         raise TypeError(f"unsupported dtype {x.dtype}; use float32, float16 or bfloat16")
-    D = x.shape[-1]
-    a = _capi.RmsNormArgs()
-    a.rows, a.dim, a.eps, a.norm = x.numel() // D, D, eps, norm
-    a.x_dtype = a.r_dtype = _DTYPES[x.dtype]
-    a.weight = _param(weight, "weight", (D,), x.device, keep)
-    r_type = x.dtype
-    if residual is not None:
-        if residual.shape != x.shape or residual.device != x.device:
-            raise ValueError(f"residual must have x's shape {tuple(x.shape)} and device")
-        r_type = residual.dtype
-        if r_type not in (x.dtype, torch.float32):
-            raise TypeError(f"residual must have x's type {x.dtype} or be float32, got {r_type}")
-        a.r_dtype = _DTYPES[r_type]
-    return a, r_type
+    if residual is None:
+        return x.dtype
+    if residual.shape != x.shape or residual.device != x.device:
+        raise ValueError(f"residual must have x's shape {tuple(x.shape)} and device")
+    if residual.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"residual must have x's type {x.dtype} or be float32, got {residual.dtype}")
+    return residual.dtype
 
 
-def _norm_run(a: _capi.RmsNormArgs, x, residual, y_ptr: int, y_stride: int, r_type, keep: list) -> Optional[torch.Tensor]:
-    a.x, a.x_stride = _flat(x, keep)
-    a.y, a.y_stride = y_ptr, y_stride
-    r = None
+def _norm_run(x, weight, eps: float, residual, y_dtype: int, y: torch.Tensor, y_stride: int, scale: Optional[torch.Tensor], norm: int = 1) -> Optional[torch.Tensor]:
+    D, keep, r, res, rp = x.shape[-1], [], None, (None, 0), None
+    r_type = _norm_types(x, residual)
     if residual is not None:
-        a.residual, a.residual_stride = _flat(residual, keep)
+        res = _flat(residual, keep)
         r = torch.empty(x.shape, dtype=r_type, device=x.device)
-        a.r, a.r_stride = r.data_ptr(), x.shape[-1]
-    a.stream = _stream(x.device)
-    _capi.rms_norm_fwd(a)
+        rp = r.data_ptr()
+    xp, xs = _flat(x, keep)
+    _capi.rms_norm_fwd(_capi.RmsNormArgs(
+        x.numel() // D, D, _DTYPES[x.dtype], _DTYPES[r_type], y_dtype, eps, norm, xp, xs, *res, rp, D, y.data_ptr(), y_stride,
+        None if scale is None else scale.data_ptr(), 0 if scale is None else scale.shape[-1], _param(weight, "weight", (D,), x.device, keep),
+        None, 0, None, 0, None, 0, None, 0, None, None, 0, _stream(x.device)))
     return r
 
 
+@_on_its_device
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5, *, residual: Optional[torch.Tensor] = None,
              out_dtype: Optional[torch.dtype] = None):
     """RMSNorm over the last dimension (1 to 16384 wide), with a residual's addition before it: r = x + residual, rounded to
     the residual's type (x's, or float32), y = r rsqrt(mean(r^2) + eps) weight. Returns ``y``, or ``(y, r)`` with a residual.
     ``out_dtype``: x's type, or float16 / bfloat16 for a float32 x. Math in float32; y and r are contiguous."""
-    _require_cuda(x)
-    keep: list = []
-    with _on(x.device):
-        a, r_type = _norm_args(x, weight, eps, residual, keep)
-        y_type = x.dtype if out_dtype is None else out_dtype
-        if y_type != x.dtype and not (x.dtype == torch.float32 and y_type in _TYPES):
-            raise TypeError(f"the norm takes {x.dtype} into its own type (and float32 into a 16-bit type), not into {y_type}")
-        a.y_dtype = _DTYPES[y_type]
-        y = torch.empty(x.shape, dtype=y_type, device=x.device)
-        r = _norm_run(a, x, residual, y.data_ptr(), x.shape[-1], r_type, keep)
+    _norm_types(x, residual)
+    y_type = x.dtype if out_dtype is None else out_dtype
+    if y_type != x.dtype and not (x.dtype == torch.float32 and y_type in _TYPES):
+        raise TypeError(f"the norm takes {x.dtype} into its own type (and float32 into a 16-bit type), not into {y_type}")
+    y = torch.empty(x.shape, dtype=y_type, device=x.device)
+    r = _norm_run(x, weight, eps, residual, _DTYPES[y_type], y, x.shape[-1], None)
     return y if residual is None else (y, r)
 
 
@@ -539,34 +532,27 @@ def _fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return q[..., :D] if D % 16 else q, torch.empty(*x.shape[:-1], (D + _BLOCK - 1) // _BLOCK, dtype=torch.float32, device=x.device)
 
 
+@_on_its_device
 def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5, *, residual: Optional[torch.Tensor] = None):
     """``rms_norm`` with an 8-bit output: ``(q, scale)``, or ``(q, scale, r)`` with a residual. Every 128 columns of a row have
     a float32 scale = max(amax |y|, 1e-30) / 448 in ``scale`` [..., ceil(D / 128)], and ``q`` (float8_e4m3fn) is y / scale
     rounded to the nearest: what ``scaled_matmul`` multiplies with."""
-    _require_cuda(x)
-    keep: list = []
-    with _on(x.device):
-        a, r_type = _norm_args(x, weight, eps, residual, keep)
-        a.y_dtype = _capi.SUBQ_E4M3
-        q, scale = _fp8_rows(x)
-        a.scale, a.scale_stride = scale.data_ptr(), scale.shape[-1]
-        r = _norm_run(a, x, residual, q.data_ptr(), (x.shape[-1] + 15) // 16 * 16, r_type, keep)
+    _norm_types(x, residual)
+    q, scale = _fp8_rows(x)
+    r = _norm_run(x, weight, eps, residual, _capi.SUBQ_E4M3, q, (x.shape[-1] + 15) // 16 * 16, scale)
     return (q, scale) if residual is None else (q, scale, r)
 
 
+@_on_its_device
 def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x in 8 bits, ``(q, scale)`` as ``rms_norm_fp8`` gives them, without a norm (a projection's input)."""
-    _require_cuda(x)
-    keep: list = []
-    with _on(x.device):
-        a, r_type = _norm_args(x, None, 0.0, None, keep, norm=0)
-        a.y_dtype = _capi.SUBQ_E4M3
-        q, scale = _fp8_rows(x)
-        a.scale, a.scale_stride = scale.data_ptr(), scale.shape[-1]
-        _norm_run(a, x, None, q.data_ptr(), (x.shape[-1] + 15) // 16 * 16, r_type, keep)
+    _norm_types(x, None)
+    q, scale = _fp8_rows(x)
+    _norm_run(x, None, 0.0, None, _capi.SUBQ_E4M3, q, (x.shape[-1] + 15) // 16 * 16, scale, norm=0)
     return q, scale
 
 
+@_on_its_device
 def rms_norm_backward(dy: torch.Tensor, r: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5, *,
                       dresidual: Optional[torch.Tensor] = None, need_dweight: bool = True
                       ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
@@ -578,27 +564,22 @@ def rms_norm_backward(dy: torch.Tensor, r: torch.Tensor, weight: Optional[torch.
     keep: list = []
     if dy.shape != r.shape or dy.device != r.device:
         raise ValueError("rms_norm_backward needs dy and r of one shape on one device")
-    with _on(r.device):
-        a, _ = _norm_args(dy, weight, eps, r, keep)
-        a.y_dtype = a.x_dtype
-        a.r, a.r_stride = _flat(r, keep)
-        a.dy, a.dy_stride = _flat(dy, keep)
-        if dresidual is not None:
-            if dresidual.shape != r.shape or dresidual.device != r.device or dresidual.dtype != r.dtype:
-                raise ValueError("dresidual must have r's shape, type and device")
-            a.dr_next, a.dr_next_stride = _flat(dresidual, keep)
-        D = r.shape[-1]
-        dres = torch.empty(r.shape, dtype=r.dtype, device=r.device)
-        dx = dres if dy.dtype == r.dtype else torch.empty(r.shape, dtype=dy.dtype, device=r.device)
-        a.dres, a.dres_stride = dres.data_ptr(), D
-        if dx is not dres:
-            a.dx, a.dx_stride = dx.data_ptr(), D
-        dw = torch.empty(D, dtype=torch.float32, device=r.device) if need_dweight else None
-        if dw is not None:
-            a.dweight = dw.data_ptr()
-            a.workspace, a.workspace_bytes = _workspace(_capi.rms_norm_bwd_workspace_bytes(a), r.device, keep)
-        a.stream = _stream(r.device)
-        _capi.rms_norm_bwd(a)
+    r_type, D = _norm_types(dy, r), r.shape[-1]
+    (rp, rs), (gp, gs), (np_, ns) = _flat(r, keep), _flat(dy, keep), (None, 0)
+    if dresidual is not None:
+        if dresidual.shape != r.shape or dresidual.device != r.device or dresidual.dtype != r_type:
+            raise ValueError("dresidual must have r's shape, type and device")
+        np_, ns = _flat(dresidual, keep)
+    dres = torch.empty(r.shape, dtype=r_type, device=r.device)
+    dx = dres if dy.dtype == r_type else torch.empty(r.shape, dtype=dy.dtype, device=r.device)
+    dw = torch.empty(D, dtype=torch.float32, device=r.device) if need_dweight else None
+    a = _capi.RmsNormArgs(
+        r.numel() // D, D, _DTYPES[dy.dtype], _DTYPES[r_type], _DTYPES[dy.dtype], eps, 1, None, 0, None, 0, rp, rs, None, 0, None, 0,
+        _param(weight, "weight", (D,), r.device, keep), gp, gs, np_, ns, None if dx is dres else dx.data_ptr(), D, dres.data_ptr(), D,
+        None if dw is None else dw.data_ptr(), None, 0, _stream(r.device))
+    if dw is not None:
+        a.workspace, a.workspace_bytes = _workspace(_capi.rms_norm_bwd_workspace_bytes(a), r.device, keep)
+    _capi.rms_norm_bwd(a)
     return dx, dres, dw
 
 
@@ -619,7 +600,14 @@ def quantize_fp8_weight(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tenso
     return q.contiguous().to(_E4M3)[:, :K], scale
 
 
-def _fp8_matrix(t: torch.Tensor, name: str, keep: list) -> Tuple[int, int]:
+def _rows(shape) -> int:
+    n = 1
+    for x in shape[:-1]:
+        n *= x
+    return n
+
+
+def _fp8_matrix(t: torch.Tensor, keep: list) -> Tuple[int, int]:
     """(address, row stride) of t as [rows, K], rows on 16-byte boundaries: t itself where it has them, else a copy."""
     K = t.shape[-1]
     if t.dim() != 2:
@@ -633,6 +621,7 @@ def _fp8_matrix(t: torch.Tensor, name: str, keep: list) -> Tuple[int, int]:
     return t.data_ptr(), t.stride(0)
 
 
+@_on_its_device
 def scaled_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
                   out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The projection of an 8-bit input with 8-bit weights: out = a b^T + bias, a [..., K] and b [N, K] float8_e4m3fn with float32
@@ -657,29 +646,22 @@ def scaled_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_sca
     if any(t.device != dev for t in (b, a_scale, b_scale)):
         raise ValueError("the operands and their scales must be on one device")
     keep: list = []
-    with _on(dev):
-        s = _capi.ScaledMatmulArgs()
-        M = 1
-        for n in a.shape[:-1]:
-            M *= n
-        s.M, s.N, s.K, s.out_dtype = M, N, K, _DTYPES[out_dtype]
-        if out is None:
-            out = torch.empty(*a.shape[:-1], N, dtype=out_dtype, device=dev)
-            s.out, s.out_stride = out.data_ptr(), N
-        else:
-            if out.shape != a.shape[:-1] + (N,) or out.dtype != out_dtype or out.device != dev:
-                raise ValueError(f"out must be {tuple(a.shape[:-1]) + (N,)} of {out_dtype} on the device of a")
-            flat = out.view(-1, N) if N else out
-            if N > 1 and flat.stride(-1) != 1:
-                raise ValueError("out must have a contiguous last dimension")
-            s.out, s.out_stride = out.data_ptr(), flat.stride(0) if M > 1 else N
-        if M and N:
-            if K:
-                s.a, s.a_stride = _fp8_matrix(a, "a", keep)
-                s.b, s.b_stride = _fp8_matrix(b, "b", keep)
-                s.a_scale, s.a_scale_stride = _flat(a_scale, keep)
-                s.b_scale, s.b_scale_stride = _flat(b_scale, keep)
-            s.bias = _param(bias, "bias", (N,), dev, keep)
-            s.stream = _stream(dev)
-            _capi.scaled_matmul(s)
+    M = _rows(a.shape)
+    if out is None:
+        out = torch.empty(*a.shape[:-1], N, dtype=out_dtype, device=dev)
+        out_stride = N
+    else:
+        if out.shape != a.shape[:-1] + (N,) or out.dtype != out_dtype or out.device != dev:
+            raise ValueError(f"out must be {tuple(a.shape[:-1]) + (N,)} of {out_dtype} on the device of a")
+        flat = out.view(-1, N) if N else out
+        if N > 1 and flat.stride(-1) != 1:
+            raise ValueError("out must have a contiguous last dimension")
+        out_stride = flat.stride(0) if M > 1 else N
+    if M and N:
+        ap, a_s, bp, b_s, sap, sa_s, sbp, sb_s = None, 0, None, 0, None, 0, None, 0
+        if K:
+            (ap, a_s), (bp, b_s) = _fp8_matrix(a, keep), _fp8_matrix(b, keep)
+            (sap, sa_s), (sbp, sb_s) = _flat(a_scale, keep), _flat(b_scale, keep)
+        _capi.scaled_matmul(_capi.ScaledMatmulArgs(M, N, K, _DTYPES[out_dtype], ap, a_s, sap, sa_s, bp, b_s, sbp, sb_s, _param(bias, "bias", (N,), dev, keep),
+                                                   out.data_ptr(), out_stride, _stream(dev)))
     return out
