@@ -27,6 +27,15 @@ from .autograd import (
     chunkwise_flash_linear_attention,
 )
 from .delta import SubQGatedDeltaAttention, SubQLayerNorm, gated_delta_attention, layer_norm
+from .state_space import (
+    SubQFp8Linear,
+    SubQRMSNorm,
+    SubQSelectiveStateSpace,
+    SubQStateSpaceBlock,
+    causal_conv,
+    rms_norm,
+    selective_scan,
+)
 from .surgery import SubQAttentionOutput, SubQBypassAttention, bypass_transformer_with_subq
 
 sys.modules.setdefault("subq_engine", _C)
@@ -58,6 +67,7 @@ __all__: List[str] = [
     "_C", "SubQEngine", "AudioStreamBuffer", "get_device_info", "AudioTransformerEngine", "Engine",
     "SubQuadraticAttention", "SubQLinearAttention", "SubQAttentionFunction", "chunkwise_flash_linear_attention",
     "gated_delta_attention", "SubQGatedDeltaAttention", "layer_norm", "SubQLayerNorm",
+    "selective_scan", "causal_conv", "rms_norm", "SubQSelectiveStateSpace", "SubQStateSpaceBlock", "SubQRMSNorm", "SubQFp8Linear",
     "bypass_transformer_with_subq", "SubQBypassAttention", "SubQAttentionOutput",
     "setup_distributed", "cleanup_distributed", "wrap_model_ddp", "create_distributed_dataloader",
     "load", "generate", "__version__",

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -75,13 +76,13 @@ def _param(w: Optional[torch.Tensor], name: str, shape: tuple, device: torch.dev
     """A float32 parameter's address (converted where it has another type or layout)."""
     if w is None:
         return None
-    if tuple(w.shape) != shape:
+    if w.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(w.shape)}")
     if w.device != device:
         raise ValueError(f"{name} must be on the device of the inputs")
-    if not w.is_floating_point():
-        raise TypeError(f"{name} must be a floating-point tensor, got {w.dtype}")
-    if w.dtype != torch.float32 or not w.is_contiguous():
+    if w.dtype is not torch.float32 or not w.is_contiguous():
+        if not w.is_floating_point():
+            raise TypeError(f"{name} must be a floating-point tensor, got {w.dtype}")
         w = w.detach().to(torch.float32).contiguous()
         keep.append(w)
     return w.data_ptr()
@@ -90,7 +91,7 @@ def _param(w: Optional[torch.Tensor], name: str, shape: tuple, device: torch.dev
 def _check_seq(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
     if t.shape != like.shape:
         raise ValueError(f"{name} must have shape {tuple(like.shape)}, got {tuple(t.shape)}")
-    if t.dtype != like.dtype:
+    if t.dtype is not like.dtype:
         raise TypeError(f"{name} must have type {like.dtype}, got {t.dtype}")
     if t.device != like.device:
         raise ValueError(f"{name} must be on the device {like.device}")
@@ -495,9 +496,9 @@ def _norm_types(x: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.dtyp
     return residual.dtype
 
 
-def _norm_run(x, weight, eps: float, residual, y_dtype: int, y: torch.Tensor, y_stride: int, scale: Optional[torch.Tensor], norm: int = 1) -> Optional[torch.Tensor]:
+def _norm_run(x, weight, eps: float, residual, r_type, y_dtype: int, y: torch.Tensor, y_stride: int, scale: Optional[torch.Tensor], norm: int = 1
+              ) -> Optional[torch.Tensor]:
     D, keep, r, res, rp = x.shape[-1], [], None, (None, 0), None
-    r_type = _norm_types(x, residual)
     if residual is not None:
         res = _flat(residual, keep)
         r = torch.empty(x.shape, dtype=r_type, device=x.device)
@@ -516,20 +517,20 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     """RMSNorm over the last dimension (1 to 16384 wide), with a residual's addition before it: r = x + residual, rounded to
     the residual's type (x's, or float32), y = r rsqrt(mean(r^2) + eps) weight. Returns ``y``, or ``(y, r)`` with a residual.
     ``out_dtype``: x's type, or float16 / bfloat16 for a float32 x. Math in float32; y and r are contiguous."""
-    _norm_types(x, residual)
+    r_type = _norm_types(x, residual)
     y_type = x.dtype if out_dtype is None else out_dtype
     if y_type != x.dtype and not (x.dtype == torch.float32 and y_type in _TYPES):
         raise TypeError(f"the norm takes {x.dtype} into its own type (and float32 into a 16-bit type), not into {y_type}")
     y = torch.empty(x.shape, dtype=y_type, device=x.device)
-    r = _norm_run(x, weight, eps, residual, _DTYPES[y_type], y, x.shape[-1], None)
+    r = _norm_run(x, weight, eps, residual, r_type, _DTYPES[y_type], y, x.shape[-1], None)
     return y if residual is None else (y, r)
 
 
 def _fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Empty e4m3 rows of x's shape that start on 16-byte boundaries (what ``scaled_matmul`` reads as it is), and their scales."""
-    D = x.shape[-1]
-    q = torch.empty(*x.shape[:-1], (D + 15) // 16 * 16, dtype=_E4M3, device=x.device)
-    return q[..., :D] if D % 16 else q, torch.empty(*x.shape[:-1], (D + _BLOCK - 1) // _BLOCK, dtype=torch.float32, device=x.device)
+    *lead, D = x.shape
+    q = torch.empty((*lead, (D + 15) // 16 * 16), dtype=_E4M3, device=x.device)
+    return q[..., :D] if D % 16 else q, torch.empty((*lead, (D + _BLOCK - 1) // _BLOCK), dtype=torch.float32, device=x.device)
 
 
 @_on_its_device
@@ -537,9 +538,9 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: fl
     """``rms_norm`` with an 8-bit output: ``(q, scale)``, or ``(q, scale, r)`` with a residual. Every 128 columns of a row have
     a float32 scale = max(amax |y|, 1e-30) / 448 in ``scale`` [..., ceil(D / 128)], and ``q`` (float8_e4m3fn) is y / scale
     rounded to the nearest: what ``scaled_matmul`` multiplies with."""
-    _norm_types(x, residual)
+    r_type = _norm_types(x, residual)
     q, scale = _fp8_rows(x)
-    r = _norm_run(x, weight, eps, residual, _capi.SUBQ_E4M3, q, (x.shape[-1] + 15) // 16 * 16, scale)
+    r = _norm_run(x, weight, eps, residual, r_type, _capi.SUBQ_E4M3, q, (x.shape[-1] + 15) // 16 * 16, scale)
     return (q, scale) if residual is None else (q, scale, r)
 
 
@@ -548,7 +549,7 @@ def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x in 8 bits, ``(q, scale)`` as ``rms_norm_fp8`` gives them, without a norm (a projection's input)."""
     _norm_types(x, None)
     q, scale = _fp8_rows(x)
-    _norm_run(x, None, 0.0, None, _capi.SUBQ_E4M3, q, (x.shape[-1] + 15) // 16 * 16, scale, norm=0)
+    _norm_run(x, None, 0.0, None, x.dtype, _capi.SUBQ_E4M3, q, (x.shape[-1] + 15) // 16 * 16, scale, norm=0)
     return q, scale
 
 
@@ -600,16 +601,11 @@ def quantize_fp8_weight(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tenso
     return q.contiguous().to(_E4M3)[:, :K], scale
 
 
-def _rows(shape) -> int:
-    n = 1
-    for x in shape[:-1]:
-        n *= x
-    return n
-
-
 def _fp8_matrix(t: torch.Tensor, keep: list) -> Tuple[int, int]:
     """(address, row stride) of t as [rows, K], rows on 16-byte boundaries: t itself where it has them, else a copy."""
     K = t.shape[-1]
+    if K % 16 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t.data_ptr(), K
     if t.dim() != 2:
         t = t.reshape(-1, K)
         keep.append(t)
@@ -629,30 +625,30 @@ def scaled_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_sca
     [ceil(N / 128), ceil(K / 128)] for every 128 x 128 of b (``quantize_fp8_weight``). Sums in float32; out [..., N] is
     float32, float16 or bfloat16. Rows that do not start on 16-byte boundaries are copied first (the quantising calls
     give rows that do). ``out`` is contiguous in its last dimension and shares no memory with the inputs."""
-    _require_cuda(a, b, a_scale, b_scale)
-    if a.dtype != _E4M3 or b.dtype != _E4M3:
+    if a.dtype is not _E4M3 or b.dtype is not _E4M3:
         raise TypeError(f"scaled_matmul takes float8_e4m3fn operands, got {a.dtype} and {b.dtype}")
     if out_dtype not in _TYPES:
         raise TypeError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
-    if a.dim() < 1 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
+    *lead, K = a.shape
+    if b.dim() != 2 or K != b.shape[1]:
         raise ValueError(f"shape mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}")
-    N, K = b.shape
-    nk, nb = (K + _BLOCK - 1) // _BLOCK, (N + _BLOCK - 1) // _BLOCK
-    if a_scale.shape != a.shape[:-1] + (nk,) or tuple(b_scale.shape) != (nb, nk):
-        raise ValueError(f"a_scale must be {tuple(a.shape[:-1]) + (nk,)} and b_scale {(nb, nk)}, got {tuple(a_scale.shape)} and {tuple(b_scale.shape)}")
-    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+    N, nk = b.shape[0], (K + _BLOCK - 1) // _BLOCK
+    if a_scale.shape != (*lead, nk) or b_scale.shape != ((N + _BLOCK - 1) // _BLOCK, nk):
+        raise ValueError(f"a_scale must be {(*lead, nk)} and b_scale {((N + _BLOCK - 1) // _BLOCK, nk)}, got {tuple(a_scale.shape)} and {tuple(b_scale.shape)}")
+    if a_scale.dtype is not torch.float32 or b_scale.dtype is not torch.float32:
         raise TypeError("scales must be float32")
     dev = a.device
-    if any(t.device != dev for t in (b, a_scale, b_scale)):
+    if not a.get_device() == b.get_device() == a_scale.get_device() == b_scale.get_device():
+        _require_cuda(b, a_scale, b_scale)
         raise ValueError("the operands and their scales must be on one device")
     keep: list = []
-    M = _rows(a.shape)
+    M = lead[0] if len(lead) == 1 else math.prod(lead)
     if out is None:
-        out = torch.empty(*a.shape[:-1], N, dtype=out_dtype, device=dev)
+        out = torch.empty((*lead, N), dtype=out_dtype, device=dev)
         out_stride = N
     else:
-        if out.shape != a.shape[:-1] + (N,) or out.dtype != out_dtype or out.device != dev:
-            raise ValueError(f"out must be {tuple(a.shape[:-1]) + (N,)} of {out_dtype} on the device of a")
+        if out.shape != (*lead, N) or out.dtype != out_dtype or out.device != dev:
+            raise ValueError(f"out must be {(*lead, N)} of {out_dtype} on the device of a")
         flat = out.view(-1, N) if N else out
         if N > 1 and flat.stride(-1) != 1:
             raise ValueError("out must have a contiguous last dimension")

@@ -237,3 +237,159 @@ def _layer_norm_bwd_fake(dy, x, weight, eps, need_dweight, need_dbias):
     D = x.shape[-1]
     return (torch.empty(x.shape, dtype=x.dtype, device=x.device), _empty_f32(x, (D if need_dweight else 0,)),
             _empty_f32(x, (D if need_dbias else 0,)))
+
+
+# The selective scan and its gradients:
+#     out, S, handover = torch.ops.subq_audio.selective_scan_fwd(u, dt, A, B, C, D, z, dt_bias, mask, S0, dt_softplus, want_state,
+#                                                                want_handover)
+#     du, ddt, dA, dB, dC, dD, dz, ddt_bias, dS0 = torch.ops.subq_audio.selective_scan_bwd(u, dt, A, B, C, dout, D, z, dt_bias,
+#                                                                mask, S0, dS, dt_softplus, handover, need_dS0)
+# (shapes as in ops.selective_scan_forward). What a call does not produce is an empty tensor; an empty handover lets the
+# backward form it again.
+def _scan_groups(B: Tensor) -> int:
+    return B.shape[2] if B.dim() == 4 else 1
+
+
+def _scan_handover(u: Tensor, A: Tensor, B: Tensor) -> int:
+    d = _capi.SelectiveDesc()
+    d.batch, d.seq_len, d.channels, d.states, d.groups = *u.shape, A.shape[1], _scan_groups(B)
+    d.dtype, d.A = ops._DTYPES[u.dtype], _FAKE_PTR
+    return _capi.selective_scan_handover_bytes(d)
+
+
+@torch.library.custom_op("subq_audio::selective_scan_fwd", mutates_args=(), device_types="cuda")
+def selective_scan_fwd(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor], z: Optional[Tensor], dt_bias: Optional[Tensor],
+                       mask: Optional[Tensor], S0: Optional[Tensor], dt_softplus: bool, want_state: bool,
+                       want_handover: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    ho = ops.ScanHandover() if want_handover else None
+    y, S = ops.selective_scan_forward(u, dt, A, B, C, D=D, z=z, dt_bias=dt_bias, dt_softplus=dt_softplus, mask=mask, state=S0,
+                                      return_state=want_state, handover=ho)
+    return y, (S if want_state else _empty_f32(u, (0,))), (ho.buf if ho is not None else torch.empty(0, dtype=torch.uint8, device=u.device))
+
+
+@selective_scan_fwd.register_fake
+def _selective_scan_fwd_fake(u, dt, A, B, C, D, z, dt_bias, mask, S0, dt_softplus, want_state, want_handover):
+    S = _empty_f32(u, (u.shape[0], u.shape[2], A.shape[1]) if want_state else (0,))
+    return (torch.empty(u.shape, dtype=u.dtype, device=u.device), S,
+            torch.empty(_scan_handover(u, A, B) if want_handover else 0, dtype=torch.uint8, device=u.device))
+
+
+@torch.library.custom_op("subq_audio::selective_scan_bwd", mutates_args=(), device_types="cuda")
+def selective_scan_bwd(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, dout: Tensor, D: Optional[Tensor], z: Optional[Tensor],
+                       dt_bias: Optional[Tensor], mask: Optional[Tensor], S0: Optional[Tensor], dS: Optional[Tensor], dt_softplus: bool, handover: Tensor,
+                       need_dS0: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    ho = None
+    if handover.numel() > 0:
+        ho = ops.ScanHandover()
+        ho.buf, ho.key = handover, (tuple(u.shape), A.shape[1], _scan_groups(B), u.dtype, u.device)
+    g = ops.selective_scan_backward(u, dt, A, B, C, dout, D=D, z=z, dt_bias=dt_bias, dt_softplus=dt_softplus, mask=mask, state=S0, dstate=dS,
+                                    need_dstate=need_dS0, handover=ho)
+    return tuple(x if x is not None else _empty_f32(u, (0,)) for x in g)
+
+
+@selective_scan_bwd.register_fake
+def _selective_scan_bwd_fake(u, dt, A, B, C, dout, D, z, dt_bias, mask, S0, dS, dt_softplus, handover, need_dS0):
+    def like(t):
+        return _empty_f32(u, (0,)) if t is None else torch.empty(t.shape, dtype=t.dtype, device=u.device)
+
+    Dn = u.shape[2]
+    return (like(u), like(dt), _empty_f32(u, A.shape), like(B), like(C), _empty_f32(u, (0 if D is None else Dn,)), like(z),
+            _empty_f32(u, (0 if dt_bias is None else Dn,)), _empty_f32(u, (u.shape[0], Dn, A.shape[1]) if need_dS0 else (0,)))
+
+
+# The short causal convolution:
+#     y, state = torch.ops.subq_audio.causal_conv_fwd(x, weight, bias, mask, state, activation, want_state)
+#     dx, dweight, dbias, dstate = torch.ops.subq_audio.causal_conv_bwd(x, weight, dout, bias, mask, state, dstate, activation, need_dstate)
+@torch.library.custom_op("subq_audio::causal_conv_fwd", mutates_args=(), device_types="cuda")
+def causal_conv_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], mask: Optional[Tensor], state: Optional[Tensor], activation: Optional[str],
+                    want_state: bool) -> Tuple[Tensor, Tensor]:
+    y, S = ops.causal_conv_forward(x, weight, bias, activation=activation, mask=mask, state=state, return_state=want_state)
+    return y, (S if want_state else x.new_empty(0))
+
+
+@causal_conv_fwd.register_fake
+def _causal_conv_fwd_fake(x, weight, bias, mask, state, activation, want_state):
+    S = x.new_empty((x.shape[0], weight.shape[1] - 1, x.shape[2]) if want_state else (0,))
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device), S
+
+
+@torch.library.custom_op("subq_audio::causal_conv_bwd", mutates_args=(), device_types="cuda")
+def causal_conv_bwd(x: Tensor, weight: Tensor, dout: Tensor, bias: Optional[Tensor], mask: Optional[Tensor], state: Optional[Tensor],
+                    dstate: Optional[Tensor], activation: Optional[str], need_dstate: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    dx, dw, db, ds = ops.causal_conv_backward(x, weight, dout, bias, activation=activation, mask=mask, state=state, dstate=dstate, need_dstate=need_dstate)
+    return dx, dw, (db if db is not None else _empty_f32(x, (0,))), (ds if ds is not None else x.new_empty(0))
+
+
+@causal_conv_bwd.register_fake
+def _causal_conv_bwd_fake(x, weight, dout, bias, mask, state, dstate, activation, need_dstate):
+    D, W = weight.shape
+    return (torch.empty(x.shape, dtype=x.dtype, device=x.device), _empty_f32(x, (D, W)), _empty_f32(x, (0 if bias is None else D,)),
+            x.new_empty((x.shape[0], W - 1, D) if need_dstate else (0,)))
+
+
+# RMSNorm with a residual's addition (r is empty without one), and its gradients from r (dx is empty where it is dres):
+#     y, r = torch.ops.subq_audio.rms_norm_fwd(x, weight, residual, eps, out_dtype)
+#     dres, dx, dweight = torch.ops.subq_audio.rms_norm_bwd(dy, r, weight, dr, eps, need_dweight)
+@torch.library.custom_op("subq_audio::rms_norm_fwd", mutates_args=(), device_types="cuda")
+def rms_norm_fwd(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float, out_dtype: Optional[torch.dtype]) -> Tuple[Tensor, Tensor]:
+    got = ops.rms_norm(x, weight, eps, residual=residual, out_dtype=out_dtype)
+    return got if residual is not None else (got, x.new_empty(0))
+
+
+@rms_norm_fwd.register_fake
+def _rms_norm_fwd_fake(x, weight, residual, eps, out_dtype):
+    r = x.new_empty(0) if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    return torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device), r
+
+
+@torch.library.custom_op("subq_audio::rms_norm_bwd", mutates_args=(), device_types="cuda")
+def rms_norm_bwd(dy: Tensor, r: Tensor, weight: Optional[Tensor], dr: Optional[Tensor], eps: float, need_dweight: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    dx, dres, dw = ops.rms_norm_backward(dy, r, weight, eps, dresidual=dr, need_dweight=need_dweight)
+    return dres, (dx if dx is not dres else dy.new_empty(0)), (dw if dw is not None else _empty_f32(r, (0,)))
+
+
+@rms_norm_bwd.register_fake
+def _rms_norm_bwd_fake(dy, r, weight, dr, eps, need_dweight):
+    dres = torch.empty(r.shape, dtype=r.dtype, device=r.device)
+    dx = dy.new_empty(0) if dy.dtype == r.dtype else torch.empty(r.shape, dtype=dy.dtype, device=r.device)
+    return dres, dx, _empty_f32(r, (r.shape[-1] if need_dweight else 0,))
+
+
+# The 8-bit forms (for inference: no gradients):
+#     q, scale, r = torch.ops.subq_audio.rms_norm_fp8(x, weight, residual, eps)
+#     q, scale = torch.ops.subq_audio.quantize_fp8(x)
+#     out = torch.ops.subq_audio.scaled_matmul(a, a_scale, b, b_scale, bias, out_dtype)
+def _fp8_fake(x):
+    q, scale = ops.block_ops._fp8_rows(x)
+    return q, scale
+
+
+@torch.library.custom_op("subq_audio::rms_norm_fp8", mutates_args=(), device_types="cuda")
+def rms_norm_fp8(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    got = ops.rms_norm_fp8(x, weight, eps, residual=residual)
+    return got if residual is not None else (*got, x.new_empty(0))
+
+
+@rms_norm_fp8.register_fake
+def _rms_norm_fp8_fake(x, weight, residual, eps):
+    return (*_fp8_fake(x), x.new_empty(0) if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device))
+
+
+@torch.library.custom_op("subq_audio::quantize_fp8", mutates_args=(), device_types="cuda")
+def quantize_fp8(x: Tensor) -> Tuple[Tensor, Tensor]:
+    return ops.quantize_fp8(x)
+
+
+@quantize_fp8.register_fake
+def _quantize_fp8_fake(x):
+    return _fp8_fake(x)
+
+
+@torch.library.custom_op("subq_audio::scaled_matmul", mutates_args=(), device_types="cuda")
+def scaled_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+    return ops.scaled_matmul(a, a_scale, b, b_scale, bias=bias, out_dtype=out_dtype)
+
+
+@scaled_matmul.register_fake
+def _scaled_matmul_fake(a, a_scale, b, b_scale, bias, out_dtype):
+    return torch.empty((*a.shape[:-1], b.shape[0]), dtype=out_dtype, device=a.device)

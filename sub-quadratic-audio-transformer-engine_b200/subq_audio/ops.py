@@ -781,6 +781,7 @@ def last_launches() -> int:
 
 
 # --------------------------------------------- a selective state space block (block_ops.py)
+from . import block_ops  # noqa: E402
 from .block_ops import (  # noqa: E402  (it uses what stands above)
     CausalConvStep, ScanHandover, SelectiveGrads, SelectiveScanStep, causal_conv_backward, causal_conv_forward, quantize_fp8,
     quantize_fp8_weight, rms_norm, rms_norm_backward, rms_norm_fp8, scaled_matmul, selective_scan_backward, selective_scan_forward)
