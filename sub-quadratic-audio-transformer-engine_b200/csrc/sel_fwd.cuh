@@ -287,19 +287,17 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 3 : 2) sel_seg_kernel(
 }
 
 // Token by token, without shared memory: a lane has four states of a channel and reads its token's values by itself. For
-// single tokens (the states' 8 N D bytes a sequence, or the launch) and calls of a few.
-template <typename T, int LPC>
+// single tokens (bound by the states' 8 N D bytes a sequence, or the launch) and calls of a few. WHOLE: four states are 16
+// bytes of the state and of A, and a piece of B and C.
+template <typename T, int LPC, bool WHOLE>
 __global__ void __launch_bounds__(kSelThreads) sel_step_kernel(const SelParams p) {
-    const int q = threadIdx.x & (LPC - 1);
-    const int64_t channel = ((int64_t)blockIdx.x * kSelThreads + threadIdx.x) / LPC;
-    const bool in = channel < (int64_t)p.B * p.D;
-    const int b = in ? (int)(channel / p.D) : 0, d = in ? (int)(channel - (int64_t)b * p.D) : 0, g = d / p.Dg;
-    const bool whole = p.N % 4 == 0;  // 16-byte accesses of the states (their base is aligned to 16 bytes, or N is not used so)
+    const int q = threadIdx.x & (LPC - 1), b = blockIdx.y;
+    const int d = (int)(blockIdx.x * (kSelThreads / LPC) + threadIdx.x / LPC);
+    const bool in = d < p.D, has = in && 4 * q < p.N;
+    const int64_t g = p.G == 1 || !in ? 0 : d / p.Dg;
     float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
     const int64_t sat = ((int64_t)b * p.D + d) * p.N + 4 * q;
-    const bool vec = whole && ((reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.S_out) | reinterpret_cast<uintptr_t>(p.A)) & 15) == 0;
-    if (vec) {
-        const bool has = in && 4 * q < p.N;
+    if (WHOLE) {
         const float4 a = has ? *reinterpret_cast<const float4*>(p.A + (int64_t)d * p.N + 4 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
         const float4 x = has && p.S_in ? *reinterpret_cast<const float4*>(p.S_in + sat) : make_float4(0.f, 0.f, 0.f, 0.f);
         A2[0] = a.x * kLog2e; A2[1] = a.y * kLog2e; A2[2] = a.z * kLog2e; A2[3] = a.w * kLog2e;
@@ -311,29 +309,34 @@ __global__ void __launch_bounds__(kSelThreads) sel_step_kernel(const SelParams p
             if (in && p.S_in && 4 * q + i < p.N) h[i] = p.S_in[sat + i];
     }
     const float bias = in && p.dt_bias ? p.dt_bias[d] : 0.f, Dw = in && p.Dw ? p.Dw[d] : 0.f;
+    const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
+    F2 h01 = f2(h[0], h[1]), h23 = f2(h[2], h[3]);
     for (int l = 0; l < p.L; ++l) {
         const bool live = in && live_at<T>(p, b, l);
         float y = 0.f, u = 0.f, z = 0.f;
         if (live) {
+            Piece<T, 4> Bp, Cp;
+            Bp.zero();
+            Cp.zero();
+            const T* Bat = row_of<T>(p.Bm, b, l, 0) + g * p.Bm.sg + 4 * q;
+            const T* Cat = row_of<T>(p.C, b, l, 0) + g * p.C.sg + 4 * q;
+            if (has) {
+                if (WHOLE) {
+                    Bp.load(Bat);
+                    Cp.load(Cat);
+                } else {
+                    Bp.load(Bat, p.N - 4 * q, false);
+                    Cp.load(Cat, p.N - 4 * q, false);
+                }
+            }
             u = to_f<T>(*row_of<T>(p.u, b, l, d));
             float dt = to_f<T>(*row_of<T>(p.dt, b, l, d)) + bias;
             if (p.z.p) z = to_f<T>(*row_of<T>(p.z, b, l, d));
-            const T* Bp = row_of<T>(p.Bm, b, l, 0) + g * p.Bm.sg + 4 * q;
-            const T* Cp = row_of<T>(p.C, b, l, 0) + g * p.C.sg + 4 * q;
-            float Bv[4], Cv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool has = 4 * q + i < p.N;
-                Bv[i] = has ? to_f<T>(Bp[i]) : 0.f;
-                Cv[i] = has ? to_f<T>(Cp[i]) : 0.f;
-            }
             if (p.softplus) dt = softplus(dt);
-            const float du = dt * u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                h[i] = fmaf(du, Bv[i], decayed(dt * A2[i], h[i]));
-                y = fmaf(Cv[i], h[i], y);
-            }
+            const F2 dt2 = f2(dt), du = f2(dt * u);
+            h01 = fma(du, f2(to_f<T>(Bp.x[0]), to_f<T>(Bp.x[1])), decayed(factor(mul(dt2, A01)), h01));
+            h23 = fma(du, f2(to_f<T>(Bp.x[2]), to_f<T>(Bp.x[3])), decayed(factor(mul(dt2, A23)), h23));
+            y = both(fma(h23, f2(to_f<T>(Cp.x[2]), to_f<T>(Cp.x[3])), mul(h01, f2(to_f<T>(Cp.x[0]), to_f<T>(Cp.x[1])))));
         }
 #pragma unroll
         for (int o = 1; o < LPC; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
@@ -343,9 +346,11 @@ __global__ void __launch_bounds__(kSelThreads) sel_step_kernel(const SelParams p
             *const_cast<T*>(row_of<T>(p.out, b, l, d)) = from_f<T>(live ? y : 0.f);
         }
     }
-    if (in && p.S_out) {
-        if (vec) {
-            if (4 * q < p.N) *reinterpret_cast<float4*>(p.S_out + sat) = make_float4(h[0], h[1], h[2], h[3]);
+    if (has && p.S_out) {
+        get(h01, h[0], h[1]);
+        get(h23, h[2], h[3]);
+        if (WHOLE) {
+            *reinterpret_cast<float4*>(p.S_out + sat) = make_float4(h[0], h[1], h[2], h[3]);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -401,8 +406,13 @@ template <typename T>
 cudaError_t launch_step(const SelParams& p, cudaStream_t st) {
     return by_lanes(p.N, [&](auto lpc) {
         constexpr int LPC = decltype(lpc)::value;
-        const int64_t threads = (int64_t)p.B * p.D * LPC;
-        sel_step_kernel<T, LPC><<<(unsigned)((threads + kSelThreads - 1) / kSelThreads), kSelThreads, 0, st>>>(p);
+        const dim3 grid((unsigned)((p.D + kSelThreads / LPC - 1) / (kSelThreads / LPC)), (unsigned)p.B);
+        const int need = 4 * (int)sizeof(T);
+        auto group_fits = [&](const SelTensor& t) { return t.vec >= need && t.sg * (int64_t)sizeof(T) % need == 0; };
+        const bool whole = p.N % 4 == 0 && group_fits(p.Bm) && group_fits(p.C) &&
+                           ((reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.S_out) | reinterpret_cast<uintptr_t>(p.A)) & 15) == 0;
+        if (whole) sel_step_kernel<T, LPC, true><<<grid, kSelThreads, 0, st>>>(p);
+        else sel_step_kernel<T, LPC, false><<<grid, kSelThreads, 0, st>>>(p);
         return cudaGetLastError();
     });
 }
