@@ -59,12 +59,12 @@ __device__ __forceinline__ bool near_border(float x) { return (__float_as_uint(x
 // y / scale of such values again in float64, from r and w themselves: the rows' norm is the same on both sides of the
 // quotient, so that q = 448 r w / max |r w|, exact but for two roundings of 2^-53. Rounded to float32 towards zero with the
 // last bit set where anything was cut off, which the rounding to e4m3 that follows sees on the right side.
-template <int V>
-__device__ __noinline__ void exact_quotients(float (&f)[V], const float (&r)[V], const float* w, int c, int n, bool near) {
+template <typename TR, int V>
+__device__ __forceinline__ void exact_quotients(float (&f)[V], const Piece<TR, V>& r, const float* w, int c, int n, bool near) {
     double t[V], top = 0.;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        t[i] = i < n ? (double)r[i] * (w ? (double)w[c + i] : 1.) : 0.;
+        t[i] = i < n ? (double)to_f<TR>(r.x[i]) * (w ? (double)w[c + i] : 1.) : 0.;
         top = fmax(top, fabs(t[i]));
     }
 #pragma unroll
@@ -73,7 +73,7 @@ __device__ __noinline__ void exact_quotients(float (&f)[V], const float (&r)[V],
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         if (!near_border(f[i])) continue;
-        const double q = 448. * t[i] / top;
+        const double q = 448. * t[i] / top;  // (the first product is exact: so is a value halfway between two)
         const float z = __double2float_rz(q);
         f[i] = (double)z == q ? z : __uint_as_float(__float_as_uint(z) | 1u);
     }
@@ -146,26 +146,20 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNo
     if (row < p.rows) load(row);
     for (; row < p.rows; row += step) {
         float f[K][V];  // r, then y, then y / scale
+        Piece<TR, V> r[K];
         float ss[1] = {0.f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = c0 + k * kStep, n = p.D - c;
-            Piece<TR, V> r;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 f[k][i] = to_f<TX>(nx[k].x[i]);
-                if (p.res) {
-                    r.x[i] = from_f<TR>(f[k][i] + to_f<TR>(nr[k].x[i]));
-                    f[k][i] = to_f<TR>(r.x[i]);
-                }
+                if (p.res) f[k][i] += to_f<TR>(nr[k].x[i]);
+                r[k].x[i] = from_f<TR>(f[k][i]);  // (without a residual a copy: TR holds x)
+                f[k][i] = to_f<TR>(r[k].x[i]);
                 ss[0] = fmaf(f[k][i], f[k][i], ss[0]);
             }
-            if (p.r && n > 0) {
-                if (!p.res)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) r.x[i] = from_f<TR>(f[k][i]);
-                rows_store<WHOLE>(r, static_cast<TR*>(p.r) + row * p.r_s + c, n);
-            }
+            if (p.r && n > 0) rows_store<WHOLE>(r[k], static_cast<TR*>(p.r) + row * p.r_s + c, n);
         }
         if (row + step < p.rows) load(row + step);
         float rms = 1.f;
@@ -173,45 +167,64 @@ __global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNo
             row_sums<NW, 1>(ss, red[group], in_row, group);
             rms = 1.f / sqrtf(ss[0] / (float)p.D + p.eps);
         }
+        if constexpr (std::is_same<TY, Fp8>::value) {
+            float top[K];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = c0 + k * kStep, n = p.D - c;
-            float rk[V], w[V];
-            weights<WHOLE>(p, c, n, w);
+            for (int k = 0; k < K; ++k) {
+                const int c = c0 + k * kStep, n = p.D - c;
+                float w[V];
+                weights<WHOLE>(p, c, n, w);
+                top[k] = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                rk[i] = f[k][i];
-                if (p.norm) f[k][i] *= rms;
-                if (p.w) f[k][i] *= w[i];
+                for (int i = 0; i < V; ++i) {
+                    f[k][i] = f[k][i] * rms * w[i];
+                    top[k] = max_nan(top[k], i < n ? fabsf(f[k][i]) : 0.f);
+                }
             }
-            if constexpr (std::is_same<TY, Fp8>::value) {
-                float top = 0.f;
 #pragma unroll
-                for (int i = 0; i < V; ++i) top = max_nan(top, i < n ? fabsf(f[k][i]) : 0.f);
+            for (int o = 8; o > 0; o >>= 1)
 #pragma unroll
-                for (int o = 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const float scale = __fdiv_rn(max_nan(top, 1e-30f), 448.f), inv = __fdiv_rn(448.f, max_nan(top, 1e-30f));
-                bool near = false;
+                for (int k = 0; k < K; ++k) top[k] = max_nan(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+            bool near[K], any = false;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int c = c0 + k * kStep, n = p.D - c;
+                const float inv = __fdiv_rn(448.f, max_nan(top[k], 1e-30f));
+                near[k] = false;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     f[k][i] *= inv;
-                    near |= near_border(f[k][i]);
+                    near[k] |= near_border(f[k][i]);
                 }
-                near = near && top > 1e-30f && top < INFINITY && n > 0;
-                if (__any_sync(0xffffffffu, near)) exact_quotients<V>(f[k], rk, p.w, c, n, near);
-                if (n > 0) {
-                    if ((lane & 15) == 0) p.scale[row * p.scale_s + c / 128] = scale;
-                    Piece<uint8_t, V> q;
+                near[k] = near[k] && top[k] > 1e-30f && top[k] < INFINITY && n > 0;
+                any |= near[k];
+            }
+            if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-                    for (int i = 0; i < V; i += 2)
-                        reinterpret_cast<__nv_fp8x2_storage_t*>(q.x)[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(f[k][i], f[k][i + 1]), __NV_SATFINITE, __NV_E4M3);
-                    uint8_t* to = static_cast<uint8_t*>(p.y) + row * p.y_s + c;
-                    rows_store<WHOLE>(q, to, n);
-                }
-            } else if (n > 0) {
+                for (int k = 0; k < K; ++k)
+                    if (__any_sync(0xffffffffu, near[k])) exact_quotients<TR, V>(f[k], r[k], p.w, c0 + k * kStep, p.D - c0 - k * kStep, near[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int c = c0 + k * kStep, n = p.D - c;
+                if (n <= 0) continue;
+                if ((lane & 15) == 0) p.scale[row * p.scale_s + c / 128] = __fdiv_rn(max_nan(top[k], 1e-30f), 448.f);
+                Piece<uint8_t, V> q;
+#pragma unroll
+                for (int i = 0; i < V; i += 2)
+                    reinterpret_cast<__nv_fp8x2_storage_t*>(q.x)[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(f[k][i], f[k][i + 1]), __NV_SATFINITE, __NV_E4M3);
+                rows_store<WHOLE>(q, static_cast<uint8_t*>(p.y) + row * p.y_s + c, n);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int c = c0 + k * kStep, n = p.D - c;
+                if (n <= 0) continue;
+                float w[V];
+                weights<WHOLE>(p, c, n, w);
                 Piece<TY, V> y;
 #pragma unroll
-                for (int i = 0; i < V; ++i) y.x[i] = from_f<TY>(f[k][i]);
+                for (int i = 0; i < V; ++i) y.x[i] = from_f<TY>(f[k][i] * rms * w[i]);
                 rows_store<WHOLE>(y, static_cast<TY*>(p.y) + row * p.y_s + c, n);
             }
         }
