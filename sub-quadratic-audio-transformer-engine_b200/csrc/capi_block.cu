@@ -96,8 +96,10 @@ int check_sel(const subq_selective_desc& d, SelParams& p) {
 // a CTA's time (at least 1.6 times: fewer warps than that leave it waiting), so what counts is how evenly the grid fills the
 // SMs. A segment costs `first` of the walk again for its sum in the launch before, 4 us for that launch, and a step of the
 // chain in front of the walk. In units of a CTA's 32 tokens, which take `tile` us when the SM is full; the least sum wins.
-// us, bf16, D = 1536, N = 16, one segment and as chosen:
-//   SPLIT_FIGURES
+// us of the forward, with one segment and as chosen (bf16, D = 1536, N = 16 where nothing else is said):
+//   1 x 65536 tokens 9263, 1509   1 x 4096 584, 125   4 x 2048 301, 206   8 x 2047, padded 452, 383   16 x 1024 303 (one is chosen)
+//   2 x 1537, D = 384, float32 214, 47   2 x 4096, D = 1024, N = 64 548, 517
+// and with its gradients: 8 x 1024 829, 672   2 x 1537, D = 384, float32 763, 134   2 x 1024, D = 1024, N = 64 540, 565 (misjudged)
 void sel_split(SelParams& p, bool back) {
     const int64_t ch = sel_channels(p.N), ctas = (int64_t)p.B * p.G * ((p.Dg + ch - 1) / ch), tiles = (p.L + kSelTile - 1) / kSelTile;
     if (ctas <= 0 || tiles <= 0) return;
@@ -252,8 +254,8 @@ int fill_conv(const subq_causal_conv_args* a, ConvParams& p, bool bwd) {
         (rc = aligned(a->state_in, es, "state_in")))
         return rc;
     if (p.D > 0 && !p.w) return fail(SUBQ_ERR_INVALID_ARGUMENT, "weight is null");
-    // (a CTA has 8 runs of 8 tokens; a grid at most 65535 rows of CTAs)
-    if ((int64_t)p.B * ((p.L + 7) / 8) > (int64_t)8 * 65535) return fail(SUBQ_ERR_UNSUPPORTED, "batch * seq_len is too large for one call (4,194,240 tokens)");
+    // (a CTA has 32 channels, or pieces of them, and 8 runs of 8 tokens)
+    if (((int64_t)p.B * ((p.L + 7) / 8) + 7) / 8 * ((p.D + 31) / 32) > 0x7fffffff) return fail(SUBQ_ERR_UNSUPPORTED, "batch * seq_len * channels is too large for one call");
     const int64_t window = (int64_t)p.B * (p.W - 1) * p.D * (int64_t)es, one = (int64_t)p.D * 4;
     if (!bwd) {
         p.S_out = a->state_out;

@@ -5,9 +5,11 @@
 //   dpre_t = dy_t act'(pre_t),   dx_s = sum_j w_j dpre_{s+W-1-j},   dw_j = sum_t dpre_t x_{t-W+1+j},   db = sum_t dpre_t.
 //
 // HBM-bound: a thread has four neighbouring channels (backward of 16-bit types: two; single ones where rows are not aligned) and a
-// run of eight tokens, all of whose rows it asks for at once, those of the tokens that its taps reach into among them (L1 has
+// run of eight tokens (backward: sixteen), all of whose rows it asks for at once, those of the tokens that its taps reach into among them (L1 has
 // them for the CTA's next run). The backward forms pre again from x; its dw and db are summed over a run, over the CTA's
 // eight runs in shared memory and then over CTAs by a second launch, in a fixed order.
+// 8 x 2047 x 1536 in bf16: forward 35 us (HBM floor 15), backward 86 us (23: nineteen sums before the activation for sixteen
+// tokens, and its derivative; instruction issue).
 #include <algorithm>
 
 #include "sel_common.cuh"
@@ -20,6 +22,7 @@ using sel::row_of;
 
 constexpr int kConvThreads = 256;
 constexpr int kRun = 8;   // tokens of a thread
+constexpr int kBack = 16;  // the same, backward (eight, at three CTAs an SM: 150 us for 133 of a step of 8 x 2047 x 1536)
 constexpr int kRows = 8;  // runs of a CTA, one after another
 
 template <typename T>
@@ -130,9 +133,9 @@ __device__ __forceinline__ void load_window(const ConvParams& p, int b, int t0, 
 
 // 32 channel pieces x 8 runs a CTA.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kConvThreads, 4) conv_fwd_kernel(const ConvParams p, int runs, int keep) {
-    const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * V;
-    const int64_t r = (int64_t)blockIdx.y * kRows + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(kConvThreads, 4) conv_fwd_kernel(const ConvParams p, int runs, int across, int keep) {
+    const int group = blockIdx.x / across, c = ((blockIdx.x - group * across) * 32 + (threadIdx.x & 31)) * V;
+    const int64_t r = (int64_t)group * kRows + (threadIdx.x >> 5);
     if (c >= p.D || r >= (int64_t)p.B * runs) return;
     const int b = (int)(r / runs), t0 = (int)(r - (int64_t)b * runs) * kRun;
     Piece<T, V> x[W - 1 + kRun];
@@ -258,11 +261,11 @@ __global__ void __launch_bounds__(kConvThreads) conv_ends_kernel(const ConvParam
 // 32 channel pieces x 8 runs. Gradients of the run's inputs (the first run's: of the carried window, too) and its part of
 // dw and db: the tokens behind the run whose taps reach into it are formed again.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kConvThreads, V == 4 ? 2 : 3) conv_bwd_kernel(const ConvParams p, const int* ends) {
+__global__ void __launch_bounds__(kConvThreads, 2) conv_bwd_kernel(const ConvParams p, const int* ends) {
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
     const int c = (blockIdx.x * 32 + lane) * V;
-    const int runs = (p.L + kRun - 1) / kRun;
-    constexpr int kTail = kRun + W - 1;
+    const int runs = (p.L + kBack - 1) / kBack;
+    constexpr int kTail = kBack + W - 1;
     constexpr int H = (V + 1) / 2;
     F2 dw[W][H], db[H];
 #pragma unroll
@@ -274,9 +277,9 @@ __global__ void __launch_bounds__(kConvThreads, V == 4 ? 2 : 3) conv_bwd_kernel(
     for (int turn = 0; turn < p.run; ++turn) {  // groups of eight runs
         const int64_t r = ((int64_t)blockIdx.y * p.run + turn) * kRows + row;
         if (c >= p.D || r >= (int64_t)p.B * runs) break;
-        const int b = (int)(r / runs), t0 = (int)(r - (int64_t)b * runs) * kRun, t1 = min(p.L, t0 + kRun);
+        const int b = (int)(r / runs), t0 = (int)(r - (int64_t)b * runs) * kBack, t1 = min(p.L, t0 + kBack);
         const int end = p.dS_out ? ends ? ends[b] : p.L : 0;
-        // tokens t0 - (W - 1) .. t0 + kRun + W - 2 of x, t0 .. of dy: the taps of the last ones reach into the run
+        // tokens t0 - (W - 1) .. t0 + kBack + W - 2 of x, t0 .. of dy: the taps of the last ones reach into the run
         Piece<T, V> x[W - 1 + kTail], g[kTail];
         load_rows<T, V, W - 1 + kTail>(p.x, p.L, b, t0 - (W - 1), c, x);
         load_rows<T, V, kTail>(p.dy, p.L, b, t0, c, g);
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(kConvThreads, V == 4 ? 2 : 3) conv_bwd_kernel(
                         const F2 sg = sel::sigmoid(pre);  // silu' = sg (1 + pre (1 - sg))
                         dp[at][i] = sel::mul(dp[at][i], sel::mul(sg, sel::fma(pre, sel::fma(sg, f2(-1.f), f2(1.f)), f2(1.f))));
                     }
-                if (k < kRun)
+                if (k < kBack)
 #pragma unroll
                     for (int i = 0; i < H; ++i) {
                         db[i] = sel::add(db[i], dp[at][i]);
@@ -415,7 +418,8 @@ cudaError_t conv_fwd(const ConvParams& p, cudaStream_t st, int* launches) {
         return cudaGetLastError();
     }
     const int runs = (p.L + kRun - 1) / kRun, keep = p.S_out && !p.mask && p.S_out != p.S_in && p.L >= W - 1;
-    conv_fwd_kernel<T, V, W><<<dim3((unsigned)((nv + 31) / 32), (unsigned)(((int64_t)p.B * runs + kRows - 1) / kRows)), kConvThreads, 0, st>>>(p, runs, keep);
+    const int across = (int)((nv + 31) / 32);
+    conv_fwd_kernel<T, V, W><<<(unsigned)(((int64_t)p.B * runs + kRows - 1) / kRows * across), kConvThreads, 0, st>>>(p, runs, across, keep);
     *launches = 1;
     if (p.S_out && !keep) {
         conv_window_kernel<T, W><<<dim3(blocks(p.D), p.B), kConvThreads, 0, st>>>(p);
@@ -460,11 +464,11 @@ cudaError_t conv_typed(const ConvParams& p, int dtype, bool bwd, cudaStream_t st
 cudaError_t launch_conv_fwd(const ConvParams& p, int dtype, cudaStream_t st, int* launches) { return conv_typed(p, dtype, false, st, launches); }
 cudaError_t launch_conv_bwd(const ConvParams& p, int dtype, cudaStream_t st, int* launches) { return conv_typed(p, dtype, true, st, launches); }
 
-// Groups of eight runs that a CTA goes through: one for each place on the card (three CTAs an SM) or so, so that there are few
+// Groups of eight runs that a CTA goes through: one for each place on the card (two CTAs an SM) or so, so that there are few
 // partial sums (and a grid has at most 65535 rows of CTAs).
 void conv_bwd_split(ConvParams& p) {
-    const int64_t groups = ((int64_t)p.B * ((p.L + kRun - 1) / kRun) + kRows - 1) / kRows, across = (p.D + 63) / 64;
-    const int64_t places = std::max<int64_t>(1, 4 * 444 / across);
+    const int64_t groups = ((int64_t)p.B * ((p.L + kBack - 1) / kBack) + kRows - 1) / kRows, across = (p.D + 63) / 64;
+    const int64_t places = std::max<int64_t>(1, 4 * 296 / across);
     p.run = (int)std::max<int64_t>(1, std::max((groups + 65534) / 65535, groups / places));
     p.parts = (int)((groups + p.run - 1) / p.run);
 }

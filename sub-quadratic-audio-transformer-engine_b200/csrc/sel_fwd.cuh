@@ -3,8 +3,9 @@
 // per token and channel and left in shared memory, the states stay in registers, and y goes back through shared memory to
 // the threads that hold u and z for the output. The next tile is on its way meanwhile.
 //
-// Bound by instruction issue and the exponential unit (one exponential and about nine packed or single operations a
-// state), not by memory. Few channels: the sequence is cut into segments; a first launch finds what each leaves of a zero
+// Bound by instruction issue and the FMA pipe (a state and token take one exponential, ten multiply-adds, half of them two at
+// a time, and three selections), not by memory: 65536 x 1536 channels of 16 states take 988 us and 518 us for the segments,
+// 124 us would be its bytes, 360 us its exponentials alone. Few channels: the sequence is cut into segments; a first launch finds what each leaves of a zero
 // state and the sum of its step sizes (a segment's decay is exp(A sum dt)), and the walk's CTAs chain those before theirs.
 #pragma once
 
