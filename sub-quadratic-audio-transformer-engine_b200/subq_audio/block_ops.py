@@ -32,6 +32,21 @@ def _stream(device: torch.device) -> int:
     return _raw_stream(device.index)
 
 
+_SIZES: dict = {}  # sizes in bytes that the library gave, by what they depend on
+
+
+def _size(query, args, *key) -> int:
+    """query(args), asked for once for each key (the call's sizes, which alone it depends on)."""
+    n = _SIZES.get((query, key))
+    if n is None:
+        n = query(args)
+        if n:  # (0 may also be the answer to arguments that the call will refuse)
+            if len(_SIZES) > 4096:
+                _SIZES.clear()
+            _SIZES[(query, key)] = n
+    return n
+
+
 def _on_its_device(call):
     """The call with the device of its first tensor as the current one."""
 
@@ -171,26 +186,24 @@ def causal_conv_backward(x: torch.Tensor, weight: torch.Tensor, dout: torch.Tens
     """Gradients of ``causal_conv_forward``: ``(dx, dweight, dbias | None, dstate | None)``, dx in x's type, dweight and
     dbias float32. ``dstate`` is the gradient of the returned state (None: 0); with ``need_dstate`` that of ``state`` comes
     back (in x's type)."""
-    _require_cuda(x, dout)
     x, dout = _inner_contig(x), _inner_contig(dout)
     _check_seq(dout, "dout", x)
     keep: list = []
     a = _conv_args(x, weight, bias, activation, mask, state, keep)
-    D, W = weight.shape
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = torch.empty((D, W), dtype=torch.float32, device=x.device)
-    db = torch.empty(D, dtype=torch.float32, device=x.device) if bias is not None else None
+    (B, L, D), W, dev = x.shape, weight.shape[1], x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dw = torch.empty((D, W), dtype=torch.float32, device=dev)
+    db = ds = None
     a.dy, a.dx, a.dweight = _t3(dout), _t3(dx), dw.data_ptr()
-    if db is not None:
+    if bias is not None:
+        db = torch.empty(D, dtype=torch.float32, device=dev)
         a.dbias = db.data_ptr()
     if dstate is not None:
         a.dstate_out = _window(dstate, "dstate", x, W, keep)
-    ds = None
     if need_dstate:
-        ds = torch.empty((x.shape[0], W - 1, D), dtype=x.dtype, device=x.device)
+        ds = torch.empty((B, W - 1, D), dtype=x.dtype, device=dev)
         a.dstate_in = ds.data_ptr()
-    a.stream = _stream(x.device)
-    a.workspace, a.workspace_bytes = _workspace(_capi.causal_conv_bwd_workspace_bytes(a), x.device, keep)
+    a.workspace, a.workspace_bytes = _workspace(_size(_capi.causal_conv_bwd_workspace_bytes, a, B, L, D, W), dev, keep)
     _capi.causal_conv_bwd(a)
     return dx, dw, db, ds
 
@@ -321,15 +334,12 @@ def _scan_inputs(u, dt, A, B, C, z):
     return G
 
 
-def _scan_desc(d: _capi.SelectiveDesc, u, A, D, dt_bias, dt_softplus, mask, G: int, keep: list) -> None:
+def _scan_desc(u, A, D, dt_bias, dt_softplus, mask, G: int, keep: list) -> _capi.SelectiveDesc:
     Bn, L, Dn = u.shape
-    d.batch, d.seq_len, d.channels, d.states, d.groups = Bn, L, Dn, A.shape[1], G
-    d.dtype = _DTYPES[u.dtype]
-    d.softplus = 1 if dt_softplus else 0
-    d.A = _param(A, "A", (Dn, A.shape[1]), u.device, keep)
-    d.D = _param(D, "D", (Dn,), u.device, keep)
-    d.dt_bias = _param(dt_bias, "dt_bias", (Dn,), u.device, keep)
-    d.mask, d.mask_stride_b = _mask(mask, Bn, L, u.device, keep)
+    dev = u.device
+    m, m_stride = (None, 0) if mask is None else _mask(mask, Bn, L, dev, keep)
+    return _capi.SelectiveDesc(Bn, L, Dn, A.shape[1], G, _DTYPES[u.dtype], 1 if dt_softplus else 0, _param(A, "A", (Dn, A.shape[1]), dev, keep),
+                               _param(D, "D", (Dn,), dev, keep), _param(dt_bias, "dt_bias", (Dn,), dev, keep), m, m_stride)
 
 
 def _state(state: Optional[torch.Tensor], name: str, u: torch.Tensor, N: int, keep: list) -> Optional[int]:
@@ -363,27 +373,26 @@ def selective_scan_forward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     u, dt, B, C = (_inner_contig(t) for t in (u, dt, B, C))
     z = None if z is None else _inner_contig(z)
     keep: list = []
-    a = _capi.SelectiveFwdArgs()
-    _scan_desc(a.desc, u, A, D, dt_bias, dt_softplus, mask, G, keep)
+    dev, N = u.device, A.shape[1]
     if out is None:
-        y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+        y = torch.empty(u.shape, dtype=u.dtype, device=dev)
     else:
         y = out
         _check_out(y, u)
-    a.u, a.dt, a.z, a.B, a.C, a.out = _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(y)
-    N = A.shape[1]
-    a.state_in = _state(state, "state", u, N, keep)
     new = None
     if return_state:
-        new = torch.empty((u.shape[0], u.shape[2], N), dtype=torch.float32, device=u.device)
-        a.state_out = new.data_ptr()
-    a.stream = _stream(u.device)
+        new = torch.empty((u.shape[0], u.shape[2], N), dtype=torch.float32, device=dev)
+    a = _capi.SelectiveFwdArgs(_scan_desc(u, A, D, dt_bias, dt_softplus, mask, G, keep), _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(y),
+                               _state(state, "state", u, N, keep), None if new is None else new.data_ptr(), None, None, 0, _stream(dev))
+    sizes = (*u.shape, N, G)
     if handover is not None:
-        handover.buf = torch.empty(_capi.selective_scan_handover_bytes(a.desc), dtype=torch.uint8, device=u.device)
-        handover.key = (tuple(u.shape), N, G, u.dtype, u.device)
+        handover.buf = torch.empty(_size(_capi.selective_scan_handover_bytes, a.desc, *sizes), dtype=torch.uint8, device=dev)
+        handover.key = (tuple(u.shape), N, G, u.dtype, dev)
         if handover.buf.numel():
             a.handover = handover.buf.data_ptr()
-    a.workspace, a.workspace_bytes = _workspace(_capi.selective_scan_fwd_workspace_bytes(a), u.device, keep)
+    nbytes = _size(_capi.selective_scan_fwd_workspace_bytes, a, *sizes, handover is not None)
+    if nbytes:
+        a.workspace, a.workspace_bytes = _workspace(nbytes, dev, keep)
     _capi.selective_scan_fwd(a)
     return y, new
 
@@ -397,16 +406,12 @@ def selective_scan_backward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, 
     """Gradients of ``selective_scan_forward``. ``dstate`` is the gradient of the returned state (None: 0); with
     ``need_dstate`` that of ``state`` comes back. Sums over channels and tokens are float32 in a fixed order: two runs give
     the same bits."""
-    _require_cuda(u, dt, B, C, dout)
     G = _scan_inputs(u, dt, A, B, C, z)
     _check_seq(dout, "dout", u)
     u, dt, B, C, dout = (_inner_contig(t) for t in (u, dt, B, C, dout))
     z = None if z is None else _inner_contig(z)
     keep: list = []
-    dev = u.device
-    a = _capi.SelectiveBwdArgs()
-    _scan_desc(a.desc, u, A, D, dt_bias, dt_softplus, mask, G, keep)
-    N = A.shape[1]
+    dev, N, (Bn, L, Dn) = u.device, A.shape[1], u.shape
 
     def like(t):
         return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
@@ -414,26 +419,22 @@ def selective_scan_backward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, 
     def f32(*shape):
         return torch.empty(shape, dtype=torch.float32, device=dev)
 
-    Dn = u.shape[2]
     g = SelectiveGrads(like(u), like(dt), f32(Dn, N), like(B), like(C), None if D is None else f32(Dn), like(z),
-                       None if dt_bias is None else f32(Dn), f32(u.shape[0], Dn, N) if need_dstate else None)
-    a.u, a.dt, a.z, a.B, a.C, a.dout = _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(dout)
-    a.du, a.ddt, a.dz, a.dB, a.dC = _t3(g.du), _t3(g.ddt), _t3(g.dz), _t3(g.dB), _t3(g.dC)
-    a.dA = g.dA.data_ptr()
-    for name, t in (("dD", g.dD), ("ddt_bias", g.ddt_bias), ("dstate_in", g.dstate)):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-    a.state_in = _state(state, "state", u, N, keep)
-    a.dstate_out = _state(dstate, "dstate", u, N, keep)
-    if handover is not None and handover.buf is not None and handover.buf.numel():
+                       None if dt_bias is None else f32(Dn), f32(Bn, Dn, N) if need_dstate else None)
+    at = [None if t is None else t.data_ptr() for t in (g.dstate, g.dA, g.dD, g.ddt_bias)]
+    a = _capi.SelectiveBwdArgs(_scan_desc(u, A, D, dt_bias, dt_softplus, mask, G, keep), _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(dout), _t3(g.du),
+                               _t3(g.ddt), _t3(g.dz), _t3(g.dB), _t3(g.dC), _state(state, "state", u, N, keep), _state(dstate, "dstate", u, N, keep), *at,
+                               None, None, 0, _stream(dev))
+    sizes = (Bn, L, Dn, N, G)
+    handed = handover is not None and handover.buf is not None and handover.buf.numel() > 0
+    if handed:
         if handover.key != (tuple(u.shape), N, G, u.dtype, dev):
             raise ValueError("handover comes from a forward of another shape, type or device")
         if (handover.buf.dtype != torch.uint8 or not handover.buf.is_contiguous()
-                or handover.buf.numel() < _capi.selective_scan_handover_bytes(a.desc)):
+                or handover.buf.numel() < _size(_capi.selective_scan_handover_bytes, a.desc, *sizes)):
             raise ValueError("handover is not a buffer that the forward of this call filled")
         a.handover = handover.buf.data_ptr()
-    a.stream = _stream(dev)
-    a.workspace, a.workspace_bytes = _workspace(_capi.selective_scan_bwd_workspace_bytes(a), dev, keep)
+    a.workspace, a.workspace_bytes = _workspace(_size(_capi.selective_scan_bwd_workspace_bytes, a, *sizes, handed), dev, keep)
     _capi.selective_scan_bwd(a)
     return g
 
@@ -462,7 +463,7 @@ class SelectiveScanStep(_Step):
         keep: list = [u, dt, A, B, C, out, state, D, z, dt_bias, mask]
         with torch.cuda.device(u.device):
             a = _capi.SelectiveFwdArgs()
-            _scan_desc(a.desc, u, A, D, dt_bias, dt_softplus, mask, G, keep)
+            a.desc = _scan_desc(u, A, D, dt_bias, dt_softplus, mask, G, keep)
             a.u, a.dt, a.z, a.B, a.C, a.out = _t3(u), _t3(dt), _t3(z), _t3(B), _t3(C), _t3(out)
             a.state_in = a.state_out = _own_buffer(state, "state", (u.shape[0], u.shape[2], N), u.device)
             a.workspace, a.workspace_bytes = _workspace(_capi.selective_scan_fwd_workspace_bytes(a), u.device, keep)
@@ -561,7 +562,6 @@ def rms_norm_backward(dy: torch.Tensor, r: torch.Tensor, weight: Optional[torch.
     ``dresidual`` is the gradient that reaches r from elsewhere (the residual stream), of r's type; dx has dy's type (x's; of
     a float32 x normalised into 16 bits give dy in float32), dres has r's, and they are one tensor where the types are one.
     dweight is float32 [D], bitwise reproducible."""
-    _require_cuda(dy, r)
     keep: list = []
     if dy.shape != r.shape or dy.device != r.device:
         raise ValueError("rms_norm_backward needs dy and r of one shape on one device")
@@ -579,7 +579,7 @@ def rms_norm_backward(dy: torch.Tensor, r: torch.Tensor, weight: Optional[torch.
         _param(weight, "weight", (D,), r.device, keep), gp, gs, np_, ns, None if dx is dres else dx.data_ptr(), D, dres.data_ptr(), D,
         None if dw is None else dw.data_ptr(), None, 0, _stream(r.device))
     if dw is not None:
-        a.workspace, a.workspace_bytes = _workspace(_capi.rms_norm_bwd_workspace_bytes(a), r.device, keep)
+        a.workspace, a.workspace_bytes = _workspace(_size(_capi.rms_norm_bwd_workspace_bytes, a, D, a.rows > 0), r.device, keep)
     _capi.rms_norm_bwd(a)
     return dx, dres, dw
 
