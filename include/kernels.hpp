@@ -338,7 +338,7 @@ size_t subq_layer_norm_bwd_workspace_bytes(const subq_layer_norm_args* args);
  * u, dt (raw), z and out are [B, L, D] views, B and C [B, L, G, N] views that the
  * D / G channels of a group share, all of one type (fp32, fp16, bf16) with
  * element strides and a contiguous innermost dimension. A masked token leaves h as
- * it is, its out and gradients are 0, and nothing of it is read. N <= 128.
+ * it is, its out and gradients are 0, and nothing of it is used. N <= 128.
  *
  * The forward can leave the states before every eighth token (handover) for the
  * backward of the same call, which forms them again without: 4 bytes x the states
@@ -399,7 +399,7 @@ size_t subq_selective_scan_handover_bytes(const subq_selective_desc* desc);
 /* Short causal convolution over [B, L, D], one filter of width 2, 3 or 4 a channel:
  *   pre_t = bias + sum_j weight[d, j] x_{t-width+1+j},   y_t = silu(pre_t) or pre_t.
  * Before the first token stand the width - 1 inputs of state_in (zeros without);
- * a masked token's input counts as 0, its y and dx are 0 and nothing of it is read;
+ * a masked token's input counts as 0, its y and dx are 0 and nothing of it is used;
  * state_out receives the width - 1 inputs up to the last live token (those of
  * state_in among them where there are fewer; state_in itself without a live
  * token). Sums in float32; weights and their gradients float32, written (not

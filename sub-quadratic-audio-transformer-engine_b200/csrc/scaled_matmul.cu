@@ -212,10 +212,10 @@ __global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_
     tc::tc_fence_after();
     const uint32_t tmem = tmem_slot;
     bool ok = true;
-    // The epilogue's sums and the 64 values that are on their way to them take 200 registers: 256 x 200 + 128 x 104 = 384 x 168.
+    // The epilogue's sums and the 64 values that are on their way to them take about 200 registers: 256 x 216 + 128 x 72 = 384 x 168.
     // (k-blocks are counted through all of the CTA's tiles: block i uses stage i % 4 and accumulator i % 2)
     if (warp >= 8) {
-    tc::regs_down<104>();
+    tc::regs_down<72>();
     if (warp == 8) {
         if (lane == 0) {
             int64_t it = 0;
@@ -258,23 +258,33 @@ __global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_
         __syncwarp();
     }
     } else {
-        tc::regs_up<200>();
+        tc::regs_up<216>();
         const int quad = warp & 3, half = warp >> 2;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         unsigned char* stage = smem + S::kStages * S::kStageBytes + warp * 32 * S::kRow;
         T* out = static_cast<T*>(p.out);
         const bool aligned = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_s * (int64_t)sizeof(T) % 16 == 0;
         int64_t it = 0;
+        // scales of a tile's first two k-blocks, asked for before the tile before it is written
+        float sa = 0.f, sb = 0.f, sa1 = 0.f, sb1 = 0.f;
+        auto begin = [&](int64_t tile, const float*& as, const float*& bs) {
+            const int64_t m = tile / ntiles * kBM + quad * 32 + lane;
+            const int n0 = (int)(tile % ntiles) * S::kBN + half * 128;
+            const bool in = m < p.M && n0 < p.N;
+            as = p.a_scale + (in ? m : 0) * p.as_s;
+            bs = p.b_scale + (in ? n0 / 128 : 0) * p.bs_s;
+            sa = as[0], sb = bs[0];
+            if (p.nk > 1) sa1 = as[1], sb1 = bs[1];
+        };
+        const float *as = nullptr, *bs = nullptr;
+        begin(blockIdx.x, as, bs);
         for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
             const int64_t mw = tile / ntiles * kBM + quad * 32, m = mw + lane;
             const int n0 = (int)(tile % ntiles) * S::kBN + half * 128;
             const bool in = m < p.M && n0 < p.N;
-            const float* as = p.a_scale + (in ? m : 0) * p.as_s;
-            const float* bs = p.b_scale + (in ? n0 / 128 : 0) * p.bs_s;
             F2 acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = f2(0.f);
-            float sa = as[0], sb = bs[0], sa1 = p.nk > 1 ? as[1] : 0.f, sb1 = p.nk > 1 ? bs[1] : 0.f;  // two k-blocks ahead
             for (int kb = 0; kb < p.nk; ++kb, ++it) {
                 const int buf = (int)(it & 1);
                 const F2 scale = f2(in ? sa * sb : 0.f);
@@ -307,6 +317,7 @@ __global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_
                 }
             }
             if (!ok) break;
+            if (tile + gridDim.x < tiles) begin(tile + gridDim.x, as, bs);
             // 64 bytes of each of the warp's 32 rows at a time, through shared memory to whole sectors of the rows
             constexpr int kC = 64 / (int)sizeof(T), kV = 16 / (int)sizeof(T);
 #pragma unroll

@@ -162,7 +162,7 @@ def causal_conv_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     y_t = act(bias + sum_j weight[:, j] x_{t-W+1+j}), act silu or (``activation=None``) nothing. Returns ``(y, state | None)``.
 
     ``state`` [B, W - 1, D] (x's type) holds the inputs before the first token (None: zeros). A masked token's input counts
-    as 0 and its output is 0; nothing of it is read. The returned state is of the W - 1 inputs up to the last live token,
+    as 0 and its output is 0; nothing of it is used. The returned state is of the W - 1 inputs up to the last live token,
     so that a padded batch of prompts goes on with its next tokens. Math in float32."""
     x = _inner_contig(x)
     keep: list = []
@@ -368,7 +368,7 @@ def selective_scan_forward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     ``u``, ``dt``, ``z`` [B, L, D] and ``B``, ``C`` [B, L, N] or [B, L, G, N] (the D / G channels of a group share them)
     have one type (float32, float16 or bfloat16); ``A`` [D, N], ``D`` [D] and ``dt_bias`` [D] are used in float32.
     ``z`` None: no gate; ``dt_softplus=False``: dt + dt_bias itself. ``mask`` [B, L]: a masked token leaves the state as it
-    is, its output is 0 and nothing of it is read. N <= 128. Math in float32, a decay near 1 applied as h + (a - 1) h."""
+    is, its output is 0 and nothing of it is used. N <= 128. Math in float32, a decay near 1 applied as h + (a - 1) h."""
     G = _scan_inputs(u, dt, A, B, C, z)
     u, dt, B, C = (_inner_contig(t) for t in (u, dt, B, C))
     z = None if z is None else _inner_contig(z)

@@ -179,6 +179,8 @@ class SubQFp8Linear(nn.Module):
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, out_dtype: torch.dtype = torch.bfloat16, device=None):
         super().__init__()
+        if not 1 <= in_features <= 16384 or out_features < 1:
+            raise ValueError(f"the 8-bit layer takes 1 to 16384 columns and at least a row, got {in_features} and {out_features}")
         self.in_features, self.out_features, self.out_dtype = in_features, out_features, out_dtype
         n, k = (out_features + 127) // 128, (in_features + 127) // 128
         self.register_buffer("weight_bytes", torch.zeros(out_features, (in_features + 15) // 16 * 16, dtype=torch.uint8, device=device))

@@ -267,3 +267,44 @@ def test_second_gradients_and_bad_states_raise():
     m = layer()
     with pytest.raises(ValueError, match="window"):
         m(torch.randn(1, 4, 48, device="cuda"), past_state=torch.zeros(1, 96, 16, device="cuda"))
+
+
+def test_a_refused_call_leaves_nothing_behind():
+    """Sizes that the library gave are kept by the calls' sizes; a refused call's answer (none) is not."""
+    x = torch.randn(3, 77, 40, device="cuda")
+    w = torch.randn(40, 4, device="cuda")
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            ops.causal_conv_backward(x, w, x[:, :76])
+        with pytest.raises(ValueError):
+            ops.selective_scan_backward(x, x, -torch.rand(40, 6, device="cuda"), x[..., :6], x[..., :6], x, z=x[:2])
+        with pytest.raises(ValueError):
+            ops.rms_norm_backward(x, x, w[:39, 0])
+    assert ops.causal_conv_backward(x, w, x)[0].shape == x.shape
+    assert ops.selective_scan_backward(x, x, -torch.rand(40, 6, device="cuda"), x[..., :6], x[..., :6], x).du.shape == x.shape
+
+
+def test_inputs_on_a_side_stream_and_many_calls_at_once():
+    """Calls of every operator on two streams at once, with their own workspaces."""
+    torch.manual_seed(3)
+    x = torch.randn(2, 600, 64, device="cuda", dtype=torch.bfloat16)
+    A, B, w = -torch.rand(64, 16, device="cuda"), torch.randn(2, 600, 16, device="cuda", dtype=torch.bfloat16), torch.randn(64, 4, device="cuda")
+    q = ops.quantize_fp8(x)
+    qw = ops.quantize_fp8_weight(torch.randn(96, 64, device="cuda"))
+
+    def everything():
+        g = ops.selective_scan_backward(x, x, A, B, B, x)
+        return (*(t for t in g if t is not None), *(t for t in ops.causal_conv_backward(x, w, x) if t is not None), *ops.rms_norm_backward(x, x),
+                ops.scaled_matmul(*q, *qw))
+
+    want = everything()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(5):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(everything())
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))

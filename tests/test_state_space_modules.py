@@ -18,6 +18,12 @@ def test_norm_widths():
             SubQRMSNorm(n)
 
 
+def test_quantised_widths():
+    for n, m in ((0, 4), (16385, 4), (4, 0)):
+        with pytest.raises(ValueError):
+            SubQFp8Linear(n, m)
+
+
 def test_quantised_weights_stay_bytes():
     m = SubQStateSpaceBlock(64).quantize()
     lin = m.mixer.in_proj
