@@ -10,7 +10,7 @@
 // Large products: 128 x 256 tiles by one CTA an SM that goes on from tile to tile (k-blocks of the next one are loaded and
 // multiplied while this one is written), eight epilogue warps with 128 columns each. A k-block's products take 512 cycles,
 // its way through the epilogue (TMEM read and multiply-add, two warps to a scheduler) about as long, its 48 KB from L2 about
-// 800: 16384 x 4096 x 1024 takes 107 us (1.28 PFLOP/s), 2048 x 4096 x 4096 51 us (1.35).
+// 800: 16384 x 4096 x 1024 takes 104 to 107 us (1.3 PFLOP/s), 2048 x 4096 x 4096 51 us (1.35).
 // Smaller ones: 128 x BN tiles, a CTA each, two to an SM.
 // A few rows (streaming steps) are bound by the weights' bytes, or by the launch: there a warp has a column of b, its lanes
 // 16 values each at a time, and every row of a.
@@ -212,10 +212,10 @@ __global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_
     tc::tc_fence_after();
     const uint32_t tmem = tmem_slot;
     bool ok = true;
-    // The epilogue's sums and the 64 values that are on their way to them take about 200 registers: 256 x 216 + 128 x 72 = 384 x 168.
+    // The epilogue's sums and the 64 values that are on their way to them take 200 registers: 256 x 200 + 128 x 104 = 384 x 168 (208 and 88, 216 and 72: 121 us for 107).
     // (k-blocks are counted through all of the CTA's tiles: block i uses stage i % 4 and accumulator i % 2)
     if (warp >= 8) {
-    tc::regs_down<72>();
+    tc::regs_down<104>();
     if (warp == 8) {
         if (lane == 0) {
             int64_t it = 0;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(384, 1) scaled_matmul_big_kernel(const __grid_
         __syncwarp();
     }
     } else {
-        tc::regs_up<216>();
+        tc::regs_up<200>();
         const int quad = warp & 3, half = warp >> 2;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         unsigned char* stage = smem + S::kStages * S::kStageBytes + warp * 32 * S::kRow;
