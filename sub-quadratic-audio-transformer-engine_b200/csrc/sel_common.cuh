@@ -82,12 +82,23 @@ __device__ __forceinline__ F2 decayed(const Factor& f, F2 h) {
     get(h, h0, h1);
     return fma(f.c, h, f2(f.n0 ? h0 : 0.f, f.n1 ? h1 : 0.f));
 }
+// Factors over many tokens where states grow (A above 0): 2^y beyond 2^127 goes in two steps, so that what is 0 stays 0.
+__device__ __forceinline__ float split_growth(float& y, float h) {
+    if (y > 127.f) {
+        h *= ex2(fminf(y, 254.f) - 127.f);
+        y = 127.f;
+    }
+    return h;
+}
 __device__ __forceinline__ float decayed(float y, float h) {
     float p = fmaf(y, 0.0013347864f, 0.00963017f);
     p = fmaf(p, y, 0.055504076f);
     p = fmaf(p, y, 0.24022631f);
     p = fmaf(p, y, 0.6931472f) * y;
-    return fabsf(y) < kNear ? fmaf(p, h, h) : ex2(y) * h;
+    p = fmaf(p, h, h);
+    const bool near = fabsf(y) < kNear;
+    h = split_growth(y, h);
+    return near ? p : ex2(y) * h;
 }
 
 __device__ __forceinline__ float rcp(float x) {

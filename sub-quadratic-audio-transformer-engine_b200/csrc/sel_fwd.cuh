@@ -3,8 +3,8 @@
 // per token and channel and left in shared memory, the states stay in registers, and y goes back through shared memory to
 // the threads that hold u and z for the output. The next tile is on its way meanwhile.
 //
-// Bound by instruction issue and the FMA pipe (a state and token take one exponential, ten multiply-adds, half of them two at
-// a time, and three selections), not by memory: 65536 x 1536 channels of 16 states take 988 us and 518 us for the segments,
+// Bound by instruction issue and the FMA pipe (a state and token take one exponential, nine multiply-adds, two states at a
+// time, and three selections), not by memory: 65536 x 1536 channels of 16 states take 988 us and 518 us for the segments,
 // 124 us would be its bytes, 360 us its exponentials alone. Few channels: the sequence is cut into segments; a first launch finds what each leaves of a zero
 // state and the sum of its step sizes (a segment's decay is exp(A sum dt)), and the walk's CTAs chain those before theirs.
 #pragma once
@@ -272,8 +272,18 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 3 : 2) sel_seg_kernel(
         }
         // behind the tiles that have been summed (weighted as far as these reach)
         const float far = sum + rest;
-        h01 = fma(f2(ex2(A2[0] * far), ex2(A2[1] * far)), t01, h01);
-        h23 = fma(f2(ex2(A2[2] * far), ex2(A2[3] * far)), t23, h23);
+        float y[4] = {A2[0] * far, A2[1] * far, A2[2] * far, A2[3] * far};
+        if (fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > 127.f) {
+            float t[4];
+            get(t01, t[0], t[1]);
+            get(t23, t[2], t[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = split_growth(y[j], t[j]);
+            t01 = f2(t[0], t[1]);
+            t23 = f2(t[2], t[3]);
+        }
+        h01 = fma(f2(ex2(y[0]), ex2(y[1])), t01, h01);
+        h23 = fma(f2(ex2(y[2]), ex2(y[3])), t23, h23);
         add_exactly(sum, rest, cum);
         __syncthreads();
     }

@@ -167,6 +167,29 @@ def test_slow_decay_keeps_its_bits():
     assert rel(h, want_h) < FWD and rel(out, want) < FWD
 
 
+def test_growing_states_behind_zeros():
+    """A above 0: factors over a segment overflow, the states of the last tokens do not.
+
+    A growing state forgets none of its roundings, so those of up to 40 steps add up: a factor 2^y is off by 1e-7 (the exponential) and by two
+    halves of a step of y (the product dt A log2 e, y < 0.6, times ln 2), the step itself by two half steps (the factor applied,
+    the input added). 40 (1e-7 + 2 x 0.42 x 2^-24 + 2 x 2^-24) = 1.1e-5 beside what a state that decays may be off.
+    """
+    grown = 40 * (1e-7 + 2 * 0.42 * 2.0 ** -24 + 2 * 2.0 ** -24)
+    s, dout, _ = inputs(1, 4096, 64, 16, 1, "fp32", state=False, gate=False)
+    s["A"] = s["A"].abs() * 0.05
+    s["dt"].fill_(0.3)
+    s["dt_bias"] = None
+    s["u"][:, :4060] = 0
+    s["D"] = None
+    out, h = call(s, dt_softplus=False, return_state=True)
+    assert ops.last_launches() == 2
+    want, want_h = definition(s, softplus=False)
+    assert bool(torch.isfinite(want_h).all()) and rel(out, want) < FWD + grown and rel(h, want_h) < FWD + grown
+    dout[:, 40:] = 0
+    g, grads = call_back(s, dout, dt_softplus=False), definition(s, softplus=False, dout=dout)
+    assert rel(g.dC, grads["C"]) < BWD + grown and bool(torch.isfinite(g.du).all()) and rel(g.du, grads["u"]) < BWD + grown
+
+
 def test_extreme_steps():
     """Steps that forget everything (exp underflows), that change nothing, and softplus of far arguments."""
     s, dout, _ = inputs(2, 64, 64, 16, 1, "fp32")
