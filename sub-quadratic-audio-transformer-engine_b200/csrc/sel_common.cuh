@@ -106,9 +106,15 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// -|x|, -128 beyond it, where exp is 0 in float32 (products of an infinite or the lowest x would be inf - inf); a NaN stays one.
+__device__ __forceinline__ float far_neg(float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(-fabsf(x)), "f"(-128.f));
+    return r;
+}
 // exp(-|x|): the product with log2 e is carried to 48 bits, so that a far x costs no accuracy (3e-7 off at most).
 __device__ __forceinline__ float exp_neg(float x) {
-    const float a = -fabsf(x), t = a * 1.4426950408889634f;
+    const float a = far_neg(x), t = a * 1.4426950408889634f;
     const float rest = fmaf(a, 1.4426950408889634f, -t);
     const float e = ex2(t);
     return fmaf(e * 0.6931472f, fmaf(a, 1.925963033e-8f, rest), e);
@@ -133,7 +139,7 @@ __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(x * -1.
 __device__ __forceinline__ F2 exp_neg(F2 x) {
     float a, b;
     get(x, a, b);
-    const F2 m = f2(-fabsf(a), -fabsf(b)), t = mul(m, f2(1.4426950408889634f));
+    const F2 m = f2(far_neg(a), far_neg(b)), t = mul(m, f2(1.4426950408889634f));
     F2 rest = fma(m, f2(1.4426950408889634f), mul(t, f2(-1.f)));
     rest = fma(m, f2(1.925963033e-8f), rest);
     get(t, a, b);
