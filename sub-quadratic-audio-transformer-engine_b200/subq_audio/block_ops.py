@@ -79,9 +79,10 @@ def _mask(mask: Optional[torch.Tensor], B: int, L: int, device: torch.device, ke
         raise ValueError(f"mask must be [B, L] = [{B}, {L}], got {tuple(m.shape)}")
     if m.device != device:
         raise ValueError("mask must be on the device of the inputs")
-    if m.dtype == torch.bool and m.stride(1) == 1:
+    rows = L <= 1 or m.stride(1) == 1  # (one token a row: its place in the row does not matter)
+    if m.dtype == torch.bool and rows:
         m = m.view(torch.uint8)
-    elif m.dtype != torch.uint8 or m.stride(1) != 1:
+    elif m.dtype != torch.uint8 or not rows:
         m = (m != 0).to(torch.uint8).contiguous()
     keep.append(m)
     return m.data_ptr(), m.stride(0)
