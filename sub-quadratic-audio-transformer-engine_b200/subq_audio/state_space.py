@@ -174,8 +174,8 @@ class SubQRMSNorm(nn.Module):
 class SubQFp8Linear(nn.Module):
     """A linear layer's weight in 8 bits with a float32 scale for every 128 x 128 of it, for inference. Takes a tensor (made 8 bits
     wide with a scale for every 128 of a row) or such a pair ``(q, scale)`` as it is. ``out_dtype`` is the result's type for
-    pairs; a tensor's result has its type. The 8-bit weight and its scales are kept as bytes, so that casting the module
-    leaves them alone."""
+    pairs, a tensor's result has its type, and a call's own ``out_dtype`` comes before both. The 8-bit weight and its scales are
+    kept as bytes, so that casting the module leaves them alone."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, out_dtype: torch.dtype = torch.bfloat16, device=None):
         super().__init__()
@@ -203,14 +203,14 @@ class SubQFp8Linear(nn.Module):
             new.bias.copy_(linear.bias)
         return new
 
-    def forward(self, x: Union[torch.Tensor, Pair]) -> torch.Tensor:
+    def forward(self, x: Union[torch.Tensor, Pair], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         if isinstance(x, tuple):
-            (q, scale), out = x, self.out_dtype
+            (q, scale), out = x, out_dtype or self.out_dtype
         else:
             if _wants_grad(x):
                 raise RuntimeError("SubQFp8Linear is for inference: it has no gradients")
             q, scale = torch.ops.subq_audio.quantize_fp8(x)
-            out = x.dtype
+            out = out_dtype or x.dtype
         w = self.weight_bytes.view(torch.float8_e4m3fn)[:, :self.in_features]
         return torch.ops.subq_audio.scaled_matmul(q, scale, w, self.scale_bytes.view(torch.float32), self.bias, out)
 
@@ -264,7 +264,11 @@ class SubQSelectiveStateSpace(nn.Module):
             S0, window = _split_state(past_state)
             if window is None:
                 raise ValueError("past_state needs the scan's state and the convolution's window (state.Z, or a pair)")
-        xz = self.in_proj(hidden_states)
+        if isinstance(hidden_states, tuple):  # (8 bits say nothing of the branch's type: what the next projection takes)
+            branch = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else self.x_proj.weight.dtype
+            xz = self.in_proj(hidden_states, branch)
+        else:
+            xz = self.in_proj(hidden_states)
         x, z = xz[..., :self.inner], xz[..., self.inner:]
         mask = _mask_of(attention_mask, x)
         x, window = causal_conv(x, self.conv_weight, self.conv_bias, "silu", None if window is None else window.to(x.dtype), mask, use_cache)
