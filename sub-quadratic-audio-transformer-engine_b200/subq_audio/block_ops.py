@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import inspect
 import math
 from typing import NamedTuple, Optional, Tuple
 
@@ -49,16 +50,20 @@ def _size(query, args, *key) -> int:
 
 def _on_its_device(call):
     """The call with the device of its first tensor as the current one."""
+    name = next(iter(inspect.signature(call).parameters))
 
     @functools.wraps(call)
-    def run(first, *args, **kwargs):
+    def run(*args, **kwargs):
+        first = args[0] if args else kwargs.get(name)
         if not (isinstance(first, torch.Tensor) and first.is_cuda):
+            if not args and name not in kwargs:
+                return call(*args, **kwargs)  # (refuses by itself)
             _require_cuda(first)
         index = first.get_device()
         if index == torch.cuda.current_device():
-            return call(first, *args, **kwargs)
+            return call(*args, **kwargs)
         with torch.cuda.device(index):
-            return call(first, *args, **kwargs)
+            return call(*args, **kwargs)
 
     return run
 
