@@ -272,18 +272,42 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 3 : 2) sel_seg_kernel(
         }
         // behind the tiles that have been summed (weighted as far as these reach)
         const float far = sum + rest;
-        float y[4] = {A2[0] * far, A2[1] * far, A2[2] * far, A2[3] * far};
-        if (fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > 127.f) {
-            float t[4];
-            get(t01, t[0], t[1]);
-            get(t23, t[2], t[3]);
+        float s[4];
+        get(t01, s[0], s[1]);
+        get(t23, s[2], s[3]);
+        if (fabsf(s[0]) + fabsf(s[1]) + fabsf(s[2]) + fabsf(s[3]) < INFINITY) {
+            float y[4] = {A2[0] * far, A2[1] * far, A2[2] * far, A2[3] * far};
+            if (fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > 127.f) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) t[j] = split_growth(y[j], t[j]);
-            t01 = f2(t[0], t[1]);
-            t23 = f2(t[2], t[3]);
+                for (int j = 0; j < 4; ++j) s[j] = split_growth(y[j], s[j]);
+                t01 = f2(s[0], s[1]);
+                t23 = f2(s[2], s[3]);
+            }
+            h01 = fma(f2(ex2(y[0]), ex2(y[1])), t01, h01);
+            h23 = fma(f2(ex2(y[2]), ex2(y[3])), t23, h23);
+        } else {  // a state that grows past 2^127 within the tile: each token by itself, its whole factor in two steps
+            float h[4];
+            get(h01, h[0], h[1]);
+            get(h23, h[2], h[3]);
+            cum = 0.f;
+#pragma unroll 1
+            for (int k = 0; k < kSelTile; ++k) {
+                const int t = BACK ? k : kSelTile - 1 - k;
+                const float2 x = sdt[t * kCh + cp];
+                const float4 Bv = *reinterpret_cast<const float4*>(sB + t * kNp + 4 * q);
+                const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
+                if (BACK) cum += x.x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float y = A2[j] * (cum + far);
+                    const float v = split_growth(y, x.y * B4[j]);
+                    h[j] = fmaf(ex2(y), v, h[j]);
+                }
+                if (!BACK) cum += x.x;
+            }
+            h01 = f2(h[0], h[1]);
+            h23 = f2(h[2], h[3]);
         }
-        h01 = fma(f2(ex2(y[0]), ex2(y[1])), t01, h01);
-        h23 = fma(f2(ex2(y[2]), ex2(y[3])), t23, h23);
         add_exactly(sum, rest, cum);
         __syncthreads();
     }

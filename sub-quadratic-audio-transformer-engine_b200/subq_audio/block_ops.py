@@ -375,9 +375,8 @@ def selective_scan_forward(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B
     have one type (float32, float16 or bfloat16); ``A`` [D, N], ``D`` [D] and ``dt_bias`` [D] are used in float32.
     ``z`` None: no gate; ``dt_softplus=False``: dt + dt_bias itself. ``mask`` [B, L]: a masked token leaves the state as it
     is, its output is 0 and nothing of it is used. N <= 128. Math in float32, a decay near 1 applied as h + (a - 1) h. A raw
-    step of -inf (or the type's lowest value) under softplus is a step of 0; one of +inf, as any state that leaves float32's
-    range, leaves infinities or NaN behind, in its channel and from its token on.
-    ``A`` is negative as a rule; where it is not and a state grows more than 2^127 times over 32 tokens, its values may be NaN."""
+    step of -inf (or the type's lowest value) under softplus is a step of 0; one of +inf, as a state or one token's factor exp(dt A) that
+    leaves float32's range, leaves infinities or NaN behind, in its channel and from its token on."""
     G = _scan_inputs(u, dt, A, B, C, z)
     u, dt, B, C = (_inner_contig(t) for t in (u, dt, B, C))
     z = None if z is None else _inner_contig(z)
