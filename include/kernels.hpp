@@ -343,7 +343,13 @@ size_t subq_layer_norm_bwd_workspace_bytes(const subq_layer_norm_args* args);
  * The forward can leave the states before every eighth token (handover) for the
  * backward of the same call, which forms them again without: 4 bytes x the states
  * rounded up to 16, 32, 64 or 128, for each channel and 8 tokens (8 bytes a token
- * and channel at N <= 16). */
+ * and channel at N <= 16).
+ *
+ * The backward's workspace holds as much again without a handover, and the parts
+ * of dB and dC: 8 n^2 / 1024 bytes a token and channel with n the states rounded up
+ * as above (2 bytes at N <= 16, 8, 32, 128), but no more than 1 GiB or a float32
+ * [B, L, D], whichever is more (or 32 tokens of each segment, where that is more):
+ * beyond that the walk back goes in ranges of tokens, two launches each. */
 typedef struct subq_tensor3 {
     void* data;
     int64_t stride_b, stride_l, stride_g; /* element strides; stride_g: B, C and their gradients only */

@@ -44,7 +44,12 @@ struct SelParams {
     float* dA;            // [D, N]
     float* dD;            // [D] or null
     float* dbias;         // [D] or null
-    float* part_bc;       // [channel blocks of a group][B][L][G][2][4 lanes]
+    // The walk back goes through every segment's tokens in ranges, from the last to the first, so that the parts of dB and dC
+    // are of one range at a time.
+    int range_tokens, range0;  // tokens of a range, a multiple of kSelTile; the begin of this launch's within a segment
+    int rows;                  // tokens that part_bc has: L, or nseg * range_tokens
+    float* carry;              // [nseg][B][D][4 lanes]: the adjoint between two ranges (null: one range)
+    float* part_bc;            // [channel blocks of a group][B][rows][G][2][4 lanes]
     float* part_a;        // [B * nseg][D][4 lanes]
     float* part_d;        // [B * nseg][2][D]: dD, dbias
 };
@@ -60,9 +65,10 @@ inline int sel_channels(int N) { return kSelThreads / sel_lanes(N); }  // channe
 enum SelPass { kSelSegments = 0, kSelWalk = 1 };
 // One launch: the segments' states (kSelSegments: seg_h, seg_dt of all but the last) or the walk itself (out, kept, S_out).
 cudaError_t launch_sel_fwd(const SelParams& p, int dtype, SelPass pass, cudaStream_t st);
-// One launch: the segments' adjoints (of all but the first) or the walk back with every gradient's part; then the sums.
+// One launch: the segments' adjoints (of all but the first) or the walk back over a range with every gradient's part; then the
+// sums of dB and dC of that range, and (`weights`, behind the last) of dA, dD and dbias.
 cudaError_t launch_sel_bwd(const SelParams& p, int dtype, SelPass pass, cudaStream_t st);
-cudaError_t launch_sel_sums(const SelParams& p, int dtype, cudaStream_t st);
+cudaError_t launch_sel_sums(const SelParams& p, int dtype, bool weights, cudaStream_t st);
 // Token by token without shared memory: single tokens and short calls.
 cudaError_t launch_sel_step(const SelParams& p, int dtype, cudaStream_t st);
 

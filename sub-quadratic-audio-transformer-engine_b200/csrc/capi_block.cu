@@ -26,8 +26,13 @@ SUBQ_TYPED(launch_sel_bwd)
         return dtype == SUBQ_BF16 ? name##_bf16(p, st) : dtype == SUBQ_FP16 ? name##_fp16(p, st) : name##_fp32(p, st); \
     }
 SUBQ_TYPED(launch_sel_step)
-SUBQ_TYPED(launch_sel_sums)
 #undef SUBQ_TYPED
+cudaError_t launch_sel_sums_bf16(const SelParams& p, bool weights, cudaStream_t st);
+cudaError_t launch_sel_sums_fp16(const SelParams& p, bool weights, cudaStream_t st);
+cudaError_t launch_sel_sums_fp32(const SelParams& p, bool weights, cudaStream_t st);
+cudaError_t launch_sel_sums(const SelParams& p, int dtype, bool weights, cudaStream_t st) {
+    return dtype == SUBQ_BF16 ? launch_sel_sums_bf16(p, weights, st) : dtype == SUBQ_FP16 ? launch_sel_sums_fp16(p, weights, st) : launch_sel_sums_fp32(p, weights, st);
+}
 
 }  // namespace subq
 
@@ -126,15 +131,34 @@ SegBytes seg_bytes(const SelParams& p) {
     const size_t n = (size_t)p.nseg * p.B * p.D;
     return {align_up(n * np_of(p) * 4), align_up(n * 4), p.S_in && p.S_in == p.S_out ? align_up((size_t)p.B * p.D * p.N * 4) : 0};
 }
+// The walk back leaves each CTA's part of dB and dC, 8 (4 lanes)^2 / 1024 bytes a token and channel: at N <= 16 half of a float32
+// [B, L, D], at N > 64 32 times it. Beyond 1 GiB and one such tensor the walk goes in ranges of tokens
+// (bf16 training steps, N = 128, all tokens at once and as cut: 1 x 16384 x 1536 18.4, 18.3 ms; 16 x 1024 x 1536 15.9, 15.0; 8 x 2048 x 2048
+// 21.0, 21.1).
+size_t bc_row_bytes(const SelParams& p) {  // of one token of all sequences
+    const size_t ch = sel_channels(p.N), blocks = (p.Dg + ch - 1) / ch;
+    return blocks * p.B * p.G * 2 * np_of(p) * 4;
+}
+int sel_ranges(const SelParams& p) { return (p.seg_tokens + p.range_tokens - 1) / p.range_tokens; }
+void sel_cut_ranges(SelParams& p) {
+    p.range_tokens = p.seg_tokens;
+    p.rows = p.L;
+    const size_t most = std::max((size_t)1 << 30, (size_t)p.B * p.L * p.D * 4), tile = bc_row_bytes(p) * p.nseg * kSelTile;
+    if (tile == 0 || (size_t)p.L <= most / bc_row_bytes(p)) return;
+    const int64_t tiles = p.seg_tokens / kSelTile, held = std::max<int64_t>(1, (int64_t)(most / tile)), ranges = (tiles + held - 1) / held;
+    if (ranges <= 1) return;
+    p.range_tokens = (int)((tiles + ranges - 1) / ranges * kSelTile);
+    p.rows = p.nseg * p.range_tokens;
+}
 struct SelBwdBytes {
     SegBytes fwd, rev;
-    size_t kept, bc, a, d;
-    size_t all() const { return std::max(fwd.all(), rev.all()) + kept + bc + a + d; }
+    size_t kept, bc, a, d, carry;
+    size_t all() const { return std::max(fwd.all(), rev.all()) + kept + bc + a + d + carry; }
 };
 SelBwdBytes sel_bwd_bytes(const SelParams& fwd, const SelParams& rev, bool handover) {
-    const size_t ch = sel_channels(rev.N), blocks = (rev.Dg + ch - 1) / ch, parts = (size_t)rev.B * rev.nseg;
-    return {handover ? SegBytes{0, 0, 0} : seg_bytes(fwd), seg_bytes(rev), handover ? 0 : kept_bytes(rev),
-            align_up(blocks * rev.B * rev.L * rev.G * 2 * np_of(rev) * 4), align_up(parts * rev.D * np_of(rev) * 4), align_up(parts * 2 * rev.D * 4)};
+    const size_t parts = (size_t)rev.B * rev.nseg, states = align_up(parts * rev.D * np_of(rev) * 4);
+    return {handover ? SegBytes{0, 0, 0} : seg_bytes(fwd), seg_bytes(rev), handover ? 0 : kept_bytes(rev), align_up(bc_row_bytes(rev) * rev.rows), states,
+            align_up(parts * 2 * rev.D * 4), sel_ranges(rev) > 1 ? states : 0};
 }
 
 int fill_sel_fwd(const subq_selective_fwd_args* a, SelParams& p, bool& step) {
@@ -218,6 +242,7 @@ int fill_sel_bwd(const subq_selective_bwd_args* a, SelParams& fwd, SelParams& re
     sel_split(fwd, false);
     // (one CTA reads the gradient that another one's result would overwrite)
     if (!(p.dS_in && p.dS_in == p.dS_out)) sel_split(rev, true);
+    sel_cut_ranges(rev);
     const int64_t state = (int64_t)p.B * p.D * p.N * 4, one = (int64_t)p.D * 4;
     return check_apart({of_rows("du", p.du, p.B, p.L, 1, p.D, t), of_rows("ddt", p.ddt, p.B, p.L, 1, p.D, t), of_rows("dz", p.dz, p.B, p.L, 1, p.D, t),
                         of_rows("dB", dB, p.B, p.L, p.G, p.N, t), of_rows("dC", dC, p.B, p.L, p.G, p.N, t), of_bytes("dstate_in", p.dS_in, state),
@@ -413,7 +438,8 @@ int subq_selective_scan_bwd(const subq_selective_bwd_args* a) {
     p.part_bc = reinterpret_cast<float*>(ws);
     p.part_a = reinterpret_cast<float*>(ws + n.bc);
     p.part_d = reinterpret_cast<float*>(ws + n.bc + n.a);
-    unsigned char* segs = ws + n.bc + n.a + n.d + n.kept;
+    if (n.carry) p.carry = reinterpret_cast<float*>(ws + n.bc + n.a + n.d + n.kept);
+    unsigned char* segs = ws + n.bc + n.a + n.d + n.kept + n.carry;
     if (!a->handover) {
         fwd.kept = p.kept = reinterpret_cast<float*>(ws + n.bc + n.a + n.d);
         fwd.out = SelTensor{};  // the states alone
@@ -424,10 +450,14 @@ int subq_selective_scan_bwd(const subq_selective_bwd_args* a) {
         err = launch_sel_bwd(p, dt, kSelSegments, st);
         ++launches;
     }
-    if (err == cudaSuccess) err = launch_sel_bwd(p, dt, kSelWalk, st);
-    if (err == cudaSuccess) err = launch_sel_sums(p, dt, st);
+    const int ranges = sel_ranges(p);
+    for (int r = ranges - 1; r >= 0 && err == cudaSuccess; --r) {
+        p.range0 = r * p.range_tokens;
+        err = launch_sel_bwd(p, dt, kSelWalk, st);
+        if (err == cudaSuccess) err = launch_sel_sums(p, dt, r == 0, st);
+    }
     if (err != cudaSuccess) return fail_cuda(err, "subq_selective_scan_bwd launch");
-    set_launches(launches + 3);
+    set_launches(launches + 2 * ranges + 1);
     return SUBQ_OK;
 }
 

@@ -108,7 +108,8 @@ struct BwdSmem {
     alignas(16) T raw[4][kSelTile * kCh];  // a thread's own pieces of u, dt, z, dout of the next tile
 };
 
-template <typename T, int LPC>
+// RANGES: this launch has one range of every segment's tokens (an instance of its own: 1 to 5 % of the walk).
+template <typename T, int LPC, bool RANGES>
 __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(const SelParams p) {
     using P = Place<T, LPC>;
     using S = BwdSmem<T, LPC>;
@@ -116,7 +117,10 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     extern __shared__ __align__(16) unsigned char smem[];
     S& s = *reinterpret_cast<S*>(smem);
     const P at(p);
-    const int seg = blockIdx.y, first = seg * p.seg_tokens, last = min(p.L, first + p.seg_tokens);
+    const int seg = blockIdx.y, seg_first = seg * p.seg_tokens, seg_last = min(p.L, seg_first + p.seg_tokens);
+    const int first = RANGES ? seg_first + p.range0 : seg_first, last = RANGES ? min(seg_last, first + p.range_tokens) : seg_last;
+    if (RANGES && first >= last) return;  // (a last segment that is shorter than the others)
+    const int row0 = RANGES ? seg * p.range_tokens - first : 0, rows = RANGES ? p.rows : p.L;  // a token's row in part_bc: row0 + token
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & (LPC - 1), ch = threadIdx.x / LPC, cp = pair_at(ch), cs = single_at(ch), d = at.d0 + ch;
     const bool in = ch < at.nch;
     constexpr int kBytes = need_vec<V * (int)sizeof(T)>();
@@ -152,7 +156,11 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     for (int i = threadIdx.x; i < kCh; i += kSelThreads) s.sbias[i] = i < at.nch && p.dt_bias ? p.dt_bias[at.d0 + i] : 0.f;
     float A2[4], g0[4] = {0.f, 0.f, 0.f, 0.f};
     load_A<LPC>(p, d, in, q, A2);
-    if (in) {
+    auto carried = [&] { return p.carry + (((int64_t)seg * p.B + at.b) * p.D + d) * kNp + 4 * q; };
+    if (RANGES && in && last < seg_last) {
+        const float4 x = *reinterpret_cast<const float4*>(carried());
+        g0[0] = x.x, g0[1] = x.y, g0[2] = x.z, g0[3] = x.w;
+    } else if (in) {
         if (p.dS_out)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -170,6 +178,16 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     // the lane's sums over its tokens (q, q + 4, ...), and its states' over all of them
     float dD = 0.f, dD_rest = 0.f, db = 0.f, db_rest = 0.f;
     float dA[4] = {0.f, 0.f, 0.f, 0.f}, dA_rest[4] = {0.f, 0.f, 0.f, 0.f};
+    if (RANGES && in && last < seg_last) {  // the ranges behind this one
+        const int64_t part = (int64_t)at.b * p.nseg + seg;
+        const float4 x = *reinterpret_cast<const float4*>(p.part_a + (part * p.D + d) * kNp + 4 * q);
+        dA[0] = x.x, dA[1] = x.y, dA[2] = x.z, dA[3] = x.w;
+        reorder(dA, order);
+        if (q == 0) {
+            dD = p.part_d[part * 2 * p.D + d];
+            db = p.part_d[(part * 2 + 1) * p.D + d];
+        }
+    }
     __syncthreads();
     for (int l0 = top; l0 >= first; l0 -= kSelTile) {
         const int l = l0 + at.row;
@@ -314,7 +332,7 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
                     for (int w = 0; w < S::kWarps; ++w) sum += s.red[w][t][k * 32 + ln];
                     int n;
                     const bool c = channel_value<LPC>(ln, k, n);
-                    if (tok < last) p.part_bc[((((int64_t)at.block(p) * p.B + at.b) * p.L + tok) * p.G + at.g) * (2 * kNp) + (c ? kNp : 0) + n] = sum;
+                    if (tok < last) p.part_bc[((((int64_t)at.block(p) * p.B + at.b) * rows + row0 + tok) * p.G + at.g) * (2 * kNp) + (c ? kNp : 0) + n] = sum;
                 }
                 __syncthreads();
             }
@@ -345,10 +363,13 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
     get(P01, g[0], g[1]);
     get(P23, g[2], g[3]);
     reorder(g, order);
-    if (in && seg == 0 && p.dS_in)
+    if (RANGES && in && first > seg_first) {
+        *reinterpret_cast<float4*>(carried()) = make_float4(g[0], g[1], g[2], g[3]);
+    } else if (in && seg == 0 && p.dS_in) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (4 * q + i < p.N) p.dS_in[((int64_t)at.b * p.D + d) * p.N + 4 * q + i] = g[i];
+    }
     const int64_t part = (int64_t)at.b * p.nseg + seg;
 #pragma unroll
     for (int i = 0; i < 4; ++i) dA[i] += dA_rest[i];
@@ -365,7 +386,7 @@ __global__ void __launch_bounds__(kSelThreads, LPC <= 8 ? 2 : 1) sel_bwd_kernel(
 // dB and dC: the parts of a group's channel blocks, added in order.
 template <typename T>
 __global__ void __launch_bounds__(256) sel_sum_bc_kernel(const SelParams p, int np, int blocks) {
-    const int64_t n = (int64_t)p.B * p.L * p.G * 2 * np;
+    const int64_t n = (int64_t)p.B * p.rows * p.G * 2 * np;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int state = (int)(i % np);
         if (state >= p.N) continue;
@@ -377,7 +398,13 @@ __global__ void __launch_bounds__(256) sel_sum_bc_kernel(const SelParams p, int 
         r >>= 1;
         const int g = (int)(r % p.G);
         r /= p.G;
-        const int64_t l = r % p.L, b = r / p.L;
+        int64_t l = r % p.rows;
+        const int64_t b = r / p.rows;
+        if (p.carry) {  // one range of several
+            const int seg = (int)l / p.range_tokens;
+            l += p.range0 + (int64_t)seg * (p.seg_tokens - p.range_tokens);
+            if (l >= min((int64_t)p.L, (int64_t)(seg + 1) * p.seg_tokens)) continue;
+        }
         if (which) static_cast<T*>(p.dC)[b * p.dC_sb + l * p.dC_sl + g * p.dC_sg + state] = from_f<T>(s);
         else static_cast<T*>(p.dB)[b * p.dB_sb + l * p.dB_sl + g * p.dB_sg + state] = from_f<T>(s);
     }
@@ -412,16 +439,17 @@ cudaError_t launch_bwd(const SelParams& p, SelPass pass, cudaStream_t st) {
     return by_lanes(p.N, [&](auto lpc) {
         constexpr int LPC = decltype(lpc)::value;
         if (pass != kSelWalk) return launch_sel(sel_seg_kernel<T, LPC, true>, seg_smem<T, LPC>(), p, p.nseg - 1, st);
-        return launch_sel(sel_bwd_kernel<T, LPC>, sizeof(BwdSmem<T, LPC>), p, p.nseg, st);
+        return p.carry ? launch_sel(sel_bwd_kernel<T, LPC, true>, sizeof(BwdSmem<T, LPC>), p, p.nseg, st)
+                       : launch_sel(sel_bwd_kernel<T, LPC, false>, sizeof(BwdSmem<T, LPC>), p, p.nseg, st);
     });
 }
 
 template <typename T>
-cudaError_t launch_sums(const SelParams& p, cudaStream_t st) {
+cudaError_t launch_sums(const SelParams& p, bool weights, cudaStream_t st) {
     const int np = 4 * sel_lanes(p.N), kCh = sel_channels(p.N), blocks = (p.Dg + kCh - 1) / kCh;
     auto grid = [](int64_t n) { return (unsigned)((n + 255) / 256 < 148 * 16 ? (n + 255) / 256 : 148 * 16); };
-    sel_sum_bc_kernel<T><<<grid((int64_t)p.B * p.L * p.G * 2 * np), 256, 0, st>>>(p, np, blocks);
-    sel_sum_weights_kernel<T><<<grid((int64_t)p.D * (np + 2)), 256, 0, st>>>(p, np);
+    sel_sum_bc_kernel<T><<<grid((int64_t)p.B * p.rows * p.G * 2 * np), 256, 0, st>>>(p, np, blocks);
+    if (weights) sel_sum_weights_kernel<T><<<grid((int64_t)p.D * (np + 2)), 256, 0, st>>>(p, np);
     return cudaGetLastError();
 }
 

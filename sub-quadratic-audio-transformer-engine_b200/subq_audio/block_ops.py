@@ -289,7 +289,8 @@ class ScanHandover:
     token): pass one instance as ``handover=`` to the forward, which fills it, and then to ``selective_scan_backward``, which
     otherwise forms them again. A carrier from a call of another shape, type or device is refused; one from a call of the
     same shape but other inputs gives wrong gradients. It holds 8 bytes for each token and channel of up to 16 states (16,
-    32 and 64 bytes up to 32, 64 and 128)."""
+    32 and 64 bytes up to 32, 64 and 128); without one the backward's workspace holds as much, beside at most 1 GiB or a float32
+    [B, L, D] (whichever is more) of parts of dB and dC."""
 
     def __init__(self) -> None:
         self.buf: Optional[torch.Tensor] = None
