@@ -4,7 +4,7 @@
 // counts as 0 and its output is 0; the window that is handed on is of the W - 1 inputs up to the last live token.
 //   dpre_t = dy_t act'(pre_t),   dx_s = sum_j w_j dpre_{s+W-1-j},   dw_j = sum_t dpre_t x_{t-W+1+j},   db = sum_t dpre_t.
 //
-// HBM-bound: a thread has four neighbouring channels (backward of 16-bit types: two; single ones where rows are not aligned) and a
+// HBM-bound: a thread has four neighbouring channels (backward: two; single ones where rows are not aligned) and a
 // run of eight tokens (backward: sixteen), all of whose rows it asks for at once, those of the tokens that its taps reach into among them (L1 has
 // them for the CTA's next run). The backward forms pre again from x; its dw and db are summed over a run, over the CTA's
 // eight runs in shared memory and then over CTAs by a second launch, in a fixed order.
@@ -393,15 +393,14 @@ __global__ void __launch_bounds__(kConvThreads) conv_sum_kernel(const ConvParams
     else if (p.db) p.db[c] = s + rest;
 }
 
-// Channels of a thread: four, or two in the backward of 16-bit types (whose eight runs of four spill).
-template <typename T>
-constexpr int pieces(bool bwd) {
-    return bwd && sizeof(T) == 2 ? 2 : 4;
-}
+// Channels of a thread: four, or two in the backward, whose sixteen tokens of four channels do not fit the registers (float32
+// training step, us, of four and two: 8 x 2047 x 1536, W = 4, padded 179, 150; 16 x 2048 x 1024, W = 3 205, 150, W = 2 174, 146;
+// 4 x 2000 x 1022 88 (single ones), 67; 4 x 1024 x 768 44, 44).
+constexpr int pieces(bool bwd) { return bwd ? 2 : 4; }
 // Do the channels come out even, and all rows' alignments allow them?
 template <typename T>
 bool pieces_fit(const ConvParams& p, bool bwd) {
-    const int n = pieces<T>(bwd), need = n * (int)sizeof(T);
+    const int n = pieces(bwd), need = n * (int)sizeof(T);
     const uintptr_t windows = bwd ? reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.dS_out) | reinterpret_cast<uintptr_t>(p.dS_in)
                                   : reinterpret_cast<uintptr_t>(p.S_in) | reinterpret_cast<uintptr_t>(p.S_out);
     if (p.D % n || windows % need || p.x.vec < need) return false;
@@ -447,8 +446,8 @@ template <typename T>
 cudaError_t conv_any(const ConvParams& p, bool bwd, cudaStream_t st, int* launches) {
     auto width = [&](auto w) {
         constexpr int W = decltype(w)::value;
-        if (bwd) return pieces_fit<T>(p, true) ? conv_bwd<T, pieces<T>(true), W>(p, st, launches) : conv_bwd<T, 1, W>(p, st, launches);
-        return pieces_fit<T>(p, false) ? conv_fwd<T, pieces<T>(false), W>(p, st, launches) : conv_fwd<T, 1, W>(p, st, launches);
+        if (bwd) return pieces_fit<T>(p, true) ? conv_bwd<T, pieces(true), W>(p, st, launches) : conv_bwd<T, 1, W>(p, st, launches);
+        return pieces_fit<T>(p, false) ? conv_fwd<T, pieces(false), W>(p, st, launches) : conv_fwd<T, 1, W>(p, st, launches);
     };
     if (p.W == 2) return width(std::integral_constant<int, 2>{});
     return p.W == 3 ? width(std::integral_constant<int, 3>{}) : width(std::integral_constant<int, 4>{});
