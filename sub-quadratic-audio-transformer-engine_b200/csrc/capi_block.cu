@@ -102,9 +102,9 @@ int check_sel(const subq_selective_desc& d, SelParams& p) {
 // SMs. A segment costs `first` of the walk again for its sum in the launch before, 4 us for that launch, and a step of the
 // chain in front of the walk. In units of a CTA's 32 tokens, which take `tile` us when the SM is full; the least sum wins.
 // us of the forward, with one segment and as chosen (bf16, D = 1536, N = 16 where nothing else is said):
-//   1 x 65536 tokens 9263, 1518   1 x 4096 584, 125   4 x 2048 301, 206   8 x 2047, padded 452, 383   16 x 1024 303 (one is chosen)
-//   2 x 1537, D = 384, float32 214, 47   2 x 4096, D = 1024, N = 64 548, 517
-// and with its gradients: 8 x 1024 829, 672   2 x 1537, D = 384, float32 763, 134   2 x 1024, D = 1024, N = 64 540, 565 (one is better)
+//   1 x 65536 tokens 9263, 1529   1 x 4096 584, 127   4 x 2048 301, 208   8 x 2047, padded 452, 385   16 x 1024 305 (one is chosen)
+//   2 x 1537, D = 384, float32 214, 47   2 x 4096, D = 1024, N = 64 548, 509
+// and with its gradients: 8 x 1024 829, 672   2 x 1537, D = 384, float32 763, 134   2 x 1024, D = 1024, N = 64 540, 558 (one is better)
 void sel_split(SelParams& p, bool back) {
     const int64_t ch = sel_channels(p.N), ctas = (int64_t)p.B * p.G * ((p.Dg + ch - 1) / ch), tiles = (p.L + kSelTile - 1) / kSelTile;
     if (ctas <= 0 || tiles <= 0) return;

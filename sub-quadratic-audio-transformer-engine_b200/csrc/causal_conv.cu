@@ -8,8 +8,9 @@
 // run of eight tokens (backward: sixteen), all of whose rows it asks for at once, those of the tokens that its taps reach into among them (L1 has
 // them for the CTA's next run). The backward forms pre again from x; its dw and db are summed over a run, over the CTA's
 // eight runs in shared memory and then over CTAs by a second launch, in a fixed order.
-// 8 x 2047 x 1536 in bf16: forward 35 us (HBM floor 15), backward 86 us (23: nineteen sums before the activation for sixteen
-// tokens, and its derivative; instruction issue).
+// 8 x 2047 x 1536 in bf16: forward 35 us (HBM floor 15; its warps wait for their rows: a thread loads its run, computes and ends),
+// backward 86 us (23; float32 94: nineteen sums before the activation for sixteen tokens, and its derivative, at 15 warps an SM
+// that wait for the instruction before). Issue slots are 0.6 used in both.
 #include <algorithm>
 
 #include "sel_common.cuh"

@@ -10,7 +10,8 @@
 // Large products: 128 x 256 tiles by one CTA an SM that goes on from tile to tile (k-blocks of the next one are loaded and
 // multiplied while this one is written), eight epilogue warps with 128 columns each. A k-block's products take 512 cycles,
 // its way through the epilogue (TMEM read and multiply-add, two warps to a scheduler) about as long, its 48 KB from L2 about
-// 800: 16384 x 4096 x 1024 takes 104 to 107 us (1.3 PFLOP/s), 2048 x 4096 x 4096 51 us (1.35).
+// 800: 16384 x 4096 x 1024 takes 107 to 118 us from card to card (1.2 to 1.3 PFLOP/s), 2048 x 4096 x 4096 51 us (1.35). That is 1600
+// cycles a k-block at K = 1024: beside L2 the stores of a finished tile, during which two more k-blocks at most are formed.
 // Smaller ones: 128 x BN tiles, a CTA each, two to an SM.
 // A few rows (streaming steps) are bound by the weights' bytes, or by the launch: there a warp has a column of b, its lanes
 // 16 values each at a time, and every row of a.

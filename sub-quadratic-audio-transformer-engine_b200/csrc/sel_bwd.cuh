@@ -10,8 +10,9 @@
 // step (lanes hold their states in an order by which nothing has to be selected), over the CTA's warps in shared memory, over CTAs by a second launch, all in a fixed order. Sums over tokens (dA, dD,
 // dbias) are added per eight tokens or tile with their rounding kept (two float32 a sum). Segments as in the forward.
 //
-// Bound by instruction issue: 412 us of the 4 x 2048 x 1536 training step (166 instructions for 32 states of a token), beside 75 us
-// for the segments and 206 us for the forward.
+// Bound by latency: 415 us of the 4 x 2048 x 1536 training step (168 instructions for 32 states of a token, beside 75 us for the
+// segments and 210 us for the forward). Two CTAs an SM are what registers and shared memory allow, 3.9 warps a scheduler that
+// wait for shuffles and shared memory and for the instruction before (issue slots 0.58 used, FMA pipe 41 %, ALU 36 %).
 #pragma once
 
 #include "sel_fwd.cuh"

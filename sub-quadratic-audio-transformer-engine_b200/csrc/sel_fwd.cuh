@@ -4,7 +4,7 @@
 // the threads that hold u and z for the output. The next tile is on its way meanwhile.
 //
 // Bound by instruction issue and the FMA pipe (a state and token take one exponential, nine multiply-adds, two states at a
-// time, and three selections), not by memory: 65536 x 1536 channels of 16 states take 1518 us, a third of them the
+// time, and three selections), not by memory: 65536 x 1536 channels of 16 states take 1529 us, a third of them the
 // segments; 124 us would be its bytes, 360 us its exponentials alone. Few channels: the sequence is cut into segments; a first launch finds what each leaves of a zero
 // state and the sum of its step sizes (a segment's decay is exp(A sum dt)), and the walk's CTAs chain those before theirs.
 #pragma once
